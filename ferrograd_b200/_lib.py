@@ -90,6 +90,11 @@ SIGNATURES = {
     "fg_softmax_bwd": (i32, [c_ctx, u32, u32, c_dev, c_dev, c_dev, i32]),
     "fg_softmax_ce_fwd_bwd": (i32, [c_ctx, c_dev, c_dev, u32, u32, f32, c_dev, c_dev, c_dev, c_dev, c_dev]),
     "fg_ce_loss_grad": (i32, [c_ctx, c_dev, c_dev, u32, u32, c_dev, c_dev]),
+    "fg_layernorm_fwd": (i32, [c_ctx, i32, u32, u32, c_dev, c_dev, c_dev, f32, c_dev, c_dev, c_dev]),
+    "fg_layernorm_bwd": (i32, [c_ctx, i32, u32, u32, c_dev, c_dev, c_dev, c_dev, c_dev, c_dev, c_dev, c_dev, i32, i32]),
+    "fg_embedding_fwd": (i32, [c_ctx, i32, u32, u32, u32, c_dev, c_dev, f32, c_dev]),
+    "fg_embedding_bwd": (i32, [c_ctx, i32, u32, u32, u32, c_dev, c_dev, f32, c_dev, i32]),
+    "fg_sample": (i32, [c_ctx, i32, u32, u32, c_dev, c_dev, c_dev, c_dev, c_dev, c_dev, c_dev, c_dev]),
     "fg_sum_f32": (i32, [c_ctx, c_dev, u64, c_dev]),
     "fg_mse_loss_grad": (i32, [c_ctx, c_dev, c_dev, u64, f32, c_dev, c_dev, c_dev]),
     "fg_bce_loss_grad": (i32, [c_ctx, c_dev, c_dev, u64, f32, c_dev, c_dev, c_dev]),

@@ -341,6 +341,25 @@ class GpuContext:
         self._check(self._c.fg_ce_loss_grad(self._h, probs, labels, rows, cols, loss,
                                              grad))
 
+    # ---- token models ----
+    def layernorm_fwd(self, x, gamma, beta, y, rows, cols, eps=1e-5, mean=None, rstd=None, dtype="f32"):
+        self._check(self._c.fg_layernorm_fwd(self._h, DTYPE[dtype], rows, cols, x, gamma, beta, eps, y, mean, rstd))
+
+    def layernorm_bwd(self, x, dy, gamma, mean, rstd, rows, cols, dx=None, dgamma=None, dbeta=None, accumulate_dx=False,
+                      accumulate_params=False, dtype="f32"):
+        self._check(self._c.fg_layernorm_bwd(self._h, DTYPE[dtype], rows, cols, x, dy, gamma, mean, rstd, dx, dgamma, dbeta,
+                                              int(accumulate_dx), int(accumulate_params)))
+
+    def embedding_fwd(self, table, ids, out, tokens, vocab, dim, scale=1.0, dtype="f32"):
+        self._check(self._c.fg_embedding_fwd(self._h, DTYPE[dtype], tokens, vocab, dim, ids, table, scale, out))
+
+    def embedding_bwd(self, ids, dout, dtable, tokens, vocab, dim, scale=1.0, accumulate=False, dtype="f32"):
+        self._check(self._c.fg_embedding_bwd(self._h, DTYPE[dtype], tokens, vocab, dim, ids, dout, scale, dtable, int(accumulate)))
+
+    def sample(self, logits, u, token, rows, cols, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, dtype="f32"):
+        """One token per row; temperature, top_k, top_p and min_p are device arrays of one value per row, or None."""
+        self._check(self._c.fg_sample(self._h, DTYPE[dtype], rows, cols, logits, u, temperature, top_k, top_p, min_p, token, prob))
+
     def mse_loss_grad(self, pred, target, n, grad_scale=1.0, loss_elem=None, loss_sum=None, grad=None):
         self._check(self._c.fg_mse_loss_grad(self._h, pred, target, n, grad_scale,
                                               loss_elem, loss_sum, grad))

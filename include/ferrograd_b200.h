@@ -296,6 +296,57 @@ int32_t fg_softmax_ce_fwd_bwd(fg_ctx* ctx, const float* logits, const uint32_t* 
 int32_t fg_ce_loss_grad(fg_ctx* ctx, const float* probs, const uint32_t* labels,
                         uint32_t rows, uint32_t cols, float* loss_out, float* grad_out);
 
+/* ---- layer norm, embedding lookup and sampling (no counterpart in the reference, whose row operator is softmax) ----
+ * What a model of tokens needs around its dense layers.  `dtype` is the storage type (fg_dtype, below) of every
+ * tensor whose type is not given; arithmetic is f32 or wider and results are rounded once.  Tensors are dense
+ * and may start at any element.
+ *
+ * y = (x - mean) * rstd * gamma + beta for each row, rstd = 1 / sqrt(variance + eps) with the variance over cols
+ * (not cols - 1).  gamma and beta ([cols]) may be NULL: ones and zeros.  mean_out and rstd_out (f32 [rows], may be
+ * NULL) are what the backward pass takes.  eps >= 0.  y may be x. */
+int32_t fg_layernorm_fwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* x,
+                         const void* gamma, const void* beta, float eps, void* y,
+                         float* mean_out, float* rstd_out);
+/* With h = (x - mean) * rstd and g = dy * gamma:
+ *   dx = rstd * (g - mean_row(g) - h * mean_row(g * h))     (skipped when dx == NULL)
+ *   dgamma [cols] = column sums of dy * h                    (skipped when NULL)
+ *   dbeta  [cols] = column sums of dy                        (skipped when NULL)
+ * accumulate_dx adds into dx and accumulate_params into dgamma and dbeta instead of overwriting them.  Sums are in
+ * f32 in an order that the sizes alone decide.  dx may be dy or x (then without accumulate_dx). */
+int32_t fg_layernorm_bwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* x, const void* dy,
+                         const void* gamma, const float* mean, const float* rstd, void* dx, void* dgamma,
+                         void* dbeta, int32_t accumulate_dx, int32_t accumulate_params);
+
+/* out[t] = scale * table[ids[t]] for `tokens` ids and a table of [vocab, dim].  An id of vocab or more (0xffffffff, say) is
+ * padding: its row of out is zero, nothing of the table is read for it, and in the backward pass it takes no part. */
+int32_t fg_embedding_fwd(fg_ctx* ctx, int32_t dtype, uint32_t tokens, uint32_t vocab, uint32_t dim,
+                         const uint32_t* ids, const void* table, float scale, void* out);
+/* dtable[v] = scale * sum of dout[t] over the tokens t with ids[t] == v, rows of other ids zero; accumulate != 0
+ * adds into dtable instead and leaves the other rows alone (fg_sgd_step and fg_adamw_step leave a gradient at zero).
+ * The tokens are sorted by id and a row's sum runs over them in f32 in an order that ids and sizes alone decide:
+ * no atomics, the same bits on every call. */
+int32_t fg_embedding_bwd(fg_ctx* ctx, int32_t dtype, uint32_t tokens, uint32_t vocab, uint32_t dim,
+                         const uint32_t* ids, const void* dout, float scale, void* dtable, int32_t accumulate);
+
+/* One index per row of logits [rows, cols], drawn with the caller's random numbers u[rows] from [0, 1).  With
+ * w = exp((x - max of the row) / temperature), these are kept:
+ *   top_k    the top_k[r] largest x, of equal ones those of the lowest index (0, or more than there are: all)
+ *   top_p    of what top_k keeps, from the largest down (of equal ones the lowest index first), the fewest that
+ *            together have at least top_p[r] of its weight; one at least (1 or more: all)
+ *   min_p    those with w >= min_p[r], the largest having w = 1 (0 or less: all; more than 1: as 1)
+ * token_out[r] is the first index, in the order of the indices, at which the running sum of the kept w exceeds u[r]
+ * times their total; prob_out[r] (f32, may be NULL) its share of the total.  Logits of -inf or NaN are never drawn; a row
+ * with no others gives FG_NO_TOKEN and probability 0.  temperature, top_k, top_p and min_p are device arrays of
+ * [rows], read when the kernel runs; NULL: 1, 0, 1, 0.  A temperature of 0 or less, or NaN, takes the first maximum, with
+ * probability 1; NaN in another parameter keeps all; u below 0 or NaN counts as 0, of 1 or more as just below 1.
+ * Weights are whole multiples of 2^-42 and their sums exact, so the token does not depend on the order of a sum.
+ * cols <= FG_SAMPLE_MAX_COLS. */
+#define FG_NO_TOKEN 0xffffffffu
+#define FG_SAMPLE_MAX_COLS 2097152u
+int32_t fg_sample(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* logits, const float* u,
+                  const float* temperature, const uint32_t* top_k, const float* top_p, const float* min_p,
+                  uint32_t* token_out, float* prob_out);
+
 /* out[0] = sum of x[0..n), reduced in a fixed order (no counterpart in the reference, whose losses stay
  * unreduced: loss/basic_loss.rs:3-133; used to hand a caller one number per step instead of the loss tensor). */
 int32_t fg_sum_f32(fg_ctx* ctx, const float* x, uint64_t n, float* out);
