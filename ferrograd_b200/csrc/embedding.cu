@@ -1,47 +1,21 @@
 // Embedding lookup with scaling, and the gradient of its table.
+//
+// The lookup copies rows and is bound by memory.  The gradient is a sum over the tokens of each id.  The tokens are sorted by id
+// (stably, so that the tokens of an id stand in their order), the sorted list is cut into chunks of one length, and a warp sums a chunk
+// for 16 bytes of columns per lane: however the ids fall, every warp has the same work.  Ids that lie in one chunk are done with that;
+// for an id that reaches over a border each chunk leaves its part in memory (f32), and the parts are added in their order.  Nothing
+// is added atomically.
+#include <cooperative_groups.h>
+
+#include <atomic>
+
 #include "rows.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
-template <typename T>
-__global__ void __launch_bounds__(256) embed_kernel(uint32_t tokens, uint32_t vocab, uint32_t dim, const uint32_t* ids, const T* table, float scale,
-                                                    T* out) {
-    fg_grid_enter();
-    for (uint32_t t = blockIdx.x; t < tokens; t += gridDim.x) {
-        const uint32_t id = ids[t];
-        const T* row = table + (uint64_t)id * dim;
-        for (uint64_t c = threadIdx.x; c < dim; c += 256) out[(uint64_t)t * dim + c] = fg_narrow<T>(id < vocab ? scale * fg_widen(row[c]) : 0.0f);
-    }
-}
-
-// One block for a row of the table and 256 columns: looks for its tokens in order.
-template <typename T>
-__global__ void __launch_bounds__(256) embed_bwd_scan_kernel(uint32_t tokens, uint32_t vocab, uint32_t dim, const uint32_t* ids, const T* dout, float scale,
-                                                             T* dtable, int accumulate) {
-    __shared__ uint32_t found[256];
-    __shared__ int count;
-    fg_grid_enter();
-    const uint64_t c = (uint64_t)blockIdx.y * 256 + threadIdx.x;
-    for (uint32_t v = blockIdx.x; v < vocab; v += gridDim.x) {
-        float s = 0.0f;
-        bool any = false;
-        for (uint64_t t0 = 0; t0 < tokens; t0 += 256) {
-            const uint64_t t = t0 + threadIdx.x;
-            found[threadIdx.x] = t < tokens ? ids[t] : 0xffffffffu;
-            if (!__syncthreads_or(found[threadIdx.x] == v)) continue;
-            for (int i = 0; i < 256 && t0 + i < tokens; ++i)
-                if (found[i] == v) {
-                    any = true;
-                    if (c < dim) s += fg_widen(dout[(t0 + i) * dim + c]);
-                }
-            __syncthreads();
-        }
-        if (c < dim && (any || !accumulate)) {
-            T* p = dtable + (uint64_t)v * dim + c;
-            *p = fg_narrow<T>(accumulate ? __fmaf_rn(scale, s, fg_widen(*p)) : scale * s);
-        }
-    }
-}
+constexpr unsigned kFull = 0xffffffffu;
 
 struct EmbedArgs {
     uint32_t tokens, vocab, dim;
@@ -52,19 +26,404 @@ struct EmbedArgs {
     int accumulate;
 };
 
+
+// ---- the tokens in order of their ids ----
+// Least significant digit first, up to 9 bits a pass, by the CTAs of one cluster: a warp holds a stretch of the list and counts its digits
+// in shared memory, the counts become places (over the warps of a CTA, over the CTAs by distributed shared memory), and the warp goes
+// over its stretch again, 32 entries at a time, and puts each at its digit's next place.  The list stays in the L2; what a
+// pass costs is its steps one after the other (some 3 us), which a grid's worth of CTAs and a launch per step would not shorten.
+// The grid's other CTAs write the zeros meanwhile: each looks through the ids for those of its rows and clears the rest.
+constexpr int kSortThreads = 1024, kSortWarps = 32, kMaxBins = 512;
+constexpr uint32_t kFillRows = 1u << 17;      // rows that a CTA marks at a time
+struct SortArgs {
+    uint32_t tokens, vocab;
+    const uint32_t* ids;
+    uint2 *a, *b;             // (id, token): pass 0 writes a, pass 1 b, ...
+    uint32_t* used;           // how many tokens have an id of the table
+    int passes, digit;
+    char* dtable;             // rows to clear (NULL: none)
+    uint64_t row_bytes;
+};
+
+__device__ void clear_row(char* p, uint64_t bytes, int lane) {
+    const uint64_t before = min((uint64_t)(-reinterpret_cast<uintptr_t>(p) & 15u), bytes), words = (bytes - before) / 16;
+    uint4* const q = reinterpret_cast<uint4*>(p + before);
+    for (uint64_t i = lane; i < words; i += 32) q[i] = make_uint4(0, 0, 0, 0);
+    for (uint64_t i = 2 * lane; i < before; i += 64) *reinterpret_cast<uint16_t*>(p + i) = 0;
+    for (uint64_t i = before + 16 * words + 2 * lane; i < bytes; i += 64) *reinterpret_cast<uint16_t*>(p + i) = 0;
+}
+__device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t parts, uint32_t* marks) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t v0 = (uint32_t)((uint64_t)s.vocab * part / parts), v1 = (uint32_t)((uint64_t)s.vocab * (part + 1) / parts);
+    for (uint32_t v = v0; v < v1; v += min(kFillRows, v1 - v)) {
+        const uint32_t n = min(kFillRows, v1 - v);
+        for (uint32_t i = tid; i < (n + 31) / 32; i += kSortThreads) marks[i] = 0;
+        __syncthreads();
+        const uint32_t head = min(s.tokens, (uint32_t)(-reinterpret_cast<uintptr_t>(s.ids) & 15u) / 4), words = (s.tokens - head) / 4;
+        auto mark = [&](uint32_t id) { if (id - v < n) atomicOr(&marks[(id - v) >> 5], 1u << ((id - v) & 31)); };
+        const uint4* const ids = reinterpret_cast<const uint4*>(s.ids + head);
+        for (uint32_t i = tid; i < words; i += kSortThreads) {
+            const uint4 q = __ldg(ids + i);
+            mark(q.x); mark(q.y); mark(q.z); mark(q.w);
+        }
+        if (tid < head) mark(s.ids[tid]);
+        if (tid < s.tokens - head - 4 * words) mark(s.ids[head + 4 * words + tid]);
+        __syncthreads();
+        for (uint32_t i = warp; i < n; i += kSortWarps)
+            if (!(marks[i >> 5] >> (i & 31) & 1u)) clear_row(s.dtable + (uint64_t)(v + i) * s.row_bytes, s.row_bytes, lane);
+        __syncthreads();
+    }
+}
+
+__global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs s) {
+    extern __shared__ uint32_t counts[];      // [warp][bin], then this CTA's totals [bin]
+    __shared__ uint32_t red[kSortWarps + 1];
+    fg_grid_enter();
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t ctas = cluster.num_blocks(), cta = cluster.block_rank();
+    if (blockIdx.x >= ctas) {
+        clear_absent(s, blockIdx.x - ctas, gridDim.x - ctas, counts);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = 1 << s.digit;
+    uint32_t* const totals = counts + kSortWarps * bins;
+    const uint64_t stretch = ((uint64_t)s.tokens + ctas * kSortWarps - 1) / (ctas * kSortWarps);
+    const uint32_t i0 = (uint32_t)min((uint64_t)s.tokens, (cta * kSortWarps + warp) * stretch), i1 = (uint32_t)min((uint64_t)s.tokens, i0 + stretch);
+    uint32_t* const mine = counts + warp * bins;
+    for (int pass = 0; pass < s.passes; ++pass) {
+        const uint2* const from = pass & 1 ? s.a : s.b;
+        uint2* const to = pass & 1 ? s.b : s.a;
+        const int shift = pass * s.digit;
+        // padding becomes the last id
+        auto entry = [&](uint32_t i) { return pass ? __ldcg(from + i) : make_uint2(min(s.ids[i], s.vocab), i); };
+        for (int i = tid; i < kSortWarps * bins; i += kSortThreads) counts[i] = 0;
+        __syncthreads();
+        uint32_t inside = 0;
+        constexpr int kAhead = 4;
+        for (uint32_t i = i0; i < i1; i += 32 * kAhead) {
+            uint32_t key[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) key[j] = i + 32 * j + lane < i1 ? entry(i + 32 * j + lane).x : 0;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (i + 32 * j + lane < i1) {
+                    atomicAdd(&mine[key[j] >> shift & (bins - 1)], 1u);
+                    inside += key[j] < s.vocab;
+                }
+        }
+        if (pass == 0) {
+            inside = __reduce_add_sync(kFull, inside);
+            if (lane == 0) red[warp] = inside;
+        }
+        __syncthreads();
+        if (tid < bins) {      // over the warps
+            uint32_t sum = 0;
+#pragma unroll 8
+            for (int w = 0; w < kSortWarps; ++w) {
+                const uint32_t c = counts[w * bins + tid];
+                counts[w * bins + tid] = sum;
+                sum += c;
+            }
+            totals[tid] = sum;
+        }
+        if (pass == 0 && warp == 0) {
+            inside = __reduce_add_sync(kFull, red[lane]);
+            __syncwarp();
+            if (lane == 0) red[kSortWarps] = inside;
+        }
+        cluster.sync();
+        uint32_t before = 0, all = 0;
+        if (tid < bins)
+            for (uint32_t c = 0; c < ctas; ++c) {
+                const uint32_t t = cluster.map_shared_rank(totals, c)[tid];
+                if (c < cta) before += t;
+                all += t;
+            }
+        if (pass == 0 && cta == 0 && tid == 0) {
+            uint32_t sum = 0;
+            for (uint32_t c = 0; c < ctas; ++c) sum += cluster.map_shared_rank(red, c)[kSortWarps];
+            *s.used = sum;
+        }
+        // where each digit begins: over the digits (bins is a multiple of 32, or one warp has them all)
+        uint32_t run = all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(kFull, run, o);
+            if (lane >= o) run += up;
+        }
+        if (lane == 31) red[warp] = run;
+        __syncthreads();
+        uint32_t base = run - all + before;
+        for (int w = 0; w < warp; ++w) base += red[w];
+        if (tid < bins)
+            for (int w = 0; w < kSortWarps; ++w) counts[w * bins + tid] += base;
+        __syncthreads();
+        for (uint32_t i = i0; i < i1; i += 32 * kAhead) {
+            uint2 e[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) e[j] = i + 32 * j + lane < i1 ? entry(i + 32 * j + lane) : make_uint2(0, 0);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const bool there = i + 32 * j + lane < i1;
+                const uint32_t d = there ? e[j].x >> shift & (bins - 1) : bins;
+                const uint32_t same = __match_any_sync(kFull, d), rank = __popc(same & ((1u << lane) - 1));
+                uint32_t place = 0;
+                if (there) place = mine[d] + rank;
+                __syncwarp();
+                if (there && rank == 0) mine[d] += __popc(same);
+                __syncwarp();
+                if (there) to[place] = e[j];
+            }
+        }
+        cluster.sync();      // the list is there, and nobody reads these totals any more
+    }
+}
+
+// ---- sums over the sorted list ----
+struct SumArgs {
+    uint32_t vocab, dim, length, tiles;      // entries per chunk, tiles of 32 packs per row
+    uint64_t chunks;
+    const uint2* list;
+    const uint32_t* used;
+    const void *dout, *dout_end;
+    void *dtable, *dtable_end;
+    float* parts;             // [chunks][2][pitch]: of the id that reaches in from the chunk before, and of the one that goes on in the next
+    uint64_t pitch;
+    float scale;
+    int accumulate;
+};
+template <typename T, bool kShift>
+__device__ __forceinline__ void store_sum(const SumArgs& s, uint32_t v, uint64_t col, uint32_t left, float (&x)[FgPack<T>::E]) {
+    constexpr int E = FgPack<T>::E;
+    T* const p = static_cast<T*>(s.dtable) + (uint64_t)v * s.dim + col;
+    float y[E];
+    if (s.accumulate) {
+        if (left) FgPack<T>::widen(fg_load_pack<T, kShift>(p, left, (const T*)s.dtable, (const T*)s.dtable_end), y);
+        if (kShift) __syncwarp();      // a lane writes what another has read
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = __fmaf_rn(s.scale, x[e], y[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = s.scale * x[e];
+    }
+    fg_store_pack<T, kShift>(p, FgPack<T>::narrow(y), left);
+}
+template <int E>
+__device__ __forceinline__ void store_part(float* p, const float (&x)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(p + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+}
+
+// A warp takes a chunk and a tile of columns.  Eight rows are on their way while they are added one by one.
+template <typename T, bool kShift>
+__global__ void __launch_bounds__(256) embed_sum_kernel(const SumArgs s) {
+    constexpr int E = FgPack<T>::E, kAhead = 8;
+    fg_grid_enter();
+    const int lane = threadIdx.x & 31;
+    const uint64_t unit = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5), chunk = unit / s.tiles;
+    const uint32_t used = *s.used;
+    const uint64_t i0 = chunk * s.length;
+    if (i0 >= used) return;
+    const uint32_t n = (uint32_t)min((uint64_t)s.length, used - i0);
+    const uint64_t col = ((unit % s.tiles) * 32 + lane) * E;
+    const uint32_t left = col < s.dim ? (uint32_t)min((uint64_t)E, s.dim - col) : 0;
+    const T* const dout = static_cast<const T*>(s.dout);
+    const uint32_t before = i0 ? s.list[i0 - 1].x : 0xffffffffu, after = i0 + n < used ? s.list[i0 + n].x : 0xffffffffu;
+    uint32_t id = s.list[i0].x;
+    bool reaches_in = id == before;
+    float acc[E] = {};
+    for (uint32_t j0 = 0; j0 < n; j0 += 32) {
+        const uint2 mine = j0 + lane < n ? s.list[i0 + j0 + lane] : make_uint2(0, 0);
+        const uint32_t m = min(32u, n - j0);
+        for (uint32_t j = 0; j < m; j += kAhead) {
+            uint4 v[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const uint32_t t = __shfl_sync(kFull, mine.y, j + k);
+                v[k] = make_uint4(0, 0, 0, 0);
+                if (j + k < m && left) v[k] = fg_load_pack<T, kShift>(dout + (uint64_t)t * s.dim + col, left, dout, (const T*)s.dout_end);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const uint32_t next = __shfl_sync(kFull, mine.x, j + k);
+                if (j + k >= m) break;
+                if (next != id) {
+                    if (reaches_in) { if (left) store_part(s.parts + 2 * chunk * s.pitch + col, acc); }
+                    else store_sum<T, kShift>(s, id, col, left, acc);
+                    reaches_in = false;
+                    id = next;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+                }
+                float x[E];
+                FgPack<T>::widen(v[k], x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += x[e];
+            }
+        }
+    }
+    if (reaches_in) { if (left) store_part(s.parts + 2 * chunk * s.pitch + col, acc); }
+    else if (id == after) { if (left) store_part(s.parts + (2 * chunk + 1) * s.pitch + col, acc); }
+    else store_sum<T, kShift>(s, id, col, left, acc);
+}
+
+// The ids that reach over borders: the warp of the chunk that such an id begins in adds its parts.
+template <typename T, bool kShift>
+__global__ void __launch_bounds__(256) embed_join_kernel(const SumArgs s) {
+    constexpr int E = FgPack<T>::E;
+    fg_grid_enter();
+    const int lane = threadIdx.x & 31;
+    const uint64_t unit = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5), chunk = unit / s.tiles, last = (chunk + 1) * s.length - 1;
+    const uint32_t used = *s.used;
+    if (last + 1 >= used) return;
+    const uint32_t id = s.list[last].x, behind = s.list[last + 1].x;
+    if (behind != id) return;
+    const uint64_t i0 = chunk * s.length;
+    if (s.list[i0].x == id && i0 && s.list[i0 - 1].x == id) return;      // it began before this chunk
+    const uint64_t col = ((unit % s.tiles) * 32 + lane) * E;
+    const uint32_t left = col < s.dim ? (uint32_t)min((uint64_t)E, s.dim - col) : 0;
+    // how many chunks behind this one it reaches into: of each, the first entry tells
+    uint64_t more = 1;
+    while (true) {
+        const uint64_t at = (chunk + 1 + more + lane) * s.length;
+        const unsigned on = __ballot_sync(kFull, at < used && s.list[at].x == id);
+        more += on == kFull ? 32 : __ffs(~on) - 1;
+        if (on != kFull) break;
+    }
+    float acc[E] = {};
+    if (left) {
+        const float* p = s.parts + (2 * chunk + 1) * s.pitch + col;      // its end of this chunk, then the beginnings of the next ones
+        for (uint64_t j = 0; j <= more;) {
+            float4 v[4][E / 4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < E / 4; ++e)
+                    v[k][e] = j + k <= more ? *reinterpret_cast<const float4*>(p + (j + k ? 2 * (j + k) - 1 : 0) * s.pitch + 4 * e) : make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < E / 4; ++e) {
+                    acc[4 * e] += v[k][e].x; acc[4 * e + 1] += v[k][e].y; acc[4 * e + 2] += v[k][e].z; acc[4 * e + 3] += v[k][e].w;
+                }
+            j += 4;
+        }
+    }
+    store_sum<T, kShift>(s, id, col, left, acc);
+}
+
+// ---- lookup ----
+// A warp takes a token and a tile of columns, four packs per lane.
+template <typename T, bool kShift>
+__global__ void __launch_bounds__(256) embed_kernel(uint32_t tokens, uint32_t vocab, uint32_t dim, uint32_t tiles, const uint32_t* ids, const T* table, const T* table_end,
+                                                    float scale, T* out) {
+    constexpr int E = FgPack<T>::E, kPacks = 4;
+    fg_grid_enter();
+    const int lane = threadIdx.x & 31;
+    const uint64_t units = (uint64_t)tokens * tiles;
+    for (uint64_t unit = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); unit < units; unit += (uint64_t)gridDim.x * 8) {
+        const uint32_t t = (uint32_t)(unit / tiles), id = ids[t];
+        const uint64_t c0 = ((unit % tiles) * (32 * kPacks) + lane) * E;
+        uint4 v[kPacks];
+        uint32_t left[kPacks];
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            const uint64_t c = c0 + (uint64_t)k * 32 * E;
+            left[k] = c < dim ? (uint32_t)min((uint64_t)E, dim - c) : 0;
+            v[k] = make_uint4(0, 0, 0, 0);
+            if (id < vocab && left[k]) v[k] = fg_load_pack<T, kShift>(table + (uint64_t)id * dim + c, left[k], table, table_end);
+        }
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            float x[E];
+            FgPack<T>::widen(v[k], x);
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = id < vocab ? x[e] * scale : 0.0f;
+            fg_store_pack<T, kShift>(out + (uint64_t)t * dim + c0 + (uint64_t)k * 32 * E, FgPack<T>::narrow(x), left[k]);
+        }
+    }
+}
+
 template <typename T>
 int32_t embed_fwd(fg_ctx* ctx, const EmbedArgs& a) {
-    const uint32_t cap = 8u * ctx->sm_count;
-    fg_launch(ctx, embed_kernel<T>, a.tokens < cap ? a.tokens : cap, 256, 0, a.tokens, a.vocab, a.dim, a.ids, (const T*)a.src, a.scale, (T*)a.dst);
+    const uint32_t tiles = (a.dim + 32 * 4 * FgPack<T>::E - 1) / (32 * 4 * FgPack<T>::E);
+    const uint64_t blocks = ((uint64_t)a.tokens * tiles + 7) / 8, cap = 32ull * ctx->sm_count;
+    const int grid = (int)(blocks < cap ? blocks : cap);
+    const T *table = (const T*)a.src, *end = table + (uint64_t)a.vocab * a.dim;
+    if (fg_rows_lie_straight(a.dim, sizeof(T), a.src, a.dst))
+        fg_launch(ctx, embed_kernel<T, false>, grid, 256, 0, a.tokens, a.vocab, a.dim, tiles, a.ids, table, end, a.scale, (T*)a.dst);
+    else fg_launch(ctx, embed_kernel<T, true>, grid, 256, 0, a.tokens, a.vocab, a.dim, tiles, a.ids, table, end, a.scale, (T*)a.dst);
     FG_LAUNCHED(ctx);
     return FG_OK;
 }
+
 template <typename T>
 int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
-    const uint32_t cap = 8u * ctx->sm_count;
-    fg_launch(ctx, embed_bwd_scan_kernel<T>, dim3(a.vocab < cap ? a.vocab : cap, (a.dim + 255) / 256), 256, 0, a.tokens, a.vocab, a.dim, a.ids,
-              (const T*)a.src, a.scale, (T*)a.dst, a.accumulate);
+    constexpr uint32_t E = FgPack<T>::E;
+    SumArgs s{};
+    s.vocab = a.vocab;
+    s.dim = a.dim;
+    s.tiles = (a.dim + 32 * E - 1) / (32 * E);
+    s.pitch = (uint64_t)s.tiles * 32 * E;
+    s.scale = a.scale;
+    s.accumulate = a.accumulate;
+    s.dout = a.src;
+    s.dout_end = (const T*)a.src + (uint64_t)a.tokens * a.dim;
+    s.dtable = a.dst;
+    s.dtable_end = (T*)a.dst + (uint64_t)a.vocab * a.dim;
+    // Chunks for two waves of warps, of 8 to 256 entries.
+    const uint64_t want = (uint64_t)a.tokens * s.tiles / (64ull * ctx->sm_count);
+    s.length = (uint32_t)(want < 8 ? 8 : want > 256 ? 256 : (want + 7) / 8 * 8);
+    s.chunks = ((uint64_t)a.tokens + s.length - 1) / s.length;
+    const uint64_t list = ((uint64_t)a.tokens * 8 + 255) / 256 * 256;
+    void* p;
+    const int32_t st = fg_ws_alloc(ctx, 2 * list + 256 + 8 * s.chunks * s.pitch, &p);
+    if (st != FG_OK) return st;
+    SortArgs o{};
+    o.tokens = a.tokens;
+    o.vocab = a.vocab;
+    o.ids = a.ids;
+    o.a = (uint2*)p;
+    o.b = (uint2*)((char*)p + list);
+    o.used = (uint32_t*)((char*)p + 2 * list);
+    s.parts = (float*)((char*)p + 2 * list + 256);
+    int bits = 1;      // of the largest key, vocab
+    while (bits < 32 && a.vocab >> bits) ++bits;
+    o.passes = (bits + 8) / 9;
+    o.digit = (bits + o.passes - 1) / o.passes;
+    s.list = o.passes & 1 ? o.a : o.b;
+    s.used = o.used;
+    unsigned ctas = 1;
+    while (ctas < 8 && (uint64_t)ctas * 2048 < a.tokens) ctas *= 2;
+    uint64_t fill = 0;
+    if (!a.accumulate) {
+        o.dtable = (char*)a.dst;
+        o.row_bytes = (uint64_t)a.dim * sizeof(T);
+        fill = 2ull * ctx->sm_count - ctas;
+        const uint64_t most = (a.vocab * o.row_bytes + 16383) / 16384;
+        fill = fill < most ? fill : most;
+        fill = fill < a.vocab ? fill : a.vocab;
+        fill = (fill + ctas - 1) / ctas * ctas;
+    }
+    const size_t bytes = sizeof(uint32_t) * (kSortWarps + 1) * kMaxBins;
+    static std::atomic<uint64_t> attr_done{0};      // one bit per device
+    if (!(attr_done.load(std::memory_order_acquire) >> (ctx->device & 63) & 1ull)) {
+        FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        attr_done.fetch_or(1ull << (ctx->device & 63), std::memory_order_release);
+    }
+    fg_launch_cluster(ctx, embed_sort_kernel, (unsigned)(ctas + fill), kSortThreads, bytes, ctas, o);
     FG_LAUNCHED(ctx);
+    const bool straight = fg_rows_lie_straight(a.dim, sizeof(T), a.src, a.dst);
+    const uint64_t blocks = (s.chunks * s.tiles + 7) / 8;
+    FG_REQUIRE(ctx, blocks < (1ull << 31), "fg_embedding_bwd: tensor too large");
+    if (straight) fg_launch(ctx, embed_sum_kernel<T, false>, (unsigned)blocks, 256, 0, s);
+    else fg_launch(ctx, embed_sum_kernel<T, true>, (unsigned)blocks, 256, 0, s);
+    FG_LAUNCHED(ctx);
+    if (s.chunks > 1) {
+        if (straight) fg_launch(ctx, embed_join_kernel<T, false>, (unsigned)blocks, 256, 0, s);
+        else fg_launch(ctx, embed_join_kernel<T, true>, (unsigned)blocks, 256, 0, s);
+        FG_LAUNCHED(ctx);
+    }
     return FG_OK;
 }
 
@@ -93,7 +452,8 @@ int32_t fg_embedding_bwd(fg_ctx* ctx, int32_t dtype, uint32_t tokens, uint32_t v
     FG_REQUIRE(ctx, fg_dtype_known(dtype), "fg_embedding_bwd: unknown dtype");
     FG_REQUIRE(ctx, ids && dout && dtable, "fg_embedding_bwd: NULL pointer");
     FG_REQUIRE(ctx, vocab >= 1 && dim >= 1, "fg_embedding_bwd: vocab and dim must be >= 1");
-    FG_REQUIRE(ctx, (uint64_t)tokens * dim < (1ull << 40) && (uint64_t)vocab * dim < (1ull << 40), "fg_embedding_bwd: tensor too large");
+    FG_REQUIRE(ctx, tokens < (1u << 31) && (uint64_t)tokens * dim < (1ull << 40) && (uint64_t)vocab * dim < (1ull << 40),
+               "fg_embedding_bwd: tensor too large");
     const uint32_t size = fg_dtype_size(dtype);
     FG_REQUIRE(ctx, fg_at_element(ids, 4) && fg_at_element(dout, size) && fg_at_element(dtable, size),
                "fg_embedding_bwd: a tensor does not start at an element");
