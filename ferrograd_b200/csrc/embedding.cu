@@ -75,9 +75,11 @@ __device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t parts, u
     }
 }
 
+// kHeld: a lane's entries (four at most) stay in registers from the counting to the placing.
+template <bool kHeld>
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs s) {
-    extern __shared__ uint32_t counts[];      // [warp][bin], then this CTA's totals [bin]
-    __shared__ uint32_t red[kSortWarps + 1];
+    extern __shared__ uint32_t counts[];      // [warp][bin]
+    __shared__ uint32_t totals[kMaxBins], bases[kMaxBins], fours[kSortThreads], red[kSortWarps + 1];
     fg_grid_enter();
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ctas = cluster.num_blocks(), cta = cluster.block_rank();
@@ -85,8 +87,8 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
         clear_absent(s, blockIdx.x - ctas, gridDim.x - ctas, counts);
         return;
     }
+    constexpr int kAhead = 4, kMaxCtas = 8;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = 1 << s.digit;
-    uint32_t* const totals = counts + kSortWarps * bins;
     const uint64_t stretch = ((uint64_t)s.tokens + ctas * kSortWarps - 1) / (ctas * kSortWarps);
     const uint32_t i0 = (uint32_t)min((uint64_t)s.tokens, (cta * kSortWarps + warp) * stretch), i1 = (uint32_t)min((uint64_t)s.tokens, i0 + stretch);
     uint32_t* const mine = counts + warp * bins;
@@ -94,21 +96,25 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
         const uint2* const from = pass & 1 ? s.a : s.b;
         uint2* const to = pass & 1 ? s.b : s.a;
         const int shift = pass * s.digit;
-        // padding becomes the last id
-        auto entry = [&](uint32_t i) { return pass ? __ldcg(from + i) : make_uint2(min(s.ids[i], s.vocab), i); };
-        for (int i = tid; i < kSortWarps * bins; i += kSortThreads) counts[i] = 0;
+        uint2 e[kAhead];
+        auto load = [&](uint32_t i) {      // padding becomes the last id
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const uint32_t k = i + 32 * j + lane;
+                e[j] = k >= i1 ? make_uint2(0, 0) : pass ? __ldcg(from + k) : make_uint2(min(s.ids[k], s.vocab), k);
+            }
+        };
+        if (kHeld) load(i0);
+        for (int i = 4 * tid; i < kSortWarps * bins; i += 4 * kSortThreads) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
         __syncthreads();
         uint32_t inside = 0;
-        constexpr int kAhead = 4;
         for (uint32_t i = i0; i < i1; i += 32 * kAhead) {
-            uint32_t key[kAhead];
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) key[j] = i + 32 * j + lane < i1 ? entry(i + 32 * j + lane).x : 0;
+            if (!kHeld) load(i);
 #pragma unroll
             for (int j = 0; j < kAhead; ++j)
                 if (i + 32 * j + lane < i1) {
-                    atomicAdd(&mine[key[j] >> shift & (bins - 1)], 1u);
-                    inside += key[j] < s.vocab;
+                    atomicAdd(&mine[e[j].x >> shift & (bins - 1)], 1u);
+                    inside += e[j].x < s.vocab;
                 }
         }
         if (pass == 0) {
@@ -116,36 +122,47 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
             if (lane == 0) red[warp] = inside;
         }
         __syncthreads();
-        if (tid < bins) {      // over the warps
-            uint32_t sum = 0;
+        // over the warps: a thread takes a digit of kSortWarps / groups warps, then adds the groups before its own
+        const int groups = bins >= kSortThreads / 2 ? 2 : 4, each = kSortWarps / groups, bin = tid & (bins - 1), group = tid >> s.digit;
+        uint32_t sum = 0;
+        if (group < groups) {
 #pragma unroll 8
-            for (int w = 0; w < kSortWarps; ++w) {
-                const uint32_t c = counts[w * bins + tid];
-                counts[w * bins + tid] = sum;
+            for (int w = group * each; w < (group + 1) * each; ++w) {
+                const uint32_t c = counts[w * bins + bin];
+                counts[w * bins + bin] = sum;
                 sum += c;
             }
-            totals[tid] = sum;
+            fours[tid] = sum;
         }
         if (pass == 0 && warp == 0) {
             inside = __reduce_add_sync(kFull, red[lane]);
-            __syncwarp();
             if (lane == 0) red[kSortWarps] = inside;
+        }
+        __syncthreads();
+        if (group < groups) {
+            uint32_t before = 0;
+            for (int g = 0; g < group; ++g) before += fours[g * bins + bin];
+            if (group == groups - 1) totals[bin] = before + sum;
+            if (before)
+#pragma unroll 8
+                for (int w = group * each; w < (group + 1) * each; ++w) counts[w * bins + bin] += before;
         }
         cluster.sync();
         uint32_t before = 0, all = 0;
-        if (tid < bins)
-            for (uint32_t c = 0; c < ctas; ++c) {
-                const uint32_t t = cluster.map_shared_rank(totals, c)[tid];
-                if (c < cta) before += t;
+        if (tid < bins) {
+#pragma unroll
+            for (uint32_t c = 0; c < kMaxCtas; ++c) {
+                const uint32_t t = c < ctas ? cluster.map_shared_rank(totals, c)[tid] : 0;
+                before += c < cta ? t : 0;
                 all += t;
             }
-        if (pass == 0 && cta == 0 && tid == 0) {
-            uint32_t sum = 0;
-            for (uint32_t c = 0; c < ctas; ++c) sum += cluster.map_shared_rank(red, c)[kSortWarps];
-            *s.used = sum;
         }
-        // where each digit begins: over the digits (bins is a multiple of 32, or one warp has them all)
-        uint32_t run = all;
+        if (pass == 0 && cta == 0 && tid == 0) {
+            uint32_t n = 0;
+            for (uint32_t c = 0; c < ctas; ++c) n += cluster.map_shared_rank(red, c)[kSortWarps];
+            *s.used = n;
+        }
+        uint32_t run = all;      // where each digit begins
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t up = __shfl_up_sync(kFull, run, o);
@@ -153,22 +170,22 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
         }
         if (lane == 31) red[warp] = run;
         __syncthreads();
-        uint32_t base = run - all + before;
-        for (int w = 0; w < warp; ++w) base += red[w];
-        if (tid < bins)
-            for (int w = 0; w < kSortWarps; ++w) counts[w * bins + tid] += base;
+        if (tid < bins) {
+            uint32_t base = run - all + before;
+            for (int w = 0; w < warp; ++w) base += red[w];
+            bases[tid] = base;
+        }
         __syncthreads();
         for (uint32_t i = i0; i < i1; i += 32 * kAhead) {
-            uint2 e[kAhead];
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) e[j] = i + 32 * j + lane < i1 ? entry(i + 32 * j + lane) : make_uint2(0, 0);
+            if (!kHeld) load(i);
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
+                if (i + 32 * j >= i1) break;
                 const bool there = i + 32 * j + lane < i1;
                 const uint32_t d = there ? e[j].x >> shift & (bins - 1) : bins;
                 const uint32_t same = __match_any_sync(kFull, d), rank = __popc(same & ((1u << lane) - 1));
                 uint32_t place = 0;
-                if (there) place = mine[d] + rank;
+                if (there) place = bases[d] + mine[d] + rank;
                 __syncwarp();
                 if (there && rank == 0) mine[d] += __popc(same);
                 __syncwarp();
@@ -181,7 +198,7 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
 
 // ---- sums over the sorted list ----
 struct SumArgs {
-    uint32_t vocab, dim, length, tiles;      // entries per chunk, tiles of 32 packs per row
+    uint32_t vocab, dim, length, tiles;      // entries per warp, tiles of 32 packs per row
     uint64_t chunks;
     const uint2* list;
     const uint32_t* used;
@@ -214,24 +231,32 @@ __device__ __forceinline__ void store_part(float* p, const float (&x)[E]) {
     for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(p + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
 }
 
-// A warp takes a chunk and a tile of columns.  Eight rows are on their way while they are added one by one.
+// A warp takes `length` entries and a tile of columns, with eight rows on their way while they are added one by one; the eight warps of a
+// block take the same columns of entries that follow each other and join their parts in shared memory, so a chunk is eight stretches.
 template <typename T, bool kShift>
-__global__ void __launch_bounds__(256) embed_sum_kernel(const SumArgs s) {
+__global__ void __launch_bounds__(256, 3) embed_sum_kernel(const SumArgs s) {
     constexpr int E = FgPack<T>::E, kAhead = 8;
+    __shared__ float4 ends[8][E / 4][32];         // a warp's part of the id that reaches in
+    __shared__ bool through[8];                   // the warp has one id alone, which reaches in and goes on
     fg_grid_enter();
-    const int lane = threadIdx.x & 31;
-    const uint64_t unit = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5), chunk = unit / s.tiles;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t chunk = blockIdx.x / s.tiles;
     const uint32_t used = *s.used;
-    const uint64_t i0 = chunk * s.length;
-    if (i0 >= used) return;
+    if (chunk * 8 * s.length >= used) return;
+    const uint64_t i0 = min((uint64_t)used, (chunk * 8 + warp) * s.length);
     const uint32_t n = (uint32_t)min((uint64_t)s.length, used - i0);
-    const uint64_t col = ((unit % s.tiles) * 32 + lane) * E;
+    const uint64_t col = ((uint64_t)(blockIdx.x % s.tiles) * 32 + lane) * E;
     const uint32_t left = col < s.dim ? (uint32_t)min((uint64_t)E, s.dim - col) : 0;
     const T* const dout = static_cast<const T*>(s.dout);
-    const uint32_t before = i0 ? s.list[i0 - 1].x : 0xffffffffu, after = i0 + n < used ? s.list[i0 + n].x : 0xffffffffu;
-    uint32_t id = s.list[i0].x;
-    bool reaches_in = id == before;
+    constexpr uint32_t kNone = 0xffffffffu;
+    const uint32_t before = i0 && n ? s.list[i0 - 1].x : kNone, after = i0 + n < used ? s.list[i0 + n].x : kNone, begin = n ? s.list[i0].x : kNone;
+    uint32_t id = begin;
+    bool reaches_in = n && id == before;
     float acc[E] = {};
+    auto leave = [&] {
+#pragma unroll
+        for (int e = 0; e < E / 4; ++e) ends[warp][e][lane] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+    };
     for (uint32_t j0 = 0; j0 < n; j0 += 32) {
         const uint2 mine = j0 + lane < n ? s.list[i0 + j0 + lane] : make_uint2(0, 0);
         const uint32_t m = min(32u, n - j0);
@@ -248,7 +273,7 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const SumArgs s) {
                 const uint32_t next = __shfl_sync(kFull, mine.x, j + k);
                 if (j + k >= m) break;
                 if (next != id) {
-                    if (reaches_in) { if (left) store_part(s.parts + 2 * chunk * s.pitch + col, acc); }
+                    if (reaches_in) leave();
                     else store_sum<T, kShift>(s, id, col, left, acc);
                     reaches_in = false;
                     id = next;
@@ -262,9 +287,40 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const SumArgs s) {
             }
         }
     }
-    if (reaches_in) { if (left) store_part(s.parts + 2 * chunk * s.pitch + col, acc); }
-    else if (id == after) { if (left) store_part(s.parts + (2 * chunk + 1) * s.pitch + col, acc); }
-    else store_sum<T, kShift>(s, id, col, left, acc);
+    const bool goes_on = n && id == after;
+    if (reaches_in) leave();
+    else if (n && !goes_on) store_sum<T, kShift>(s, id, col, left, acc);
+    if (lane == 0) through[warp] = reaches_in && goes_on;
+    __syncthreads();
+    // Now the ids that cross a stretch's end.  The warp that one begins in adds what the next ones left of it; the block's first warp does so for
+    // the id that reaches into the block.
+    const bool begins = goes_on && !reaches_in, enters = warp == 0 && n && begin == before;
+    if (enters) {
+        float sum[E] = {};
+        for (int w = 0; w < 8; ++w) {
+#pragma unroll
+            for (int e = 0; e < E / 4; ++e) {
+                const float4 p = ends[w][e][lane];
+                sum[4 * e] += p.x; sum[4 * e + 1] += p.y; sum[4 * e + 2] += p.z; sum[4 * e + 3] += p.w;
+            }
+            if (!through[w]) break;
+        }
+        if (left) store_part(s.parts + 2 * chunk * s.pitch + col, sum);
+    }
+    if (begins) {
+        bool out = warp == 7;
+        for (int w = warp + 1; w < 8; ++w) {
+#pragma unroll
+            for (int e = 0; e < E / 4; ++e) {
+                const float4 p = ends[w][e][lane];
+                acc[4 * e] += p.x; acc[4 * e + 1] += p.y; acc[4 * e + 2] += p.z; acc[4 * e + 3] += p.w;
+            }
+            if (!through[w]) break;
+            out = w == 7;
+        }
+        if (out) { if (left) store_part(s.parts + (2 * chunk + 1) * s.pitch + col, acc); }
+        else store_sum<T, kShift>(s, id, col, left, acc);
+    }
 }
 
 // The ids that reach over borders: the warp of the chunk that such an id begins in adds its parts.
@@ -273,19 +329,19 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const SumArgs s) {
     constexpr int E = FgPack<T>::E;
     fg_grid_enter();
     const int lane = threadIdx.x & 31;
-    const uint64_t unit = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5), chunk = unit / s.tiles, last = (chunk + 1) * s.length - 1;
+    const uint64_t unit = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5), chunk = unit / s.tiles, size = 8ull * s.length, last = (chunk + 1) * size - 1;
     const uint32_t used = *s.used;
     if (last + 1 >= used) return;
     const uint32_t id = s.list[last].x, behind = s.list[last + 1].x;
     if (behind != id) return;
-    const uint64_t i0 = chunk * s.length;
+    const uint64_t i0 = chunk * size;
     if (s.list[i0].x == id && i0 && s.list[i0 - 1].x == id) return;      // it began before this chunk
     const uint64_t col = ((unit % s.tiles) * 32 + lane) * E;
     const uint32_t left = col < s.dim ? (uint32_t)min((uint64_t)E, s.dim - col) : 0;
     // how many chunks behind this one it reaches into: of each, the first entry tells
     uint64_t more = 1;
     while (true) {
-        const uint64_t at = (chunk + 1 + more + lane) * s.length;
+        const uint64_t at = (chunk + 1 + more + lane) * size;
         const unsigned on = __ballot_sync(kFull, at < used && s.list[at].x == id);
         more += on == kFull ? 32 : __ffs(~on) - 1;
         if (on != kFull) break;
@@ -371,10 +427,10 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     s.dout_end = (const T*)a.src + (uint64_t)a.tokens * a.dim;
     s.dtable = a.dst;
     s.dtable_end = (T*)a.dst + (uint64_t)a.vocab * a.dim;
-    // Chunks for two waves of warps, of 8 to 256 entries.
-    const uint64_t want = (uint64_t)a.tokens * s.tiles / (64ull * ctx->sm_count);
-    s.length = (uint32_t)(want < 8 ? 8 : want > 256 ? 256 : (want + 7) / 8 * 8);
-    s.chunks = ((uint64_t)a.tokens + s.length - 1) / s.length;
+    // Stretches for two waves of warps, of 8 to 128 entries; a chunk is the eight stretches of a block.
+    const uint64_t want = (uint64_t)a.tokens * s.tiles / (48ull * ctx->sm_count);
+    s.length = (uint32_t)(want < 8 ? 8 : want > 128 ? 128 : (want + 7) / 8 * 8);
+    s.chunks = ((uint64_t)a.tokens + 8ull * s.length - 1) / (8ull * s.length);
     const uint64_t list = ((uint64_t)a.tokens * 8 + 255) / 256 * 256;
     void* p;
     const int32_t st = fg_ws_alloc(ctx, 2 * list + 256 + 8 * s.chunks * s.pitch, &p);
@@ -394,7 +450,8 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     s.list = o.passes & 1 ? o.a : o.b;
     s.used = o.used;
     unsigned ctas = 1;
-    while (ctas < 8 && (uint64_t)ctas * 2048 < a.tokens) ctas *= 2;
+    while (ctas < 8 && (uint64_t)ctas * 4096 < a.tokens) ctas *= 2;
+    const bool held = (uint64_t)ctas * 4096 >= a.tokens;
     uint64_t fill = 0;
     if (!a.accumulate) {
         o.dtable = (char*)a.dst;
@@ -405,23 +462,24 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
         fill = fill < a.vocab ? fill : a.vocab;
         fill = (fill + ctas - 1) / ctas * ctas;
     }
-    const size_t bytes = sizeof(uint32_t) * (kSortWarps + 1) * kMaxBins;
+    const size_t bytes = sizeof(uint32_t) * kSortWarps * kMaxBins;
     static std::atomic<uint64_t> attr_done{0};      // one bit per device
     if (!(attr_done.load(std::memory_order_acquire) >> (ctx->device & 63) & 1ull)) {
-        FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(embed_sort_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(embed_sort_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
         attr_done.fetch_or(1ull << (ctx->device & 63), std::memory_order_release);
     }
-    fg_launch_cluster(ctx, embed_sort_kernel, (unsigned)(ctas + fill), kSortThreads, bytes, ctas, o);
+    fg_launch_cluster(ctx, held ? embed_sort_kernel<true> : embed_sort_kernel<false>, (unsigned)(ctas + fill), kSortThreads, bytes, ctas, o);
     FG_LAUNCHED(ctx);
     const bool straight = fg_rows_lie_straight(a.dim, sizeof(T), a.src, a.dst);
-    const uint64_t blocks = (s.chunks * s.tiles + 7) / 8;
+    const uint64_t blocks = s.chunks * s.tiles, joins = (blocks + 7) / 8;
     FG_REQUIRE(ctx, blocks < (1ull << 31), "fg_embedding_bwd: tensor too large");
     if (straight) fg_launch(ctx, embed_sum_kernel<T, false>, (unsigned)blocks, 256, 0, s);
     else fg_launch(ctx, embed_sum_kernel<T, true>, (unsigned)blocks, 256, 0, s);
     FG_LAUNCHED(ctx);
     if (s.chunks > 1) {
-        if (straight) fg_launch(ctx, embed_join_kernel<T, false>, (unsigned)blocks, 256, 0, s);
-        else fg_launch(ctx, embed_join_kernel<T, true>, (unsigned)blocks, 256, 0, s);
+        if (straight) fg_launch(ctx, embed_join_kernel<T, false>, (unsigned)joins, 256, 0, s);
+        else fg_launch(ctx, embed_join_kernel<T, true>, (unsigned)joins, 256, 0, s);
         FG_LAUNCHED(ctx);
     }
     return FG_OK;
