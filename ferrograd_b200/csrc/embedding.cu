@@ -33,14 +33,14 @@ struct EmbedArgs {
 // over its stretch again, 32 entries at a time, and puts each at its digit's next place.  The list stays in the L2; what a
 // pass costs is its steps one after the other (some 3 us), which a grid's worth of CTAs and a launch per step would not shorten.
 // The grid's other CTAs write the zeros meanwhile: each looks through the ids for those of its rows and clears the rest.
-constexpr int kSortThreads = 1024, kSortWarps = 32, kMaxBins = 512;
+constexpr int kSortThreads = 1024, kSortWarps = 32, kMaxBins = 512, kHeldEntries = 4096;      // entries that a CTA holds in registers
 constexpr uint32_t kFillRows = 1u << 17;      // rows that a CTA marks at a time
 struct SortArgs {
     uint32_t tokens, vocab;
     const uint32_t* ids;
     uint2 *a, *b;             // (id, token): pass 0 writes a, pass 1 b, ...
     uint32_t* used;           // how many tokens have an id of the table
-    int passes, digit;
+    int passes, digit, group, shares;
     char* dtable;             // rows to clear (NULL: none)
     uint64_t row_bytes;
 };
@@ -52,16 +52,27 @@ __device__ void clear_row(char* p, uint64_t bytes, int lane) {
     for (uint64_t i = 2 * lane; i < before; i += 64) *reinterpret_cast<uint16_t*>(p + i) = 0;
     for (uint64_t i = before + 16 * words + 2 * lane; i < bytes; i += 64) *reinterpret_cast<uint16_t*>(p + i) = 0;
 }
-__device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t parts, uint32_t* marks) {
+// The rows are dealt out in groups of 2^group (4 KB or a row), since the ids of a batch crowd together, to 2^shares CTAs.
+__device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t* marks) {
+    const uint32_t parts = 1u << s.shares;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t v0 = (uint32_t)((uint64_t)s.vocab * part / parts), v1 = (uint32_t)((uint64_t)s.vocab * (part + 1) / parts);
-    for (uint32_t v = v0; v < v1; v += min(kFillRows, v1 - v)) {
-        const uint32_t n = min(kFillRows, v1 - v);
+    const uint32_t groups = (uint32_t)(((uint64_t)s.vocab + (1u << s.group) - 1) >> s.group);
+    const uint32_t own = part < groups ? (groups - part + parts - 1) / parts : 0;      // groups part, part + parts, ...
+    const uint32_t step = kFillRows >> s.group;      // groups marked at a time
+    for (uint32_t g = 0; g < own; g += min(step, own - g)) {
+        const uint32_t n = min(step, own - g) << s.group;
         for (uint32_t i = tid; i < (n + 31) / 32; i += kSortThreads) marks[i] = 0;
         __syncthreads();
         const uint32_t head = min(s.tokens, (uint32_t)(-reinterpret_cast<uintptr_t>(s.ids) & 15u) / 4), words = (s.tokens - head) / 4;
-        auto mark = [&](uint32_t id) { if (id - v < n) atomicOr(&marks[(id - v) >> 5], 1u << ((id - v) & 31)); };
+        auto mark = [&](uint32_t id) {
+            const uint32_t q = id >> s.group, at = (q >> s.shares) - g;
+            if ((q & (parts - 1)) == part && at < (n >> s.group)) {
+                const uint32_t k = (at << s.group) + (id & ((1u << s.group) - 1));
+                atomicOr(&marks[k >> 5], 1u << (k & 31));
+            }
+        };
         const uint4* const ids = reinterpret_cast<const uint4*>(s.ids + head);
+#pragma unroll 4
         for (uint32_t i = tid; i < words; i += kSortThreads) {
             const uint4 q = __ldg(ids + i);
             mark(q.x); mark(q.y); mark(q.z); mark(q.w);
@@ -69,8 +80,10 @@ __device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t parts, u
         if (tid < head) mark(s.ids[tid]);
         if (tid < s.tokens - head - 4 * words) mark(s.ids[head + 4 * words + tid]);
         __syncthreads();
-        for (uint32_t i = warp; i < n; i += kSortWarps)
-            if (!(marks[i >> 5] >> (i & 31) & 1u)) clear_row(s.dtable + (uint64_t)(v + i) * s.row_bytes, s.row_bytes, lane);
+        for (uint32_t i = warp; i < n; i += kSortWarps) {
+            const uint64_t v = (((uint64_t)(g + (i >> s.group)) * parts + part) << s.group) + (i & ((1u << s.group) - 1));
+            if (v < s.vocab && !(marks[i >> 5] >> (i & 31) & 1u)) clear_row(s.dtable + v * s.row_bytes, s.row_bytes, lane);
+        }
         __syncthreads();
     }
 }
@@ -78,13 +91,13 @@ __device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t parts, u
 // kHeld: a lane's entries (four at most) stay in registers from the counting to the placing.
 template <bool kHeld>
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs s) {
-    extern __shared__ uint32_t counts[];      // [warp][bin]
-    __shared__ uint32_t totals[kMaxBins], bases[kMaxBins], fours[kSortThreads], red[kSortWarps + 1];
+    extern __shared__ uint32_t counts[];      // [warp][bin], then (kHeld) the CTA's entries in order
+    __shared__ uint32_t totals[kMaxBins], bases[kMaxBins], begins[kMaxBins], fours[kSortThreads], red[kSortWarps + 1], red_cta[kSortWarps];
     fg_grid_enter();
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ctas = cluster.num_blocks(), cta = cluster.block_rank();
     if (blockIdx.x >= ctas) {
-        clear_absent(s, blockIdx.x - ctas, gridDim.x - ctas, counts);
+        if (blockIdx.x - ctas < 1u << s.shares) clear_absent(s, blockIdx.x - ctas, counts);
         return;
     }
     constexpr int kAhead = 4, kMaxCtas = 8;
@@ -92,6 +105,7 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
     const uint64_t stretch = ((uint64_t)s.tokens + ctas * kSortWarps - 1) / (ctas * kSortWarps);
     const uint32_t i0 = (uint32_t)min((uint64_t)s.tokens, (cta * kSortWarps + warp) * stretch), i1 = (uint32_t)min((uint64_t)s.tokens, i0 + stretch);
     uint32_t* const mine = counts + warp * bins;
+    uint2* const staged = reinterpret_cast<uint2*>(counts + kSortWarps * bins);
     for (int pass = 0; pass < s.passes; ++pass) {
         const uint2* const from = pass & 1 ? s.a : s.b;
         uint2* const to = pass & 1 ? s.b : s.a;
@@ -162,34 +176,52 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
             for (uint32_t c = 0; c < ctas; ++c) n += cluster.map_shared_rank(red, c)[kSortWarps];
             *s.used = n;
         }
-        uint32_t run = all;      // where each digit begins
+        const uint32_t here = tid < bins ? totals[tid] : 0;
+        uint32_t run = all, run_cta = here;      // where each digit begins in the list, and among the CTA's entries
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t up = __shfl_up_sync(kFull, run, o);
-            if (lane >= o) run += up;
+            const uint32_t up = __shfl_up_sync(kFull, run, o), up_cta = __shfl_up_sync(kFull, run_cta, o);
+            if (lane >= o) { run += up; run_cta += up_cta; }
         }
-        if (lane == 31) red[warp] = run;
+        if (lane == 31) { red[warp] = run; red_cta[warp] = run_cta; }
         __syncthreads();
         if (tid < bins) {
-            uint32_t base = run - all + before;
-            for (int w = 0; w < warp; ++w) base += red[w];
-            bases[tid] = base;
+            uint32_t base = run - all + before, begin = run_cta - here;
+            for (int w = 0; w < warp; ++w) { base += red[w]; begin += red_cta[w]; }
+            bases[tid] = kHeld ? base - begin : base;
+            begins[tid] = begin;
         }
         __syncthreads();
         for (uint32_t i = i0; i < i1; i += 32 * kAhead) {
             if (!kHeld) load(i);
+            unsigned same[kAhead];      // the lanes with this digit (a ballot per bit: matching in one instruction takes as long as there are digits)
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) same[j] = __ballot_sync(kFull, i + 32 * j + lane < i1);
+            for (int b = 0; b < s.digit; ++b)
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    const unsigned bit = e[j].x >> (shift + b) & 1u, ones = __ballot_sync(kFull, bit);
+                    same[j] &= bit ? ones : ~ones;
+                }
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 if (i + 32 * j >= i1) break;
                 const bool there = i + 32 * j + lane < i1;
-                const uint32_t d = there ? e[j].x >> shift & (bins - 1) : bins;
-                const uint32_t same = __match_any_sync(kFull, d), rank = __popc(same & ((1u << lane) - 1));
+                const uint32_t d = e[j].x >> shift & (bins - 1), rank = __popc(same[j] & ((1u << lane) - 1));
                 uint32_t place = 0;
-                if (there) place = bases[d] + mine[d] + rank;
+                if (there) place = (kHeld ? begins[d] : bases[d]) + mine[d] + rank;
                 __syncwarp();
-                if (there && rank == 0) mine[d] += __popc(same);
+                if (there && rank == 0) mine[d] += __popc(same[j]);
                 __syncwarp();
-                if (there) to[place] = e[j];
+                if (there) (kHeld ? staged : to)[place] = e[j];
+            }
+        }
+        if (kHeld) {      // entries of a digit lie together now: written one by one from the registers, each costs two cycles of the SM
+            __syncthreads();
+            const uint32_t c0 = (uint32_t)min((uint64_t)s.tokens, cta * kSortWarps * stretch), own = (uint32_t)min((uint64_t)s.tokens, c0 + kSortWarps * stretch) - c0;
+            for (uint32_t i = tid; i < own; i += kSortThreads) {
+                const uint2 v = staged[i];
+                to[bases[v.x >> shift & (bins - 1)] + i] = v;
             }
         }
         cluster.sync();      // the list is there, and nobody reads these totals any more
@@ -198,7 +230,7 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
 
 // ---- sums over the sorted list ----
 struct SumArgs {
-    uint32_t vocab, dim, length, tiles;      // entries per warp, tiles of 32 packs per row
+    uint32_t tokens, dim, length, tiles;      // entries per warp, tiles of 32 packs per row
     uint64_t chunks;
     const uint2* list;
     const uint32_t* used;
@@ -207,23 +239,29 @@ struct SumArgs {
     float* parts;             // [chunks][2][pitch]: of the id that reaches in from the chunk before, and of the one that goes on in the next
     uint64_t pitch;
     float scale;
-    int accumulate;
 };
 template <typename T, bool kShift>
-__device__ __forceinline__ void store_sum(const SumArgs& s, uint32_t v, uint64_t col, uint32_t left, float (&x)[FgPack<T>::E]) {
+__device__ __forceinline__ uint4 load_old(const SumArgs& s, uint32_t v, uint64_t col, uint32_t left) {
+    return fg_load_pack<T, kShift>(static_cast<const T*>(s.dtable) + (uint64_t)v * s.dim + col, left, (const T*)s.dtable, (const T*)s.dtable_end);
+}
+template <typename T, bool kShift, bool kAdd>
+__device__ __forceinline__ void store_sum(const SumArgs& s, uint32_t v, uint64_t col, uint32_t left, const float (&x)[FgPack<T>::E], const uint4& old) {
     constexpr int E = FgPack<T>::E;
-    T* const p = static_cast<T*>(s.dtable) + (uint64_t)v * s.dim + col;
     float y[E];
-    if (s.accumulate) {
-        if (left) FgPack<T>::widen(fg_load_pack<T, kShift>(p, left, (const T*)s.dtable, (const T*)s.dtable_end), y);
-        if (kShift) __syncwarp();      // a lane writes what another has read
+    if (kAdd) {
+        FgPack<T>::widen(old, y);
+        if (kShift) __syncwarp();      // a lane writes words that others have read
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] = __fmaf_rn(s.scale, x[e], y[e]);
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] = s.scale * x[e];
     }
-    fg_store_pack<T, kShift>(p, FgPack<T>::narrow(y), left);
+    fg_store_pack<T, kShift>(static_cast<T*>(s.dtable) + (uint64_t)v * s.dim + col, FgPack<T>::narrow(y), left);
+}
+template <typename T, bool kShift, bool kAdd>
+__device__ __forceinline__ void store_sum(const SumArgs& s, uint32_t v, uint64_t col, uint32_t left, const float (&x)[FgPack<T>::E]) {
+    store_sum<T, kShift, kAdd>(s, v, col, left, x, kAdd && left ? load_old<T, kShift>(s, v, col, left) : make_uint4(0, 0, 0, 0));
 }
 template <int E>
 __device__ __forceinline__ void store_part(float* p, const float (&x)[E]) {
@@ -233,68 +271,78 @@ __device__ __forceinline__ void store_part(float* p, const float (&x)[E]) {
 
 // A warp takes `length` entries and a tile of columns, with eight rows on their way while they are added one by one; the eight warps of a
 // block take the same columns of entries that follow each other and join their parts in shared memory, so a chunk is eight stretches.
-template <typename T, bool kShift>
+template <typename T, bool kShift, bool kAdd>
 __global__ void __launch_bounds__(256, 3) embed_sum_kernel(const SumArgs s) {
-    constexpr int E = FgPack<T>::E, kAhead = 8;
+    constexpr int E = FgPack<T>::E, kAhead = kAdd ? 4 : 8;
     __shared__ float4 ends[8][E / 4][32];         // a warp's part of the id that reaches in
     __shared__ bool through[8];                   // the warp has one id alone, which reaches in and goes on
     fg_grid_enter();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint64_t chunk = blockIdx.x / s.tiles;
-    const uint32_t used = *s.used;
-    if (chunk * 8 * s.length >= used) return;
-    const uint64_t i0 = min((uint64_t)used, (chunk * 8 + warp) * s.length);
-    const uint32_t n = (uint32_t)min((uint64_t)s.length, used - i0);
+    const uint64_t chunk = blockIdx.x / s.tiles, i0 = min((uint64_t)s.tokens, (chunk * 8 + warp) * s.length), i1 = min((uint64_t)s.tokens, i0 + s.length);
     const uint64_t col = ((uint64_t)(blockIdx.x % s.tiles) * 32 + lane) * E;
     const uint32_t left = col < s.dim ? (uint32_t)min((uint64_t)E, s.dim - col) : 0;
     const T* const dout = static_cast<const T*>(s.dout);
-    constexpr uint32_t kNone = 0xffffffffu;
-    const uint32_t before = i0 && n ? s.list[i0 - 1].x : kNone, after = i0 + n < used ? s.list[i0 + n].x : kNone, begin = n ? s.list[i0].x : kNone;
-    uint32_t id = begin;
-    bool reaches_in = n && id == before;
+    constexpr uint32_t kNone = 0xffffffffu;      // no id of the table
+    const uint32_t before = i0 ? s.list[i0 - 1].x : kNone, after = i1 < s.tokens ? s.list[i1].x : kNone;
+    uint2 mine = i0 + lane < i1 ? s.list[i0 + lane] : make_uint2(0, 0);
+    uint32_t behind = i0 + lane + 1 < i1 ? s.list[i0 + lane + 1].x : after;      // the id after each entry's
+    const uint32_t used = *s.used;      // padding has the last places
+    if (chunk * 8 * s.length >= used) return;
+    const uint32_t n = (uint32_t)(min((uint64_t)used, i1) - min((uint64_t)used, i0));
+    bool reaches_in = n && __shfl_sync(kFull, mine.x, 0) == before, open = false;      // open: the id of the last entry goes on
+    const bool enters = warp == 0 && reaches_in;
     float acc[E] = {};
     auto leave = [&] {
 #pragma unroll
         for (int e = 0; e < E / 4; ++e) ends[warp][e][lane] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
     };
     for (uint32_t j0 = 0; j0 < n; j0 += 32) {
-        const uint2 mine = j0 + lane < n ? s.list[i0 + j0 + lane] : make_uint2(0, 0);
+        if (j0) {
+            mine = i0 + j0 + lane < i1 ? s.list[i0 + j0 + lane] : make_uint2(0, 0);
+            behind = i0 + j0 + lane + 1 < i1 ? s.list[i0 + j0 + lane + 1].x : after;
+        }
         const uint32_t m = min(32u, n - j0);
+        const unsigned ending = __ballot_sync(kFull, behind != mine.x);      // the last of their id
+        open = !(ending >> (m - 1) & 1u);
         for (uint32_t j = 0; j < m; j += kAhead) {
-            uint4 v[kAhead];
+            uint4 v[kAhead], old[kAdd ? kAhead : 1];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 const uint32_t t = __shfl_sync(kFull, mine.y, j + k);
                 v[k] = make_uint4(0, 0, 0, 0);
                 if (j + k < m && left) v[k] = fg_load_pack<T, kShift>(dout + (uint64_t)t * s.dim + col, left, dout, (const T*)s.dout_end);
             }
+            if constexpr (kAdd) {
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const uint32_t id = __shfl_sync(kFull, mine.x, j + k);
+                    old[k] = make_uint4(0, 0, 0, 0);
+                    if (j + k < m && left && (ending >> (j + k) & 1u)) old[k] = load_old<T, kShift>(s, id, col, left);
+                }
+            }
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                const uint32_t next = __shfl_sync(kFull, mine.x, j + k);
                 if (j + k >= m) break;
-                if (next != id) {
-                    if (reaches_in) leave();
-                    else store_sum<T, kShift>(s, id, col, left, acc);
-                    reaches_in = false;
-                    id = next;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-                }
                 float x[E];
                 FgPack<T>::widen(v[k], x);
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[e] += x[e];
+                if (ending >> (j + k) & 1u) {
+                    const uint32_t id = __shfl_sync(kFull, mine.x, j + k);
+                    if (reaches_in) leave();
+                    else store_sum<T, kShift, kAdd>(s, id, col, left, acc, old[kAdd ? k : 0]);
+                    reaches_in = false;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+                }
             }
         }
     }
-    const bool goes_on = n && id == after;
-    if (reaches_in) leave();
-    else if (n && !goes_on) store_sum<T, kShift>(s, id, col, left, acc);
-    if (lane == 0) through[warp] = reaches_in && goes_on;
+    if (open && reaches_in) leave();
+    if (lane == 0) through[warp] = open && reaches_in;
     __syncthreads();
     // Now the ids that cross a stretch's end.  The warp that one begins in adds what the next ones left of it; the block's first warp does so for
     // the id that reaches into the block.
-    const bool begins = goes_on && !reaches_in, enters = warp == 0 && n && begin == before;
     if (enters) {
         float sum[E] = {};
         for (int w = 0; w < 8; ++w) {
@@ -307,7 +355,7 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(const SumArgs s) {
         }
         if (left) store_part(s.parts + 2 * chunk * s.pitch + col, sum);
     }
-    if (begins) {
+    if (open && !reaches_in) {
         bool out = warp == 7;
         for (int w = warp + 1; w < 8; ++w) {
 #pragma unroll
@@ -319,12 +367,12 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(const SumArgs s) {
             out = w == 7;
         }
         if (out) { if (left) store_part(s.parts + (2 * chunk + 1) * s.pitch + col, acc); }
-        else store_sum<T, kShift>(s, id, col, left, acc);
+        else store_sum<T, kShift, kAdd>(s, after, col, left, acc);
     }
 }
 
 // The ids that reach over borders: the warp of the chunk that such an id begins in adds its parts.
-template <typename T, bool kShift>
+template <typename T, bool kShift, bool kAdd>
 __global__ void __launch_bounds__(256) embed_join_kernel(const SumArgs s) {
     constexpr int E = FgPack<T>::E;
     fg_grid_enter();
@@ -365,11 +413,12 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const SumArgs s) {
             j += 4;
         }
     }
-    store_sum<T, kShift>(s, id, col, left, acc);
+    store_sum<T, kShift, kAdd>(s, id, col, left, acc);
 }
 
 // ---- lookup ----
-// A warp takes a token and a tile of columns, four packs per lane.
+// A warp takes a token and a tile of columns, four packs per lane.  Rows off 16-byte boundaries: a lane owns words of the output as they lie in
+// memory, turns what it reads, and the ends of a row go element by element.
 template <typename T, bool kShift>
 __global__ void __launch_bounds__(256) embed_kernel(uint32_t tokens, uint32_t vocab, uint32_t dim, uint32_t tiles, const uint32_t* ids, const T* table, const T* table_end,
                                                     float scale, T* out) {
@@ -378,24 +427,35 @@ __global__ void __launch_bounds__(256) embed_kernel(uint32_t tokens, uint32_t vo
     const int lane = threadIdx.x & 31;
     const uint64_t units = (uint64_t)tokens * tiles;
     for (uint64_t unit = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); unit < units; unit += (uint64_t)gridDim.x * 8) {
-        const uint32_t t = (uint32_t)(unit / tiles), id = ids[t];
-        const uint64_t c0 = ((unit % tiles) * (32 * kPacks) + lane) * E;
+        const uint32_t t = (uint32_t)(unit / tiles), tile = (uint32_t)(unit % tiles), id = ids[t];
+        const bool inside = id < vocab;
+        const T* const row = table + (uint64_t)id * dim;
+        T* const to = out + (uint64_t)t * dim;
+        uint32_t head = 0;
+        if constexpr (kShift) {
+            head = min(dim, (uint32_t)(-reinterpret_cast<uintptr_t>(to) & 15u) / (uint32_t)sizeof(T));
+            const uint32_t tail = (dim - head) % E;
+            if (tile == 0 && lane < 2 * E) {      // before the first word, behind the last
+                const uint32_t c = lane < E ? lane : dim - tail + (lane - E);
+                if (lane < E ? lane < head : lane - E < tail) to[c] = fg_narrow<T>(inside ? fg_widen(row[c]) * scale : 0.0f);
+            }
+        }
+        const uint32_t words = (dim - head) / E;
         uint4 v[kPacks];
-        uint32_t left[kPacks];
 #pragma unroll
         for (int k = 0; k < kPacks; ++k) {
-            const uint64_t c = c0 + (uint64_t)k * 32 * E;
-            left[k] = c < dim ? (uint32_t)min((uint64_t)E, dim - c) : 0;
+            const uint32_t i = (tile * kPacks + k) * 32 + lane;
             v[k] = make_uint4(0, 0, 0, 0);
-            if (id < vocab && left[k]) v[k] = fg_load_pack<T, kShift>(table + (uint64_t)id * dim + c, left[k], table, table_end);
+            if (inside && i < words) v[k] = fg_load_pack<T, kShift>(row + head + (uint64_t)i * E, E, table, table_end);
         }
 #pragma unroll
         for (int k = 0; k < kPacks; ++k) {
+            const uint32_t i = (tile * kPacks + k) * 32 + lane;
             float x[E];
             FgPack<T>::widen(v[k], x);
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = id < vocab ? x[e] * scale : 0.0f;
-            fg_store_pack<T, kShift>(out + (uint64_t)t * dim + c0 + (uint64_t)k * 32 * E, FgPack<T>::narrow(x), left[k]);
+            for (int e = 0; e < E; ++e) x[e] = inside ? x[e] * scale : 0.0f;
+            if (i < words) *reinterpret_cast<uint4*>(to + head + (uint64_t)i * E) = FgPack<T>::narrow(x);
         }
     }
 }
@@ -417,12 +477,11 @@ template <typename T>
 int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     constexpr uint32_t E = FgPack<T>::E;
     SumArgs s{};
-    s.vocab = a.vocab;
+    s.tokens = a.tokens;
     s.dim = a.dim;
     s.tiles = (a.dim + 32 * E - 1) / (32 * E);
     s.pitch = (uint64_t)s.tiles * 32 * E;
     s.scale = a.scale;
-    s.accumulate = a.accumulate;
     s.dout = a.src;
     s.dout_end = (const T*)a.src + (uint64_t)a.tokens * a.dim;
     s.dtable = a.dst;
@@ -450,36 +509,37 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     s.list = o.passes & 1 ? o.a : o.b;
     s.used = o.used;
     unsigned ctas = 1;
-    while (ctas < 8 && (uint64_t)ctas * 4096 < a.tokens) ctas *= 2;
-    const bool held = (uint64_t)ctas * 4096 >= a.tokens;
+    while (ctas < 8 && (uint64_t)ctas * 1024 < a.tokens) ctas *= 2;
+    const bool held = (uint64_t)ctas * kHeldEntries >= a.tokens;
     uint64_t fill = 0;
     if (!a.accumulate) {
         o.dtable = (char*)a.dst;
         o.row_bytes = (uint64_t)a.dim * sizeof(T);
-        fill = 2ull * ctx->sm_count - ctas;
-        const uint64_t most = (a.vocab * o.row_bytes + 16383) / 16384;
-        fill = fill < most ? fill : most;
-        fill = fill < a.vocab ? fill : a.vocab;
-        fill = (fill + ctas - 1) / ctas * ctas;
+        while (o.group < 12 && o.row_bytes << (o.group + 1) <= 4096) ++o.group;
+        const uint64_t groups = (a.vocab + (1ull << o.group) - 1) >> o.group;
+        while (o.shares < 8 && (1ull << o.shares) < groups && a.vocab * o.row_bytes >> (o.shares + 14)) ++o.shares;      // from 16 KB each
+        fill = ((1ull << o.shares) + ctas - 1) / ctas * ctas;
     }
-    const size_t bytes = sizeof(uint32_t) * kSortWarps * kMaxBins;
+    const size_t most = sizeof(uint32_t) * kSortWarps * kMaxBins + sizeof(uint2) * kHeldEntries, marks = kFillRows / 8;
+    size_t bytes = (sizeof(uint32_t) * kSortWarps << o.digit) + (held ? sizeof(uint2) * kHeldEntries : 0);
+    bytes = bytes < marks ? marks : bytes;
     static std::atomic<uint64_t> attr_done{0};      // one bit per device
     if (!(attr_done.load(std::memory_order_acquire) >> (ctx->device & 63) & 1ull)) {
-        FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(embed_sort_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(embed_sort_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(embed_sort_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+        FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(embed_sort_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
         attr_done.fetch_or(1ull << (ctx->device & 63), std::memory_order_release);
     }
     fg_launch_cluster(ctx, held ? embed_sort_kernel<true> : embed_sort_kernel<false>, (unsigned)(ctas + fill), kSortThreads, bytes, ctas, o);
     FG_LAUNCHED(ctx);
-    const bool straight = fg_rows_lie_straight(a.dim, sizeof(T), a.src, a.dst);
-    const uint64_t blocks = s.chunks * s.tiles, joins = (blocks + 7) / 8;
+    const uint64_t blocks = s.chunks * s.tiles;
     FG_REQUIRE(ctx, blocks < (1ull << 31), "fg_embedding_bwd: tensor too large");
-    if (straight) fg_launch(ctx, embed_sum_kernel<T, false>, (unsigned)blocks, 256, 0, s);
-    else fg_launch(ctx, embed_sum_kernel<T, true>, (unsigned)blocks, 256, 0, s);
+    const bool straight = fg_rows_lie_straight(a.dim, sizeof(T), a.src, a.dst), add = a.accumulate != 0;
+    fg_launch(ctx, add ? straight ? embed_sum_kernel<T, false, true> : embed_sum_kernel<T, true, true>
+                       : straight ? embed_sum_kernel<T, false, false> : embed_sum_kernel<T, true, false>, (unsigned)blocks, 256, 0, s);
     FG_LAUNCHED(ctx);
     if (s.chunks > 1) {
-        if (straight) fg_launch(ctx, embed_join_kernel<T, false>, (unsigned)joins, 256, 0, s);
-        else fg_launch(ctx, embed_join_kernel<T, true>, (unsigned)joins, 256, 0, s);
+        fg_launch(ctx, add ? straight ? embed_join_kernel<T, false, true> : embed_join_kernel<T, true, true>
+                           : straight ? embed_join_kernel<T, false, false> : embed_join_kernel<T, true, false>, (unsigned)((blocks + 7) / 8), 256, 0, s);
         FG_LAUNCHED(ctx);
     }
     return FG_OK;
