@@ -45,20 +45,24 @@ struct SortArgs {
     uint64_t row_bytes;
 };
 
-__device__ void clear_row(char* p, uint64_t bytes, int lane) {
-    const uint64_t before = min((uint64_t)(-reinterpret_cast<uintptr_t>(p) & 15u), bytes), words = (bytes - before) / 16;
+constexpr uint32_t kSegment = 2048;      // bytes that a warp clears at a time
+__device__ __forceinline__ void clear_bytes(char* p, uint32_t bytes, int lane) {
+    const uint32_t before = min((uint32_t)(-reinterpret_cast<uintptr_t>(p) & 15u), bytes), words = (bytes - before) / 16;
     uint4* const q = reinterpret_cast<uint4*>(p + before);
-    for (uint64_t i = lane; i < words; i += 32) q[i] = make_uint4(0, 0, 0, 0);
-    for (uint64_t i = 2 * lane; i < before; i += 64) *reinterpret_cast<uint16_t*>(p + i) = 0;
-    for (uint64_t i = before + 16 * words + 2 * lane; i < bytes; i += 64) *reinterpret_cast<uint16_t*>(p + i) = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kSegment / 512; ++k)
+        if (32 * k + lane < words) q[32 * k + lane] = make_uint4(0, 0, 0, 0);
+    if (2 * lane < before) *reinterpret_cast<uint16_t*>(p + 2 * lane) = 0;
+    if (2 * lane < bytes - before - 16 * words) *reinterpret_cast<uint16_t*>(p + before + 16 * words + 2 * lane) = 0;
 }
-// The rows are dealt out in groups of 2^group (4 KB or a row), since the ids of a batch crowd together, to 2^shares CTAs.
+// The rows are dealt out in groups of 2^group (64 KB, where there are many), since the ids of a batch crowd together, to 2^shares CTAs.
 __device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t* marks) {
     const uint32_t parts = 1u << s.shares;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t groups = (uint32_t)(((uint64_t)s.vocab + (1u << s.group) - 1) >> s.group);
     const uint32_t own = part < groups ? (groups - part + parts - 1) / parts : 0;      // groups part, part + parts, ...
     const uint32_t step = kFillRows >> s.group;      // groups marked at a time
+    const uint64_t segments = (s.row_bytes + kSegment - 1) / kSegment;
     for (uint32_t g = 0; g < own; g += min(step, own - g)) {
         const uint32_t n = min(step, own - g) << s.group;
         for (uint32_t i = tid; i < (n + 31) / 32; i += kSortThreads) marks[i] = 0;
@@ -80,9 +84,13 @@ __device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t* marks) 
         if (tid < head) mark(s.ids[tid]);
         if (tid < s.tokens - head - 4 * words) mark(s.ids[head + 4 * words + tid]);
         __syncthreads();
-        for (uint32_t i = warp; i < n; i += kSortWarps) {
+        const uint64_t units = n * segments;      // the warps side by side
+        for (uint64_t k = warp; k < units; k += kSortWarps) {
+            const uint32_t i = (uint32_t)(k / segments);
             const uint64_t v = (((uint64_t)(g + (i >> s.group)) * parts + part) << s.group) + (i & ((1u << s.group) - 1));
-            if (v < s.vocab && !(marks[i >> 5] >> (i & 31) & 1u)) clear_row(s.dtable + v * s.row_bytes, s.row_bytes, lane);
+            const uint64_t from = k % segments * kSegment;
+            if (v < s.vocab && !(marks[i >> 5] >> (i & 31) & 1u))
+                clear_bytes(s.dtable + v * s.row_bytes + from, (uint32_t)min((uint64_t)kSegment, s.row_bytes - from), lane);
         }
         __syncthreads();
     }
@@ -194,15 +202,10 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
         __syncthreads();
         for (uint32_t i = i0; i < i1; i += 32 * kAhead) {
             if (!kHeld) load(i);
-            unsigned same[kAhead];      // the lanes with this digit (a ballot per bit: matching in one instruction takes as long as there are digits)
+            unsigned same[kAhead];      // the lanes with this digit
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) same[j] = __ballot_sync(kFull, i + 32 * j + lane < i1);
-            for (int b = 0; b < s.digit; ++b)
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j) {
-                    const unsigned bit = e[j].x >> (shift + b) & 1u, ones = __ballot_sync(kFull, bit);
-                    same[j] &= bit ? ones : ~ones;
-                }
+            for (int j = 0; j < kAhead; ++j)
+                same[j] = i + 32 * j < i1 ? __match_any_sync(kFull, i + 32 * j + lane < i1 ? e[j].x >> shift & (bins - 1) : bins) : 0;
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 if (i + 32 * j >= i1) break;
@@ -296,30 +299,29 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(const SumArgs s) {
 #pragma unroll
         for (int e = 0; e < E / 4; ++e) ends[warp][e][lane] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
     };
+    // `kAhead` rows are on their way: as one is added, the one `kAhead` entries behind it is asked for.
+    uint4 v[kAhead], old[kAdd ? kAhead : 1];
+    auto ask = [&](int k, uint32_t j, const uint2& from, unsigned ending) {      // entry j, one of the 32 in `from`
+        const uint32_t t = __shfl_sync(kFull, from.y, j), id = kAdd ? __shfl_sync(kFull, from.x, j) : 0;
+        if (left) v[k] = fg_load_pack<T, kShift>(dout + (uint64_t)t * s.dim + col, left, dout, (const T*)s.dout_end);
+        if (kAdd && left && (ending >> j & 1u)) old[kAdd ? k : 0] = load_old<T, kShift>(s, id, col, left);
+    };
+    unsigned ending = __ballot_sync(kFull, behind != mine.x);      // the last of their id
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+        v[k] = make_uint4(0, 0, 0, 0);
+        if (kAdd) old[k] = v[k];
+        if ((uint32_t)k < n) ask(k, k, mine, ending);
+    }
     for (uint32_t j0 = 0; j0 < n; j0 += 32) {
-        if (j0) {
-            mine = i0 + j0 + lane < i1 ? s.list[i0 + j0 + lane] : make_uint2(0, 0);
-            behind = i0 + j0 + lane + 1 < i1 ? s.list[i0 + j0 + lane + 1].x : after;
-        }
+        const uint64_t i = i0 + j0 + 32 + lane;      // the next 32
+        const uint2 next = i < i1 ? s.list[i] : make_uint2(0, 0);
+        const uint32_t next_behind = i + 1 < i1 ? s.list[i + 1].x : after;
+        const unsigned next_ending = __ballot_sync(kFull, next_behind != next.x);
         const uint32_t m = min(32u, n - j0);
-        const unsigned ending = __ballot_sync(kFull, behind != mine.x);      // the last of their id
         open = !(ending >> (m - 1) & 1u);
+#pragma unroll 1
         for (uint32_t j = 0; j < m; j += kAhead) {
-            uint4 v[kAhead], old[kAdd ? kAhead : 1];
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const uint32_t t = __shfl_sync(kFull, mine.y, j + k);
-                v[k] = make_uint4(0, 0, 0, 0);
-                if (j + k < m && left) v[k] = fg_load_pack<T, kShift>(dout + (uint64_t)t * s.dim + col, left, dout, (const T*)s.dout_end);
-            }
-            if constexpr (kAdd) {
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k) {
-                    const uint32_t id = __shfl_sync(kFull, mine.x, j + k);
-                    old[k] = make_uint4(0, 0, 0, 0);
-                    if (j + k < m && left && (ending >> (j + k) & 1u)) old[k] = load_old<T, kShift>(s, id, col, left);
-                }
-            }
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 if (j + k >= m) break;
@@ -335,8 +337,14 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(const SumArgs s) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
                 }
+                if (j0 + j + k + kAhead < n) {
+                    const bool here = j + kAhead < 32;
+                    ask(k, (j + k + kAhead) & 31, here ? mine : next, here ? ending : next_ending);
+                }
             }
         }
+        mine = next;
+        ending = next_ending;
     }
     if (open && reaches_in) leave();
     if (lane == 0) through[warp] = open && reaches_in;
@@ -486,8 +494,8 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     s.dout_end = (const T*)a.src + (uint64_t)a.tokens * a.dim;
     s.dtable = a.dst;
     s.dtable_end = (T*)a.dst + (uint64_t)a.vocab * a.dim;
-    // Stretches for two waves of warps, of 8 to 128 entries; a chunk is the eight stretches of a block.
-    const uint64_t want = (uint64_t)a.tokens * s.tiles / (48ull * ctx->sm_count);
+    // Stretches for four waves of warps, of 8 to 128 entries; a chunk is the eight stretches of a block.
+    const uint64_t want = (uint64_t)a.tokens * s.tiles / (96ull * ctx->sm_count);
     s.length = (uint32_t)(want < 8 ? 8 : want > 128 ? 128 : (want + 7) / 8 * 8);
     s.chunks = ((uint64_t)a.tokens + 8ull * s.length - 1) / (8ull * s.length);
     const uint64_t list = ((uint64_t)a.tokens * 8 + 255) / 256 * 256;
@@ -515,7 +523,7 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     if (!a.accumulate) {
         o.dtable = (char*)a.dst;
         o.row_bytes = (uint64_t)a.dim * sizeof(T);
-        while (o.group < 12 && o.row_bytes << (o.group + 1) <= 4096) ++o.group;
+        while (o.group < 11 && o.row_bytes << (o.group + 1) <= 65536 && a.vocab >> (o.group + 10)) ++o.group;
         const uint64_t groups = (a.vocab + (1ull << o.group) - 1) >> o.group;
         while (o.shares < 8 && (1ull << o.shares) < groups && a.vocab * o.row_bytes >> (o.shares + 14)) ++o.shares;      // from 16 KB each
         fill = ((1ull << o.shares) + ctas - 1) / ctas * ctas;
