@@ -41,8 +41,9 @@ struct SortArgs {
     uint2 *a, *b;             // (id, token): pass 0 writes a, pass 1 b, ...
     uint32_t* used;           // how many tokens have an id of the table
     int passes, digit, group, shares;
-    char* dtable;             // rows to clear (NULL: none)
+    char* dtable;             // rows that no token has, of those from `first_row` on, are cleared
     uint64_t row_bytes;
+    uint32_t first_row;
 };
 
 constexpr uint32_t kSegment = 2048;      // bytes that a warp clears at a time
@@ -59,7 +60,7 @@ __device__ __forceinline__ void clear_bytes(char* p, uint32_t bytes, int lane) {
 __device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t* marks) {
     const uint32_t parts = 1u << s.shares;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t groups = (uint32_t)(((uint64_t)s.vocab + (1u << s.group) - 1) >> s.group);
+    const uint32_t rows = s.vocab - s.first_row, groups = (uint32_t)(((uint64_t)rows + (1u << s.group) - 1) >> s.group);
     const uint32_t own = part < groups ? (groups - part + parts - 1) / parts : 0;      // groups part, part + parts, ...
     const uint32_t step = kFillRows >> s.group;      // groups marked at a time
     const uint64_t segments = (s.row_bytes + kSegment - 1) / kSegment;
@@ -69,6 +70,7 @@ __device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t* marks) 
         __syncthreads();
         const uint32_t head = min(s.tokens, (uint32_t)(-reinterpret_cast<uintptr_t>(s.ids) & 15u) / 4), words = (s.tokens - head) / 4;
         auto mark = [&](uint32_t id) {
+            id -= s.first_row;      // ids below it come out behind all rows
             const uint32_t q = id >> s.group, at = (q >> s.shares) - g;
             if ((q & (parts - 1)) == part && at < (n >> s.group)) {
                 const uint32_t k = (at << s.group) + (id & ((1u << s.group) - 1));
@@ -89,8 +91,8 @@ __device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t* marks) 
             const uint32_t i = (uint32_t)(k / segments);
             const uint64_t v = (((uint64_t)(g + (i >> s.group)) * parts + part) << s.group) + (i & ((1u << s.group) - 1));
             const uint64_t from = k % segments * kSegment;
-            if (v < s.vocab && !(marks[i >> 5] >> (i & 31) & 1u))
-                clear_bytes(s.dtable + v * s.row_bytes + from, (uint32_t)min((uint64_t)kSegment, s.row_bytes - from), lane);
+            if (v < rows && !(marks[i >> 5] >> (i & 31) & 1u))
+                clear_bytes(s.dtable + (s.first_row + v) * s.row_bytes + from, (uint32_t)min((uint64_t)kSegment, s.row_bytes - from), lane);
         }
         __syncthreads();
     }
@@ -202,10 +204,16 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
         __syncthreads();
         for (uint32_t i = i0; i < i1; i += 32 * kAhead) {
             if (!kHeld) load(i);
-            unsigned same[kAhead];      // the lanes with this digit
+            unsigned same[kAhead];      // the lanes with this digit, a bit at a time (one matching instruction takes as long as it finds values)
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                same[j] = i + 32 * j < i1 ? __match_any_sync(kFull, i + 32 * j + lane < i1 ? e[j].x >> shift & (bins - 1) : bins) : 0;
+            for (int j = 0; j < kAhead; ++j) same[j] = __ballot_sync(kFull, i + 32 * j + lane < i1);
+            for (int b = 0; b < s.digit; ++b)
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    if (i + 32 * j < i1) {
+                        const unsigned bit = e[j].x >> (shift + b) & 1u, ones = __ballot_sync(kFull, bit);
+                        same[j] &= bit ? ones : ~ones;
+                    }
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 if (i + 32 * j >= i1) break;
@@ -242,7 +250,46 @@ struct SumArgs {
     float* parts;             // [chunks][2][pitch]: of the id that reaches in from the chunk before, and of the one that goes on in the next
     uint64_t pitch;
     float scale;
+    uint32_t blocks, fills, group, fill_rows;      // blocks that sum, and blocks among them that clear 2^group rows each of the first fill_rows
+    uint64_t row_bytes;
 };
+
+// Index of the first entry whose id is not below `id`: 32 probes at a time, by a whole warp.
+__device__ __forceinline__ uint32_t first_not_below(const uint2* list, uint32_t n, uint64_t id, int lane) {
+    uint32_t lo = 0;
+    while (n > 0) {
+        const uint32_t step = (n + 31) / 32, at = (uint32_t)lane * step;
+        const int c = __popc(__ballot_sync(kFull, at < n && list[lo + at].x < id));
+        if (c == 0) return lo;
+        const uint32_t past = (uint32_t)(c - 1) * step + 1;
+        lo += past;
+        n = min(step - 1, n - past);
+    }
+    return lo;
+}
+// A block clears the rows of its group that the sorted list does not name.
+__device__ void clear_group(const SumArgs& s, uint32_t fill, uint32_t* marks, uint32_t* ends) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint64_t v0 = (uint64_t)fill << s.group, v1 = min((uint64_t)s.fill_rows, v0 + (1u << s.group));
+    for (uint32_t i = tid; i < ((1u << s.group) + 31) / 32; i += 256) marks[i] = 0;
+    if (warp < 2) {
+        const uint32_t at = first_not_below(s.list, *s.used, warp ? v1 : v0, lane);
+        if (lane == 0) ends[warp] = at;
+    }
+    __syncthreads();
+    for (uint64_t i = ends[0] + tid; i < ends[1]; i += 256) {
+        const uint32_t k = s.list[i].x - (uint32_t)v0;
+        atomicOr(&marks[k >> 5], 1u << (k & 31));
+    }
+    __syncthreads();
+    const uint64_t segments = (s.row_bytes + kSegment - 1) / kSegment, units = (v1 - v0) * segments;
+    for (uint64_t k = warp; k < units; k += 8) {
+        const uint32_t i = (uint32_t)(k / segments);
+        const uint64_t from = k % segments * kSegment;
+        if (!(marks[i >> 5] >> (i & 31) & 1u))
+            clear_bytes(static_cast<char*>(s.dtable) + (v0 + i) * s.row_bytes + from, (uint32_t)min((uint64_t)kSegment, s.row_bytes - from), lane);
+    }
+}
 template <typename T, bool kShift>
 __device__ __forceinline__ uint4 load_old(const SumArgs& s, uint32_t v, uint64_t col, uint32_t left) {
     return fg_load_pack<T, kShift>(static_cast<const T*>(s.dtable) + (uint64_t)v * s.dim + col, left, (const T*)s.dtable, (const T*)s.dtable_end);
@@ -281,8 +328,18 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(const SumArgs s) {
     __shared__ bool through[8];                   // the warp has one id alone, which reaches in and goes on
     fg_grid_enter();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint64_t chunk = blockIdx.x / s.tiles, i0 = min((uint64_t)s.tokens, (chunk * 8 + warp) * s.length), i1 = min((uint64_t)s.tokens, i0 + s.length);
-    const uint64_t col = ((uint64_t)(blockIdx.x % s.tiles) * 32 + lane) * E;
+    uint32_t block = blockIdx.x;
+    if constexpr (!kAdd) {      // the blocks that clear are spread evenly among the others: writes alone run at two thirds of the rate of reads and writes
+        const uint32_t all = s.blocks + s.fills, before = (uint32_t)((uint64_t)block * s.fills / all), past = (uint32_t)((uint64_t)(block + 1) * s.fills / all);
+        if (past != before) {
+            uint32_t* const room = reinterpret_cast<uint32_t*>(&ends[0][0][0]);      // 4 KB at least
+            clear_group(s, before, room + 2, room);
+            return;
+        }
+        block -= before;
+    }
+    const uint64_t chunk = block / s.tiles, i0 = min((uint64_t)s.tokens, (chunk * 8 + warp) * s.length), i1 = min((uint64_t)s.tokens, i0 + s.length);
+    const uint64_t col = ((uint64_t)(block % s.tiles) * 32 + lane) * E;
     const uint32_t left = col < s.dim ? (uint32_t)min((uint64_t)E, s.dim - col) : 0;
     const T* const dout = static_cast<const T*>(s.dout);
     constexpr uint32_t kNone = 0xffffffffu;      // no id of the table
@@ -520,14 +577,23 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     while (ctas < 8 && (uint64_t)ctas * 1024 < a.tokens) ctas *= 2;
     const bool held = (uint64_t)ctas * kHeldEntries >= a.tokens;
     uint64_t fill = 0;
+    const uint64_t blocks = s.chunks * s.tiles;
     if (!a.accumulate) {
+        // While the tokens are sorted (10 to 20 us) there is time to clear some 40 MB, beginning with the last rows, which are the rarest; the
+        // other rows are cleared while the sums are made.
+        const uint64_t row = (uint64_t)a.dim * sizeof(T), room = (40u << 20) / row, rows = room < a.vocab ? (room ? room : 1) : a.vocab;
         o.dtable = (char*)a.dst;
-        o.row_bytes = (uint64_t)a.dim * sizeof(T);
-        while (o.group < 11 && o.row_bytes << (o.group + 1) <= 65536 && a.vocab >> (o.group + 10)) ++o.group;
-        const uint64_t groups = (a.vocab + (1ull << o.group) - 1) >> o.group;
-        while (o.shares < 8 && (1ull << o.shares) < groups && a.vocab * o.row_bytes >> (o.shares + 14)) ++o.shares;      // from 16 KB each
+        o.row_bytes = s.row_bytes = row;
+        o.first_row = s.fill_rows = (uint32_t)(a.vocab - rows);
+        while (o.group < 11 && row << (o.group + 1) <= 65536 && rows >> (o.group + 10)) ++o.group;
+        const uint64_t groups = (rows + (1ull << o.group) - 1) >> o.group;
+        while (o.shares < 8 && (1ull << o.shares) < groups && rows * row >> (o.shares + 14)) ++o.shares;      // from 16 KB each
         fill = ((1ull << o.shares) + ctas - 1) / ctas * ctas;
+        while (s.group < 11 && row << (s.group + 1) <= 131072) ++s.group;
+        s.fills = (uint32_t)(((uint64_t)s.fill_rows + (1ull << s.group) - 1) >> s.group);
     }
+    FG_REQUIRE(ctx, blocks + s.fills < (1ull << 31), "fg_embedding_bwd: tensor too large");
+    s.blocks = (uint32_t)blocks;
     const size_t most = sizeof(uint32_t) * kSortWarps * kMaxBins + sizeof(uint2) * kHeldEntries, marks = kFillRows / 8;
     size_t bytes = (sizeof(uint32_t) * kSortWarps << o.digit) + (held ? sizeof(uint2) * kHeldEntries : 0);
     bytes = bytes < marks ? marks : bytes;
@@ -539,11 +605,9 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     }
     fg_launch_cluster(ctx, held ? embed_sort_kernel<true> : embed_sort_kernel<false>, (unsigned)(ctas + fill), kSortThreads, bytes, ctas, o);
     FG_LAUNCHED(ctx);
-    const uint64_t blocks = s.chunks * s.tiles;
-    FG_REQUIRE(ctx, blocks < (1ull << 31), "fg_embedding_bwd: tensor too large");
     const bool straight = fg_rows_lie_straight(a.dim, sizeof(T), a.src, a.dst), add = a.accumulate != 0;
     fg_launch(ctx, add ? straight ? embed_sum_kernel<T, false, true> : embed_sum_kernel<T, true, true>
-                       : straight ? embed_sum_kernel<T, false, false> : embed_sum_kernel<T, true, false>, (unsigned)blocks, 256, 0, s);
+                       : straight ? embed_sum_kernel<T, false, false> : embed_sum_kernel<T, true, false>, (unsigned)(blocks + s.fills), 256, 0, s);
     FG_LAUNCHED(ctx);
     if (s.chunks > 1) {
         fg_launch(ctx, add ? straight ? embed_join_kernel<T, false, true> : embed_join_kernel<T, true, true>

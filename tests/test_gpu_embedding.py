@@ -91,6 +91,24 @@ def test_long_batches(ctx, n, vocab, kind):
     assert np.array_equal(grad.get(), want.astype(np.float32))
 
 
+@pytest.mark.parametrize("dtype,vocab,dim,shift", [("f32", 20011, 777, 1), ("f16", 30000, 1024, 0), ("bf16", 700, 40001, 3)])
+@pytest.mark.parametrize("kind", ["words", "padded", "one"])
+def test_large_tables(ctx, dtype, vocab, dim, shift, kind):
+    # tables whose rows are cleared in both launches; sums of whole numbers, rounded once
+    r = np.random.Generator(np.random.Philox(vocab))
+    n = 1500
+    ids, dout = tokens_of(kind, n, vocab, r), r.integers(-2, 3, (n, dim)).astype(np.float32)
+    if kind == "words":
+        ids[:700] = r.permutation(vocab)[:700]
+    dout[200:] *= kind != "one"
+    grad = empty(ctx, (vocab, dim), dtype, shift)
+    ctx.embedding_bwd(Placed(ctx, ids, "u32"), Placed(ctx, dout, dtype, shift), grad, n, vocab, dim, dtype=dtype)
+    inside = ids < vocab
+    want = np.zeros((vocab, dim), np.float32)
+    np.add.at(want, ids[inside], dout[inside])
+    assert np.array_equal(grad.get(), rounded(want, dtype))
+
+
 def test_values_out_of_the_ordinary(ctx):
     # an infinity or NaN in a padded place is not read; in a used one it stays in its row and column
     ids = np.array([2, PAD, 0, 2], np.uint32)
