@@ -23,6 +23,299 @@ struct NormBwdArgs {
     int accumulate_dx, accumulate_params;
 };
 
+// ---- rows that a group of threads holds ----
+// A group of warps takes a row at a time, a thread the same columns of each: pack `thread`, `thread` + threads, ... of 16 bytes.  What comes
+// from memory is asked for two or three rows ahead: rows that lie straight by asynchronous copies into slots of shared memory that belong
+// to the thread alone, turned rows (kShift) as loads one row ahead.
+__host__ __device__ constexpr int stages_of(int packs) { return packs >= 4 ? 3 : 4; }      // by the packs of all tensors in a stage: 1024 threads fit
+struct Group {
+    int index, threads, thread, warps, warp, lane;      // of the block's groups; a group's threads; within the group
+    __device__ __forceinline__ explicit Group(int threads_) : threads(threads_) {
+        warps = threads >> 5;
+        index = (threadIdx.x >> 5) / warps;
+        thread = threadIdx.x - index * threads;
+        warp = thread >> 5;
+        lane = threadIdx.x & 31;
+    }
+    // Two sums over the group, in all of its threads.  `red` is the group's [64] floats, another one from one call to the next.
+    __device__ __forceinline__ float2 sum(float a, float b, float* red) const {
+        a = fg_warp_sum(a);
+        b = fg_warp_sum(b);
+        if (warps == 1) return make_float2(a, b);
+        if (lane == 0) { red[warp] = a; red[32 + warp] = b; }
+        fg_group_barrier(index, threads);
+        a = fg_warp_sum(lane < warps ? red[lane] : 0.0f);
+        b = fg_warp_sum(lane < warps ? red[32 + lane] : 0.0f);
+        return make_float2(a, b);
+    }
+};
+// A block of up to 1024 threads; a group's sums alternate between four buffers (a row has two).
+constexpr int kMaxGroups = 8;
+
+template <typename T, int kPacks, bool kShift>
+__global__ void __launch_bounds__(1024) norm_held_kernel(const NormArgs a, int threads) {
+    constexpr int E = FgPack<T>::E, kStages = stages_of(kPacks);
+    extern __shared__ uint4 slots[];      // [stage][pack][thread]
+    __shared__ float red[kMaxGroups][4][64];
+    fg_grid_enter();
+    const Group group(threads);
+    const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups, first = blockIdx.x * groups + group.index;
+    const float n = (float)a.cols;
+    const T *const x = static_cast<const T*>(a.x), *const x_end = x + (uint64_t)a.rows * a.cols, *const gamma = static_cast<const T*>(a.gamma),
+            *const beta = static_cast<const T*>(a.beta);
+    uint32_t col[kPacks], left[kPacks];
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) {
+        col[k] = (group.thread + k * threads) * E;
+        left[k] = col[k] < a.cols ? min((uint32_t)E, a.cols - col[k]) : 0;
+    }
+    uint4 ahead[kPacks];
+    auto ask = [&](uint64_t r, int stage) {
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k)
+            if (r < a.rows && left[k]) {
+                if constexpr (kShift) ahead[k] = fg_load_pack<T, true>(x + r * a.cols + col[k], left[k], x, x_end);
+                else fg_copy_async(&slots[(stage * kPacks + k) * blockDim.x + threadIdx.x], x + r * a.cols + col[k]);
+            }
+        if constexpr (!kShift) fg_copies_end();
+    };
+    if constexpr (kShift) ask(first, 0);
+    else
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) ask(first + (uint64_t)i * step, i);
+    int stage = 0, turn = 0;
+    for (uint64_t r = first; r < a.rows; r += step) {
+        float v[kPacks][E];
+        if constexpr (!kShift) fg_copies_wait<kStages - 2>();
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (left[k]) {
+                if constexpr (kShift) w = ahead[k];
+                else w = slots[(stage * kPacks + k) * blockDim.x + threadIdx.x];
+            }
+            FgPack<T>::widen(w, v[k]);
+            if (kShift && left[k] < E)
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (e >= left[k]) v[k][e] = 0.0f;
+        }
+        if constexpr (kShift) ask(r + step, 0);
+        else ask(r + (uint64_t)(kStages - 1) * step, (stage + kStages - 1) % kStages);
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k)
+#pragma unroll
+            for (int e = 0; e < E; ++e) s += v[k][e];
+        const float m = group.sum(s, 0.0f, red[group.index][turn]).x / n;
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                v[k][e] -= m;
+                if (kShift ? e < left[k] : left[k] != 0) {
+                    s1 += v[k][e];
+                    s2 = __fmaf_rn(v[k][e], v[k][e], s2);
+                }
+            }
+        const float2 t = group.sum(s1, s2, red[group.index][turn + 1]);
+        const float rest = t.x / n, rstd = 1.0f / sqrtf(fmaxf(__fmaf_rn(-rest, rest, t.y / n), 0.0f) + a.eps);
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            if (!kShift && !left[k]) continue;      // (turned rows are stored by whole warps)
+            float g[E], b[E];
+            if (gamma && left[k]) FgPack<T>::widen(fg_load_pack<T, kShift>(gamma + col[k], left[k], gamma, gamma + a.cols), g);
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e) g[e] = 1.0f;
+            if (beta && left[k]) FgPack<T>::widen(fg_load_pack<T, kShift>(beta + col[k], left[k], beta, beta + a.cols), b);
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e) b[e] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) g[e] = __fmaf_rn((v[k][e] - rest) * rstd, g[e], b[e]);
+            fg_store_pack<T, kShift>(static_cast<T*>(a.y) + r * a.cols + col[k], FgPack<T>::narrow(g), left[k]);
+        }
+        if (group.thread == 0) {
+            if (a.mean) a.mean[r] = m + rest;
+            if (a.rstd) a.rstd[r] = rstd;
+        }
+        stage = (stage + 1) % kStages;
+        turn ^= 2;
+    }
+}
+
+// The backward pass the same way.  With the gradients of the parameters (kParams) a thread sums its columns over the rows of its group, a
+// block adds its groups and leaves one row of parts: [block][2][pitch].
+template <typename T, int kPacks, bool kShift, bool kParams>
+__global__ void __launch_bounds__(1024) norm_bwd_held_kernel(const NormBwdArgs a, int threads, float* parts, uint32_t pitch) {
+    constexpr int E = FgPack<T>::E, kStages = stages_of(2 * kPacks);
+    extern __shared__ uint4 slots[];      // [stage][x, dy][pack][thread]; at the end the groups' sums
+    __shared__ float red[kMaxGroups][2][64];
+    fg_grid_enter();
+    const Group group(threads);
+    const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups, first = blockIdx.x * groups + group.index;
+    const float n = (float)a.cols;
+    const uint64_t size = (uint64_t)a.rows * a.cols;
+    const T *const x = static_cast<const T*>(a.x), *const dy = static_cast<const T*>(a.dy), *const gamma = static_cast<const T*>(a.gamma);
+    T* const dx = static_cast<T*>(a.dx);
+    uint32_t col[kPacks], left[kPacks];
+    uint4 gammas[kPacks];
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) {
+        col[k] = (group.thread + k * threads) * E;
+        left[k] = col[k] < a.cols ? min((uint32_t)E, a.cols - col[k]) : 0;
+        gammas[k] = make_uint4(0, 0, 0, 0);
+        if (gamma && left[k]) gammas[k] = fg_load_pack<T, kShift>(gamma + col[k], left[k], gamma, gamma + a.cols);
+    }
+    uint4 ahead[2][kPacks];
+    float mean = 0.0f, rstd = 0.0f;
+    auto ask = [&](uint64_t r, int stage) {
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k)
+            if (r < a.rows && left[k]) {
+                const uint64_t at = r * a.cols + col[k];
+                if constexpr (kShift) {
+                    ahead[0][k] = fg_load_pack<T, true>(x + at, left[k], x, x + size);
+                    ahead[1][k] = fg_load_pack<T, true>(dy + at, left[k], dy, dy + size);
+                } else {
+                    fg_copy_async(&slots[(stage * 2 * kPacks + k) * blockDim.x + threadIdx.x], x + at);
+                    fg_copy_async(&slots[((stage * 2 + 1) * kPacks + k) * blockDim.x + threadIdx.x], dy + at);
+                }
+            }
+        if constexpr (!kShift) fg_copies_end();
+    };
+    auto ask_row = [&](uint64_t r) {
+        if (r < a.rows) { mean = a.mean[r]; rstd = a.rstd[r]; }
+    };
+    if constexpr (kShift) ask(first, 0);
+    else
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) ask(first + (uint64_t)i * step, i);
+    ask_row(first);
+    float dg[kPacks][E] = {}, db[kPacks][E] = {};
+    int stage = 0, turn = 0;
+    for (uint64_t r = first; r < a.rows; r += step) {
+        float h[kPacks][E], g[kPacks][E];
+        const float m = mean, sd = rstd;
+        ask_row(r + step);
+        if constexpr (!kShift) fg_copies_wait<kStages - 2>();
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            uint4 v = make_uint4(0, 0, 0, 0), w = v;
+            if (left[k]) {
+                if constexpr (kShift) { v = ahead[0][k]; w = ahead[1][k]; }
+                else {
+                    v = slots[(stage * 2 * kPacks + k) * blockDim.x + threadIdx.x];
+                    w = slots[((stage * 2 + 1) * kPacks + k) * blockDim.x + threadIdx.x];
+                }
+            }
+            FgPack<T>::widen(v, h[k]);
+            FgPack<T>::widen(w, g[k]);
+            if (kShift ? left[k] < E : left[k] == 0)      // columns behind the row's end count for nothing
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (e >= left[k]) { h[k][e] = m; g[k][e] = 0.0f; }
+            float gm[E];
+            if (gamma) FgPack<T>::widen(gammas[k], gm);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                h[k][e] = (h[k][e] - m) * sd;
+                if (kParams) {
+                    dg[k][e] = __fmaf_rn(g[k][e], h[k][e], dg[k][e]);
+                    db[k][e] += g[k][e];
+                }
+                if (gamma) g[k][e] *= gm[e];
+                s1 += g[k][e];
+                s2 = __fmaf_rn(g[k][e], h[k][e], s2);
+            }
+        }
+        if constexpr (kShift) ask(r + step, 0);
+        else ask(r + (uint64_t)(kStages - 1) * step, (stage + kStages - 1) % kStages);
+        if (dx) {
+            const float2 t = group.sum(s1, s2, red[group.index][turn]);
+            const float m1 = t.x / n, m2 = t.y / n;
+#pragma unroll
+            for (int k = 0; k < kPacks; ++k) {
+                if (!kShift && !left[k]) continue;
+#pragma unroll
+                for (int e = 0; e < E; ++e) g[k][e] = sd * __fmaf_rn(-h[k][e], m2, g[k][e] - m1);
+                T* const p = dx + r * a.cols + col[k];
+                if (a.accumulate_dx) {
+                    float old[E] = {};
+                    if (left[k]) FgPack<T>::widen(fg_load_pack<T, kShift>(p, left[k], dx, dx + size), old);
+                    if (kShift) __syncwarp();      // a lane writes words that others have read
+#pragma unroll
+                    for (int e = 0; e < E; ++e) g[k][e] += old[e];
+                }
+                fg_store_pack<T, kShift>(p, FgPack<T>::narrow(g[k]), left[k]);
+            }
+        }
+        stage = (stage + 1) % kStages;
+        turn ^= 1;
+    }
+    if constexpr (kParams) {
+        float* const mine = parts + (uint64_t)blockIdx.x * 2 * pitch;
+        if (groups > 1) {      // the groups one after the other, in shared memory: [2][pitch]
+            if constexpr (!kShift) fg_copies_wait<0>();
+            float* const sums = reinterpret_cast<float*>(slots);
+            for (uint32_t i = 0; i < groups; ++i) {
+                __syncthreads();
+                if (group.index == (int)i)
+#pragma unroll
+                    for (int k = 0; k < kPacks; ++k)
+                        if (left[k])
+#pragma unroll
+                            for (int e = 0; e < E; ++e) {
+                                float *const p = sums + col[k] + e, *const q = p + pitch;
+                                const float u = i ? *p + dg[k][e] : dg[k][e], w = i ? *q + db[k][e] : db[k][e];
+                                if (i + 1 < groups) { *p = u; *q = w; }
+                                else { mine[col[k] + e] = u; mine[pitch + col[k] + e] = w; }
+                            }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPacks; ++k)
+                if (left[k])
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) {
+                        *reinterpret_cast<float4*>(mine + col[k] + e) = make_float4(dg[k][e], dg[k][e + 1], dg[k][e + 2], dg[k][e + 3]);
+                        *reinterpret_cast<float4*>(mine + pitch + col[k] + e) = make_float4(db[k][e], db[k][e + 1], db[k][e + 2], db[k][e + 3]);
+                    }
+        }
+    }
+}
+
+// Adds the blocks' parts: 128 columns per block, a warp takes every 32nd part.  pitch is a multiple of 128.
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_parts_kernel(const NormBwdArgs a, const float* parts, uint32_t count, uint32_t pitch) {
+    __shared__ float4 red[32][32];
+    fg_grid_enter();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t at = blockIdx.x * 128 + 4 * lane;      // dgamma's columns, then dbeta's
+    T* const out = static_cast<T*>(at < pitch ? a.dgamma : a.dbeta);
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t i0 = warp; i0 < count; i0 += 32 * 8) {
+        float4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            v[j] = i0 + 32 * j < count ? *reinterpret_cast<const float4*>(parts + (uint64_t)(i0 + 32 * j) * 2 * pitch + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { s.x += v[j].x; s.y += v[j].y; s.z += v[j].z; s.w += v[j].w; }
+    }
+    red[warp][lane] = s;
+    __syncthreads();
+    if (threadIdx.x < 128) {
+        const uint32_t c = blockIdx.x * 128 + threadIdx.x - (at < pitch ? 0 : pitch);
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 32; ++w) sum += reinterpret_cast<const float*>(red[w])[threadIdx.x];
+        if (out && c < a.cols) out[c] = fg_narrow<T>(a.accumulate_params ? fg_widen(out[c]) + sum : sum);
+    }
+}
+
 // Any row: one block each, the row read once per sum.
 template <typename T>
 __global__ void __launch_bounds__(256) norm_stream_kernel(const NormArgs a) {
@@ -121,22 +414,97 @@ __global__ void __launch_bounds__(256) norm_fold_kernel(const NormBwdArgs a, con
 
 int rows_grid(const fg_ctx* ctx, uint32_t rows) { return (int)(rows < 8u * ctx->sm_count ? rows : 8u * ctx->sm_count); }
 
+// How a kernel that holds rows is launched: packs per thread, the threads of a group, the groups of a block, its shared memory, the blocks.
+struct HeldPlan { int packs, threads, groups; size_t bytes; int grid; };
+// Threads hold up to `most` packs; of few rows, and where a warp is enough, one each.
+HeldPlan held_plan(const fg_ctx* ctx, uint32_t rows, uint32_t cols, uint32_t elements, int most, int block, int slots) {
+    const uint64_t packs = ((uint64_t)cols + elements - 1) / elements;
+    HeldPlan p{1, 0, 1, 0, 0};
+    while (p.packs < most && (packs > 1024ull * p.packs || (rows > 2u * ctx->sm_count && packs > 32ull * p.packs))) p.packs *= 2;
+    if (packs > 1024ull * p.packs) return p;      // threads = 0: no
+    p.threads = (int)((packs + 32 * p.packs - 1) / (32 * p.packs) * 32);
+    p.groups = block / p.threads < 1 ? 1 : block / p.threads > kMaxGroups ? kMaxGroups : block / p.threads;
+    while (p.groups > 1 && (uint64_t)rows * 2 <= (uint64_t)p.groups * ctx->sm_count) p.groups /= 2;      // few rows: over the SMs first
+    p.bytes = sizeof(uint4) * stages_of(slots * p.packs) * slots * p.packs * p.threads * p.groups;
+    // What the SMs hold at once: 1024 threads of 64 registers, 220 KB with the static part.
+    const uint64_t by_threads = 1024 / (p.threads * p.groups), by_memory = 220 * 1024 / (p.bytes + 9 * 1024), per_sm = by_threads < by_memory ? by_threads : by_memory;
+    const uint64_t need = ((uint64_t)rows + p.groups - 1) / p.groups, cap = (uint64_t)ctx->sm_count * (per_sm ? per_sm : 1);
+    p.grid = (int)(need < cap ? need : cap);
+    return p;
+}
+template <typename K>
+int32_t allow_shared(fg_ctx* ctx, K kernel, size_t bytes) {
+    if (bytes > 32 * 1024) FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    return FG_OK;
+}
+
+template <typename T, int kPacks, bool kShift>
+int32_t launch_held(fg_ctx* ctx, const NormArgs& a, HeldPlan p) {
+    const size_t bytes = p.bytes;
+    const int32_t s = allow_shared(ctx, norm_held_kernel<T, kPacks, kShift>, bytes);
+    if (s != FG_OK) return s;
+    fg_launch(ctx, norm_held_kernel<T, kPacks, kShift>, p.grid, p.threads * p.groups, bytes, a, p.threads);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
+}
 template <typename T>
 int32_t norm_fwd(fg_ctx* ctx, const NormArgs& a) {
+    const bool straight = fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.y, a.gamma, a.beta);
+    const HeldPlan p = held_plan(ctx, a.rows, a.cols, FgPack<T>::E, straight || sizeof(T) == 4 ? 4 : 2, 256, straight ? 1 : 0);
+    if (p.threads) {
+        if (straight) return p.packs == 1 ? launch_held<T, 1, false>(ctx, a, p) : p.packs == 2 ? launch_held<T, 2, false>(ctx, a, p) : launch_held<T, 4, false>(ctx, a, p);
+        if (p.packs == 1) return launch_held<T, 1, true>(ctx, a, p);
+        if (p.packs == 2) return launch_held<T, 2, true>(ctx, a, p);
+        if constexpr (sizeof(T) == 4) return launch_held<T, 4, true>(ctx, a, p);
+    }
     fg_launch(ctx, norm_stream_kernel<T>, rows_grid(ctx, a.rows), 256, 0, a);
     FG_LAUNCHED(ctx);
     return FG_OK;
 }
 
+template <typename T, int kPacks, bool kShift, bool kParams>
+int32_t launch_bwd_held(fg_ctx* ctx, const NormBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch) {
+    const size_t sums = kParams && p.groups > 1 ? 8ull * pitch : 0, bytes = p.bytes < sums ? sums : p.bytes;
+    const int32_t s = allow_shared(ctx, norm_bwd_held_kernel<T, kPacks, kShift, kParams>, bytes);
+    if (s != FG_OK) return s;
+    fg_launch(ctx, norm_bwd_held_kernel<T, kPacks, kShift, kParams>, p.grid, p.threads * p.groups, bytes, a, p.threads, parts, pitch);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
+}
+template <typename T, int kPacks>
+int32_t choose_bwd_held(fg_ctx* ctx, const NormBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch, bool straight) {
+    if (parts) return straight ? launch_bwd_held<T, kPacks, false, true>(ctx, a, p, parts, pitch) : launch_bwd_held<T, kPacks, true, true>(ctx, a, p, parts, pitch);
+    return straight ? launch_bwd_held<T, kPacks, false, false>(ctx, a, p, parts, pitch) : launch_bwd_held<T, kPacks, true, false>(ctx, a, p, parts, pitch);
+}
+
 template <typename T>
 int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
+    const bool straight = fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.dy, a.gamma, a.dx);
+    const HeldPlan p = held_plan(ctx, a.rows, a.cols, FgPack<T>::E, sizeof(T) == 4 ? 2 : 1, 512, straight ? 2 : 0);
+    if (p.threads) {
+        float* parts = nullptr;
+        const uint32_t pitch = (a.cols + 127) / 128 * 128;
+        if (a.dgamma || a.dbeta) {
+            void* w;
+            const int32_t s = fg_ws_alloc(ctx, 8ull * pitch * p.grid, &w);
+            if (s != FG_OK) return s;
+            parts = (float*)w;
+        }
+        int32_t s = FG_OK;
+        if (p.packs == 1) s = choose_bwd_held<T, 1>(ctx, a, p, parts, pitch, straight);
+        else if constexpr (sizeof(T) == 4) s = choose_bwd_held<T, 2>(ctx, a, p, parts, pitch, straight);
+        if (s != FG_OK || !parts) return s;
+        fg_launch(ctx, norm_parts_kernel<T>, pitch / 64, 1024, 0, a, (const float*)parts, (uint32_t)p.grid, pitch);
+        FG_LAUNCHED(ctx);
+        return FG_OK;
+    }
     float* part = nullptr;
     const uint32_t chunks = (a.rows + kChunk - 1) / kChunk;
     if (a.dgamma || a.dbeta) {      // before dx, which may be dy or x
-        void* p;
-        const int32_t s = fg_ws_alloc(ctx, 8ull * chunks * a.cols, &p);
+        void* w;
+        const int32_t s = fg_ws_alloc(ctx, 8ull * chunks * a.cols, &w);
         if (s != FG_OK) return s;
-        part = (float*)p;
+        part = (float*)w;
         fg_launch(ctx, norm_columns_kernel<T>, dim3((a.cols + 31) / 32, chunks), dim3(32, 8), 0, a, part);
         FG_LAUNCHED(ctx);
         fg_launch(ctx, norm_fold_kernel<T>, dim3((a.cols + 255) / 256, 2), 256, 0, a, (const float*)part, chunks);

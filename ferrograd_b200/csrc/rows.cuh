@@ -29,6 +29,16 @@ __device__ __forceinline__ float fg_warp_sum(float v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+// A barrier over one of a block's groups of warps (0 to 14).
+__device__ __forceinline__ void fg_group_barrier(int group, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory"); }
+// Sixteen bytes on their way from memory to shared memory, past the L1; a thread waits for its own.
+__device__ __forceinline__ void fg_copy_async(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void fg_copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>      // all but the last kLeft groups have arrived
+__device__ __forceinline__ void fg_copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
 // Two sums over a block of whole warps, in every thread; `red` is 64 floats, free again after the call's last barrier.
 __device__ __forceinline__ float2 fg_block_sum2(float a, float b, float* red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
