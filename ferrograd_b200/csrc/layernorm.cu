@@ -27,7 +27,7 @@ struct NormBwdArgs {
 // A group of warps takes a row at a time, a thread the same columns of each: pack `thread`, `thread` + threads, ... of 16 bytes.  What comes
 // from memory is asked for two or three rows ahead: rows that lie straight by asynchronous copies into slots of shared memory that belong
 // to the thread alone, turned rows (kShift) as loads one row ahead.
-__host__ __device__ constexpr int stages_of(int packs) { return packs >= 4 ? 3 : 4; }      // by the packs of all tensors in a stage: 1024 threads fit
+__host__ __device__ constexpr int stages_of(int packs) { return packs >= 8 ? 3 : 4; }      // by the packs of all tensors in a stage: 512 threads fit
 struct Group {
     int index, threads, thread, warps, warp, lane;      // of the block's groups; a group's threads; within the group
     __device__ __forceinline__ explicit Group(int threads_) : threads(threads_) {
@@ -49,34 +49,44 @@ struct Group {
         return make_float2(a, b);
     }
 };
-// A block of up to 1024 threads; a group's sums alternate between four buffers (a row has two).
 constexpr int kMaxGroups = 8;
 
 template <typename T, int kPacks, bool kShift>
-__global__ void __launch_bounds__(1024) norm_held_kernel(const NormArgs a, int threads) {
-    constexpr int E = FgPack<T>::E, kStages = stages_of(kPacks);
+__global__ void __launch_bounds__(512) norm_held_kernel(const NormArgs a, int threads) {
+    constexpr int E = FgPack<T>::E, P = E / 2, kStages = stages_of(kPacks);
+    constexpr bool kHeldParams = kPacks <= 4;      // gamma and beta stay in registers
     extern __shared__ uint4 slots[];      // [stage][pack][thread]
     __shared__ float red[kMaxGroups][4][64];
     fg_grid_enter();
     const Group group(threads);
     const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups, first = blockIdx.x * groups + group.index;
-    const float n = (float)a.cols;
+    const float n = (float)a.cols, inv_n = 1.0f / n;
     const T *const x = static_cast<const T*>(a.x), *const x_end = x + (uint64_t)a.rows * a.cols, *const gamma = static_cast<const T*>(a.gamma),
             *const beta = static_cast<const T*>(a.beta);
     uint32_t col[kPacks], left[kPacks];
+    uint4 gammas[kHeldParams ? kPacks : 1], betas[kHeldParams ? kPacks : 1];
+    auto load_params = [&](int k, uint4& g, uint4& b) {
+        g = b = make_uint4(0, 0, 0, 0);
+        if (gamma && left[k]) g = fg_load_pack<T, kShift>(gamma + col[k], left[k], gamma, gamma + a.cols);
+        if (beta && left[k]) b = fg_load_pack<T, kShift>(beta + col[k], left[k], beta, beta + a.cols);
+    };
 #pragma unroll
     for (int k = 0; k < kPacks; ++k) {
         col[k] = (group.thread + k * threads) * E;
         left[k] = col[k] < a.cols ? min((uint32_t)E, a.cols - col[k]) : 0;
+        if constexpr (kHeldParams) load_params(k, gammas[k], betas[k]);
     }
     uint4 ahead[kPacks];
     auto ask = [&](uint64_t r, int stage) {
+        if (r < a.rows) {
+            const T* const row = x + r * a.cols;
 #pragma unroll
-        for (int k = 0; k < kPacks; ++k)
-            if (r < a.rows && left[k]) {
-                if constexpr (kShift) ahead[k] = fg_load_pack<T, true>(x + r * a.cols + col[k], left[k], x, x_end);
-                else fg_copy_async(&slots[(stage * kPacks + k) * blockDim.x + threadIdx.x], x + r * a.cols + col[k]);
-            }
+            for (int k = 0; k < kPacks; ++k)
+                if (left[k]) {
+                    if constexpr (kShift) ahead[k] = fg_load_pack<T, true>(row + col[k], left[k], x, x_end);
+                    else fg_copy_async(&slots[(stage * kPacks + k) * blockDim.x + threadIdx.x], row + col[k]);
+                }
+        }
         if constexpr (!kShift) fg_copies_end();
     };
     if constexpr (kShift) ask(first, 0);
@@ -85,8 +95,9 @@ __global__ void __launch_bounds__(1024) norm_held_kernel(const NormArgs a, int t
         for (int i = 0; i < kStages - 1; ++i) ask(first + (uint64_t)i * step, i);
     int stage = 0, turn = 0;
     for (uint64_t r = first; r < a.rows; r += step) {
-        float v[kPacks][E];
+        float2 v[kPacks][P];
         if constexpr (!kShift) fg_copies_wait<kStages - 2>();
+        float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int k = 0; k < kPacks; ++k) {
             uint4 w = make_uint4(0, 0, 0, 0);
@@ -97,66 +108,75 @@ __global__ void __launch_bounds__(1024) norm_held_kernel(const NormArgs a, int t
             FgPack<T>::widen(w, v[k]);
             if (kShift && left[k] < E)
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (e >= left[k]) v[k][e] = 0.0f;
+                for (int e = 0; e < P; ++e) {
+                    if (2 * e >= left[k]) v[k][e].x = 0.0f;
+                    if (2 * e + 1 >= left[k]) v[k][e].y = 0.0f;
+                }
+#pragma unroll
+            for (int e = 0; e < P; ++e) s = fg_add2(s, v[k][e]);
         }
         if constexpr (kShift) ask(r + step, 0);
-        else ask(r + (uint64_t)(kStages - 1) * step, (stage + kStages - 1) % kStages);
-        float s = 0.0f;
+        else ask(r + (uint64_t)(kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
+        const float m = group.sum(s.x + s.y, 0.0f, red[group.index][turn]).x / n;
+        const float2 less = make_float2(-m, -m);
+        float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
 #pragma unroll
-        for (int k = 0; k < kPacks; ++k)
+        for (int k = 0; k < kPacks; ++k) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) s += v[k][e];
-        const float m = group.sum(s, 0.0f, red[group.index][turn]).x / n;
-        float s1 = 0.0f, s2 = 0.0f;
+            for (int e = 0; e < P; ++e) v[k][e] = fg_add2(v[k][e], less);
+            if (left[k] < E)      // columns behind the row's end count for nothing
 #pragma unroll
-        for (int k = 0; k < kPacks; ++k)
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                v[k][e] -= m;
-                if (kShift ? e < left[k] : left[k] != 0) {
-                    s1 += v[k][e];
-                    s2 = __fmaf_rn(v[k][e], v[k][e], s2);
+                for (int e = 0; e < P; ++e) {
+                    if (2 * e >= left[k]) v[k][e].x = 0.0f;
+                    if (2 * e + 1 >= left[k]) v[k][e].y = 0.0f;
                 }
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                s1 = fg_add2(s1, v[k][e]);
+                s2 = fg_fma2(v[k][e], v[k][e], s2);
             }
-        const float2 t = group.sum(s1, s2, red[group.index][turn + 1]);
-        const float rest = t.x / n, rstd = 1.0f / sqrtf(fmaxf(__fmaf_rn(-rest, rest, t.y / n), 0.0f) + a.eps);
+        }
+        const float2 t = group.sum(s1.x + s1.y, s2.x + s2.y, red[group.index][turn + 1]);
+        const float rest = t.x * inv_n, rstd = 1.0f / sqrtf(fmaxf(__fmaf_rn(-rest, rest, t.y * inv_n), 0.0f) + a.eps);
+        T* const out = static_cast<T*>(a.y) + r * a.cols;
+        const float2 less_rest = make_float2(-rest, -rest), by = make_float2(rstd, rstd);
 #pragma unroll
         for (int k = 0; k < kPacks; ++k) {
             if (!kShift && !left[k]) continue;      // (turned rows are stored by whole warps)
-            float g[E], b[E];
-            if (gamma && left[k]) FgPack<T>::widen(fg_load_pack<T, kShift>(gamma + col[k], left[k], gamma, gamma + a.cols), g);
-            else
+            uint4 gw, bw;
+            if constexpr (kHeldParams) { gw = gammas[k]; bw = betas[k]; }
+            else load_params(k, gw, bw);
+            float2 g[P], b[P];
+            FgPack<T>::widen(gw, g);
+            FgPack<T>::widen(bw, b);
 #pragma unroll
-                for (int e = 0; e < E; ++e) g[e] = 1.0f;
-            if (beta && left[k]) FgPack<T>::widen(fg_load_pack<T, kShift>(beta + col[k], left[k], beta, beta + a.cols), b);
-            else
-#pragma unroll
-                for (int e = 0; e < E; ++e) b[e] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) g[e] = __fmaf_rn((v[k][e] - rest) * rstd, g[e], b[e]);
-            fg_store_pack<T, kShift>(static_cast<T*>(a.y) + r * a.cols + col[k], FgPack<T>::narrow(g), left[k]);
+            for (int e = 0; e < P; ++e) {
+                const float2 h = fg_mul2(fg_add2(v[k][e], less_rest), by);
+                g[e] = gamma ? fg_fma2(h, g[e], b[e]) : fg_add2(h, b[e]);
+            }
+            fg_store_pack<T, kShift>(out + col[k], FgPack<T>::narrow(g), left[k]);
         }
         if (group.thread == 0) {
             if (a.mean) a.mean[r] = m + rest;
             if (a.rstd) a.rstd[r] = rstd;
         }
-        stage = (stage + 1) % kStages;
+        stage = stage == kStages - 1 ? 0 : stage + 1;
         turn ^= 2;
     }
 }
 
-// The backward pass the same way.  With the gradients of the parameters (kParams) a thread sums its columns over the rows of its group, a
-// block adds its groups and leaves one row of parts: [block][2][pitch].
+// The backward pass the same way, 16 columns at most per thread.  With the gradients of the parameters (kParams) a thread sums its columns
+// over the rows of its group, a block adds its groups and leaves one row of parts: [block][2][pitch].
+// With c = x - mean, dx = rstd * g + (-rstd * m1) + c * (-rstd^2 * m2), where m1 and m2 are the means of g and of g * h.
 template <typename T, int kPacks, bool kShift, bool kParams>
-__global__ void __launch_bounds__(1024) norm_bwd_held_kernel(const NormBwdArgs a, int threads, float* parts, uint32_t pitch) {
-    constexpr int E = FgPack<T>::E, kStages = stages_of(2 * kPacks);
+__global__ void __launch_bounds__(512) norm_bwd_held_kernel(const NormBwdArgs a, int threads, float* parts, uint32_t pitch) {
+    constexpr int E = FgPack<T>::E, P = E / 2, kStages = stages_of(2 * kPacks);
     extern __shared__ uint4 slots[];      // [stage][x, dy][pack][thread]; at the end the groups' sums
     __shared__ float red[kMaxGroups][2][64];
     fg_grid_enter();
     const Group group(threads);
     const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups, first = blockIdx.x * groups + group.index;
-    const float n = (float)a.cols;
+    const float inv_n = 1.0f / (float)a.cols;
     const uint64_t size = (uint64_t)a.rows * a.cols;
     const T *const x = static_cast<const T*>(a.x), *const dy = static_cast<const T*>(a.dy), *const gamma = static_cast<const T*>(a.gamma);
     T* const dx = static_cast<T*>(a.dx);
@@ -172,18 +192,20 @@ __global__ void __launch_bounds__(1024) norm_bwd_held_kernel(const NormBwdArgs a
     uint4 ahead[2][kPacks];
     float mean = 0.0f, rstd = 0.0f;
     auto ask = [&](uint64_t r, int stage) {
+        if (r < a.rows) {
+            const T *const x_row = x + r * a.cols, *const dy_row = dy + r * a.cols;
 #pragma unroll
-        for (int k = 0; k < kPacks; ++k)
-            if (r < a.rows && left[k]) {
-                const uint64_t at = r * a.cols + col[k];
-                if constexpr (kShift) {
-                    ahead[0][k] = fg_load_pack<T, true>(x + at, left[k], x, x + size);
-                    ahead[1][k] = fg_load_pack<T, true>(dy + at, left[k], dy, dy + size);
-                } else {
-                    fg_copy_async(&slots[(stage * 2 * kPacks + k) * blockDim.x + threadIdx.x], x + at);
-                    fg_copy_async(&slots[((stage * 2 + 1) * kPacks + k) * blockDim.x + threadIdx.x], dy + at);
+            for (int k = 0; k < kPacks; ++k)
+                if (left[k]) {
+                    if constexpr (kShift) {
+                        ahead[0][k] = fg_load_pack<T, true>(x_row + col[k], left[k], x, x + size);
+                        ahead[1][k] = fg_load_pack<T, true>(dy_row + col[k], left[k], dy, dy + size);
+                    } else {
+                        fg_copy_async(&slots[(stage * 2 * kPacks + k) * blockDim.x + threadIdx.x], x_row + col[k]);
+                        fg_copy_async(&slots[((stage * 2 + 1) * kPacks + k) * blockDim.x + threadIdx.x], dy_row + col[k]);
+                    }
                 }
-            }
+        }
         if constexpr (!kShift) fg_copies_end();
     };
     auto ask_row = [&](uint64_t r) {
@@ -194,14 +216,19 @@ __global__ void __launch_bounds__(1024) norm_bwd_held_kernel(const NormBwdArgs a
 #pragma unroll
         for (int i = 0; i < kStages - 1; ++i) ask(first + (uint64_t)i * step, i);
     ask_row(first);
-    float dg[kPacks][E] = {}, db[kPacks][E] = {};
+    float2 dg[kPacks][P], db[kPacks][P];
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k)
+#pragma unroll
+        for (int e = 0; e < P; ++e) dg[k][e] = db[k][e] = make_float2(0.0f, 0.0f);
     int stage = 0, turn = 0;
     for (uint64_t r = first; r < a.rows; r += step) {
-        float h[kPacks][E], g[kPacks][E];
+        float2 c[kPacks][P], g[kPacks][P];
         const float m = mean, sd = rstd;
+        const float2 less = make_float2(-m, -m), by = make_float2(sd, sd);
         ask_row(r + step);
         if constexpr (!kShift) fg_copies_wait<kStages - 2>();
-        float s1 = 0.0f, s2 = 0.0f;
+        float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
 #pragma unroll
         for (int k = 0; k < kPacks; ++k) {
             uint4 v = make_uint4(0, 0, 0, 0), w = v;
@@ -212,77 +239,81 @@ __global__ void __launch_bounds__(1024) norm_bwd_held_kernel(const NormBwdArgs a
                     w = slots[((stage * 2 + 1) * kPacks + k) * blockDim.x + threadIdx.x];
                 }
             }
-            FgPack<T>::widen(v, h[k]);
+            FgPack<T>::widen(v, c[k]);
             FgPack<T>::widen(w, g[k]);
-            if (kShift ? left[k] < E : left[k] == 0)      // columns behind the row's end count for nothing
+            float2 gm[P];
+            FgPack<T>::widen(gammas[k], gm);
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (e >= left[k]) { h[k][e] = m; g[k][e] = 0.0f; }
-            float gm[E];
-            if (gamma) FgPack<T>::widen(gammas[k], gm);
+            for (int e = 0; e < P; ++e) c[k][e] = fg_add2(c[k][e], less);
+            if (left[k] < E)      // columns behind the row's end count for nothing
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                h[k][e] = (h[k][e] - m) * sd;
-                if (kParams) {
-                    dg[k][e] = __fmaf_rn(g[k][e], h[k][e], dg[k][e]);
-                    db[k][e] += g[k][e];
+                for (int e = 0; e < P; ++e) {
+                    if (2 * e >= left[k]) c[k][e].x = g[k][e].x = 0.0f;
+                    if (2 * e + 1 >= left[k]) c[k][e].y = g[k][e].y = 0.0f;
                 }
-                if (gamma) g[k][e] *= gm[e];
-                s1 += g[k][e];
-                s2 = __fmaf_rn(g[k][e], h[k][e], s2);
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                if (kParams) {
+                    dg[k][e] = fg_fma2(g[k][e], fg_mul2(c[k][e], by), dg[k][e]);
+                    db[k][e] = fg_add2(db[k][e], g[k][e]);
+                }
+                if (gamma) g[k][e] = fg_mul2(g[k][e], gm[e]);
+                s1 = fg_add2(s1, g[k][e]);
+                s2 = fg_fma2(g[k][e], c[k][e], s2);
             }
         }
         if constexpr (kShift) ask(r + step, 0);
-        else ask(r + (uint64_t)(kStages - 1) * step, (stage + kStages - 1) % kStages);
+        else ask(r + (uint64_t)(kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
         if (dx) {
-            const float2 t = group.sum(s1, s2, red[group.index][turn]);
-            const float m1 = t.x / n, m2 = t.y / n;
+            const float2 t = group.sum(s1.x + s1.y, s2.x + s2.y, red[group.index][turn]);
+            const float u1 = -sd * (t.x * inv_n), u2 = -sd * sd * (sd * (t.y * inv_n));
+            const float2 add = make_float2(u1, u1), slope = make_float2(u2, u2);
+            T* const row = dx + r * a.cols;
 #pragma unroll
             for (int k = 0; k < kPacks; ++k) {
                 if (!kShift && !left[k]) continue;
 #pragma unroll
-                for (int e = 0; e < E; ++e) g[k][e] = sd * __fmaf_rn(-h[k][e], m2, g[k][e] - m1);
-                T* const p = dx + r * a.cols + col[k];
+                for (int e = 0; e < P; ++e) g[k][e] = fg_fma2(g[k][e], by, fg_fma2(c[k][e], slope, add));
                 if (a.accumulate_dx) {
-                    float old[E] = {};
-                    if (left[k]) FgPack<T>::widen(fg_load_pack<T, kShift>(p, left[k], dx, dx + size), old);
+                    float2 old[P];
+                    FgPack<T>::widen(left[k] ? fg_load_pack<T, kShift>(row + col[k], left[k], dx, dx + size) : make_uint4(0, 0, 0, 0), old);
                     if (kShift) __syncwarp();      // a lane writes words that others have read
 #pragma unroll
-                    for (int e = 0; e < E; ++e) g[k][e] += old[e];
+                    for (int e = 0; e < P; ++e) g[k][e] = fg_add2(g[k][e], old[e]);
                 }
-                fg_store_pack<T, kShift>(p, FgPack<T>::narrow(g[k]), left[k]);
+                fg_store_pack<T, kShift>(row + col[k], FgPack<T>::narrow(g[k]), left[k]);
             }
         }
-        stage = (stage + 1) % kStages;
+        stage = stage == kStages - 1 ? 0 : stage + 1;
         turn ^= 1;
     }
     if constexpr (kParams) {
-        float* const mine = parts + (uint64_t)blockIdx.x * 2 * pitch;
-        if (groups > 1) {      // the groups one after the other, in shared memory: [2][pitch]
-            if constexpr (!kShift) fg_copies_wait<0>();
-            float* const sums = reinterpret_cast<float*>(slots);
-            for (uint32_t i = 0; i < groups; ++i) {
-                __syncthreads();
-                if (group.index == (int)i)
+        // the groups one after the other, in shared memory: [2][pack][pair][thread]
+        float2* const sums = reinterpret_cast<float2*>(slots);
+        if constexpr (!kShift) fg_copies_wait<0>();
+        for (uint32_t i = 0; i + 1 < groups; ++i) {
+            __syncthreads();
+            if (group.index == (int)i)
 #pragma unroll
-                    for (int k = 0; k < kPacks; ++k)
-                        if (left[k])
+                for (int k = 0; k < kPacks; ++k)
 #pragma unroll
-                            for (int e = 0; e < E; ++e) {
-                                float *const p = sums + col[k] + e, *const q = p + pitch;
-                                const float u = i ? *p + dg[k][e] : dg[k][e], w = i ? *q + db[k][e] : db[k][e];
-                                if (i + 1 < groups) { *p = u; *q = w; }
-                                else { mine[col[k] + e] = u; mine[pitch + col[k] + e] = w; }
-                            }
-            }
-        } else {
+                    for (int e = 0; e < P; ++e) {
+                        float2 *const p = sums + (k * P + e) * threads + group.thread, *const q = p + kPacks * P * threads;
+                        *p = i ? fg_add2(*p, dg[k][e]) : dg[k][e];
+                        *q = i ? fg_add2(*q, db[k][e]) : db[k][e];
+                    }
+        }
+        __syncthreads();
+        if (group.index + 1 == (int)groups) {
+            float* const mine = parts + (uint64_t)blockIdx.x * 2 * pitch;
 #pragma unroll
             for (int k = 0; k < kPacks; ++k)
                 if (left[k])
 #pragma unroll
-                    for (int e = 0; e < E; e += 4) {
-                        *reinterpret_cast<float4*>(mine + col[k] + e) = make_float4(dg[k][e], dg[k][e + 1], dg[k][e + 2], dg[k][e + 3]);
-                        *reinterpret_cast<float4*>(mine + pitch + col[k] + e) = make_float4(db[k][e], db[k][e + 1], db[k][e + 2], db[k][e + 3]);
+                    for (int e = 0; e < P; ++e) {
+                        const float2 *const p = sums + (k * P + e) * threads + group.thread, *const q = p + kPacks * P * threads;
+                        *reinterpret_cast<float2*>(mine + col[k] + 2 * e) = groups > 1 ? fg_add2(*p, dg[k][e]) : dg[k][e];
+                        *reinterpret_cast<float2*>(mine + pitch + col[k] + 2 * e) = groups > 1 ? fg_add2(*q, db[k][e]) : db[k][e];
                     }
         }
     }
@@ -416,18 +447,18 @@ int rows_grid(const fg_ctx* ctx, uint32_t rows) { return (int)(rows < 8u * ctx->
 
 // How a kernel that holds rows is launched: packs per thread, the threads of a group, the groups of a block, its shared memory, the blocks.
 struct HeldPlan { int packs, threads, groups; size_t bytes; int grid; };
-// Threads hold up to `most` packs; of few rows, and where a warp is enough, one each.
-HeldPlan held_plan(const fg_ctx* ctx, uint32_t rows, uint32_t cols, uint32_t elements, int most, int block, int slots) {
+// A block has 256 threads or, for a longer row, up to 512.  Threads hold up to `most` packs; of few rows, and where a warp is enough, one.
+HeldPlan held_plan(const fg_ctx* ctx, uint32_t rows, uint32_t cols, uint32_t elements, int most, int slots) {
     const uint64_t packs = ((uint64_t)cols + elements - 1) / elements;
     HeldPlan p{1, 0, 1, 0, 0};
-    while (p.packs < most && (packs > 1024ull * p.packs || (rows > 2u * ctx->sm_count && packs > 32ull * p.packs))) p.packs *= 2;
-    if (packs > 1024ull * p.packs) return p;      // threads = 0: no
+    while (p.packs < most && (packs > 512ull * p.packs || (p.packs < 4 && rows > 2u * ctx->sm_count && packs > 32ull * p.packs))) p.packs *= 2;
+    if (packs > 512ull * p.packs) return p;      // threads = 0: no
     p.threads = (int)((packs + 32 * p.packs - 1) / (32 * p.packs) * 32);
-    p.groups = block / p.threads < 1 ? 1 : block / p.threads > kMaxGroups ? kMaxGroups : block / p.threads;
+    p.groups = 256 / p.threads < 1 ? 1 : 256 / p.threads;
     while (p.groups > 1 && (uint64_t)rows * 2 <= (uint64_t)p.groups * ctx->sm_count) p.groups /= 2;      // few rows: over the SMs first
     p.bytes = sizeof(uint4) * stages_of(slots * p.packs) * slots * p.packs * p.threads * p.groups;
-    // What the SMs hold at once: 1024 threads of 64 registers, 220 KB with the static part.
-    const uint64_t by_threads = 1024 / (p.threads * p.groups), by_memory = 220 * 1024 / (p.bytes + 9 * 1024), per_sm = by_threads < by_memory ? by_threads : by_memory;
+    // What the SMs hold at once: 512 threads of 128 registers, 220 KB with the static part.
+    const uint64_t by_threads = 512 / (p.threads * p.groups), by_memory = 220 * 1024 / (p.bytes + 9 * 1024), per_sm = by_threads < by_memory ? by_threads : by_memory;
     const uint64_t need = ((uint64_t)rows + p.groups - 1) / p.groups, cap = (uint64_t)ctx->sm_count * (per_sm ? per_sm : 1);
     p.grid = (int)(need < cap ? need : cap);
     return p;
@@ -447,16 +478,16 @@ int32_t launch_held(fg_ctx* ctx, const NormArgs& a, HeldPlan p) {
     FG_LAUNCHED(ctx);
     return FG_OK;
 }
+template <typename T, bool kShift>
+int32_t choose_held(fg_ctx* ctx, const NormArgs& a, HeldPlan p) {
+    return p.packs == 1 ? launch_held<T, 1, kShift>(ctx, a, p) : p.packs == 2 ? launch_held<T, 2, kShift>(ctx, a, p)
+           : p.packs == 4 ? launch_held<T, 4, kShift>(ctx, a, p) : launch_held<T, 8, kShift>(ctx, a, p);
+}
 template <typename T>
 int32_t norm_fwd(fg_ctx* ctx, const NormArgs& a) {
     const bool straight = fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.y, a.gamma, a.beta);
-    const HeldPlan p = held_plan(ctx, a.rows, a.cols, FgPack<T>::E, straight || sizeof(T) == 4 ? 4 : 2, 256, straight ? 1 : 0);
-    if (p.threads) {
-        if (straight) return p.packs == 1 ? launch_held<T, 1, false>(ctx, a, p) : p.packs == 2 ? launch_held<T, 2, false>(ctx, a, p) : launch_held<T, 4, false>(ctx, a, p);
-        if (p.packs == 1) return launch_held<T, 1, true>(ctx, a, p);
-        if (p.packs == 2) return launch_held<T, 2, true>(ctx, a, p);
-        if constexpr (sizeof(T) == 4) return launch_held<T, 4, true>(ctx, a, p);
-    }
+    const HeldPlan p = held_plan(ctx, a.rows, a.cols, FgPack<T>::E, 8, straight ? 1 : 0);
+    if (p.threads) return straight ? choose_held<T, false>(ctx, a, p) : choose_held<T, true>(ctx, a, p);
     fg_launch(ctx, norm_stream_kernel<T>, rows_grid(ctx, a.rows), 256, 0, a);
     FG_LAUNCHED(ctx);
     return FG_OK;
@@ -464,7 +495,7 @@ int32_t norm_fwd(fg_ctx* ctx, const NormArgs& a) {
 
 template <typename T, int kPacks, bool kShift, bool kParams>
 int32_t launch_bwd_held(fg_ctx* ctx, const NormBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch) {
-    const size_t sums = kParams && p.groups > 1 ? 8ull * pitch : 0, bytes = p.bytes < sums ? sums : p.bytes;
+    const size_t sums = kParams && p.groups > 1 ? 8ull * FgPack<T>::E * kPacks * p.threads : 0, bytes = p.bytes < sums ? sums : p.bytes;
     const int32_t s = allow_shared(ctx, norm_bwd_held_kernel<T, kPacks, kShift, kParams>, bytes);
     if (s != FG_OK) return s;
     fg_launch(ctx, norm_bwd_held_kernel<T, kPacks, kShift, kParams>, p.grid, p.threads * p.groups, bytes, a, p.threads, parts, pitch);
@@ -480,7 +511,7 @@ int32_t choose_bwd_held(fg_ctx* ctx, const NormBwdArgs& a, HeldPlan p, float* pa
 template <typename T>
 int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
     const bool straight = fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.dy, a.gamma, a.dx);
-    const HeldPlan p = held_plan(ctx, a.rows, a.cols, FgPack<T>::E, sizeof(T) == 4 ? 2 : 1, 512, straight ? 2 : 0);
+    const HeldPlan p = held_plan(ctx, a.rows, a.cols, FgPack<T>::E, sizeof(T) == 4 ? 4 : 2, straight ? 2 : 0);
     if (p.threads) {
         float* parts = nullptr;
         const uint32_t pitch = (a.cols + 127) / 128 * 128;
@@ -492,7 +523,8 @@ int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
         }
         int32_t s = FG_OK;
         if (p.packs == 1) s = choose_bwd_held<T, 1>(ctx, a, p, parts, pitch, straight);
-        else if constexpr (sizeof(T) == 4) s = choose_bwd_held<T, 2>(ctx, a, p, parts, pitch, straight);
+        else if (p.packs == 2) s = choose_bwd_held<T, 2>(ctx, a, p, parts, pitch, straight);
+        else if constexpr (sizeof(T) == 4) s = choose_bwd_held<T, 4>(ctx, a, p, parts, pitch, straight);
         if (s != FG_OK || !parts) return s;
         fg_launch(ctx, norm_parts_kernel<T>, pitch / 64, 1024, 0, a, (const float*)parts, (uint32_t)p.grid, pitch);
         FG_LAUNCHED(ctx);

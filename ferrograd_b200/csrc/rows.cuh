@@ -52,6 +52,25 @@ __device__ __forceinline__ float2 fg_block_sum2(float a, float b, float* red) {
     return make_float2(a, b);
 }
 
+// ---- two f32 operations in one instruction ----
+__device__ __forceinline__ uint64_t fg_bits2(float2 a) { return (uint64_t)__float_as_uint(a.y) << 32 | __float_as_uint(a.x); }
+__device__ __forceinline__ float2 fg_floats2(uint64_t a) { return make_float2(__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)(a >> 32))); }
+__device__ __forceinline__ float2 fg_add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(fg_bits2(a)), "l"(fg_bits2(b)));
+    return fg_floats2(r);
+}
+__device__ __forceinline__ float2 fg_mul2(float2 a, float2 b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(fg_bits2(a)), "l"(fg_bits2(b)));
+    return fg_floats2(r);
+}
+__device__ __forceinline__ float2 fg_fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(fg_bits2(a)), "l"(fg_bits2(b)), "l"(fg_bits2(c)));
+    return fg_floats2(r);
+}
+
 // ---- sixteen bytes of a row at a time ----
 // A row whose tensors start on 16-byte boundaries and whose length is a whole number of packs is moved as it lies (kShift = false).  Any
 // other row is moved in 16-byte words of memory too: a thread owns the same columns in every row and every tensor, and turns what it
@@ -76,6 +95,18 @@ struct FgPack {
                 }
             }
         }
+    }
+    static __device__ __forceinline__ void widen(const uint4& v, float2 (&x)[E / 2]) {
+        float y[E];
+        widen(v, y);
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) x[i] = make_float2(y[2 * i], y[2 * i + 1]);
+    }
+    static __device__ __forceinline__ uint4 narrow(const float2 (&x)[E / 2]) {
+        float y[E];
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) { y[2 * i] = x[i].x; y[2 * i + 1] = x[i].y; }
+        return narrow(y);
     }
     static __device__ __forceinline__ uint4 narrow(const float (&x)[E]) {
         uint32_t w[4];
