@@ -24,10 +24,11 @@ struct NormBwdArgs {
 };
 
 // ---- rows that a group of threads holds ----
-// A group of warps takes a row at a time, a thread the same columns of each: pack `thread`, `thread` + threads, ... of 16 bytes.  What comes
-// from memory is asked for two or three rows ahead: rows that lie straight by asynchronous copies into slots of shared memory that belong
-// to the thread alone, turned rows (kShift) as loads one row ahead.
-__host__ __device__ constexpr int stages_of(int packs) { return packs >= 8 ? 3 : 4; }      // by the packs of all tensors in a stage: 512 threads fit
+// A group of warps takes a row at a time, a thread the same columns of each.  What bounds these kernels beside the memory is instructions:
+// 400 to 600 per warp and row of 16 columns a thread in a first form, most of them addresses and zeros for columns that are not there,
+// so rows that fill their threads have code of their own (kFull), two f32 operations go in one instruction and the two sums of a
+// row share their shuffles.
+constexpr int kMaxGroups = 8, kMaxThreads = 512;
 struct Group {
     int index, threads, thread, warps, warp, lane;      // of the block's groups; a group's threads; within the group
     __device__ __forceinline__ explicit Group(int threads_) : threads(threads_) {
@@ -37,130 +38,221 @@ struct Group {
         warp = thread >> 5;
         lane = threadIdx.x & 31;
     }
-    // Two sums over the group, in all of its threads.  `red` is the group's [64] floats, another one from one call to the next.
+    // The sum of a in lanes 0 to 15, of b in 16 to 31.
+    __device__ __forceinline__ float halves(float a, float b) const {
+        const float mine = lane < 16 ? a : b, other = lane < 16 ? b : a;
+        float v = mine + __shfl_xor_sync(0xffffffffu, other, 16);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+    // Two sums over the group, in all of its threads.  `red` is the group's [32] floats, others from one call to the next; 16 warps at most.
     __device__ __forceinline__ float2 sum(float a, float b, float* red) const {
+        float v = halves(a, b);
+        if (warps > 1) {
+            if ((lane & 15) == 0) red[lane + warp] = v;
+            fg_group_barrier(index, threads);
+            v = (lane & 15) < warps ? red[lane] : 0.0f;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        }
+        return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
+    }
+    __device__ __forceinline__ float sum(float a, float* red) const {
         a = fg_warp_sum(a);
-        b = fg_warp_sum(b);
-        if (warps == 1) return make_float2(a, b);
-        if (lane == 0) { red[warp] = a; red[32 + warp] = b; }
+        if (warps == 1) return a;
+        if (lane == 0) red[warp] = a;
         fg_group_barrier(index, threads);
-        a = fg_warp_sum(lane < warps ? red[lane] : 0.0f);
-        b = fg_warp_sum(lane < warps ? red[32 + lane] : 0.0f);
-        return make_float2(a, b);
+        a = (lane & 15) < warps ? red[lane & 15] : 0.0f;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        return a;
     }
 };
-constexpr int kMaxGroups = 8;
 
-template <typename T, int kPacks, bool kShift>
-__global__ void __launch_bounds__(512) norm_held_kernel(const NormArgs a, int threads) {
-    constexpr int E = FgPack<T>::E, P = E / 2, kStages = stages_of(kPacks);
-    constexpr bool kHeldParams = kPacks <= 4;      // gamma and beta stay in registers
-    extern __shared__ uint4 slots[];      // [stage][pack][thread]
-    __shared__ float red[kMaxGroups][4][64];
-    fg_grid_enter();
-    const Group group(threads);
-    const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups, first = blockIdx.x * groups + group.index;
-    const float n = (float)a.cols, inv_n = 1.0f / n;
-    const T *const x = static_cast<const T*>(a.x), *const x_end = x + (uint64_t)a.rows * a.cols, *const gamma = static_cast<const T*>(a.gamma),
-            *const beta = static_cast<const T*>(a.beta);
-    uint32_t col[kPacks], left[kPacks];
-    uint4 gammas[kHeldParams ? kPacks : 1], betas[kHeldParams ? kPacks : 1];
-    auto load_params = [&](int k, uint4& g, uint4& b) {
-        g = b = make_uint4(0, 0, 0, 0);
-        if (gamma && left[k]) g = fg_load_pack<T, kShift>(gamma + col[k], left[k], gamma, gamma + a.cols);
-        if (beta && left[k]) b = fg_load_pack<T, kShift>(beta + col[k], left[k], beta, beta + a.cols);
-    };
-#pragma unroll
-    for (int k = 0; k < kPacks; ++k) {
-        col[k] = (group.thread + k * threads) * E;
-        left[k] = col[k] < a.cols ? min((uint32_t)E, a.cols - col[k]) : 0;
-        if constexpr (kHeldParams) load_params(k, gammas[k], betas[k]);
+// Rows that lie straight: a thread has packs `thread`, `thread` + threads, ... of 16 bytes, asked for two or three rows ahead by asynchronous
+// copies into slots of shared memory that are the thread's own.
+__host__ __device__ constexpr int stages_of(int packs) { return packs >= 4 ? 3 : 4; }      // by the packs of all tensors in a stage: 512 threads fit
+template <typename T_, int kPacks, bool kFull, int kTensors>
+struct Straight {
+    using T = T_;
+    static constexpr int E = FgPack<T>::E, P = E / 2, N = kPacks * E, kStages = stages_of(kTensors * kPacks);
+    static constexpr bool kAhead = true;
+    uint32_t slots, block, offset, pitch, have;      // shared address of the thread's first slot, bytes of a block's packs, of the thread, of a group's packs
+    uint32_t put = 0, take = 0;                      // stages
+    __device__ __forceinline__ Straight(const Group& g, uint32_t cols, const void* shared) {
+        slots = (uint32_t)__cvta_generic_to_shared(shared) + threadIdx.x * 16;
+        block = blockDim.x * 16;
+        offset = g.thread * 16;
+        pitch = g.threads * 16;
+        const uint32_t packs = cols / E;
+        have = (uint32_t)g.thread < packs ? min((uint32_t)kPacks, (packs - g.thread + g.threads - 1) / g.threads) : 0;
     }
-    uint4 ahead[kPacks];
-    auto ask = [&](uint64_t r, int stage) {
-        if (r < a.rows) {
-            const T* const row = x + r * a.cols;
+    __device__ __forceinline__ bool has(int k) const { return kFull || k < have; }
+    __device__ __forceinline__ uint32_t slot(uint32_t stage, int t, int k) const { return slots + ((stage * kTensors + t) * kPacks + k) * block; }
+    __device__ __forceinline__ void ask(int t, const T* row) {
+        const char* const p = reinterpret_cast<const char*>(row) + offset;
 #pragma unroll
-            for (int k = 0; k < kPacks; ++k)
-                if (left[k]) {
-                    if constexpr (kShift) ahead[k] = fg_load_pack<T, true>(row + col[k], left[k], x, x_end);
-                    else fg_copy_async(&slots[(stage * kPacks + k) * blockDim.x + threadIdx.x], row + col[k]);
-                }
-        }
-        if constexpr (!kShift) fg_copies_end();
-    };
-    if constexpr (kShift) ask(first, 0);
-    else
+        for (int k = 0; k < kPacks; ++k)
+            if (has(k)) fg_copy_async(slot(put, t, k), p + k * pitch);
+    }
+    __device__ __forceinline__ void asked() {
+        fg_copies_end();
+        put = put == kStages - 1 ? 0 : put + 1;
+    }
+    __device__ __forceinline__ void arrived() const { fg_copies_wait<kStages - 2>(); }
+    __device__ __forceinline__ void taken() { take = take == kStages - 1 ? 0 : take + 1; }
+    __device__ __forceinline__ void spread(int k, const uint4& w, float2* v) const {
+        float2 x[P];
+        FgPack<T>::widen(w, x);
 #pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) ask(first + (uint64_t)i * step, i);
-    int stage = 0, turn = 0;
-    for (uint64_t r = first; r < a.rows; r += step) {
-        float2 v[kPacks][P];
-        if constexpr (!kShift) fg_copies_wait<kStages - 2>();
-        float2 s = make_float2(0.0f, 0.0f);
+        for (int e = 0; e < P; ++e) v[k * P + e] = has(k) ? x[e] : make_float2(0.0f, 0.0f);
+    }
+    __device__ __forceinline__ void get(int t, const T*, float2 (&v)[N / 2]) const {
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) spread(k, fg_load_shared(slot(take, t, k)), v);
+    }
+    __device__ __forceinline__ void load(const T* row, float2 (&v)[N / 2]) const {
 #pragma unroll
         for (int k = 0; k < kPacks; ++k) {
             uint4 w = make_uint4(0, 0, 0, 0);
-            if (left[k]) {
-                if constexpr (kShift) w = ahead[k];
-                else w = slots[(stage * kPacks + k) * blockDim.x + threadIdx.x];
-            }
-            FgPack<T>::widen(w, v[k]);
-            if (kShift && left[k] < E)
-#pragma unroll
-                for (int e = 0; e < P; ++e) {
-                    if (2 * e >= left[k]) v[k][e].x = 0.0f;
-                    if (2 * e + 1 >= left[k]) v[k][e].y = 0.0f;
-                }
-#pragma unroll
-            for (int e = 0; e < P; ++e) s = fg_add2(s, v[k][e]);
+            if (has(k)) w = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(row) + offset + k * pitch);
+            spread(k, w, v);
         }
-        if constexpr (kShift) ask(r + step, 0);
-        else ask(r + (uint64_t)(kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
-        const float m = group.sum(s.x + s.y, 0.0f, red[group.index][turn]).x / n;
-        const float2 less = make_float2(-m, -m);
-        float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
+    }
+    __device__ __forceinline__ void mask(float2 (&v)[N / 2]) const {      // columns that are not there count for nothing
+        if (!kFull)
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i)
+                if (!has(i / P)) v[i] = make_float2(0.0f, 0.0f);
+    }
+    __device__ __forceinline__ void store(T* row, const float2 (&v)[N / 2]) const {
 #pragma unroll
         for (int k = 0; k < kPacks; ++k) {
+            float2 x[P];
 #pragma unroll
-            for (int e = 0; e < P; ++e) v[k][e] = fg_add2(v[k][e], less);
-            if (left[k] < E)      // columns behind the row's end count for nothing
+            for (int e = 0; e < P; ++e) x[e] = v[k * P + e];
+            if (has(k)) *reinterpret_cast<uint4*>(reinterpret_cast<char*>(row) + offset + k * pitch) = FgPack<T>::narrow(x);
+        }
+    }
+    __device__ __forceinline__ void store_sums(float* row, const float2 (&v)[N / 2]) const {
 #pragma unroll
-                for (int e = 0; e < P; ++e) {
-                    if (2 * e >= left[k]) v[k][e].x = 0.0f;
-                    if (2 * e + 1 >= left[k]) v[k][e].y = 0.0f;
-                }
+        for (int i = 0; i < N / 2; ++i)
+            if (has(i / P)) *reinterpret_cast<float2*>(row + (offset + (i / P) * pitch) / sizeof(T) + 2 * (i % P)) = v[i];
+    }
+};
+
+// Any other row: a thread has the elements `thread`, `thread` + threads, ... of it.  (Words turned by the row's distance from a 16-byte boundary
+// took three times the instructions.)
+template <typename T_, int kCount, int kTensors>
+struct Ragged {
+    using T = T_;
+    static constexpr int N = kCount, kStages = 1;
+    static constexpr bool kAhead = false;
+    uint32_t thread, threads, cols;
+    __device__ __forceinline__ Ragged(const Group& g, uint32_t cols_, const void*) : thread(g.thread), threads(g.threads), cols(cols_) {}
+    __device__ __forceinline__ void ask(int, const T*) {}
+    __device__ __forceinline__ void asked() {}
+    __device__ __forceinline__ void arrived() const {}
+    __device__ __forceinline__ void taken() {}
+    __device__ __forceinline__ void get(int, const T* row, float2 (&v)[N / 2]) const { load(row, v); }
+    __device__ __forceinline__ void load(const T* row, float2 (&v)[N / 2]) const {
+        T w[N];
 #pragma unroll
-            for (int e = 0; e < P; ++e) {
-                s1 = fg_add2(s1, v[k][e]);
-                s2 = fg_fma2(v[k][e], v[k][e], s2);
-            }
+        for (int i = 0; i < N; ++i) {
+            const uint32_t c = thread + i * threads;
+            w[i] = c < cols ? row[c] : fg_narrow<T>(0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fg_widen(w[2 * i]), fg_widen(w[2 * i + 1]));
+    }
+    __device__ __forceinline__ void mask(float2 (&v)[N / 2]) const {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            if (thread + 2 * i * threads >= cols) v[i].x = 0.0f;
+            if (thread + (2 * i + 1) * threads >= cols) v[i].y = 0.0f;
+        }
+    }
+    template <typename U>
+    __device__ __forceinline__ void put(U* row, const float2 (&v)[N / 2]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t c = thread + i * threads;
+            if (c < cols) row[c] = fg_narrow<U>(i & 1 ? v[i / 2].y : v[i / 2].x);
+        }
+    }
+    __device__ __forceinline__ void store(T* row, const float2 (&v)[N / 2]) const { put(row, v); }
+    __device__ __forceinline__ void store_sums(float* row, const float2 (&v)[N / 2]) const { put(row, v); }
+};
+
+template <typename C>
+__global__ void __launch_bounds__(kMaxThreads, C::N <= 16 ? 2 : 1) norm_held_kernel(const NormArgs a, int threads) {
+    using T = typename C::T;
+    constexpr int H = C::N / 2;
+    extern __shared__ uint4 shared[];
+    __shared__ float red[kMaxGroups][4][32];
+    fg_grid_enter();
+    const Group group(threads);
+    C columns(group, a.cols, shared);
+    const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups, first = blockIdx.x * groups + group.index;
+    const float n = (float)a.cols, inv_n = 1.0f / n;
+    const T *const gamma = static_cast<const T*>(a.gamma), *const beta = static_cast<const T*>(a.beta);
+    const uint64_t stride = (uint64_t)step * a.cols;
+    const T *x = static_cast<const T*>(a.x) + (uint64_t)first * a.cols, *ahead = x;
+    T* y = static_cast<T*>(a.y) + (uint64_t)first * a.cols;
+    uint64_t next = first;      // the next row to ask for
+    auto ask = [&] {
+        if (next < a.rows) columns.ask(0, ahead);
+        columns.asked();
+        next += step;
+        ahead += stride;
+    };
+    if (C::kAhead)
+#pragma unroll
+        for (int i = 0; i < C::kStages - 1; ++i) ask();
+    int turn = 0;
+    for (uint64_t r = first; r < a.rows; r += step, x += stride, y += stride) {
+        float2 v[H];
+        columns.arrived();
+        columns.get(0, x, v);
+        columns.taken();
+        if (C::kAhead) ask();
+        float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < H; ++i) s = fg_add2(s, v[i]);
+        const float m = group.sum(s.x + s.y, red[group.index][turn]) / n;
+        const float2 less = make_float2(-m, -m);
+#pragma unroll
+        for (int i = 0; i < H; ++i) v[i] = fg_add2(v[i], less);
+        columns.mask(v);
+        float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            s1 = fg_add2(s1, v[i]);
+            s2 = fg_fma2(v[i], v[i], s2);
         }
         const float2 t = group.sum(s1.x + s1.y, s2.x + s2.y, red[group.index][turn + 1]);
         const float rest = t.x * inv_n, rstd = 1.0f / sqrtf(fmaxf(__fmaf_rn(-rest, rest, t.y * inv_n), 0.0f) + a.eps);
-        T* const out = static_cast<T*>(a.y) + r * a.cols;
         const float2 less_rest = make_float2(-rest, -rest), by = make_float2(rstd, rstd);
 #pragma unroll
-        for (int k = 0; k < kPacks; ++k) {
-            if (!kShift && !left[k]) continue;      // (turned rows are stored by whole warps)
-            uint4 gw, bw;
-            if constexpr (kHeldParams) { gw = gammas[k]; bw = betas[k]; }
-            else load_params(k, gw, bw);
-            float2 g[P], b[P];
-            FgPack<T>::widen(gw, g);
-            FgPack<T>::widen(bw, b);
+        for (int i = 0; i < H; ++i) v[i] = fg_mul2(fg_add2(v[i], less_rest), by);
+        if (gamma) {
+            float2 g[H];
+            columns.load(gamma, g);
 #pragma unroll
-            for (int e = 0; e < P; ++e) {
-                const float2 h = fg_mul2(fg_add2(v[k][e], less_rest), by);
-                g[e] = gamma ? fg_fma2(h, g[e], b[e]) : fg_add2(h, b[e]);
-            }
-            fg_store_pack<T, kShift>(out + col[k], FgPack<T>::narrow(g), left[k]);
+            for (int i = 0; i < H; ++i) v[i] = fg_mul2(v[i], g[i]);
         }
+        if (beta) {
+            float2 b[H];
+            columns.load(beta, b);
+#pragma unroll
+            for (int i = 0; i < H; ++i) v[i] = fg_add2(v[i], b[i]);
+        }
+        columns.store(y, v);
         if (group.thread == 0) {
             if (a.mean) a.mean[r] = m + rest;
             if (a.rstd) a.rstd[r] = rstd;
         }
-        stage = stage == kStages - 1 ? 0 : stage + 1;
         turn ^= 2;
     }
 }
@@ -168,153 +260,110 @@ __global__ void __launch_bounds__(512) norm_held_kernel(const NormArgs a, int th
 // The backward pass the same way, 16 columns at most per thread.  With the gradients of the parameters (kParams) a thread sums its columns
 // over the rows of its group, a block adds its groups and leaves one row of parts: [block][2][pitch].
 // With c = x - mean, dx = rstd * g + (-rstd * m1) + c * (-rstd^2 * m2), where m1 and m2 are the means of g and of g * h.
-template <typename T, int kPacks, bool kShift, bool kParams>
-__global__ void __launch_bounds__(512) norm_bwd_held_kernel(const NormBwdArgs a, int threads, float* parts, uint32_t pitch) {
-    constexpr int E = FgPack<T>::E, P = E / 2, kStages = stages_of(2 * kPacks);
-    extern __shared__ uint4 slots[];      // [stage][x, dy][pack][thread]; at the end the groups' sums
-    __shared__ float red[kMaxGroups][2][64];
+template <typename C, bool kParams>
+__global__ void __launch_bounds__(kMaxThreads, C::N <= 8 ? 2 : 1) norm_bwd_held_kernel(const NormBwdArgs a, int threads, float* parts, uint32_t pitch) {
+    using T = typename C::T;
+    constexpr int H = C::N / 2;
+    extern __shared__ uint4 shared[];      // the slots; at the end the groups' sums
+    __shared__ float red[kMaxGroups][2][32];
     fg_grid_enter();
     const Group group(threads);
+    C columns(group, a.cols, shared);
     const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups, first = blockIdx.x * groups + group.index;
     const float inv_n = 1.0f / (float)a.cols;
-    const uint64_t size = (uint64_t)a.rows * a.cols;
-    const T *const x = static_cast<const T*>(a.x), *const dy = static_cast<const T*>(a.dy), *const gamma = static_cast<const T*>(a.gamma);
-    T* const dx = static_cast<T*>(a.dx);
-    uint32_t col[kPacks], left[kPacks];
-    uint4 gammas[kPacks];
-#pragma unroll
-    for (int k = 0; k < kPacks; ++k) {
-        col[k] = (group.thread + k * threads) * E;
-        left[k] = col[k] < a.cols ? min((uint32_t)E, a.cols - col[k]) : 0;
-        gammas[k] = make_uint4(0, 0, 0, 0);
-        if (gamma && left[k]) gammas[k] = fg_load_pack<T, kShift>(gamma + col[k], left[k], gamma, gamma + a.cols);
-    }
-    uint4 ahead[2][kPacks];
-    float mean = 0.0f, rstd = 0.0f;
-    auto ask = [&](uint64_t r, int stage) {
-        if (r < a.rows) {
-            const T *const x_row = x + r * a.cols, *const dy_row = dy + r * a.cols;
-#pragma unroll
-            for (int k = 0; k < kPacks; ++k)
-                if (left[k]) {
-                    if constexpr (kShift) {
-                        ahead[0][k] = fg_load_pack<T, true>(x_row + col[k], left[k], x, x + size);
-                        ahead[1][k] = fg_load_pack<T, true>(dy_row + col[k], left[k], dy, dy + size);
-                    } else {
-                        fg_copy_async(&slots[(stage * 2 * kPacks + k) * blockDim.x + threadIdx.x], x_row + col[k]);
-                        fg_copy_async(&slots[((stage * 2 + 1) * kPacks + k) * blockDim.x + threadIdx.x], dy_row + col[k]);
-                    }
-                }
-        }
-        if constexpr (!kShift) fg_copies_end();
-    };
-    auto ask_row = [&](uint64_t r) {
-        if (r < a.rows) { mean = a.mean[r]; rstd = a.rstd[r]; }
-    };
-    if constexpr (kShift) ask(first, 0);
+    const T* const gamma = static_cast<const T*>(a.gamma);
+    float2 gm[H];
+    if (gamma) columns.load(gamma, gm);
     else
 #pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) ask(first + (uint64_t)i * step, i);
-    ask_row(first);
-    float2 dg[kPacks][P], db[kPacks][P];
+        for (int i = 0; i < H; ++i) gm[i] = make_float2(1.0f, 1.0f);
+    const uint64_t stride = (uint64_t)step * a.cols, at = (uint64_t)first * a.cols;
+    const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at, *x_ahead = x, *dy_ahead = dy;
+    T* dx = a.dx ? static_cast<T*>(a.dx) + at : nullptr;
+    uint64_t next = first;
+    auto ask = [&] {
+        if (next < a.rows) {
+            columns.ask(0, x_ahead);
+            columns.ask(1, dy_ahead);
+        }
+        columns.asked();
+        next += step;
+        x_ahead += stride;
+        dy_ahead += stride;
+    };
+    if (C::kAhead)
 #pragma unroll
-    for (int k = 0; k < kPacks; ++k)
+        for (int i = 0; i < C::kStages - 1; ++i) ask();
+    float mean = 0.0f, rstd = 0.0f;
+    if (first < a.rows) { mean = a.mean[first]; rstd = a.rstd[first]; }
+    float2 dg[H], db[H];
 #pragma unroll
-        for (int e = 0; e < P; ++e) dg[k][e] = db[k][e] = make_float2(0.0f, 0.0f);
-    int stage = 0, turn = 0;
-    for (uint64_t r = first; r < a.rows; r += step) {
-        float2 c[kPacks][P], g[kPacks][P];
-        const float m = mean, sd = rstd;
-        const float2 less = make_float2(-m, -m), by = make_float2(sd, sd);
-        ask_row(r + step);
-        if constexpr (!kShift) fg_copies_wait<kStages - 2>();
+    for (int i = 0; i < H; ++i) dg[i] = db[i] = make_float2(0.0f, 0.0f);
+    int turn = 0;
+    for (uint64_t r = first; r < a.rows; r += step, x += stride, dy += stride) {
+        float2 c[H], g[H];
+        const float sd = rstd;
+        const float2 less = make_float2(-mean, -mean), by = make_float2(sd, sd);
+        columns.arrived();
+        columns.get(0, x, c);
+        columns.get(1, dy, g);
+        columns.taken();
+        if (r + step < a.rows) { mean = a.mean[r + step]; rstd = a.rstd[r + step]; }
+        if (C::kAhead) ask();
+#pragma unroll
+        for (int i = 0; i < H; ++i) c[i] = fg_add2(c[i], less);
+        columns.mask(c);      // (dy is zero there)
         float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
 #pragma unroll
-        for (int k = 0; k < kPacks; ++k) {
-            uint4 v = make_uint4(0, 0, 0, 0), w = v;
-            if (left[k]) {
-                if constexpr (kShift) { v = ahead[0][k]; w = ahead[1][k]; }
-                else {
-                    v = slots[(stage * 2 * kPacks + k) * blockDim.x + threadIdx.x];
-                    w = slots[((stage * 2 + 1) * kPacks + k) * blockDim.x + threadIdx.x];
-                }
+        for (int i = 0; i < H; ++i) {
+            if (kParams) {
+                dg[i] = fg_fma2(g[i], fg_mul2(c[i], by), dg[i]);
+                db[i] = fg_add2(db[i], g[i]);
             }
-            FgPack<T>::widen(v, c[k]);
-            FgPack<T>::widen(w, g[k]);
-            float2 gm[P];
-            FgPack<T>::widen(gammas[k], gm);
-#pragma unroll
-            for (int e = 0; e < P; ++e) c[k][e] = fg_add2(c[k][e], less);
-            if (left[k] < E)      // columns behind the row's end count for nothing
-#pragma unroll
-                for (int e = 0; e < P; ++e) {
-                    if (2 * e >= left[k]) c[k][e].x = g[k][e].x = 0.0f;
-                    if (2 * e + 1 >= left[k]) c[k][e].y = g[k][e].y = 0.0f;
-                }
-#pragma unroll
-            for (int e = 0; e < P; ++e) {
-                if (kParams) {
-                    dg[k][e] = fg_fma2(g[k][e], fg_mul2(c[k][e], by), dg[k][e]);
-                    db[k][e] = fg_add2(db[k][e], g[k][e]);
-                }
-                if (gamma) g[k][e] = fg_mul2(g[k][e], gm[e]);
-                s1 = fg_add2(s1, g[k][e]);
-                s2 = fg_fma2(g[k][e], c[k][e], s2);
-            }
+            g[i] = fg_mul2(g[i], gm[i]);
+            s1 = fg_add2(s1, g[i]);
+            s2 = fg_fma2(g[i], c[i], s2);
         }
-        if constexpr (kShift) ask(r + step, 0);
-        else ask(r + (uint64_t)(kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
         if (dx) {
             const float2 t = group.sum(s1.x + s1.y, s2.x + s2.y, red[group.index][turn]);
             const float u1 = -sd * (t.x * inv_n), u2 = -sd * sd * (sd * (t.y * inv_n));
             const float2 add = make_float2(u1, u1), slope = make_float2(u2, u2);
-            T* const row = dx + r * a.cols;
 #pragma unroll
-            for (int k = 0; k < kPacks; ++k) {
-                if (!kShift && !left[k]) continue;
+            for (int i = 0; i < H; ++i) g[i] = fg_fma2(g[i], by, fg_fma2(c[i], slope, add));
+            if (a.accumulate_dx) {
+                columns.load(dx, c);
 #pragma unroll
-                for (int e = 0; e < P; ++e) g[k][e] = fg_fma2(g[k][e], by, fg_fma2(c[k][e], slope, add));
-                if (a.accumulate_dx) {
-                    float2 old[P];
-                    FgPack<T>::widen(left[k] ? fg_load_pack<T, kShift>(row + col[k], left[k], dx, dx + size) : make_uint4(0, 0, 0, 0), old);
-                    if (kShift) __syncwarp();      // a lane writes words that others have read
-#pragma unroll
-                    for (int e = 0; e < P; ++e) g[k][e] = fg_add2(g[k][e], old[e]);
-                }
-                fg_store_pack<T, kShift>(row + col[k], FgPack<T>::narrow(g[k]), left[k]);
+                for (int i = 0; i < H; ++i) g[i] = fg_add2(g[i], c[i]);
             }
+            columns.store(dx, g);
+            dx += stride;
         }
-        stage = stage == kStages - 1 ? 0 : stage + 1;
         turn ^= 1;
     }
     if constexpr (kParams) {
-        // the groups one after the other, in shared memory: [2][pack][pair][thread]
-        float2* const sums = reinterpret_cast<float2*>(slots);
-        if constexpr (!kShift) fg_copies_wait<0>();
+        float2* const sums = reinterpret_cast<float2*>(shared);      // the groups one after the other: [2][pair][thread]
+        if (C::kAhead) fg_copies_wait<0>();
         for (uint32_t i = 0; i + 1 < groups; ++i) {
             __syncthreads();
             if (group.index == (int)i)
 #pragma unroll
-                for (int k = 0; k < kPacks; ++k)
-#pragma unroll
-                    for (int e = 0; e < P; ++e) {
-                        float2 *const p = sums + (k * P + e) * threads + group.thread, *const q = p + kPacks * P * threads;
-                        *p = i ? fg_add2(*p, dg[k][e]) : dg[k][e];
-                        *q = i ? fg_add2(*q, db[k][e]) : db[k][e];
-                    }
+                for (int e = 0; e < H; ++e) {
+                    float2 *const p = sums + e * threads + group.thread, *const q = p + H * threads;
+                    *p = i ? fg_add2(*p, dg[e]) : dg[e];
+                    *q = i ? fg_add2(*q, db[e]) : db[e];
+                }
         }
         __syncthreads();
         if (group.index + 1 == (int)groups) {
+            if (groups > 1)
+#pragma unroll
+                for (int e = 0; e < H; ++e) {
+                    dg[e] = fg_add2(sums[e * threads + group.thread], dg[e]);
+                    db[e] = fg_add2(sums[(H + e) * threads + group.thread], db[e]);
+                }
             float* const mine = parts + (uint64_t)blockIdx.x * 2 * pitch;
-#pragma unroll
-            for (int k = 0; k < kPacks; ++k)
-                if (left[k])
-#pragma unroll
-                    for (int e = 0; e < P; ++e) {
-                        const float2 *const p = sums + (k * P + e) * threads + group.thread, *const q = p + kPacks * P * threads;
-                        *reinterpret_cast<float2*>(mine + col[k] + 2 * e) = groups > 1 ? fg_add2(*p, dg[k][e]) : dg[k][e];
-                        *reinterpret_cast<float2*>(mine + pitch + col[k] + 2 * e) = groups > 1 ? fg_add2(*q, db[k][e]) : db[k][e];
-                    }
+            columns.store_sums(mine, dg);
+            columns.store_sums(mine + pitch, db);
         }
     }
 }
@@ -445,20 +494,23 @@ __global__ void __launch_bounds__(256) norm_fold_kernel(const NormBwdArgs a, con
 
 int rows_grid(const fg_ctx* ctx, uint32_t rows) { return (int)(rows < 8u * ctx->sm_count ? rows : 8u * ctx->sm_count); }
 
-// How a kernel that holds rows is launched: packs per thread, the threads of a group, the groups of a block, its shared memory, the blocks.
-struct HeldPlan { int packs, threads, groups; size_t bytes; int grid; };
-// A block has 256 threads or, for a longer row, up to 512.  Threads hold up to `most` packs; of few rows, and where a warp is enough, one.
-HeldPlan held_plan(const fg_ctx* ctx, uint32_t rows, uint32_t cols, uint32_t elements, int most, int slots) {
-    const uint64_t packs = ((uint64_t)cols + elements - 1) / elements;
-    HeldPlan p{1, 0, 1, 0, 0};
-    while (p.packs < most && (packs > 512ull * p.packs || (p.packs < 4 && rows > 2u * ctx->sm_count && packs > 32ull * p.packs))) p.packs *= 2;
-    if (packs > 512ull * p.packs) return p;      // threads = 0: no
-    p.threads = (int)((packs + 32 * p.packs - 1) / (32 * p.packs) * 32);
+// How a kernel that holds rows is launched: a thread's packs (or elements, of ragged rows), the threads of a group, the groups of a block, the
+// bytes of its slots, the blocks; threads = 0: not at all.
+struct HeldPlan { int units, threads, groups; bool full; size_t bytes; int grid; };
+// A block has 256 threads or, for a longer row, up to 512.  Threads hold `usual` units, or up to `most` where the row asks for it; of few rows,
+// and where a warp is enough, `least`.  `resident`: threads that an SM has registers for, at the usual units.
+HeldPlan held_plan(const fg_ctx* ctx, uint32_t rows, uint64_t units, int least, int usual, int most, int tensors, int resident) {
+    HeldPlan p{least, 0, 1, false, 0, 0};
+    while (p.units < most && (units > (uint64_t)kMaxThreads * p.units || (p.units < usual && rows > 2u * ctx->sm_count && units > 32ull * p.units))) p.units *= 2;
+    if (units > (uint64_t)kMaxThreads * p.units) return p;
+    p.threads = (int)((units + 32 * p.units - 1) / (32 * p.units) * 32);
+    p.full = units == (uint64_t)p.threads * p.units;
     p.groups = 256 / p.threads < 1 ? 1 : 256 / p.threads;
     while (p.groups > 1 && (uint64_t)rows * 2 <= (uint64_t)p.groups * ctx->sm_count) p.groups /= 2;      // few rows: over the SMs first
-    p.bytes = sizeof(uint4) * stages_of(slots * p.packs) * slots * p.packs * p.threads * p.groups;
-    // What the SMs hold at once: 512 threads of 128 registers, 220 KB with the static part.
-    const uint64_t by_threads = 512 / (p.threads * p.groups), by_memory = 220 * 1024 / (p.bytes + 9 * 1024), per_sm = by_threads < by_memory ? by_threads : by_memory;
+    p.bytes = sizeof(uint4) * stages_of(tensors * p.units) * tensors * p.units * p.threads * p.groups;
+    // What the SMs hold at once: threads by their registers, 220 KB with the static part.
+    const uint64_t by_threads = (p.units <= usual ? resident : kMaxThreads) / (p.threads * p.groups), by_memory = 220 * 1024 / (p.bytes + 5 * 1024),
+                   per_sm = by_threads < by_memory ? by_threads : by_memory;
     const uint64_t need = ((uint64_t)rows + p.groups - 1) / p.groups, cap = (uint64_t)ctx->sm_count * (per_sm ? per_sm : 1);
     p.grid = (int)(need < cap ? need : cap);
     return p;
@@ -469,49 +521,57 @@ int32_t allow_shared(fg_ctx* ctx, K kernel, size_t bytes) {
     return FG_OK;
 }
 
-template <typename T, int kPacks, bool kShift>
+template <typename C>
 int32_t launch_held(fg_ctx* ctx, const NormArgs& a, HeldPlan p) {
-    const size_t bytes = p.bytes;
-    const int32_t s = allow_shared(ctx, norm_held_kernel<T, kPacks, kShift>, bytes);
+    const int32_t s = allow_shared(ctx, norm_held_kernel<C>, p.bytes);
     if (s != FG_OK) return s;
-    fg_launch(ctx, norm_held_kernel<T, kPacks, kShift>, p.grid, p.threads * p.groups, bytes, a, p.threads);
+    fg_launch(ctx, norm_held_kernel<C>, p.grid, p.threads * p.groups, p.bytes, a, p.threads);
     FG_LAUNCHED(ctx);
     return FG_OK;
 }
-template <typename T, bool kShift>
-int32_t choose_held(fg_ctx* ctx, const NormArgs& a, HeldPlan p) {
-    return p.packs == 1 ? launch_held<T, 1, kShift>(ctx, a, p) : p.packs == 2 ? launch_held<T, 2, kShift>(ctx, a, p)
-           : p.packs == 4 ? launch_held<T, 4, kShift>(ctx, a, p) : launch_held<T, 8, kShift>(ctx, a, p);
+template <typename T, int kPacks>
+int32_t launch_straight(fg_ctx* ctx, const NormArgs& a, HeldPlan p) {
+    return p.full ? launch_held<Straight<T, kPacks, true, 1>>(ctx, a, p) : launch_held<Straight<T, kPacks, false, 1>>(ctx, a, p);
 }
 template <typename T>
 int32_t norm_fwd(fg_ctx* ctx, const NormArgs& a) {
-    const bool straight = fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.y, a.gamma, a.beta);
-    const HeldPlan p = held_plan(ctx, a.rows, a.cols, FgPack<T>::E, 8, straight ? 1 : 0);
-    if (p.threads) return straight ? choose_held<T, false>(ctx, a, p) : choose_held<T, true>(ctx, a, p);
+    constexpr int usual = 16 / FgPack<T>::E;      // 16 columns a thread
+    if (fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.y, a.gamma, a.beta)) {
+        const HeldPlan p = held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 1, usual, 8, 1, 1024);
+        if (p.threads)
+            return p.units == 1 ? launch_straight<T, 1>(ctx, a, p) : p.units == 2 ? launch_straight<T, 2>(ctx, a, p)
+                   : p.units == 4 ? launch_straight<T, 4>(ctx, a, p) : launch_straight<T, 8>(ctx, a, p);
+    } else {
+        HeldPlan p = held_plan(ctx, a.rows, a.cols, 4, 16, 32, 0, 1024);
+        if (p.threads)
+            return p.units == 4 ? launch_held<Ragged<T, 4, 1>>(ctx, a, p) : p.units == 8 ? launch_held<Ragged<T, 8, 1>>(ctx, a, p)
+                   : p.units == 16 ? launch_held<Ragged<T, 16, 1>>(ctx, a, p) : launch_held<Ragged<T, 32, 1>>(ctx, a, p);
+    }
     fg_launch(ctx, norm_stream_kernel<T>, rows_grid(ctx, a.rows), 256, 0, a);
     FG_LAUNCHED(ctx);
     return FG_OK;
 }
 
-template <typename T, int kPacks, bool kShift, bool kParams>
+template <typename C>
 int32_t launch_bwd_held(fg_ctx* ctx, const NormBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch) {
-    const size_t sums = kParams && p.groups > 1 ? 8ull * FgPack<T>::E * kPacks * p.threads : 0, bytes = p.bytes < sums ? sums : p.bytes;
-    const int32_t s = allow_shared(ctx, norm_bwd_held_kernel<T, kPacks, kShift, kParams>, bytes);
+    const size_t sums = parts && p.groups > 1 ? 8ull * C::N * p.threads : 0, bytes = p.bytes < sums ? sums : p.bytes;
+    const auto kernel = parts ? norm_bwd_held_kernel<C, true> : norm_bwd_held_kernel<C, false>;
+    const int32_t s = allow_shared(ctx, kernel, bytes);
     if (s != FG_OK) return s;
-    fg_launch(ctx, norm_bwd_held_kernel<T, kPacks, kShift, kParams>, p.grid, p.threads * p.groups, bytes, a, p.threads, parts, pitch);
+    fg_launch(ctx, kernel, p.grid, p.threads * p.groups, bytes, a, p.threads, parts, pitch);
     FG_LAUNCHED(ctx);
     return FG_OK;
 }
 template <typename T, int kPacks>
-int32_t choose_bwd_held(fg_ctx* ctx, const NormBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch, bool straight) {
-    if (parts) return straight ? launch_bwd_held<T, kPacks, false, true>(ctx, a, p, parts, pitch) : launch_bwd_held<T, kPacks, true, true>(ctx, a, p, parts, pitch);
-    return straight ? launch_bwd_held<T, kPacks, false, false>(ctx, a, p, parts, pitch) : launch_bwd_held<T, kPacks, true, false>(ctx, a, p, parts, pitch);
+int32_t launch_bwd_straight(fg_ctx* ctx, const NormBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch) {
+    return p.full ? launch_bwd_held<Straight<T, kPacks, true, 2>>(ctx, a, p, parts, pitch) : launch_bwd_held<Straight<T, kPacks, false, 2>>(ctx, a, p, parts, pitch);
 }
 
 template <typename T>
 int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
+    constexpr int usual = 16 / FgPack<T>::E;
     const bool straight = fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.dy, a.gamma, a.dx);
-    const HeldPlan p = held_plan(ctx, a.rows, a.cols, FgPack<T>::E, sizeof(T) == 4 ? 4 : 2, straight ? 2 : 0);
+    const HeldPlan p = straight ? held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 1, usual, usual, 2, 512) : held_plan(ctx, a.rows, a.cols, 4, 8, 16, 0, 1024);
     if (p.threads) {
         float* parts = nullptr;
         const uint32_t pitch = (a.cols + 127) / 128 * 128;
@@ -521,10 +581,14 @@ int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
             if (s != FG_OK) return s;
             parts = (float*)w;
         }
-        int32_t s = FG_OK;
-        if (p.packs == 1) s = choose_bwd_held<T, 1>(ctx, a, p, parts, pitch, straight);
-        else if (p.packs == 2) s = choose_bwd_held<T, 2>(ctx, a, p, parts, pitch, straight);
-        else if constexpr (sizeof(T) == 4) s = choose_bwd_held<T, 4>(ctx, a, p, parts, pitch, straight);
+        int32_t s;
+        if (straight) {
+            if (p.units == 1) s = launch_bwd_straight<T, 1>(ctx, a, p, parts, pitch);
+            else if (p.units == 2) s = launch_bwd_straight<T, 2>(ctx, a, p, parts, pitch);
+            else s = launch_bwd_straight<T, usual>(ctx, a, p, parts, pitch);
+        } else if (p.units == 4) s = launch_bwd_held<Ragged<T, 4, 2>>(ctx, a, p, parts, pitch);
+        else if (p.units == 8) s = launch_bwd_held<Ragged<T, 8, 2>>(ctx, a, p, parts, pitch);
+        else s = launch_bwd_held<Ragged<T, 16, 2>>(ctx, a, p, parts, pitch);
         if (s != FG_OK || !parts) return s;
         fg_launch(ctx, norm_parts_kernel<T>, pitch / 64, 1024, 0, a, (const float*)parts, (uint32_t)p.grid, pitch);
         FG_LAUNCHED(ctx);

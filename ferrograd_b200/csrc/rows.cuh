@@ -32,8 +32,13 @@ __device__ __forceinline__ float fg_warp_sum(float v) {
 // A barrier over one of a block's groups of warps (0 to 14).
 __device__ __forceinline__ void fg_group_barrier(int group, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory"); }
 // Sixteen bytes on their way from memory to shared memory, past the L1; a thread waits for its own.
-__device__ __forceinline__ void fg_copy_async(void* to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+__device__ __forceinline__ void fg_copy_async(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ uint4 fg_load_shared(uint32_t from) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+    return v;
 }
 __device__ __forceinline__ void fg_copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft>      // all but the last kLeft groups have arrived
