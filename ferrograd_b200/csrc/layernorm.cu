@@ -72,7 +72,7 @@ struct Group {
 
 // Rows that lie straight: a thread has packs `thread`, `thread` + threads, ... of 16 bytes, asked for two or three rows ahead by asynchronous
 // copies into slots of shared memory that are the thread's own.
-__host__ __device__ constexpr int stages_of(int packs) { return packs >= 4 ? 3 : 4; }      // by the packs of all tensors in a stage: 512 threads fit
+__host__ __device__ constexpr int stages_of(int packs) { return packs > 4 ? 3 : 4; }      // by the packs of all tensors in a stage: 512 threads fit
 template <typename T_, int kPacks, bool kFull, int kTensors>
 struct Straight {
     using T = T_;
@@ -120,6 +120,24 @@ struct Straight {
             spread(k, w, v);
         }
     }
+    // A parameter's columns, kept for all rows (of up to 4 packs: read from the L1 and, where slots leave it little room, from the L2 for every
+    // row, they cost a fifth of the time).
+    static constexpr bool kKeep = kPacks <= 4;
+    struct Kept { uint4 w[kKeep ? kPacks : 1]; };
+    __device__ __forceinline__ void keep(const T* p, Kept& kept) const {
+        if (!kKeep) return;
+#pragma unroll
+        for (int k = 0; k < (kKeep ? kPacks : 0); ++k) {
+            kept.w[k] = make_uint4(0, 0, 0, 0);
+            if (has(k)) kept.w[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + offset + k * pitch);
+        }
+    }
+    __device__ __forceinline__ void kept(const Kept& kept, const T* p, float2 (&v)[N / 2]) const {
+        if constexpr (kKeep) {
+#pragma unroll
+            for (int k = 0; k < kPacks; ++k) spread(k, kept.w[k], v);
+        } else load(p, v);
+    }
     __device__ __forceinline__ void mask(float2 (&v)[N / 2]) const {      // columns that are not there count for nothing
         if (!kFull)
 #pragma unroll
@@ -166,6 +184,9 @@ struct Ragged {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fg_widen(w[2 * i]), fg_widen(w[2 * i + 1]));
     }
+    struct Kept {};      // (read again for every row)
+    __device__ __forceinline__ void keep(const T*, Kept&) const {}
+    __device__ __forceinline__ void kept(const Kept&, const T* p, float2 (&v)[N / 2]) const { load(p, v); }
     __device__ __forceinline__ void mask(float2 (&v)[N / 2]) const {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
@@ -186,7 +207,7 @@ struct Ragged {
 };
 
 template <typename C>
-__global__ void __launch_bounds__(kMaxThreads, C::N <= 16 ? 2 : 1) norm_held_kernel(const NormArgs a, int threads) {
+__global__ void __launch_bounds__(kMaxThreads, !C::kAhead && C::N <= 16 ? 2 : 1) norm_held_kernel(const NormArgs a, int threads) {
     using T = typename C::T;
     constexpr int H = C::N / 2;
     extern __shared__ uint4 shared[];
@@ -197,6 +218,9 @@ __global__ void __launch_bounds__(kMaxThreads, C::N <= 16 ? 2 : 1) norm_held_ker
     const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups, first = blockIdx.x * groups + group.index;
     const float n = (float)a.cols, inv_n = 1.0f / n;
     const T *const gamma = static_cast<const T*>(a.gamma), *const beta = static_cast<const T*>(a.beta);
+    typename C::Kept gammas, betas;
+    if (gamma) columns.keep(gamma, gammas);
+    if (beta) columns.keep(beta, betas);
     const uint64_t stride = (uint64_t)step * a.cols;
     const T *x = static_cast<const T*>(a.x) + (uint64_t)first * a.cols, *ahead = x;
     T* y = static_cast<T*>(a.y) + (uint64_t)first * a.cols;
@@ -238,13 +262,13 @@ __global__ void __launch_bounds__(kMaxThreads, C::N <= 16 ? 2 : 1) norm_held_ker
         for (int i = 0; i < H; ++i) v[i] = fg_mul2(fg_add2(v[i], less_rest), by);
         if (gamma) {
             float2 g[H];
-            columns.load(gamma, g);
+            columns.kept(gammas, gamma, g);
 #pragma unroll
             for (int i = 0; i < H; ++i) v[i] = fg_mul2(v[i], g[i]);
         }
         if (beta) {
             float2 b[H];
-            columns.load(beta, b);
+            columns.kept(betas, beta, b);
 #pragma unroll
             for (int i = 0; i < H; ++i) v[i] = fg_add2(v[i], b[i]);
         }
@@ -261,7 +285,7 @@ __global__ void __launch_bounds__(kMaxThreads, C::N <= 16 ? 2 : 1) norm_held_ker
 // over the rows of its group, a block adds its groups and leaves one row of parts: [block][2][pitch].
 // With c = x - mean, dx = rstd * g + (-rstd * m1) + c * (-rstd^2 * m2), where m1 and m2 are the means of g and of g * h.
 template <typename C, bool kParams>
-__global__ void __launch_bounds__(kMaxThreads, C::N <= 8 ? 2 : 1) norm_bwd_held_kernel(const NormBwdArgs a, int threads, float* parts, uint32_t pitch) {
+__global__ void __launch_bounds__(kMaxThreads, !C::kAhead && C::N <= 4 ? 2 : 1) norm_bwd_held_kernel(const NormBwdArgs a, int threads, float* parts, uint32_t pitch) {
     using T = typename C::T;
     constexpr int H = C::N / 2;
     extern __shared__ uint4 shared[];      // the slots; at the end the groups' sums
@@ -537,7 +561,7 @@ template <typename T>
 int32_t norm_fwd(fg_ctx* ctx, const NormArgs& a) {
     constexpr int usual = 16 / FgPack<T>::E;      // 16 columns a thread
     if (fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.y, a.gamma, a.beta)) {
-        const HeldPlan p = held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 1, usual, 8, 1, 1024);
+        const HeldPlan p = held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 1, usual, 8, 1, 512);
         if (p.threads)
             return p.units == 1 ? launch_straight<T, 1>(ctx, a, p) : p.units == 2 ? launch_straight<T, 2>(ctx, a, p)
                    : p.units == 4 ? launch_straight<T, 4>(ctx, a, p) : launch_straight<T, 8>(ctx, a, p);
@@ -571,7 +595,7 @@ template <typename T>
 int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
     constexpr int usual = 16 / FgPack<T>::E;
     const bool straight = fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.dy, a.gamma, a.dx);
-    const HeldPlan p = straight ? held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 1, usual, usual, 2, 512) : held_plan(ctx, a.rows, a.cols, 4, 8, 16, 0, 1024);
+    const HeldPlan p = straight ? held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 1, usual, usual, 2, 512) : held_plan(ctx, a.rows, a.cols, 4, 4, 16, 0, 1024);
     if (p.threads) {
         float* parts = nullptr;
         const uint32_t pitch = (a.cols + 127) / 128 * 128;
