@@ -67,11 +67,15 @@ template <typename T>
 struct Weights {
     const double* roots;
     double m, c;              // the largest logit; log2(e) / T
+    float top, rate;          // the same in f32
     uint32_t kmax;
-    __device__ __forceinline__ double scaled(uint32_t key) const {      // 2^42 w, not rounded; 0 below 2^-44
-        if (key == kmax) return kOne;
-        const double t = ((double)logit_of<T>(key) - m) * c;
-        if (!(t > -44.0)) return 0.0;
+    bool ordinary;            // finite in f32: bins and the test for small weights can be trusted
+    // 2^42 w, not rounded; 0 for weights that round to 0, -inf and NaN
+    __device__ __forceinline__ double scaled(float x) const {
+        if (x == top) return kOne;
+        const float d = (top - x) * rate;
+        if (ordinary ? !(d < 44.0f) : !(x > -INFINITY) || !(((double)x - m) * c > -44.0)) return 0.0;
+        const double t = ((double)x - m) * c;
         constexpr double kMagic = 6755399441055744.0;      // 1.5 * 2^52: a sum with it has its whole part in the low word
         const double y = __fma_rn(t, 64.0, kMagic);
         const int j = __double2loint(y);
@@ -83,10 +87,16 @@ struct Weights {
         p = __fma_rn(r, p, l);
         p = __fma_rn(r, p, 1.0);
         const double v = roots[j & 63] * p;
-        return __hiloint2double(__double2hiint(v) + ((j >> 6) + 42 << 20), __double2loint(v));
+        return __hiloint2double(__double2hiint(v) + (((j >> 6) + 42) << 20), __double2loint(v));
     }
     static __device__ __forceinline__ uint64_t whole(double v) { return (uint64_t)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull; }
-    __device__ __forceinline__ uint64_t operator()(uint32_t key) const { return whole(scaled(key)); }
+    __device__ __forceinline__ uint64_t operator()(float x) const { return whole(scaled(x)); }
+    __device__ __forceinline__ uint64_t of_key(uint32_t key) const { return whole(scaled(logit_of<T>(key))); }
+    // Bins of a 32nd of an octave below the largest; the last one has all that is far below, and what is never drawn.  Grows as x falls.
+    __device__ __forceinline__ uint32_t bin(float x) const {
+        const float d = (top - x) * rate;
+        return d < (float)(kBins / 32) ? (uint32_t)(d * 32.0f) : (uint32_t)kBins - 1;
+    }
 };
 
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
@@ -101,27 +111,23 @@ struct Shared {
     double roots[64];
     uint64_t hist[2][256];
     uint64_t slots[2][2];                 // what a CTA tells the others
-    uint64_t red[kWarps], mass[kWarps], ties[kWarps];
-    uint32_t bins[kBins];
+    uint64_t red[kWarps], red2[kWarps];
+    uint32_t bins[kBins];                 // later the candidates for the end of a nucleus
     uint2 local[kLocal];                  // (key, column)
     Border border;
-    uint32_t next_lo, next_hi, found;
+    uint32_t next_lo, next_hi;
 };
 
-// What the functions below go over: units of kPer keys, in the order of the columns.
+// What the functions below go over: units of kPer logits, in the order of the columns; a thread owns `stretch` units in a row.
 template <typename T>
 struct HeldSlice {      // a slice in shared memory, by 16-byte words; masked where a word reaches over the slice's ends
     static constexpr int kPer = FgPack<T>::E;
     const uint4* words;
     uint32_t units, column;               // of the first word's first element (it may lie before the slice)
     __device__ __forceinline__ void values(uint32_t u, float (&x)[kPer]) const { FgPack<T>::widen(words[u], x); }
-    __device__ __forceinline__ void keys(uint32_t u, uint32_t (&k)[kPer]) const {
-        float x[kPer];
-        values(u, x);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) k[e] = key_of<T>(x[e]);
-    }
-    __device__ __forceinline__ uint32_t column_of(uint32_t u, int e) const { return column + u * kPer + e; }
+    __device__ __forceinline__ float value(uint32_t i) const { return fg_widen(reinterpret_cast<const T*>(words)[i]); }
+    __device__ __forceinline__ uint32_t column_of(uint32_t i) const { return column + i; }
+    __device__ __forceinline__ uint32_t stretch() const { return ((units + kThreads - 1) / kThreads) | 1; }      // odd: no two lanes on one bank
 };
 template <typename T>
 struct FarSlice {       // a slice that shared memory does not hold
@@ -129,15 +135,19 @@ struct FarSlice {       // a slice that shared memory does not hold
     const T* data;
     uint32_t units, column;
     __device__ __forceinline__ void values(uint32_t u, float (&x)[1]) const { x[0] = fg_widen(data[u]); }
-    __device__ __forceinline__ void keys(uint32_t u, uint32_t (&k)[1]) const { k[0] = key_of<T>(fg_widen(data[u])); }
-    __device__ __forceinline__ uint32_t column_of(uint32_t u, int) const { return column + u; }
+    __device__ __forceinline__ float value(uint32_t i) const { return fg_widen(data[i]); }
+    __device__ __forceinline__ uint32_t column_of(uint32_t i) const { return column + i; }
+    __device__ __forceinline__ uint32_t stretch() const { return (units + kThreads - 1) / kThreads; }
 };
-struct List {
+template <typename T>
+struct List {           // entries (key, column)
     static constexpr int kPer = 1;
     const uint2* entries;
     uint32_t units;
-    __device__ __forceinline__ void keys(uint32_t u, uint32_t (&k)[1]) const { k[0] = entries[u].x; }
-    __device__ __forceinline__ uint32_t column_of(uint32_t u, int) const { return entries[u].y; }
+    __device__ __forceinline__ void values(uint32_t u, float (&x)[1]) const { x[0] = logit_of<T>(entries[u].x); }
+    __device__ __forceinline__ float value(uint32_t i) const { return logit_of<T>(entries[i].x); }
+    __device__ __forceinline__ uint32_t column_of(uint32_t i) const { return entries[i].y; }
+    __device__ __forceinline__ uint32_t stretch() const { return ((units + kThreads - 1) / kThreads) | 1; }
 };
 
 // A block and, where kAll, the other CTAs of its cluster.
@@ -167,6 +177,28 @@ struct Team {
         for (int w = 0; w < kWarps; ++w) v = max(v, (uint32_t)sh.red[w]);
         return v;
     }
+    // Sums of a and b over the threads before this one; the block's in all_a and all_b.
+    __device__ __forceinline__ void prefix(uint64_t& a, uint64_t& b, uint64_t& all_a, uint64_t& all_b) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        uint64_t x = a, y = b;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t up = __shfl_up_sync(kFull, x, o), up2 = __shfl_up_sync(kFull, y, o);
+            if (lane >= o) { x += up; y += up2; }
+        }
+        __syncthreads();
+        if (lane == 31) { sh.red[warp] = x; sh.red2[warp] = y; }
+        __syncthreads();
+        a = x - a;
+        b = y - b;
+        all_a = all_b = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == warp) { a += all_a; b += all_b; }
+            all_a += sh.red[w];
+            all_b += sh.red2[w];
+        }
+    }
     // Every CTA's pair, to every thread: f(cta, a, b) in the order of the CTAs.
     template <typename F>
     __device__ __forceinline__ void exchange(uint64_t a, uint64_t b, F f) {
@@ -181,28 +213,29 @@ struct Team {
     }
 };
 
-// The border at which the sum over the keys from kmax down to lo (counts, or weights) reaches `target`; all of them together do.
+// The border at which `above` and the sum over the keys from kmax down to lo (counts, or weights) reach `target`; all of them together do.
 template <bool kAll, typename S, typename T>
-__device__ Border find_border(Team& team, const S& source, const Weights<T>& w, uint32_t lo, uint64_t target, bool by_weight) {
+__device__ Border find_border(Team& team, const S& source, const Weights<T>& w, uint32_t lo, uint64_t above, uint64_t target, bool by_weight) {
     Shared& sh = team.sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t hi = w.kmax;
     Border at{};
-    uint64_t above = 0;
     for (int round = 0; round < 5; ++round) {      // 32 bits of range, eight less after each
         const int bits = 32 - __clz(hi - lo), shift = bits > 8 ? bits - 8 : 0;
         uint64_t* const hist = sh.hist[team.round ^= 1];
         hist[tid] = 0;
         __syncthreads();
         for (uint32_t u = tid; u < source.units; u += kThreads) {
-            uint32_t k[S::kPer];
-            source.keys(u, k);
+            float x[S::kPer];
+            source.values(u, x);
 #pragma unroll
-            for (int e = 0; e < S::kPer; ++e)
-                if (k[e] >= lo && k[e] <= hi) {
-                    const uint64_t v = by_weight ? w(k[e]) : 1;
-                    if (v) atomicAdd((unsigned long long*)&hist[(k[e] - lo) >> shift], (unsigned long long)v);
+            for (int e = 0; e < S::kPer; ++e) {
+                const uint32_t k = key_of<T>(x[e]);
+                if (k >= lo && k <= hi) {
+                    const uint64_t v = by_weight ? w(x[e]) : 1;
+                    if (v) atomicAdd((unsigned long long*)&hist[(k - lo) >> shift], (unsigned long long)v);
                 }
+            }
         }
         uint64_t v = 0;
         if (kAll) {
@@ -236,151 +269,140 @@ __device__ Border find_border(Team& team, const S& source, const Weights<T>& w, 
     __syncthreads();
     return at;
 }
+// The nucleus ends at `at`: as many ties as it takes to reach the target, of at most `most`.
+template <typename T>
+__device__ __forceinline__ uint64_t ties_to_reach(const Weights<T>& w, const Border& at, uint64_t target, uint64_t most) {
+    const uint64_t each = w.of_key(at.key);
+    return each ? min(most, (target - at.above + each - 1) / each) : 0;
+}
+__device__ __forceinline__ uint64_t nucleus(float p, uint64_t weight) {
+    return max((uint64_t)1, (uint64_t)__double2ull_ru((double)max(p, 0.0f) * (double)weight));
+}
 
-// Keys above `cut` and the first `ties` of those at it, of weight `least` (in parts of 2^42) or more: the first at which their running sum
-// exceeds u times the total.
+// What is kept: keys above `cut` and the first `ties` of those at it, of weight `least` (in parts of 2^42) or more.
+struct Kept { uint32_t cut; uint64_t ties; double least; };
+
+// The first at which the running sum over what is kept exceeds u times the total.  mass and same: the kept weight above the cut, and the
+// keys at it, of the thread's stretch.
 template <bool kAll, typename S, typename T>
-__device__ void draw(Team& team, const S& source, const Weights<T>& w, uint32_t cut, uint64_t ties, double least, float u, uint32_t* token, float* prob) {
-    Shared& sh = team.sh;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const double cut_scaled = cut ? w.scaled(cut) : 0.0;
-    const uint64_t at_cut = cut_scaled >= least ? w.whole(cut_scaled) : 0;
-    auto weigh = [&](uint32_t key) -> uint64_t {
-        if (key <= cut) return 0;
-        const double v = w.scaled(key);
-        return v >= least ? w.whole(v) : 0;
-    };
-    const uint32_t len = ((source.units + kWarps - 1) / kWarps + 31) / 32 * 32;      // a warp's stretch
-    const uint32_t u0 = min(source.units, warp * len), u1 = min(source.units, u0 + len);
-    uint64_t s = 0, t = 0;
-    for (uint32_t i = u0 + lane; i < u1; i += 32) {
-        uint32_t k[S::kPer];
-        source.keys(i, k);
-#pragma unroll
-        for (int e = 0; e < S::kPer; ++e) {
-            s += weigh(k[e]);
-            t += k[e] == cut && cut;
-        }
-    }
-    s = warp_sum64(s);
-    t = warp_sum64(t);
-    __syncthreads();
-    if (lane == 0) { sh.mass[warp] = s; sh.ties[warp] = t; }
-    __syncthreads();
-    uint64_t before = 0, total = 0, room = ties;      // before this CTA; room for ties at the cut
-    auto add = [&](uint64_t mass, uint64_t same) {
-        const uint64_t kept = min(room, same);
-        room -= kept;
-        return mass + kept * at_cut;
-    };
-    uint64_t own_mass = 0, own_ties = 0;
-#pragma unroll
-    for (int j = 0; j < kWarps; ++j) { own_mass += sh.mass[j]; own_ties += sh.ties[j]; }
-    uint64_t own_room = ties;
-    if (kAll)
-        team.exchange(own_mass, own_ties, [&](uint32_t c, uint64_t mass, uint64_t same) {
-            if (c == team.cta) { before = total; own_room = room; }
-            total += add(mass, same);
+__device__ void locate(Team& team, const S& source, const Weights<T>& w, const Kept& keep, uint64_t mass, uint64_t same, float u, uint32_t* token, float* prob) {
+    const int lane = threadIdx.x & 31;
+    const double cut_scaled = keep.cut ? w.scaled(logit_of<T>(keep.cut)) : 0.0;
+    const uint64_t at_cut = cut_scaled >= keep.least ? w.whole(cut_scaled) : 0;
+    uint64_t m = mass, t = same, all_m, all_t;
+    team.prefix(m, t, all_m, all_t);
+    if (kAll) {
+        uint64_t sum_m = 0, sum_t = 0, before_m = 0, before_t = 0;
+        team.exchange(all_m, all_t, [&](uint32_t c, uint64_t x, uint64_t y) {
+            if (c == team.cta) { before_m = sum_m; before_t = sum_t; }
+            sum_m += x;
+            sum_t += y;
         });
-    else total = add(own_mass, own_ties);
-    const uint64_t goal = (uint64_t)((double)(u > 0.0f ? min(u, 0.99999994f) : 0.0f) * (double)total);
-    room = own_room;
-    for (int j = 0; j < warp; ++j) before += add(sh.mass[j], sh.ties[j]);
-    uint64_t left = room;
-    if (before <= goal && goal < before + add(sh.mass[warp], sh.ties[warp])) {
-        uint64_t sum = before;
-        for (uint32_t i = u0; i < u1; i += 32) {
-            uint32_t k[S::kPer];
-            uint64_t v[S::kPer], run = 0, same = 0;
-#pragma unroll
-            for (int e = 0; e < S::kPer; ++e) k[e] = 0;
-            if (i + lane < u1) source.keys(i + lane, k);
-#pragma unroll
-            for (int e = 0; e < S::kPer; ++e) same += k[e] == cut && cut;
-            uint64_t upto = same;      // ties in this lane and those before it
-            if (__any_sync(kFull, same != 0))
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint64_t up = __shfl_up_sync(kFull, upto, o);
-                    if (lane >= o) upto += up;
-                }
-            uint64_t rank = upto - same;
-#pragma unroll
-            for (int e = 0; e < S::kPer; ++e) {
-                v[e] = weigh(k[e]);
-                if (k[e] == cut && cut) v[e] = rank++ < left ? at_cut : 0;
-                run += v[e];
-            }
-            uint64_t through = run;
+        m += before_m; t += before_t;
+        all_m = sum_m; all_t = sum_t;
+        cg::this_cluster().barrier_arrive();      // nobody reads another's memory from here on
+    }
+    auto upto = [&](uint64_t x, uint64_t y) { return x + min(keep.ties, y) * at_cut; };
+    const uint64_t total = upto(all_m, all_t), goal = (uint64_t)((double)(u > 0.0f ? min(u, 0.99999994f) : 0.0f) * (double)total), before = upto(m, t);
+    const unsigned holds = __ballot_sync(kFull, before <= goal && goal < upto(m + mass, t + same));
+    if (holds) {      // the warp goes over that thread's stretch once more
+        const int from = __ffs(holds) - 1;
+        const uint32_t stretch = source.stretch(), u0 = (threadIdx.x - lane + from) * stretch;
+        const uint32_t i1 = min(source.units, u0 + stretch) * S::kPer;
+        uint64_t sum = __shfl_sync(kFull, before, from), ties = __shfl_sync(kFull, t, from);
+        for (uint32_t i = u0 * S::kPer; i < i1; i += 32) {
+            const float x = i + lane < i1 ? source.value(i + lane) : -INFINITY;
+            const uint32_t key = key_of<T>(x);
+            const unsigned tied = __ballot_sync(kFull, key == keep.cut && key);
+            uint64_t v = 0;
+            if (key > keep.cut) {
+                const double s = w.scaled(x);
+                v = s >= keep.least ? w.whole(s) : 0;
+            } else if (key && key == keep.cut && ties + __popc(tied & ((1u << lane) - 1)) < keep.ties) v = at_cut;
+            uint64_t run = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const uint64_t up = __shfl_up_sync(kFull, through, o);
-                if (lane >= o) through += up;
+                const uint64_t up = __shfl_up_sync(kFull, run, o);
+                if (lane >= o) run += up;
             }
-            const unsigned over = __ballot_sync(kFull, sum + through > goal);
+            const unsigned over = __ballot_sync(kFull, sum + run > goal);
             if (over) {
                 if (lane == __ffs(over) - 1) {
-                    uint64_t at = sum + through - run;
-                    bool done = false;
-#pragma unroll
-                    for (int e = 0; e < S::kPer; ++e) {
-                        at += v[e];
-                        if (!done && at > goal) {
-                            done = true;
-                            *token = source.column_of(i + lane, e);
-                            if (prob) *prob = (float)((double)v[e] / (double)total);
-                        }
-                    }
+                    *token = source.column_of(i + lane);
+                    if (prob) *prob = (float)((double)v / (double)total);
                 }
                 break;
             }
-            sum += __shfl_sync(kFull, through, 31);
-            left -= min(left, __shfl_sync(kFull, upto, 31));
+            sum += __shfl_sync(kFull, run, 31);
+            ties += __popc(tied);
         }
     }
+    if (kAll) cg::this_cluster().barrier_wait();
+}
+template <bool kAll, typename S, typename T>
+__device__ void draw(Team& team, const S& source, const Weights<T>& w, const Kept& keep, float u, uint32_t* token, float* prob) {
+    const uint32_t stretch = source.stretch(), u0 = min(source.units, threadIdx.x * stretch), u1 = min(source.units, u0 + stretch);
+    uint64_t mass = 0, same = 0;
+    if (keep.cut == 0 && keep.least == 0.0) {      // all of it
+        for (uint32_t i = u0; i < u1; ++i) {
+            float x[S::kPer];
+            source.values(i, x);
+#pragma unroll
+            for (int e = 0; e < S::kPer; ++e) mass += w(x[e]);
+        }
+    } else
+        for (uint32_t i = u0; i < u1; ++i) {
+            float x[S::kPer];
+            source.values(i, x);
+#pragma unroll
+            for (int e = 0; e < S::kPer; ++e) {
+                const uint32_t key = key_of<T>(x[e]);
+                if (key > keep.cut) {
+                    const double s = w.scaled(x[e]);
+                    if (s >= keep.least) mass += w.whole(s);
+                }
+                same += key == keep.cut && key;
+            }
+        }
+    locate<kAll>(team, source, w, keep, mass, same, u, token, prob);
 }
 
-// The filters on what `source` holds: all that can be drawn, and with kAll all of the row.  `count`: of keys; `all_weight`: of the row, when it
-// is known (0: it is that of the source).
+// The filters on what `source` holds: all that can be drawn, and with kAll all of the row.  `count`: of keys.
 template <bool kAll, typename S, typename T>
-__device__ void filter_and_draw(Team& team, const S& source, const Weights<T>& w, uint32_t kmin, uint64_t count, uint64_t all_weight, uint32_t k, float p, double least,
-                                float u, uint32_t* token, float* prob) {
-    uint32_t cut = 0;
-    uint64_t ties = 0;
+__device__ void filter_and_draw(Team& team, const S& source, const Weights<T>& w, uint32_t kmin, uint64_t count, uint32_t k, float p, double least, float u, uint32_t* token,
+                                float* prob) {
+    Kept keep{0, 0, least};
     if (k != 0 && k < count) {
-        const Border at = find_border<kAll>(team, source, w, kmin, k, false);
-        cut = at.key;
-        ties = k - at.above;
+        const Border at = find_border<kAll>(team, source, w, kmin, 0, k, false);
+        keep.cut = at.key;
+        keep.ties = k - at.above;
     }
     if (p < 1.0f) {
-        if (cut || all_weight == 0) {
-            uint64_t s = 0, t = 0;
-            for (uint32_t i = threadIdx.x; i < source.units; i += kThreads) {
-                uint32_t key[S::kPer];
-                source.keys(i, key);
+        uint64_t s = 0, t = 0;
+        for (uint32_t i = threadIdx.x; i < source.units; i += kThreads) {
+            float x[S::kPer];
+            source.values(i, x);
 #pragma unroll
-                for (int e = 0; e < S::kPer; ++e) {
-                    if (key[e] > cut) s += w(key[e]);
-                    t += key[e] == cut && cut;
-                }
+            for (int e = 0; e < S::kPer; ++e) {
+                const uint32_t key = key_of<T>(x[e]);
+                if (key > keep.cut) s += w(x[e]);
+                t += key == keep.cut && key;
             }
-            s = team.block_sum(s);
-            t = team.block_sum(t);
-            if (kAll) {
-                uint64_t s_all = 0, t_all = 0;
-                team.exchange(s, t, [&](uint32_t, uint64_t a, uint64_t b) { s_all += a; t_all += b; });
-                s = s_all;
-                t = t_all;
-            }
-            all_weight = s + (cut ? min(t, ties) * w(cut) : 0);
         }
-        const uint64_t target = max((uint64_t)1, (uint64_t)__double2ull_ru((double)max(p, 0.0f) * (double)all_weight));
-        const Border at = find_border<kAll>(team, source, w, cut ? cut : kmin, target, true);
-        const uint64_t each = w(at.key), need = each ? (target - at.above + each - 1) / each : 0;
-        ties = at.key == cut ? min(ties, need) : need;
-        cut = at.key;
+        s = team.block_sum(s);
+        t = team.block_sum(t);
+        if (kAll) {
+            uint64_t s_all = 0, t_all = 0;
+            team.exchange(s, t, [&](uint32_t, uint64_t a, uint64_t b) { s_all += a; t_all += b; });
+            s = s_all;
+            t = t_all;
+        }
+        const uint64_t target = nucleus(p, s + (keep.cut ? min(t, keep.ties) * w.of_key(keep.cut) : 0));
+        const Border at = find_border<kAll>(team, source, w, keep.cut ? keep.cut : kmin, 0, target, true);
+        keep.ties = ties_to_reach(w, at, target, at.key == keep.cut ? keep.ties : ~0ull);
+        keep.cut = at.key;
     }
-    draw<kAll>(team, source, w, cut, ties, least, u, token, prob);
+    draw<kAll>(team, source, w, keep, u, token, prob);
 }
 
 template <typename T, bool kHeld>
@@ -441,11 +463,11 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         uint32_t first = 0;
         if (largest == kmax && key_of<T>(mine) == kmax)
             for (uint32_t u = tid; u < slice.units; u += kThreads) {
-                uint32_t k[Slice::kPer];
-                slice.keys(u, k);
+                float x[Slice::kPer];
+                slice.values(u, x);
 #pragma unroll
-                for (int e = Slice::kPer - 1; e >= 0; --e)
-                    if (k[e] == kmax) first = max(first, ~slice.column_of(u, e));
+                for (int e = 0; e < Slice::kPer; ++e)
+                    if (key_of<T>(x[e]) == kmax) first = max(first, ~slice.column_of(u * Slice::kPer + e));
             }
         first = team.block_max(first);
         team.exchange(first, 0, [&](uint32_t, uint64_t inverse, uint64_t) { first = max(first, (uint32_t)inverse); });
@@ -454,34 +476,26 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         return;
     }
     const float top = logit_of<T>(kmax);
-    const Weights<T> w{sh.roots, (double)top, 1.4426950408889634 / (double)temperature, kmax};
-    const float rate = (float)w.c, u = a.u[r], p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
-    const uint32_t k = a.top_k ? a.top_k[r] : 0;
+    const double per_octave = 1.4426950408889634 / (double)temperature;
+    const Weights<T> w{sh.roots, (double)top, per_octave, top, (float)per_octave, kmax, top < INFINITY && per_octave < 1e30 && per_octave > 1e-30};
+    const float u = a.u[r], p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
+    const uint32_t k = a.top_k && a.top_k[r] < a.cols ? a.top_k[r] : 0;
     const double least = mp > 0.0f ? (double)min(mp, 1.0f) * kOne : 0.0;
-    const bool by_k = k != 0 && k < a.cols, by_p = p < 1.0f;
-    if (!by_k && !by_p) {
-        draw<true>(team, slice, w, 0, 0, least, u, token, prob);
-        cluster.sync();
+    if (!k && !(p < 1.0f)) {
+        draw<true>(team, slice, w, Kept{0, 0, least}, u, token, prob);
         return;
     }
+    const uint32_t stretch = slice.stretch(), u0 = min(slice.units, tid * stretch), u1 = min(slice.units, u0 + stretch);
 
-    // A bound below the border: `bound` bins of a 32nd of an octave below the largest.
-    auto bin_of = [&](float x) {      // grows as x falls
-        const float d = (top - x) * rate;
-        return d < (float)(kBins / 32) ? (uint32_t)(d * 32.0f) : (uint32_t)kBins - 1;
-    };
-    uint32_t bound = kBins - 1;
-    uint64_t all_weight = 0;
-    const bool ordinary = top < INFINITY && rate < 1e30f;      // else bins say nothing
-    if (ordinary && by_k) {
+    if (w.ordinary && k) {
         // k threads with a value of a bin or above it say that the k-th largest is not below it; so do k / ctas threads in each CTA.
-        const uint32_t bin = key_of<T>(mine) ? bin_of(mine) : kBins;
+        const uint32_t own_bin = key_of<T>(mine) ? w.bin(mine) : kBins;
         auto reached = [&](uint32_t want) {
             uint32_t b = kBins - 1;
             if (want <= kThreads)
                 for (uint32_t lo = 0, hi = kBins - 1; lo <= hi;) {      // 11 steps
                     const uint32_t mid = (lo + hi) / 2;
-                    if ((uint32_t)__syncthreads_count(bin <= mid) >= want) {
+                    if ((uint32_t)__syncthreads_count(own_bin <= mid) >= want) {
                         b = mid;
                         if (mid == 0) break;
                         hi = mid - 1;
@@ -492,34 +506,71 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         const uint32_t share = reached((k + team.ctas - 1) / team.ctas), whole = team.ctas > 1 ? reached(k) : share;
         uint32_t worst = 0, best = kBins - 1;
         team.exchange(share, whole, [&](uint32_t, uint64_t x, uint64_t y) { worst = max(worst, (uint32_t)x); best = min(best, (uint32_t)y); });
-        bound = min(worst, best);
-    } else if (ordinary) {
-        // The weight of the row, exactly, and how many of its tokens lie in each bin: their weight is at least that of the bin's end.
+        const uint32_t bound = min(worst, best);
+        // What is not below it goes to the first CTA, in order: count, then places.
+        auto candidate = [&](float x) { return x > -INFINITY && w.bin(x) <= bound; };
+        uint64_t count = 0, none = 0, own, unused;
+        for (uint32_t i = u0; i < u1; ++i) {
+            float x[Slice::kPer];
+            slice.values(i, x);
+#pragma unroll
+            for (int e = 0; e < Slice::kPer; ++e) count += candidate(x[e]);
+        }
+        const bool any = count != 0;
+        team.prefix(count, none, own, unused);
+        if (any && own <= kLocal)
+            for (uint32_t i = u0; i < u1; ++i) {
+                float x[Slice::kPer];
+                slice.values(i, x);
+#pragma unroll
+                for (int e = 0; e < Slice::kPer; ++e)
+                    if (candidate(x[e])) sh.local[count++] = make_uint2(key_of<T>(x[e]), slice.column_of(i * Slice::kPer + e));
+            }
+        bool fits = true;
+        uint32_t offset = 0, listed = 0;
+        team.exchange(own, 0, [&](uint32_t c, uint64_t n_c, uint64_t) {
+            if (c == team.cta) offset = listed;
+            listed += (uint32_t)min(n_c, (uint64_t)kGathered + 1);
+            fits = fits && n_c <= kLocal;
+        });
+        if (fits && listed <= kGathered) {
+            uint2* const list = reinterpret_cast<uint2*>(dynamic);      // nobody reads a slice any more
+            uint2* const to = cluster.map_shared_rank(list, 0) + offset;
+            for (uint32_t i = tid; i < (uint32_t)own; i += kThreads) to[i] = sh.local[i];
+            cluster.sync();
+            if (team.cta) return;
+            uint32_t inverse = 0;
+            for (uint32_t i = tid; i < listed; i += kThreads) inverse = max(inverse, ~list[i].x);
+            inverse = team.block_max(inverse);
+            filter_and_draw<false>(team, List<T>{list, listed}, w, ~inverse, listed, k, p, least, u, token, prob);
+            return;
+        }
+    } else if (w.ordinary) {
+        // The weight of the row, exactly, and how many of its tokens lie in each bin.  A bin's tokens weigh between what its two ends would, so the
+        // counts say in which bins the nucleus may end: what lies above them is kept for sure, what lies in them goes to the first CTA.
         for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
         __syncthreads();
-        uint64_t s = 0;
+        uint64_t weight = 0, all_weight = 0;
         for (uint32_t i = tid; i < slice.units; i += kThreads) {
             float x[Slice::kPer];
             slice.values(i, x);
 #pragma unroll
             for (int e = 0; e < Slice::kPer; ++e) {
-                const uint32_t b = bin_of(x[e]);
-                if (b < kBins - 1) {
-                    s += w(key_of<T>(x[e]));
-                    atomicAdd(&sh.bins[b], 1u);
-                }
+                const uint32_t b = w.bin(x[e]);
+                weight += w(x[e]);
+                if (b < kBins - 1) atomicAdd(&sh.bins[b], 1u);
             }
         }
-        s = team.block_sum(s);
-        team.exchange(s, 0, [&](uint32_t, uint64_t part, uint64_t) { all_weight += part; });
-        // (the exchange has all CTAs' bins complete)  A thread takes eight bins, then a prefix over the threads.
-        float sum = 0.0f, part[kBins / kThreads];
+        weight = team.block_sum(weight);
+        team.exchange(weight, 0, [&](uint32_t, uint64_t part, uint64_t) { all_weight += part; });
+        const uint64_t target = nucleus(p, all_weight);
+        constexpr int kEach = kBins / kThreads;      // a thread takes eight bins
+        float sum = 0.0f, part[kEach];
 #pragma unroll
-        for (int j = 0; j < kBins / kThreads; ++j) {
-            const uint32_t b = tid * (kBins / kThreads) + j;
+        for (int j = 0; j < kEach; ++j) {
             uint32_t in_bin = 0;
-            for (uint32_t c = 0; c < team.ctas; ++c) in_bin += cluster.map_shared_rank(sh.bins, c)[b];
-            part[j] = sum += (float)in_bin * exp2f(-(float)(b + 1) / 32.0f);
+            for (uint32_t c = 0; c < team.ctas; ++c) in_bin += cluster.map_shared_rank(sh.bins, c)[tid * kEach + j];
+            part[j] = sum += (float)in_bin * exp2f(-(float)(tid * kEach + j) / 32.0f);      // at the bin's upper end
         }
         float run = sum;
 #pragma unroll
@@ -527,98 +578,112 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             const float up = __shfl_up_sync(kFull, run, o);
             if (lane >= o) run += up;
         }
-        float* const sums = reinterpret_cast<float*>(sh.red);
+        float* const sums = reinterpret_cast<float*>(sh.red2);
         if (lane == 31) sums[warp] = run;
         __syncthreads();
         float before = run - sum;
         for (int j = 0; j < warp; ++j) before += sums[j];
-        const float goal = (float)((double)max(p, 0.0f) * (double)all_weight / kOne) * 1.001f;      // bins and sums in f32: a thousandth covers what they lose
-        uint32_t b = kBins - 1;
+        // f32 sums and bins are good to 1e-4; the lower end is 2^(-1/32) of the upper one
+        const float goal = (float)((double)target / kOne);
+        uint32_t first = kBins - 1, last = kBins - 1;
 #pragma unroll
-        for (int j = kBins / kThreads - 1; j >= 0; --j)
-            if (before + part[j] >= goal) b = tid * (kBins / kThreads) + j;
-        bound = kBins - 1 - team.block_max(kBins - 1 - b);
+        for (int j = kEach - 1; j >= 0; --j) {
+            if (before + part[j] >= goal * 0.999f) first = tid * kEach + j;
+            if ((before + part[j]) * 0.97857f >= goal * 1.001f) last = tid * kEach + j;
+        }
+        first = kBins - 1 - team.block_max(kBins - 1 - first);
+        last = kBins - 1 - team.block_max(kBins - 1 - last);
+        cluster.sync();      // the bins have been read: the first CTA's take the candidates
+        uint64_t sure = 0, kept = 0, count = 0, none = 0, own, unused;      // weight above the bins; of it, what min_p keeps; candidates
+        for (uint32_t i = u0; i < u1; ++i) {
+            float x[Slice::kPer];
+            slice.values(i, x);
+            unsigned above = 0;
+#pragma unroll
+            for (int e = 0; e < Slice::kPer; ++e) {
+                const uint32_t b = w.bin(x[e]);
+                above |= (unsigned)(b < first) << e;
+                count += b >= first && b <= last && x[e] > -INFINITY;
+            }
+            for (; above; above &= above - 1) {      // few: one at a time
+                const double v = w.scaled(slice.value(i * Slice::kPer + __ffs(above) - 1));
+                const uint64_t q = w.whole(v);
+                sure += q;
+                if (v >= least) kept += q;
+            }
+        }
+        uint32_t place = (uint32_t)count, end;
+        const bool any = count != 0;
+        team.prefix(count, none, own, unused);
+        end = (uint32_t)count + place;
+        place = (uint32_t)count;
+        if (any && own <= kLocal)
+            for (uint32_t i = u0, at = place; i < u1; ++i) {
+                float x[Slice::kPer];
+                slice.values(i, x);
+#pragma unroll
+                for (int e = 0; e < Slice::kPer; ++e) {
+                    const uint32_t b = w.bin(x[e]);
+                    if (b >= first && b <= last && x[e] > -INFINITY) sh.local[at++] = make_uint2(key_of<T>(x[e]), slice.column_of(i * Slice::kPer + e));
+                }
+            }
+        const uint64_t own_sure = team.block_sum(sure);
+        bool fits = true;
+        uint32_t offset = 0, listed = 0;
+        uint64_t all_sure = 0;
+        team.exchange(own_sure, own, [&](uint32_t c, uint64_t s, uint64_t n_c) {
+            if (c == team.cta) offset = listed;
+            listed += (uint32_t)min(n_c, (uint64_t)kLocal + 1);
+            all_sure += s;
+            fits = fits && n_c <= kLocal;
+        });
+        if (fits && listed && listed <= kBins / 2) {
+            uint2* const list = reinterpret_cast<uint2*>(sh.bins);
+            uint2* const to = cluster.map_shared_rank(list, 0) + offset;
+            for (uint32_t i = tid; i < (uint32_t)own; i += kThreads) to[i] = sh.local[i];
+            cluster.sync();
+            Kept keep{0, 0, least};
+            if (team.cta == 0) {
+                uint32_t inverse = 0;
+                for (uint32_t i = tid; i < listed; i += kThreads) inverse = max(inverse, ~list[i].x);
+                inverse = team.block_max(inverse);
+                const Border at = find_border<false>(team, List<T>{list, listed}, w, ~inverse, all_sure, target, true);
+                keep.cut = at.key;
+                keep.ties = ties_to_reach(w, at, target, ~0ull);
+            }
+            team.exchange(keep.cut, keep.ties, [&](uint32_t c, uint64_t x, uint64_t y) {
+                if (c == 0) { keep.cut = (uint32_t)x; keep.ties = y; }
+            });
+            uint64_t same = 0;
+            for (uint32_t i = place; any && i < end; ++i) {
+                const uint32_t key = sh.local[i].x;
+                same += key == keep.cut;
+                if (key > keep.cut) {
+                    const double v = w.scaled(logit_of<T>(key));
+                    if (v >= least) kept += w.whole(v);
+                }
+            }
+            locate<true>(team, slice, w, keep, kept, same, u, token, prob);
+            return;
+        }
     }
-
-    // What lies above it, in order: count, then places.
-    const uint32_t len = ((slice.units + kWarps - 1) / kWarps + 31) / 32 * 32;
-    const uint32_t u0 = min(slice.units, warp * len), u1 = min(slice.units, u0 + len);
-    uint32_t candidates = 0;
-    auto chosen = [&](float x) { return x > -INFINITY && (!ordinary || bin_of(x) <= bound); };
-    for (uint32_t i = u0 + lane; i < u1; i += 32) {
+    // Too many candidates: on the row as it lies.
+    uint32_t inverse = 0;
+    uint64_t count = 0, count_all = 0;
+    for (uint32_t i = tid; i < slice.units; i += kThreads) {
         float x[Slice::kPer];
         slice.values(i, x);
 #pragma unroll
-        for (int e = 0; e < Slice::kPer; ++e) candidates += chosen(x[e]);
-    }
-    candidates = __reduce_add_sync(kFull, candidates);
-    __syncthreads();
-    if (lane == 0) sh.red[warp] = candidates;
-    __syncthreads();
-    uint32_t place = 0, own = 0;
-#pragma unroll
-    for (int j = 0; j < kWarps; ++j) {
-        if (j == warp) place = own;
-        own += (uint32_t)sh.red[j];
-    }
-    if (own <= kLocal && candidates)
-        for (uint32_t i = u0; i < u1; i += 32) {
-            float x[Slice::kPer];
-            uint32_t count = 0;
-#pragma unroll
-            for (int e = 0; e < Slice::kPer; ++e) x[e] = -INFINITY;
-            if (i + lane < u1) slice.values(i + lane, x);
-#pragma unroll
-            for (int e = 0; e < Slice::kPer; ++e) count += chosen(x[e]);
-            if (!__any_sync(kFull, count != 0)) continue;
-            uint32_t upto = count;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t up = __shfl_up_sync(kFull, upto, o);
-                if (lane >= o) upto += up;
-            }
-            uint32_t at = place + upto - count;
-#pragma unroll
-            for (int e = 0; e < Slice::kPer; ++e)
-                if (chosen(x[e])) sh.local[at++] = make_uint2(key_of<T>(x[e]), slice.column_of(i + lane, e));
-            place += __shfl_sync(kFull, upto, 31);
+        for (int e = 0; e < Slice::kPer; ++e) {
+            const uint32_t key = key_of<T>(x[e]);
+            if (key) { inverse = max(inverse, ~key); ++count; }
         }
-    bool fits = true;
-    uint32_t offset = 0, listed = 0;
-    team.exchange(own, 0, [&](uint32_t c, uint64_t count, uint64_t) {
-        if (c == team.cta) offset = listed;
-        listed += (uint32_t)min(count, (uint64_t)kGathered + 1);
-        fits = fits && count <= kLocal;
-    });
-    if (fits && listed <= kGathered) {
-        uint2* const list = reinterpret_cast<uint2*>(dynamic);      // nobody reads a slice any more
-        uint2* const to = cluster.map_shared_rank(list, 0) + offset;
-        for (uint32_t i = tid; i < own; i += kThreads) to[i] = sh.local[i];
-        cluster.sync();
-        if (team.cta) return;
-        const List source{list, listed};
-        uint32_t smallest = 0;
-        for (uint32_t i = tid; i < listed; i += kThreads) smallest = max(smallest, ~list[i].x);
-        const uint32_t kmin = ~team.block_max(smallest);
-        filter_and_draw<false>(team, source, w, kmin, listed, all_weight, by_k ? k : 0, p, least, u, token, prob);
-        return;
     }
-    uint32_t smallest = 0;
-    uint64_t count = 0;
-    for (uint32_t i = tid; i < slice.units; i += kThreads) {
-        uint32_t key[Slice::kPer];
-        slice.keys(i, key);
-#pragma unroll
-        for (int e = 0; e < Slice::kPer; ++e)
-            if (key[e]) { smallest = max(smallest, ~key[e]); ++count; }
-    }
-    smallest = team.block_max(smallest);
+    inverse = team.block_max(inverse);
     count = team.block_sum(count);
-    uint64_t count_all = 0;
-    uint32_t inverse = 0;
-    team.exchange(smallest, count, [&](uint32_t, uint64_t x, uint64_t y) { inverse = max(inverse, (uint32_t)x); count_all += y; });
-    filter_and_draw<true>(team, slice, w, ~inverse, count_all, 0, by_k ? k : 0, p, least, u, token, prob);
-    cluster.sync();
+    const uint32_t own_inverse = inverse;
+    team.exchange(own_inverse, count, [&](uint32_t, uint64_t x, uint64_t y) { inverse = max(inverse, (uint32_t)x); count_all += y; });
+    filter_and_draw<true>(team, slice, w, ~inverse, count_all, k, p, least, u, token, prob);
 }
 
 template <typename T, bool kHeld>
