@@ -94,8 +94,8 @@ struct Weights {
     __device__ __forceinline__ uint64_t of_key(uint32_t key) const { return whole(scaled(logit_of<T>(key))); }
     // Bins of a 32nd of an octave below the largest; the last one has all that is far below, and what is never drawn.  Grows as x falls.
     __device__ __forceinline__ uint32_t bin(float x) const {
-        const float d = (top - x) * rate;
-        return d < (float)(kBins / 32) ? (uint32_t)(d * 32.0f) : (uint32_t)kBins - 1;
+        const float d = (top - x) * (rate * 32.0f);
+        return d < (float)(kBins - 1) ? (uint32_t)d : (uint32_t)kBins - 1;
     }
 };
 
@@ -546,8 +546,9 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             return;
         }
     } else if (w.ordinary) {
-        // The weight of the row, exactly, and how many of its tokens lie in each bin.  A bin's tokens weigh between what its two ends would, so the
-        // counts say in which bins the nucleus may end: what lies above them is kept for sure, what lies in them goes to the first CTA.
+        // The weight of the row, exactly, and of each bin, to a thousandth.  That says in which one or two bins the nucleus ends: what lies above
+        // them is kept for sure, what lies in them goes to the first CTA.  (Counts alone leave a 2 % wide strip, with thousands of tokens
+        // of a flat row.)
         for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
         __syncthreads();
         uint64_t weight = 0, all_weight = 0;
@@ -556,9 +557,12 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             slice.values(i, x);
 #pragma unroll
             for (int e = 0; e < Slice::kPer; ++e) {
-                const uint32_t b = w.bin(x[e]);
                 weight += w(x[e]);
-                if (b < kBins - 1) atomicAdd(&sh.bins[b], 1u);
+                const float d = (top - x[e]) * (w.rate * 32.0f);
+                if (d < (float)(kBins - 1)) {
+                    const uint32_t b = (uint32_t)d;
+                    atomicAdd(&sh.bins[b], 2048u - (uint32_t)((d - (float)b) * 43.87f));      // 2^11 of its weight over the bin's upper end: 2^(-1/32) at the lower
+                }
             }
         }
         weight = team.block_sum(weight);
@@ -570,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         for (int j = 0; j < kEach; ++j) {
             uint32_t in_bin = 0;
             for (uint32_t c = 0; c < team.ctas; ++c) in_bin += cluster.map_shared_rank(sh.bins, c)[tid * kEach + j];
-            part[j] = sum += (float)in_bin * exp2f(-(float)(tid * kEach + j) / 32.0f);      // at the bin's upper end
+            part[j] = sum += (float)in_bin * (exp2f(-(float)(tid * kEach + j) / 32.0f) / 2048.0f);
         }
         float run = sum;
 #pragma unroll
@@ -583,13 +587,13 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         __syncthreads();
         float before = run - sum;
         for (int j = 0; j < warp; ++j) before += sums[j];
-        // f32 sums and bins are good to 1e-4; the lower end is 2^(-1/32) of the upper one
+        // a weight in a bin is off by 2^-11 at most (its rounding, and the chord for the exponential: 6e-5), its bin's place and the f32 sums by 1e-5
         const float goal = (float)((double)target / kOne);
         uint32_t first = kBins - 1, last = kBins - 1;
 #pragma unroll
         for (int j = kEach - 1; j >= 0; --j) {
             if (before + part[j] >= goal * 0.999f) first = tid * kEach + j;
-            if ((before + part[j]) * 0.97857f >= goal * 1.001f) last = tid * kEach + j;
+            if (before + part[j] >= goal * 1.001f) last = tid * kEach + j;
         }
         first = kBins - 1 - team.block_max(kBins - 1 - first);
         last = kBins - 1 - team.block_max(kBins - 1 - last);
