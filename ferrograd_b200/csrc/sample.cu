@@ -112,7 +112,7 @@ struct Shared {
     uint64_t hist[2][256];
     uint64_t slots[2][2];                 // what a CTA tells the others
     uint64_t red[kWarps], red2[kWarps];
-    uint32_t bins[kBins];                 // later the candidates for the end of a nucleus
+    alignas(16) uint32_t bins[kBins];
     uint2 local[kLocal];                  // (key, column)
     Border border;
     uint32_t next_lo, next_hi;
@@ -205,20 +205,23 @@ struct Team {
         cg::cluster_group cluster = cg::this_cluster();
         if (threadIdx.x == 0) { sh.slots[turn][0] = a; sh.slots[turn][1] = b; }
         cluster.sync();
-        for (uint32_t c = 0; c < ctas; ++c) {
-            const uint64_t* const p = cluster.map_shared_rank(&sh.slots[turn][0], c);
-            f(c, p[0], p[1]);
+        uint64_t x = 0, y = 0;
+        const uint32_t lane = threadIdx.x & 31;
+        if (lane < ctas) {
+            const uint64_t* const p = cluster.map_shared_rank(&sh.slots[turn][0], lane);
+            x = p[0];
+            y = p[1];
         }
+        for (uint32_t c = 0; c < ctas; ++c) f(c, __shfl_sync(kFull, x, c), __shfl_sync(kFull, y, c));
         turn ^= 1;
     }
 };
 
-// The border at which `above` and the sum over the keys from kmax down to lo (counts, or weights) reach `target`; all of them together do.
+// The border at which `above` and the sum over the keys from hi down to lo (counts, or weights) reach `target`; all of them together do.
 template <bool kAll, typename S, typename T>
-__device__ Border find_border(Team& team, const S& source, const Weights<T>& w, uint32_t lo, uint64_t above, uint64_t target, bool by_weight) {
+__device__ Border find_border(Team& team, const S& source, const Weights<T>& w, uint32_t lo, uint32_t hi, uint64_t above, uint64_t target, bool by_weight) {
     Shared& sh = team.sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t hi = w.kmax;
     Border at{};
     for (int round = 0; round < 5; ++round) {      // 32 bits of range, eight less after each
         const int bits = 32 - __clz(hi - lo), shift = bits > 8 ? bits - 8 : 0;
@@ -241,7 +244,8 @@ __device__ Border find_border(Team& team, const S& source, const Weights<T>& w, 
         if (kAll) {
             cg::cluster_group cluster = cg::this_cluster();
             cluster.sync();
-            for (uint32_t c = 0; c < team.ctas; ++c) v += cluster.map_shared_rank(hist, c)[tid];
+#pragma unroll
+            for (uint32_t c = 0; c < kMaxCtas; ++c) v += c < team.ctas ? cluster.map_shared_rank(hist, c)[tid] : 0;
         } else {
             __syncthreads();
             v = hist[tid];
@@ -373,7 +377,7 @@ __device__ void filter_and_draw(Team& team, const S& source, const Weights<T>& w
                                 float* prob) {
     Kept keep{0, 0, least};
     if (k != 0 && k < count) {
-        const Border at = find_border<kAll>(team, source, w, kmin, 0, k, false);
+        const Border at = find_border<kAll>(team, source, w, kmin, w.kmax, 0, k, false);
         keep.cut = at.key;
         keep.ties = k - at.above;
     }
@@ -398,7 +402,7 @@ __device__ void filter_and_draw(Team& team, const S& source, const Weights<T>& w
             t = t_all;
         }
         const uint64_t target = nucleus(p, s + (keep.cut ? min(t, keep.ties) * w.of_key(keep.cut) : 0));
-        const Border at = find_border<kAll>(team, source, w, keep.cut ? keep.cut : kmin, 0, target, true);
+        const Border at = find_border<kAll>(team, source, w, keep.cut ? keep.cut : kmin, w.kmax, 0, target, true);
         keep.ties = ties_to_reach(w, at, target, at.key == keep.cut ? keep.ties : ~0ull);
         keep.cut = at.key;
     }
@@ -547,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         }
     } else if (w.ordinary) {
         // The weight of the row, exactly, and of each bin, to a thousandth.  That says in which one or two bins the nucleus ends: what lies above
-        // them is kept for sure, what lies in them goes to the first CTA.  (Counts alone leave a 2 % wide strip, with thousands of tokens
+        // them is kept for sure, what lies in them is listed.  (Counts alone leave a 2 % wide strip, with thousands of tokens
         // of a flat row.)
         for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
         __syncthreads();
@@ -570,11 +574,20 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         const uint64_t target = nucleus(p, all_weight);
         constexpr int kEach = kBins / kThreads;      // a thread takes eight bins
         float sum = 0.0f, part[kEach];
+        uint32_t in_bin[kEach] = {};
+#pragma unroll
+        for (uint32_t c = 0; c < kMaxCtas; ++c)
+            if (c < team.ctas) {
+                const uint4* const q = reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.bins, c)) + tid * (kEach / 4);
+#pragma unroll
+                for (int j = 0; j < kEach / 4; ++j) {
+                    const uint4 v = q[j];
+                    in_bin[4 * j] += v.x; in_bin[4 * j + 1] += v.y; in_bin[4 * j + 2] += v.z; in_bin[4 * j + 3] += v.w;
+                }
+            }
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            uint32_t in_bin = 0;
-            for (uint32_t c = 0; c < team.ctas; ++c) in_bin += cluster.map_shared_rank(sh.bins, c)[tid * kEach + j];
-            part[j] = sum += (float)in_bin * (exp2f(-(float)(tid * kEach + j) / 32.0f) / 2048.0f);
+            part[j] = sum += (float)in_bin[j] * (exp2f(-(float)(tid * kEach + j) / 32.0f) / 2048.0f);
         }
         float run = sum;
 #pragma unroll
@@ -597,7 +610,6 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         }
         first = kBins - 1 - team.block_max(kBins - 1 - first);
         last = kBins - 1 - team.block_max(kBins - 1 - last);
-        cluster.sync();      // the bins have been read: the first CTA's take the candidates
         uint64_t sure = 0, kept = 0, count = 0, none = 0, own, unused;      // weight above the bins; of it, what min_p keeps; candidates
         for (uint32_t i = u0; i < u1; ++i) {
             float x[Slice::kPer];
@@ -633,31 +645,28 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             }
         const uint64_t own_sure = team.block_sum(sure);
         bool fits = true;
-        uint32_t offset = 0, listed = 0;
-        uint64_t all_sure = 0;
-        team.exchange(own_sure, own, [&](uint32_t c, uint64_t s, uint64_t n_c) {
-            if (c == team.cta) offset = listed;
-            listed += (uint32_t)min(n_c, (uint64_t)kLocal + 1);
+        uint64_t all_sure = 0, listed = 0;
+        team.exchange(own_sure, own, [&](uint32_t, uint64_t s, uint64_t n_c) {
             all_sure += s;
+            listed += n_c;
             fits = fits && n_c <= kLocal;
         });
-        if (fits && listed && listed <= kBins / 2) {
-            uint2* const list = reinterpret_cast<uint2*>(sh.bins);
-            uint2* const to = cluster.map_shared_rank(list, 0) + offset;
-            for (uint32_t i = tid; i < (uint32_t)own; i += kThreads) to[i] = sh.local[i];
-            cluster.sync();
-            Kept keep{0, 0, least};
-            if (team.cta == 0) {
-                uint32_t inverse = 0;
-                for (uint32_t i = tid; i < listed; i += kThreads) inverse = max(inverse, ~list[i].x);
-                inverse = team.block_max(inverse);
-                const Border at = find_border<false>(team, List<T>{list, listed}, w, ~inverse, all_sure, target, true);
-                keep.cut = at.key;
-                keep.ties = ties_to_reach(w, at, target, ~0ull);
+        if (fits && listed) {
+            const List<T> list{sh.local, (uint32_t)own};
+            uint32_t inverse = 0, most = 0;
+            for (uint32_t i = tid; i < (uint32_t)own; i += kThreads) {
+                inverse = max(inverse, ~list.entries[i].x);
+                most = max(most, list.entries[i].x);
             }
-            team.exchange(keep.cut, keep.ties, [&](uint32_t c, uint64_t x, uint64_t y) {
-                if (c == 0) { keep.cut = (uint32_t)x; keep.ties = y; }
+            inverse = team.block_max(inverse);
+            most = team.block_max(most);
+            uint32_t low = 0, high = 0;
+            team.exchange(inverse, most, [&](uint32_t, uint64_t x, uint64_t y) {
+                low = max(low, (uint32_t)x);
+                high = max(high, (uint32_t)y);
             });
+            const Border at = find_border<true>(team, list, w, ~low, high, all_sure, target, true);
+            const Kept keep{at.key, ties_to_reach(w, at, target, ~0ull), least};
             uint64_t same = 0;
             for (uint32_t i = place; any && i < end; ++i) {
                 const uint32_t key = sh.local[i].x;
