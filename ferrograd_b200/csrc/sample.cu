@@ -62,32 +62,39 @@ __device__ const double kRoots[64] = {
     1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062, 1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
     1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656, 1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
 
-// round(2^42 exp((x - m) / T)), by 2^t = 2^(n / 64) 2^r with |r| <= 1 / 128 and five terms of the series of 2^r (2^-54 of it).
+// round(2^42 exp(t)) with t = (x - m) / T: exp(t) = 2^(n / 64) exp(r) for the n that leaves |r| <= ln(2) / 128, and five terms of the series
+// of exp(r) (2^-54 of it; 1/6, 1/24 and 1/120 are cut to 20 bits, which moves it by 2^-46, so that they fit an instruction).
 template <typename T>
 struct Weights {
     const double* roots;
-    double m, c;              // the largest logit; log2(e) / T
-    float top, rate;          // the same in f32
+    double m, c;              // the largest logit; 1 / T
+    float top, rate;          // in f32, and log2(e) / T
     uint32_t kmax;
-    bool ordinary;            // finite in f32: bins and the test for small weights can be trusted
-    // 2^42 w, not rounded; 0 for weights that round to 0, -inf and NaN
-    __device__ __forceinline__ double scaled(float x) const {
-        if (x == top) return kOne;
-        const float d = (top - x) * rate;
-        if (ordinary ? !(d < 44.0f) : !(x > -INFINITY) || !(((double)x - m) * c > -44.0)) return 0.0;
-        const double t = ((double)x - m) * c;
+    bool ordinary;            // nothing overflows in f32: bins and the test for small weights can be trusted
+    // 2^42 w, not rounded, for a w of 2^-44 or more
+    __device__ __forceinline__ double series(float x) const {
         constexpr double kMagic = 6755399441055744.0;      // 1.5 * 2^52: a sum with it has its whole part in the low word
-        const double y = __fma_rn(t, 64.0, kMagic);
+        const double t = ((double)x - m) * c;
+        const double y = __fma_rn(t, __hiloint2double(0x40571547, 0), kMagic);      // 64 / ln(2)
         const int j = __double2loint(y);
-        const double r = __fma_rn(y - kMagic, -0.015625, t);
-        constexpr double l = 0.69314718055994530942, c2 = l * l / 2, c3 = l * l * l / 6, c4 = l * l * l * l / 24, c5 = l * l * l * l * l / 120;
-        double p = __fma_rn(r, c5, c4);
-        p = __fma_rn(r, p, c3);
-        p = __fma_rn(r, p, c2);
-        p = __fma_rn(r, p, l);
+        const double r = __fma_rn(y - kMagic, -0.69314718055994530942 / 64, t);
+        double p = __fma_rn(r, __hiloint2double(0x3f811111, 0), __hiloint2double(0x3fa55555, 0));
+        p = __fma_rn(r, p, __hiloint2double(0x3fc55555, 0));
+        p = __fma_rn(r, p, 0.5);
+        p = __fma_rn(r, p, 1.0);
         p = __fma_rn(r, p, 1.0);
         const double v = roots[j & 63] * p;
         return __hiloint2double(__double2hiint(v) + (((j >> 6) + 42) << 20), __double2loint(v));
+    }
+    // 0 for weights that round to 0, -inf and NaN.  (Of an ordinary row without a branch: the early ways out cost as much as the series.)
+    __device__ __forceinline__ double usual(float x) const {
+        const double v = series(x);
+        return (top - x) * rate < 44.0f ? v : 0.0;
+    }
+    __device__ __forceinline__ double scaled(float x) const {
+        if (ordinary) return usual(x);
+        if (x == top) return kOne;
+        return x > -INFINITY && ((double)x - m) * c > -30.0 ? series(x) : 0.0;      // 2^-43
     }
     static __device__ __forceinline__ uint64_t whole(double v) { return (uint64_t)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull; }
     __device__ __forceinline__ uint64_t operator()(float x) const { return whole(scaled(x)); }
@@ -347,12 +354,12 @@ template <bool kAll, typename S, typename T>
 __device__ void draw(Team& team, const S& source, const Weights<T>& w, const Kept& keep, float u, uint32_t* token, float* prob) {
     const uint32_t stretch = source.stretch(), u0 = min(source.units, threadIdx.x * stretch), u1 = min(source.units, u0 + stretch);
     uint64_t mass = 0, same = 0;
-    if (keep.cut == 0 && keep.least == 0.0) {      // all of it
+    if (keep.cut == 0 && keep.least == 0.0 && w.ordinary) {      // all of it
         for (uint32_t i = u0; i < u1; ++i) {
             float x[S::kPer];
             source.values(i, x);
 #pragma unroll
-            for (int e = 0; e < S::kPer; ++e) mass += w(x[e]);
+            for (int e = 0; e < S::kPer; ++e) mass += w.whole(w.usual(x[e]));
         }
     } else
         for (uint32_t i = u0; i < u1; ++i) {
@@ -480,8 +487,8 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         return;
     }
     const float top = logit_of<T>(kmax);
-    const double per_octave = 1.4426950408889634 / (double)temperature;
-    const Weights<T> w{sh.roots, (double)top, per_octave, top, (float)per_octave, kmax, top < INFINITY && per_octave < 1e30 && per_octave > 1e-30};
+    const double per_unit = 1.0 / (double)temperature;
+    const Weights<T> w{sh.roots, (double)top, per_unit, top, (float)(1.4426950408889634 * per_unit), kmax, top < INFINITY && per_unit < 1e30 && per_unit > 1e-30};
     const float u = a.u[r], p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
     const uint32_t k = a.top_k && a.top_k[r] < a.cols ? a.top_k[r] : 0;
     const double least = mp > 0.0f ? (double)min(mp, 1.0f) * kOne : 0.0;
@@ -513,17 +520,20 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         const uint32_t bound = min(worst, best);
         // What is not below it goes to the first CTA, in order: count, then places.
         auto candidate = [&](float x) { return x > -INFINITY && w.bin(x) <= bound; };
-        uint64_t count = 0, none = 0, own, unused;
+        uint64_t count = 0, none = 0, own, unused, where = 0;      // where: the units with candidates (of a longer stretch, by their number modulo 64)
         for (uint32_t i = u0; i < u1; ++i) {
             float x[Slice::kPer];
+            uint32_t found = 0;
             slice.values(i, x);
 #pragma unroll
-            for (int e = 0; e < Slice::kPer; ++e) count += candidate(x[e]);
+            for (int e = 0; e < Slice::kPer; ++e) found += candidate(x[e]);
+            count += found;
+            where |= (uint64_t)(found != 0) << ((i - u0) & 63);
         }
-        const bool any = count != 0;
         team.prefix(count, none, own, unused);
-        if (any && own <= kLocal)
+        if (where && own <= kLocal)
             for (uint32_t i = u0; i < u1; ++i) {
+                if (!(where >> ((i - u0) & 63) & 1)) continue;
                 float x[Slice::kPer];
                 slice.values(i, x);
 #pragma unroll
@@ -561,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             slice.values(i, x);
 #pragma unroll
             for (int e = 0; e < Slice::kPer; ++e) {
-                weight += w(x[e]);
+                weight += w.whole(w.usual(x[e]));
                 const float d = (top - x[e]) * (w.rate * 32.0f);
                 if (d < (float)(kBins - 1)) {
                     const uint32_t b = (uint32_t)d;
@@ -610,37 +620,40 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         }
         first = kBins - 1 - team.block_max(kBins - 1 - first);
         last = kBins - 1 - team.block_max(kBins - 1 - last);
-        uint64_t sure = 0, kept = 0, count = 0, none = 0, own, unused;      // weight above the bins; of it, what min_p keeps; candidates
+        uint64_t sure = 0, kept = 0, count = 0, none = 0, own, unused, where = 0;      // weight above the bins; of it, what min_p keeps; candidates, and their units
         for (uint32_t i = u0; i < u1; ++i) {
             float x[Slice::kPer];
             slice.values(i, x);
             unsigned above = 0;
+            uint32_t found = 0;
 #pragma unroll
             for (int e = 0; e < Slice::kPer; ++e) {
                 const uint32_t b = w.bin(x[e]);
                 above |= (unsigned)(b < first) << e;
-                count += b >= first && b <= last && x[e] > -INFINITY;
+                found += b - first <= last - first && x[e] > -INFINITY;
             }
+            count += found;
+            where |= (uint64_t)(found != 0) << ((i - u0) & 63);
             for (; above; above &= above - 1) {      // few: one at a time
-                const double v = w.scaled(slice.value(i * Slice::kPer + __ffs(above) - 1));
+                const double v = w.usual(slice.value(i * Slice::kPer + __ffs(above) - 1));
                 const uint64_t q = w.whole(v);
                 sure += q;
                 if (v >= least) kept += q;
             }
         }
         uint32_t place = (uint32_t)count, end;
-        const bool any = count != 0;
         team.prefix(count, none, own, unused);
         end = (uint32_t)count + place;
         place = (uint32_t)count;
-        if (any && own <= kLocal)
+        if (where && own <= kLocal)
             for (uint32_t i = u0, at = place; i < u1; ++i) {
+                if (!(where >> ((i - u0) & 63) & 1)) continue;
                 float x[Slice::kPer];
                 slice.values(i, x);
 #pragma unroll
                 for (int e = 0; e < Slice::kPer; ++e) {
                     const uint32_t b = w.bin(x[e]);
-                    if (b >= first && b <= last && x[e] > -INFINITY) sh.local[at++] = make_uint2(key_of<T>(x[e]), slice.column_of(i * Slice::kPer + e));
+                    if (b - first <= last - first && x[e] > -INFINITY) sh.local[at++] = make_uint2(key_of<T>(x[e]), slice.column_of(i * Slice::kPer + e));
                 }
             }
         const uint64_t own_sure = team.block_sum(sure);
@@ -668,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             const Border at = find_border<true>(team, list, w, ~low, high, all_sure, target, true);
             const Kept keep{at.key, ties_to_reach(w, at, target, ~0ull), least};
             uint64_t same = 0;
-            for (uint32_t i = place; any && i < end; ++i) {
+            for (uint32_t i = place; i < end; ++i) {
                 const uint32_t key = sh.local[i].x;
                 same += key == keep.cut;
                 if (key > keep.cut) {
