@@ -22,7 +22,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxCtas = 8;
-constexpr int kBins = 2048;                   // of a 32nd of an octave of weight
+constexpr int kBins = 2048;                   // of a 64th of an octave of weight
 constexpr uint32_t kLocal = 1024, kGathered = 4096;      // candidates of a CTA, of a row
 constexpr unsigned kFull = 0xffffffffu;
 constexpr double kOne = 4398046511104.0;      // 2^42
@@ -71,14 +71,14 @@ struct Weights {
     float top, rate;          // in f32, and log2(e) / T
     uint32_t kmax;
     bool ordinary;            // nothing overflows in f32: bins and the test for small weights can be trusted
-    // 2^42 w, not rounded, for a w of 2^-44 or more
-    __device__ __forceinline__ double series(float x) const {
+    // 2^42 w, not rounded, for a w of 2^-44 or more; and the 64th of an octave that it lies in, w being p times the middle of it
+    __device__ __forceinline__ double series(float x, int& j, double& p) const {
         constexpr double kMagic = 6755399441055744.0;      // 1.5 * 2^52: a sum with it has its whole part in the low word
         const double t = ((double)x - m) * c;
         const double y = __fma_rn(t, __hiloint2double(0x40571547, 0), kMagic);      // 64 / ln(2)
-        const int j = __double2loint(y);
+        j = __double2loint(y);
         const double r = __fma_rn(y - kMagic, -0.69314718055994530942 / 64, t);
-        double p = __fma_rn(r, __hiloint2double(0x3f811111, 0), __hiloint2double(0x3fa55555, 0));
+        p = __fma_rn(r, __hiloint2double(0x3f811111, 0), __hiloint2double(0x3fa55555, 0));
         p = __fma_rn(r, p, __hiloint2double(0x3fc55555, 0));
         p = __fma_rn(r, p, 0.5);
         p = __fma_rn(r, p, 1.0);
@@ -88,22 +88,23 @@ struct Weights {
     }
     // 0 for weights that round to 0, -inf and NaN.  (Of an ordinary row without a branch: the early ways out cost as much as the series.)
     __device__ __forceinline__ double usual(float x) const {
-        const double v = series(x);
+        int j;
+        double p;
+        const double v = series(x, j, p);
         return (top - x) * rate < 44.0f ? v : 0.0;
     }
     __device__ __forceinline__ double scaled(float x) const {
         if (ordinary) return usual(x);
         if (x == top) return kOne;
-        return x > -INFINITY && ((double)x - m) * c > -30.0 ? series(x) : 0.0;      // 2^-43
+        int j;
+        double p;
+        return x > -INFINITY && ((double)x - m) * c > -30.0 ? series(x, j, p) : 0.0;      // 2^-43
     }
     static __device__ __forceinline__ uint64_t whole(double v) { return (uint64_t)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull; }
     __device__ __forceinline__ uint64_t operator()(float x) const { return whole(scaled(x)); }
     __device__ __forceinline__ uint64_t of_key(uint32_t key) const { return whole(scaled(logit_of<T>(key))); }
-    // Bins of a 32nd of an octave below the largest; the last one has all that is far below, and what is never drawn.  Grows as x falls.
-    __device__ __forceinline__ uint32_t bin(float x) const {
-        const float d = (top - x) * (rate * 32.0f);
-        return d < (float)(kBins - 1) ? (uint32_t)d : (uint32_t)kBins - 1;
-    }
+    // How far x lies below the largest, in 64ths of an octave of weight; NaN or infinite for what is never drawn.  Grows as x falls.
+    __device__ __forceinline__ float below(float x) const { return (top - x) * (rate * 64.0f); }
 };
 
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
@@ -500,9 +501,10 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
 
     if (w.ordinary && k) {
         // k threads with a value of a bin or above it say that the k-th largest is not below it; so do k / ctas threads in each CTA.
-        const uint32_t own_bin = key_of<T>(mine) ? w.bin(mine) : kBins;
+        const float own_below = w.below(mine);
+        const uint32_t own_bin = own_below < (float)kBins ? (uint32_t)own_below : kBins;
         auto reached = [&](uint32_t want) {
-            uint32_t b = kBins - 1;
+            uint32_t b = kBins;      // not by any bin
             if (want <= kThreads)
                 for (uint32_t lo = 0, hi = kBins - 1; lo <= hi;) {      // 11 steps
                     const uint32_t mid = (lo + hi) / 2;
@@ -515,11 +517,12 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             return b;
         };
         const uint32_t share = reached((k + team.ctas - 1) / team.ctas), whole = team.ctas > 1 ? reached(k) : share;
-        uint32_t worst = 0, best = kBins - 1;
+        uint32_t worst = 0, best = kBins;
         team.exchange(share, whole, [&](uint32_t, uint64_t x, uint64_t y) { worst = max(worst, (uint32_t)x); best = min(best, (uint32_t)y); });
         const uint32_t bound = min(worst, best);
+        const float limit = bound < (uint32_t)kBins ? (float)(bound + 1) : INFINITY;
         // What is not below it goes to the first CTA, in order: count, then places.
-        auto candidate = [&](float x) { return x > -INFINITY && w.bin(x) <= bound; };
+        auto candidate = [&](float x) { return w.below(x) < limit; };
         uint64_t count = 0, none = 0, own, unused, where = 0;      // where: the units with candidates (of a longer stretch, by their number modulo 64)
         for (uint32_t i = u0; i < u1; ++i) {
             float x[Slice::kPer];
@@ -571,12 +574,13 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             slice.values(i, x);
 #pragma unroll
             for (int e = 0; e < Slice::kPer; ++e) {
-                weight += w.whole(w.usual(x[e]));
-                const float d = (top - x[e]) * (w.rate * 32.0f);
-                if (d < (float)(kBins - 1)) {
-                    const uint32_t b = (uint32_t)d;
-                    atomicAdd(&sh.bins[b], 2048u - (uint32_t)((d - (float)b) * 43.87f));      // 2^11 of its weight over the bin's upper end: 2^(-1/32) at the lower
-                }
+                int j;
+                double relative;
+                const double v = w.series(x[e], j, relative);
+                const float d = w.below(x[e]);
+                weight += w.whole(d < 44.0f * 64.0f ? v : 0.0);
+                // 2^13 of its weight over the middle of its bin
+                if (d < (float)(kBins - 1)) atomicAdd(&sh.bins[-j], (uint32_t)__double2loint(relative + 824633720832.0));      // 1.5 * 2^39: the whole part in the low word
             }
         }
         weight = team.block_sum(weight);
@@ -597,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             }
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            part[j] = sum += (float)in_bin[j] * (exp2f(-(float)(tid * kEach + j) / 32.0f) / 2048.0f);
+            part[j] = sum += (float)in_bin[j] * (exp2f(-(float)(tid * kEach + j) / 64.0f) / 8192.0f);
         }
         float run = sum;
 #pragma unroll
@@ -610,16 +614,18 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         __syncthreads();
         float before = run - sum;
         for (int j = 0; j < warp; ++j) before += sums[j];
-        // a weight in a bin is off by 2^-11 at most (its rounding, and the chord for the exponential: 6e-5), its bin's place and the f32 sums by 1e-5
+        // a weight in a bin is off by 2^-14 of it at most, the f32 sums by some 1e-6
         const float goal = (float)((double)target / kOne);
         uint32_t first = kBins - 1, last = kBins - 1;
 #pragma unroll
         for (int j = kEach - 1; j >= 0; --j) {
-            if (before + part[j] >= goal * 0.999f) first = tid * kEach + j;
-            if (before + part[j] >= goal * 1.001f) last = tid * kEach + j;
+            if (before + part[j] >= goal * 0.9999f) first = tid * kEach + j;
+            if (before + part[j] >= goal * 1.0001f) last = tid * kEach + j;
         }
         first = kBins - 1 - team.block_max(kBins - 1 - first);
         last = kBins - 1 - team.block_max(kBins - 1 - last);
+        // Bin b reaches from b - 1/2 to b + 1/2.  What the f32 distance is off by (3e-4) decides between sure and listed at most.
+        const float sure_end = (float)first - 0.51f, list_end = last < (uint32_t)kBins - 1 ? (float)last + 0.51f : INFINITY;
         uint64_t sure = 0, kept = 0, count = 0, none = 0, own, unused, where = 0;      // weight above the bins; of it, what min_p keeps; candidates, and their units
         for (uint32_t i = u0; i < u1; ++i) {
             float x[Slice::kPer];
@@ -628,9 +634,9 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             uint32_t found = 0;
 #pragma unroll
             for (int e = 0; e < Slice::kPer; ++e) {
-                const uint32_t b = w.bin(x[e]);
-                above |= (unsigned)(b < first) << e;
-                found += b - first <= last - first && x[e] > -INFINITY;
+                const float d = w.below(x[e]);
+                if (d < sure_end) above |= 1u << e;
+                else if (d < list_end) ++found;
             }
             count += found;
             where |= (uint64_t)(found != 0) << ((i - u0) & 63);
@@ -652,8 +658,8 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
                 slice.values(i, x);
 #pragma unroll
                 for (int e = 0; e < Slice::kPer; ++e) {
-                    const uint32_t b = w.bin(x[e]);
-                    if (b - first <= last - first && x[e] > -INFINITY) sh.local[at++] = make_uint2(key_of<T>(x[e]), slice.column_of(i * Slice::kPer + e));
+                    const float d = w.below(x[e]);
+                    if (!(d < sure_end) && d < list_end) sh.local[at++] = make_uint2(key_of<T>(x[e]), slice.column_of(i * Slice::kPer + e));
                 }
             }
         const uint64_t own_sure = team.block_sum(sure);
@@ -666,19 +672,10 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         });
         if (fits && listed) {
             const List<T> list{sh.local, (uint32_t)own};
-            uint32_t inverse = 0, most = 0;
-            for (uint32_t i = tid; i < (uint32_t)own; i += kThreads) {
-                inverse = max(inverse, ~list.entries[i].x);
-                most = max(most, list.entries[i].x);
-            }
-            inverse = team.block_max(inverse);
-            most = team.block_max(most);
-            uint32_t low = 0, high = 0;
-            team.exchange(inverse, most, [&](uint32_t, uint64_t x, uint64_t y) {
-                low = max(low, (uint32_t)x);
-                high = max(high, (uint32_t)y);
-            });
-            const Border at = find_border<true>(team, list, w, ~low, high, all_sure, target, true);
+            // its keys lie between those half a bin further out
+            const float per_bin = 1.0f / (w.rate * 64.0f), lowest = top - (list_end + 0.5f) * per_bin, highest = top - fmaxf(sure_end - 0.5f, 0.0f) * per_bin;
+            const uint32_t low = max(1u, key_of<T>(lowest)), high = min(kmax, key_of<T>(highest));
+            const Border at = find_border<true>(team, list, w, low, high, all_sure, target, true);
             const Kept keep{at.key, ties_to_reach(w, at, target, ~0ull), least};
             uint64_t same = 0;
             for (uint32_t i = place; i < end; ++i) {
