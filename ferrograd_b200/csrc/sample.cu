@@ -22,7 +22,8 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxCtas = 8;
-constexpr int kBins = 2048;                   // of a 64th of an octave of weight
+constexpr int kSteps = 2048;                  // 64ths of an octave of weight that a bound is looked for in
+constexpr int kBins = 512;                    // 16ths of an octave that a row's weight is added up in
 constexpr uint32_t kLocal = 1024, kGathered = 4096;      // candidates of a CTA, of a row
 constexpr unsigned kFull = 0xffffffffu;
 constexpr double kOne = 4398046511104.0;      // 2^42
@@ -71,14 +72,14 @@ struct Weights {
     float top, rate;          // in f32, and log2(e) / T
     uint32_t kmax;
     bool ordinary;            // nothing overflows in f32: bins and the test for small weights can be trusted
-    // 2^42 w, not rounded, for a w of 2^-44 or more; and the 64th of an octave that it lies in, w being p times the middle of it
-    __device__ __forceinline__ double series(float x, int& j, double& p) const {
+    // 2^42 w, not rounded, for a w of 2^-44 or more
+    __device__ __forceinline__ double series(float x) const {
         constexpr double kMagic = 6755399441055744.0;      // 1.5 * 2^52: a sum with it has its whole part in the low word
         const double t = ((double)x - m) * c;
         const double y = __fma_rn(t, __hiloint2double(0x40571547, 0), kMagic);      // 64 / ln(2)
-        j = __double2loint(y);
+        const int j = __double2loint(y);
         const double r = __fma_rn(y - kMagic, -0.69314718055994530942 / 64, t);
-        p = __fma_rn(r, __hiloint2double(0x3f811111, 0), __hiloint2double(0x3fa55555, 0));
+        double p = __fma_rn(r, __hiloint2double(0x3f811111, 0), __hiloint2double(0x3fa55555, 0));
         p = __fma_rn(r, p, __hiloint2double(0x3fc55555, 0));
         p = __fma_rn(r, p, 0.5);
         p = __fma_rn(r, p, 1.0);
@@ -88,17 +89,13 @@ struct Weights {
     }
     // 0 for weights that round to 0, -inf and NaN.  (Of an ordinary row without a branch: the early ways out cost as much as the series.)
     __device__ __forceinline__ double usual(float x) const {
-        int j;
-        double p;
-        const double v = series(x, j, p);
+        const double v = series(x);
         return (top - x) * rate < 44.0f ? v : 0.0;
     }
     __device__ __forceinline__ double scaled(float x) const {
         if (ordinary) return usual(x);
         if (x == top) return kOne;
-        int j;
-        double p;
-        return x > -INFINITY && ((double)x - m) * c > -30.0 ? series(x, j, p) : 0.0;      // 2^-43
+        return x > -INFINITY && ((double)x - m) * c > -30.0 ? series(x) : 0.0;      // 2^-43
     }
     static __device__ __forceinline__ uint64_t whole(double v) { return (uint64_t)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull; }
     __device__ __forceinline__ uint64_t operator()(float x) const { return whole(scaled(x)); }
@@ -502,11 +499,11 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
     if (w.ordinary && k) {
         // k threads with a value of a bin or above it say that the k-th largest is not below it; so do k / ctas threads in each CTA.
         const float own_below = w.below(mine);
-        const uint32_t own_bin = own_below < (float)kBins ? (uint32_t)own_below : kBins;
+        const uint32_t own_bin = own_below < (float)kSteps ? (uint32_t)own_below : kSteps;
         auto reached = [&](uint32_t want) {
-            uint32_t b = kBins;      // not by any bin
+            uint32_t b = kSteps;      // not by any bin
             if (want <= kThreads)
-                for (uint32_t lo = 0, hi = kBins - 1; lo <= hi;) {      // 11 steps
+                for (uint32_t lo = 0, hi = kSteps - 1; lo <= hi;) {      // 11 steps
                     const uint32_t mid = (lo + hi) / 2;
                     if ((uint32_t)__syncthreads_count(own_bin <= mid) >= want) {
                         b = mid;
@@ -517,13 +514,13 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             return b;
         };
         const uint32_t share = reached((k + team.ctas - 1) / team.ctas), whole = team.ctas > 1 ? reached(k) : share;
-        uint32_t worst = 0, best = kBins;
+        uint32_t worst = 0, best = kSteps;
         team.exchange(share, whole, [&](uint32_t, uint64_t x, uint64_t y) { worst = max(worst, (uint32_t)x); best = min(best, (uint32_t)y); });
         const uint32_t bound = min(worst, best);
-        const float limit = bound < (uint32_t)kBins ? (float)(bound + 1) : INFINITY;
+        const float limit = bound < (uint32_t)kSteps ? (float)(bound + 1) : INFINITY;
         // What is not below it goes to the first CTA, in order: count, then places.
         auto candidate = [&](float x) { return w.below(x) < limit; };
-        uint64_t count = 0, none = 0, own, unused, where = 0;      // where: the units with candidates (of a longer stretch, by their number modulo 64)
+        uint64_t count = 0, none = 0, own, unused, where = 0;      // where: the units with candidates, of a stretch of up to 64
         for (uint32_t i = u0; i < u1; ++i) {
             float x[Slice::kPer];
             uint32_t found = 0;
@@ -536,7 +533,11 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         team.prefix(count, none, own, unused);
         if (where && own <= kLocal)
             for (uint32_t i = u0; i < u1; ++i) {
-                if (!(where >> ((i - u0) & 63) & 1)) continue;
+                if (stretch <= 64) {
+                    const uint64_t more = where >> (i - u0);
+                    if (!more) break;
+                    i += __ffsll(more) - 1;
+                }
                 float x[Slice::kPer];
                 slice.values(i, x);
 #pragma unroll
@@ -563,46 +564,50 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             return;
         }
     } else if (w.ordinary) {
-        // The weight of the row, exactly, and of each bin, to a thousandth.  That says in which one or two bins the nucleus ends: what lies above
-        // them is kept for sure, what lies in them is listed.  (Counts alone leave a 2 % wide strip, with thousands of tokens
-        // of a flat row.)
+        // The weight of the row, exactly; then that of each bin, to 6e-5.  That says in which one or two bins the nucleus ends: what lies above them is
+        // kept for sure, what lies in them is listed.
         for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
-        __syncthreads();
         uint64_t weight = 0, all_weight = 0;
         for (uint32_t i = tid; i < slice.units; i += kThreads) {
             float x[Slice::kPer];
             slice.values(i, x);
 #pragma unroll
-            for (int e = 0; e < Slice::kPer; ++e) {
-                int j;
-                double relative;
-                const double v = w.series(x[e], j, relative);
-                const float d = w.below(x[e]);
-                weight += w.whole(d < 44.0f * 64.0f ? v : 0.0);
-                // 2^13 of its weight over the middle of its bin
-                if (d < (float)(kBins - 1)) atomicAdd(&sh.bins[-j], (uint32_t)__double2loint(relative + 824633720832.0));      // 1.5 * 2^39: the whole part in the low word
-            }
+            for (int e = 0; e < Slice::kPer; ++e) weight += w.whole(w.usual(x[e]));
         }
         weight = team.block_sum(weight);
         team.exchange(weight, 0, [&](uint32_t, uint64_t part, uint64_t) { all_weight += part; });
         const uint64_t target = nucleus(p, all_weight);
-        constexpr int kEach = kBins / kThreads;      // a thread takes eight bins
+        // All tokens of a weight below (1 - p) / cols of the row's together do not reach the 1 - p of it that may be left out: the nucleus ends above them.
+        // An SM adds to shared memory one lane at a time, so binning them too took as long as everything else.
+        const double rest = ((double)all_weight - (double)target) / kOne / a.cols;
+        const float far = rest > 1e-9 ? fminf(kBins - 1.0f, 16.0f * -log2f((float)rest) + 1.0f) : kBins - 1.0f;
+        for (uint32_t i = tid; i < slice.units; i += kThreads) {
+            float x[Slice::kPer];
+            slice.values(i, x);
+#pragma unroll
+            for (int e = 0; e < Slice::kPer; ++e) {
+                const float d = w.below(x[e]) * 0.25f;
+                if (d < far) {      // 2^13 of its weight over the middle of its bin: 2^(r / 16) for |r| <= 1/2, by two terms (off by 2e-6)
+                    constexpr float l = 0.693147181f / 16.0f, kRound = 12582912.0f;      // 1.5 * 2^23: a sum with it has its whole part in the low bits
+                    const float y = d + kRound, r = (y - kRound) - d;
+                    const uint32_t b = __float_as_uint(y) & 0xfffu;
+                    atomicAdd(&sh.bins[b], __float_as_uint(__fmaf_rn(r, __fmaf_rn(r, 4096.0f * l * l, 8192.0f * l), 8192.0f + 8388608.0f)) - 0x4b000000u);
+                }
+            }
+        }
+        cluster.sync();
+        constexpr int kEach = kBins / kThreads;      // a thread takes two bins
         float sum = 0.0f, part[kEach];
         uint32_t in_bin[kEach] = {};
 #pragma unroll
         for (uint32_t c = 0; c < kMaxCtas; ++c)
             if (c < team.ctas) {
-                const uint4* const q = reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.bins, c)) + tid * (kEach / 4);
-#pragma unroll
-                for (int j = 0; j < kEach / 4; ++j) {
-                    const uint4 v = q[j];
-                    in_bin[4 * j] += v.x; in_bin[4 * j + 1] += v.y; in_bin[4 * j + 2] += v.z; in_bin[4 * j + 3] += v.w;
-                }
+                const uint2 v = reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.bins, c))[tid];
+                in_bin[0] += v.x;
+                in_bin[1] += v.y;
             }
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            part[j] = sum += (float)in_bin[j] * (exp2f(-(float)(tid * kEach + j) / 64.0f) / 8192.0f);
-        }
+        for (int j = 0; j < kEach; ++j) part[j] = sum += (float)in_bin[j] * (exp2f(-(float)(tid * kEach + j) / 16.0f) / 8192.0f);
         float run = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -614,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         __syncthreads();
         float before = run - sum;
         for (int j = 0; j < warp; ++j) before += sums[j];
-        // a weight in a bin is off by 2^-14 of it at most, the f32 sums by some 1e-6
+        // a weight in a bin is off by 6e-5 of it at most, the f32 sums by some 1e-6
         const float goal = (float)((double)target / kOne);
         uint32_t first = kBins - 1, last = kBins - 1;
 #pragma unroll
@@ -624,8 +629,8 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         }
         first = kBins - 1 - team.block_max(kBins - 1 - first);
         last = kBins - 1 - team.block_max(kBins - 1 - last);
-        // Bin b reaches from b - 1/2 to b + 1/2.  What the f32 distance is off by (3e-4) decides between sure and listed at most.
-        const float sure_end = (float)first - 0.51f, list_end = last < (uint32_t)kBins - 1 ? (float)last + 0.51f : INFINITY;
+        // Bin b reaches from b - 1/2 to b + 1/2, in 64ths four times that.  What the f32 distance is off by decides between sure and listed at most.
+        const float sure_end = 4.0f * (float)first - 2.01f, list_end = last < (uint32_t)kBins - 1 ? 4.0f * (float)last + 2.01f : INFINITY;
         uint64_t sure = 0, kept = 0, count = 0, none = 0, own, unused, where = 0;      // weight above the bins; of it, what min_p keeps; candidates, and their units
         for (uint32_t i = u0; i < u1; ++i) {
             float x[Slice::kPer];
@@ -653,7 +658,11 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         place = (uint32_t)count;
         if (where && own <= kLocal)
             for (uint32_t i = u0, at = place; i < u1; ++i) {
-                if (!(where >> ((i - u0) & 63) & 1)) continue;
+                if (stretch <= 64) {
+                    const uint64_t more = where >> (i - u0);
+                    if (!more) break;
+                    i += __ffsll(more) - 1;
+                }
                 float x[Slice::kPer];
                 slice.values(i, x);
 #pragma unroll
