@@ -94,7 +94,7 @@ template <typename T>
 struct Weights {
     const double* roots;
     double m, c, mc;          // the largest logit; 1 / T; their product
-    float top, rate;          // in f32, and log2(e) / T
+    float top, rate, bottom;  // in f32, and log2(e) / T; 44 octaves below the largest: nothing that counts is lower
     uint32_t kmax;
     bool ordinary;            // nothing overflows in f32, and mc is good to 2^-33: the short cuts hold
     // 2^42 w, not rounded, for a w of 2^-44 or more
@@ -107,14 +107,14 @@ struct Weights {
         double p = __fma_rn(r, __hiloint2double(0x3fc55555, 0), 0.5);
         p = __fma_rn(r, p, 1.0);
         p = __fma_rn(r, p, 1.0);
-        const double v = roots[j & 255] * p;
-        return __hiloint2double(__double2hiint(v) + (((j >> 8) + 42) << 20), __double2loint(v));
+        const double root = roots[j & 255];      // 2^42 times it, less what j's low bits add to the exponent here
+        return __hiloint2double(__double2hiint(root) + (j << 12), __double2loint(root)) * p;
     }
-    // 0 for weights that round to 0, -inf and NaN.  (Of an ordinary row without a branch: the early ways out cost as much as the series.)
-    __device__ __forceinline__ double usual(float x) const {
-        const double v = series(x);
-        return (top - x) * rate < 44.0f ? v : 0.0;
-    }
+    // The same for any x of an ordinary row, without a branch: what lies below `bottom`, -inf and NaN are taken for it, a quarter of 2^-42.
+    __device__ __forceinline__ double usual(float x) const { return series(fmaxf(x, bottom)); }
+    // Its rounded value as the low bits of a sum with 2^52; kBias too much.
+    static constexpr uint64_t kBias = 0x4330000000000000ull;
+    __device__ __forceinline__ uint64_t biased(float x) const { return (uint64_t)__double_as_longlong(usual(x) + 4503599627370496.0); }
     __device__ __forceinline__ double scaled(float x) const {
         if (ordinary) return usual(x);
         if (x == top) return kOne;
@@ -381,8 +381,9 @@ __device__ void draw(Team& team, const S& source, const Weights<T>& w, const Kep
             float x[S::kPer];
             source.values(i, x);
 #pragma unroll
-            for (int e = 0; e < S::kPer; ++e) mass += w.whole(w.usual(x[e]));
+            for (int e = 0; e < S::kPer; ++e) mass += w.biased(x[e]);
         }
+        mass -= (u1 - u0) * (uint64_t)S::kPer * w.kBias;
     } else
         for (uint32_t i = u0; i < u1; ++i) {
             float x[S::kPer];
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
     const uint32_t c0 = min(a.cols, team.cta * a.slice), n = min(a.cols - c0, a.slice);
     const T* const data = static_cast<const T*>(a.logits) + (uint64_t)r * a.cols + c0;
     Slice slice;
-    sh.roots[tid] = kRoots[tid];
+    sh.roots[tid] = __hiloint2double(__double2hiint(kRoots[tid]) + (42 << 20) - (tid << 12), __double2loint(kRoots[tid]));
     if constexpr (kHeld) {
         const uint32_t o = (uint32_t)(reinterpret_cast<uintptr_t>(data) & 15u) / sizeof(T), words = n ? (o + n + E - 1) / E : 0;
         const uint32_t base = (uint32_t)__cvta_generic_to_shared(dynamic);
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
     }
     const float top = logit_of<T>(kmax);
     const double per_unit = 1.0 / (double)temperature;
-    const Weights<T> w{sh.roots, (double)top, per_unit, (double)top * per_unit, top, (float)(1.4426950408889634 * per_unit), kmax,
+    const Weights<T> w{sh.roots, (double)top, per_unit, (double)top * per_unit, top, (float)(1.4426950408889634 * per_unit), (float)((double)top - 30.5 / per_unit), kmax,
                        fabs((double)top * per_unit) < 1e6 && per_unit < 1e30 && per_unit > 1e-30};
     const float u = a.u[r], p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
     const uint32_t k = a.top_k && a.top_k[r] < a.cols ? a.top_k[r] : 0;
@@ -597,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             float x[Slice::kPer];
             slice.values(i, x);
 #pragma unroll
-            for (int e = 0; e < Slice::kPer; ++e) weight += w.whole(w.usual(x[e]));
+            for (int e = 0; e < Slice::kPer; ++e) weight += w.biased(x[e]) - w.kBias;
         }
         weight = team.block_sum(weight);
         team.exchange(weight, 0, [&](uint32_t, uint64_t part, uint64_t) { all_weight += part; });
