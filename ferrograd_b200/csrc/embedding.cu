@@ -16,6 +16,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
+constexpr int kPacks = 4;      // of the lookup
 
 struct EmbedArgs {
     uint32_t tokens, vocab, dim;
@@ -482,58 +483,49 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const SumArgs s) {
 }
 
 // ---- lookup ----
-// A warp takes a token and a tile of columns, four packs per lane.  Rows off 16-byte boundaries: a lane owns words of the output as they lie in
-// memory, turns what it reads, and the ends of a row go element by element.
-template <typename T, bool kShift>
-__global__ void __launch_bounds__(256) embed_kernel(uint32_t tokens, uint32_t vocab, uint32_t dim, uint32_t tiles, const uint32_t* ids, const T* table, const T* table_end,
-                                                    float scale, T* out) {
-    constexpr int E = FgPack<T>::E, kPacks = 4;
+// A warp takes a token and a tile of columns, `kPacks` packs of 16 bytes per lane or, off 16-byte boundaries, as many single elements side by side
+// (words turned by a row's distance from the boundary took more instructions than the elements do).
+template <typename T, bool kStraight>
+__global__ void __launch_bounds__(256) embed_kernel(uint32_t tokens, uint32_t vocab, uint32_t dim, uint32_t tiles, const uint32_t* ids, const T* table, float scale, T* out) {
+    using Unit = std::conditional_t<kStraight, uint4, T>;
+    constexpr int E = sizeof(Unit) / sizeof(T), kUnits = kStraight ? kPacks : kPacks * 4;
     fg_grid_enter();
     const int lane = threadIdx.x & 31;
-    const uint64_t units = (uint64_t)tokens * tiles;
-    for (uint64_t unit = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); unit < units; unit += (uint64_t)gridDim.x * 8) {
-        const uint32_t t = (uint32_t)(unit / tiles), tile = (uint32_t)(unit % tiles), id = ids[t];
+    const uint32_t units = dim / E;      // of a row
+    const uint64_t work = (uint64_t)tokens * tiles;
+    for (uint64_t k = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); k < work; k += (uint64_t)gridDim.x * 8) {
+        const uint32_t t = (uint32_t)(k / tiles), first = (uint32_t)(k % tiles) * (32 * kUnits) + lane, id = ids[t];
         const bool inside = id < vocab;
-        const T* const row = table + (uint64_t)id * dim;
-        T* const to = out + (uint64_t)t * dim;
-        uint32_t head = 0;
-        if constexpr (kShift) {
-            head = min(dim, (uint32_t)(-reinterpret_cast<uintptr_t>(to) & 15u) / (uint32_t)sizeof(T));
-            const uint32_t tail = (dim - head) % E;
-            if (tile == 0 && lane < 2 * E) {      // before the first word, behind the last
-                const uint32_t c = lane < E ? lane : dim - tail + (lane - E);
-                if (lane < E ? lane < head : lane - E < tail) to[c] = fg_narrow<T>(inside ? fg_widen(row[c]) * scale : 0.0f);
-            }
-        }
-        const uint32_t words = (dim - head) / E;
-        uint4 v[kPacks];
+        const Unit* const from = reinterpret_cast<const Unit*>(table + (uint64_t)id * dim);
+        Unit* const to = reinterpret_cast<Unit*>(out + (uint64_t)t * dim);
+        Unit v[kUnits];
 #pragma unroll
-        for (int k = 0; k < kPacks; ++k) {
-            const uint32_t i = (tile * kPacks + k) * 32 + lane;
-            v[k] = make_uint4(0, 0, 0, 0);
-            if (inside && i < words) v[k] = fg_load_pack<T, kShift>(row + head + (uint64_t)i * E, E, table, table_end);
+        for (int j = 0; j < kUnits; ++j) {
+            v[j] = Unit{};
+            if (inside && first + 32 * j < units) v[j] = from[first + 32 * j];
         }
 #pragma unroll
-        for (int k = 0; k < kPacks; ++k) {
-            const uint32_t i = (tile * kPacks + k) * 32 + lane;
-            float x[E];
-            FgPack<T>::widen(v[k], x);
+        for (int j = 0; j < kUnits; ++j) {
+            if constexpr (kStraight) {
+                float x[E];
+                FgPack<T>::widen(v[j], x);
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = inside ? x[e] * scale : 0.0f;
-            if (i < words) *reinterpret_cast<uint4*>(to + head + (uint64_t)i * E) = FgPack<T>::narrow(x);
+                for (int e = 0; e < E; ++e) x[e] *= scale;
+                v[j] = FgPack<T>::narrow(x);
+            } else v[j] = fg_narrow<T>(fg_widen(v[j]) * scale);
+            if (!inside) v[j] = Unit{};
+            if (first + 32 * j < units) to[first + 32 * j] = v[j];
         }
     }
 }
 
 template <typename T>
 int32_t embed_fwd(fg_ctx* ctx, const EmbedArgs& a) {
-    const uint32_t tiles = (a.dim + 32 * 4 * FgPack<T>::E - 1) / (32 * 4 * FgPack<T>::E);
+    const bool straight = fg_rows_lie_straight(a.dim, sizeof(T), a.src, a.dst);
+    const uint32_t tile = 32 * kPacks * (straight ? FgPack<T>::E : 4), tiles = (uint32_t)(((uint64_t)a.dim + tile - 1) / tile);
     const uint64_t blocks = ((uint64_t)a.tokens * tiles + 7) / 8, cap = 32ull * ctx->sm_count;
-    const int grid = (int)(blocks < cap ? blocks : cap);
-    const T *table = (const T*)a.src, *end = table + (uint64_t)a.vocab * a.dim;
-    if (fg_rows_lie_straight(a.dim, sizeof(T), a.src, a.dst))
-        fg_launch(ctx, embed_kernel<T, false>, grid, 256, 0, a.tokens, a.vocab, a.dim, tiles, a.ids, table, end, a.scale, (T*)a.dst);
-    else fg_launch(ctx, embed_kernel<T, true>, grid, 256, 0, a.tokens, a.vocab, a.dim, tiles, a.ids, table, end, a.scale, (T*)a.dst);
+    fg_launch(ctx, straight ? embed_kernel<T, true> : embed_kernel<T, false>, (unsigned)(blocks < cap ? blocks : cap), 256, 0, a.tokens, a.vocab, a.dim, tiles, a.ids,
+              (const T*)a.src, a.scale, (T*)a.dst);
     FG_LAUNCHED(ctx);
     return FG_OK;
 }

@@ -77,7 +77,7 @@ template <typename T_, int kPacks, bool kFull, int kTensors>
 struct Straight {
     using T = T_;
     static constexpr int E = FgPack<T>::E, P = E / 2, N = kPacks * E, kStages = stages_of(kTensors * kPacks);
-    static constexpr bool kAhead = true;
+    static constexpr bool kAhead = true, kTight = false;
     uint32_t slots, block, offset, pitch, have;      // shared address of the thread's first slot, bytes of a block's packs, of the thread, of a group's packs
     uint32_t put = 0, take = 0;                      // stages
     __device__ __forceinline__ Straight(const Group& g, uint32_t cols, const void* shared) {
@@ -165,15 +165,29 @@ struct Straight {
 template <typename T_, int kCount, int kTensors>
 struct Ragged {
     using T = T_;
-    static constexpr int N = kCount, kStages = 1;
-    static constexpr bool kAhead = false;
+    static constexpr int N = kCount, kStages = 2;
+    static constexpr bool kAhead = kTensors * kCount <= 8;       // the next row's elements are on their way, in registers
+    static constexpr bool kTight = true;                         // 64 registers, for 1024 threads an SM
     uint32_t thread, threads, cols;
+    T next[kAhead ? kTensors : 1][kAhead ? N : 1];
     __device__ __forceinline__ Ragged(const Group& g, uint32_t cols_, const void*) : thread(g.thread), threads(g.threads), cols(cols_) {}
-    __device__ __forceinline__ void ask(int, const T*) {}
+    __device__ __forceinline__ void ask(int t, const T* row) {
+        if constexpr (kAhead)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const uint32_t c = thread + i * threads;
+                next[t][i] = c < cols ? row[c] : fg_narrow<T>(0.0f);
+            }
+    }
     __device__ __forceinline__ void asked() {}
     __device__ __forceinline__ void arrived() const {}
     __device__ __forceinline__ void taken() {}
-    __device__ __forceinline__ void get(int, const T* row, float2 (&v)[N / 2]) const { load(row, v); }
+    __device__ __forceinline__ void get(int t, const T* row, float2 (&v)[N / 2]) const {
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fg_widen(next[t][2 * i]), fg_widen(next[t][2 * i + 1]));
+        } else load(row, v);
+    }
     __device__ __forceinline__ void load(const T* row, float2 (&v)[N / 2]) const {
         T w[N];
 #pragma unroll
@@ -207,7 +221,7 @@ struct Ragged {
 };
 
 template <typename C>
-__global__ void __launch_bounds__(kMaxThreads, !C::kAhead && C::N <= 16 ? 2 : 1) norm_held_kernel(const NormArgs a, int threads) {
+__global__ void __launch_bounds__(kMaxThreads, C::kTight && C::N <= 16 ? 2 : 1) norm_held_kernel(const NormArgs a, int threads) {
     using T = typename C::T;
     constexpr int H = C::N / 2;
     extern __shared__ uint4 shared[];
@@ -285,7 +299,7 @@ __global__ void __launch_bounds__(kMaxThreads, !C::kAhead && C::N <= 16 ? 2 : 1)
 // over the rows of its group, a block adds its groups and leaves one row of parts: [block][2][pitch].
 // With c = x - mean, dx = rstd * g + (-rstd * m1) + c * (-rstd^2 * m2), where m1 and m2 are the means of g and of g * h.
 template <typename C, bool kParams>
-__global__ void __launch_bounds__(kMaxThreads, !C::kAhead && C::N <= 4 ? 2 : 1) norm_bwd_held_kernel(const NormBwdArgs a, int threads, float* parts, uint32_t pitch) {
+__global__ void __launch_bounds__(kMaxThreads, C::kTight && C::N <= 4 ? 2 : 1) norm_bwd_held_kernel(const NormBwdArgs a, int threads, float* parts, uint32_t pitch) {
     using T = typename C::T;
     constexpr int H = C::N / 2;
     extern __shared__ uint4 shared[];      // the slots; at the end the groups' sums
