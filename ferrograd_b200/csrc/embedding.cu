@@ -47,6 +47,7 @@ struct SortArgs {
     uint32_t first_row;
 };
 
+constexpr uint32_t kMaxGroup = 2048;     // rows that a block of the second launch marks
 constexpr uint32_t kSegment = 2048;      // bytes that a warp clears at a time
 __device__ __forceinline__ void clear_bytes(char* p, uint32_t bytes, int lane) {
     const uint32_t before = min((uint32_t)(-reinterpret_cast<uintptr_t>(p) & 15u), bytes), words = (bytes - before) / 16;
@@ -268,6 +269,16 @@ __device__ __forceinline__ uint32_t first_not_below(const uint2* list, uint32_t 
     }
     return lo;
 }
+// A block of 8 warps clears those of n rows from `rows` on that are not marked.
+__device__ __forceinline__ void clear_unmarked(char* rows, uint32_t n, uint64_t row_bytes, const uint32_t* marks) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t segments = (row_bytes + kSegment - 1) / kSegment, units = n * segments;
+    for (uint64_t k = warp; k < units; k += 8) {
+        const uint32_t i = (uint32_t)(k / segments);
+        const uint64_t from = k % segments * kSegment;
+        if (!(marks[i >> 5] >> (i & 31) & 1u)) clear_bytes(rows + i * row_bytes + from, (uint32_t)min((uint64_t)kSegment, row_bytes - from), lane);
+    }
+}
 // A block clears the rows of its group that the sorted list does not name.
 __device__ void clear_group(const SumArgs& s, uint32_t fill, uint32_t* marks, uint32_t* ends) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -283,13 +294,7 @@ __device__ void clear_group(const SumArgs& s, uint32_t fill, uint32_t* marks, ui
         atomicOr(&marks[k >> 5], 1u << (k & 31));
     }
     __syncthreads();
-    const uint64_t segments = (s.row_bytes + kSegment - 1) / kSegment, units = (v1 - v0) * segments;
-    for (uint64_t k = warp; k < units; k += 8) {
-        const uint32_t i = (uint32_t)(k / segments);
-        const uint64_t from = k % segments * kSegment;
-        if (!(marks[i >> 5] >> (i & 31) & 1u))
-            clear_bytes(static_cast<char*>(s.dtable) + (v0 + i) * s.row_bytes + from, (uint32_t)min((uint64_t)kSegment, s.row_bytes - from), lane);
-    }
+    clear_unmarked(static_cast<char*>(s.dtable) + v0 * s.row_bytes, (uint32_t)(v1 - v0), s.row_bytes, marks);
 }
 template <typename T, bool kShift>
 __device__ __forceinline__ uint4 load_old(const SumArgs& s, uint32_t v, uint64_t col, uint32_t left) {
@@ -482,6 +487,95 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const SumArgs s) {
     store_sum<T, kShift, kAdd>(s, id, col, left, acc);
 }
 
+// ---- few tokens ----
+// Up to kFew of them need no sorting: a block takes a token and two tiles of columns, finds by ballots where else its id stands, and if nowhere
+// before, adds those rows, four warps a quarter of them each where there are many.  Blocks behind these clear the other rows.  One launch
+// instead of three, added to the table: 129 tokens of 1024 f32 columns 16 -> 4 us, 256 of 777 25 -> 7, 512 of 1024 17 -> 10; from there on the
+// blocks of tokens that are not their id's first cost more than the sort.
+constexpr uint32_t kFew = 512;
+template <typename T, bool kShift, bool kAdd>
+__global__ void __launch_bounds__(256) embed_few_kernel(const SumArgs s, const uint32_t* ids) {
+    constexpr int E = FgPack<T>::E, kAhead = 8, kWords = kFew / 32;
+    __shared__ uint32_t marks[kMaxGroup / 32];
+    __shared__ unsigned where[kWords];
+    __shared__ float4 parts[8][E / 4][32];
+    fg_grid_enter();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (!kAdd && blockIdx.x >= s.blocks) {
+        const uint64_t v0 = (uint64_t)(blockIdx.x - s.blocks) << s.group;
+        const uint32_t n = (uint32_t)(min((uint64_t)s.fill_rows, v0 + (1u << s.group)) - v0);
+        for (uint32_t i = threadIdx.x; i < (n + 31) / 32; i += 256) marks[i] = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < s.tokens; i += 256) {
+            const uint32_t k = ids[i] - (uint32_t)v0;
+            if (k < n) atomicOr(&marks[k >> 5], 1u << (k & 31));
+        }
+        __syncthreads();
+        clear_unmarked(static_cast<char*>(s.dtable) + v0 * s.row_bytes, n, s.row_bytes, marks);
+        return;
+    }
+    const uint32_t pairs = (s.tiles + 1) / 2, t = blockIdx.x / pairs, tile = blockIdx.x % pairs * 2 + (warp >> 2), quarter = warp & 3;
+    const uint64_t col = ((uint64_t)tile * 32 + lane) * E;
+    const uint32_t left = col < s.dim ? (uint32_t)min((uint64_t)E, s.dim - col) : 0, id = ids[t];
+    if (id >= s.fill_rows) return;      // padding
+    uint4 old = make_uint4(0, 0, 0, 0);
+    if (kAdd && left && quarter == 0) old = load_old<T, kShift>(s, id, col, left);
+#pragma unroll
+    for (int j = warp; j < kWords; j += 8) {
+        const unsigned found = __ballot_sync(kFull, 32 * j + lane < s.tokens && ids[min(32 * j + lane, s.tokens - 1)] == id);
+        if (lane == 0) where[j] = found;
+    }
+    __syncthreads();
+    uint32_t count = 0, first = kFew;
+#pragma unroll
+    for (int j = kWords - 1; j >= 0; --j) {
+        count += __popc(where[j]);
+        if (where[j]) first = 32 * j + __ffs(where[j]) - 1;
+    }
+    if (first < t) return;      // its first token adds
+    const bool shared = count >= 8;
+    const uint32_t from = shared ? count * quarter / 4 : 0, n = shared ? count * (quarter + 1) / 4 - from : quarter ? 0 : count;
+    uint32_t word = 0, skip = from;
+    while (n && skip >= (uint32_t)__popc(where[word])) skip -= __popc(where[word++]);
+    unsigned bits = n ? where[word] : 0;
+    for (; skip; --skip) bits &= bits - 1;
+    const T* const dout = static_cast<const T*>(s.dout);
+    float acc[E] = {};
+    for (uint32_t i = 0; i < n; i += kAhead) {
+        uint4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            v[k] = make_uint4(0, 0, 0, 0);
+            if (i + k < n) {
+                while (!bits) bits = where[++word];
+                const uint64_t row = 32 * word + __ffs(bits) - 1;
+                bits &= bits - 1;
+                if (left) v[k] = fg_load_pack<T, kShift>(dout + row * s.dim + col, left, dout, (const T*)s.dout_end);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (i + k < n) {
+                float x[E];
+                FgPack<T>::widen(v[k], x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += x[e];
+            }
+    }
+    if (shared) {
+#pragma unroll
+        for (int e = 0; e < E / 4; ++e) parts[warp][e][lane] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+        __syncthreads();
+        for (int q = 1; q < 4 && quarter == 0; ++q)
+#pragma unroll
+            for (int e = 0; e < E / 4; ++e) {
+                const float4 p = parts[warp + q][e][lane];
+                acc[4 * e] += p.x; acc[4 * e + 1] += p.y; acc[4 * e + 2] += p.z; acc[4 * e + 3] += p.w;
+            }
+    }
+    if (quarter == 0) store_sum<T, kShift, kAdd>(s, id, col, left, acc, old);
+}
+
 // ---- lookup ----
 // A warp takes a token and a tile of columns, `kPacks` packs of 16 bytes per lane or, off 16-byte boundaries, as many single elements side by side
 // (words turned by a row's distance from the boundary took more instructions than the elements do).
@@ -543,6 +637,19 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     s.dout_end = (const T*)a.src + (uint64_t)a.tokens * a.dim;
     s.dtable = a.dst;
     s.dtable_end = (T*)a.dst + (uint64_t)a.vocab * a.dim;
+    const bool straight = fg_rows_lie_straight(a.dim, sizeof(T), a.src, a.dst), add = a.accumulate != 0;
+    if (a.tokens <= kFew) {
+        s.row_bytes = (uint64_t)a.dim * sizeof(T);
+        s.fill_rows = a.vocab;
+        while (1u << s.group < kMaxGroup && s.row_bytes << (s.group + 1) <= 32768) ++s.group;
+        const uint64_t work = (uint64_t)a.tokens * ((s.tiles + 1) / 2), fills = add ? 0 : ((uint64_t)a.vocab + (1ull << s.group) - 1) >> s.group;
+        FG_REQUIRE(ctx, work + fills < (1ull << 31), "fg_embedding_bwd: tensor too large");
+        s.blocks = (uint32_t)work;
+        fg_launch(ctx, add ? straight ? embed_few_kernel<T, false, true> : embed_few_kernel<T, true, true>
+                           : straight ? embed_few_kernel<T, false, false> : embed_few_kernel<T, true, false>, (unsigned)(work + fills), 256, 0, s, a.ids);
+        FG_LAUNCHED(ctx);
+        return FG_OK;
+    }
     // Stretches for four waves of warps, of 8 to 128 entries; a chunk is the eight stretches of a block.
     const uint64_t want = (uint64_t)a.tokens * s.tiles / (96ull * ctx->sm_count);
     s.length = (uint32_t)(want < 8 ? 8 : want > 128 ? 128 : (want + 7) / 8 * 8);
@@ -581,7 +688,7 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
         const uint64_t groups = (rows + (1ull << o.group) - 1) >> o.group;
         while (o.shares < 8 && (1ull << o.shares) < groups && rows * row >> (o.shares + 14)) ++o.shares;      // from 16 KB each
         fill = ((1ull << o.shares) + ctas - 1) / ctas * ctas;
-        while (s.group < 11 && row << (s.group + 1) <= 131072) ++s.group;
+        while (1u << s.group < kMaxGroup && row << (s.group + 1) <= 131072) ++s.group;
         s.fills = (uint32_t)(((uint64_t)s.fill_rows + (1ull << s.group) - 1) >> s.group);
     }
     FG_REQUIRE(ctx, blocks + s.fills < (1ull << 31), "fg_embedding_bwd: tensor too large");
@@ -597,7 +704,6 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     }
     fg_launch_cluster(ctx, held ? embed_sort_kernel<true> : embed_sort_kernel<false>, (unsigned)(ctas + fill), kSortThreads, bytes, ctas, o);
     FG_LAUNCHED(ctx);
-    const bool straight = fg_rows_lie_straight(a.dim, sizeof(T), a.src, a.dst), add = a.accumulate != 0;
     fg_launch(ctx, add ? straight ? embed_sum_kernel<T, false, true> : embed_sum_kernel<T, true, true>
                        : straight ? embed_sum_kernel<T, false, false> : embed_sum_kernel<T, true, false>, (unsigned)(blocks + s.fills), 256, 0, s);
     FG_LAUNCHED(ctx);
