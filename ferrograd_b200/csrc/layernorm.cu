@@ -4,6 +4,8 @@
 // mean is m + r and the variance q - r * r: rows far from zero lose nothing to the subtraction.
 // Backward, with h = (x - mean) * rstd and g = dy * gamma: dx = rstd * (g - mean(g) - h * mean(g * h)); dgamma and dbeta are column
 // sums of dy * h and dy.
+#include <atomic>
+
 #include "rows.cuh"
 
 namespace {
@@ -70,9 +72,9 @@ struct Group {
     }
 };
 
-// Rows that lie straight: a thread has packs `thread`, `thread` + threads, ... of 16 bytes, asked for two or three rows ahead by asynchronous
+// Rows that lie straight: a thread has packs `thread`, `thread` + threads, ... of 16 bytes, asked for one to four rows ahead by asynchronous
 // copies into slots of shared memory that are the thread's own.
-__host__ __device__ constexpr int stages_of(int packs) { return packs > 4 ? 3 : 4; }      // by the packs of all tensors in a stage: 512 threads fit
+__host__ __device__ constexpr int stages_of(int packs) { return packs > 8 ? 1 : packs > 4 ? 3 : 4; }      // by the packs of all tensors in a stage: 512 threads fit
 template <typename T_, int kPacks, bool kFull, int kTensors>
 struct Straight {
     using T = T_;
@@ -100,7 +102,7 @@ struct Straight {
         fg_copies_end();
         put = put == kStages - 1 ? 0 : put + 1;
     }
-    __device__ __forceinline__ void arrived() const { fg_copies_wait<kStages - 2>(); }
+    __device__ __forceinline__ void arrived() const { fg_copies_wait<kStages - 1>(); }
     __device__ __forceinline__ void taken() { take = take == kStages - 1 ? 0 : take + 1; }
     __device__ __forceinline__ void spread(int k, const uint4& w, float2* v) const {
         float2 x[P];
@@ -165,7 +167,7 @@ struct Straight {
 template <typename T_, int kCount, int kTensors>
 struct Ragged {
     using T = T_;
-    static constexpr int N = kCount, kStages = 2;
+    static constexpr int N = kCount, kStages = 1;
     static constexpr bool kAhead = kTensors * kCount <= 8;       // the next row's elements are on their way, in registers
     static constexpr bool kTight = true;                         // 64 registers, for 1024 threads an SM
     uint32_t thread, threads, cols;
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(kMaxThreads, C::kTight && C::N <= 16 ? 2 : 1) 
     };
     if (C::kAhead)
 #pragma unroll
-        for (int i = 0; i < C::kStages - 1; ++i) ask();
+        for (int i = 0; i < C::kStages; ++i) ask();
     int turn = 0;
     for (uint64_t r = first; r < a.rows; r += step, x += stride, y += stride) {
         float2 v[H];
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(kMaxThreads, C::kTight && C::N <= 4 ? 2 : 1) n
     };
     if (C::kAhead)
 #pragma unroll
-        for (int i = 0; i < C::kStages - 1; ++i) ask();
+        for (int i = 0; i < C::kStages; ++i) ask();
     float mean = 0.0f, rstd = 0.0f;
     if (first < a.rows) { mean = a.mean[first]; rstd = a.rstd[first]; }
     float2 dg[H], db[H];
@@ -493,30 +495,57 @@ __global__ void __launch_bounds__(256) norm_bwd_stream_kernel(const NormBwdArgs 
     }
 }
 
-// Column sums of dy * h and dy over a chunk of rows: 32 columns by 8 rows per block.  part: [2][chunks][cols].
+// Rows that are too long for a thread to keep its columns' sums beside them: the parameters' gradients first, by columns, over chunks of rows.
+// A warp takes 32 columns, or as many packs of rows that lie straight, and every 8th row of the chunk.  part: [2][chunks][cols].
 constexpr uint32_t kChunk = 256;
-template <typename T>
+template <typename T, bool kPacked>
 __global__ void __launch_bounds__(256) norm_columns_kernel(const NormBwdArgs a, float* part) {
-    __shared__ float red[2][8][32];
+    constexpr int E = kPacked ? FgPack<T>::E : 1, kRows = 4;
+    __shared__ float red[2][8][32][E];
     fg_grid_enter();
-    const uint64_t c = (uint64_t)blockIdx.x * 32 + threadIdx.x, chunks = gridDim.y;
+    const uint64_t c = ((uint64_t)blockIdx.x * 32 + threadIdx.x) * E, chunks = gridDim.y;
     const uint32_t r0 = blockIdx.y * kChunk, r1 = min(a.rows, r0 + kChunk);
-    float s1 = 0.0f, s2 = 0.0f;
+    const T *const x = static_cast<const T*>(a.x) + c, *const dy = static_cast<const T*>(a.dy) + c;
+    float s1[E] = {}, s2[E] = {};
     if (c < a.cols)
-        for (uint32_t r = r0 + threadIdx.y; r < r1; r += 8) {
-            const float dy = fg_widen(static_cast<const T*>(a.dy)[(uint64_t)r * a.cols + c]);
-            s1 = __fmaf_rn(dy, (fg_widen(static_cast<const T*>(a.x)[(uint64_t)r * a.cols + c]) - a.mean[r]) * a.rstd[r], s1);
-            s2 += dy;
-        }
-    red[0][threadIdx.y][threadIdx.x] = s1;
-    red[1][threadIdx.y][threadIdx.x] = s2;
-    __syncthreads();
-    if (threadIdx.y < 2 && c < a.cols) {
-        float s = 0.0f;
+        for (uint32_t r = r0 + threadIdx.y; r < r1; r += 8 * kRows) {
+            float u[kRows][E], v[kRows][E], mean[kRows], rstd[kRows];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += red[threadIdx.y][i][threadIdx.x];
-        part[(threadIdx.y * chunks + blockIdx.y) * a.cols + c] = s;
+            for (int j = 0; j < kRows; ++j) {
+                const uint32_t row = r + 8 * j;
+                const bool there = row < r1;
+                mean[j] = there ? a.mean[row] : 0.0f;
+                rstd[j] = there ? a.rstd[row] : 0.0f;
+                if constexpr (kPacked) {
+                    FgPack<T>::widen(there ? *reinterpret_cast<const uint4*>(x + (uint64_t)row * a.cols) : make_uint4(0, 0, 0, 0), u[j]);
+                    FgPack<T>::widen(there ? *reinterpret_cast<const uint4*>(dy + (uint64_t)row * a.cols) : make_uint4(0, 0, 0, 0), v[j]);
+                } else {
+                    u[j][0] = there ? fg_widen(x[(uint64_t)row * a.cols]) : 0.0f;
+                    v[j][0] = there ? fg_widen(dy[(uint64_t)row * a.cols]) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kRows; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    s1[e] = __fmaf_rn(v[j][e], (u[j][e] - mean[j]) * rstd[j], s1[e]);
+                    s2[e] += v[j][e];
+                }
+        }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        red[0][threadIdx.y][threadIdx.x][e] = s1[e];
+        red[1][threadIdx.y][threadIdx.x][e] = s2[e];
     }
+    __syncthreads();
+    if (threadIdx.y < 2 && c < a.cols)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += red[threadIdx.y][i][threadIdx.x][e];
+            part[(threadIdx.y * chunks + blockIdx.y) * a.cols + c + e] = s;
+        }
 }
 template <typename T>
 __global__ void __launch_bounds__(256) norm_fold_kernel(const NormBwdArgs a, const float* part, uint32_t chunks) {
@@ -553,15 +582,19 @@ HeldPlan held_plan(const fg_ctx* ctx, uint32_t rows, uint64_t units, int least, 
     p.grid = (int)(need < cap ? need : cap);
     return p;
 }
+// More shared memory than a kernel may have by default, once per kernel (`done`) and device.
 template <typename K>
-int32_t allow_shared(fg_ctx* ctx, K kernel, size_t bytes) {
-    if (bytes > 32 * 1024) FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+int32_t allow_shared(fg_ctx* ctx, std::atomic<uint64_t>& done, K kernel, size_t bytes) {
+    if (bytes <= 32 * 1024 || done.load(std::memory_order_acquire) >> (ctx->device & 63) & 1ull) return FG_OK;
+    FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024));
+    done.fetch_or(1ull << (ctx->device & 63), std::memory_order_release);
     return FG_OK;
 }
 
 template <typename C>
 int32_t launch_held(fg_ctx* ctx, const NormArgs& a, HeldPlan p) {
-    const int32_t s = allow_shared(ctx, norm_held_kernel<C>, p.bytes);
+    static std::atomic<uint64_t> done{0};
+    const int32_t s = allow_shared(ctx, done, norm_held_kernel<C>, p.bytes);
     if (s != FG_OK) return s;
     fg_launch(ctx, norm_held_kernel<C>, p.grid, p.threads * p.groups, p.bytes, a, p.threads);
     FG_LAUNCHED(ctx);
@@ -590,15 +623,19 @@ int32_t norm_fwd(fg_ctx* ctx, const NormArgs& a) {
     return FG_OK;
 }
 
-template <typename C>
-int32_t launch_bwd_held(fg_ctx* ctx, const NormBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch) {
-    const size_t sums = parts && p.groups > 1 ? 8ull * C::N * p.threads : 0, bytes = p.bytes < sums ? sums : p.bytes;
-    const auto kernel = parts ? norm_bwd_held_kernel<C, true> : norm_bwd_held_kernel<C, false>;
-    const int32_t s = allow_shared(ctx, kernel, bytes);
+template <typename C, bool kParams>
+int32_t launch_bwd(fg_ctx* ctx, const NormBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch) {
+    const size_t sums = kParams && p.groups > 1 ? 8ull * C::N * p.threads : 0, bytes = p.bytes < sums ? sums : p.bytes;
+    static std::atomic<uint64_t> done{0};
+    const int32_t s = allow_shared(ctx, done, norm_bwd_held_kernel<C, kParams>, bytes);
     if (s != FG_OK) return s;
-    fg_launch(ctx, kernel, p.grid, p.threads * p.groups, bytes, a, p.threads, parts, pitch);
+    fg_launch(ctx, norm_bwd_held_kernel<C, kParams>, p.grid, p.threads * p.groups, bytes, a, p.threads, parts, pitch);
     FG_LAUNCHED(ctx);
     return FG_OK;
+}
+template <typename C>
+int32_t launch_bwd_held(fg_ctx* ctx, const NormBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch) {
+    return parts ? launch_bwd<C, true>(ctx, a, p, parts, pitch) : launch_bwd<C, false>(ctx, a, p, parts, pitch);
 }
 template <typename T, int kPacks>
 int32_t launch_bwd_straight(fg_ctx* ctx, const NormBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch) {
@@ -632,22 +669,24 @@ int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
         FG_LAUNCHED(ctx);
         return FG_OK;
     }
-    float* part = nullptr;
-    const uint32_t chunks = (a.rows + kChunk - 1) / kChunk;
     if (a.dgamma || a.dbeta) {      // before dx, which may be dy or x
+        const uint32_t chunks = (a.rows + kChunk - 1) / kChunk, E = straight ? FgPack<T>::E : 1;
         void* w;
         const int32_t s = fg_ws_alloc(ctx, 8ull * chunks * a.cols, &w);
         if (s != FG_OK) return s;
-        part = (float*)w;
-        fg_launch(ctx, norm_columns_kernel<T>, dim3((a.cols + 31) / 32, chunks), dim3(32, 8), 0, a, part);
+        fg_launch(ctx, straight ? norm_columns_kernel<T, true> : norm_columns_kernel<T, false>, dim3((a.cols + 32 * E - 1) / (32 * E), chunks), dim3(32, 8), 0, a, (float*)w);
         FG_LAUNCHED(ctx);
-        fg_launch(ctx, norm_fold_kernel<T>, dim3((a.cols + 255) / 256, 2), 256, 0, a, (const float*)part, chunks);
-        FG_LAUNCHED(ctx);
-    }
-    if (a.dx) {
-        fg_launch(ctx, norm_bwd_stream_kernel<T>, rows_grid(ctx, a.rows), 256, 0, a);
+        fg_launch(ctx, norm_fold_kernel<T>, dim3((a.cols + 255) / 256, 2), 256, 0, a, (const float*)w, chunks);
         FG_LAUNCHED(ctx);
     }
+    if (!a.dx) return FG_OK;
+    // dx alone leaves a thread room for 32 columns.
+    const HeldPlan q = straight ? held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 2 * usual, 2 * usual, 2 * usual, 2, 512) : HeldPlan{};
+    if (q.threads) return launch_bwd<Straight<T, 2 * usual, false, 2>, false>(ctx, a, q, nullptr, 0);
+    const HeldPlan e = straight ? HeldPlan{} : held_plan(ctx, a.rows, a.cols, 32, 32, 32, 0, 512);
+    if (e.threads) return launch_bwd<Ragged<T, 32, 2>, false>(ctx, a, e, nullptr, 0);
+    fg_launch(ctx, norm_bwd_stream_kernel<T>, rows_grid(ctx, a.rows), 256, 0, a);
+    FG_LAUNCHED(ctx);
     return FG_OK;
 }
 
@@ -684,6 +723,7 @@ int32_t fg_layernorm_bwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t col
     FG_REQUIRE(ctx, fg_at_element(x, size) && fg_at_element(dy, size) && fg_at_element(gamma, size) && fg_at_element(dx, size) &&
                         fg_at_element(dgamma, size) && fg_at_element(dbeta, size) && fg_at_element(mean, 4) && fg_at_element(rstd, 4),
                "fg_layernorm_bwd: a tensor does not start at an element");
+    FG_REQUIRE(ctx, dx || dgamma || dbeta, "fg_layernorm_bwd: no output");
     FG_REQUIRE(ctx, !accumulate_dx || (dx != dy && dx != x), "fg_layernorm_bwd: accumulate_dx needs a dx of its own");
     const uint64_t bytes = (uint64_t)rows * cols * size;
     FG_REQUIRE(ctx, (dx == x || !fg_ranges_meet(x, bytes, dx, bytes)) && (dx == dy || !fg_ranges_meet(dy, bytes, dx, bytes)),
