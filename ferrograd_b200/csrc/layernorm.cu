@@ -200,9 +200,21 @@ struct Ragged {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fg_widen(w[2 * i]), fg_widen(w[2 * i + 1]));
     }
-    struct Kept {};      // (read again for every row)
-    __device__ __forceinline__ void keep(const T*, Kept&) const {}
-    __device__ __forceinline__ void kept(const Kept&, const T* p, float2 (&v)[N / 2]) const { load(p, v); }
+    static constexpr bool kKeep = kCount <= 8;
+    struct Kept { T w[kKeep ? N : 1]; };
+    __device__ __forceinline__ void keep(const T* p, Kept& kept) const {
+#pragma unroll
+        for (int i = 0; i < (kKeep ? N : 0); ++i) {
+            const uint32_t c = thread + i * threads;
+            kept.w[i] = c < cols ? p[c] : fg_narrow<T>(0.0f);
+        }
+    }
+    __device__ __forceinline__ void kept(const Kept& kept, const T* p, float2 (&v)[N / 2]) const {
+        if constexpr (kKeep) {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fg_widen(kept.w[2 * i]), fg_widen(kept.w[2 * i + 1]));
+        } else load(p, v);
+    }
     __device__ __forceinline__ void mask(float2 (&v)[N / 2]) const {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
@@ -564,11 +576,14 @@ int rows_grid(const fg_ctx* ctx, uint32_t rows) { return (int)(rows < 8u * ctx->
 // How a kernel that holds rows is launched: a thread's packs (or elements, of ragged rows), the threads of a group, the groups of a block, the
 // bytes of its slots, the blocks; threads = 0: not at all.
 struct HeldPlan { int units, threads, groups; bool full; size_t bytes; int grid; };
-// A block has 256 threads or, for a longer row, up to 512.  Threads hold `usual` units, or up to `most` where the row asks for it; of few rows,
-// and where a warp is enough, `least`.  `resident`: threads that an SM has registers for, at the usual units.
+// A block has 256 threads or, for a longer row, up to 512.  Threads hold `usual` units, or up to `most` where the row asks for it (up to 4, which
+// registers hold, from 256 threads on: an SM has two rows to switch between then; 7000 x 8192 bf16 forward 62.7 -> 44.7 us); of few rows, and where
+// a warp is enough, `least`.  `resident`: threads that an SM has registers for, at the usual units.
 HeldPlan held_plan(const fg_ctx* ctx, uint32_t rows, uint64_t units, int least, int usual, int most, int tensors, int resident) {
     HeldPlan p{least, 0, 1, false, 0, 0};
-    while (p.units < most && (units > (uint64_t)kMaxThreads * p.units || (p.units < usual && rows > 2u * ctx->sm_count && units > 32ull * p.units))) p.units *= 2;
+    const bool many = rows > 2u * ctx->sm_count;
+    while (p.units < most && (units > (uint64_t)kMaxThreads * p.units || (many && units > (p.units < usual ? 32ull : p.units < 4 ? 256ull : ~0ull / p.units) * p.units)))
+        p.units *= 2;
     if (units > (uint64_t)kMaxThreads * p.units) return p;
     p.threads = (int)((units + 32 * p.units - 1) / (32 * p.units) * 32);
     p.full = units == (uint64_t)p.threads * p.units;
@@ -613,7 +628,7 @@ int32_t norm_fwd(fg_ctx* ctx, const NormArgs& a) {
             return p.units == 1 ? launch_straight<T, 1>(ctx, a, p) : p.units == 2 ? launch_straight<T, 2>(ctx, a, p)
                    : p.units == 4 ? launch_straight<T, 4>(ctx, a, p) : launch_straight<T, 8>(ctx, a, p);
     } else {
-        HeldPlan p = held_plan(ctx, a.rows, a.cols, 4, 16, 32, 0, 1024);
+        HeldPlan p = held_plan(ctx, a.rows, a.cols, 4, 8, 32, 0, 1024);
         if (p.threads)
             return p.units == 4 ? launch_held<Ragged<T, 4, 1>>(ctx, a, p) : p.units == 8 ? launch_held<Ragged<T, 8, 1>>(ctx, a, p)
                    : p.units == 16 ? launch_held<Ragged<T, 16, 1>>(ctx, a, p) : launch_held<Ragged<T, 32, 1>>(ctx, a, p);
