@@ -162,14 +162,15 @@ struct Straight {
     }
 };
 
-// Any other row: a thread has the elements `thread`, `thread` + threads, ... of it.  (Words turned by the row's distance from a 16-byte boundary
-// took three times the instructions.)
+// Any other row: a thread has the elements `thread`, `thread` + threads, ... of it.  (Taking 16-byte words through shared memory and turning them by
+// the row's distance from the boundary is no faster: what turning and the ends of rows take is what addresses and tests take here; 30000 x 777 f16
+// forward 53 us and 54, backward 85 and 72.)
 template <typename T_, int kCount, int kTensors>
 struct Ragged {
     using T = T_;
     static constexpr int N = kCount, kStages = 1;
     static constexpr bool kAhead = kTensors * kCount <= 8;       // the next row's elements are on their way, in registers
-    static constexpr bool kTight = true;                         // 64 registers, for 1024 threads an SM
+    static constexpr bool kTight = kCount <= 8;                  // 64 registers, for 1024 threads an SM
     uint32_t thread, threads, cols;
     T next[kAhead ? kTensors : 1][kAhead ? N : 1];
     __device__ __forceinline__ Ragged(const Group& g, uint32_t cols_, const void*) : thread(g.thread), threads(g.threads), cols(cols_) {}
@@ -200,7 +201,7 @@ struct Ragged {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fg_widen(w[2 * i]), fg_widen(w[2 * i + 1]));
     }
-    static constexpr bool kKeep = kCount <= 8;
+    static constexpr bool kKeep = kCount <= 16;
     struct Kept { T w[kKeep ? N : 1]; };
     __device__ __forceinline__ void keep(const T* p, Kept& kept) const {
 #pragma unroll
@@ -576,13 +577,14 @@ int rows_grid(const fg_ctx* ctx, uint32_t rows) { return (int)(rows < 8u * ctx->
 // How a kernel that holds rows is launched: a thread's packs (or elements, of ragged rows), the threads of a group, the groups of a block, the
 // bytes of its slots, the blocks; threads = 0: not at all.
 struct HeldPlan { int units, threads, groups; bool full; size_t bytes; int grid; };
-// A block has 256 threads or, for a longer row, up to 512.  Threads hold `usual` units, or up to `most` where the row asks for it (up to 4, which
-// registers hold, from 256 threads on: an SM has two rows to switch between then; 7000 x 8192 bf16 forward 62.7 -> 44.7 us); of few rows, and where
+// A block has 256 threads or, for a longer row, up to 512.  Threads hold `usual` units, or up to `most` where the row asks for it (up to 4 packs, which
+// registers hold, where a warp is enough with them, and from 256 threads on: an SM has two rows to switch between then; 7000 x 8192 bf16 forward
+// 62.7 -> 44.7 us); of few rows, and where
 // a warp is enough, `least`.  `resident`: threads that an SM has registers for, at the usual units.
 HeldPlan held_plan(const fg_ctx* ctx, uint32_t rows, uint64_t units, int least, int usual, int most, int tensors, int resident) {
     HeldPlan p{least, 0, 1, false, 0, 0};
     const bool many = rows > 2u * ctx->sm_count;
-    while (p.units < most && (units > (uint64_t)kMaxThreads * p.units || (many && units > (p.units < usual ? 32ull : p.units < 4 ? 256ull : ~0ull / p.units) * p.units)))
+    while (p.units < most && (units > (uint64_t)kMaxThreads * p.units || (many && units > (p.units < usual || (p.units < 4 && units <= 128) ? 32ull : p.units < 4 ? 256ull : ~0ull / p.units) * p.units)))
         p.units *= 2;
     if (units > (uint64_t)kMaxThreads * p.units) return p;
     p.threads = (int)((units + 32 * p.units - 1) / (32 * p.units) * 32);
