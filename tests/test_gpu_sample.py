@@ -153,6 +153,30 @@ def test_border_of_top_k_among_equals(ctx):
         run(ctx, x, r.random(64).astype(np.float32), top_k=r.integers(5, 30, 64).astype(np.uint32), min_p=np.full(64, 0.2, np.float32))
 
 
+@pytest.mark.parametrize("dtype,rows,cols", [("f32", 2, 500_001), ("f16", 2, 1_000_003), ("bf16", 1, 2_097_152)])
+def test_rows_that_no_cluster_holds(ctx, dtype, rows, cols):
+    r = np.random.Generator(np.random.Philox(cols))
+    x = r.standard_normal((rows, cols)) * 3
+    x[r.random((rows, cols)) < 0.2] = -np.inf
+    x, u = rounded(x, dtype), r.random(rows).astype(np.float32)
+    for names in ((), ("top_k",), ("top_p",), ("top_k", "top_p", "min_p"), ("temperature", "min_p")):
+        run(ctx, x, u, dtype, 1, **params_of(names, rows, cols, r))
+
+
+@pytest.mark.parametrize("cols,k", [(5000, 2500), (20000, 300), (20000, 3000), (50000, 49_999), (130000, 1500), (130000, 20_000)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_wide_filters(ctx, cols, k, dtype):
+    # more candidates than a list has room for, and nuclei of most of a row
+    r = np.random.Generator(np.random.Philox(cols + k))
+    x, u = rounded(r.standard_normal((4, cols)) * 2, dtype), r.random(4).astype(np.float32)
+    x[2] *= np.float32(0.0625)          # nearly flat
+    x[3] = np.sort(x[3])                # all that counts is in the last CTA
+    run(ctx, x, u, dtype, top_k=np.full(4, k, np.uint32))
+    run(ctx, x, u, dtype, top_k=np.full(4, k, np.uint32), top_p=np.full(4, 0.97, np.float32))
+    for p in (0.05, 0.5, 0.95, 0.999, 0.9999999):
+        run(ctx, x, u, dtype, top_p=np.full(4, p, np.float32), min_p=np.array([0, 0.01, 0, 0.1], np.float32))
+
+
 def test_draws_follow_the_weights(ctx):
     # 4096 draws from one row: each count within five deviations of its share
     cols, rows = 50, 4096
