@@ -103,7 +103,7 @@ __device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t* marks) 
 // kHeld: a lane's entries (four at most) stay in registers from the counting to the placing.
 template <bool kHeld>
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs s) {
-    extern __shared__ uint32_t counts[];      // [warp][bin], then (kHeld) the CTA's entries in order
+    extern __shared__ __align__(16) uint32_t counts[];      // [warp][bin], then (kHeld) the CTA's entries in order
     __shared__ uint32_t totals[kMaxBins], bases[kMaxBins], begins[kMaxBins], fours[kSortThreads], red[kSortWarps + 1], red_cta[kSortWarps];
     fg_grid_enter();
     cg::cluster_group cluster = cg::this_cluster();
@@ -730,6 +730,7 @@ int32_t fg_embedding_fwd(fg_ctx* ctx, int32_t dtype, uint32_t tokens, uint32_t v
     FG_REQUIRE(ctx, fg_at_element(ids, 4) && fg_at_element(table, size) && fg_at_element(out, size),
                "fg_embedding_fwd: a tensor does not start at an element");
     FG_REQUIRE(ctx, !fg_ranges_meet(table, (uint64_t)vocab * dim * size, out, (uint64_t)tokens * dim * size), "fg_embedding_fwd: out overlaps the table");
+    FG_REQUIRE(ctx, !fg_ranges_meet(ids, 4ull * tokens, out, (uint64_t)tokens * dim * size), "fg_embedding_fwd: out overlaps ids");
     if (tokens == 0) return FG_OK;
     return FG_BY_DTYPE(dtype, embed_fwd, ctx, EmbedArgs{tokens, vocab, dim, ids, table, scale, out, 0});
 }
@@ -746,6 +747,7 @@ int32_t fg_embedding_bwd(fg_ctx* ctx, int32_t dtype, uint32_t tokens, uint32_t v
     FG_REQUIRE(ctx, fg_at_element(ids, 4) && fg_at_element(dout, size) && fg_at_element(dtable, size),
                "fg_embedding_bwd: a tensor does not start at an element");
     FG_REQUIRE(ctx, !fg_ranges_meet(dtable, (uint64_t)vocab * dim * size, dout, (uint64_t)tokens * dim * size), "fg_embedding_bwd: dtable overlaps dout");
+    FG_REQUIRE(ctx, !fg_ranges_meet(ids, 4ull * tokens, dtable, (uint64_t)vocab * dim * size), "fg_embedding_bwd: dtable overlaps ids");
     if (tokens == 0) {      // empty sums
         if (!accumulate) FG_CUDA(ctx, FG_ERR_FAILED_BUFFER_COPY, cudaMemsetAsync(dtable, 0, (uint64_t)vocab * dim * size, ctx->stream));
         return FG_OK;

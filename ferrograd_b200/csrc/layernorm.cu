@@ -724,6 +724,8 @@ int32_t fg_layernorm_fwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t col
                         fg_at_element(mean_out, 4) && fg_at_element(rstd_out, 4), "fg_layernorm_fwd: a tensor does not start at an element");
     const uint64_t bytes = (uint64_t)rows * cols * size;
     FG_REQUIRE(ctx, y == x || !fg_ranges_meet(x, bytes, y, bytes), "fg_layernorm_fwd: y overlaps x but is not x");
+    const uint64_t line = (uint64_t)cols * size;
+    FG_REQUIRE(ctx, !fg_ranges_meet(y, bytes, gamma, line) && !fg_ranges_meet(y, bytes, beta, line), "fg_layernorm_fwd: y overlaps gamma or beta");
     if (rows == 0) return FG_OK;
     return FG_BY_DTYPE(dtype, norm_fwd, ctx, NormArgs{x, gamma, beta, y, mean_out, rstd_out, rows, cols, eps});
 }
@@ -745,6 +747,12 @@ int32_t fg_layernorm_bwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t col
     const uint64_t bytes = (uint64_t)rows * cols * size;
     FG_REQUIRE(ctx, (dx == x || !fg_ranges_meet(x, bytes, dx, bytes)) && (dx == dy || !fg_ranges_meet(dy, bytes, dx, bytes)),
                "fg_layernorm_bwd: dx overlaps x or dy but is neither");
+    const uint64_t line = (uint64_t)cols * size;
+    FG_REQUIRE(ctx, !fg_ranges_meet(dx, bytes, gamma, line), "fg_layernorm_bwd: dx overlaps gamma");
+    for (const void* out : {dgamma, dbeta})
+        FG_REQUIRE(ctx, !fg_ranges_meet(out, line, x, bytes) && !fg_ranges_meet(out, line, dy, bytes) && !fg_ranges_meet(out, line, gamma, line) &&
+                            !fg_ranges_meet(out, line, dx, bytes), "fg_layernorm_bwd: a parameter's gradient overlaps another tensor");
+    FG_REQUIRE(ctx, !fg_ranges_meet(dgamma, line, dbeta, line), "fg_layernorm_bwd: dgamma overlaps dbeta");
     if (rows == 0) {      // empty sums
         if (dgamma && !accumulate_params) FG_CUDA(ctx, FG_ERR_FAILED_BUFFER_COPY, cudaMemsetAsync(dgamma, 0, (uint64_t)cols * size, ctx->stream));
         if (dbeta && !accumulate_params) FG_CUDA(ctx, FG_ERR_FAILED_BUFFER_COPY, cudaMemsetAsync(dbeta, 0, (uint64_t)cols * size, ctx->stream));

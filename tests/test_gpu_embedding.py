@@ -190,11 +190,11 @@ def test_empty_and_refusals(ctx):
         assert e.value.kind == "FG_ERR_INVALID_ARGUMENT"
 
     for kw in (dict(table=None), dict(ids=None), dict(out=None), dict(vocab=0), dict(dim=0), dict(table=p + 2), dict(ids=p + 514), dict(out=p + 257),
-               dict(out=p + 16), dict(vocab=1 << 31, dim=1 << 31)):
+               dict(out=p + 16), dict(vocab=1 << 31, dim=1 << 31), dict(ids=p + 260)):
         a = dict(table=p, ids=p + 512, out=p + 256, tokens=2, vocab=4, dim=4) | kw
         refuse(lambda: ctx.embedding_fwd(**a))
     for kw in (dict(dout=None), dict(ids=None), dict(dtable=None), dict(vocab=0), dict(dim=0), dict(dtable=p + 2), dict(ids=p + 514), dict(dout=p + 257),
-               dict(dtable=p + 272), dict(vocab=1 << 31, dim=1 << 31)):
+               dict(dtable=p + 272), dict(vocab=1 << 31, dim=1 << 31), dict(ids=p + 60), dict(tokens=1 << 31)):
         a = dict(ids=p + 512, dout=p + 256, dtable=p, tokens=2, vocab=4, dim=4) | kw
         refuse(lambda: ctx.embedding_bwd(**a))
     assert ctx.lib.fg_embedding_fwd(ctx.handle, 3, 1, 4, 4, p, p + 64, 1.0, p + 256) == 1

@@ -239,11 +239,12 @@ def test_refusals(ctx):
         assert e.value.kind == "FG_ERR_INVALID_ARGUMENT"
 
     for kw in (dict(x=None), dict(y=None), dict(cols=0), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")), dict(x=p + 2), dict(y=p + 1),
-               dict(mean=p + 2), dict(rows=1 << 31, cols=1 << 31), dict(y=p + 4), dict(gamma=p + 1)):
+               dict(mean=p + 2), dict(rows=1 << 31, cols=1 << 31), dict(y=p + 4), dict(gamma=p + 1), dict(gamma=p + 140), dict(beta=p + 120)):
         a = dict(x=p, gamma=None, beta=None, y=p + 128, rows=2, cols=4, eps=1e-5, mean=None) | kw
         refuse(lambda: ctx.layernorm_fwd(**a))
     for kw in (dict(x=None), dict(dy=None), dict(mean=None), dict(rstd=None), dict(cols=0), dict(dx=p + 4), dict(dx=p, accumulate_dx=True), dict(dx=p + 36),
-               dict(dgamma=p + 1), dict(rows=1 << 31, cols=1 << 31)):
+               dict(dgamma=p + 1), dict(rows=1 << 31, cols=1 << 31), dict(dx=None), dict(dgamma=p + 8), dict(dbeta=p + 40), dict(dgamma=p + 156), dict(gamma=p + 132),
+               dict(dgamma=p + 192, dbeta=p + 204), dict(gamma=p + 192, dgamma=p + 192)):
         a = dict(x=p, dy=p + 32, gamma=None, mean=p + 64, rstd=p + 80, rows=2, cols=4, dx=p + 128) | kw
         refuse(lambda: ctx.layernorm_bwd(**a))
     with pytest.raises(KeyError):
