@@ -100,6 +100,23 @@ __device__ void clear_absent(const SortArgs& s, uint32_t part, uint32_t* marks) 
     }
 }
 
+// Leaves in same[j] the lanes whose entry has this lane's digit.  Without a test per set of 32 entries: the ballots of several
+// bits are in flight together (a pass's placing of up to 32 entries per warp 2130 cycles, with the tests 3300; of 128 6150 and 6500).
+template <int kSets>
+__device__ __forceinline__ void same_digit(const uint2* e, unsigned* same, int shift, int digit) {
+    uint32_t d[kSets];
+#pragma unroll
+    for (int j = 0; j < kSets; ++j) d[j] = e[j].x >> shift;
+#pragma unroll 4
+    for (int b = 0; b < digit; ++b)
+#pragma unroll
+        for (int j = 0; j < kSets; ++j) {
+            const bool bit = d[j] >> b & 1u;
+            const unsigned ones = __ballot_sync(kFull, bit);
+            same[j] &= bit ? ones : ~ones;
+        }
+}
+
 // kHeld: a lane's entries (four at most) stay in registers from the counting to the placing.
 template <bool kHeld>
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs s) {
@@ -209,13 +226,10 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
             unsigned same[kAhead];      // the lanes with this digit, a bit at a time (one matching instruction takes as long as it finds values)
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) same[j] = __ballot_sync(kFull, i + 32 * j + lane < i1);
-            for (int b = 0; b < s.digit; ++b)
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j)
-                    if (i + 32 * j < i1) {
-                        const unsigned bit = e[j].x >> (shift + b) & 1u, ones = __ballot_sync(kFull, bit);
-                        same[j] &= bit ? ones : ~ones;
-                    }
+            const uint32_t sets = (min(i1 - i, 32u * kAhead) + 31) / 32;
+            if (sets == 1) same_digit<1>(e, same, shift, s.digit);
+            else if (sets == 2) same_digit<2>(e, same, shift, s.digit);
+            else same_digit<kAhead>(e, same, shift, s.digit);
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 if (i + 32 * j >= i1) break;
