@@ -3,8 +3,8 @@
 // The lookup copies rows and is bound by memory.  The gradient is a sum over the tokens of each id.  The tokens are sorted by id
 // (stably, so that the tokens of an id stand in their order), the sorted list is cut into chunks of one length, and a warp sums a chunk
 // for 16 bytes of columns per lane: however the ids fall, every warp has the same work.  Ids that lie in one chunk are done with that;
-// for an id that reaches over a border each chunk leaves its part in memory (f32), and the parts are added in their order.  Nothing
-// is added atomically.
+// for an id that reaches over a border each chunk leaves its part in memory (f32), and the warp that brings the last part adds
+// them in their order: only arrivals are counted atomically.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -45,6 +45,8 @@ struct SortArgs {
     char* dtable;             // rows that no token has, of those from `first_row` on, are cleared
     uint64_t row_bytes;
     uint32_t first_row;
+    uint32_t* arrived;        // counters of the second launch
+    uint64_t borders;
 };
 
 constexpr uint32_t kMaxGroup = 2048;     // rows that a block of the second launch marks
@@ -135,6 +137,7 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
     const uint32_t i0 = (uint32_t)min((uint64_t)s.tokens, (cta * kSortWarps + warp) * stretch), i1 = (uint32_t)min((uint64_t)s.tokens, i0 + stretch);
     uint32_t* const mine = counts + warp * bins;
     uint2* const staged = reinterpret_cast<uint2*>(counts + kSortWarps * bins);
+    for (uint64_t i = cta * kSortThreads + tid; i < s.borders; i += ctas * kSortThreads) s.arrived[i] = 0;
     for (int pass = 0; pass < s.passes; ++pass) {
         const uint2* const from = pass & 1 ? s.a : s.b;
         uint2* const to = pass & 1 ? s.b : s.a;
@@ -265,6 +268,7 @@ struct SumArgs {
     void *dtable, *dtable_end;
     float* parts;             // [chunks][2][pitch]: of the id that reaches in from the chunk before, and of the one that goes on in the next
     uint64_t pitch;
+    uint32_t* arrived;        // [chunks][tiles], zero at the start: parts there of the id that goes on behind the chunk
     float scale;
     uint32_t blocks, fills, group, fill_rows;      // blocks that sum, and blocks among them that clear 2^group rows each of the first fill_rows
     uint64_t row_bytes;
@@ -337,6 +341,59 @@ template <int E>
 __device__ __forceinline__ void store_part(float* p, const float (&x)[E]) {
 #pragma unroll
     for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(p + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+}
+
+// A part of an id that reaches over chunks, from `first` to `end`, is written.  The warp that brings the last one adds them, in their order
+// whoever it is, and nobody waits.  A launch of its own for that took 1.9 us of 31.1 (8192 tokens, 1024 f32 columns) and 2.1 of 114.0
+// (32768 tokens, 4096 bf16 columns).
+template <typename T, bool kShift, bool kAdd>
+__device__ __forceinline__ void join_parts(const SumArgs& s, uint32_t id, uint64_t first, uint64_t end, uint32_t tile, uint64_t col, uint32_t left, int lane) {
+    constexpr int E = FgPack<T>::E;
+    __threadfence();      // the part, before its arrival
+    __syncwarp();
+    uint32_t there = 0;
+    if (lane == 0) there = atomicAdd(&s.arrived[first * s.tiles + tile], 1u);
+    const uint64_t more = end - first;
+    if (__shfl_sync(kFull, there, 0) != more) return;
+    __threadfence();
+    float acc[E] = {};
+    if (left) {
+        const float* p = s.parts + (2 * first + 1) * s.pitch + col;      // its end of the first chunk, then the beginnings of the next ones
+        for (uint64_t j = 0; j <= more; j += 4) {
+            float4 v[4][E / 4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < E / 4; ++e)
+                    v[k][e] = j + k <= more ? __ldcg(reinterpret_cast<const float4*>(p + (j + k ? 2 * (j + k) - 1 : 0) * s.pitch + 4 * e)) : make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < E / 4; ++e) {
+                    acc[4 * e] += v[k][e].x; acc[4 * e + 1] += v[k][e].y; acc[4 * e + 2] += v[k][e].z; acc[4 * e + 3] += v[k][e].w;
+                }
+        }
+    }
+    store_sum<T, kShift, kAdd>(s, id, col, left, acc);
+}
+// The last chunk that the id behind chunk c's end reaches into; the first one that the id which reaches into chunk c began in.
+__device__ __forceinline__ uint64_t last_chunk_of(const SumArgs& s, uint32_t id, uint64_t c, int lane) {
+    const uint64_t size = 8ull * s.length;
+    while (true) {
+        const uint64_t at = (c + 1 + lane) * size;
+        const unsigned on = __ballot_sync(kFull, at < s.tokens && s.list[at].x == id);
+        if (on != kFull) return c + __ffs(~on) - 1;
+        c += 32;
+    }
+}
+__device__ __forceinline__ uint64_t first_chunk_of(const SumArgs& s, uint32_t id, uint64_t c, int lane) {
+    const uint64_t size = 8ull * s.length;
+    while (true) {
+        const uint64_t at = c > (uint64_t)lane ? (c - lane) * size : 0;      // 0: the list's beginning
+        const unsigned on = __ballot_sync(kFull, at && s.list[at - 1].x == id);
+        if (on != kFull) return c - (__ffs(~on) - 1);
+        c -= 32;
+    }
 }
 
 // A warp takes `length` entries and a tile of columns, with eight rows on their way while they are added one by one; the eight warps of a
@@ -430,15 +487,18 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(const SumArgs s) {
     // the id that reaches into the block.
     if (enters) {
         float sum[E] = {};
+        bool on = true;      // it goes on behind the chunk
         for (int w = 0; w < 8; ++w) {
 #pragma unroll
             for (int e = 0; e < E / 4; ++e) {
                 const float4 p = ends[w][e][lane];
                 sum[4 * e] += p.x; sum[4 * e + 1] += p.y; sum[4 * e + 2] += p.z; sum[4 * e + 3] += p.w;
             }
-            if (!through[w]) break;
+            on = through[w];
+            if (!on) break;
         }
         if (left) store_part(s.parts + 2 * chunk * s.pitch + col, sum);
+        join_parts<T, kShift, kAdd>(s, before, first_chunk_of(s, before, chunk, lane), on ? last_chunk_of(s, before, chunk, lane) : chunk, block % s.tiles, col, left, lane);
     }
     if (open && !reaches_in) {
         bool out = warp == 7;
@@ -451,60 +511,17 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(const SumArgs s) {
             if (!through[w]) break;
             out = w == 7;
         }
-        if (out) { if (left) store_part(s.parts + (2 * chunk + 1) * s.pitch + col, acc); }
-        else store_sum<T, kShift, kAdd>(s, after, col, left, acc);
+        if (out) {
+            if (left) store_part(s.parts + (2 * chunk + 1) * s.pitch + col, acc);
+            join_parts<T, kShift, kAdd>(s, after, chunk, last_chunk_of(s, after, chunk, lane), block % s.tiles, col, left, lane);
+        } else store_sum<T, kShift, kAdd>(s, after, col, left, acc);
     }
-}
-
-// The ids that reach over borders: the warp of the chunk that such an id begins in adds its parts.
-template <typename T, bool kShift, bool kAdd>
-__global__ void __launch_bounds__(256) embed_join_kernel(const SumArgs s) {
-    constexpr int E = FgPack<T>::E;
-    fg_grid_enter();
-    const int lane = threadIdx.x & 31;
-    const uint64_t unit = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5), chunk = unit / s.tiles, size = 8ull * s.length, last = (chunk + 1) * size - 1;
-    const uint32_t used = *s.used;
-    if (last + 1 >= used) return;
-    const uint32_t id = s.list[last].x, behind = s.list[last + 1].x;
-    if (behind != id) return;
-    const uint64_t i0 = chunk * size;
-    if (s.list[i0].x == id && i0 && s.list[i0 - 1].x == id) return;      // it began before this chunk
-    const uint64_t col = ((unit % s.tiles) * 32 + lane) * E;
-    const uint32_t left = col < s.dim ? (uint32_t)min((uint64_t)E, s.dim - col) : 0;
-    // how many chunks behind this one it reaches into: of each, the first entry tells
-    uint64_t more = 1;
-    while (true) {
-        const uint64_t at = (chunk + 1 + more + lane) * size;
-        const unsigned on = __ballot_sync(kFull, at < used && s.list[at].x == id);
-        more += on == kFull ? 32 : __ffs(~on) - 1;
-        if (on != kFull) break;
-    }
-    float acc[E] = {};
-    if (left) {
-        const float* p = s.parts + (2 * chunk + 1) * s.pitch + col;      // its end of this chunk, then the beginnings of the next ones
-        for (uint64_t j = 0; j <= more;) {
-            float4 v[4][E / 4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int e = 0; e < E / 4; ++e)
-                    v[k][e] = j + k <= more ? *reinterpret_cast<const float4*>(p + (j + k ? 2 * (j + k) - 1 : 0) * s.pitch + 4 * e) : make_float4(0, 0, 0, 0);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int e = 0; e < E / 4; ++e) {
-                    acc[4 * e] += v[k][e].x; acc[4 * e + 1] += v[k][e].y; acc[4 * e + 2] += v[k][e].z; acc[4 * e + 3] += v[k][e].w;
-                }
-            j += 4;
-        }
-    }
-    store_sum<T, kShift, kAdd>(s, id, col, left, acc);
 }
 
 // ---- few tokens ----
 // Up to kFew of them need no sorting: a block takes a token and two tiles of columns, finds by ballots where else its id stands, and if nowhere
 // before, adds those rows, four warps a quarter of them each where there are many.  Blocks behind these clear the other rows.  One launch
-// instead of three, added to the table: 129 tokens of 1024 f32 columns 16 -> 4 us, 256 of 777 25 -> 7, 512 of 1024 17 -> 10; from there on the
+// instead of several, added to the table: 129 tokens of 1024 f32 columns 16 -> 4 us, 256 of 777 25 -> 7, 512 of 1024 17 -> 10; from there on the
 // blocks of tokens that are not their id's first cost more than the sort.
 constexpr uint32_t kFew = 512;
 template <typename T, bool kShift, bool kAdd>
@@ -670,7 +687,8 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     s.chunks = ((uint64_t)a.tokens + 8ull * s.length - 1) / (8ull * s.length);
     const uint64_t list = ((uint64_t)a.tokens * 8 + 255) / 256 * 256;
     void* p;
-    const int32_t st = fg_ws_alloc(ctx, 2 * list + 256 + 8 * s.chunks * s.pitch, &p);
+    const uint64_t parts = 8 * s.chunks * s.pitch, blocks = s.chunks * s.tiles;
+    const int32_t st = fg_ws_alloc(ctx, 2 * list + 256 + parts + 4 * blocks, &p);
     if (st != FG_OK) return st;
     SortArgs o{};
     o.tokens = a.tokens;
@@ -680,6 +698,8 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     o.b = (uint2*)((char*)p + list);
     o.used = (uint32_t*)((char*)p + 2 * list);
     s.parts = (float*)((char*)p + 2 * list + 256);
+    s.arrived = o.arrived = (uint32_t*)((char*)s.parts + parts);
+    o.borders = blocks;
     int bits = 1;      // of the largest key, vocab
     while (bits < 32 && a.vocab >> bits) ++bits;
     o.passes = (bits + 8) / 9;
@@ -690,7 +710,6 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     while (ctas < 8 && (uint64_t)ctas * 1024 < a.tokens) ctas *= 2;
     const bool held = (uint64_t)ctas * kHeldEntries >= a.tokens;
     uint64_t fill = 0;
-    const uint64_t blocks = s.chunks * s.tiles;
     if (!a.accumulate) {
         // While the tokens are sorted (10 to 20 us) there is time to clear some 40 MB, beginning with the last rows, which are the rarest; the
         // other rows are cleared while the sums are made.
@@ -721,11 +740,6 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     fg_launch(ctx, add ? straight ? embed_sum_kernel<T, false, true> : embed_sum_kernel<T, true, true>
                        : straight ? embed_sum_kernel<T, false, false> : embed_sum_kernel<T, true, false>, (unsigned)(blocks + s.fills), 256, 0, s);
     FG_LAUNCHED(ctx);
-    if (s.chunks > 1) {
-        fg_launch(ctx, add ? straight ? embed_join_kernel<T, false, true> : embed_join_kernel<T, true, true>
-                           : straight ? embed_join_kernel<T, false, false> : embed_join_kernel<T, true, false>, (unsigned)((blocks + 7) / 8), 256, 0, s);
-        FG_LAUNCHED(ctx);
-    }
     return FG_OK;
 }
 
