@@ -726,6 +726,11 @@ int32_t fg_layernorm_fwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t col
     FG_REQUIRE(ctx, y == x || !fg_ranges_meet(x, bytes, y, bytes), "fg_layernorm_fwd: y overlaps x but is not x");
     const uint64_t line = (uint64_t)cols * size;
     FG_REQUIRE(ctx, !fg_ranges_meet(y, bytes, gamma, line) && !fg_ranges_meet(y, bytes, beta, line), "fg_layernorm_fwd: y overlaps gamma or beta");
+    const uint64_t column = 4ull * rows;
+    for (const void* out : {(const void*)mean_out, (const void*)rstd_out})
+        FG_REQUIRE(ctx, !fg_ranges_meet(out, column, x, bytes) && !fg_ranges_meet(out, column, y, bytes) && !fg_ranges_meet(out, column, gamma, line) &&
+                            !fg_ranges_meet(out, column, beta, line), "fg_layernorm_fwd: statistics overlap another tensor");
+    FG_REQUIRE(ctx, !fg_ranges_meet(mean_out, column, rstd_out, column), "fg_layernorm_fwd: mean_out overlaps rstd_out");
     if (rows == 0) return FG_OK;
     return FG_BY_DTYPE(dtype, norm_fwd, ctx, NormArgs{x, gamma, beta, y, mean_out, rstd_out, rows, cols, eps});
 }
@@ -753,6 +758,10 @@ int32_t fg_layernorm_bwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t col
         FG_REQUIRE(ctx, !fg_ranges_meet(out, line, x, bytes) && !fg_ranges_meet(out, line, dy, bytes) && !fg_ranges_meet(out, line, gamma, line) &&
                             !fg_ranges_meet(out, line, dx, bytes), "fg_layernorm_bwd: a parameter's gradient overlaps another tensor");
     FG_REQUIRE(ctx, !fg_ranges_meet(dgamma, line, dbeta, line), "fg_layernorm_bwd: dgamma overlaps dbeta");
+    const uint64_t column = 4ull * rows;
+    for (const void* in : {(const void*)mean, (const void*)rstd})
+        FG_REQUIRE(ctx, !fg_ranges_meet(in, column, dx, bytes) && !fg_ranges_meet(in, column, dgamma, line) && !fg_ranges_meet(in, column, dbeta, line),
+                   "fg_layernorm_bwd: a gradient overlaps the statistics");
     if (rows == 0) {      // empty sums
         if (dgamma && !accumulate_params) FG_CUDA(ctx, FG_ERR_FAILED_BUFFER_COPY, cudaMemsetAsync(dgamma, 0, (uint64_t)cols * size, ctx->stream));
         if (dbeta && !accumulate_params) FG_CUDA(ctx, FG_ERR_FAILED_BUFFER_COPY, cudaMemsetAsync(dbeta, 0, (uint64_t)cols * size, ctx->stream));

@@ -776,6 +776,13 @@ extern "C" int32_t fg_sample(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t
     FG_REQUIRE(ctx, fg_at_element(logits, fg_dtype_size(dtype)) && fg_at_element(u, 4) && fg_at_element(temperature, 4) && fg_at_element(top_k, 4) &&
                         fg_at_element(top_p, 4) && fg_at_element(min_p, 4) && fg_at_element(token_out, 4) && fg_at_element(prob_out, 4),
                "fg_sample: a tensor does not start at an element");
+    const uint64_t line = 4ull * rows;
+    for (const void* out : {(const void*)token_out, (const void*)prob_out}) {
+        bool meets = fg_ranges_meet(out, line, logits, (uint64_t)rows * cols * fg_dtype_size(dtype)) || fg_ranges_meet(out, line, u, line);
+        for (const void* in : {(const void*)temperature, (const void*)top_k, (const void*)top_p, (const void*)min_p}) meets = meets || fg_ranges_meet(out, line, in, line);
+        FG_REQUIRE(ctx, !meets, "fg_sample: an output overlaps an input");
+    }
+    FG_REQUIRE(ctx, !fg_ranges_meet(token_out, line, prob_out, line), "fg_sample: token_out overlaps prob_out");
     if (rows == 0) return FG_OK;
     return FG_BY_DTYPE(dtype, sample, ctx, SampleArgs{logits, u, temperature, top_k, top_p, min_p, token_out, prob_out, rows, cols});
 }

@@ -312,7 +312,8 @@ int32_t fg_layernorm_fwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t col
  *   dgamma [cols] = column sums of dy * h                    (skipped when NULL)
  *   dbeta  [cols] = column sums of dy                        (skipped when NULL; one of the three is wanted)
  * accumulate_dx adds into dx and accumulate_params into dgamma and dbeta instead of overwriting them.  Sums are in
- * f32 in an order that the sizes alone decide.  dx may be dy or x (then without accumulate_dx). */
+ * f32 in an order that the sizes alone decide.  dx may be dy or x (then without accumulate_dx); any other overlap of an
+ * output with a tensor of the call is refused, here and in the forward pass. */
 int32_t fg_layernorm_bwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* x, const void* dy,
                          const void* gamma, const float* mean, const float* rstd, void* dx, void* dgamma,
                          void* dbeta, int32_t accumulate_dx, int32_t accumulate_params);
@@ -340,7 +341,7 @@ int32_t fg_embedding_bwd(fg_ctx* ctx, int32_t dtype, uint32_t tokens, uint32_t v
  * [rows], read when the kernel runs; NULL: 1, 0, 1, 0.  A temperature of 0 or less, or NaN, takes the first maximum, with
  * probability 1; NaN in another parameter keeps all; u below 0 or NaN counts as 0, of 1 or more as just below 1.
  * Weights are whole multiples of 2^-42 and their sums exact, so the token does not depend on the order of a sum.
- * cols <= FG_SAMPLE_MAX_COLS. */
+ * cols <= FG_SAMPLE_MAX_COLS.  An output that overlaps another tensor is refused. */
 #define FG_NO_TOKEN 0xffffffffu
 #define FG_SAMPLE_MAX_COLS 2097152u
 int32_t fg_sample(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* logits, const float* u,

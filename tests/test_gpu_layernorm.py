@@ -251,3 +251,20 @@ def test_refusals(ctx):
         ctx.layernorm_fwd(p, None, None, p, 1, 4, dtype="f64")
     assert ctx.lib.fg_layernorm_fwd(ctx.handle, 3, 1, 4, p, None, None, 1e-5, p, None, None) == 1
     assert ctx.lib.fg_layernorm_bwd(ctx.handle, -1, 1, 4, p, p, None, p, p, p, None, None, 0, 0) == 1
+
+
+def test_statistics_that_overlap_are_refused(ctx):
+    from ferrograd_b200 import FgError
+    p = ctx.new_tensor((64,)).ptr      # x: 32 bytes at 0, y or dx at 128, lines of 16 bytes
+    forward = dict(x=p, gamma=p + 64, beta=p + 80, y=p + 128, rows=2, cols=4, mean=p + 192, rstd=p + 200)
+    for kw in (dict(mean=p + 28), dict(mean=p + 124), dict(rstd=p + 156), dict(mean=p + 76), dict(rstd=p + 92), dict(rstd=p + 196), dict(mean=p + 200)):
+        with pytest.raises(FgError) as e:
+            ctx.layernorm_fwd(**(forward | kw))
+        assert e.value.kind == "FG_ERR_INVALID_ARGUMENT"
+    ctx.layernorm_fwd(**forward)
+    backward = dict(x=p, dy=p + 32, gamma=None, mean=p + 192, rstd=p + 200, rows=2, cols=4, dx=p + 128, dgamma=p + 160, dbeta=p + 176)
+    for kw in (dict(mean=p + 156), dict(rstd=p + 124), dict(mean=p + 172), dict(rstd=p + 188)):
+        with pytest.raises(FgError) as e:
+            ctx.layernorm_bwd(**(backward | kw))
+        assert e.value.kind == "FG_ERR_INVALID_ARGUMENT"
+    ctx.layernorm_bwd(**backward)

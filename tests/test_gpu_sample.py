@@ -233,3 +233,18 @@ def test_empty_and_refusals(ctx):
                dict(temperature=p + 1), dict(top_k=p + 2), dict(top_p=p + 3), dict(min_p=p + 6), dict(prob=p + 6)):
         refuse(**kw)
     assert ctx.lib.fg_sample(ctx.handle, 3, 1, 4, p, p, None, None, None, None, p, None) == 1
+
+
+def test_outputs_that_overlap_are_refused(ctx):
+    from ferrograd_b200 import FgError
+    p = ctx.new_tensor((64,)).ptr      # 2 x 4 logits: 32 bytes; the others 8 bytes each
+    given = dict(logits=p, u=p + 32, token=p + 128, rows=2, cols=4, temperature=p + 40, top_k=p + 48, top_p=p + 56, min_p=p + 64, prob=p + 136)
+    for at in (0, 28, 32, 36, 44, 52, 60, 68):
+        for out in ("token", "prob"):
+            with pytest.raises(FgError) as e:
+                ctx.sample(**(given | {out: p + at}))
+            assert e.value.kind == "FG_ERR_INVALID_ARGUMENT"
+    for kw in (dict(prob=p + 128), dict(prob=p + 132), dict(token=p + 140)):
+        with pytest.raises(FgError):
+            ctx.sample(**(given | kw))
+    ctx.sample(**given)
