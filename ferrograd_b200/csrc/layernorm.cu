@@ -79,10 +79,10 @@ template <typename T_, int kPacks, bool kFull, int kTensors>
 struct Straight {
     using T = T_;
     static constexpr int E = FgPack<T>::E, P = E / 2, N = kPacks * E, kStages = stages_of(kTensors * kPacks);
-    static constexpr bool kAhead = true, kTight = false;
+    static constexpr bool kAhead = true, kTight = false, kApart = false;
     uint32_t slots, block, offset, pitch, have;      // shared address of the thread's first slot, bytes of a block's packs, of the thread, of a group's packs
     uint32_t put = 0, take = 0;                      // stages
-    __device__ __forceinline__ Straight(const Group& g, uint32_t cols, const void* shared) {
+    __device__ __forceinline__ Straight(const Group& g, uint32_t cols, uint32_t, const void* shared) {
         slots = (uint32_t)__cvta_generic_to_shared(shared) + threadIdx.x * 16;
         block = blockDim.x * 16;
         offset = g.thread * 16;
@@ -122,6 +122,7 @@ struct Straight {
             spread(k, w, v);
         }
     }
+    __device__ __forceinline__ void parameter(const T* p, float2 (&v)[N / 2]) const { load(p, v); }
     // A parameter's columns, kept for all rows (of up to 4 packs: read from the L1 and, where slots leave it little room, from the L2 for every
     // row, they cost a fifth of the time).
     static constexpr bool kKeep = kPacks <= 4;
@@ -162,18 +163,149 @@ struct Straight {
     }
 };
 
-// Any other row: a thread has the elements `thread`, `thread` + threads, ... of it.  (Taking 16-byte words through shared memory and turning them by
-// the row's distance from the boundary is no faster: what turning and the ends of rows take is what addresses and tests take here; 30000 x 777 f16
-// forward 53 us and 54, backward 85 and 72.)
+// Rows of any length in tensors that start on 16-byte boundaries.  The distance of a row's start from a boundary comes back every E rows at the
+// latest, so if the rows of a group, and of all groups of a block, lie a multiple of that apart (kApart: they are a grid apart), it is one number
+// for them, and the thread's words hold the same columns of every row.  The words at a row's ends are shared with other rows.
+// Against single elements, forward and backward, us: 4099 x 1001 f16 9.4 and 14.2 (10.3 and 18.0), 30000 x 777 f16 34.5 and 49.1 (53.6 and
+// 72.1), 3000 x 5001 f32 35.9 and 45.5 (73.6 and 162), 10000 x 4097 bf16 80.6 and 91.9 (137 and 178).  What is over the time of rows that lie
+// straight (30000 x 776: 24.7 and 41.8) are the ends: the warps that have one mask it and store it by elements (a lane per element was no faster).
+template <typename T_, int kPacks, int kTensors>
+struct Shifted {
+    using T = T_;
+    static constexpr int E = FgPack<T>::E, P = E / 2, N = kPacks * E, kStages = stages_of(kTensors * kPacks);
+    static constexpr bool kAhead = true, kTight = false, kApart = true;
+    static constexpr uint32_t kAll = N == 32 ? ~0u : (1u << (N & 31)) - 1, kWord = (1u << E) - 1;
+    uint32_t slots, block, pitch, valid = 0, tail, tail_bytes;      // valid: a bit per element that belongs to the row; tail: which pack is the row's last word
+    uint32_t head[4];                                               // what the first pack has of the row
+    int32_t column;                                                 // of the first element; negative where it belongs to the row before
+    uint32_t put = 0, take = 0;
+    __device__ __forceinline__ Shifted(const Group& g, uint32_t cols, uint32_t first, const void* shared) {
+        slots = (uint32_t)__cvta_generic_to_shared(shared) + threadIdx.x * 16;
+        block = blockDim.x * 16;
+        pitch = g.threads * E;
+        const uint32_t off = (uint32_t)((uint64_t)first * cols % E), last = (off + cols - 1) / E;
+        column = (int32_t)(g.thread * E) - (int32_t)off;
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            const uint32_t w = g.thread + k * g.threads;
+            uint32_t bits = w > last ? 0 : w == last ? (2u << ((off + cols - 1) & (E - 1))) - 1 : kWord;
+            if (w == 0) bits &= ~((1u << off) - 1);
+            valid |= bits << (k * E);
+        }
+        tail = last % g.threads == (uint32_t)g.thread ? last / g.threads : kPacks;
+        tail_bytes = (((off + cols - 1) & (E - 1)) + 1) * sizeof(T);
+        const uint32_t cut = g.thread == 0 ? off * sizeof(T) : 0;      // bytes of the row before
+#pragma unroll
+        for (int i = 0; i < 4; ++i) head[i] = cut <= 4 * i ? ~0u : cut >= 4 * i + 4 ? 0u : 0xffff0000u;
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k)
+            if (!has(k))
+                for (int i = 0; i < kStages * kTensors; ++i) fg_store_shared(slots + (i * kPacks + k) * block, make_uint4(0, 0, 0, 0));
+    }
+    __device__ __forceinline__ bool has(int k) const { return valid >> (k * E) & kWord; }
+    __device__ __forceinline__ bool whole(int k) const { return (valid >> (k * E) & kWord) == kWord; }
+    __device__ __forceinline__ bool bit(int i) const { return valid >> i & 1u; }
+    __device__ __forceinline__ uint32_t slot(uint32_t stage, int t, int k) const { return slots + ((stage * kTensors + t) * kPacks + k) * block; }
+    __device__ __forceinline__ void ask(int t, const T* row) {      // nothing behind the row, which may be the tensor's last
+        const T* const p = row + column;
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k)
+            if (has(k)) fg_copy_async(slot(put, t, k), p + k * pitch, (uint32_t)k == tail ? tail_bytes : 16);
+    }
+    __device__ __forceinline__ void asked() {
+        fg_copies_end();
+        put = put == kStages - 1 ? 0 : put + 1;
+    }
+    __device__ __forceinline__ void arrived() const { fg_copies_wait<kStages - 1>(); }
+    __device__ __forceinline__ void taken() { take = take == kStages - 1 ? 0 : take + 1; }
+    __device__ __forceinline__ void spread(const uint4& w, int k, float2 (&v)[N / 2]) const {
+        float2 x[P];
+        FgPack<T>::widen(w, x);
+#pragma unroll
+        for (int e = 0; e < P; ++e) v[k * P + e] = x[e];
+    }
+    __device__ __forceinline__ void mask(float2 (&v)[N / 2]) const {
+        if (valid != kAll)      // the ends of rows
+#pragma unroll
+            for (int k = 0; k < kPacks; ++k)
+                if (!whole(k))
+#pragma unroll
+                    for (int i = k * P; i < (k + 1) * P; ++i) v[i] = make_float2(bit(2 * i) ? v[i].x : 0.0f, bit(2 * i + 1) ? v[i].y : 0.0f);
+    }
+    __device__ __forceinline__ void get(int t, const T*, float2 (&v)[N / 2]) const {
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {      // zero outside of the row: packs and parts of packs behind it never arrive
+            uint4 w = fg_load_shared(slot(take, t, k));
+            if (k == 0) w = make_uint4(w.x & head[0], w.y & head[1], w.z & head[2], w.w & head[3]);
+            spread(w, k, v);
+        }
+    }
+    __device__ __forceinline__ void elements(const T* p, int k, float2 (&v)[N / 2]) const {      // p: the pack's first
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float x = bit(k * E + e) ? fg_widen(p[e]) : 0.0f;
+            if (e & 1) v[k * P + e / 2].y = x;
+            else v[k * P + e / 2].x = x;
+        }
+    }
+    __device__ __forceinline__ void load(const T* row, float2 (&v)[N / 2]) const {
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            const T* const p = row + column + (int64_t)(k * pitch);
+            if (whole(k)) spread(*reinterpret_cast<const uint4*>(p), k, v);
+            else elements(p, k, v);
+        }
+    }
+    // Parameters lie as they like; they are read once.
+    __device__ __forceinline__ void parameter(const T* p, float2 (&v)[N / 2]) const {
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) elements(p + column + (int64_t)(k * pitch), k, v);
+    }
+    struct Kept { uint4 w[kPacks]; };
+    __device__ __forceinline__ void keep(const T* p, Kept& kept) const {
+        float2 v[N / 2];
+        parameter(p, v);
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) kept.w[k] = pack(v, k);
+    }
+    __device__ __forceinline__ void kept(const Kept& kept, const T*, float2 (&v)[N / 2]) const {
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) spread(kept.w[k], k, v);
+    }
+    static __device__ __forceinline__ uint4 pack(const float2 (&v)[N / 2], int k) {
+        float2 x[P];
+#pragma unroll
+        for (int e = 0; e < P; ++e) x[e] = v[k * P + e];
+        return FgPack<T>::narrow(x);
+    }
+    __device__ __forceinline__ void store(T* row, const float2 (&v)[N / 2]) const {
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            T* const p = row + column + (int64_t)(k * pitch);
+            if (whole(k)) *reinterpret_cast<uint4*>(p) = pack(v, k);
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (bit(k * E + e)) p[e] = fg_narrow<T>(e & 1 ? v[k * P + e / 2].y : v[k * P + e / 2].x);
+        }
+    }
+    __device__ __forceinline__ void store_sums(float* row, const float2 (&v)[N / 2]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (bit(i)) row[column + (int64_t)((i / E) * pitch) + i % E] = i & 1 ? v[i / 2].y : v[i / 2].x;
+    }
+};
+
+// Any other row (tensors off 16-byte boundaries, and short rows forward): a thread has the elements `thread`, `thread` + threads, ... of it.
 template <typename T_, int kCount, int kTensors>
 struct Ragged {
     using T = T_;
     static constexpr int N = kCount, kStages = 1;
     static constexpr bool kAhead = kTensors * kCount <= 8;       // the next row's elements are on their way, in registers
-    static constexpr bool kTight = kCount <= 8;                  // 64 registers, for 1024 threads an SM
+    static constexpr bool kTight = kCount <= 8, kApart = false;  // kTight: 64 registers, for 1024 threads an SM
     uint32_t thread, threads, cols;
     T next[kAhead ? kTensors : 1][kAhead ? N : 1];
-    __device__ __forceinline__ Ragged(const Group& g, uint32_t cols_, const void*) : thread(g.thread), threads(g.threads), cols(cols_) {}
+    __device__ __forceinline__ Ragged(const Group& g, uint32_t cols_, uint32_t, const void*) : thread(g.thread), threads(g.threads), cols(cols_) {}
     __device__ __forceinline__ void ask(int t, const T* row) {
         if constexpr (kAhead)
 #pragma unroll
@@ -201,6 +333,7 @@ struct Ragged {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fg_widen(w[2 * i]), fg_widen(w[2 * i + 1]));
     }
+    __device__ __forceinline__ void parameter(const T* p, float2 (&v)[N / 2]) const { load(p, v); }
     static constexpr bool kKeep = kCount <= 16;
     struct Kept { T w[kKeep ? N : 1]; };
     __device__ __forceinline__ void keep(const T* p, Kept& kept) const {
@@ -243,8 +376,9 @@ __global__ void __launch_bounds__(kMaxThreads, C::kTight && C::N <= 16 ? 2 : 1) 
     __shared__ float red[kMaxGroups][4][32];
     fg_grid_enter();
     const Group group(threads);
-    C columns(group, a.cols, shared);
-    const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups, first = blockIdx.x * groups + group.index;
+    const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups;
+    const uint32_t first = C::kApart ? group.index * gridDim.x + blockIdx.x : blockIdx.x * groups + group.index;
+    C columns(group, a.cols, first, shared);
     const float n = (float)a.cols, inv_n = 1.0f / n;
     const T *const gamma = static_cast<const T*>(a.gamma), *const beta = static_cast<const T*>(a.beta);
     typename C::Kept gammas, betas;
@@ -321,12 +455,13 @@ __global__ void __launch_bounds__(kMaxThreads, C::kTight && C::N <= 4 ? 2 : 1) n
     __shared__ float red[kMaxGroups][2][32];
     fg_grid_enter();
     const Group group(threads);
-    C columns(group, a.cols, shared);
-    const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups, first = blockIdx.x * groups + group.index;
+    const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups;
+    const uint32_t first = C::kApart ? group.index * gridDim.x + blockIdx.x : blockIdx.x * groups + group.index;
+    C columns(group, a.cols, first, shared);
     const float inv_n = 1.0f / (float)a.cols;
     const T* const gamma = static_cast<const T*>(a.gamma);
     float2 gm[H];
-    if (gamma) columns.load(gamma, gm);
+    if (gamma) columns.parameter(gamma, gm);
     else
 #pragma unroll
         for (int i = 0; i < H; ++i) gm[i] = make_float2(1.0f, 1.0f);
@@ -364,8 +499,7 @@ __global__ void __launch_bounds__(kMaxThreads, C::kTight && C::N <= 4 ? 2 : 1) n
         if (r + step < a.rows) { mean = a.mean[r + step]; rstd = a.rstd[r + step]; }
         if (C::kAhead) ask();
 #pragma unroll
-        for (int i = 0; i < H; ++i) c[i] = fg_add2(c[i], less);
-        columns.mask(c);      // (dy is zero there)
+        for (int i = 0; i < H; ++i) c[i] = fg_add2(c[i], less);      // (columns that are not there: dy is zero)
         float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
 #pragma unroll
         for (int i = 0; i < H; ++i) {
@@ -599,6 +733,19 @@ HeldPlan held_plan(const fg_ctx* ctx, uint32_t rows, uint64_t units, int least, 
     p.grid = (int)(need < cap ? need : cap);
     return p;
 }
+// The same for rows that begin anywhere in a word: a grid of as many blocks as bring a row's start back to its place in one.
+template <typename T>
+HeldPlan shifted_plan(const fg_ctx* ctx, uint32_t rows, uint32_t cols, int usual, int most, int tensors) {
+    constexpr uint32_t E = FgPack<T>::E;
+    HeldPlan p = held_plan(ctx, rows, ((uint64_t)cols + 2 * E - 2) / E, 1, usual, most, tensors, 512);
+    if (!p.threads) return p;
+    int period = 1;
+    while ((uint64_t)period * cols % E) period *= 2;
+    const bool all = (uint64_t)p.grid * p.groups >= rows;      // a row each: some blocks more
+    p.grid = (p.grid + (all ? period - 1 : 0)) / period * period;
+    if (p.grid == 0) p.grid = period;
+    return p;
+}
 // More shared memory than a kernel may have by default, once per kernel (`done`) and device.
 template <typename K>
 int32_t allow_shared(fg_ctx* ctx, std::atomic<uint64_t>& done, K kernel, size_t bytes) {
@@ -630,6 +777,12 @@ int32_t norm_fwd(fg_ctx* ctx, const NormArgs& a) {
             return p.units == 1 ? launch_straight<T, 1>(ctx, a, p) : p.units == 2 ? launch_straight<T, 2>(ctx, a, p)
                    : p.units == 4 ? launch_straight<T, 4>(ctx, a, p) : launch_straight<T, 8>(ctx, a, p);
     } else {
+        // Rows that a warp holds by four elements a lane (eight of f32) are faster so: 20000 x 81 bf16 7.0 us against 9.6, 20000 x 201 f32 10.3 against 11.0.
+        if (a.cols > 64 * sizeof(T) && fg_aligned16(a.x) && fg_aligned16(a.y)) {
+            const HeldPlan p = shifted_plan<T>(ctx, a.rows, a.cols, usual, 4, 1);
+            if (p.threads)
+                return p.units == 1 ? launch_held<Shifted<T, 1, 1>>(ctx, a, p) : p.units == 2 ? launch_held<Shifted<T, 2, 1>>(ctx, a, p) : launch_held<Shifted<T, 4, 1>>(ctx, a, p);
+        }
         HeldPlan p = held_plan(ctx, a.rows, a.cols, 4, 8, 32, 0, 1024);
         if (p.threads)
             return p.units == 4 ? launch_held<Ragged<T, 4, 1>>(ctx, a, p) : p.units == 8 ? launch_held<Ragged<T, 8, 1>>(ctx, a, p)
@@ -663,7 +816,11 @@ template <typename T>
 int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
     constexpr int usual = 16 / FgPack<T>::E;
     const bool straight = fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.dy, a.gamma, a.dx);
-    const HeldPlan p = straight ? held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 1, usual, usual, 2, 512) : held_plan(ctx, a.rows, a.cols, 4, 4, 16, 0, 1024);
+    HeldPlan p{};
+    if (straight) p = held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 1, usual, usual, 2, 512);
+    else if (fg_aligned16(a.x) && fg_aligned16(a.dy) && fg_aligned16(a.dx)) p = shifted_plan<T>(ctx, a.rows, a.cols, usual, usual, 2);
+    const bool shifted = !straight && p.threads;
+    if (!straight && !shifted) p = held_plan(ctx, a.rows, a.cols, 4, 4, 16, 0, 1024);
     if (p.threads) {
         float* parts = nullptr;
         const uint32_t pitch = (a.cols + 127) / 128 * 128;
@@ -678,6 +835,10 @@ int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
             if (p.units == 1) s = launch_bwd_straight<T, 1>(ctx, a, p, parts, pitch);
             else if (p.units == 2) s = launch_bwd_straight<T, 2>(ctx, a, p, parts, pitch);
             else s = launch_bwd_straight<T, usual>(ctx, a, p, parts, pitch);
+        } else if (shifted) {
+            if (p.units == 1) s = launch_bwd_held<Shifted<T, 1, 2>>(ctx, a, p, parts, pitch);
+            else if (p.units == 2) s = launch_bwd_held<Shifted<T, 2, 2>>(ctx, a, p, parts, pitch);
+            else s = launch_bwd_held<Shifted<T, usual, 2>>(ctx, a, p, parts, pitch);
         } else if (p.units == 4) s = launch_bwd_held<Ragged<T, 4, 2>>(ctx, a, p, parts, pitch);
         else if (p.units == 8) s = launch_bwd_held<Ragged<T, 8, 2>>(ctx, a, p, parts, pitch);
         else s = launch_bwd_held<Ragged<T, 16, 2>>(ctx, a, p, parts, pitch);

@@ -35,10 +35,17 @@ __device__ __forceinline__ void fg_group_barrier(int group, int threads) { asm v
 __device__ __forceinline__ void fg_copy_async(uint32_t to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+// The first `bytes` of them, zeros behind.
+__device__ __forceinline__ void fg_copy_async(uint32_t to, const void* from, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ uint4 fg_load_shared(uint32_t from) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
     return v;
+}
+__device__ __forceinline__ void fg_store_shared(uint32_t to, const uint4& v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ void fg_copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft>      // all but the last kLeft groups have arrived

@@ -268,3 +268,56 @@ def test_statistics_that_overlap_are_refused(ctx):
             ctx.layernorm_bwd(**(backward | kw))
         assert e.value.kind == "FG_ERR_INVALID_ARGUMENT"
     ctx.layernorm_bwd(**backward)
+
+
+# Rows whose starts lie at 8, 4, 2 places of a 16-byte word, more of them than are worked on at a time, and a word or an element over a border.
+RAGGED = [("f16", 6001, 129), ("bf16", 5003, 257), ("f16", 2501, 1001), ("bf16", 3001, 1002), ("f16", 3000, 1004), ("bf16", 1203, 4097), ("f16", 700, 8191),
+          ("f32", 5003, 257), ("f32", 2600, 777), ("f32", 1300, 1002), ("f32", 701, 4099), ("bf16", 4001, 5), ("f32", 3001, 1), ("bf16", 650, 9001)]
+
+
+@pytest.mark.parametrize("dtype,rows,cols", RAGGED)
+def test_many_ragged_rows(ctx, dtype, rows, cols):
+    x, dy, gamma, beta = make(rows, cols, dtype)
+    xd, dyd, gd, bd = Placed(ctx, x, dtype), Placed(ctx, dy, dtype), Placed(ctx, gamma, dtype, 1), Placed(ctx, beta, dtype, 3)
+    y, mean, rstd = empty(ctx, x.shape, dtype), empty(ctx, (rows,)), empty(ctx, (rows,))
+    ctx.layernorm_fwd(xd, gd, bd, y, rows, cols, mean=mean, rstd=rstd, dtype=dtype)
+    check_forward(y.get(), mean.get(), rstd.get(), x, gamma, beta, 1e-5, dtype)
+    outs = run_backward(ctx, dtype, x, dy, gamma, mean.get(), rstd.get(), xd, dyd, gd, mean, rstd, 0)
+    # in place: words at the ends of rows are read for one row while another's elements are written
+    over = Placed(ctx, x, dtype)
+    ctx.layernorm_fwd(over, gd, bd, over, rows, cols, dtype=dtype)
+    assert np.array_equal(over.bits(), y.bits())
+    for place in range(2):
+        a = [Placed(ctx, x, dtype), Placed(ctx, dy, dtype)]
+        dg, db = empty(ctx, (cols,), dtype), empty(ctx, (cols,), dtype, 1)
+        ctx.layernorm_bwd(*a, gd, mean, rstd, rows, cols, dx=a[place], dgamma=dg, dbeta=db, dtype=dtype)
+        for got, want in zip((a[place], dg, db), outs):
+            assert np.array_equal(got.bits(), want.bits())
+    # dx alone, and added to
+    base = rounded(np.full(x.shape, 0.75), dtype)
+    alone, added = empty(ctx, x.shape, dtype), Placed(ctx, base, dtype)
+    ctx.layernorm_bwd(xd, dyd, gd, mean, rstd, rows, cols, dx=alone, dtype=dtype)
+    ctx.layernorm_bwd(xd, dyd, gd, mean, rstd, rows, cols, dx=added, accumulate_dx=True, dtype=dtype)
+    want, bound = backward64(x, dy, gamma, mean.get(), rstd.get())[0], bounds(x, dy, gamma, mean.get(), rstd.get(), dtype)[0]
+    check(alone.get(), want, bound, "dx alone")
+    check(added.get(), want + 0.75, bound + 2 * HALF_ULP[dtype] * (0.75 + np.abs(want)), "dx added")
+
+
+@pytest.mark.parametrize("dtype,rows,cols", [("f16", 2500, 1001), ("bf16", 3001, 257), ("f32", 1300, 777), ("bf16", 640, 4097), ("f32", 900, 3), ("f16", 40, 9)])
+def test_ragged_rows_beside_values_out_of_the_ordinary(ctx, dtype, rows, cols):
+    # every third row is inf or NaN: the others come out as if it were not
+    x, dy, gamma, beta = make(rows, cols, dtype)
+    gd, bd = Placed(ctx, gamma, dtype), Placed(ctx, beta, dtype)
+
+    def run(x, dy):
+        xd, dyd = Placed(ctx, x, dtype), Placed(ctx, dy, dtype)
+        y, dx, mean, rstd = empty(ctx, x.shape, dtype), empty(ctx, x.shape, dtype), empty(ctx, (rows,)), empty(ctx, (rows,))
+        ctx.layernorm_fwd(xd, gd, bd, y, rows, cols, mean=mean, rstd=rstd, dtype=dtype)
+        ctx.layernorm_bwd(xd, dyd, gd, mean, rstd, rows, cols, dx=dx, dtype=dtype)
+        return [t.bits().copy() for t in (y, dx, mean, rstd)]
+
+    plain = run(x, dy)
+    bad, bad_dy = x.copy(), dy.copy()
+    bad[0::3], bad_dy[0::3] = np.where(np.arange(len(bad[0::3]))[:, None] % 2, np.inf, np.nan), np.nan
+    for a, b in zip(plain, run(bad, bad_dy)):
+        assert np.array_equal(a[1::3], b[1::3]) and np.array_equal(a[2::3], b[2::3])
