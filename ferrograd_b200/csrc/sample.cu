@@ -138,7 +138,7 @@ struct Border { uint32_t key; uint64_t above, at; };      // the sum over larger
 
 struct Shared {
     double roots[256];
-    uint64_t hist[2][256];
+    alignas(8) uint32_t hist[2][3][256];  // parts of sums
     uint64_t slots[2][2];                 // what a CTA tells the others
     uint64_t red[kWarps], red2[kWarps];
     alignas(16) uint32_t bins[kBins];
@@ -151,6 +151,7 @@ struct Shared {
 template <typename T>
 struct HeldSlice {      // a slice in shared memory, by 16-byte words; masked where a word reaches over the slice's ends
     static constexpr int kPer = FgPack<T>::E;
+    static constexpr bool kLong = false;  // 180 KB: fewer than 2^17 elements
     const uint4* words;
     uint32_t units, column;               // of the first word's first element (it may lie before the slice)
     __device__ __forceinline__ void values(uint32_t u, float (&x)[kPer]) const { FgPack<T>::widen(words[u], x); }
@@ -161,6 +162,7 @@ struct HeldSlice {      // a slice in shared memory, by 16-byte words; masked wh
 template <typename T>
 struct FarSlice {       // a slice that shared memory does not hold
     static constexpr int kPer = 1;
+    static constexpr bool kLong = true;
     const T* data;
     uint32_t units, column;
     __device__ __forceinline__ void values(uint32_t u, float (&x)[1]) const { x[0] = fg_widen(data[u]); }
@@ -171,6 +173,7 @@ struct FarSlice {       // a slice that shared memory does not hold
 template <typename T>
 struct List {           // entries (key, column)
     static constexpr int kPer = 1;
+    static constexpr bool kLong = false;
     const uint2* entries;
     uint32_t units;
     __device__ __forceinline__ void values(uint32_t u, float (&x)[1]) const { x[0] = logit_of<T>(entries[u].x); }
@@ -254,8 +257,8 @@ __device__ Border find_border(Team& team, const S& source, const Weights<T>& w, 
     Border at{};
     for (int round = 0; round < 5; ++round) {      // 32 bits of range, eight less after each
         const int bits = 32 - __clz(hi - lo), shift = bits > 8 ? bits - 8 : 0;
-        uint64_t* const hist = sh.hist[team.round ^= 1];
-        hist[tid] = 0;
+        uint32_t (*const hist)[256] = sh.hist[team.round ^= 1];
+        hist[0][tid] = hist[1][tid] = hist[2][tid] = 0;
         __syncthreads();
         for (uint32_t u = tid; u < source.units; u += kThreads) {
             float x[S::kPer];
@@ -264,20 +267,36 @@ __device__ Border find_border(Team& team, const S& source, const Weights<T>& w, 
             for (int e = 0; e < S::kPer; ++e) {
                 const uint32_t k = key_of<T>(x[e]);
                 if (k >= lo && k <= hi) {
-                    const uint64_t v = by_weight ? w(x[e]) : 1;
-                    if (v) atomicAdd((unsigned long long*)&hist[(k - lo) >> shift], (unsigned long long)v);
+                    // A 64-bit addition in shared memory is a loop (a top-k of 3000 of 256 x 128003 took 1308 us with it, 182 with 32 bits), so a weight
+                    // is added in parts of 15, 15 and 13 bits, which 2^17 elements do not carry over.
+                    const uint32_t at = (k - lo) >> shift;
+                    if (!by_weight) {
+                        atomicAdd(&hist[0][at], 1u);
+                    } else if (const uint64_t v = w(x[e])) {
+                        if constexpr (S::kLong) atomicAdd(reinterpret_cast<unsigned long long*>(hist) + at, (unsigned long long)v);      // over the first two planes
+                        else {
+                            if (const uint32_t part = (uint32_t)v & 0x7fffu) atomicAdd(&hist[0][at], part);
+                            if (const uint32_t part = (uint32_t)(v >> 15) & 0x7fffu) atomicAdd(&hist[1][at], part);
+                            if (const uint32_t part = (uint32_t)(v >> 30)) atomicAdd(&hist[2][at], part);
+                        }
+                    }
                 }
             }
         }
+        auto sum_of = [&](const uint32_t* planes) {
+            if (!by_weight) return (uint64_t)planes[tid];
+            if constexpr (S::kLong) return reinterpret_cast<const uint64_t*>(planes)[tid];
+            else return planes[tid] + ((uint64_t)planes[256 + tid] << 15) + ((uint64_t)planes[512 + tid] << 30);
+        };
         uint64_t v = 0;
         if (kAll) {
             cg::cluster_group cluster = cg::this_cluster();
             cluster.sync();
 #pragma unroll
-            for (uint32_t c = 0; c < kMaxCtas; ++c) v += c < team.ctas ? cluster.map_shared_rank(hist, c)[tid] : 0;
+            for (uint32_t c = 0; c < kMaxCtas; ++c) v += c < team.ctas ? sum_of(cluster.map_shared_rank(&hist[0][0], c)) : 0;
         } else {
             __syncthreads();
-            v = hist[tid];
+            v = sum_of(&hist[0][0]);
         }
         uint64_t from = v;      // the sum over this piece and those above it
 #pragma unroll
