@@ -743,6 +743,29 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
             locate<true>(team, slice, w, keep, kept, same, u, token, prob);
             return;
         }
+        if (listed) {      // the border among the row's keys that would be in the lists; starting over took 525 us where this takes 362 (256 x 128003 bf16, 0.9999)
+            uint32_t largest_listed = 0, inverse = 0;
+            for (uint32_t i = tid; i < slice.units; i += kThreads) {
+                float x[Slice::kPer];
+                slice.values(i, x);
+#pragma unroll
+                for (int e = 0; e < Slice::kPer; ++e) {
+                    const float d = w.below(x[e]);
+                    if (!(d < sure_end) && d < list_end) {
+                        const uint32_t key = key_of<T>(x[e]);
+                        largest_listed = max(largest_listed, key);
+                        inverse = max(inverse, ~key);
+                    }
+                }
+            }
+            largest_listed = team.block_max(largest_listed);
+            inverse = team.block_max(inverse);
+            uint32_t high = 0, low = 0;
+            team.exchange(largest_listed, inverse, [&](uint32_t, uint64_t a, uint64_t b) { high = max(high, (uint32_t)a); low = max(low, (uint32_t)b); });
+            const Border at = find_border<true>(team, slice, w, ~low, high, all_sure, target, true);
+            draw<true>(team, slice, w, Kept{at.key, ties_to_reach(w, at, target, ~0ull), least}, u, token, prob);
+            return;
+        }
     }
     // Too many candidates: on the row as it lies.
     uint32_t inverse = 0;

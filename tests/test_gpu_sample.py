@@ -248,3 +248,16 @@ def test_outputs_that_overlap_are_refused(ctx):
         with pytest.raises(FgError):
             ctx.sample(**(given | kw))
     ctx.sample(**given)
+
+
+@pytest.mark.parametrize("dtype,cols", [("f32", 360_001), ("bf16", 730_001), ("f16", 730_008)])
+@pytest.mark.parametrize("spread", [0.0, 0.02, 1.0, 3.0])
+def test_wide_nuclei_of_the_longest_rows_held(ctx, dtype, cols, spread):
+    # the largest sums that a CTA adds up in parts: 46000 and 92000 weights of up to one, and lists that no CTA has room for
+    r = np.random.Generator(np.random.Philox(cols + int(100 * spread)))
+    x = rounded(r.standard_normal((3, cols)) * spread, dtype)
+    x[1, r.random(cols) < 0.5] = -np.inf
+    u = r.random(3).astype(np.float32)
+    for p in (0.3, 0.9, 0.9999, 0.99999):
+        run(ctx, x, u, dtype, top_p=np.full(3, p, np.float32), min_p=np.array([0, 0, 0.05], np.float32))
+    run(ctx, x, u, dtype, top_p=np.full(3, 0.9, np.float32), top_k=np.array([cols // 2, cols // 3, 5000], np.uint32))
