@@ -167,8 +167,9 @@ struct Straight {
 // latest, so if the rows of a group, and of all groups of a block, lie a multiple of that apart (kApart: they are a grid apart), it is one number
 // for them, and the thread's words hold the same columns of every row.  The words at a row's ends are shared with other rows.
 // Against single elements, forward and backward, us: 4099 x 1001 f16 9.4 and 14.2 (10.3 and 18.0), 30000 x 777 f16 34.5 and 49.1 (53.6 and
-// 72.1), 3000 x 5001 f32 35.9 and 45.5 (73.6 and 162), 10000 x 4097 bf16 80.6 and 91.9 (137 and 178).  What is over the time of rows that lie
-// straight (30000 x 776: 24.7 and 41.8) are the ends: the warps that have one mask it and store it by elements (a lane per element was no faster).
+// 72.1), 3000 x 5001 f32 35.9 and 45.5 (73.6 and 162), 10000 x 4097 bf16 80.6 and 91.9 (137 and 178), 3000 x 12001 f32 120 and 178
+// (210 and 223).  What is over the time of rows that lie straight (30000 x 776: 24.7 and 41.8) are the ends: the warps that have one mask it
+// and store it by elements (a lane per element was no faster).
 template <typename T_, int kPacks, int kTensors>
 struct Shifted {
     using T = T_;
@@ -256,21 +257,26 @@ struct Shifted {
             else elements(p, k, v);
         }
     }
-    // Parameters lie as they like; they are read once.
+    // Parameters lie as they like; of up to 4 packs they are read once.
     __device__ __forceinline__ void parameter(const T* p, float2 (&v)[N / 2]) const {
 #pragma unroll
         for (int k = 0; k < kPacks; ++k) elements(p + column + (int64_t)(k * pitch), k, v);
     }
-    struct Kept { uint4 w[kPacks]; };
+    static constexpr bool kKeep = kPacks <= 4;
+    struct Kept { uint4 w[kKeep ? kPacks : 1]; };
     __device__ __forceinline__ void keep(const T* p, Kept& kept) const {
-        float2 v[N / 2];
-        parameter(p, v);
+        if constexpr (kKeep) {
+            float2 v[N / 2];
+            parameter(p, v);
 #pragma unroll
-        for (int k = 0; k < kPacks; ++k) kept.w[k] = pack(v, k);
+            for (int k = 0; k < kPacks; ++k) kept.w[k] = pack(v, k);
+        }
     }
-    __device__ __forceinline__ void kept(const Kept& kept, const T*, float2 (&v)[N / 2]) const {
+    __device__ __forceinline__ void kept(const Kept& kept, const T* p, float2 (&v)[N / 2]) const {
+        if constexpr (kKeep) {
 #pragma unroll
-        for (int k = 0; k < kPacks; ++k) spread(kept.w[k], k, v);
+            for (int k = 0; k < kPacks; ++k) spread(kept.w[k], k, v);
+        } else parameter(p, v);
     }
     static __device__ __forceinline__ uint4 pack(const float2 (&v)[N / 2], int k) {
         float2 x[P];
@@ -735,9 +741,9 @@ HeldPlan held_plan(const fg_ctx* ctx, uint32_t rows, uint64_t units, int least, 
 }
 // The same for rows that begin anywhere in a word: a grid of as many blocks as bring a row's start back to its place in one.
 template <typename T>
-HeldPlan shifted_plan(const fg_ctx* ctx, uint32_t rows, uint32_t cols, int usual, int most, int tensors) {
+HeldPlan shifted_plan(const fg_ctx* ctx, uint32_t rows, uint32_t cols, int least, int usual, int most, int tensors) {
     constexpr uint32_t E = FgPack<T>::E;
-    HeldPlan p = held_plan(ctx, rows, ((uint64_t)cols + 2 * E - 2) / E, 1, usual, most, tensors, 512);
+    HeldPlan p = held_plan(ctx, rows, ((uint64_t)cols + 2 * E - 2) / E, least, usual, most, tensors, 512);
     if (!p.threads) return p;
     int period = 1;
     while ((uint64_t)period * cols % E) period *= 2;
@@ -779,9 +785,11 @@ int32_t norm_fwd(fg_ctx* ctx, const NormArgs& a) {
     } else {
         // Rows that a warp holds by four elements a lane (eight of f32) are faster so: 20000 x 81 bf16 7.0 us against 9.6, 20000 x 201 f32 10.3 against 11.0.
         if (a.cols > 64 * sizeof(T) && fg_aligned16(a.x) && fg_aligned16(a.y)) {
-            const HeldPlan p = shifted_plan<T>(ctx, a.rows, a.cols, usual, 4, 1);
+            constexpr int most = 32 / FgPack<T>::E;      // a bit per column of a thread
+            const HeldPlan p = shifted_plan<T>(ctx, a.rows, a.cols, 1, usual, most, 1);
             if (p.threads)
-                return p.units == 1 ? launch_held<Shifted<T, 1, 1>>(ctx, a, p) : p.units == 2 ? launch_held<Shifted<T, 2, 1>>(ctx, a, p) : launch_held<Shifted<T, 4, 1>>(ctx, a, p);
+                return p.units == 1 ? launch_held<Shifted<T, 1, 1>>(ctx, a, p) : p.units == 2 ? launch_held<Shifted<T, 2, 1>>(ctx, a, p)
+                       : p.units == 4 ? launch_held<Shifted<T, 4, 1>>(ctx, a, p) : launch_held<Shifted<T, most, 1>>(ctx, a, p);
         }
         HeldPlan p = held_plan(ctx, a.rows, a.cols, 4, 8, 32, 0, 1024);
         if (p.threads)
@@ -818,7 +826,7 @@ int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
     const bool straight = fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.dy, a.gamma, a.dx);
     HeldPlan p{};
     if (straight) p = held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 1, usual, usual, 2, 512);
-    else if (fg_aligned16(a.x) && fg_aligned16(a.dy) && fg_aligned16(a.dx)) p = shifted_plan<T>(ctx, a.rows, a.cols, usual, usual, 2);
+    else if (fg_aligned16(a.x) && fg_aligned16(a.dy) && fg_aligned16(a.dx)) p = shifted_plan<T>(ctx, a.rows, a.cols, 1, usual, usual, 2);
     const bool shifted = !straight && p.threads;
     if (!straight && !shifted) p = held_plan(ctx, a.rows, a.cols, 4, 4, 16, 0, 1024);
     if (p.threads) {
@@ -861,6 +869,10 @@ int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
     // dx alone leaves a thread room for 32 columns.
     const HeldPlan q = straight ? held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 2 * usual, 2 * usual, 2 * usual, 2, 512) : HeldPlan{};
     if (q.threads) return launch_bwd<Straight<T, 2 * usual, false, 2>, false>(ctx, a, q, nullptr, 0);
+    if (!straight && fg_aligned16(a.x) && fg_aligned16(a.dy) && fg_aligned16(a.dx)) {
+        const HeldPlan w = shifted_plan<T>(ctx, a.rows, a.cols, 2 * usual, 2 * usual, 2 * usual, 2);
+        if (w.threads) return launch_bwd<Shifted<T, 2 * usual, 2>, false>(ctx, a, w, nullptr, 0);
+    }
     const HeldPlan e = straight ? HeldPlan{} : held_plan(ctx, a.rows, a.cols, 32, 32, 32, 0, 512);
     if (e.threads) return launch_bwd<Ragged<T, 32, 2>, false>(ctx, a, e, nullptr, 0);
     fg_launch(ctx, norm_bwd_stream_kernel<T>, rows_grid(ctx, a.rows), 256, 0, a);

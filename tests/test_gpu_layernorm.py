@@ -272,7 +272,8 @@ def test_statistics_that_overlap_are_refused(ctx):
 
 # Rows whose starts lie at 8, 4, 2 places of a 16-byte word, more of them than are worked on at a time, and a word or an element over a border.
 RAGGED = [("f16", 6001, 129), ("bf16", 5003, 257), ("f16", 2501, 1001), ("bf16", 3001, 1002), ("f16", 3000, 1004), ("bf16", 1203, 4097), ("f16", 700, 8191),
-          ("f32", 5003, 257), ("f32", 2600, 777), ("f32", 1300, 1002), ("f32", 701, 4099), ("bf16", 4001, 5), ("f32", 3001, 1), ("bf16", 650, 9001)]
+          ("f32", 5003, 257), ("f32", 2600, 777), ("f32", 1300, 1002), ("f32", 701, 4099), ("bf16", 4001, 5), ("f32", 3001, 1), ("bf16", 650, 9001),
+          ("f32", 310, 12001), ("f16", 310, 16001), ("f32", 300, 8194)]
 
 
 @pytest.mark.parametrize("dtype,rows,cols", RAGGED)
