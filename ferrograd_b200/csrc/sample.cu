@@ -534,7 +534,8 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
                        fabs((double)top * per_unit) < 1e6 && per_unit < 1e30 && per_unit > 1e-30};
     const float u = a.u[r], p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
     const uint32_t k = a.top_k && a.top_k[r] < a.cols ? a.top_k[r] : 0;
-    const double least = mp > 0.0f ? (double)min(mp, 1.0f) * kOne : 0.0;
+    // Against the largest logit's weight as it is computed, which mc's rounding may leave a little above or below 2^42: it is always kept.
+    const double least = mp > 0.0f ? (double)min(mp, 1.0f) * w.scaled(top) : 0.0;
     if (!k && !(p < 1.0f)) {
         draw<true>(team, slice, w, Kept{0, 0, least}, u, token, prob);
         return;

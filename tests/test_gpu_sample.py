@@ -261,3 +261,18 @@ def test_wide_nuclei_of_the_longest_rows_held(ctx, dtype, cols, spread):
     for p in (0.3, 0.9, 0.9999, 0.99999):
         run(ctx, x, u, dtype, top_p=np.full(3, p, np.float32), min_p=np.array([0, 0, 0.05], np.float32))
     run(ctx, x, u, dtype, top_p=np.full(3, 0.9, np.float32), top_k=np.array([cols // 2, cols // 3, 5000], np.uint32))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(64, 1), (64, 50), (64, 3000), (24, 40000), (2, 750_001)])
+def test_min_p_of_one_keeps_the_largest(ctx, dtype, rows, cols):
+    # at any temperature, with every other filter: the largest logit, and those equal to it, are all that is left
+    r = np.random.Generator(np.random.Philox(rows + cols))
+    x = rounded(r.standard_normal((rows, cols)) * 3 + 4 * r.standard_normal((rows, 1)), dtype)
+    x[::5, cols // 2] = x[::5].max(1)
+    u = r.random(rows).astype(np.float32)
+    given = {"temperature": (0.3 + 1.2 * r.random(rows)).astype(np.float32), "min_p": r.choice([1.0, 2.0, 0.99999994, np.inf], rows).astype(np.float32)}
+    k, p = r.integers(1, 60, rows).astype(np.uint32), r.random(rows).astype(np.float32)
+    for more in ({}, {"top_k": k}, {"top_p": p}, {"top_k": k, "top_p": p}):
+        got = run(ctx, x, u, dtype, **given, **more)
+        assert (x[np.arange(rows), got] == x.max(1)).all()
