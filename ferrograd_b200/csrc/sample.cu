@@ -308,7 +308,8 @@ __device__ Border find_border(Team& team, const S& source, const Weights<T>& w, 
         __syncthreads();
         for (int j = warp + 1; j < kWarps; ++j) from += sh.red[j];
         from += above;
-        if (from >= target ? from - v < target : tid == 0) {
+        // One thread has the border; should `above` reach the target already, it is the highest key, should nothing, the lowest.
+        if (from >= target ? from - v < target || tid == (hi - lo) >> shift : tid == 0) {
             sh.border = Border{lo + ((uint32_t)tid << shift), from - v, v};
             sh.next_lo = lo + ((uint32_t)tid << shift);
             sh.next_hi = sh.next_lo + min(hi - sh.next_lo, (1u << shift) - 1);
@@ -325,7 +326,7 @@ __device__ Border find_border(Team& team, const S& source, const Weights<T>& w, 
 template <typename T>
 __device__ __forceinline__ uint64_t ties_to_reach(const Weights<T>& w, const Border& at, uint64_t target, uint64_t most) {
     const uint64_t each = w.of_key(at.key);
-    return each ? min(most, (target - at.above + each - 1) / each) : 0;
+    return each && at.above < target ? min(most, (target - at.above + each - 1) / each) : 0;
 }
 __device__ __forceinline__ uint64_t nucleus(float p, uint64_t weight) {
     return max((uint64_t)1, (uint64_t)__double2ull_ru((double)max(p, 0.0f) * (double)weight));
@@ -644,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
         cluster.sync();
         constexpr int kEach = kBins / kThreads;      // a thread takes two bins
         float sum = 0.0f, part[kEach];
-        uint32_t in_bin[kEach] = {};
+        uint64_t in_bin[kEach] = {};      // a CTA's part fits in 32 bits (2^18 columns of 8371 at most), eight of them do not
 #pragma unroll
         for (uint32_t c = 0; c < kMaxCtas; ++c)
             if (c < team.ctas) {

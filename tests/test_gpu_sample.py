@@ -276,3 +276,15 @@ def test_min_p_of_one_keeps_the_largest(ctx, dtype, rows, cols):
     for more in ({}, {"top_k": k}, {"top_p": p}, {"top_k": k, "top_p": p}):
         got = run(ctx, x, u, dtype, **given, **more)
         assert (x[np.arange(rows), got] == x.max(1)).all()
+
+
+@pytest.mark.parametrize("dtype,cols,spread,temperature", [("bf16", 700_001, 0.02, 1.0), ("f32", 1_048_576, 0.02, 1.0), ("f16", 1_048_576, 0.1, 1.0), ("bf16", 1_500_000, 0.02, 1.0),
+                                                           ("f32", 2_097_152, 0.0, 1.0), ("bf16", 2_097_152, 0.02, 0.7), ("f32", 600_001, 1.0, 30.0)])
+def test_nuclei_of_the_longest_flat_rows(ctx, dtype, cols, spread, temperature):
+    # more columns near one weight than 32 bits count in parts of 2^-13
+    r = np.random.Generator(np.random.Philox(cols))
+    x = rounded(r.standard_normal((4, cols)) * spread, dtype)
+    x[3, r.permutation(cols)[:cols // 3]] = -1e9 if dtype != "f16" else -6e4          # masks that are numbers
+    u, t = r.random(4).astype(np.float32), np.full(4, temperature, np.float32)
+    run(ctx, x, u, dtype, temperature=t, top_p=np.array([0.1, 0.3, 0.6, 0.6], np.float32))
+    run(ctx, x, u, dtype, temperature=t, top_p=np.array([0.9, 0.5, 0.99, 0.3], np.float32), min_p=np.array([0, 0, 0.5, 1], np.float32))
