@@ -15,6 +15,8 @@
 // equal logits at the border the first ones are kept.
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "rows.cuh"
 
 namespace cg = cooperative_groups;
@@ -27,6 +29,7 @@ constexpr int kBins = 512;                    // 16ths of an octave that a row's
 constexpr uint32_t kLocal = 1024, kGathered = 4096;      // candidates of a CTA, of a row
 constexpr unsigned kFull = 0xffffffffu;
 constexpr double kOne = 4398046511104.0;      // 2^42
+constexpr size_t kHeldBytes = 180 * 1024;     // of a slice in shared memory
 
 struct SampleArgs {
     const void* logits;
@@ -790,7 +793,11 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
 
 template <typename T, bool kHeld>
 int32_t launch_sample(fg_ctx* ctx, const SampleArgs& a, unsigned ctas, size_t bytes) {
-    if (bytes > 16 * 1024) FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(sample_kernel<T, kHeld>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    static std::atomic<uint64_t> attr_done{0};      // one bit per device; never less than the largest, which another thread's call may be about to use
+    if (!(attr_done.load(std::memory_order_acquire) >> (ctx->device & 63) & 1ull)) {
+        FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(sample_kernel<T, kHeld>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kHeld ? kHeldBytes : sizeof(uint2) * kGathered)));
+        attr_done.fetch_or(1ull << (ctx->device & 63), std::memory_order_release);
+    }
     fg_launch_cluster(ctx, sample_kernel<T, kHeld>, a.rows * ctas, kThreads, bytes, ctas, a);
     FG_LAUNCHED(ctx);
     return FG_OK;
@@ -804,7 +811,7 @@ int32_t sample(fg_ctx* ctx, SampleArgs a) {
     a.slice = ((a.cols + ctas - 1) / ctas + 7) / 8 * 8;
     const size_t held = ((size_t)a.slice * sizeof(T) + 31) / 16 * 16, list = sizeof(uint2) * (a.cols < kGathered ? a.cols : kGathered);
     FG_REQUIRE(ctx, (uint64_t)a.rows * ctas < (1ull << 31), "fg_sample: too many rows");
-    if (held <= 180 * 1024) return launch_sample<T, true>(ctx, a, ctas, held < list ? list : held);
+    if (held <= kHeldBytes) return launch_sample<T, true>(ctx, a, ctas, held < list ? list : held);
     return launch_sample<T, false>(ctx, a, ctas, list);
 }
 

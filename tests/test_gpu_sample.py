@@ -288,3 +288,50 @@ def test_nuclei_of_the_longest_flat_rows(ctx, dtype, cols, spread, temperature):
     u, t = r.random(4).astype(np.float32), np.full(4, temperature, np.float32)
     run(ctx, x, u, dtype, temperature=t, top_p=np.array([0.1, 0.3, 0.6, 0.6], np.float32))
     run(ctx, x, u, dtype, temperature=t, top_p=np.array([0.9, 0.5, 0.99, 0.3], np.float32), min_p=np.array([0, 0, 0.5, 1], np.float32))
+
+
+def test_long_and_short_rows_at_once():
+    # two host threads, a context each: neither's shared memory is limited by the other's call
+    import threading
+
+    from ferrograd_b200 import GpuContext
+    sizes, calls, failed = (300_001, 40_000), 1500, []
+    contexts = [GpuContext(0) for _ in sizes]
+    r = np.random.Generator(np.random.Philox(8))
+    x = [r.standard_normal((1, cols)).astype(np.float32) for cols in sizes]
+    u = np.array([0.37], np.float32)
+    given = [(Placed(c, a), Placed(c, u), empty(c, (1,), "u32")) for c, a in zip(contexts, x)]
+
+    def work(c, logits, u, token, cols):
+        try:
+            for _ in range(calls):
+                c._check(c.lib.fg_sample(c.handle, 0, 1, cols, logits.ptr, u.ptr, None, None, None, None, token.ptr, None))
+        except Exception as e:   # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(c, *g, cols)) for c, g, cols in zip(contexts, given, sizes)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for c, (_, _, token), a in zip(contexts, given, x):
+        assert token.get()[0] == definition(a[0], u[0])[0]
+        assert c.device_status() == 0
+        c.destroy()
+
+
+def test_long_and_short_rows_in_one_plan(ctx):
+    r = np.random.Generator(np.random.Philox(9))
+    x = [r.standard_normal((2, cols)).astype(np.float32) for cols in (300_001, 40_000, 100)]
+    u = r.random(2).astype(np.float32)
+    given = [(Placed(ctx, a), Placed(ctx, u), empty(ctx, (2,), "u32")) for a in x]
+    ctx.plan_begin()
+    for (logits, ud, token), a in zip(given, x):
+        ctx.sample(logits, ud, token, *a.shape)
+    plan = ctx.plan_end()
+    ctx.sample(*given[1], *x[1].shape)
+    plan.launch()
+    for (_, _, token), a in zip(given, x):
+        assert np.array_equal(token.get(), [definition(a[i], u[i])[0] for i in range(2)])
+    plan.destroy()
