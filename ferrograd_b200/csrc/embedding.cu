@@ -661,7 +661,7 @@ int32_t embed_bwd(fg_ctx* ctx, const EmbedArgs& a) {
     SumArgs s{};
     s.tokens = a.tokens;
     s.dim = a.dim;
-    s.tiles = (a.dim + 32 * E - 1) / (32 * E);
+    s.tiles = (uint32_t)(((uint64_t)a.dim + 32 * E - 1) / (32 * E));
     s.pitch = (uint64_t)s.tiles * 32 * E;
     s.scale = a.scale;
     s.dout = a.src;

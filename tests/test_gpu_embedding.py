@@ -199,3 +199,34 @@ def test_empty_and_refusals(ctx):
         refuse(lambda: ctx.embedding_bwd(**a))
     assert ctx.lib.fg_embedding_fwd(ctx.handle, 3, 1, 4, 4, p, p + 64, 1.0, p + 256) == 1
     assert ctx.lib.fg_embedding_bwd(ctx.handle, -1, 1, 4, 4, p, p + 64, 1.0, p + 256, 0) == 1
+
+
+def test_rows_of_the_most_columns():
+    # one row of 2^32 - 1 columns: the number of its tiles is no 32-bit sum
+    from ferrograd_b200 import GpuContext
+    from ferrograd_b200.backend import to_bf16_bits
+    ctx, dim = GpuContext(0), (1 << 32) - 1
+    source, grad = (ctx.new_tensor((dim,), np.uint16) for _ in range(2))
+    r, at = np.random.Generator(np.random.Philox(4)), (0, dim // 3, dim - 300)
+    parts = [to_bf16_bits(r.integers(1, 9, 300).astype(np.float32)) for _ in at]
+    ids, got = Placed(ctx, [0], "u32"), np.empty(300, np.uint16)
+
+    def expect(times):
+        for i, part in zip(at, parts):
+            ctx.download(grad.data, got, src_off=2 * i)
+            assert np.array_equal(got, to_bf16_bits(times * (part.astype(np.uint32) << 16).view(np.float32)))
+
+    ctx.memset_zero(source, 2 * dim)
+    for i, part in zip(at, parts):
+        ctx.upload(source.data, part, dst_off=2 * i)
+        ctx.upload(grad.data, np.full(300, 0x7fc0, np.uint16), dst_off=2 * i)          # NaN
+    ctx.embedding_fwd(source, ids, grad, 1, 1, dim, scale=2.0, dtype="bf16")
+    expect(2)
+    ctx.embedding_bwd(ids, source, grad, 1, 1, dim, dtype="bf16")
+    expect(1)
+    ctx.embedding_bwd(ids, source, grad, 1, 1, dim, accumulate=True, dtype="bf16")
+    expect(2)
+    assert ctx.device_status() == 0
+    for t in (source, grad):
+        t.data.free()
+    ctx.destroy()
