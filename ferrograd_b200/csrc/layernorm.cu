@@ -860,9 +860,9 @@ int32_t norm_bwd(fg_ctx* ctx, const NormBwdArgs& a) {
         void* w;
         const int32_t s = fg_ws_alloc(ctx, 8ull * chunks * a.cols, &w);
         if (s != FG_OK) return s;
-        fg_launch(ctx, straight ? norm_columns_kernel<T, true> : norm_columns_kernel<T, false>, dim3((a.cols + 32 * E - 1) / (32 * E), chunks), dim3(32, 8), 0, a, (float*)w);
+        fg_launch(ctx, straight ? norm_columns_kernel<T, true> : norm_columns_kernel<T, false>, dim3((unsigned)(((uint64_t)a.cols + 32 * E - 1) / (32 * E)), chunks), dim3(32, 8), 0, a, (float*)w);
         FG_LAUNCHED(ctx);
-        fg_launch(ctx, norm_fold_kernel<T>, dim3((a.cols + 255) / 256, 2), 256, 0, a, (const float*)w, chunks);
+        fg_launch(ctx, norm_fold_kernel<T>, dim3((unsigned)(((uint64_t)a.cols + 255) / 256), 2), 256, 0, a, (const float*)w, chunks);
         FG_LAUNCHED(ctx);
     }
     if (!a.dx) return FG_OK;

@@ -322,3 +322,25 @@ def test_ragged_rows_beside_values_out_of_the_ordinary(ctx, dtype, rows, cols):
     bad[0::3], bad_dy[0::3] = np.where(np.arange(len(bad[0::3]))[:, None] % 2, np.inf, np.nan), np.nan
     for a, b in zip(plain, run(bad, bad_dy)):
         assert np.array_equal(a[1::3], b[1::3]) and np.array_equal(a[2::3], b[2::3])
+
+
+def test_gradients_of_the_most_columns():
+    # one row of 2^32 - 1 columns: the grids over its columns are no 32-bit sums
+    from ferrograd_b200 import GpuContext
+    ctx, cols = GpuContext(0), (1 << 32) - 1
+    x, dgamma = (ctx.new_tensor((cols,), np.uint16) for _ in range(2))
+    r, at = np.random.Generator(np.random.Philox(6)), (0, cols // 3, cols - 300)
+    parts = [r.integers(-8, 9, 300).astype(np.float16) for _ in at]
+    got = np.empty(300, np.float16)
+    ctx.memset_zero(x, 2 * cols)
+    for i, part in zip(at, parts):
+        ctx.upload(x.data, part, dst_off=2 * i)
+        ctx.upload(dgamma.data, np.full(300, np.nan, np.float16), dst_off=2 * i)
+    ctx.layernorm_bwd(x, x, None, Placed(ctx, [0.5]), Placed(ctx, [2.0]), 1, cols, dgamma=dgamma, dtype="f16")
+    for i, part in zip(at, parts):
+        ctx.download(dgamma.data, got, src_off=2 * i)
+        assert np.array_equal(got, part * (part - np.float16(0.5)) * 2)          # whole numbers: exact
+    assert ctx.device_status() == 0
+    for t in (x, dgamma):
+        t.data.free()
+    ctx.destroy()
