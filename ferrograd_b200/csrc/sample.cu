@@ -258,6 +258,7 @@ __device__ Border find_border(Team& team, const S& source, const Weights<T>& w, 
     Shared& sh = team.sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Border at{};
+    target = max(target, above + 1);               // one thread finds the border in any case: should `above` be there already, among the highest keys
     for (int round = 0; round < 5; ++round) {      // 32 bits of range, eight less after each
         const int bits = 32 - __clz(hi - lo), shift = bits > 8 ? bits - 8 : 0;
         uint32_t (*const hist)[256] = sh.hist[team.round ^= 1];
@@ -311,8 +312,7 @@ __device__ Border find_border(Team& team, const S& source, const Weights<T>& w, 
         __syncthreads();
         for (int j = warp + 1; j < kWarps; ++j) from += sh.red[j];
         from += above;
-        // One thread has the border; should `above` reach the target already, it is the highest key, should nothing, the lowest.
-        if (from >= target ? from - v < target || tid == (hi - lo) >> shift : tid == 0) {
+        if (from >= target ? from - v < target : tid == 0) {
             sh.border = Border{lo + ((uint32_t)tid << shift), from - v, v};
             sh.next_lo = lo + ((uint32_t)tid << shift);
             sh.next_hi = sh.next_lo + min(hi - sh.next_lo, (1u << shift) - 1);
@@ -538,8 +538,9 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 4 : 2) sample_kernel(const S
                        fabs((double)top * per_unit) < 1e6 && per_unit < 1e30 && per_unit > 1e-30};
     const float u = a.u[r], p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
     const uint32_t k = a.top_k && a.top_k[r] < a.cols ? a.top_k[r] : 0;
-    // Against the largest logit's weight as it is computed, which mc's rounding may leave a little above or below 2^42: it is always kept.
-    const double least = mp > 0.0f ? (double)min(mp, 1.0f) * w.scaled(top) : 0.0;
+    // The largest logit itself comes out up to |mc| 2^-53 and a rounding off 2^42, which must not put it below a min_p of 1; |mc| 2^-52 lets in no other,
+    // whose distance is 2^-24 of it at least.  (Its own computed weight as the bound takes 38.8 us where this takes 38.3: 512 x 32000 f32.)
+    const double least = mp > 0.0f ? (double)min(mp, 1.0f) * (w.ordinary ? kOne - fabs(w.mc) * 0x1p-10 : kOne) : 0.0;
     if (!k && !(p < 1.0f)) {
         draw<true>(team, slice, w, Kept{0, 0, least}, u, token, prob);
         return;
