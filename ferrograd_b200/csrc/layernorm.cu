@@ -717,15 +717,27 @@ int rows_grid(const fg_ctx* ctx, uint32_t rows) { return (int)(rows < 8u * ctx->
 // How a kernel that holds rows is launched: a thread's packs (or elements, of ragged rows), the threads of a group, the groups of a block, the
 // bytes of its slots, the blocks; threads = 0: not at all.
 struct HeldPlan { int units, threads, groups; bool full; size_t bytes; int grid; };
-// A block has 256 threads or, for a longer row, up to 512.  Threads hold `usual` units, or up to `most` where the row asks for it (up to 4 packs, which
-// registers hold, where a warp is enough with them, and from 256 threads on: an SM has two rows to switch between then; 7000 x 8192 bf16 forward
-// 62.7 -> 44.7 us); of few rows, and where
-// a warp is enough, `least`.  `resident`: threads that an SM has registers for, at the usual units.
+// How many units a thread holds: `least`, doubled (to `most` at most) while the row would take more threads than are good for it.  us, forward of
+// bf16 unless said otherwise, by packs:
+//   two rows per SM or fewer      512 (a block): more threads answer sooner (296 x 4096 backward 8.9 by 1, 12.0 by 2; forward 64 x 1024 1.8 and 1.9,
+//                                 but 296 x 4096 3.4 and 2.7)
+//   below `usual`                 32 (a warp): its sums need no barrier, and less of a row is instructions (16384 x 512 7.7 by 2, 12.9 by 1; 600 x 4096
+//                                 4.4 and 6.0; f32 16384 x 4096 82 to 86 by 4, 118 by 2), but no more than a warp is for (16384 x 256 5.8 by 1, 8.7 by 2)
+//   2 packs, and 4 make a warp    32 (16384 x 1024 11.0 by 4, 16.5 by 2)
+//   2 packs, longer rows          256: an SM has two rows to switch between then (7000 x 8192 44.1 by 4, 61.8 by 2)
+//   4 packs and more              512: registers hold no more (f32 16384 x 4096 82 by 4, 101 by 8; 7000 x 12288 75 by 4, 68 by 8)
+int units_of(uint64_t units, bool many, int least, int usual, int most) {
+    int each = least;
+    while (each < most) {
+        const uint32_t enough = !many || (each >= usual && each >= 4) ? kMaxThreads : each < usual || units <= 128 ? 32 : 256;
+        if (units <= (uint64_t)enough * each) break;
+        each *= 2;
+    }
+    return each;
+}
+// A block has 256 threads or, for a longer row, up to 512.  `resident`: threads that an SM has registers for, at the usual units.
 HeldPlan held_plan(const fg_ctx* ctx, uint32_t rows, uint64_t units, int least, int usual, int most, int tensors, int resident) {
-    HeldPlan p{least, 0, 1, false, 0, 0};
-    const bool many = rows > 2u * ctx->sm_count;
-    while (p.units < most && (units > (uint64_t)kMaxThreads * p.units || (many && units > (p.units < usual || (p.units < 4 && units <= 128) ? 32ull : p.units < 4 ? 256ull : ~0ull / p.units) * p.units)))
-        p.units *= 2;
+    HeldPlan p{units_of(units, rows > 2u * ctx->sm_count, least, usual, most), 0, 1, false, 0, 0};
     if (units > (uint64_t)kMaxThreads * p.units) return p;
     p.threads = (int)((units + 32 * p.units - 1) / (32 * p.units) * 32);
     p.full = units == (uint64_t)p.threads * p.units;
