@@ -91,8 +91,8 @@ __device__ const double kRoots[256] = {
     1.9571441241754002, 1.9624504802089273, 1.9677712232331759, 1.9731063922552343, 1.978456026387951, 1.9838201648502194, 1.9891988469672663, 1.9945921121709402};
 
 // round(2^42 exp(t)) with t = (x - m) / T: exp(t) = 2^(n / 256) exp(r) for the n that leaves |r| <= ln(2) / 512, and four terms of the series
-// of exp(r), off by 2^-42.7 at most (1/6 is cut to 20 bits, which is 2^-52 of the result, so that it fits an instruction).  The 64-bit
-// operations are what a pass over a row takes its time for; a table of 64 and six terms needs two more.
+// of exp(r), off by 2^-42.7 at most (1/6 is cut to 20 bits, which is 2^-52 of the result, so that it fits an instruction).  Of the
+// 44 instructions that a logit of a row with a temperature alone takes, ten are 64-bit ones; a table of 64 and six terms needs two more.
 template <typename T>
 struct Weights {
     const double* roots;

@@ -312,8 +312,9 @@ int32_t fg_layernorm_fwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t col
  *   dgamma [cols] = column sums of dy * h                    (skipped when NULL)
  *   dbeta  [cols] = column sums of dy                        (skipped when NULL; one of the three is wanted)
  * accumulate_dx adds into dx and accumulate_params into dgamma and dbeta instead of overwriting them.  Sums are in
- * f32 in an order that the sizes alone decide.  dx may be dy or x (then without accumulate_dx); any other overlap of an
- * output with a tensor of the call is refused, here and in the forward pass. */
+ * f32 in an order that the sizes, the type, the tensors' places on 16-byte boundaries and the device's number of SMs
+ * decide: the same call on tensors placed alike gives the same bits.  dx may be dy or x (then without accumulate_dx); any
+ * other overlap of an output with a tensor of the call is refused, here and in the forward pass. */
 int32_t fg_layernorm_bwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* x, const void* dy,
                          const void* gamma, const float* mean, const float* rstd, void* dx, void* dgamma,
                          void* dbeta, int32_t accumulate_dx, int32_t accumulate_params);
@@ -324,8 +325,8 @@ int32_t fg_embedding_fwd(fg_ctx* ctx, int32_t dtype, uint32_t tokens, uint32_t v
                          const uint32_t* ids, const void* table, float scale, void* out);
 /* dtable[v] = scale * sum of dout[t] over the tokens t with ids[t] == v, rows of other ids zero; accumulate != 0
  * adds into dtable instead and leaves the other rows alone (fg_sgd_step and fg_adamw_step leave a gradient at zero).
- * The tokens are sorted by id and a row's sum runs over them in f32 in an order that ids and sizes alone decide:
- * no sum is added atomically, so every call gives the same bits. */
+ * The tokens are sorted by id and a row's sum runs over them in f32 in an order that the ids, the sizes, the type and the
+ * device's number of SMs decide: no sum is added atomically, so the same call gives the same bits. */
 int32_t fg_embedding_bwd(fg_ctx* ctx, int32_t dtype, uint32_t tokens, uint32_t vocab, uint32_t dim,
                          const uint32_t* ids, const void* dout, float scale, void* dtable, int32_t accumulate);
 
