@@ -331,9 +331,14 @@ __device__ __forceinline__ uint64_t ties_to_reach(const Weights<T>& w, const Bor
     const uint64_t each = w.of_key(at.key);
     return each && at.above < target ? min(most, (target - at.above + each - 1) / each) : 0;
 }
-__device__ __forceinline__ uint64_t nucleus(float p, uint64_t weight) {
-    return max((uint64_t)1, (uint64_t)__double2ull_ru((double)max(p, 0.0f) * (double)weight));
+// f times n, f from [0, 1), rounded down or up from the exact product: n has up to 63 bits, and in 64-bit floating point a border that the product
+// hits exactly moves by a token.  f goes in parts of 2^-64, which is all of it from 2^-40 on; below that f n is less than 2^23, the largest weight 2^42.
+template <bool kUp>
+__device__ __forceinline__ uint64_t part_of(float f, uint64_t n) {
+    const uint64_t parts = __float2ull_rz(f * 18446744073709551616.0f);
+    return __umul64hi(parts, n) + (kUp && parts * n != 0);
 }
+__device__ __forceinline__ uint64_t nucleus(float p, uint64_t weight) { return max((uint64_t)1, part_of<true>(p > 0.0f ? p : 0.0f, weight)); }
 
 // What is kept: keys above `cut` and the first `ties` of those at it, of weight `least` (in parts of 2^42) or more.
 struct Kept { uint32_t cut; uint64_t ties; double least; };
@@ -359,7 +364,7 @@ __device__ void locate(Team& team, const S& source, const Weights<T>& w, const K
         cg::this_cluster().barrier_arrive();      // nobody reads another's memory from here on
     }
     auto upto = [&](uint64_t x, uint64_t y) { return x + min(keep.ties, y) * at_cut; };
-    const uint64_t total = upto(all_m, all_t), goal = (uint64_t)((double)(u > 0.0f ? min(u, 0.99999994f) : 0.0f) * (double)total), before = upto(m, t);
+    const uint64_t total = upto(all_m, all_t), goal = part_of<false>(u > 0.0f ? min(u, 0.99999994f) : 0.0f, total), before = upto(m, t);
     const unsigned holds = __ballot_sync(kFull, before <= goal && goal < upto(m + mass, t + same));
     if (holds) {      // the warp goes over that thread's stretch once more
         const int from = __ffs(holds) - 1;

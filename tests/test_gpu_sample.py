@@ -335,3 +335,18 @@ def test_long_and_short_rows_in_one_plan(ctx):
     for (_, _, token), a in zip(given, x):
         assert np.array_equal(token.get(), [definition(a[i], u[i])[0] for i in range(2)])
     plan.destroy()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [40, 2500, 17074, 46571, 300_000])
+def test_equal_logits_far_from_zero(ctx, dtype, cols):
+    # equal weights that are not quite 2^42, and whose sums 53 bits do not hold: borders at u and top_p times the total are hit exactly all the same
+    r = np.random.Generator(np.random.Philox(cols))
+    n = 24 if cols < 100_000 else 6
+    x = np.repeat(rounded(r.choice([-1.0, 1.0], (n, 1)) * (300 + 3000 * r.random((n, 1))), dtype), cols, 1)
+    given = {"temperature": (0.05 + r.random(n)).astype(np.float32)}
+    u = r.choice(np.array([0.5, 0.25, 0.75, 0.125, 0.99999994, 2.0 ** -30], np.float32), n)
+    p = r.choice(np.array([0.5, 0.25, 0.75, 0.375], np.float32), n)
+    run(ctx, x, u, dtype, **given)
+    run(ctx, x, u, dtype, **given, top_p=p)
+    run(ctx, x, u, dtype, **given, top_p=p, min_p=np.full(n, 1, np.float32), top_k=np.full(n, max(1, cols // 2), np.uint32))
