@@ -97,6 +97,7 @@ inline int32_t fg_fail(fg_ctx* ctx, int32_t code, const char* msg) {
 }
 
 inline int32_t fg_fail_cuda(fg_ctx* ctx, int32_t code, const char* what, cudaError_t e) {
+    cudaGetLastError();      // reported here: the next launch must not find it (an allocation that was refused, say)
     if (ctx) snprintf(ctx->err, sizeof(ctx->err), "%s: %s", what, cudaGetErrorString(e));
     return code;
 }

@@ -344,3 +344,16 @@ def test_gradients_of_the_most_columns():
     for t in (x, dgamma):
         t.data.free()
     ctx.destroy()
+
+
+def test_a_refused_workspace_leaves_the_next_call_alone():
+    from ferrograd_b200 import FgError, GpuContext
+    ctx = GpuContext(0)
+    x, y = Placed(ctx, [[1.0, 3.0]]), empty(ctx, (1, 2))
+    for refused in (lambda: ctx.alloc(1 << 46), lambda: ctx.reserve_workspace(1 << 46)):          # 64 TB
+        with pytest.raises(FgError) as e:
+            refused()
+        assert e.value.kind == "FG_ERR_OUT_OF_MEMORY"
+        ctx.layernorm_fwd(x, None, None, y, 1, 2, eps=0.0)
+        assert np.array_equal(y.get(), [[-1.0, 1.0]])
+    ctx.destroy()
