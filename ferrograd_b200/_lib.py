@@ -95,6 +95,14 @@ SIGNATURES = {
     "fg_embedding_fwd": (i32, [c_ctx, i32, u32, u32, u32, c_dev, c_dev, f32, c_dev]),
     "fg_embedding_bwd": (i32, [c_ctx, i32, u32, u32, u32, c_dev, c_dev, f32, c_dev, i32]),
     "fg_sample": (i32, [c_ctx, i32, u32, u32, c_dev, c_dev, c_dev, c_dev, c_dev, c_dev, c_dev, c_dev]),
+    "fg_attention_fwd": (i32, [c_ctx, i32, u32, u32, u32, u32, u32, u32, c_dev, c_dev, c_dev, c_dev, u64, c_dev, u64, c_dev, u64, f32, i32, c_dev, c_dev]),
+    "fg_attention_bwd": (i32, [c_ctx, i32, u32, u32, u32, u32, u32, u32, c_dev, c_dev, c_dev, c_dev, u64, c_dev, u64, c_dev, u64, f32, i32, c_dev, c_dev, c_dev, c_dev,
+                               c_dev, c_dev]),
+    "fg_rmsnorm_fwd": (i32, [c_ctx, i32, u32, u32, c_dev, c_dev, c_dev, f32, c_dev, c_dev, c_dev]),
+    "fg_rmsnorm_fwd_e4m3": (i32, [c_ctx, i32, u32, u32, c_dev, c_dev, c_dev, f32, u32, c_dev, c_dev, c_dev, c_dev]),
+    "fg_rmsnorm_bwd": (i32, [c_ctx, i32, u32, u32, c_dev, c_dev, c_dev, c_dev, c_dev, c_dev, c_dev, i32]),
+    "fg_logprobs_fwd": (i32, [c_ctx, i32, u32, u32, c_dev, c_dev, f32, c_dev, c_dev, c_dev, u32, c_dev, c_dev]),
+    "fg_logprobs_bwd": (i32, [c_ctx, i32, u32, u32, c_dev, c_dev, f32, c_dev, c_dev, c_dev, c_dev, c_dev]),
     "fg_sum_f32": (i32, [c_ctx, c_dev, u64, c_dev]),
     "fg_mse_loss_grad": (i32, [c_ctx, c_dev, c_dev, u64, f32, c_dev, c_dev, c_dev]),
     "fg_bce_loss_grad": (i32, [c_ctx, c_dev, c_dev, u64, f32, c_dev, c_dev, c_dev]),

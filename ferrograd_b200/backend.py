@@ -360,6 +360,35 @@ class GpuContext:
         """One token per row; temperature, top_k, top_p and min_p are device arrays of one value per row, or None."""
         self._check(self._c.fg_sample(self._h, DTYPE[dtype], rows, cols, logits, u, temperature, top_k, top_p, min_p, token, prob))
 
+    def attention_fwd(self, q, k, v, out, q_starts, k_starts, sequences, queries, keys, heads, kv_heads, head_dim, scale=None, causal=True,
+                      lse=None, q_stride=0, k_stride=0, v_stride=0, k_lengths=None, dtype="bf16"):
+        """Attention over packed sequences; scale is 1 / sqrt(head_dim) unless given, strides are elements between tokens (0: dense)."""
+        self._check(self._c.fg_attention_fwd(self._h, DTYPE[dtype], sequences, queries, keys, heads, kv_heads, head_dim, q_starts, k_starts, k_lengths,
+                                             q, q_stride, k, k_stride, v, v_stride, head_dim ** -0.5 if scale is None else scale, int(causal), out, lse))
+
+    def attention_bwd(self, q, k, v, out, lse, dout, q_starts, k_starts, sequences, queries, keys, heads, kv_heads, head_dim, dq=None, dk=None, dv=None,
+                      scale=None, causal=True, q_stride=0, k_stride=0, v_stride=0, k_lengths=None, dtype="bf16"):
+        self._check(self._c.fg_attention_bwd(self._h, DTYPE[dtype], sequences, queries, keys, heads, kv_heads, head_dim, q_starts, k_starts, k_lengths,
+                                             q, q_stride, k, k_stride, v, v_stride, head_dim ** -0.5 if scale is None else scale, int(causal), out, lse,
+                                             dout, dq, dk, dv))
+
+    def rmsnorm_fwd(self, x, gamma, y, rows, cols, eps=1e-5, residual=None, sum=None, rstd=None, dtype="f32"):
+        self._check(self._c.fg_rmsnorm_fwd(self._h, DTYPE[dtype], rows, cols, x, residual, gamma, eps, sum, y, rstd))
+
+    def rmsnorm_fwd_e4m3(self, x, gamma, y, scale, rows, cols, group=0, eps=1e-5, residual=None, sum=None, rstd=None, dtype="f32"):
+        """rmsnorm_fwd with y in 8 bits and a scale (f32) per group of columns, or per row (group 0)."""
+        self._check(self._c.fg_rmsnorm_fwd_e4m3(self._h, DTYPE[dtype], rows, cols, x, residual, gamma, eps, group, sum, y, scale, rstd))
+
+    def rmsnorm_bwd(self, x, dy, gamma, rstd, rows, cols, dx=None, dgamma=None, dsum=None, accumulate_params=False, dtype="f32"):
+        self._check(self._c.fg_rmsnorm_bwd(self._h, DTYPE[dtype], rows, cols, x, dy, gamma, rstd, dsum, dx, dgamma, int(accumulate_params)))
+
+    def logprobs_fwd(self, logits, targets, logprob, rows, cols, scale=1.0, entropy=None, lse=None, top=0, top_ids=None, top_logprobs=None, dtype="f32"):
+        """Log probabilities of the targets under softmax(scale * logits), and what else is asked for of each row."""
+        self._check(self._c.fg_logprobs_fwd(self._h, DTYPE[dtype], rows, cols, logits, targets, scale, logprob, entropy, lse, top, top_ids, top_logprobs))
+
+    def logprobs_bwd(self, logits, targets, lse, rows, cols, dlogits, scale=1.0, dlogprob=None, entropy=None, dentropy=None, dtype="f32"):
+        self._check(self._c.fg_logprobs_bwd(self._h, DTYPE[dtype], rows, cols, logits, targets, scale, lse, entropy, dlogprob, dentropy, dlogits))
+
     def mse_loss_grad(self, pred, target, n, grad_scale=1.0, loss_elem=None, loss_sum=None, grad=None):
         self._check(self._c.fg_mse_loss_grad(self._h, pred, target, n, grad_scale,
                                               loss_elem, loss_sum, grad))

@@ -1,0 +1,616 @@
+// Attention over packed sequences with grouped heads, forward and backward: the entry points and the kernels in plain FMAs.
+//
+// Forward, per head: s_ij = scale * q_i . k_j for the keys j that row i sees, o_i = sum_j p_ij v_j with p_ij = exp(s_ij - m) / l, where m is the
+// largest s_ij and l the sum of exp(s_ij - m).  One pass over the keys: when a tile of keys raises m, what was summed so far is multiplied by
+// exp(old m - new m).  Exponents are powers of two (s * log2 e).  lse_i = m + log l is what the backward pass takes.
+// Backward, with delta_i = dout_i . out_i: p_ij = exp(s_ij - lse_i); ds_ij = p_ij * (dout_i . v_j - delta_i); dq_i = scale * sum_j ds_ij k_j;
+// dk_j = scale * sum_i ds_ij q_i; dv_j = sum_i p_ij dout_i.  One kernel has a block of rows and goes over their keys for dq, another a block of
+// keys and goes over their rows, those of all heads of the group, for dk and dv: nothing is added in memory, so the order of sums is fixed.
+#include <atomic>
+
+#include "attention.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr uint32_t kMaxDim = 256;
+
+// ---- plain FMAs: f32, and 16-bit tensors that the tensor cores' kernels do not take ----
+// Threads are 16 x 16: thread (y, x) has rows y * RT .. and keys x, x + 16, .. of a tile's scores, and the same rows (backward over keys: keys) by
+// columns 4 x .. + 64 j of a sum.  Rows of a tile are (query, head of the group) pairs, so the heads of a group share the keys' tile.
+// Rows in shared memory are f32, padded by four words: 16 threads that read 16 bytes each of 16 rows take two passes, the least for 256 bytes.
+__host__ __device__ constexpr int tile_of(int dm) { return dm > 128 ? 32 : 64; }
+
+// Rows [first, first + n) of a tensor's `dim` columns into shared memory, zeros behind the last row and column.
+template <typename T, int kRows, int DM, typename F>
+__device__ __forceinline__ void fetch(float* to, uint32_t n, uint32_t dim, F row) {
+    constexpr int kPitch = DM + 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll 4
+    for (int r = warp; r < kRows; r += kThreads / 32) {
+        const T* p = (uint32_t)r < n ? row((uint32_t)r) : nullptr;
+#pragma unroll
+        for (int c = 0; c < DM; c += 32) to[r * kPitch + c + lane] = p && (uint32_t)(c + lane) < dim ? fg_widen(p[c + lane]) : 0.0f;
+    }
+}
+// RT x CT products of rows of two tiles: a's rows a0 + i, b's rows b0 + 16 * j.
+template <int RT, int CT, int DM>
+__device__ __forceinline__ void dots(const float* a, const float* b, uint32_t dim, int a0, int b0, float (&s)[RT][CT]) {
+    constexpr int kPitch = DM + 4;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j) s[i][j] = 0.0f;
+    for (uint32_t d = 0; d < dim; d += 4) {
+        float4 x[RT], y[CT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) x[i] = *reinterpret_cast<const float4*>(a + (a0 + i) * kPitch + d);
+#pragma unroll
+        for (int j = 0; j < CT; ++j) y[j] = *reinterpret_cast<const float4*>(b + (b0 + 16 * j) * kPitch + d);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < CT; ++j)
+                s[i][j] = __fmaf_rn(x[i].w, y[j].w, __fmaf_rn(x[i].z, y[j].z, __fmaf_rn(x[i].y, y[j].y, __fmaf_rn(x[i].x, y[j].x, s[i][j]))));
+    }
+}
+// acc[i] += w_i * row of b: one row of b's columns 4 x .. + 64 j.
+template <int RT, int DM>
+__device__ __forceinline__ void add_row(const float* b, int x, const float (&w)[RT], float4 (&acc)[RT][DM / 64]) {
+#pragma unroll
+    for (int j = 0; j < DM / 64; ++j) {
+        const float4 v = *reinterpret_cast<const float4*>(b + 4 * x + 64 * j);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            acc[i][j].x = __fmaf_rn(w[i], v.x, acc[i][j].x);
+            acc[i][j].y = __fmaf_rn(w[i], v.y, acc[i][j].y);
+            acc[i][j].z = __fmaf_rn(w[i], v.z, acc[i][j].z);
+            acc[i][j].w = __fmaf_rn(w[i], v.w, acc[i][j].w);
+        }
+    }
+}
+template <int DM>
+__device__ __forceinline__ void put_row(float* to, int x, uint32_t dim, const float4 (&v)[DM / 64], float by) {
+#pragma unroll
+    for (int j = 0; j < DM / 64; ++j) {
+        const float e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if ((uint32_t)(4 * x + 64 * j + c) < dim) to[4 * x + 64 * j + c] = e[c] * by;
+    }
+}
+template <typename T, int DM>
+__device__ __forceinline__ void put_row(T* to, int x, uint32_t dim, const float4 (&v)[DM / 64], float by) {
+#pragma unroll
+    for (int j = 0; j < DM / 64; ++j) {
+        const float e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if ((uint32_t)(4 * x + 64 * j + c) < dim) to[4 * x + 64 * j + c] = fg_narrow<T>(e[c] * by);
+    }
+}
+__device__ __forceinline__ float half_warp_max(float v) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float half_warp_sum(float v) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// The keys of share z of a sequence.
+__device__ __forceinline__ void share(const FgAttnArgs& a, uint32_t nk, uint32_t z, uint32_t* lo, uint32_t* hi) {
+    const uint32_t least = (nk / a.splits + 64) / 64 * 64, each = a.splits == 1 ? nk : least > a.chunk ? least : a.chunk;
+    const uint64_t from = (uint64_t)z * each;
+    *lo = from < nk ? (uint32_t)from : nk;
+    *hi = from + each < nk ? (uint32_t)(from + each) : nk;
+}
+
+constexpr int kKeys = 64;
+constexpr size_t rows_bytes(int rt, int dm) { return sizeof(float) * ((size_t)(16 * rt + 2 * kKeys) * (dm + 4) + 16 * rt * (kKeys + 4)); }
+template <typename T, int RT, int DM>
+__global__ void __launch_bounds__(kThreads) attn_rows_kernel(const FgAttnArgs a) {
+    constexpr int R = 16 * RT, kPitch = DM + 4, kP = kKeys + 4;
+    extern __shared__ float shared[];
+    float *const qs = shared, *const ks = qs + R * kPitch, *const vs = ks + kKeys * kPitch, *const ps = vs + kKeys * kPitch;
+    fg_grid_enter();
+    uint32_t tile;
+    const int b = fg_attn_find(a.q_starts, a.sequences, a.queries, a.group, R, gridDim.x - 1 - blockIdx.x, &tile);
+    if (b < 0) return;
+    const FgAttnSeq s(a, b);
+    const uint64_t rows = (uint64_t)s.nq * a.group, first = (uint64_t)tile * R;
+    if (first >= rows) return;
+    const uint32_t n = rows - first < R ? (uint32_t)(rows - first) : R, kv = blockIdx.y, dim = a.dim;
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+    const T *const q = static_cast<const T*>(a.q), *const k = static_cast<const T*>(a.k) + (uint64_t)s.k0 * a.k_stride + (uint64_t)kv * dim,
+                  *const v = static_cast<const T*>(a.v) + (uint64_t)s.k0 * a.v_stride + (uint64_t)kv * dim;
+    fetch<T, R, DM>(qs, n, dim, [&](uint32_t r) {
+        const uint64_t at = first + r;
+        const uint32_t i = (uint32_t)(at / a.group), g = (uint32_t)(at - (uint64_t)i * a.group);
+        return q + (uint64_t)(s.q0 + i) * a.q_stride + (uint64_t)(kv * a.group + g) * dim;
+    });
+    uint32_t seen[RT];
+    float top[RT], sum[RT];
+    float4 acc[RT][DM / 64];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const uint32_t r = y * RT + i;
+        seen[i] = r < n ? s.seen(a, (uint32_t)((first + r) / a.group)) : 0;
+        top[i] = -INFINITY;
+        sum[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < DM / 64; ++j) acc[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    uint32_t lo, hi;
+    share(a, s.nk, blockIdx.z, &lo, &hi);
+    hi = min(hi, s.seen(a, (uint32_t)((first + n - 1) / a.group)));
+    const float by = a.scale * kFgLog2e;
+    for (uint32_t j0 = lo; j0 < hi; j0 += kKeys) {
+        const uint32_t there = min((uint32_t)kKeys, s.nk - j0);
+        __syncthreads();
+        fetch<T, kKeys, DM>(ks, there, dim, [&](uint32_t r) { return k + (uint64_t)(j0 + r) * a.k_stride; });
+        fetch<T, kKeys, DM>(vs, there, dim, [&](uint32_t r) { return v + (uint64_t)(j0 + r) * a.v_stride; });
+        __syncthreads();
+        float p[RT][4];
+        dots<RT, 4, DM>(qs, ks, dim, y * RT, x, p);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t key = j0 + x + 16 * j;
+                p[i][j] = key < seen[i] && key < hi ? p[i][j] * by : -INFINITY;
+                most = fmaxf(most, p[i][j]);
+            }
+            most = fmaxf(half_warp_max(most), top[i]);
+            const float base = most == -INFINITY ? 0.0f : most, less = fg_ex2_fast(top[i] - base);
+            float l = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                p[i][j] = fg_ex2_fast(p[i][j] - base);
+                l += p[i][j];
+                ps[(y * RT + i) * kP + x + 16 * j] = p[i][j];
+            }
+            top[i] = most;
+            sum[i] = __fmaf_rn(sum[i], less, half_warp_sum(l));
+#pragma unroll
+            for (int j = 0; j < DM / 64; ++j) { acc[i][j].x *= less; acc[i][j].y *= less; acc[i][j].z *= less; acc[i][j].w *= less; }
+        }
+        __syncwarp();
+        for (int c = 0; c < kKeys; c += 4) {
+            float4 w[RT];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) w[i] = *reinterpret_cast<const float4*>(ps + (y * RT + i) * kP + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float u[RT];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) u[i] = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+                add_row<RT, DM>(vs + (c + e) * kPitch, x, u, acc);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const uint32_t r = y * RT + i;
+        if (r >= n) continue;
+        const uint64_t at = first + r;
+        const uint32_t row = s.q0 + (uint32_t)(at / a.group), head = kv * a.group + (uint32_t)(at % a.group);
+        const uint64_t line = (uint64_t)row * a.heads + head;
+        if (a.splits > 1) {
+            const uint64_t part = (uint64_t)blockIdx.z * a.queries * a.heads + line;
+            put_row<DM>(a.part_out + part * dim, x, dim, acc[i], 1.0f);
+            if (x == 0) a.part_stat[part] = make_float2(top[i], sum[i]);
+        } else {
+            put_row<T, DM>(static_cast<T*>(a.out) + line * dim, x, dim, acc[i], sum[i] == 0.0f ? 0.0f : 1.0f / sum[i]);
+            if (x == 0 && a.lse) a.lse[(uint64_t)head * a.queries + row] = (top[i] + __log2f(sum[i])) * kFgLn2;
+        }
+    }
+}
+
+// Shares of the keys joined: a warp per row.  The same numbering of rows as the kernel before it, 8 rows a block.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) attn_join_kernel(const FgAttnArgs a) {
+    fg_grid_enter();
+    uint32_t tile;
+    const int b = fg_attn_find(a.q_starts, a.sequences, a.queries, a.heads, 8, blockIdx.x, &tile);
+    if (b < 0) return;
+    const FgAttnSeq s(a, b);
+    const uint64_t at = (uint64_t)tile * 8 + (threadIdx.x >> 5);
+    if (at >= (uint64_t)s.nq * a.heads) return;
+    const uint32_t lane = threadIdx.x & 31, row = s.q0 + (uint32_t)(at / a.heads), head = (uint32_t)(at % a.heads);
+    const uint64_t line = (uint64_t)row * a.heads + head, pitch = (uint64_t)a.queries * a.heads;
+    float top = -INFINITY;
+    for (uint32_t z = lane; z < a.splits; z += 32) top = fmaxf(top, a.part_stat[z * pitch + line].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, acc[kMaxDim / 32];
+#pragma unroll
+    for (int c = 0; c < (int)kMaxDim / 32; ++c) acc[c] = 0.0f;
+    for (uint32_t z = 0; z < a.splits; ++z) {
+        const float2 st = a.part_stat[z * pitch + line];
+        if (st.y == 0.0f) continue;
+        const float w = fg_ex2_fast(st.x - base), *const p = a.part_out + (z * pitch + line) * a.dim;
+        sum = __fmaf_rn(w, st.y, sum);
+#pragma unroll
+        for (int c = 0; c < (int)kMaxDim / 32; ++c)
+            if (lane + 32 * c < a.dim) acc[c] = __fmaf_rn(w, p[lane + 32 * c], acc[c]);
+    }
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* const out = static_cast<T*>(a.out) + line * a.dim;
+#pragma unroll
+    for (int c = 0; c < (int)kMaxDim / 32; ++c)
+        if (lane + 32 * c < a.dim) out[lane + 32 * c] = fg_narrow<T>(acc[c] * by);
+    if (lane == 0 && a.lse) a.lse[(uint64_t)head * a.queries + row] = (top + __log2f(sum)) * kFgLn2;
+}
+
+// delta_i = dout_i . out_i, a warp per row; [heads][queries].
+template <typename T>
+__global__ void __launch_bounds__(kThreads) attn_delta_kernel(const T* out, const T* dout, float* delta, uint32_t queries, uint32_t heads, uint32_t dim) {
+    fg_grid_enter();
+    const uint64_t line = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (line >= (uint64_t)queries * heads) return;
+    const uint32_t lane = threadIdx.x & 31;
+    float s = 0.0f;
+    for (uint32_t d = lane; d < dim; d += 32) s = __fmaf_rn(fg_widen(out[line * dim + d]), fg_widen(dout[line * dim + d]), s);
+    s = fg_warp_sum(s);
+    if (lane == 0) delta[(line % heads) * queries + line / heads] = s;
+}
+
+constexpr size_t bwd_bytes(int dm) { return sizeof(float) * (4 * (size_t)tile_of(dm) * (dm + 4) + 2 * tile_of(dm) * (tile_of(dm) + 4) + 2 * tile_of(dm)); }
+// The weights and the gradients of the scores of a tile of rows and keys, in shared memory by row.
+template <typename T, int DM>
+struct BwdTile {
+    static constexpr int N = tile_of(DM), RT = N / 16, kPitch = DM + 4, kP = N + 4;
+    float *qs, *dos, *ks, *vs, *ps, *ds, *stat;      // stat: lse in powers of two, delta
+    __device__ __forceinline__ explicit BwdTile(float* shared) {
+        qs = shared;
+        dos = qs + N * kPitch;
+        ks = dos + N * kPitch;
+        vs = ks + N * kPitch;
+        ps = vs + N * kPitch;
+        ds = ps + N * kP;
+        stat = ds + N * kP;
+    }
+    __device__ __forceinline__ void keys(const FgAttnArgs& a, const FgAttnSeq& s, uint32_t kv, uint32_t j0) {
+        const uint32_t n = s.nk - j0;
+        fetch<T, N, DM>(ks, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.k) + (uint64_t)(s.k0 + j0 + r) * a.k_stride + (uint64_t)kv * a.dim; });
+        fetch<T, N, DM>(vs, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.v) + (uint64_t)(s.k0 + j0 + r) * a.v_stride + (uint64_t)kv * a.dim; });
+    }
+    __device__ __forceinline__ void rows(const FgAttnArgs& a, const FgAttnSeq& s, uint32_t kv, uint64_t first, uint32_t n) {
+        auto place = [&](uint32_t r, uint32_t* i, uint32_t* head) {
+            const uint64_t at = first + r;
+            *i = s.q0 + (uint32_t)(at / a.group);
+            *head = kv * a.group + (uint32_t)(at % a.group);
+        };
+        fetch<T, N, DM>(qs, n, a.dim, [&](uint32_t r) {
+            uint32_t i, h;
+            place(r, &i, &h);
+            return static_cast<const T*>(a.q) + (uint64_t)i * a.q_stride + (uint64_t)h * a.dim;
+        });
+        fetch<T, N, DM>(dos, n, a.dim, [&](uint32_t r) {
+            uint32_t i, h;
+            place(r, &i, &h);
+            return static_cast<const T*>(a.dout) + ((uint64_t)i * a.heads + h) * a.dim;
+        });
+        if (threadIdx.x < N) {
+            uint32_t i = 0, h = 0;
+            float lse = 0.0f, delta = 0.0f;
+            if (threadIdx.x < n) {
+                place(threadIdx.x, &i, &h);
+                lse = a.lse_in[(uint64_t)h * a.queries + i];
+                delta = a.delta[(uint64_t)h * a.queries + i];
+            }
+            stat[threadIdx.x] = lse == -INFINITY ? INFINITY : lse * kFgLog2e;      // a row that saw nothing weighs nothing
+            stat[N + threadIdx.x] = delta;
+        }
+    }
+    // Rows first .. first + n of the sequence against keys from j0 on; p is left out where it is not wanted.
+    template <bool kP_>
+    __device__ __forceinline__ void weights(const FgAttnArgs& a, const FgAttnSeq& s, uint64_t first, uint32_t n, uint32_t j0) {
+        const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+        float p[RT][RT], dp[RT][RT];
+        dots<RT, RT, DM>(qs, ks, a.dim, y * RT, x, p);
+        dots<RT, RT, DM>(dos, vs, a.dim, y * RT, x, dp);
+        const float by = a.scale * kFgLog2e;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const uint32_t r = y * RT + i, seen = r < n ? s.seen(a, (uint32_t)((first + r) / a.group)) : 0;
+            const float lse = stat[r], delta = stat[N + r];
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                const float w = j0 + x + 16 * j < seen ? fg_ex2_fast(__fmaf_rn(p[i][j], by, -lse)) : 0.0f;
+                if (kP_) ps[r * kP + x + 16 * j] = w;
+                ds[r * kP + x + 16 * j] = w == 0.0f ? 0.0f : w * (dp[i][j] - delta);
+            }
+        }
+    }
+};
+
+template <typename T, int DM>
+__global__ void __launch_bounds__(kThreads) attn_dq_kernel(const FgAttnArgs a) {
+    using B = BwdTile<T, DM>;
+    constexpr int N = B::N, RT = B::RT;
+    extern __shared__ float shared[];
+    fg_grid_enter();
+    B t(shared);
+    uint32_t tile;
+    const int b = fg_attn_find(a.q_starts, a.sequences, a.queries, a.group, N, gridDim.x - 1 - blockIdx.x, &tile);
+    if (b < 0) return;
+    const FgAttnSeq s(a, b);
+    const uint64_t rows = (uint64_t)s.nq * a.group, first = (uint64_t)tile * N;
+    if (first >= rows) return;
+    const uint32_t n = rows - first < N ? (uint32_t)(rows - first) : N, kv = blockIdx.y;
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+    t.rows(a, s, kv, first, n);
+    float4 acc[RT][DM / 64] = {};
+    const uint32_t hi = s.seen(a, (uint32_t)((first + n - 1) / a.group));
+    for (uint32_t j0 = 0; j0 < hi; j0 += N) {
+        __syncthreads();
+        t.keys(a, s, kv, j0);
+        __syncthreads();
+        t.template weights<false>(a, s, first, n, j0);
+        __syncwarp();
+        for (int c = 0; c < N; c += 4) {
+            float4 w[RT];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) w[i] = *reinterpret_cast<const float4*>(t.ds + (y * RT + i) * B::kP + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float u[RT];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) u[i] = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+                add_row<RT, DM>(t.ks + (c + e) * B::kPitch, x, u, acc);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const uint32_t r = y * RT + i;
+        if (r >= n) continue;
+        const uint64_t at = first + r;
+        T* const to = static_cast<T*>(a.dq) + (s.q0 + at / a.group) * a.q_stride + (kv * a.group + at % a.group) * a.dim;
+        put_row<T, DM>(to, x, a.dim, acc[i], a.scale);
+    }
+}
+
+template <typename T, int DM>
+__global__ void __launch_bounds__(kThreads) attn_dkv_kernel(const FgAttnArgs a) {
+    using B = BwdTile<T, DM>;
+    constexpr int N = B::N, RT = B::RT;
+    extern __shared__ float shared[];
+    fg_grid_enter();
+    B t(shared);
+    uint32_t tile;
+    const int b = fg_attn_find(a.k_starts, a.sequences, a.keys, 1, N, blockIdx.x, &tile);
+    if (b < 0) return;
+    const FgAttnSeq s(a, b);
+    const uint64_t j0_ = (uint64_t)tile * N;
+    if (j0_ >= s.nk) return;
+    const uint32_t j0 = (uint32_t)j0_, kv = blockIdx.y;
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+    t.keys(a, s, kv, j0);
+    float4 dk[RT][DM / 64] = {}, dv[RT][DM / 64] = {};
+    const uint64_t rows = (uint64_t)s.nq * a.group;
+    for (uint64_t first = (uint64_t)s.first_query(a, j0) * a.group; first < rows; first += N) {
+        const uint32_t n = rows - first < N ? (uint32_t)(rows - first) : N;
+        __syncthreads();
+        t.rows(a, s, kv, first, n);
+        __syncthreads();
+        t.template weights<true>(a, s, first, n, j0);
+        __syncthreads();
+        for (int r = 0; r < N; ++r) {
+            float p[RT], d[RT];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                p[i] = t.ps[r * B::kP + y * RT + i];
+                d[i] = t.ds[r * B::kP + y * RT + i];
+            }
+            add_row<RT, DM>(t.dos + r * B::kPitch, x, p, dv);
+            add_row<RT, DM>(t.qs + r * B::kPitch, x, d, dk);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const uint32_t j = j0 + y * RT + i;
+        if (j >= s.nk) continue;
+        put_row<T, DM>(static_cast<T*>(a.dk) + (uint64_t)(s.k0 + j) * a.k_stride + (uint64_t)kv * a.dim, x, a.dim, dk[i], a.scale);
+        put_row<T, DM>(static_cast<T*>(a.dv) + (uint64_t)(s.k0 + j) * a.v_stride + (uint64_t)kv * a.dim, x, a.dim, dv[i], 1.0f);
+    }
+}
+
+// More shared memory than a kernel may have by default, to the most it is ever given: once per kernel (`done`) and device.
+template <typename K>
+int32_t allow_shared(fg_ctx* ctx, std::atomic<uint64_t>& done, K kernel, size_t bytes) {
+    if (bytes <= 48 * 1024 || done.load(std::memory_order_acquire) >> (ctx->device & 63) & 1ull) return FG_OK;
+    FG_CUDA(ctx, FG_ERR_INTERNAL, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    done.fetch_or(1ull << (ctx->device & 63), std::memory_order_release);
+    return FG_OK;
+}
+template <typename K>
+int32_t launch(fg_ctx* ctx, std::atomic<uint64_t>& done, K kernel, dim3 grid, size_t bytes, const FgAttnArgs& a) {
+    const int32_t s = allow_shared(ctx, done, kernel, bytes);
+    if (s != FG_OK) return s;
+    fg_launch(ctx, kernel, grid, kThreads, bytes, a);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
+}
+template <typename T, int RT, int DM>
+int32_t rows_launch(fg_ctx* ctx, const FgAttnArgs& a) {
+    static std::atomic<uint64_t> done{0};
+    const dim3 grid((unsigned)fg_attn_tiles(a.sequences, a.queries, a.group, 16 * RT), a.kv_heads, a.splits);
+    return launch(ctx, done, attn_rows_kernel<T, RT, DM>, grid, rows_bytes(RT, DM), a);
+}
+template <typename T, int DM>
+int32_t dq_launch(fg_ctx* ctx, const FgAttnArgs& a) {
+    static std::atomic<uint64_t> done{0};
+    return launch(ctx, done, attn_dq_kernel<T, DM>, dim3((unsigned)fg_attn_tiles(a.sequences, a.queries, a.group, tile_of(DM)), a.kv_heads), bwd_bytes(DM), a);
+}
+template <typename T, int DM>
+int32_t dkv_launch(fg_ctx* ctx, const FgAttnArgs& a) {
+    static std::atomic<uint64_t> done{0};
+    return launch(ctx, done, attn_dkv_kernel<T, DM>, dim3((unsigned)fg_attn_tiles(a.sequences, a.keys, 1, tile_of(DM)), a.kv_heads), bwd_bytes(DM), a);
+}
+
+// Few queries per sequence leave few blocks of rows, so their keys go in shares, about eight blocks for an SM; one share has 256 keys at least.
+int32_t in_shares(fg_ctx* ctx, FgAttnArgs& a) {
+    const uint64_t units = (uint64_t)a.keys * a.kv_heads / (8ull * ctx->sm_count);
+    const uint64_t chunk = (units < 256 ? 256 : units > 4096 ? 4096 : units) / 64 * 64, usual = a.keys / a.sequences + 1;
+    uint64_t splits = (a.sequences == 1 ? usual : 4 * usual) / chunk + 1;
+    if (splits > 128) splits = 128;
+    a.chunk = (uint32_t)chunk;
+    a.splits = (uint32_t)splits;
+    if (splits == 1) return FG_OK;
+    const uint64_t lines = splits * a.queries * a.heads;
+    void* w;
+    const int32_t s = fg_ws_alloc(ctx, lines * (4ull * a.dim + 8), &w);
+    if (s != FG_OK) return s;
+    a.part_stat = (float2*)w;
+    a.part_out = (float*)w + 2 * lines;
+    return FG_OK;
+}
+
+template <typename T>
+int32_t attention_fwd(fg_ctx* ctx, FgAttnArgs a) {
+    const bool few = (uint64_t)a.queries * a.group <= 16ull * a.sequences;
+    a.splits = 1;
+    if (few) {
+        const int32_t s = in_shares(ctx, a);
+        if (s != FG_OK) return s;
+    }
+    int32_t s;
+    if (few) s = a.dim <= 64 ? rows_launch<T, 1, 64>(ctx, a) : a.dim <= 128 ? rows_launch<T, 1, 128>(ctx, a) : rows_launch<T, 1, 256>(ctx, a);
+    else s = a.dim <= 64 ? rows_launch<T, 4, 64>(ctx, a) : a.dim <= 128 ? rows_launch<T, 4, 128>(ctx, a) : rows_launch<T, 4, 256>(ctx, a);
+    if (s != FG_OK || a.splits == 1) return s;
+    fg_launch(ctx, attn_join_kernel<T>, (unsigned)fg_attn_tiles(a.sequences, a.queries, a.heads, 8), kThreads, 0, a);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
+}
+
+template <typename T>
+int32_t attention_bwd(fg_ctx* ctx, FgAttnArgs a) {
+    a.splits = 1;
+    const uint64_t lines = (uint64_t)a.queries * a.heads;
+    void* w;
+    int32_t s = fg_ws_alloc(ctx, 4 * lines, &w);
+    if (s != FG_OK) return s;
+    a.delta = (const float*)w;
+    if (lines) {
+        fg_launch(ctx, attn_delta_kernel<T>, (unsigned)((lines + 7) / 8), kThreads, 0, (const T*)a.out, (const T*)a.dout, (float*)w, a.queries, a.heads, a.dim);
+        FG_LAUNCHED(ctx);
+    }
+    if (a.dq && lines) {
+        s = a.dim <= 64 ? dq_launch<T, 64>(ctx, a) : a.dim <= 128 ? dq_launch<T, 128>(ctx, a) : dq_launch<T, 256>(ctx, a);
+        if (s != FG_OK) return s;
+    }
+    if (a.dk && a.keys) {
+        s = a.dim <= 64 ? dkv_launch<T, 64>(ctx, a) : a.dim <= 128 ? dkv_launch<T, 128>(ctx, a) : dkv_launch<T, 256>(ctx, a);
+        if (s != FG_OK) return s;
+    }
+    return FG_OK;
+}
+
+// Bytes from the first to behind the last element of a tensor of `rows` tokens.
+uint64_t extent(uint64_t rows, uint64_t stride, uint64_t line, uint32_t size) { return rows ? ((rows - 1) * stride + line) * size : 0; }
+
+// What both passes ask of their arguments; strides of 0 become those of dense tensors.
+int32_t check(fg_ctx* ctx, int32_t dtype, FgAttnArgs& a) {
+    FG_REQUIRE(ctx, fg_dtype_known(dtype), "attention: unknown dtype");
+    FG_REQUIRE(ctx, a.heads >= 1 && a.kv_heads >= 1 && a.heads % a.kv_heads == 0, "attention: heads must be a multiple of kv_heads");
+    FG_REQUIRE(ctx, a.kv_heads <= 65535, "attention: too many heads");
+    FG_REQUIRE(ctx, a.dim >= 1 && a.dim <= kMaxDim, "attention: head_dim must be 1 to 256");
+    FG_REQUIRE(ctx, a.queries < (1u << 31) && a.keys < (1u << 31) && a.sequences < (1u << 24) && a.heads < (1u << 20), "attention: tensor too large");
+    FG_REQUIRE(ctx, a.scale >= -3.402823466e38f && a.scale <= 3.402823466e38f, "attention: scale must be a number");
+    const uint64_t q_line = (uint64_t)a.heads * a.dim, k_line = (uint64_t)a.kv_heads * a.dim;
+    if (!a.q_stride) a.q_stride = q_line;
+    if (!a.k_stride) a.k_stride = k_line;
+    if (!a.v_stride) a.v_stride = k_line;
+    FG_REQUIRE(ctx, a.q_stride >= q_line && a.k_stride >= k_line && a.v_stride >= k_line, "attention: a stride is shorter than a token's heads");
+    FG_REQUIRE(ctx, a.q_stride < (1u << 30) && a.k_stride < (1u << 30) && a.v_stride < (1u << 30), "attention: stride too large");
+    a.group = a.heads / a.kv_heads;
+    FG_REQUIRE(ctx, fg_attn_tiles(a.sequences, a.queries, a.heads, 8) < (1ull << 31), "attention: tensor too large");
+    FG_REQUIRE(ctx, !a.queries || (a.q && a.out), "attention: NULL pointer");
+    FG_REQUIRE(ctx, !a.keys || (a.k && a.v), "attention: NULL pointer");
+    FG_REQUIRE(ctx, !a.sequences || (a.q_starts && a.k_starts), "attention: NULL pointer");
+    const uint32_t size = fg_dtype_size(dtype);
+    FG_REQUIRE(ctx, fg_at_element(a.q, size) && fg_at_element(a.k, size) && fg_at_element(a.v, size) && fg_at_element(a.out, size) && fg_at_element(a.lse, 4) &&
+                        fg_at_element(a.lse_in, 4) && fg_at_element(a.dout, size) && fg_at_element(a.dq, size) && fg_at_element(a.dk, size) &&
+                        fg_at_element(a.dv, size) && fg_at_element(a.q_starts, 4) && fg_at_element(a.k_starts, 4) && fg_at_element(a.k_lengths, 4),
+               "attention: a tensor does not start at an element");
+    return FG_OK;
+}
+struct Range { const void* p; uint64_t n; };
+// Do two tensors of tokens share an element?  Rows of `line` bytes, `stride` apart: q, k and v of one product lie between each other's rows.
+bool rows_meet(const void* p, uint64_t np, const void* q, uint64_t nq, uint64_t stride, uint64_t p_line, uint64_t q_line) {
+    if (!fg_ranges_meet(p, np, q, nq)) return false;
+    const int64_t d = (int64_t)(reinterpret_cast<intptr_t>(q) - reinterpret_cast<intptr_t>(p));
+    int64_t r = d % (int64_t)stride;
+    if (r < 0) r += stride;
+    return (uint64_t)r < p_line || (uint64_t)r + q_line > stride;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t fg_attention_fwd(fg_ctx* ctx, int32_t dtype, uint32_t sequences, uint32_t queries, uint32_t keys, uint32_t heads, uint32_t kv_heads,
+                         uint32_t head_dim, const uint32_t* q_starts, const uint32_t* k_starts, const uint32_t* k_lengths, const void* q,
+                         uint64_t q_stride, const void* k, uint64_t k_stride, const void* v, uint64_t v_stride, float scale, int32_t causal,
+                         void* out, float* lse_out) {
+    FG_ENTER(ctx);
+    FgAttnArgs a{};
+    a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse_out;
+    a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
+    a.q_starts = q_starts; a.k_starts = k_starts; a.k_lengths = k_lengths;
+    a.sequences = sequences; a.queries = queries; a.keys = keys; a.heads = heads; a.kv_heads = kv_heads; a.dim = head_dim;
+    a.scale = scale; a.causal = causal != 0; a.dev_status = ctx->dev_status;
+    const int32_t s = check(ctx, dtype, a);
+    if (s != FG_OK) return s;
+    const uint32_t size = fg_dtype_size(dtype);
+    const uint64_t q_line = (uint64_t)heads * head_dim, k_line = (uint64_t)kv_heads * head_dim, out_bytes = queries * q_line * size, lse_bytes = 4ull * queries * heads;
+    const Range in[] = {{q, extent(queries, a.q_stride, q_line, size)}, {k, extent(keys, a.k_stride, k_line, size)}, {v, extent(keys, a.v_stride, k_line, size)},
+                        {q_starts, 4ull * sequences + 4}, {k_starts, 4ull * sequences + 4}, {k_lengths, 4ull * sequences}};
+    for (const Range& r : in)
+        FG_REQUIRE(ctx, !fg_ranges_meet(out, out_bytes, r.p, r.n) && !fg_ranges_meet(lse_out, lse_bytes, r.p, r.n), "fg_attention_fwd: an output overlaps another tensor");
+    FG_REQUIRE(ctx, !fg_ranges_meet(out, out_bytes, lse_out, lse_bytes), "fg_attention_fwd: an output overlaps another tensor");
+    if (!queries || !sequences) return FG_OK;
+    return FG_BY_DTYPE(dtype, attention_fwd, ctx, a);
+}
+
+int32_t fg_attention_bwd(fg_ctx* ctx, int32_t dtype, uint32_t sequences, uint32_t queries, uint32_t keys, uint32_t heads, uint32_t kv_heads,
+                         uint32_t head_dim, const uint32_t* q_starts, const uint32_t* k_starts, const uint32_t* k_lengths, const void* q,
+                         uint64_t q_stride, const void* k, uint64_t k_stride, const void* v, uint64_t v_stride, float scale, int32_t causal,
+                         const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv) {
+    FG_ENTER(ctx);
+    FgAttnArgs a{};
+    a.q = q; a.k = k; a.v = v; a.out = const_cast<void*>(out); a.lse_in = lse; a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv;
+    a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
+    a.q_starts = q_starts; a.k_starts = k_starts; a.k_lengths = k_lengths;
+    a.sequences = sequences; a.queries = queries; a.keys = keys; a.heads = heads; a.kv_heads = kv_heads; a.dim = head_dim;
+    a.scale = scale; a.causal = causal != 0; a.dev_status = ctx->dev_status;
+    const int32_t s = check(ctx, dtype, a);
+    if (s != FG_OK) return s;
+    FG_REQUIRE(ctx, dq || dk || dv, "fg_attention_bwd: no output");
+    FG_REQUIRE(ctx, !dk == !dv, "fg_attention_bwd: dk and dv go together");
+    FG_REQUIRE(ctx, !queries || (lse && dout), "fg_attention_bwd: NULL pointer");
+    const uint32_t size = fg_dtype_size(dtype);
+    const uint64_t q_line = (uint64_t)heads * head_dim, k_line = (uint64_t)kv_heads * head_dim, out_bytes = queries * q_line * size;
+    const uint64_t nq = extent(queries, a.q_stride, q_line, size), nk = extent(keys, a.k_stride, k_line, size), nv = extent(keys, a.v_stride, k_line, size);
+    const Range in[] = {{q, nq}, {k, nk}, {v, nv}, {out, out_bytes}, {dout, out_bytes}, {lse, 4ull * queries * heads},
+                        {q_starts, 4ull * sequences + 4}, {k_starts, 4ull * sequences + 4}, {k_lengths, 4ull * sequences}};
+    for (const Range& r : in)
+        FG_REQUIRE(ctx, !fg_ranges_meet(dq, nq, r.p, r.n) && !fg_ranges_meet(dk, nk, r.p, r.n) && !fg_ranges_meet(dv, nv, r.p, r.n),
+                   "fg_attention_bwd: a gradient overlaps another tensor");
+    // The gradients may be rows of one tensor, as q, k and v are: between each other's rows, not in them.
+    auto apart = [&](const void* p, uint64_t np, uint64_t ps, uint64_t pl, const void* r, uint64_t nr, uint64_t rs, uint64_t rl) {
+        return ps == rs ? !rows_meet(p, np, r, nr, ps * size, pl * size, rl * size) : !fg_ranges_meet(p, np, r, nr);
+    };
+    FG_REQUIRE(ctx, apart(dq, nq, a.q_stride, q_line, dk, nk, a.k_stride, k_line) && apart(dq, nq, a.q_stride, q_line, dv, nv, a.v_stride, k_line) &&
+                        apart(dk, nk, a.k_stride, k_line, dv, nv, a.v_stride, k_line), "fg_attention_bwd: gradients overlap");
+    if (!sequences) return FG_OK;
+    return FG_BY_DTYPE(dtype, attention_bwd, ctx, a);
+}
+
+}  // extern "C"

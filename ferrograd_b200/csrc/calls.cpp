@@ -181,6 +181,8 @@ PyMethodDef methods[] = {
     FG_METHOD(fg_gemm_batched_f32), FG_METHOD(fg_gemm_batched_bwd_f32), FG_METHOD(fg_gemm_lowp), FG_METHOD(fg_gemm_bwd_lowp),
     FG_METHOD(fg_bias_act_fwd), FG_METHOD(fg_act_bwd), FG_METHOD(fg_softmax_fwd), FG_METHOD(fg_softmax_bwd),
     FG_METHOD(fg_softmax_ce_fwd_bwd), FG_METHOD(fg_layernorm_fwd), FG_METHOD(fg_layernorm_bwd), FG_METHOD(fg_embedding_fwd), FG_METHOD(fg_embedding_bwd),
+    FG_METHOD(fg_attention_fwd), FG_METHOD(fg_attention_bwd), FG_METHOD(fg_rmsnorm_fwd), FG_METHOD(fg_rmsnorm_fwd_e4m3), FG_METHOD(fg_rmsnorm_bwd),
+    FG_METHOD(fg_logprobs_fwd), FG_METHOD(fg_logprobs_bwd),
     FG_METHOD(fg_sample), FG_METHOD(fg_ce_loss_grad), FG_METHOD(fg_mse_loss_grad), FG_METHOD(fg_bce_loss_grad),
     FG_METHOD(fg_sgd_step), FG_METHOD(fg_convert), FG_METHOD(fg_plan_launch),
     FG_METHOD(fg_exec_dispatch_forward), FG_METHOD(fg_exec_dispatch_loss), FG_METHOD(fg_exec_dispatch_backward), FG_METHOD(fg_exec_dispatch_optim),

@@ -349,6 +349,78 @@ int32_t fg_sample(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, cons
                   const float* temperature, const uint32_t* top_k, const float* top_p, const float* min_p,
                   uint32_t* token_out, float* prob_out);
 
+/* ---- a decoder block and a policy's loss: attention, root-mean-square norm, log probabilities (no counterpart in the reference) ----
+ * Attention over packed sequences.  q and out hold `queries` rows (tokens) of heads x head_dim, k and v `keys` rows of
+ * kv_heads x head_dim; heads is a multiple of kv_heads, and query head h uses head h / (heads / kv_heads) of k and v.  Sequence b has the
+ * queries q_starts[b] to q_starts[b + 1] and, from row k_starts[b] on, k_starts[b + 1] - k_starts[b] keys, or k_lengths[b] of them where
+ * k_lengths is given (a cache's slots; NULL: all).  Starts are device arrays of [sequences + 1] that must not decrease, read when the
+ * kernels run and held to the tensors' sizes there.  With nq queries and nk keys, query i of a sequence sees
+ *   causal != 0   keys j <= i + nk - nq: the last query sees all keys, and queries that have none before them see nothing
+ *   causal == 0   all keys
+ * out = softmax_j(scale * q_i . k_j) v_j for each head.  A row that sees nothing (or only scores of -inf) is zero.  lse_out (f32 [heads, queries], may be
+ * NULL) is log(sum_j exp(scale * q_i . k_j)), -inf for a row that sees nothing; the backward pass takes it.  Rows that belong to no sequence are
+ * left as they were, and so are their gradients.  A key behind its sequence's end reaches nothing, whatever its rows hold.  A NaN or an infinity in v
+ * (in the backward pass: in any tensor) may reach the rows of its own sequence that do not see it.
+ * q_stride, k_stride and v_stride are elements from a token to the next, 0 for dense ones: q, k and v may be columns of
+ * one tensor.  head_dim is at most 256.  16-bit tensors with head_dim a multiple of 8 up to 128, on 16-byte boundaries with strides that are multiples of 8, are
+ * multiplied on the tensor cores: the weights, and backward the gradients of the scores, are then rounded to the
+ * storage type before they are multiplied with v, dout, k and q.  Everything else runs in f32.  Up to 16 (query, head of a group) rows per
+ * sequence on average (generated tokens) the keys of a sequence are shared out over the device.  An output that overlaps an
+ * input is refused. */
+int32_t fg_attention_fwd(fg_ctx* ctx, int32_t dtype, uint32_t sequences, uint32_t queries, uint32_t keys,
+                         uint32_t heads, uint32_t kv_heads, uint32_t head_dim, const uint32_t* q_starts,
+                         const uint32_t* k_starts, const uint32_t* k_lengths, const void* q, uint64_t q_stride,
+                         const void* k, uint64_t k_stride, const void* v, uint64_t v_stride, float scale,
+                         int32_t causal, void* out, float* lse_out);
+/* The gradients of q, k and v, of the gradient dout of out; out and lse are the forward pass's.  dq, dk and dv lie as q, k and v do (the same
+ * strides: they may be columns of one tensor); dq may be NULL, and dk with dv.  Sums run in an order that the lengths and sizes
+ * decide, no sum is added atomically: the same call gives the same bits. */
+int32_t fg_attention_bwd(fg_ctx* ctx, int32_t dtype, uint32_t sequences, uint32_t queries, uint32_t keys,
+                         uint32_t heads, uint32_t kv_heads, uint32_t head_dim, const uint32_t* q_starts,
+                         const uint32_t* k_starts, const uint32_t* k_lengths, const void* q, uint64_t q_stride,
+                         const void* k, uint64_t k_stride, const void* v, uint64_t v_stride, float scale,
+                         int32_t causal, const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                         void* dv);
+
+/* h = x + residual (rounded to the storage type; residual may be NULL: h = x), y = h * rstd * gamma for each row with
+ * rstd = 1 / sqrt(mean(h * h) + eps), eps > 0.  gamma ([cols]) may be NULL: ones.  sum_out gets h (may be NULL), rstd_out (f32 [rows], may be NULL) is what the backward
+ * pass takes.  sum_out and y may each be x or the residual, but are two tensors; any other overlap of an output with a tensor of the call is refused. */
+int32_t fg_rmsnorm_fwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* x, const void* residual,
+                       const void* gamma, float eps, void* sum_out, void* y, float* rstd_out);
+/* The same with y in 8 bits (e4m3: 4 bits of exponent, 3 of fraction, largest number 448): for each group of `group` columns (32, 64, 128 or
+ * 256; the last group of a row may be shorter; 0: the whole row) scale_out[row, group] = (largest |y| of the group) / 448, and the bytes are y / scale,
+ * rounded to nearest even.  scale_out is f32 [rows, groups of a row].  A group of zeros has scale 0 and bytes 0. */
+int32_t fg_rmsnorm_fwd_e4m3(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* x,
+                            const void* residual, const void* gamma, float eps, uint32_t group, void* sum_out,
+                            uint8_t* y, float* scale_out, float* rstd_out);
+/* x is h of the forward pass (sum_out, or x where no residual was given).  With n = x * rstd and g = dy * gamma:
+ *   dx = dsum + rstd * (g - n * mean_row(g * n))     (skipped when NULL; dsum, what reaches h by other ways, may be NULL)
+ *   dgamma [cols] = column sums of dy * n            (skipped when NULL; accumulate_params adds into it)
+ * dx is the gradient of x and of the residual alike.  dx may be x, dy or dsum; any other overlap is refused.  Orders of sums as for fg_layernorm_bwd. */
+int32_t fg_rmsnorm_bwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* x, const void* dy,
+                       const void* gamma, const float* rstd, const void* dsum, void* dx, void* dgamma,
+                       int32_t accumulate_params);
+
+/* For each row of logits [rows, cols], with z = scale * logits (scale > 0: one over a temperature):
+ *   lse_out      log(sum(exp(z)))                               f32 [rows]
+ *   logprob_out  z[targets[row]] - lse                          f32 [rows]
+ *   entropy_out  -sum(p * log p) with p = exp(z - lse)          f32 [rows]
+ *   top_ids_out, top_logprobs_out [rows, top]: the top largest logits from the largest down, of equal ones the lowest index
+ *                first, and their log probabilities; top <= 64 and <= cols, 0: none
+ * Each output may be NULL, not all of them.  targets may be NULL where logprob_out is; a target of cols or more (0xffffffff, say) is padding: the row's
+ * numbers are 0 and its top entries FG_NO_TOKEN and -inf.  Logits of -inf have no weight and are never among the
+ * top; a row with no others has lse and log probability -inf, entropy 0.  A row with NaN or +inf has NaN statistics, and NaN is never among the top.
+ * An output that overlaps another tensor is refused. */
+int32_t fg_logprobs_fwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* logits,
+                        const uint32_t* targets, float scale, float* logprob_out, float* entropy_out, float* lse_out,
+                        uint32_t top, uint32_t* top_ids_out, float* top_logprobs_out);
+/* dlogits of the gradients dlogprob and dentropy (f32 [rows]; one may be NULL), with lse and (for dentropy) entropy of the forward pass:
+ *   dlogits[c] = scale * (dlogprob * ([c == target] - p_c) - dentropy * p_c * (log p_c + entropy))
+ * A row of padding, or with no logit above -inf, has a gradient of zero.  dlogits may be logits. */
+int32_t fg_logprobs_bwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* logits,
+                        const uint32_t* targets, float scale, const float* lse, const float* entropy,
+                        const float* dlogprob, const float* dentropy, void* dlogits);
+
 /* out[0] = sum of x[0..n), reduced in a fixed order (no counterpart in the reference, whose losses stay
  * unreduced: loss/basic_loss.rs:3-133; used to hand a caller one number per step instead of the loss tensor). */
 int32_t fg_sum_f32(fg_ctx* ctx, const float* x, uint64_t n, float* out);
