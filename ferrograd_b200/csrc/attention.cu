@@ -8,7 +8,7 @@
 // keys and goes over their rows, those of all heads of the group, for dk and dv: nothing is added in memory, so the order of sums is fixed.
 #include <atomic>
 
-#include "attention.cuh"
+#include "attention_tc.cuh"
 
 namespace {
 
@@ -476,6 +476,10 @@ template <typename T>
 int32_t attention_fwd(fg_ctx* ctx, FgAttnArgs a) {
     const bool few = (uint64_t)a.queries * a.group <= 16ull * a.sequences;
     a.splits = 1;
+    if constexpr (sizeof(T) == 2) {
+        constexpr int32_t dtype = std::is_same_v<T, __half> ? FG_DTYPE_F16 : FG_DTYPE_BF16;
+        if (!few && fg_attn_tc_suits(ctx, dtype, a)) return fg_attn_tc_fwd(ctx, dtype, a);
+    }
     if (few) {
         const int32_t s = in_shares(ctx, a);
         if (s != FG_OK) return s;
