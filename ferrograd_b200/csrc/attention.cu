@@ -496,6 +496,10 @@ int32_t attention_fwd(fg_ctx* ctx, FgAttnArgs a) {
 template <typename T>
 int32_t attention_bwd(fg_ctx* ctx, FgAttnArgs a) {
     a.splits = 1;
+    if constexpr (sizeof(T) == 2) {
+        constexpr int32_t dtype = std::is_same_v<T, __half> ? FG_DTYPE_F16 : FG_DTYPE_BF16;
+        if (fg_attn_tc_suits(ctx, dtype, a)) return fg_attn_tc_bwd(ctx, dtype, a);
+    }
     const uint64_t lines = (uint64_t)a.queries * a.heads;
     void* w;
     int32_t s = fg_ws_alloc(ctx, 4 * lines, &w);

@@ -19,7 +19,7 @@ struct FgAttnArgs {
     const void* dout;
     const float *lse_in, *delta;
     void *dq, *dk, *dv;
-    const float* gradient_scale;      // f16: the power of two that the tensor cores' operands are multiplied by, and its reciprocal
+    const uint32_t* most;      // f16 on the tensor cores: the largest |dout| and |v|, as bits
     int* dev_status;
 };
 
@@ -75,5 +75,3 @@ __device__ __forceinline__ int fg_attn_find(const uint32_t* starts, uint32_t seq
 inline uint64_t fg_attn_tiles(uint32_t sequences, uint32_t total, uint32_t per, uint32_t rows) { return (uint64_t)total * per / rows + sequences; }
 
 constexpr float kFgLog2e = 1.4426950408889634f, kFgLn2 = 0.6931471805599453f;
-// 2^(a - b) for b finite, or a = -inf.
-__device__ __forceinline__ float fg_pow2_fast(float a) { return fg_ex2_fast(a); }

@@ -60,7 +60,7 @@ attn_tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                    const __grid_constant__ FgAttnArgs a, uint32_t tokens, uint32_t tiles) {
     using Cfg = FwdCfg<DP>;
     constexpr int S = Cfg::kStages;
-    extern __shared__ unsigned char raw[];
+    extern __shared__ __align__(1024) unsigned char raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     const uint32_t qs = base, ring = base + 2 * Cfg::kTile, bar0 = ring + S * Cfg::kTile;
     auto q_full = [&](uint32_t s) { return bar0 + 8 * s; };
@@ -313,6 +313,567 @@ attn_tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     }
 }
 
+// ---- backward ----
+// Both kernels have a row (of dq) or a key (of dk, dv) per lane, two groups of four warps with half of the columns each, warp 8 loads, warp 9
+// multiplies.  Weights are made again from lse.  What a tile's threads leave in tensor memory as an A operand takes the place of what they
+// read: columns c / 2 behind the group's first.
+//
+// dq, by tiles of rows (their q and dout stay): for each tile of keys S = q k', dP = dout v', dS = P (dP - delta), dq += dS k.  Scores have two places, so
+// S(j + 1) is there when the weights of j + 1 are wanted: dP(j + 1) dq(j) S(j + 2) are multiplied while the threads work on j + 1.
+// dk and dv, by tiles of keys (their k and v stay): for each tile of rows S' = k q', dP' = v dout', dv += P' dout, dk += dS' q, in the order dv(i) S(i + 1)
+// dk(i) dP(i + 1): the weights of i + 1 are made while dk(i) and dP(i + 1) are multiplied, dS(i + 1) during dv(i + 1) and S(i + 2).
+// 7 products where one kernel that adds dq in memory would have 5, but no sum depends on who comes first, and nothing is read and written again.
+template <int DP>
+struct BwdCfg {
+    static constexpr int kTile = kHalfBytes * (DP / 64), kTwice = DP == 128 ? 3 : 4, kOnce = DP == 128 ? 2 : 3, kThreads = 384;
+    static constexpr int kBars = 1 + 2 * kTwice + 2 * kOnce + 2 + 1 + 2 + 1 + 2 + 2 + 1;
+    // the two tensors that stay, the rings, lse and delta of two tiles of rows, barriers, the tensor memory's address and a flag
+    static constexpr size_t kUsed = (size_t)(2 + kTwice + kOnce) * kTile + 2 * 2 * kRows * 4 + 8 * kBars + 16;
+    static constexpr size_t kSmem = kUsed + (kUsed + 1024 <= 227 * 1024 ? 1024 : 227 * 1024 - kUsed);
+};
+// The f16 operands' factor: a power of two that brings the largest gradient of a score near 2^13, if dout and v are as large as they can be.
+__device__ __forceinline__ float gradient_factor(const uint32_t* most, uint32_t dim) {
+    const float m = __uint_as_float(most[0]) * __uint_as_float(most[1]) * (float)dim;
+    if (!(m > 0.0f && m < INFINITY)) return 1.0f;
+    const int e = 13 - ilogbf(m);
+    return ldexpf(1.0f, e > 60 ? 60 : e < -60 ? -60 : e);
+}
+// What both kernels begin and end with.
+template <int DP>
+struct BwdBlock {
+    using Cfg = BwdCfg<DP>;
+    uint32_t base, bar0, tmem;
+    bool go;
+    int warp, lane;
+    __device__ __forceinline__ uint32_t stay(uint32_t i) const { return base + i * Cfg::kTile; }                              // the tensors that stay
+    __device__ __forceinline__ uint32_t twice(uint32_t i) const { return base + (2 + i) * Cfg::kTile; }                       // the ring of what two products read
+    __device__ __forceinline__ uint32_t once(uint32_t i) const { return base + (2 + Cfg::kTwice + i) * Cfg::kTile; }          // the other
+    __device__ __forceinline__ uint32_t stats(uint32_t i) const { return base + (2 + Cfg::kTwice + Cfg::kOnce) * Cfg::kTile + i * (2 * kRows * 4); }
+    __device__ __forceinline__ uint32_t stay_full() const { return bar0; }
+    __device__ __forceinline__ uint32_t twice_full(uint32_t i) const { return bar0 + 8 * (1 + i); }
+    __device__ __forceinline__ uint32_t twice_empty(uint32_t i) const { return bar0 + 8 * (1 + Cfg::kTwice + i); }
+    __device__ __forceinline__ uint32_t once_full(uint32_t i) const { return bar0 + 8 * (1 + 2 * Cfg::kTwice + i); }
+    __device__ __forceinline__ uint32_t once_empty(uint32_t i) const { return bar0 + 8 * (1 + 2 * Cfg::kTwice + Cfg::kOnce + i); }
+    __device__ __forceinline__ uint32_t more(uint32_t i) const { return bar0 + 8 * (1 + 2 * Cfg::kTwice + 2 * Cfg::kOnce + i); }
+    __device__ __forceinline__ uint32_t s_full(uint32_t i) const { return more(i); }          // 2
+    __device__ __forceinline__ uint32_t dp_full() const { return more(2); }
+    __device__ __forceinline__ uint32_t p_ready() const { return more(3); }
+    __device__ __forceinline__ uint32_t ds_ready() const { return more(4); }
+    __device__ __forceinline__ uint32_t done() const { return more(5); }
+    __device__ __forceinline__ uint32_t stats_full(uint32_t i) const { return more(6 + i); }  // 2
+    __device__ __forceinline__ uint32_t stats_empty(uint32_t i) const { return more(8 + i); } // 2
+    __device__ __forceinline__ uint32_t drained() const { return more(10); }
+    // Dynamic shared memory starts on 1024 bytes, which the tiles need and the largest block has no room to make up for.
+    static __device__ __forceinline__ bool fits(const unsigned char* raw, const FgAttnArgs& a) {
+        const uint32_t at = smem_u32(raw);
+        if (((at + 1023u) & ~1023u) - at + Cfg::kUsed <= Cfg::kSmem) return true;
+        if (threadIdx.x == 0) atomicOr(a.dev_status, FG_DEVERR_TMA_WAIT);
+        return false;
+    }
+    __device__ __forceinline__ BwdBlock(unsigned char* raw, const FgAttnArgs& a) {
+        base = (smem_u32(raw) + 1023u) & ~1023u;
+        bar0 = stats(2);
+        unsigned char* const tail = raw + (bar0 + 8 * Cfg::kBars - smem_u32(raw));
+        volatile uint32_t* const slot = reinterpret_cast<volatile uint32_t*>(tail);
+        warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+        lane = threadIdx.x & 31;
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < Cfg::kBars; ++i) {
+                const int m = i - (1 + 2 * Cfg::kTwice + 2 * Cfg::kOnce);
+                mbar_init(bar0 + 8 * i, m == 3 || m == 4 || m == 8 || m == 9 ? 256 : m == 6 || m == 7 ? 64 : 1);
+            }
+            fence_mbar_init();
+        }
+        if (warp == 9) {
+            tmem_alloc(bar0 + 8 * Cfg::kBars, kTmemCols);
+            tmem_relinquish();
+        }
+        fg_grid_enter();
+        if (threadIdx.x == 0) slot[1] = (uint32_t)*reinterpret_cast<volatile int*>(a.dev_status);
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        tmem = __shfl_sync(0xffffffffu, slot[0], 0);
+        go = __all_sync(0xffffffffu, slot[1] == 0);
+    }
+    __device__ __forceinline__ void end() const {
+        __syncwarp();
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 9) {
+            tc_fence_after();
+            tmem_dealloc(tmem, kTmemCols);
+        }
+    }
+    // Loads are waited for by the warp that asked for them, and products by the one that issued them, whatever became of the other roles.
+    __device__ __forceinline__ void await_loads(uint32_t n, const FgAttnArgs& a) const {
+        if (!await(stay_full(), 0, a.dev_status, FG_DEVERR_TMA_WAIT)) return;
+        for (uint32_t i = n > (uint32_t)Cfg::kTwice ? n - Cfg::kTwice : 0; i < n; ++i)
+            if (!await(twice_full(i % Cfg::kTwice), (i / Cfg::kTwice) & 1, a.dev_status, FG_DEVERR_TMA_WAIT)) return;
+        for (uint32_t i = n > (uint32_t)Cfg::kOnce ? n - Cfg::kOnce : 0; i < n; ++i)
+            if (!await(once_full(i % Cfg::kOnce), (i / Cfg::kOnce) & 1, a.dev_status, FG_DEVERR_TMA_WAIT)) return;
+    }
+    __device__ __forceinline__ void drain(const FgAttnArgs& a) const {
+        if (elect_one()) mma_commit(drained());
+        __syncwarp();
+        await(drained(), 0, a.dev_status, FG_DEVERR_MMA_WAIT);
+    }
+    // Zeros for rows `from` on of a tile, as far as a product of 16 rows at a time reads.
+    __device__ __forceinline__ void clear(uint32_t tile, uint32_t from) const {
+        const uint32_t end = round_up(from, 16);
+        for (uint32_t i = from * 8 + lane; i < end * 8; i += 32)
+#pragma unroll
+            for (int h = 0; h < DP / 64; ++h) fg_store_shared(tile + h * kHalfBytes + i * 16, make_uint4(0, 0, 0, 0));
+        fence_proxy_async();
+        __syncwarp();
+    }
+    // 128 x n products of two tiles' rows over head_dim.
+    __device__ __forceinline__ void rows_by_rows(uint32_t d, uint32_t x, uint32_t y, uint32_t id, uint32_t steps) const {
+        const uint64_t x_d = make_desc_kmajor<128>(x), y_d = make_desc_kmajor<128>(y);
+        for (uint32_t c = 0; c < steps; ++c) {
+            const uint64_t at = (uint64_t)((c & 3) * 2 + (c >> 2) * (kHalfBytes >> 4));
+            mma_f16(d, x_d + at, y_d + at, id, c != 0);
+        }
+    }
+    // d += (what the two groups left behind `w`) times the first 16 * steps rows of a tile.
+    __device__ __forceinline__ void weights_by_rows(uint32_t d, uint32_t w, uint32_t tile, uint32_t id, uint32_t steps, uint32_t add) const {
+        const uint64_t t_d = make_desc_mnmajor(tile, kHalfBytes, 1024, 2);
+        for (uint32_t c = 0; c < steps; ++c) mma_f16_ta(d, w + (c & 3) * 8 + (c >> 2) * 64, t_d + (uint64_t)(c * 128), id, add | c);
+    }
+};
+
+// 64 sums of a lane, times f, as 16-bit columns from `to` on (`columns` of them are there).
+template <typename T, int N>
+__device__ __forceinline__ void put_sums(uint32_t from, T* to, bool there, int columns, float f) {
+#pragma unroll
+    for (int c = 0; c < N; c += 32) {
+        uint32_t o[32];
+        tmem_ld_32x32(from + c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+            const uint4 v = make_uint4(pack2<T>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f), pack2<T>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f),
+                                       pack2<T>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f), pack2<T>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f));
+            if (there && c + e < columns) *reinterpret_cast<uint4*>(to + c + e) = v;
+        }
+    }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(BwdCfg<DP>::kThreads, 1)
+attn_tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FgAttnArgs a, uint32_t tokens, uint32_t tiles) {
+    using Cfg = BwdCfg<DP>;
+    extern __shared__ __align__(1024) unsigned char raw[];
+    if (!BwdBlock<DP>::fits(raw, a)) return;
+    const BwdBlock<DP> blk(raw, a);
+    const int warp = blk.warp;
+    const uint32_t tmem = blk.tmem, t_dp = tmem + 256, t_dq = tmem + 384;      // scores at 0 and 128
+    const uint32_t kv = blockIdx.x % a.kv_heads;
+    uint32_t tile;
+    const int b = blk.go ? fg_attn_find(a.q_starts, a.sequences, a.queries, 1, tokens, tiles - 1 - blockIdx.x / a.kv_heads, &tile) : -1;
+    if (b >= 0) {
+        const FgAttnSeq s(a, b);
+        const uint64_t tok0_ = (uint64_t)tile * tokens;
+        const uint32_t tok0 = tok0_ < s.nq ? (uint32_t)tok0_ : s.nq, n_tok = min(tokens, s.nq - tok0);
+        const uint32_t hi = n_tok ? s.seen(a, tok0 + n_tok - 1) : 0, n = (hi + kRows - 1) / kRows;
+        const uint32_t fmt = kFormat<T>, dim16 = round_up(a.dim, 16), steps = dim16 / 16;
+        if (warp >= 8) reg_release<72>();
+        if (warp == 8) {
+            // ---- loads: q and dout, then k (read twice) and v ----
+            uint32_t j = 0;
+            for (; j < n; ++j) {
+                const uint32_t u = j % Cfg::kTwice, w = j % Cfg::kOnce;
+                if (!await(blk.twice_empty(u), ((j / Cfg::kTwice) & 1) ^ 1, a.dev_status, FG_DEVERR_TMA_WAIT)) break;
+                if (!await(blk.once_empty(w), ((j / Cfg::kOnce) & 1) ^ 1, a.dev_status, FG_DEVERR_TMA_WAIT)) break;
+                if (elect_one()) {
+                    if (j == 0) {
+                        mbar_expect_tx(blk.stay_full(), 2 * (DP / 64) * 128 * tokens * a.group);
+#pragma unroll
+                        for (int h = 0; h < DP / 64; ++h) {
+                            tma_load_3d(blk.stay(0) + h * kHalfBytes, &tm_q, blk.stay_full(), 64 * h, (int)(kv * a.group), (int)(s.q0 + tok0));
+                            tma_load_3d(blk.stay(1) + h * kHalfBytes, &tm_do, blk.stay_full(), 64 * h, (int)(kv * a.group), (int)(s.q0 + tok0));
+                        }
+                    }
+                    mbar_expect_tx(blk.twice_full(u), Cfg::kTile);
+                    mbar_expect_tx(blk.once_full(w), Cfg::kTile);
+#pragma unroll
+                    for (int h = 0; h < DP / 64; ++h) {
+                        tma_load_3d(blk.twice(u) + h * kHalfBytes, &tm_k, blk.twice_full(u), 64 * h, (int)kv, (int)(s.k0 + j * kRows));
+                        tma_load_3d(blk.once(w) + h * kHalfBytes, &tm_v, blk.once_full(w), 64 * h, (int)kv, (int)(s.k0 + j * kRows));
+                    }
+                }
+                __syncwarp();
+            }
+            if (j) blk.await_loads(j, a);
+        } else if (warp == 9) {
+            // ---- products ----
+            const uint32_t id_dq = make_idesc(fmt, 128, dim16) | kIdescBMnMajor;
+            auto cols = [&](uint32_t j) { return round_up(min((uint32_t)kRows, hi - j * kRows), 16); };
+            bool ok = n != 0 && await(blk.stay_full(), 0, a.dev_status, FG_DEVERR_MMA_WAIT);
+            auto scores = [&](uint32_t j) {
+                const uint32_t u = j % Cfg::kTwice;
+                if (!(ok = await(blk.twice_full(u), (j / Cfg::kTwice) & 1, a.dev_status, FG_DEVERR_MMA_WAIT))) return;
+                const uint32_t left = s.nk - j * kRows;
+                if (left < kRows && (left & 15)) blk.clear(blk.twice(u), left);      // dS of these keys is zero, k need not be a number
+                tc_fence_after();
+                if (elect_one()) {
+                    blk.rows_by_rows(tmem + (j & 1) * 128, blk.stay(0), blk.twice(u), make_idesc(fmt, 128, cols(j)), steps);
+                    mma_commit(blk.s_full(j & 1));
+                }
+                __syncwarp();
+            };
+            auto dp = [&](uint32_t j) {
+                const uint32_t w = j % Cfg::kOnce;
+                if (!(ok = await(blk.once_full(w), (j / Cfg::kOnce) & 1, a.dev_status, FG_DEVERR_MMA_WAIT))) return;
+                tc_fence_after();
+                if (elect_one()) {
+                    blk.rows_by_rows(t_dp, blk.stay(1), blk.once(w), make_idesc(fmt, 128, cols(j)), steps);
+                    mma_commit(blk.dp_full());
+                    mma_commit(blk.once_empty(w));
+                }
+                __syncwarp();
+            };
+            if (ok) scores(0);
+            if (ok) dp(0);
+            if (ok && n > 1) scores(1);
+            for (uint32_t j = 0; ok && j < n; ++j) {
+                if (!(ok = await(blk.ds_ready(), j & 1, a.dev_status, FG_DEVERR_MMA_WAIT))) break;
+                tc_fence_after();
+                if (j + 1 < n) dp(j + 1);
+                if (!ok) break;
+                if (elect_one()) {
+                    const uint32_t u = j % Cfg::kTwice;
+                    blk.weights_by_rows(t_dq, tmem + (j & 1) * 128, blk.twice(u), id_dq, cols(j) / 16, j);
+                    mma_commit(blk.twice_empty(u));
+                    if (j + 1 == n) mma_commit(blk.done());
+                }
+                __syncwarp();
+                if (j + 2 < n) scores(j + 2);
+            }
+            blk.drain(a);
+        } else if (warp < 8) {
+            reg_acquire<216>();
+            const uint32_t side = warp >> 2, r = threadIdx.x & 127, i = tok0 + r / a.group, head = kv * a.group + r % a.group;
+            const bool there = r / a.group < n_tok;
+            const uint32_t seen = there ? s.seen(a, i) : 0, lanes = (uint32_t)(warp & 3) << 21;
+            float lse = INFINITY, delta = 0.0f;
+            if (there) {
+                const uint64_t line = (uint64_t)head * a.queries + s.q0 + i;
+                lse = a.lse_in[line];
+                lse = lse == -INFINITY ? INFINITY : lse * kFgLog2e;
+                delta = a.delta[line];
+            }
+            const float factor = std::is_same_v<T, __half> ? gradient_factor(a.most, a.dim) : 1.0f, by = a.scale * kFgLog2e;
+            const float2 by2 = make_float2(by, by), lse2 = make_float2(-lse, -lse), factor2 = make_float2(factor, factor), delta2 = make_float2(-delta * factor, -delta * factor);
+            bool ok = true;
+            for (uint32_t j = 0; j < n; ++j) {
+                const uint32_t t_s = tmem + lanes + (j & 1) * 128 + side * 64;
+                if (!(ok = await(blk.s_full(j & 1), (j >> 1) & 1, a.dev_status, FG_DEVERR_EPI_WAIT))) break;
+                tc_fence_after();
+                uint32_t x[2][32], y[2][32];
+                tmem_ld_32x32(t_s, x[0]);
+                tmem_ld_32x32(t_s + 32, x[1]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) {
+                    const float2 e = fg_fma2(make_float2(__uint_as_float(x[c / 32][c % 32]), __uint_as_float(x[c / 32][c % 32 + 1])), by2, lse2);
+                    x[c / 32][c % 32] = __float_as_uint(fg_ex2_fast(e.x));
+                    x[c / 32][c % 32 + 1] = __float_as_uint(fg_ex2_fast(e.y));
+                }
+                if (!(ok = await(blk.dp_full(), j & 1, a.dev_status, FG_DEVERR_EPI_WAIT))) break;
+                tc_fence_after();
+                tmem_ld_32x32(t_dp + lanes + side * 64, y[0]);
+                tmem_ld_32x32(t_dp + lanes + side * 64 + 32, y[1]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) {
+                    float2 e = fg_fma2(make_float2(__uint_as_float(y[c / 32][c % 32]), __uint_as_float(y[c / 32][c % 32 + 1])), factor2, delta2);
+                    e = fg_mul2(e, make_float2(__uint_as_float(x[c / 32][c % 32]), __uint_as_float(x[c / 32][c % 32 + 1])));
+                    y[c / 32][c % 32] = __float_as_uint(e.x);
+                    y[c / 32][c % 32 + 1] = __float_as_uint(e.y);
+                }
+                const uint32_t from = j * kRows + side * 64, end = from < seen ? seen - from : 0;
+                if (__any_sync(0xffffffffu, end < 64))
+#pragma unroll
+                    for (int c = 0; c < 64; ++c)
+                        if ((uint32_t)c >= end) y[c / 32][c % 32] = 0;
+                uint32_t p[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) p[c] = pack2<T>(__uint_as_float(y[c / 16][c % 16 * 2]), __uint_as_float(y[c / 16][c % 16 * 2 + 1]));
+                tmem_st_32x32(t_s, p);
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(blk.ds_ready());
+            }
+            if (ok && n) ok = await(blk.done(), 0, a.dev_status, FG_DEVERR_EPI_WAIT);
+            if (ok && n_tok) {
+                tc_fence_after();
+                T* const to = static_cast<T*>(a.dq) + (uint64_t)(s.q0 + i) * a.q_stride + (uint64_t)head * a.dim + side * (DP / 2);
+                const int columns = (int)a.dim - (int)side * (DP / 2);
+                if (n) put_sums<T, DP / 2>(t_dq + lanes + side * (DP / 2), to, there, columns, a.scale / factor);
+                else if (there)
+                    for (int c = 0; c < DP / 2 && c < columns; c += 8) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
+            }
+        }
+    }
+    blk.end();
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(BwdCfg<DP>::kThreads, 1)
+attn_tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_k,
+                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FgAttnArgs a, uint32_t tokens) {
+    using Cfg = BwdCfg<DP>;
+    extern __shared__ __align__(1024) unsigned char raw[];
+    if (!BwdBlock<DP>::fits(raw, a)) return;
+    const BwdBlock<DP> blk(raw, a);
+    const int warp = blk.warp, lane = blk.lane;
+    const uint32_t tmem = blk.tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;      // scores at 0
+    const uint32_t kv = blockIdx.x % a.kv_heads;
+    uint32_t tile;
+    const int b = blk.go ? fg_attn_find(a.k_starts, a.sequences, a.keys, 1, kRows, blockIdx.x / a.kv_heads, &tile) : -1;
+    if (b >= 0) {
+        const FgAttnSeq s(a, b);
+        const uint64_t j0_ = (uint64_t)tile * kRows;
+        const uint32_t j0 = j0_ < s.nk ? (uint32_t)j0_ : s.nk, n_key = min((uint32_t)kRows, s.nk - j0);
+        const uint32_t tok0 = n_key ? s.first_query(a, j0) : s.nq, n = (s.nq - tok0 + tokens - 1) / tokens;
+        const uint32_t fmt = kFormat<T>, dim16 = round_up(a.dim, 16), steps = dim16 / 16;
+        auto n_row = [&](uint32_t i) { return min(tokens, s.nq - tok0 - i * tokens) * a.group; };
+        if (warp >= 8) reg_release<72>();
+        if (warp == 8) {
+            // ---- loads: k and v, then q (read twice, and last) and dout ----
+            const uint32_t bytes = DP / 64 * 128 * tokens * a.group;
+            uint32_t i = 0;
+            for (; i < n; ++i) {
+                const uint32_t u = i % Cfg::kTwice, w = i % Cfg::kOnce;
+                const int at = (int)(s.q0 + tok0 + i * tokens);
+                if (!await(blk.twice_empty(u), ((i / Cfg::kTwice) & 1) ^ 1, a.dev_status, FG_DEVERR_TMA_WAIT)) break;
+                if (!await(blk.once_empty(w), ((i / Cfg::kOnce) & 1) ^ 1, a.dev_status, FG_DEVERR_TMA_WAIT)) break;
+                if (elect_one()) {
+                    if (i == 0) {
+                        mbar_expect_tx(blk.stay_full(), 2 * Cfg::kTile);
+#pragma unroll
+                        for (int h = 0; h < DP / 64; ++h) {
+                            tma_load_3d(blk.stay(0) + h * kHalfBytes, &tm_k, blk.stay_full(), 64 * h, (int)kv, (int)(s.k0 + j0));
+                            tma_load_3d(blk.stay(1) + h * kHalfBytes, &tm_v, blk.stay_full(), 64 * h, (int)kv, (int)(s.k0 + j0));
+                        }
+                    }
+                    mbar_expect_tx(blk.twice_full(u), bytes);
+                    mbar_expect_tx(blk.once_full(w), bytes);
+#pragma unroll
+                    for (int h = 0; h < DP / 64; ++h) {
+                        tma_load_3d(blk.twice(u) + h * kHalfBytes, &tm_q, blk.twice_full(u), 64 * h, (int)(kv * a.group), at);
+                        tma_load_3d(blk.once(w) + h * kHalfBytes, &tm_do, blk.once_full(w), 64 * h, (int)(kv * a.group), at);
+                    }
+                }
+                __syncwarp();
+            }
+            if (i) blk.await_loads(i, a);
+        } else if (warp == 9) {
+            // ---- products ----
+            const uint32_t id_sum = make_idesc(fmt, 128, dim16) | kIdescBMnMajor;
+            bool ok = n != 0 && await(blk.stay_full(), 0, a.dev_status, FG_DEVERR_MMA_WAIT);
+            // (rows behind the sequence's end weigh nothing, but may not be numbers: zeros, and no product goes further)
+            auto scores = [&](uint32_t i) {
+                const uint32_t u = i % Cfg::kTwice, rows = n_row(i);
+                if (!(ok = await(blk.twice_full(u), (i / Cfg::kTwice) & 1, a.dev_status, FG_DEVERR_MMA_WAIT))) return;
+                if (rows & 15) blk.clear(blk.twice(u), rows);
+                tc_fence_after();
+                if (elect_one()) {
+                    blk.rows_by_rows(tmem, blk.stay(0), blk.twice(u), make_idesc(fmt, 128, round_up(rows, 16)), steps);
+                    mma_commit(blk.s_full(0));
+                }
+                __syncwarp();
+            };
+            auto dp = [&](uint32_t i) {
+                const uint32_t w = i % Cfg::kOnce, rows = n_row(i);
+                if (!(ok = await(blk.once_full(w), (i / Cfg::kOnce) & 1, a.dev_status, FG_DEVERR_MMA_WAIT))) return;
+                if (rows & 15) blk.clear(blk.once(w), rows);
+                tc_fence_after();
+                if (elect_one()) {
+                    blk.rows_by_rows(t_dp, blk.stay(1), blk.once(w), make_idesc(fmt, 128, round_up(rows, 16)), steps);
+                    mma_commit(blk.dp_full());
+                }
+                __syncwarp();
+            };
+            if (ok) scores(0);
+            if (ok) dp(0);
+            for (uint32_t i = 0; ok && i < n; ++i) {
+                const uint32_t row_steps = (n_row(i) + 15) / 16;
+                if (!(ok = await(blk.p_ready(), i & 1, a.dev_status, FG_DEVERR_MMA_WAIT))) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    blk.weights_by_rows(t_dv, tmem, blk.once(i % Cfg::kOnce), id_sum, row_steps, i);
+                    mma_commit(blk.once_empty(i % Cfg::kOnce));
+                }
+                __syncwarp();
+                if (i + 1 < n) scores(i + 1);
+                if (!ok || !(ok = await(blk.ds_ready(), i & 1, a.dev_status, FG_DEVERR_MMA_WAIT))) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    blk.weights_by_rows(t_dk, t_dp, blk.twice(i % Cfg::kTwice), id_sum, row_steps, i);
+                    mma_commit(blk.twice_empty(i % Cfg::kTwice));
+                    if (i + 1 == n) mma_commit(blk.done());
+                }
+                __syncwarp();
+                if (i + 1 < n) dp(i + 1);
+            }
+            blk.drain(a);
+        } else if (warp >= 10) {
+            // ---- lse (in powers of two; infinite where a row weighs nothing) and delta of the tiles' rows ----
+            const float factor = std::is_same_v<T, __half> ? gradient_factor(a.most, a.dim) : 1.0f;
+            const uint32_t first = (warp - 10) * 32 + lane;
+            for (uint32_t i = 0; i < n; ++i) {
+                if (!await(blk.stats_empty(i & 1), ((i >> 1) & 1) ^ 1, a.dev_status, FG_DEVERR_TMA_WAIT)) break;
+                const uint32_t rows = n_row(i);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t r = first + 64 * h;
+                    float lse = INFINITY, delta = 0.0f;
+                    if (r < rows) {
+                        const uint64_t line = (uint64_t)(kv * a.group + r % a.group) * a.queries + s.q0 + tok0 + i * tokens + r / a.group;
+                        lse = a.lse_in[line];
+                        lse = lse == -INFINITY ? INFINITY : lse * kFgLog2e;
+                        delta = a.delta[line] * factor;
+                    }
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(blk.stats(i & 1) + 4 * r), "f"(-lse) : "memory");
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(blk.stats(i & 1) + 4 * (kRows + r)), "f"(-delta) : "memory");
+                }
+                mbar_arrive(blk.stats_full(i & 1));
+            }
+        } else {
+            reg_acquire<216>();
+            const uint32_t side = warp >> 2, key = j0 + (threadIdx.x & 127), lanes = (uint32_t)(warp & 3) << 21;
+            const bool there = (threadIdx.x & 127) < n_key;
+            const uint32_t first = there ? s.first_query(a, key) : s.nq;      // the first query that sees the key
+            const float factor = std::is_same_v<T, __half> ? gradient_factor(a.most, a.dim) : 1.0f, by = a.scale * kFgLog2e;
+            const float2 by2 = make_float2(by, by), factor2 = make_float2(factor, factor);
+            bool ok = true;
+            for (uint32_t i = 0; i < n; ++i) {
+                const uint32_t t_s = tmem + lanes + side * 64, stat = blk.stats(i & 1) + side * 256;
+                if (!(ok = await(blk.stats_full(i & 1), (i >> 1) & 1, a.dev_status, FG_DEVERR_EPI_WAIT))) break;
+                if (!(ok = await(blk.s_full(0), i & 1, a.dev_status, FG_DEVERR_EPI_WAIT))) break;
+                tc_fence_after();
+                uint32_t x[2][32], y[2][32], p[32];
+                tmem_ld_32x32(t_s, x[0]);
+                tmem_ld_32x32(t_s + 32, x[1]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 64; c += 4) {
+                    const uint4 l = fg_load_shared(stat + 4 * c);
+                    float2 e = fg_fma2(make_float2(__uint_as_float(x[c / 32][c % 32]), __uint_as_float(x[c / 32][c % 32 + 1])), by2, make_float2(__uint_as_float(l.x), __uint_as_float(l.y)));
+                    x[c / 32][c % 32] = __float_as_uint(fg_ex2_fast(e.x));
+                    x[c / 32][c % 32 + 1] = __float_as_uint(fg_ex2_fast(e.y));
+                    e = fg_fma2(make_float2(__uint_as_float(x[c / 32][c % 32 + 2]), __uint_as_float(x[c / 32][c % 32 + 3])), by2, make_float2(__uint_as_float(l.z), __uint_as_float(l.w)));
+                    x[c / 32][c % 32 + 2] = __float_as_uint(fg_ex2_fast(e.x));
+                    x[c / 32][c % 32 + 3] = __float_as_uint(fg_ex2_fast(e.y));
+                }
+                // Columns before `start` do not see the key.
+                const uint32_t at = tok0 + i * tokens, skip = (first > at ? min(first - at, tokens) : 0) * a.group, start = skip > side * 64 ? skip - side * 64 : 0;
+                const bool some = __any_sync(0xffffffffu, start != 0);
+                if (some)
+#pragma unroll
+                    for (int c = 0; c < 64; ++c)
+                        if ((uint32_t)c < start) x[c / 32][c % 32] = 0;
+#pragma unroll
+                for (int c = 0; c < 32; ++c) p[c] = pack2<T>(__uint_as_float(x[c / 16][c % 16 * 2]), __uint_as_float(x[c / 16][c % 16 * 2 + 1]));
+                tmem_st_32x32(t_s, p);
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(blk.p_ready());
+                if (!(ok = await(blk.dp_full(), i & 1, a.dev_status, FG_DEVERR_EPI_WAIT))) break;
+                tc_fence_after();
+                tmem_ld_32x32(t_s + 128, y[0]);
+                tmem_ld_32x32(t_s + 160, y[1]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 64; c += 4) {
+                    const uint4 l = fg_load_shared(stat + 4 * (kRows + c));
+                    float2 e = fg_fma2(make_float2(__uint_as_float(y[c / 32][c % 32]), __uint_as_float(y[c / 32][c % 32 + 1])), factor2, make_float2(__uint_as_float(l.x), __uint_as_float(l.y)));
+                    e = fg_mul2(e, make_float2(__uint_as_float(x[c / 32][c % 32]), __uint_as_float(x[c / 32][c % 32 + 1])));
+                    y[c / 32][c % 32] = __float_as_uint(e.x);
+                    y[c / 32][c % 32 + 1] = __float_as_uint(e.y);
+                    e = fg_fma2(make_float2(__uint_as_float(y[c / 32][c % 32 + 2]), __uint_as_float(y[c / 32][c % 32 + 3])), factor2, make_float2(__uint_as_float(l.z), __uint_as_float(l.w)));
+                    e = fg_mul2(e, make_float2(__uint_as_float(x[c / 32][c % 32 + 2]), __uint_as_float(x[c / 32][c % 32 + 3])));
+                    y[c / 32][c % 32 + 2] = __float_as_uint(e.x);
+                    y[c / 32][c % 32 + 3] = __float_as_uint(e.y);
+                }
+                mbar_arrive(blk.stats_empty(i & 1));
+                if (some)
+#pragma unroll
+                    for (int c = 0; c < 64; ++c)
+                        if ((uint32_t)c < start) y[c / 32][c % 32] = 0;
+#pragma unroll
+                for (int c = 0; c < 32; ++c) p[c] = pack2<T>(__uint_as_float(y[c / 16][c % 16 * 2]), __uint_as_float(y[c / 16][c % 16 * 2 + 1]));
+                tmem_st_32x32(t_s + 128, p);
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(blk.ds_ready());
+            }
+            if (ok && n) ok = await(blk.done(), 0, a.dev_status, FG_DEVERR_EPI_WAIT);
+            if (ok && n_key) {
+                tc_fence_after();
+                T* const to = side ? static_cast<T*>(a.dk) + (uint64_t)(s.k0 + key) * a.k_stride + (uint64_t)kv * a.dim
+                                   : static_cast<T*>(a.dv) + (uint64_t)(s.k0 + key) * a.v_stride + (uint64_t)kv * a.dim;
+                if (n) put_sums<T, DP>((side ? t_dk : t_dv) + lanes, to, there, (int)a.dim, side ? a.scale / factor : 1.0f);
+                else if (there)
+                    for (uint32_t c = 0; c < a.dim; c += 8) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
+            }
+        }
+    }
+    blk.end();
+}
+
+// delta_i = dout_i . out_i: L lanes of 16 bytes per row of a head, [heads][queries].
+template <typename T, int L>
+__global__ void __launch_bounds__(256) attn_tc_delta_kernel(const FgAttnArgs a, float* delta) {
+    constexpr int kLines = 256 / L * 4;      // of (query, head): four per thread
+    fg_grid_enter();
+    const uint32_t sub = threadIdx.x % L;
+    const uint64_t lines = (uint64_t)a.queries * a.heads, first = (uint64_t)blockIdx.x * kLines + threadIdx.x / L;
+    uint4 x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint64_t line = first + i * (256 / L), at = line * a.dim + sub * 8;
+        const bool there = line < lines && sub * 8 < a.dim;
+        x[i] = there ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.out) + at) : make_uint4(0, 0, 0, 0);
+        y[i] = there ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dout) + at) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint64_t line = first + i * (256 / L);
+        float u[8], v[8], d = 0.0f;
+        FgPack<T>::widen(x[i], u);
+        FgPack<T>::widen(y[i], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d = __fmaf_rn(u[e], v[e], d);
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        if (sub == 0 && line < lines) delta[line % a.heads * a.queries + line / a.heads] = d;
+    }
+}
+// The largest |x| of the sequences' rows (as bits, so NaN is larger than infinity): 64 rows of `line` 16-byte words a block.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_most_kernel(const FgAttnArgs a, const T* x, uint64_t stride, uint32_t line, int keys, uint32_t* most) {
+    fg_grid_enter();
+    uint32_t tile;
+    const int b = fg_attn_find(keys ? a.k_starts : a.q_starts, a.sequences, keys ? a.keys : a.queries, 1, 64, blockIdx.x, &tile);
+    if (b < 0) return;
+    const FgAttnSeq s(a, b);
+    const uint64_t n = keys ? s.nk : s.nq, r0 = (uint64_t)tile * 64;
+    uint32_t m = 0;
+    for (uint64_t r = r0 + (threadIdx.x >> 5); r < n && r < r0 + 64; r += 8)
+        for (uint32_t c = threadIdx.x & 31; c < line; c += 32) {
+            float v[8];
+            FgPack<T>::widen(*reinterpret_cast<const uint4*>(x + ((keys ? s.k0 : s.q0) + r) * stride + c * 8), v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(fabsf(v[e])));
+        }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((threadIdx.x & 31) == 0 && m) atomicMax(most, m);      // (the largest of numbers: whoever comes first)
+}
+
 // ---- host ----
 typedef CUresult (*pfn_encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -359,10 +920,60 @@ int32_t fwd_launch(fg_ctx* ctx, const FgAttnArgs& a) {
     return FG_OK;
 }
 
+template <typename T, int DP>
+int32_t bwd_launch(fg_ctx* ctx, FgAttnArgs a) {
+    using Cfg = BwdCfg<DP>;
+    constexpr bool half = std::is_same_v<T, __half>;
+    const uint64_t lines = (uint64_t)a.queries * a.heads;
+    void* w;
+    int32_t s = fg_ws_alloc(ctx, 256 + 4 * lines, &w);
+    if (s != FG_OK) return s;
+    uint32_t* const most = static_cast<uint32_t*>(w);
+    float* const delta = static_cast<float*>(w) + 64;
+    a.most = most;
+    a.delta = delta;
+    const uint32_t lanes = a.dim > 64 ? 16 : a.dim > 32 ? 8 : a.dim > 16 ? 4 : a.dim > 8 ? 2 : 1, per = 1024 / lanes;
+    const auto kernel = lanes == 16 ? attn_tc_delta_kernel<T, 16> : lanes == 8 ? attn_tc_delta_kernel<T, 8> : lanes == 4 ? attn_tc_delta_kernel<T, 4>
+                        : lanes == 2 ? attn_tc_delta_kernel<T, 2> : attn_tc_delta_kernel<T, 1>;
+    if (lines) {
+        fg_launch(ctx, kernel, (unsigned)((lines + per - 1) / per), 256, 0, a, delta);
+        FG_LAUNCHED(ctx);
+    }
+    if (half) {
+        FG_CUDA(ctx, FG_ERR_FAILED_BUFFER_COPY, cudaMemsetAsync(most, 0, 8, ctx->stream));
+        fg_launch(ctx, attn_most_kernel<T>, (unsigned)fg_attn_tiles(a.sequences, a.queries, 1, 64), 256, 0, a, (const T*)a.dout, (uint64_t)a.heads * a.dim,
+                  a.heads * a.dim / 8, 0, most);
+        FG_LAUNCHED(ctx);
+        fg_launch(ctx, attn_most_kernel<T>, (unsigned)fg_attn_tiles(a.sequences, a.keys, 1, 64), 256, 0, a, (const T*)a.v, a.v_stride, a.kv_heads * a.dim / 8, 1, most + 1);
+        FG_LAUNCHED(ctx);
+    }
+    const uint32_t tokens = kRows / a.group;
+    CUtensorMap q, d, k, v;
+    if ((s = make_map(ctx, &q, a.q, half, a.dim, a.heads, a.queries, a.q_stride, a.group, tokens)) != FG_OK) return s;
+    if ((s = make_map(ctx, &d, a.dout, half, a.dim, a.heads, a.queries, (uint64_t)a.heads * a.dim, a.group, tokens)) != FG_OK) return s;
+    if ((s = make_map(ctx, &k, a.k, half, a.dim, a.kv_heads, a.keys, a.k_stride, 1, kRows)) != FG_OK) return s;
+    if ((s = make_map(ctx, &v, a.v, half, a.dim, a.kv_heads, a.keys, a.v_stride, 1, kRows)) != FG_OK) return s;
+    const uint64_t row_tiles = fg_attn_tiles(a.sequences, a.queries, 1, tokens), key_tiles = fg_attn_tiles(a.sequences, a.keys, 1, kRows);
+    if (row_tiles * a.kv_heads >= 1ull << 31 || key_tiles * a.kv_heads >= 1ull << 31) return fg_fail(ctx, FG_ERR_INVALID_ARGUMENT, "attention: tensor too large");
+    if (a.dq) {
+        static std::atomic<uint64_t> done{0};
+        if ((s = allow_shared(ctx, done, attn_tc_dq_kernel<T, DP>, Cfg::kSmem)) != FG_OK) return s;
+        fg_launch(ctx, attn_tc_dq_kernel<T, DP>, (unsigned)(row_tiles * a.kv_heads), Cfg::kThreads, Cfg::kSmem, q, d, k, v, a, tokens, (uint32_t)row_tiles);
+        FG_LAUNCHED(ctx);
+    }
+    if (a.dk) {
+        static std::atomic<uint64_t> done{0};
+        if ((s = allow_shared(ctx, done, attn_tc_dkv_kernel<T, DP>, Cfg::kSmem)) != FG_OK) return s;
+        fg_launch(ctx, attn_tc_dkv_kernel<T, DP>, (unsigned)(key_tiles * a.kv_heads), Cfg::kThreads, Cfg::kSmem, q, d, k, v, a, tokens);
+        FG_LAUNCHED(ctx);
+    }
+    return FG_OK;
+}
+
 }  // namespace
 
 bool fg_attn_tc_suits(const fg_ctx* ctx, int32_t dtype, const FgAttnArgs& a) {
-    if (dtype == FG_DTYPE_F32 || !ctx->tmap_encode || a.dim % 8 || a.dim > 128 || a.group > (uint32_t)kRows || !(a.scale > 0.0f) || !a.keys) return false;
+    if (dtype == FG_DTYPE_F32 || !ctx->tmap_encode || a.dim % 8 || a.dim > 128 || a.group > (uint32_t)kRows || !(a.scale > 0.0f) || !a.keys || !a.queries) return false;
     const uint64_t strides = a.q_stride | a.k_stride | a.v_stride;
     return strides % 8 == 0 && fg_aligned16(a.q) && fg_aligned16(a.k) && fg_aligned16(a.v) && fg_aligned16(a.out) && fg_aligned16(a.dout) && fg_aligned16(a.dq) &&
            fg_aligned16(a.dk) && fg_aligned16(a.dv);
@@ -370,4 +981,8 @@ bool fg_attn_tc_suits(const fg_ctx* ctx, int32_t dtype, const FgAttnArgs& a) {
 int32_t fg_attn_tc_fwd(fg_ctx* ctx, int32_t dtype, const FgAttnArgs& a) {
     if (dtype == FG_DTYPE_F16) return a.dim <= 64 ? fwd_launch<__half, 64>(ctx, a) : fwd_launch<__half, 128>(ctx, a);
     return a.dim <= 64 ? fwd_launch<__nv_bfloat16, 64>(ctx, a) : fwd_launch<__nv_bfloat16, 128>(ctx, a);
+}
+int32_t fg_attn_tc_bwd(fg_ctx* ctx, int32_t dtype, const FgAttnArgs& a) {
+    if (dtype == FG_DTYPE_F16) return a.dim <= 64 ? bwd_launch<__half, 64>(ctx, a) : bwd_launch<__half, 128>(ctx, a);
+    return a.dim <= 64 ? bwd_launch<__nv_bfloat16, 64>(ctx, a) : bwd_launch<__nv_bfloat16, 128>(ctx, a);
 }
