@@ -99,14 +99,6 @@ __device__ __forceinline__ float half_warp_sum(float v) {
     for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// The keys of share z of a sequence.
-__device__ __forceinline__ void share(const FgAttnArgs& a, uint32_t nk, uint32_t z, uint32_t* lo, uint32_t* hi) {
-    const uint32_t least = (nk / a.splits + 64) / 64 * 64, each = a.splits == 1 ? nk : least > a.chunk ? least : a.chunk;
-    const uint64_t from = (uint64_t)z * each;
-    *lo = from < nk ? (uint32_t)from : nk;
-    *hi = from + each < nk ? (uint32_t)(from + each) : nk;
-}
-
 constexpr int kKeys = 64;
 constexpr size_t rows_bytes(int rt, int dm) { return sizeof(float) * ((size_t)(16 * rt + 2 * kKeys) * (dm + 4) + 16 * rt * (kKeys + 4)); }
 template <typename T, int RT, int DM>
@@ -143,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const FgAttnArgs a)
         for (int j = 0; j < DM / 64; ++j) acc[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
     uint32_t lo, hi;
-    share(a, s.nk, blockIdx.z, &lo, &hi);
+    if (!s.share(a, blockIdx.z, &lo, &hi)) return;
     hi = min(hi, s.seen(a, (uint32_t)((first + n - 1) / a.group)));
     const float by = a.scale * kFgLog2e;
     for (uint32_t j0 = lo; j0 < hi; j0 += kKeys) {
@@ -221,15 +213,16 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(const FgAttnArgs a)
     if (at >= (uint64_t)s.nq * a.heads) return;
     const uint32_t lane = threadIdx.x & 31, row = s.q0 + (uint32_t)(at / a.heads), head = (uint32_t)(at % a.heads);
     const uint64_t line = (uint64_t)row * a.heads + head, pitch = (uint64_t)a.queries * a.heads;
+    const uint32_t splits = s.shares(a);
     float top = -INFINITY;
-    for (uint32_t z = lane; z < a.splits; z += 32) top = fmaxf(top, a.part_stat[z * pitch + line].x);
+    for (uint32_t z = lane; z < splits; z += 32) top = fmaxf(top, a.part_stat[z * pitch + line].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float base = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f, acc[kMaxDim / 32];
 #pragma unroll
     for (int c = 0; c < (int)kMaxDim / 32; ++c) acc[c] = 0.0f;
-    for (uint32_t z = 0; z < a.splits; ++z) {
+    for (uint32_t z = 0; z < splits; ++z) {
         const float2 st = a.part_stat[z * pitch + line];
         if (st.y == 0.0f) continue;
         const float w = fg_ex2_fast(st.x - base), *const p = a.part_out + (z * pitch + line) * a.dim;
@@ -454,10 +447,11 @@ int32_t dkv_launch(fg_ctx* ctx, const FgAttnArgs& a) {
     return launch(ctx, done, attn_dkv_kernel<T, DM>, dim3((unsigned)fg_attn_tiles(a.sequences, a.keys, 1, tile_of(DM)), a.kv_heads), bwd_bytes(DM), a);
 }
 
-// Few queries per sequence leave few blocks of rows, so their keys go in shares, about eight blocks for an SM; one share has 256 keys at least.
+// Few queries per sequence leave few blocks of rows, so their keys go in shares: about 24 blocks for an SM, each with 64 keys at least and
+// 4096 at most.
 int32_t in_shares(fg_ctx* ctx, FgAttnArgs& a) {
-    const uint64_t units = (uint64_t)a.keys * a.kv_heads / (8ull * ctx->sm_count);
-    const uint64_t chunk = (units < 256 ? 256 : units > 4096 ? 4096 : units) / 64 * 64, usual = a.keys / a.sequences + 1;
+    const uint64_t units = (uint64_t)a.keys * a.kv_heads / (24ull * ctx->sm_count);
+    const uint64_t chunk = (units < 64 ? 64 : units > 4096 ? 4096 : units) / 64 * 64, usual = a.keys / a.sequences + 1;
     uint64_t splits = (a.sequences == 1 ? usual : 4 * usual) / chunk + 1;
     if (splits > 128) splits = 128;
     a.chunk = (uint32_t)chunk;
@@ -472,20 +466,21 @@ int32_t in_shares(fg_ctx* ctx, FgAttnArgs& a) {
     return FG_OK;
 }
 
+template <typename T> constexpr int32_t dtype_of = sizeof(T) == 4 ? FG_DTYPE_F32 : std::is_same_v<T, __half> ? FG_DTYPE_F16 : FG_DTYPE_BF16;
+
 template <typename T>
 int32_t attention_fwd(fg_ctx* ctx, FgAttnArgs a) {
-    const bool few = (uint64_t)a.queries * a.group <= 16ull * a.sequences;
+    const uint64_t rows = ((uint64_t)a.queries * a.group + a.sequences - 1) / a.sequences;      // of a sequence, on average
+    const bool tc = fg_attn_tc_suits(ctx, dtype_of<T>, a), few = rows <= (tc ? 64 : 16);
     a.splits = 1;
-    if constexpr (sizeof(T) == 2) {
-        constexpr int32_t dtype = std::is_same_v<T, __half> ? FG_DTYPE_F16 : FG_DTYPE_BF16;
-        if (!few && fg_attn_tc_suits(ctx, dtype, a)) return fg_attn_tc_fwd(ctx, dtype, a);
-    }
+    if (tc && !few) return fg_attn_tc_fwd(ctx, dtype_of<T>, a);
     if (few) {
         const int32_t s = in_shares(ctx, a);
         if (s != FG_OK) return s;
     }
     int32_t s;
-    if (few) s = a.dim <= 64 ? rows_launch<T, 1, 64>(ctx, a) : a.dim <= 128 ? rows_launch<T, 1, 128>(ctx, a) : rows_launch<T, 1, 256>(ctx, a);
+    if (tc) s = fg_attn_few(ctx, dtype_of<T>, a, (uint32_t)rows);
+    else if (few) s = a.dim <= 64 ? rows_launch<T, 1, 64>(ctx, a) : a.dim <= 128 ? rows_launch<T, 1, 128>(ctx, a) : rows_launch<T, 1, 256>(ctx, a);
     else s = a.dim <= 64 ? rows_launch<T, 4, 64>(ctx, a) : a.dim <= 128 ? rows_launch<T, 4, 128>(ctx, a) : rows_launch<T, 4, 256>(ctx, a);
     if (s != FG_OK || a.splits == 1) return s;
     fg_launch(ctx, attn_join_kernel<T>, (unsigned)fg_attn_tiles(a.sequences, a.queries, a.heads, 8), kThreads, 0, a);
@@ -496,10 +491,7 @@ int32_t attention_fwd(fg_ctx* ctx, FgAttnArgs a) {
 template <typename T>
 int32_t attention_bwd(fg_ctx* ctx, FgAttnArgs a) {
     a.splits = 1;
-    if constexpr (sizeof(T) == 2) {
-        constexpr int32_t dtype = std::is_same_v<T, __half> ? FG_DTYPE_F16 : FG_DTYPE_BF16;
-        if (fg_attn_tc_suits(ctx, dtype, a)) return fg_attn_tc_bwd(ctx, dtype, a);
-    }
+    if (fg_attn_tc_suits(ctx, dtype_of<T>, a)) return fg_attn_tc_bwd(ctx, dtype_of<T>, a);
     const uint64_t lines = (uint64_t)a.queries * a.heads;
     void* w;
     int32_t s = fg_ws_alloc(ctx, 4 * lines, &w);

@@ -12,7 +12,7 @@ struct FgAttnArgs {
     void* out;
     float* lse;
     // keys in shares (few queries): a share leaves sums for the rows instead of rows.  splits == 1: none
-    uint32_t splits, chunk;      // keys of a share, a multiple of 64, if the sequence has no more than splits of them
+    uint32_t splits, chunk;      // a sequence has one share per chunk of keys (a multiple of 64), at most splits
     float* part_out;             // [splits][queries][heads][dim]
     float2* part_stat;           // [splits][queries][heads]: the largest score (in powers of 2) and the sum of weights
     // backward
@@ -34,6 +34,17 @@ struct FgAttnSeq {
         nq = q1 > q0 ? q1 - q0 : 0;
         nk = k1 > k0 ? k1 - k0 : 0;
         if (a.k_lengths) nk = min(nk, a.k_lengths[b]);
+    }
+    // Shares of this sequence's keys, equal ones of whole 64s; the keys of share z (false: there is none).
+    __device__ __forceinline__ uint32_t shares(const FgAttnArgs& a) const { return max(1u, min(a.splits, (nk + a.chunk - 1) / a.chunk)); }
+    __device__ __forceinline__ bool share(const FgAttnArgs& a, uint32_t z, uint32_t* lo, uint32_t* hi) const {
+        *lo = 0;
+        *hi = nk;
+        if (a.splits == 1) return true;
+        const uint32_t n = shares(a), each = ((nk + 63) / 64 + n - 1) / n * 64;
+        *lo = (uint32_t)min((uint64_t)nk, (uint64_t)z * each);
+        *hi = (uint32_t)min((uint64_t)nk, (uint64_t)*lo + each);
+        return z < n;
     }
     // Keys that query i sees, from the sequence's first on.
     __device__ __forceinline__ uint32_t seen(const FgAttnArgs& a, uint32_t i) const {

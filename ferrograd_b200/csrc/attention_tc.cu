@@ -313,6 +313,236 @@ attn_tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     }
 }
 
+// ---- few rows: generated tokens over a cache ----
+// What bounds this is the reading of the keys, so a block keeps 96 KB of them on their way, and 16 rows at a time ((query, head of the group) pairs) are
+// multiplied by the warps' own instructions.  A block has one share of a sequence's keys and one head of k and v.  Of its four warps kW have 16 rows each
+// (as many as a sequence has on average), the others the same rows against other keys of a stage; they are joined at the end.
+__device__ __forceinline__ void load_matrices(uint32_t from, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(from) : "memory");
+}
+__device__ __forceinline__ void load_matrices_turned(uint32_t from, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(from) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<T, __half>)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <int DP>
+struct FewCfg {
+    static constexpr int kKeys = 64, kHalf = kKeys * 128, kTile = kHalf * (DP / 64), kStages = 3 * 128 / DP, kThreads = 128;
+    static constexpr size_t kSmem = 1024 + (size_t)2 * kStages * kTile;
+};
+template <typename T, int DP, int kW>
+__global__ void __launch_bounds__(128)
+attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FgAttnArgs a) {
+    using Cfg = FewCfg<DP>;
+    constexpr int S = Cfg::kStages, kOwn = 16 * kW, kCols = kOwn / 8;      // keys of a stage that a warp has
+    extern __shared__ __align__(1024) unsigned char raw[];
+    __shared__ unsigned long long bars[S];
+    __shared__ float2 stat[4][16];
+    __shared__ int s_stop;
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u, bar0 = smem_u32(bars);
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp / kW;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i) mbar_init(bar0 + 8 * i, 1);
+        fence_mbar_init();
+    }
+    fg_grid_enter();
+    if (threadIdx.x == 0) s_stop = *reinterpret_cast<volatile int*>(a.dev_status);
+    __syncthreads();
+    const uint32_t kv = blockIdx.x % a.kv_heads, z = blockIdx.x / a.kv_heads % a.splits, b = blockIdx.x / a.kv_heads / a.splits;
+    const FgAttnSeq s(a, b);
+    uint32_t lo, hi_share;
+    if (s_stop || !s.nq || !s.share(a, z, &lo, &hi_share)) return;
+    const uint64_t rows = (uint64_t)s.nq * a.group;
+    const uint32_t steps = (a.dim + 15) / 16;
+    const float by = a.scale * kFgLog2e;
+    uint32_t g = 0;      // stages so far
+    for (uint64_t r0 = 0; r0 < rows; r0 += 16 * kW) {
+        const uint32_t n_row = (uint32_t)min((uint64_t)(16 * kW), rows - r0);
+        const uint32_t hi = min(hi_share, s.seen(a, (uint32_t)((r0 + n_row - 1) / a.group)));
+        const uint32_t n = hi > lo ? (hi - lo + Cfg::kKeys - 1) / Cfg::kKeys : 0;
+        auto ask = [&](uint32_t i) {      // by one thread
+            const uint32_t st = (g + i) % S, bar = bar0 + 8 * st, to = base + 2 * st * Cfg::kTile;
+            mbar_expect_tx(bar, 2 * Cfg::kTile);
+#pragma unroll
+            for (int h = 0; h < DP / 64; ++h) {
+                tma_load_3d(to + h * Cfg::kHalf, &tm_k, bar, 64 * h, (int)kv, (int)(s.k0 + lo + i * Cfg::kKeys));
+                tma_load_3d(to + Cfg::kTile + h * Cfg::kHalf, &tm_v, bar, 64 * h, (int)kv, (int)(s.k0 + lo + i * Cfg::kKeys));
+            }
+        };
+        if (threadIdx.x == 0)
+            for (uint32_t i = 0; i < n && i < (uint32_t)S; ++i) ask(i);
+        // Rows of this thread: lane / 4 and 8 more, of the warp's 16.
+        uint32_t q[DP / 16][4], seen[2];
+        const uint32_t own = (warp % kW) * 16 + lane / 4;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t r = own + 8 * e;
+            const bool there = r < n_row;
+            const uint32_t i = there ? (uint32_t)((r0 + r) / a.group) : 0, h = there ? (uint32_t)((r0 + r) % a.group) : 0;
+            seen[e] = there ? min(hi, s.seen(a, i)) : 0;
+            const T* const row = static_cast<const T*>(a.q) + (uint64_t)(s.q0 + i) * a.q_stride + (uint64_t)(kv * a.group + h) * a.dim;
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                    const uint32_t d = 16 * c + 8 * f + 2 * (lane % 4);
+                    q[c][2 * f + e] = there && d < a.dim ? *reinterpret_cast<const uint32_t*>(row + d) : 0;
+                }
+        }
+        float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, o[DP / 8][4];
+#pragma unroll
+        for (int c = 0; c < DP / 8; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[c][e] = 0.0f;
+        for (uint32_t i = 0; i < n; ++i) {
+            const uint32_t st = (g + i) % S, ks = base + 2 * st * Cfg::kTile, vs = ks + Cfg::kTile, j0 = lo + i * Cfg::kKeys;
+            if (!mbar_wait_bounded(bar0 + 8 * st, ((g + i) / S) & 1, kWaitCycles)) {
+                atomicOr(a.dev_status, FG_DEVERR_TMA_WAIT);
+                s_stop = 1;
+            }
+            if (j0 + Cfg::kKeys > s.nk) {      // v behind the sequence's end has a weight of zero, but need not be a number
+                const uint32_t from = s.nk - j0;
+                for (uint32_t w = from * 8 + threadIdx.x; w < Cfg::kKeys * 8; w += 128)
+#pragma unroll
+                    for (int h = 0; h < DP / 64; ++h) fg_store_shared(vs + h * Cfg::kHalf + w * 16, make_uint4(0, 0, 0, 0));
+                __syncthreads();
+            }
+            float p[kCols][4];
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[c][e] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) {
+                if ((uint32_t)c >= steps) break;
+#pragma unroll
+                for (int t = 0; t < kCols; t += 2) {
+                    uint32_t m[4];
+                    const uint32_t key = part * kOwn + 8 * t + (lane & 7) + (lane >> 4) * 8, chunk = 2 * (c & 3) + (lane >> 3 & 1);
+                    load_matrices(ks + (c >> 2) * Cfg::kHalf + key * 128 + ((chunk ^ (key & 7)) << 4), m);
+                    mma_16x8x16<T>(p[t], q[c], m[0], m[1]);
+                    mma_16x8x16<T>(p[t + 1], q[c], m[2], m[3]);
+                }
+            }
+            float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t key = j0 + part * kOwn + 8 * c + 2 * (lane % 4) + (e & 1);
+                    p[c][e] = key < seen[e >> 1] ? p[c][e] * by : -INFINITY;
+                    most[e >> 1] = fmaxf(most[e >> 1], p[c][e]);
+                }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], 1));
+                most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], 2));
+            }
+            if (__any_sync(0xffffffffu, most[0] > top[0] + 8.0f || most[1] > top[1] + 8.0f)) {      // (as in the kernel above)
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float next = fmaxf(top[e], most[e]);
+                    f[e] = next == -INFINITY ? 1.0f : fg_ex2_fast(top[e] - next);
+                    top[e] = next;
+                    sum[e] *= f[e];
+                }
+#pragma unroll
+                for (int c = 0; c < DP / 8; ++c)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[c][e] *= f[e >> 1];
+            }
+            const float less[2] = {top[0] == -INFINITY ? 0.0f : top[0], top[1] == -INFINITY ? 0.0f : top[1]};
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[c][e] = fg_ex2_fast(p[c][e] - less[e >> 1]);
+                    sum[e >> 1] += p[c][e];
+                }
+#pragma unroll
+            for (int t = 0; t < kCols; t += 2) {
+                const uint32_t w[4] = {pack2<T>(p[t][0], p[t][1]), pack2<T>(p[t][2], p[t][3]), pack2<T>(p[t + 1][0], p[t + 1][1]), pack2<T>(p[t + 1][2], p[t + 1][3])};
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) {
+                    if ((uint32_t)c >= steps) break;
+                    uint32_t m[4];
+                    const uint32_t key = part * kOwn + 8 * t + (lane & 15), chunk = 2 * (c & 3) + (lane >> 4);
+                    load_matrices_turned(vs + (c >> 2) * Cfg::kHalf + key * 128 + ((chunk ^ (key & 7)) << 4), m);
+                    mma_16x8x16<T>(o[2 * c], w, m[0], m[1]);
+                    mma_16x8x16<T>(o[2 * c + 1], w, m[2], m[3]);
+                }
+            }
+            __syncthreads();      // the stage is free
+            if (s_stop) {      // a wait ran out: nothing is on its way when the block ends
+                for (uint32_t l = i; l < n && l < i + S; ++l) mbar_wait_bounded(bar0 + 8 * ((g + l) % S), ((g + l) / S) & 1, kWaitCycles);
+                return;
+            }
+            if (threadIdx.x == 0 && i + S < n) ask(i + S);
+        }
+        g += n;
+        // The warps' sums, over those that had the same rows.
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
+            sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+            if (lane % 4 == 0) stat[warp][lane / 4 + 8 * e] = make_float2(top[e], sum[e]);
+        }
+        __syncthreads();
+        float* const sums = reinterpret_cast<float*>(raw + (base - smem_u32(raw)));      // [4][16][DP + 4], where the stages were
+        constexpr int kPitch = DP + 4;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float all = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4 / kW; ++w) all = fmaxf(all, stat[w * kW + warp % kW][lane / 4 + 8 * e].x);
+            const float f = top[e] == -INFINITY ? 0.0f : fg_ex2_fast(top[e] - all);
+#pragma unroll
+            for (int c = 0; c < DP / 8; ++c)
+                *reinterpret_cast<float2*>(sums + (warp * 16 + lane / 4 + 8 * e) * kPitch + 8 * c + 2 * (lane % 4)) = make_float2(o[c][2 * e] * f, o[c][2 * e + 1] * f);
+        }
+        __syncthreads();
+        for (uint32_t r = warp; r < n_row; r += 4) {
+            const uint32_t w0 = r / 16, in = r % 16;
+            float all = -INFINITY, total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4 / kW; ++w) all = fmaxf(all, stat[w * kW + w0][in].x);
+#pragma unroll
+            for (int w = 0; w < 4 / kW; ++w) {
+                const float2 st = stat[w * kW + w0][in];
+                if (st.x != -INFINITY) total = __fmaf_rn(fg_ex2_fast(st.x - all), st.y, total);
+            }
+            const uint32_t row = s.q0 + (uint32_t)((r0 + r) / a.group), head = kv * a.group + (uint32_t)((r0 + r) % a.group);
+            const uint64_t line = (uint64_t)row * a.heads + head;
+            const float f = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) {
+                const uint32_t d = 32 * c + lane;
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4 / kW; ++w) v += sums[((w * kW + w0) * 16 + in) * kPitch + d];
+                if (d < a.dim) {
+                    if (a.splits > 1) a.part_out[((uint64_t)z * a.queries * a.heads + line) * a.dim + d] = v;
+                    else static_cast<T*>(a.out)[line * a.dim + d] = fg_narrow<T>(v * f);
+                }
+            }
+            if (lane == 0) {
+                if (a.splits > 1) a.part_stat[(uint64_t)z * a.queries * a.heads + line] = make_float2(all, total);
+                else if (a.lse) a.lse[(uint64_t)head * a.queries + row] = (all + __log2f(total)) * kFgLn2;
+            }
+        }
+        fence_proxy_async();      // the stages are loaded again
+        __syncthreads();
+    }
+}
+
 // ---- backward ----
 // Both kernels have a row (of dq) or a key (of dk, dv) per lane, two groups of four warps with half of the columns each, warp 8 loads, warp 9
 // multiplies.  Weights are made again from lse.  What a tile's threads leave in tensor memory as an A operand takes the place of what they
@@ -970,6 +1200,28 @@ int32_t bwd_launch(fg_ctx* ctx, FgAttnArgs a) {
     return FG_OK;
 }
 
+template <typename T, int DP, int kW>
+int32_t few_launch(fg_ctx* ctx, const FgAttnArgs& a) {
+    using Cfg = FewCfg<DP>;
+    constexpr bool half = std::is_same_v<T, __half>;
+    static std::atomic<uint64_t> done{0};
+    int32_t s = allow_shared(ctx, done, attn_few_kernel<T, DP, kW>, Cfg::kSmem);
+    if (s != FG_OK) return s;
+    CUtensorMap k, v;
+    if ((s = make_map(ctx, &k, a.k, half, a.dim, a.kv_heads, a.keys, a.k_stride, 1, Cfg::kKeys)) != FG_OK) return s;
+    if ((s = make_map(ctx, &v, a.v, half, a.dim, a.kv_heads, a.keys, a.v_stride, 1, Cfg::kKeys)) != FG_OK) return s;
+    const uint64_t blocks = (uint64_t)a.sequences * a.splits * a.kv_heads;
+    if (blocks >= 1ull << 31) return fg_fail(ctx, FG_ERR_INVALID_ARGUMENT, "attention: tensor too large");
+    fg_launch(ctx, attn_few_kernel<T, DP, kW>, (unsigned)blocks, Cfg::kThreads, Cfg::kSmem, k, v, a);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
+}
+template <typename T>
+int32_t few(fg_ctx* ctx, const FgAttnArgs& a, uint32_t rows) {
+    if (a.dim <= 64) return rows <= 16 ? few_launch<T, 64, 1>(ctx, a) : rows <= 32 ? few_launch<T, 64, 2>(ctx, a) : few_launch<T, 64, 4>(ctx, a);
+    return rows <= 16 ? few_launch<T, 128, 1>(ctx, a) : rows <= 32 ? few_launch<T, 128, 2>(ctx, a) : few_launch<T, 128, 4>(ctx, a);
+}
+
 }  // namespace
 
 bool fg_attn_tc_suits(const fg_ctx* ctx, int32_t dtype, const FgAttnArgs& a) {
@@ -985,4 +1237,7 @@ int32_t fg_attn_tc_fwd(fg_ctx* ctx, int32_t dtype, const FgAttnArgs& a) {
 int32_t fg_attn_tc_bwd(fg_ctx* ctx, int32_t dtype, const FgAttnArgs& a) {
     if (dtype == FG_DTYPE_F16) return a.dim <= 64 ? bwd_launch<__half, 64>(ctx, a) : bwd_launch<__half, 128>(ctx, a);
     return a.dim <= 64 ? bwd_launch<__nv_bfloat16, 64>(ctx, a) : bwd_launch<__nv_bfloat16, 128>(ctx, a);
+}
+int32_t fg_attn_few(fg_ctx* ctx, int32_t dtype, const FgAttnArgs& a, uint32_t rows) {
+    return dtype == FG_DTYPE_F16 ? few<__half>(ctx, a, rows) : few<__nv_bfloat16>(ctx, a, rows);
 }
