@@ -6,9 +6,7 @@
 // dgamma = column sums of dy * n.
 #include <cuda_fp8.h>
 
-#include <atomic>
-
-#include "rows.cuh"
+#include "norm_rows.cuh"
 
 namespace {
 
@@ -28,13 +26,273 @@ struct RmsBwdArgs {
 };
 constexpr float kE4m3Max = 448.0f;
 
-// y / s in e4m3; s that has no finite reciprocal divides.
+// y / s in e4m3.  1 / s has to be finite and normal, or y is divided; a group of zeros stays one.
+__device__ __forceinline__ bool has_inverse(float s) { return s > 1e-37f && s < 1e37f; }
+__device__ __forceinline__ float divided(float y, float s) { return s > 0.0f ? y / s : y * 0.0f; }
 __device__ __forceinline__ uint8_t to_e4m3(float y, float s) {
-    const float v = s > 0.0f ? (s > 1e-37f ? y * (1.0f / s) : y / s) : y * 0.0f;
-    return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+    return (uint8_t)__nv_cvt_float_to_fp8(has_inverse(s) ? y * (1.0f / s) : divided(y, s), __NV_SATFINITE, __NV_E4M3);
+}
+// 2 * P of them, four in a word.
+template <int P>
+__device__ __forceinline__ void put_e4m3(float (&y)[2 * P], float s, uint32_t (&w)[P / 2]) {
+    if (has_inverse(s)) {
+        const float by = 1.0f / s;
+#pragma unroll
+        for (int e = 0; e < 2 * P; ++e) y[e] *= by;
+    } else
+#pragma unroll
+        for (int e = 0; e < 2 * P; ++e) y[e] = divided(y[e], s);
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i)
+        w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[4 * i], y[4 * i + 1]), __NV_SATFINITE, __NV_E4M3) |
+               (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[4 * i + 2], y[4 * i + 3]), __NV_SATFINITE, __NV_E4M3) << 16;
 }
 
-// Any row: one block each.
+// A row per group of threads (norm_rows.cuh), kRes: with a residual.  y in 8 bits (k8) is for rows that lie straight: a thread's pack belongs to one group of columns,
+// whose largest |y| is found among `lanes` neighbouring lanes, or (lanes = 0) over the row.
+template <typename C, bool kRes, bool k8>
+__global__ void __launch_bounds__(kMaxThreads, C::kTight && C::N <= 16 ? 2 : 1) rms_held_kernel(const RmsArgs a, int threads, int lanes) {
+    using T = typename C::T;
+    constexpr int H = C::N / 2;
+    extern __shared__ uint4 shared[];
+    __shared__ float red[kMaxGroups][k8 ? 4 : 2][32];
+    fg_grid_enter();
+    const Group group(threads);
+    const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups;
+    const uint32_t first = C::kApart ? group.index * gridDim.x + blockIdx.x : blockIdx.x * groups + group.index;
+    C columns(group, a.cols, first, shared);
+    const float inv_n = 1.0f / (float)a.cols;
+    const T* const gamma = static_cast<const T*>(a.gamma);
+    typename C::Kept gammas;
+    if (gamma) columns.keep(gamma, gammas);
+    const uint64_t stride = (uint64_t)step * a.cols, at = (uint64_t)first * a.cols;
+    const T *x = static_cast<const T*>(a.x) + at, *res = kRes ? static_cast<const T*>(a.residual) + at : nullptr, *x_ahead = x, *res_ahead = res;
+    T *sum = a.sum ? static_cast<T*>(a.sum) + at : nullptr, *y = k8 ? nullptr : static_cast<T*>(a.y) + at;
+    uint8_t* y8 = k8 ? static_cast<uint8_t*>(a.y) + at : nullptr;
+    uint64_t next = first;
+    auto ask = [&] {
+        if (next < a.rows) {
+            columns.ask(0, x_ahead);
+            if (kRes) columns.ask(1, res_ahead);
+        }
+        columns.asked();
+        next += step;
+        x_ahead += stride;
+        if (kRes) res_ahead += stride;
+    };
+    if (C::kAhead)
+#pragma unroll
+        for (int i = 0; i < C::kStages; ++i) ask();
+    int turn = 0;
+    for (uint64_t r = first; r < a.rows; r += step, x += stride) {
+        float2 v[H];
+        columns.arrived();
+        columns.get(0, x, v);
+        if (kRes) {
+            float2 u[H];
+            columns.get(1, res, u);
+            res += stride;
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                v[i] = fg_add2(v[i], u[i]);
+                if (sizeof(T) == 2) v[i] = make_float2(fg_widen(fg_narrow<T>(v[i].x)), fg_widen(fg_narrow<T>(v[i].y)));
+            }
+        }
+        columns.taken();
+        if (C::kAhead) ask();
+        if (sum) {
+            columns.store(sum, v);
+            sum += stride;
+        }
+        float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < H; ++i) s = fg_fma2(v[i], v[i], s);
+        const float rstd = 1.0f / sqrtf(__fmaf_rn(group.sum(s.x + s.y, red[group.index][turn]), inv_n, a.eps));
+        const float2 by = make_float2(rstd, rstd);
+#pragma unroll
+        for (int i = 0; i < H; ++i) v[i] = fg_mul2(v[i], by);
+        if (gamma) {
+            float2 g[H];
+            columns.kept(gammas, gamma, g);
+#pragma unroll
+            for (int i = 0; i < H; ++i) v[i] = fg_mul2(v[i], g[i]);
+        }
+        if constexpr (!k8) {
+            columns.store(y, v);
+            y += stride;
+        } else {
+            constexpr int P = C::P, K = H / P;      // pairs of a pack, packs
+            float most[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                most[k] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < P; ++e) most[k] = fmaxf(most[k], fmaxf(fabsf(v[k * P + e].x), fabsf(v[k * P + e].y)));
+            }
+            if (lanes) {
+                for (int o = lanes / 2; o > 0; o >>= 1)
+#pragma unroll
+                    for (int k = 0; k < K; ++k) most[k] = fmaxf(most[k], __shfl_xor_sync(0xffffffffu, most[k], o));
+            } else {
+#pragma unroll
+                for (int k = 1; k < K; ++k) most[0] = fmaxf(most[0], most[k]);
+                most[0] = group.max(most[0], red[group.index][2 + turn]);
+#pragma unroll
+                for (int k = 1; k < K; ++k) most[k] = most[0];
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (!columns.has(k)) continue;
+                const float scale = most[k] / kE4m3Max;
+                const uint32_t c = (group.thread + k * threads) * (2 * P);      // the pack's first column
+                if (lanes ? (group.lane & (lanes - 1)) == 0 : k == 0 && group.thread == 0) a.scale[r * a.groups + (lanes ? c / a.group : 0)] = scale;
+                float q[2 * P];
+#pragma unroll
+                for (int e = 0; e < P; ++e) { q[2 * e] = v[k * P + e].x; q[2 * e + 1] = v[k * P + e].y; }
+                uint32_t w[P / 2];
+                put_e4m3<P>(q, scale, w);
+                if constexpr (P == 4) *reinterpret_cast<uint2*>(y8 + c) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint32_t*>(y8 + c) = w[0];
+            }
+            y8 += stride;
+        }
+        if (group.thread == 0 && a.rstd) a.rstd[r] = rstd;
+        turn ^= 1;
+    }
+}
+
+// The backward pass the same way: kSum with what reaches h by other ways.  With the parameter's gradient (kParams) a thread sums its columns over the rows of its
+// group, a block adds its groups and leaves one row of parts: [block][pitch].
+template <typename C, bool kSum, bool kParams>
+__global__ void __launch_bounds__(kMaxThreads, C::kTight && C::N <= 4 ? 2 : 1) rms_bwd_held_kernel(const RmsBwdArgs a, int threads, float* parts, uint32_t pitch) {
+    using T = typename C::T;
+    constexpr int H = C::N / 2;
+    extern __shared__ uint4 shared[];      // the slots; at the end the groups' sums
+    __shared__ float red[kMaxGroups][2][32];
+    fg_grid_enter();
+    const Group group(threads);
+    const uint32_t groups = blockDim.x / threads, step = gridDim.x * groups;
+    const uint32_t first = C::kApart ? group.index * gridDim.x + blockIdx.x : blockIdx.x * groups + group.index;
+    C columns(group, a.cols, first, shared);
+    const float inv_n = 1.0f / (float)a.cols;
+    const T* const gamma = static_cast<const T*>(a.gamma);
+    typename C::Kept gammas;
+    if (gamma) columns.keep(gamma, gammas);
+    const uint64_t stride = (uint64_t)step * a.cols, at = (uint64_t)first * a.cols;
+    const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at, *ds = kSum ? static_cast<const T*>(a.dsum) + at : nullptr;
+    const T *x_ahead = x, *dy_ahead = dy, *ds_ahead = ds;
+    T* dx = a.dx ? static_cast<T*>(a.dx) + at : nullptr;
+    uint64_t next = first;
+    auto ask = [&] {
+        if (next < a.rows) {
+            columns.ask(0, x_ahead);
+            columns.ask(1, dy_ahead);
+            if (kSum) columns.ask(2, ds_ahead);
+        }
+        columns.asked();
+        next += step;
+        x_ahead += stride;
+        dy_ahead += stride;
+        if (kSum) ds_ahead += stride;
+    };
+    if (C::kAhead)
+#pragma unroll
+        for (int i = 0; i < C::kStages; ++i) ask();
+    float rstd = first < a.rows ? a.rstd[first] : 0.0f;
+    float2 dg[H];
+#pragma unroll
+    for (int i = 0; i < H; ++i) dg[i] = make_float2(0.0f, 0.0f);
+    int turn = 0;
+    for (uint64_t r = first; r < a.rows; r += step, x += stride, dy += stride) {
+        float2 c[H], g[H], d[kSum ? H : 1];
+        const float sd = rstd;
+        const float2 by = make_float2(sd, sd);
+        columns.arrived();
+        columns.get(0, x, c);
+        columns.get(1, dy, g);
+        if constexpr (kSum) {
+            columns.get(2, ds, d);
+            ds += stride;
+        }
+        columns.taken();
+        if (r + step < a.rows) rstd = a.rstd[r + step];
+        if (C::kAhead) ask();
+        if (kParams)
+#pragma unroll
+            for (int i = 0; i < H; ++i) dg[i] = fg_fma2(g[i], fg_mul2(c[i], by), dg[i]);      // (columns that are not there: dy is zero)
+        if (dx) {
+            if (gamma) {
+                float2 gm[H];
+                columns.kept(gammas, gamma, gm);
+#pragma unroll
+                for (int i = 0; i < H; ++i) g[i] = fg_mul2(g[i], gm[i]);
+            }
+            float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < H; ++i) s = fg_fma2(g[i], c[i], s);
+            const float t = group.sum(s.x + s.y, red[group.index][turn]), u = -sd * sd * (sd * (t * inv_n));
+            const float2 slope = make_float2(u, u);
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                g[i] = fg_fma2(g[i], by, fg_mul2(c[i], slope));
+                if constexpr (kSum) g[i] = fg_add2(g[i], d[i]);
+            }
+            columns.store(dx, g);
+            dx += stride;
+        }
+        turn ^= 1;
+    }
+    if constexpr (kParams) {
+        float2* const sums = reinterpret_cast<float2*>(shared);      // the groups one after the other: [pair][thread]
+        if (C::kAhead) fg_copies_wait<0>();
+        for (uint32_t i = 0; i + 1 < groups; ++i) {
+            __syncthreads();
+            if (group.index == (int)i)
+#pragma unroll
+                for (int e = 0; e < H; ++e) {
+                    float2* const p = sums + e * threads + group.thread;
+                    *p = i ? fg_add2(*p, dg[e]) : dg[e];
+                }
+        }
+        __syncthreads();
+        if (group.index + 1 == (int)groups) {
+            if (groups > 1)
+#pragma unroll
+                for (int e = 0; e < H; ++e) dg[e] = fg_add2(sums[e * threads + group.thread], dg[e]);
+            columns.store_sums(parts + (uint64_t)blockIdx.x * pitch, dg);
+        }
+    }
+}
+
+// Adds the blocks' parts: 128 columns per block, a warp takes every 32nd part.  pitch is a multiple of 128.
+template <typename T>
+__global__ void __launch_bounds__(1024) rms_parts_kernel(const RmsBwdArgs a, const float* parts, uint32_t count, uint32_t pitch) {
+    __shared__ float4 red[32][32];
+    fg_grid_enter();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t at = blockIdx.x * 128 + 4 * lane;
+    T* const out = static_cast<T*>(a.dgamma);
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t i0 = warp; i0 < count; i0 += 32 * 8) {
+        float4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            v[j] = i0 + 32 * j < count ? *reinterpret_cast<const float4*>(parts + (uint64_t)(i0 + 32 * j) * pitch + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { s.x += v[j].x; s.y += v[j].y; s.z += v[j].z; s.w += v[j].w; }
+    }
+    red[warp][lane] = s;
+    __syncthreads();
+    if (threadIdx.x < 128) {
+        const uint32_t c = blockIdx.x * 128 + threadIdx.x;
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 32; ++w) sum += reinterpret_cast<const float*>(red[w])[threadIdx.x];
+        if (c < a.cols) out[c] = fg_narrow<T>(a.accumulate ? fg_widen(out[c]) + sum : sum);
+    }
+}
+
+// Any row: one block each, read once per sum.
 template <typename T, bool k8>
 __global__ void __launch_bounds__(256) rms_stream_kernel(const RmsArgs a) {
     __shared__ float red[64];
@@ -154,16 +412,123 @@ __global__ void __launch_bounds__(256) rms_fold_kernel(const RmsBwdArgs a, const
     out[c] = fg_narrow<T>(a.accumulate ? fg_widen(out[c]) + s : s);
 }
 
-int rows_grid(const fg_ctx* ctx, uint32_t rows) { return (int)(rows < 8u * ctx->sm_count ? rows : 8u * ctx->sm_count); }
-
+template <typename C, bool kRes, bool k8 = false>
+int32_t launch_held(fg_ctx* ctx, const RmsArgs& a, HeldPlan p, int lanes = 0) {
+    static std::atomic<uint64_t> done{0};
+    const int32_t s = allow_shared(ctx, done, rms_held_kernel<C, kRes, k8>, p.bytes);
+    if (s != FG_OK) return s;
+    fg_launch(ctx, rms_held_kernel<C, kRes, k8>, p.grid, p.threads * p.groups, p.bytes, a, p.threads, lanes);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
+}
+template <typename T, int kPacks, bool kRes, bool k8>
+int32_t launch_straight(fg_ctx* ctx, const RmsArgs& a, HeldPlan p, int lanes) {
+    constexpr int kTensors = kRes ? 2 : 1;
+    return p.full ? launch_held<Straight<T, kPacks, true, kTensors>, kRes, k8>(ctx, a, p, lanes) : launch_held<Straight<T, kPacks, false, kTensors>, kRes, k8>(ctx, a, p, lanes);
+}
+// A thread holds 16 columns, more where the row is longer than a block's threads have so, fewer for few rows: held_plan() has what that was measured at.
+template <typename T, bool kRes, bool k8>
+int32_t fwd_straight(fg_ctx* ctx, const RmsArgs& a, int lanes, bool* took) {
+    constexpr int usual = 16 / FgPack<T>::E;
+    const HeldPlan p = held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 1, usual, 8, kRes ? 2 : 1, 512);
+    *took = p.threads != 0;
+    if (!p.threads) return FG_OK;
+    return p.units == 1 ? launch_straight<T, 1, kRes, k8>(ctx, a, p, lanes) : p.units == 2 ? launch_straight<T, 2, kRes, k8>(ctx, a, p, lanes)
+           : p.units == 4 ? launch_straight<T, 4, kRes, k8>(ctx, a, p, lanes) : launch_straight<T, 8, kRes, k8>(ctx, a, p, lanes);
+}
+template <typename T, bool kRes>
+int32_t fwd_ragged(fg_ctx* ctx, const RmsArgs& a, bool* took) {
+    constexpr int usual = 16 / FgPack<T>::E, kTensors = kRes ? 2 : 1;
+    *took = true;
+    if (a.cols > 64 * sizeof(T) && fg_aligned16(a.x) && fg_aligned16(a.residual) && fg_aligned16(a.sum) && fg_aligned16(a.y)) {
+        constexpr int most = 32 / FgPack<T>::E;      // a bit per column of a thread
+        const HeldPlan p = shifted_plan<T>(ctx, a.rows, a.cols, 1, usual, most, kTensors);
+        if (p.threads)
+            return p.units == 1 ? launch_held<Shifted<T, 1, kTensors>, kRes>(ctx, a, p) : p.units == 2 ? launch_held<Shifted<T, 2, kTensors>, kRes>(ctx, a, p)
+                   : p.units == 4 ? launch_held<Shifted<T, 4, kTensors>, kRes>(ctx, a, p) : launch_held<Shifted<T, most, kTensors>, kRes>(ctx, a, p);
+    }
+    const HeldPlan p = held_plan(ctx, a.rows, a.cols, 4, 8, 32, 0, 1024);
+    if (p.threads)
+        return p.units == 4 ? launch_held<Ragged<T, 4, kTensors>, kRes>(ctx, a, p) : p.units == 8 ? launch_held<Ragged<T, 8, kTensors>, kRes>(ctx, a, p)
+               : p.units == 16 ? launch_held<Ragged<T, 16, kTensors>, kRes>(ctx, a, p) : launch_held<Ragged<T, 32, kTensors>, kRes>(ctx, a, p);
+    *took = false;
+    return FG_OK;
+}
 template <typename T>
 int32_t rms_fwd(fg_ctx* ctx, const RmsArgs& a) {
+    constexpr uint32_t E = FgPack<T>::E;
+    const bool res = a.residual, straight = fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.residual, a.gamma, a.sum);
+    bool took = false;
+    int32_t s = FG_OK;
+    if (a.scale) {
+        const uint32_t lanes = a.group == a.cols && a.groups == 1 ? 0 : a.group / E;      // 256 columns of f32 are two warps
+        if (straight && reinterpret_cast<uintptr_t>(a.y) % E == 0 && lanes <= 32)
+            s = res ? fwd_straight<T, true, true>(ctx, a, (int)lanes, &took) : fwd_straight<T, false, true>(ctx, a, (int)lanes, &took);
+    } else if (straight && fg_aligned16(a.y)) s = res ? fwd_straight<T, true, false>(ctx, a, 0, &took) : fwd_straight<T, false, false>(ctx, a, 0, &took);
+    else s = res ? fwd_ragged<T, true>(ctx, a, &took) : fwd_ragged<T, false>(ctx, a, &took);
+    if (took) return s;
     fg_launch(ctx, a.scale ? rms_stream_kernel<T, true> : rms_stream_kernel<T, false>, rows_grid(ctx, a.rows), 256, 0, a);
     FG_LAUNCHED(ctx);
     return FG_OK;
 }
+
+template <typename C, bool kSum, bool kParams>
+int32_t launch_bwd(fg_ctx* ctx, const RmsBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch) {
+    const size_t sums = kParams && p.groups > 1 ? 4ull * C::N * p.threads : 0, bytes = p.bytes < sums ? sums : p.bytes;
+    static std::atomic<uint64_t> done{0};
+    const int32_t s = allow_shared(ctx, done, rms_bwd_held_kernel<C, kSum, kParams>, bytes);
+    if (s != FG_OK) return s;
+    fg_launch(ctx, rms_bwd_held_kernel<C, kSum, kParams>, p.grid, p.threads * p.groups, bytes, a, p.threads, parts, pitch);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
+}
+template <template <typename, int, int> class R, typename T, int kUnits>
+int32_t launch_bwd_held(fg_ctx* ctx, const RmsBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch) {
+    if (a.dsum && a.dx) return parts ? launch_bwd<R<T, kUnits, 3>, true, true>(ctx, a, p, parts, pitch) : launch_bwd<R<T, kUnits, 3>, true, false>(ctx, a, p, parts, pitch);
+    return parts ? launch_bwd<R<T, kUnits, 2>, false, true>(ctx, a, p, parts, pitch) : launch_bwd<R<T, kUnits, 2>, false, false>(ctx, a, p, parts, pitch);
+}
+template <typename T, int kUnits, int kTensors> using StraightFull = Straight<T, kUnits, true, kTensors>;
+template <typename T, int kUnits, int kTensors> using StraightPart = Straight<T, kUnits, false, kTensors>;
+template <typename T, int kUnits>
+int32_t launch_bwd_straight(fg_ctx* ctx, const RmsBwdArgs& a, HeldPlan p, float* parts, uint32_t pitch) {
+    return p.full ? launch_bwd_held<StraightFull, T, kUnits>(ctx, a, p, parts, pitch) : launch_bwd_held<StraightPart, T, kUnits>(ctx, a, p, parts, pitch);
+}
 template <typename T>
 int32_t rms_bwd(fg_ctx* ctx, const RmsBwdArgs& a) {
+    constexpr int usual = 16 / FgPack<T>::E;
+    const int tensors = a.dsum && a.dx ? 3 : 2;
+    const bool straight = fg_rows_lie_straight(a.cols, sizeof(T), a.x, a.dy, a.gamma, a.dx) && fg_aligned16(a.dsum);
+    HeldPlan p{};
+    if (straight) p = held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 1, usual, usual, tensors, 512);
+    else if (fg_aligned16(a.x) && fg_aligned16(a.dy) && fg_aligned16(a.dx) && fg_aligned16(a.dsum)) p = shifted_plan<T>(ctx, a.rows, a.cols, 1, usual, usual, tensors);
+    const bool shifted = !straight && p.threads;
+    if (!straight && !shifted) p = held_plan(ctx, a.rows, a.cols, 4, 4, 16, 0, 1024);
+    if (p.threads) {
+        float* parts = nullptr;
+        const uint32_t pitch = (a.cols + 127) / 128 * 128;
+        if (a.dgamma) {
+            void* w;
+            const int32_t s = fg_ws_alloc(ctx, 4ull * pitch * p.grid, &w);
+            if (s != FG_OK) return s;
+            parts = (float*)w;
+        }
+        int32_t s;
+        if (straight) {
+            if (p.units == 1) s = launch_bwd_straight<T, 1>(ctx, a, p, parts, pitch);
+            else if (p.units == 2) s = launch_bwd_straight<T, 2>(ctx, a, p, parts, pitch);
+            else s = launch_bwd_straight<T, usual>(ctx, a, p, parts, pitch);
+        } else if (shifted) {
+            if (p.units == 1) s = launch_bwd_held<Shifted, T, 1>(ctx, a, p, parts, pitch);
+            else if (p.units == 2) s = launch_bwd_held<Shifted, T, 2>(ctx, a, p, parts, pitch);
+            else s = launch_bwd_held<Shifted, T, usual>(ctx, a, p, parts, pitch);
+        } else if (p.units == 4) s = launch_bwd_held<Ragged, T, 4>(ctx, a, p, parts, pitch);
+        else if (p.units == 8) s = launch_bwd_held<Ragged, T, 8>(ctx, a, p, parts, pitch);
+        else s = launch_bwd_held<Ragged, T, 16>(ctx, a, p, parts, pitch);
+        if (s != FG_OK || !parts) return s;
+        fg_launch(ctx, rms_parts_kernel<T>, pitch / 128, 1024, 0, a, (const float*)parts, (uint32_t)p.grid, pitch);
+        FG_LAUNCHED(ctx);
+        return FG_OK;
+    }
     if (a.dgamma) {      // before dx, which may be dy, x or dsum
         const uint32_t chunks = (a.rows + kChunk - 1) / kChunk;
         void* w;
