@@ -50,8 +50,9 @@ struct RowWords {
 };
 
 // A part of a row in powers of two: the largest entry, with y = (x - m) * scale * log2(e) the sum of 2^y, and of 2^y * y.
-struct Part {
+struct alignas(16) Part {
     float m, l, e;
+    uint32_t count;      // of alternatives (between blocks)
     // Another part.  sum w (y + d) = sum w y + d sum w; a part whose weights vanish beside the other's adds nothing, whatever its distance.
     __device__ __forceinline__ void join(const Part& o, float by) {
         const float top = fmaxf(m, o.m);
@@ -87,7 +88,7 @@ struct Scan {
     static constexpr int E = FgPack<T>::E;
     Part p{-INFINITY, 0.0f, 0.0f};      // (its largest; the sums by pairs)
     float2 l2 = make_float2(0.0f, 0.0f), e2 = l2;
-    uint64_t best = 0;      // order_key of the largest entry
+    uint64_t best = 0;      // order_key of the largest entry, or of its value and a later index
     float by;
     __device__ __forceinline__ explicit Scan(float by_) : by(by_) {}
     __device__ __forceinline__ void rise(float top, uint64_t key) {
@@ -118,25 +119,25 @@ struct Scan {
 #pragma unroll
             for (int i = 0; i < kWords; ++i)
                 if (w + i * step < end) v[i] = __ldg(at + w + i * step);
-            float top = -INFINITY;
+            float most[kWords], top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < kWords; ++i) {
                 if (w + i * step < end) FgPack<T>::widen(v[i], x[i]);
                 else
 #pragma unroll
                     for (int e = 0; e < E / 2; ++e) x[i][e] = make_float2(-INFINITY, -INFINITY);
+                most[i] = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < E / 2; ++e) top = max3(top, x[i][e].x, x[i][e].y);
+                for (int e = 0; e < E / 2; ++e) most[i] = max3(most[i], x[i][e].x, x[i][e].y);
+                top = fmaxf(top, most[i]);
             }
             if (top > p.m) {
-                uint64_t key = 0;
+                uint32_t at_word = w;      // the first word that has it; its last index stands for the entry's, so that the key is no larger
                 if (kTop)
 #pragma unroll
-                    for (int i = 0; i < kWords; ++i)
-#pragma unroll
-                        for (int e = 0; e < E; ++e)
-                            if ((e & 1 ? x[i][e / 2].y : x[i][e / 2].x) == top && !key) key = order_key(top, head + (w + i * step) * E + e);
-                rise(top, key);
+                    for (int i = kWords - 1; i >= 0; --i)
+                        if (most[i] == top) at_word = w + i * step;
+                rise(top, kTop ? order_key(top, head + at_word * E + E - 1) : 0);
             }
             const float2 from = make_float2(less(), less());
 #pragma unroll
@@ -186,17 +187,28 @@ __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const LogprobArg
     if (lane == 0) write_statistics(a, (uint32_t)r, p, at_target);
 }
 
+// Places of a list's entries in the order of the alternatives: how many are larger.  `put` gets those below `top`.
+template <typename F>
+__device__ __forceinline__ void place_entries(const uint64_t* list, uint32_t n, uint32_t top, F put) {
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+        const uint64_t k = list[i];
+        uint32_t larger = 0;
+#pragma unroll 8
+        for (uint32_t j = 0; j < n; ++j) larger += list[j] > k;
+        if (larger < top) put(larger, k);
+    }
+}
+
 // A row per cluster of blocks, each with a stretch of it.
-// The alternatives: the top-th largest of the threads' largest entries is a bound that top entries reach, and few others do: a second reading (from the
-// L2) lists those, and the list is put in order by counting how many are larger.  Where more than the list holds reach the bound (they are all a few
-// threads'), the largest below the one before is sought top times over.
+// The alternatives: each of the 8 warps' ceil(top / 8) largest among its lanes' largest entries are `top` entries or more, so the least of them is a bound that
+// the top entries reach, and few others do: a second reading (from the L2) lists those, and the list is put in order by counting how many are larger.  Where
+// more than the list holds reach the bound (a few threads have them), the largest below the one before is sought top times over.  The blocks' lists go to
+// the first, which puts them in order the same way.
 template <typename T, bool kEntropy, bool kTop>
-__global__ void __launch_bounds__(kThreads) logprob_row_kernel(const LogprobArgs a) {
-    constexpr int E = FgPack<T>::E;
-    __shared__ Part parts[kThreads / 32];
-    __shared__ Part mine;
-    __shared__ uint64_t keys[kTop ? kThreads : 1], list[kTop ? kList : 1], sorted[kTop ? kMaxTop : 1], all[kTop ? kMaxTop * kMaxCluster : 1];
-    __shared__ uint64_t bound;
+__global__ void __launch_bounds__(kThreads, 4) logprob_row_kernel(const LogprobArgs a) {
+    constexpr int E = FgPack<T>::E, kWarps = kThreads / 32;
+    __shared__ Part parts[kWarps], others[kMaxCluster];
+    __shared__ uint64_t keys[kWarps], list[kTop ? kList : 1], sorted[kTop ? kMaxTop : 1], all[kTop ? kMaxTop * kMaxCluster : 1];
     __shared__ uint32_t count;
     fg_grid_enter();
     const uint32_t blocks = a.blocks, rank = blockIdx.x % blocks, r = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31;
@@ -207,6 +219,7 @@ __global__ void __launch_bounds__(kThreads) logprob_row_kernel(const LogprobArgs
     }
     const T* const row = static_cast<const T*>(a.x) + (uint64_t)r * a.cols;
     const RowWords<T> w(row, a.cols);
+    if (blocks > 1) fgptx::cluster_arrive();
     const uint32_t from = (uint32_t)((uint64_t)w.words * rank / blocks), to = (uint32_t)((uint64_t)w.words * (rank + 1) / blocks);
     const float by = a.scale * kLog2e, at_target = rank == 0 ? fg_widen(row[target]) : 0.0f;
     Scan<T, kEntropy, kTop> scan(by);
@@ -218,25 +231,31 @@ __global__ void __launch_bounds__(kThreads) logprob_row_kernel(const LogprobArgs
     p.join_lanes(by);
     if (lane == 0) parts[tid >> 5] = p;
     if (kTop) {
-        keys[tid] = scan.best;
-        if (tid == 0) { bound = 1; count = 0; }      // 1: every entry that may be an alternative
+        uint32_t v = (uint32_t)(scan.best >> 32);
+        uint64_t least = ~0ull;
+        for (uint32_t i = 0; i < a.top; i += kWarps) {
+            const uint32_t most = __reduce_max_sync(0xffffffffu, v), from_lane = __ffs(__ballot_sync(0xffffffffu, v == most)) - 1;
+            const uint64_t k = __shfl_sync(0xffffffffu, scan.best, from_lane);
+            if (k < least) least = k;
+            if (lane == from_lane) v = 0;
+            if (most == 0) least = 0;      // fewer than that
+        }
+        if (lane == 0) keys[tid >> 5] = least;
+        if (tid == 0) count = 0;
         if (tid < kMaxTop) sorted[tid] = 0;
     }
     __syncthreads();
+    p = lane < kWarps ? parts[lane] : Part{-INFINITY, 0.0f, 0.0f};
+    p.join_lanes(by);      // (every warp)
+    uint32_t n = 0;        // of this block's alternatives
     if (kTop) {
-        uint32_t larger = 0;
-        for (int i = 0; i < kThreads; ++i) larger += keys[i] > scan.best;
-        if (larger == a.top - 1 && scan.best) bound = scan.best;      // (keys differ)
-    }
-    if (tid < 32) {
-        p = lane < kThreads / 32 ? parts[lane] : Part{-INFINITY, 0.0f, 0.0f};
-        p.join_lanes(by);
-        if (lane == 0) mine = p;
-    }
-    __syncthreads();
-    if (kTop) {
-        const uint64_t least = bound;
-        auto each = [&](auto take) {      // all entries of this block
+        uint64_t least = keys[0];
+#pragma unroll
+        for (int i = 1; i < kWarps; ++i) least = least < keys[i] ? least : keys[i];
+        if (least == 0) least = 1;      // every entry that may be an alternative
+        // The entries of this block that reach `floor`: found by words, their indices from a short loop (unrolled into every entry's place it took longer to
+        // fetch than to run).
+        auto each = [&](float floor, auto take) {
             if (has_head) take(fg_widen(row[tid]), tid);
             if (has_tail) take(fg_widen(row[a.cols - w.tail + tid]), a.cols - w.tail + tid);
             const uint4* const at = reinterpret_cast<const uint4*>(row + w.head);
@@ -245,41 +264,41 @@ __global__ void __launch_bounds__(kThreads) logprob_row_kernel(const LogprobArgs
 #pragma unroll
                 for (int j = 0; j < kWords; ++j)
                     if (i + j * kThreads < to) v[j] = __ldg(at + i + j * kThreads);
+                uint32_t reach = 0;
 #pragma unroll
                 for (int j = 0; j < kWords; ++j)
                     if (i + j * kThreads < to) {
                         float x[E];
                         FgPack<T>::widen(v[j], x);
 #pragma unroll
-                        for (int e = 0; e < E; ++e) take(x[e], w.head + (i + j * kThreads) * E + e);
+                        for (int e = 0; e < E; ++e) reach |= (x[e] >= floor ? 1u : 0u) << (j * E + e);
                     }
+                while (reach) {
+                    const uint32_t bit = __ffs(reach) - 1, c = w.head + (i + bit / E * kThreads) * E + bit % E;
+                    reach &= reach - 1;
+                    take(fg_widen(row[c]), c);
+                }
             }
         };
         // The value of the bound: no key is made for what lies below.
         const uint32_t hi = (uint32_t)(least >> 32);
         const float floor = least == 1 ? -INFINITY : __uint_as_float(hi & 0x80000000u ? hi & 0x7fffffffu : ~hi);
         if (scan.p.m >= floor)      // (no entry of other threads reaches it)
-            each([&](float x, uint32_t c) {
-                if (x < floor) return;
+            each(floor, [&](float x, uint32_t c) {
                 const uint64_t k = order_key(x, c);
                 if (k < least) return;
-                const uint32_t n = atomicAdd(&count, 1);      // (the order in the list does not matter)
-                if (n < kList) list[n] = k;
+                const uint32_t i = atomicAdd(&count, 1);      // (the order in the list does not matter)
+                if (i < kList) list[i] = k;
             });
         __syncthreads();
-        const uint32_t n = count;
+        n = count;
         if (n <= kList) {
-            for (uint32_t i = tid; i < n; i += kThreads) {
-                const uint64_t k = list[i];
-                uint32_t larger = 0;
-                for (uint32_t j = 0; j < n && larger < a.top; ++j) larger += list[j] > k;
-                if (larger < a.top) sorted[larger] = k;
-            }
+            place_entries(list, n, a.top, [&](uint32_t i, uint64_t k) { sorted[i] = k; });
         } else {
             uint64_t last = ~0ull;
             for (uint32_t i = 0; i < a.top; ++i) {
                 uint64_t k = 0;
-                each([&](float x, uint32_t c) {
+                each(-INFINITY, [&](float x, uint32_t c) {
                     const uint64_t o = order_key(x, c);
                     if (o < last) k = max64(k, o);
                 });
@@ -288,40 +307,44 @@ __global__ void __launch_bounds__(kThreads) logprob_row_kernel(const LogprobArgs
                 __syncthreads();
                 if (lane == 0) keys[tid >> 5] = k;
                 __syncthreads();
-                for (int i2 = 0; i2 < kThreads / 32; ++i2) k = max64(k, keys[i2]);
+                for (int i2 = 0; i2 < kWarps; ++i2) k = max64(k, keys[i2]);
                 if (tid == 0) sorted[i] = k;
                 last = k;
             }
         }
+        n = min(n, a.top);
         __syncthreads();
     }
-    if (blocks > 1) {      // the first block joins the others' parts
-        fgptx::cluster_sync_all();
-        if (rank == 0) {
-            p = mine;
-            for (uint32_t o = 1; o < blocks; ++o) {
-                const uint32_t at = fgptx::map_to_cta((uint32_t)__cvta_generic_to_shared(&mine), o);
-                p.join(Part{fgptx::ld_cluster_f(at), fgptx::ld_cluster_f(at + 4), fgptx::ld_cluster_f(at + 8)}, by);
+    if (blocks > 1) {
+        fgptx::cluster_wait();      // (the first block has been there since the arrival above)
+        if (rank != 0) {
+            if (kTop && tid < n) {
+                const uint32_t at = fgptx::map_to_cta((uint32_t)__cvta_generic_to_shared(all + rank * kMaxTop + tid), 0);
+                fgptx::st_cluster(at, (uint32_t)sorted[tid], (uint32_t)(sorted[tid] >> 32));
             }
-            if (kTop)
-                for (uint32_t i = tid; i < blocks * a.top; i += kThreads) {
-                    const uint32_t at = fgptx::map_to_cta((uint32_t)__cvta_generic_to_shared(sorted + i % a.top), i / a.top);
-                    all[i] = (uint64_t)__float_as_uint(fgptx::ld_cluster_f(at + 4)) << 32 | __float_as_uint(fgptx::ld_cluster_f(at));
-                }
+            if (tid == 0) {
+                const uint32_t at = fgptx::map_to_cta((uint32_t)__cvta_generic_to_shared(others + rank), 0);
+                fgptx::st_cluster(at, __float_as_uint(p.m), __float_as_uint(p.l));
+                fgptx::st_cluster(at + 8, __float_as_uint(p.e), n);
+            }
         }
-        fgptx::cluster_sync_all();      // (no block ends while it is read)
+        fgptx::cluster_sync_all();
         if (rank != 0) return;
         if (kTop) {
-            if (tid < kMaxTop) sorted[tid] = 0;
-            __syncthreads();
-            for (uint32_t i = tid; i < blocks * a.top; i += kThreads) {
-                uint32_t larger = 0;
-                for (uint32_t j = 0; j < blocks * a.top; ++j) larger += all[j] > all[i];
-                if (all[i] && larger < a.top) sorted[larger] = all[i];
+            // The lists behind one another, then in order.
+            uint32_t total = n;
+            if (tid < n) list[tid] = sorted[tid];
+            for (uint32_t o = 1; o < blocks; ++o) {
+                const uint32_t m = others[o].count;
+                if (tid < m) list[total + tid] = all[o * kMaxTop + tid];
+                total += m;
             }
             __syncthreads();
+            place_entries(list, total, a.top, [&](uint32_t i, uint64_t k) { sorted[i] = k; });      // (there are as many as before, or more)
+            __syncthreads();
         }
-    } else p = mine;
+        for (uint32_t o = 1; o < blocks; ++o) p.join(others[o], by);
+    }
     if (tid == 0) write_statistics(a, r, p, at_target);
     if (kTop && tid < a.top) {
         const uint64_t k = sorted[tid];
