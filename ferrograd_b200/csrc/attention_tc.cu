@@ -42,40 +42,56 @@ __device__ __forceinline__ bool await(uint32_t bar, uint32_t parity, int* dev_st
 }
 
 // ---- forward ----
-// A block has two tiles of rows, one after the other in the sequence, that take turns: while the threads of one turn scores into weights, the tensor cores
-// multiply for the other.  Warps 0 to 3 and 4 to 7 have a row of their tile per thread, warp 8 loads, warp 9 multiplies.
-// Tensor memory: scores of tile s at column 128 s, where the weights then lie as the A operand of the product with v; sums of out at 256 + 128 s.
+// A block has two tiles of rows, one behind the other in the sequence, that take turns: while the threads of one turn scores into weights, the tensor cores
+// multiply for the other.  Warps 0 to 3 and 4 to 7 have a row of their tile per thread, warp 8 loads, warp 9 multiplies.  A block
+// stays on its SM and takes one pair of tiles after the other from a counter, longest first, so that loads and the first products of the next pair
+// run while the last sums of this one are written.
+// Tensor memory: scores of tile t at column 128 t, where the weights then lie as the A operand of the product with v; sums of out at 256 + 128 t.
 // Order of the products: S0(0) S1(0), then for each tile of keys j: PV0(j) S0(j+1) PV1(j) S1(j+1).  The scores of j + 1 come after PV(j) in this order, so they
 // may take the weights' place, and whoever has seen them arrive knows that out holds everything up to j.
+// A pair of tiles (more = 0: none is left): queries of each tile, keys that its last query sees, tiles of them.
+struct FwdWork { uint32_t more, kv, q0, nq, k0, nk, tok0, tok_0, tok_1, hi_0, hi_1, n_0, n_1; };
+// F(field) for each.
+#define FG_FWD_WORK(F) F(more) F(kv) F(q0) F(nq) F(k0) F(nk) F(tok0) F(tok_0) F(tok_1) F(hi_0) F(hi_1) F(n_0) F(n_1)
 template <int DP>
 struct FwdCfg {
-    static constexpr int kTile = kHalfBytes * (DP / 64), kStages = DP == 128 ? 5 : 8, kThreads = 384;
-    static constexpr int kBars = 2 + 2 * kStages + 7;
-    static constexpr size_t kSmem = 1024 + (size_t)(2 + kStages) * kTile + 8 * kBars + 16;
+    static constexpr int kTile = kHalfBytes * (DP / 64), kStages = DP == 128 ? 5 : 8, kThreads = 384, kSlots = 2;
+    static constexpr int kBars = 2 * kStages + 2 * 6 + 2 * kSlots + 1;
+    static constexpr size_t kUsed = (size_t)(2 + kStages) * kTile + 8 * kBars + sizeof(FwdWork) * kSlots + 16, kSmem = kUsed + 1024;
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(FwdCfg<DP>::kThreads, 1)
 attn_tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                   const __grid_constant__ FgAttnArgs a, uint32_t tokens, uint32_t tiles) {
+                   const __grid_constant__ FgAttnArgs a, uint32_t tokens, uint32_t tiles, unsigned* counter) {
     using Cfg = FwdCfg<DP>;
-    constexpr int S = Cfg::kStages;
+    constexpr int S = Cfg::kStages, W = Cfg::kSlots;
     extern __shared__ __align__(1024) unsigned char raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     const uint32_t qs = base, ring = base + 2 * Cfg::kTile, bar0 = ring + S * Cfg::kTile;
-    auto q_full = [&](uint32_t s) { return bar0 + 8 * s; };
-    auto kv_full = [&](uint32_t i) { return bar0 + 8 * (2 + i); };
-    auto kv_empty = [&](uint32_t i) { return bar0 + 8 * (2 + S + i); };
-    auto s_full = [&](uint32_t s) { return bar0 + 8 * (2 + 2 * S + s); };
-    auto p_full = [&](uint32_t s) { return bar0 + 8 * (4 + 2 * S + s); };
-    auto o_full = [&](uint32_t s) { return bar0 + 8 * (6 + 2 * S + s); };
-    const uint32_t drained = bar0 + 8 * (8 + 2 * S);
-    __shared__ uint32_t tmem_slot;
-    __shared__ int s_abort;
+    auto kv_full = [&](uint32_t i) { return bar0 + 8 * i; };
+    auto kv_empty = [&](uint32_t i) { return bar0 + 8 * (S + i); };
+    auto tile_bar = [&](uint32_t which, uint32_t t) { return bar0 + 8 * (2 * S + 2 * which + t); };
+    auto q_full = [&](uint32_t t) { return tile_bar(0, t); };
+    auto q_empty = [&](uint32_t t) { return tile_bar(1, t); };
+    auto s_full = [&](uint32_t t) { return tile_bar(2, t); };
+    auto p_full = [&](uint32_t t) { return tile_bar(3, t); };
+    auto o_full = [&](uint32_t t) { return tile_bar(4, t); };
+    auto o_empty = [&](uint32_t t) { return tile_bar(5, t); };
+    auto work_full = [&](uint32_t i) { return bar0 + 8 * (2 * S + 12 + i); };
+    auto work_empty = [&](uint32_t i) { return bar0 + 8 * (2 * S + 12 + W + i); };
+    const uint32_t drained = bar0 + 8 * (2 * S + 12 + 2 * W);
+    unsigned char* const tail = raw + (bar0 + 8 * Cfg::kBars - smem_u32(raw));
+    volatile uint32_t* const slot = reinterpret_cast<volatile uint32_t*>(tail);      // the tensor memory's address, a flag
+    volatile FwdWork* const works = reinterpret_cast<volatile FwdWork*>(tail + 16);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < 2; ++s) { mbar_init(q_full(s), 1); mbar_init(s_full(s), 1); mbar_init(p_full(s), 128); mbar_init(o_full(s), 1); }
         for (int i = 0; i < S; ++i) { mbar_init(kv_full(i), 1); mbar_init(kv_empty(i), 1); }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(q_full(t), 1); mbar_init(q_empty(t), 1); mbar_init(s_full(t), 1);
+            mbar_init(p_full(t), 128); mbar_init(o_full(t), 1); mbar_init(o_empty(t), 128);
+        }
+        for (int i = 0; i < W; ++i) { mbar_init(work_full(i), 1); mbar_init(work_empty(i), 9); }
         mbar_init(drained, 1);
         fence_mbar_init();
         prefetch_tmap(&tm_q);
@@ -83,124 +99,200 @@ attn_tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         prefetch_tmap(&tm_v);
     }
     if (warp == 9) {
-        tmem_alloc(smem_u32(&tmem_slot), kTmemCols);
+        tmem_alloc(bar0 + 8 * Cfg::kBars, kTmemCols);
         tmem_relinquish();
     }
     fg_grid_enter();
-    if (threadIdx.x == 0) s_abort = *reinterpret_cast<volatile int*>(a.dev_status);
+    if (threadIdx.x == 0) slot[1] = (uint32_t)*reinterpret_cast<volatile int*>(a.dev_status);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-    const bool go = __all_sync(0xffffffffu, s_abort == 0);
+    const uint32_t tmem = __shfl_sync(0xffffffffu, slot[0], 0);
+    const bool go = __all_sync(0xffffffffu, slot[1] == 0);
 
-    const uint32_t kv = blockIdx.x % a.kv_heads;
-    uint32_t tile;
-    const int b = go ? fg_attn_find(a.q_starts, a.sequences, a.queries, 1, 2 * tokens, tiles - 1 - blockIdx.x / a.kv_heads, &tile) : -1;
-    if (b >= 0) {
-        const FgAttnSeq s(a, b);
-        // (the numbering leaves gaps: a tile may lie behind its sequence's end)
-        const uint64_t tok0_ = (uint64_t)tile * 2 * tokens;
-        const uint32_t tok0 = tok0_ < s.nq ? (uint32_t)tok0_ : s.nq, left = s.nq - tok0;
-        const uint32_t tok_0 = min(tokens, left), tok_1 = left > tokens ? min(tokens, left - tokens) : 0;
-        // Keys that the tile's last query sees, and tiles of them.
-        const uint32_t hi_0 = tok_0 ? s.seen(a, tok0 + tok_0 - 1) : 0, hi_1 = tok_1 ? s.seen(a, tok0 + tokens + tok_1 - 1) : 0;
-        const uint32_t n_0 = (hi_0 + kRows - 1) / kRows, n_1 = (hi_1 + kRows - 1) / kRows, n_all = max(n_0, n_1);
-        const uint32_t fmt = kFormat<T>, dim16 = round_up(a.dim, 16);
-
-        if (warp >= 8) reg_release<40>();      // (all four warps of the group)
+    // The next pair of tiles, for the warps that work on it (false: none, or a wait ran out).
+    uint32_t taken = 0;
+    auto next = [&](FwdWork& w, bool& ok) {
+        if (!(ok = await(work_full(taken % W), (taken / W) & 1, a.dev_status, FG_DEVERR_EPI_WAIT))) return false;
+        volatile const FwdWork& from = works[taken % W];
+#define FG_TAKE(field) w.field = __shfl_sync(0xffffffffu, from.field, 0);
+        FG_FWD_WORK(FG_TAKE)
+#undef FG_TAKE
+        __syncwarp();
+        if (lane == 0) mbar_arrive(work_empty(taken % W));
+        ++taken;
+        return w.more != 0;
+    };
+    const uint32_t fmt = kFormat<T>, dim16 = round_up(a.dim, 16);
+    if (go) {
+        if (warp >= 8) reg_release<56>();      // (all four warps of the group)
         if (warp == 8) {
-            // ---- loads ----
-            const uint32_t q_bytes = DP / 64 * 128 * tokens * a.group;
-            auto load_q = [&](uint32_t t) {
-                mbar_expect_tx(q_full(t), q_bytes);
-#pragma unroll
-                for (int h = 0; h < DP / 64; ++h)
-                    tma_load_3d(qs + t * Cfg::kTile + h * kHalfBytes, &tm_q, q_full(t), 64 * h, (int)(kv * a.group), (int)(s.q0 + tok0 + t * tokens));
-            };
-            uint32_t g = 0;
-            for (uint32_t i = 0; i < 2 * n_all; ++i, ++g) {
-                const uint32_t st = g % S;
-                if (!await(kv_empty(st), ((g / S) & 1) ^ 1, a.dev_status, FG_DEVERR_TMA_WAIT)) break;
-                if (elect_one()) {
-                    if (i == 0 && n_0) load_q(0);
-                    mbar_expect_tx(kv_full(st), Cfg::kTile);
-#pragma unroll
-                    for (int h = 0; h < DP / 64; ++h)
-                        tma_load_3d(ring + st * Cfg::kTile + h * kHalfBytes, i & 1 ? &tm_v : &tm_k, kv_full(st), 64 * h, (int)kv, (int)(s.k0 + i / 2 * kRows));
-                    if (i == 0 && n_1) load_q(1);
+            // ---- work and loads: the next pair of tiles is taken when the last load of this one is under way ----
+            const uint32_t all = tiles * a.kv_heads, q_bytes = DP / 64 * 128 * tokens * a.group;
+            uint32_t g = 0, q_loads[2] = {0, 0};      // tiles of keys and values, tiles of queries so far
+            bool ok = true;
+            for (uint32_t count = 0; ok; ++count) {
+                FwdWork w = {};
+                for (;;) {      // tiles are numbered with gaps, which are passed over here
+                    uint32_t item = 0;
+                    if (lane == 0) item = atomicInc(counter, all + gridDim.x - 1);      // (each block takes one too many: the last one leaves zero)
+                    item = __shfl_sync(0xffffffffu, item, 0);
+                    w.more = item < all;
+                    if (!w.more) break;
+                    w.kv = item % a.kv_heads;
+                    uint32_t tile;
+                    const int b = fg_attn_find(a.q_starts, a.sequences, a.queries, 1, 2 * tokens, tiles - 1 - item / a.kv_heads, &tile);
+                    if (b < 0) continue;
+                    const FgAttnSeq s(a, b);
+                    const uint64_t tok0 = (uint64_t)tile * 2 * tokens;
+                    if (tok0 >= s.nq) continue;
+                    w.q0 = s.q0; w.nq = s.nq; w.k0 = s.k0; w.nk = s.nk;
+                    w.tok0 = (uint32_t)tok0;
+                    const uint32_t left = s.nq - w.tok0;
+                    w.tok_0 = min(tokens, left);
+                    w.tok_1 = left > tokens ? min(tokens, left - tokens) : 0;
+                    w.hi_0 = s.seen(a, w.tok0 + w.tok_0 - 1);
+                    w.hi_1 = w.tok_1 ? s.seen(a, w.tok0 + tokens + w.tok_1 - 1) : 0;
+                    w.n_0 = (w.hi_0 + kRows - 1) / kRows;
+                    w.n_1 = (w.hi_1 + kRows - 1) / kRows;
+                    break;
+                }
+                if (!(ok = await(work_empty(count % W), ((count / W) & 1) ^ 1, a.dev_status, FG_DEVERR_EPI_WAIT))) break;
+                if (lane == 0) {
+                    volatile FwdWork& to = works[count % W];
+#define FG_LEAVE(field) to.field = w.field;
+                    FG_FWD_WORK(FG_LEAVE)
+#undef FG_LEAVE
+                    mbar_arrive(work_full(count % W));
                 }
                 __syncwarp();
+                if (!w.more) break;
+                const uint32_t n_all = max(w.n_0, w.n_1);
+                for (uint32_t i = 0; i < 2 * n_all; ++i, ++g) {
+                    const uint32_t st = g % S;
+                    if (!(ok = await(kv_empty(st), ((g / S) & 1) ^ 1, a.dev_status, FG_DEVERR_TMA_WAIT))) break;
+                    if (elect_one()) {
+                        mbar_expect_tx(kv_full(st), Cfg::kTile);
+#pragma unroll
+                        for (int h = 0; h < DP / 64; ++h)
+                            tma_load_3d(ring + st * Cfg::kTile + h * kHalfBytes, i & 1 ? &tm_v : &tm_k, kv_full(st), 64 * h, (int)w.kv, (int)(w.k0 + i / 2 * kRows));
+                    }
+                    __syncwarp();
+                    if (i) continue;
+#pragma unroll
+                    for (uint32_t t = 0; t < 2; ++t) {
+                        if (!(t ? w.n_1 : w.n_0) || !ok) continue;
+                        if (!(ok = await(q_empty(t), (q_loads[t] & 1) ^ 1, a.dev_status, FG_DEVERR_TMA_WAIT))) continue;
+                        if (elect_one()) {
+                            mbar_expect_tx(q_full(t), q_bytes);
+#pragma unroll
+                            for (int h = 0; h < DP / 64; ++h)
+                                tma_load_3d(qs + t * Cfg::kTile + h * kHalfBytes, &tm_q, q_full(t), 64 * h, (int)(w.kv * a.group), (int)(w.q0 + w.tok0 + t * tokens));
+                        }
+                        __syncwarp();
+                        ++q_loads[t];
+                    }
+                    if (!ok) { ++g; break; }
+                }
             }
             // Nothing of this block is on its way when it ends, whatever became of the other roles.
             for (uint32_t i = g > (uint32_t)S ? g - S : 0; i < g; ++i)
                 if (!await(kv_full(i % S), (i / S) & 1, a.dev_status, FG_DEVERR_TMA_WAIT)) break;
-            for (uint32_t t = 0; g && t < 2; ++t)
-                if (t ? n_1 : n_0) await(q_full(t), 0, a.dev_status, FG_DEVERR_TMA_WAIT);
+#pragma unroll
+            for (uint32_t t = 0; t < 2; ++t)
+                if (q_loads[t]) await(q_full(t), (q_loads[t] - 1) & 1, a.dev_status, FG_DEVERR_TMA_WAIT);
         } else if (warp == 9) {
             // ---- products ----
             const uint32_t o_desc = make_idesc(fmt, 128, dim16) | kIdescBMnMajor, steps = dim16 / 16;
-            bool ok = true;
+            uint32_t g = 0, p_seen[2] = {0, 0}, pairs[2] = {0, 0};      // position in the ring (k0 v0 k1 v1 ..), weights so far, tiles of rows so far
+            FwdWork w = {};
+            bool ok;
+            const bool whole = dim16 == DP;      // (unrolled: an instruction per product and few beside it)
             auto scores = [&](uint32_t t, uint32_t j, uint32_t st) {
-                const uint32_t cols = round_up(min((uint32_t)kRows, (t ? hi_1 : hi_0) - j * kRows), 16);
+                const uint32_t cols = round_up(min((uint32_t)kRows, (t ? w.hi_1 : w.hi_0) - j * kRows), 16);
                 const uint32_t id = make_idesc(fmt, 128, cols);
                 const uint64_t q_d = make_desc_kmajor<128>(qs + t * Cfg::kTile), k_d = make_desc_kmajor<128>(ring + st * Cfg::kTile);
-                for (uint32_t c = 0; c < steps; ++c) {
-                    const uint64_t at = (uint64_t)((c & 3) * 2 + (c >> 2) * (kHalfBytes >> 4));
-                    mma_f16(tmem + t * 128, q_d + at, k_d + at, id, c != 0);
-                }
-                mma_commit(s_full(t));
-            };
-            uint32_t g = 0;      // position in the ring: k0 v0 k1 v1 ..
-            if (n_all) {
-                ok = await(kv_full(0), 0, a.dev_status, FG_DEVERR_MMA_WAIT);
-                for (uint32_t t = 0; ok && t < 2; ++t) {
-                    if (!(t ? n_1 : n_0)) continue;
-                    ok = await(q_full(t), 0, a.dev_status, FG_DEVERR_MMA_WAIT);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) scores(t, 0, 0);
-                    __syncwarp();
-                }
-                if (ok && elect_one()) mma_commit(kv_empty(0));
-                __syncwarp();
-                g = 1;
-            }
-            for (uint32_t j = 0; ok && j < n_all; ++j, g += 2) {
-                const uint32_t vs = g % S, ks = (g + 1) % S;
-                const bool more = j + 1 < n_all;
-                if (!await(kv_full(vs), (g / S) & 1, a.dev_status, FG_DEVERR_MMA_WAIT)) break;
-                // The rows of v behind the sequence's end have a weight of zero, but what stands there may be NaN: zeros for those that the last step multiplies.
-                const uint32_t left = s.nk - j * kRows;
-                if (left < kRows && (left & 15)) {
-                    const uint32_t end = round_up(left, 16);
-                    for (uint32_t i = left * 8 + lane; i < end * 8; i += 32)
+                if (whole) {
 #pragma unroll
-                        for (int h = 0; h < DP / 64; ++h) fg_store_shared(ring + vs * Cfg::kTile + h * kHalfBytes + i * 16, make_uint4(0, 0, 0, 0));
-                    fence_proxy_async();
+                    for (uint32_t c = 0; c < DP / 16; ++c) {
+                        const uint64_t at = (uint64_t)((c & 3) * 2 + (c >> 2) * (kHalfBytes >> 4));
+                        mma_f16(tmem + t * 128, q_d + at, k_d + at, id, c != 0);
+                    }
+                } else
+                    for (uint32_t c = 0; c < steps; ++c) {
+                        const uint64_t at = (uint64_t)((c & 3) * 2 + (c >> 2) * (kHalfBytes >> 4));
+                        mma_f16(tmem + t * 128, q_d + at, k_d + at, id, c != 0);
+                    }
+                mma_commit(s_full(t));
+                if (j + 1 == (t ? w.n_1 : w.n_0)) mma_commit(q_empty(t));
+            };
+            while (next(w, ok)) {
+                const uint32_t n_all = max(w.n_0, w.n_1);
+                if (!n_all) continue;
+                if (!(ok = await(kv_full(g % S), (g / S) & 1, a.dev_status, FG_DEVERR_MMA_WAIT))) break;
+#pragma unroll
+                for (uint32_t t = 0; t < 2; ++t) {
+                    if (!(t ? w.n_1 : w.n_0) || !ok) continue;
+                    if (!(ok = await(q_full(t), pairs[t] & 1, a.dev_status, FG_DEVERR_MMA_WAIT))) continue;
+                    tc_fence_after();
+                    if (elect_one()) scores(t, 0, g % S);
                     __syncwarp();
                 }
-                if (more && !await(kv_full(ks), ((g + 1) / S) & 1, a.dev_status, FG_DEVERR_MMA_WAIT)) break;
-                for (uint32_t t = 0; t < 2; ++t) {
-                    if (j < (t ? n_1 : n_0)) {
-                        ok = await(p_full(t), j & 1, a.dev_status, FG_DEVERR_MMA_WAIT);
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (elect_one()) {
-                            const uint32_t key_steps = (min((uint32_t)kRows, (t ? hi_1 : hi_0) - j * kRows) + 15) / 16;
-                            const uint64_t v_d = make_desc_mnmajor(ring + vs * Cfg::kTile, kHalfBytes, 1024, 2);
-                            for (uint32_t c = 0; c < key_steps; ++c) mma_f16_ta(tmem + 256 + t * 128, tmem + t * 128 + c * 8, v_d + (uint64_t)(c * 128), o_desc, j | c);
-                            if (j + 1 < (t ? n_1 : n_0)) scores(t, j + 1, ks);
-                            else mma_commit(o_full(t));
+                // Before the first products into out: the sums of the tiles before have been read.  (Waited for inside of the loop, by a test of j, this
+                // took a tenth of the kernel's time: the products' operands no longer stayed in uniform registers.)
+#pragma unroll
+                for (uint32_t t = 0; t < 2; ++t)
+                    if (ok && (t ? w.n_1 : w.n_0)) ok = await(o_empty(t), (pairs[t] & 1) ^ 1, a.dev_status, FG_DEVERR_MMA_WAIT);
+                if (!ok) break;
+                if (elect_one()) mma_commit(kv_empty(g % S));
+                __syncwarp();
+                ++g;
+                for (uint32_t j = 0; ok && j < n_all; ++j, g += j < n_all ? 2 : 1) {
+                    const uint32_t vs = g % S, ks = (g + 1) % S;
+                    const bool more = j + 1 < n_all;
+                    if (!(ok = await(kv_full(vs), (g / S) & 1, a.dev_status, FG_DEVERR_MMA_WAIT))) break;
+                    // The rows of v behind the sequence's end have a weight of zero, but what stands there may be NaN: zeros for those that the last step multiplies.
+                    const uint32_t left = w.nk - j * kRows;
+                    if (left < kRows && (left & 15)) {
+                        const uint32_t end = round_up(left, 16);
+                        for (uint32_t i = left * 8 + lane; i < end * 8; i += 32)
+#pragma unroll
+                            for (int h = 0; h < DP / 64; ++h) fg_store_shared(ring + vs * Cfg::kTile + h * kHalfBytes + i * 16, make_uint4(0, 0, 0, 0));
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                    if (more && !(ok = await(kv_full(ks), ((g + 1) / S) & 1, a.dev_status, FG_DEVERR_MMA_WAIT))) break;
+#pragma unroll
+                    for (uint32_t t = 0; t < 2; ++t) {
+                        if (ok && j < (t ? w.n_1 : w.n_0)) {
+                            ok = await(p_full(t), p_seen[t] & 1, a.dev_status, FG_DEVERR_MMA_WAIT);
+                            ++p_seen[t];
+                            if (ok) {
+                                tc_fence_after();
+                                if (elect_one()) {
+                                    const uint32_t key_steps = (min((uint32_t)kRows, (t ? w.hi_1 : w.hi_0) - j * kRows) + 15) / 16;
+                                    const uint64_t v_d = make_desc_mnmajor(ring + vs * Cfg::kTile, kHalfBytes, 1024, 2);
+                                    if (key_steps == 8) {
+#pragma unroll
+                                        for (uint32_t c = 0; c < 8; ++c) mma_f16_ta(tmem + 256 + t * 128, tmem + t * 128 + c * 8, v_d + (uint64_t)(c * 128), o_desc, j | c);
+                                    } else
+                                        for (uint32_t c = 0; c < key_steps; ++c) mma_f16_ta(tmem + 256 + t * 128, tmem + t * 128 + c * 8, v_d + (uint64_t)(c * 128), o_desc, j | c);
+                                    if (j + 1 < (t ? w.n_1 : w.n_0)) scores(t, j + 1, ks);
+                                    else mma_commit(o_full(t));
+                                }
+                                __syncwarp();
+                            }
+                        }
+                        if (t == 1 && ok && elect_one()) {
+                            mma_commit(kv_empty(vs));
+                            if (more) mma_commit(kv_empty(ks));
                         }
                         __syncwarp();
                     }
-                    if (t == 1 && elect_one()) {
-                        mma_commit(kv_empty(vs));
-                        if (more) mma_commit(kv_empty(ks));
-                    }
-                    __syncwarp();
                 }
+                if (!ok) break;
+#pragma unroll
+                for (uint32_t t = 0; t < 2; ++t) pairs[t] += (t ? w.n_1 : w.n_0) != 0;
             }
             // (a product may still run where a wait ran out)
             if (elect_one()) mma_commit(drained);
@@ -208,99 +300,115 @@ attn_tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             await(drained, 0, a.dev_status, FG_DEVERR_MMA_WAIT);
         } else if (warp < 8) {
             // ---- weights: a row per thread ----
-            reg_acquire<232>();
-            const uint32_t t = warp >> 2, r = threadIdx.x & 127, i = tok0 + t * tokens + r / a.group, head = kv * a.group + r % a.group;
-            const bool there = r / a.group < (t ? tok_1 : tok_0);
-            const uint32_t seen = there ? s.seen(a, i) : 0;
+            reg_acquire<224>();
+            const uint32_t t = warp >> 2, r = threadIdx.x & 127, row_tok = r / a.group, row_head = r % a.group;
             const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), t_s = lanes + t * 128, t_o = lanes + 256 + t * 128;
             const float by = a.scale * kFgLog2e;
-            float top = -INFINITY;
-            float2 sum = make_float2(0.0f, 0.0f);
-            bool ok = true;
-            for (uint32_t j = 0; j < (t ? n_1 : n_0); ++j) {
-                if (!(ok = await(s_full(t), j & 1, a.dev_status, FG_DEVERR_EPI_WAIT))) break;
-                tc_fence_after();
-                uint32_t w[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + c * 32, w[c]);
-                tmem_ld_wait();
-                const uint32_t end = j * kRows < seen ? seen - j * kRows : 0;
-                if (__any_sync(0xffffffffu, end < kRows)) {
-#pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if ((uint32_t)c >= end) w[c / 32][c % 32] = __float_as_uint(-INFINITY);
+            uint32_t steps = 0, pairs = 0;      // tiles of keys, tiles of rows so far
+            FwdWork w = {};
+            bool ok;
+            while (next(w, ok)) {
+                const uint32_t n = t ? w.n_1 : w.n_0, n_tok = t ? w.tok_1 : w.tok_0;
+                const uint32_t i = w.tok0 + t * tokens + row_tok, head = w.kv * a.group + row_head;
+                const bool there = row_tok < n_tok;
+                uint32_t seen = 0;
+                if (there) {
+                    const int64_t last = a.causal ? (int64_t)i + 1 + (int64_t)w.nk - (int64_t)w.nq : (int64_t)w.nk;
+                    seen = last < 0 ? 0 : (uint32_t)last;
                 }
-                float most = -INFINITY, m1 = -INFINITY;
+                float top = -INFINITY;
+                float2 sum = make_float2(0.0f, 0.0f);
+                for (uint32_t j = 0; j < n; ++j, ++steps) {
+                    if (!(ok = await(s_full(t), steps & 1, a.dev_status, FG_DEVERR_EPI_WAIT))) break;
+                    tc_fence_after();
+                    uint32_t x[4][32];
 #pragma unroll
-                for (int c = 0; c < 128; c += 4) {
-                    most = max3(most, __uint_as_float(w[c / 32][c % 32]), __uint_as_float(w[c / 32][c % 32 + 1]));
-                    m1 = max3(m1, __uint_as_float(w[c / 32][c % 32 + 2]), __uint_as_float(w[c / 32][c % 32 + 3]));
+                    for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + c * 32, x[c]);
+                    tmem_ld_wait();
+                    const uint32_t end = j * kRows < seen ? seen - j * kRows : 0;
+                    if (__any_sync(0xffffffffu, end < kRows)) {
+#pragma unroll
+                        for (int c = 0; c < 128; ++c)
+                            if ((uint32_t)c >= end) x[c / 32][c % 32] = __float_as_uint(-INFINITY);
+                    }
+                    float most = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 128; c += 4) {
+                        most = max3(most, __uint_as_float(x[c / 32][c % 32]), __uint_as_float(x[c / 32][c % 32 + 1]));
+                        m1 = max3(m1, __uint_as_float(x[c / 32][c % 32 + 2]), __uint_as_float(x[c / 32][c % 32 + 3]));
+                    }
+                    most = fmaxf(most, m1) * by;
+                    // The base of the exponents follows the largest score only when that has grown by more than 8: weights stay below 2^8, and out is
+                    // seldom gone over again.
+                    if (j == 0) top = most;
+                    else if (__any_sync(0xffffffffu, most > top + 8.0f)) {
+                        const float up = fmaxf(top, most), f = up == -INFINITY ? 1.0f : fg_ex2_fast(top - up);
+                        top = up;
+                        sum = make_float2(sum.x * f, sum.y * f);
+#pragma unroll
+                        for (int c = 0; c < DP; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld_32x16(t_o + c, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st_32x16(t_o + c, o);
+                        }
+                    }
+                    const float less = top == -INFINITY ? 0.0f : -top;
+                    const float2 by2 = make_float2(by, by), less2 = make_float2(less, less);
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            float2 e = make_float2(__uint_as_float(x[h][2 * c]), __uint_as_float(x[h][2 * c + 1]));
+                            e = fg_fma2(e, by2, less2);
+                            e = make_float2(fg_ex2_fast(e.x), fg_ex2_fast(e.y));
+                            sum = fg_add2(sum, e);
+                            p[c] = pack2<T>(e.x, e.y);
+                        }
+                        tmem_st_32x16(t_s + h * 16, p);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(p_full(t));
                 }
-                most = fmaxf(most, m1) * by;
-                // The base of the exponents follows the largest score only when that has grown by more than 8: weights stay below 2^8, and out is
-                // seldom gone over again.
-                if (j == 0) top = most;
-                else if (__any_sync(0xffffffffu, most > top + 8.0f)) {
-                    const float next = fmaxf(top, most), f = next == -INFINITY ? 1.0f : fg_ex2_fast(top - next);
-                    top = next;
-                    sum = make_float2(sum.x * f, sum.y * f);
+                const float total = sum.x + sum.y;
+                if (ok && n) ok = await(o_full(t), pairs & 1, a.dev_status, FG_DEVERR_EPI_WAIT);
+                if (!ok) break;
+                if (n_tok) {
+                    tc_fence_after();
+                    const uint32_t row = w.q0 + i;
+                    const float f = total == 0.0f ? 0.0f : 1.0f / total;
+                    T* const out = static_cast<T*>(a.out) + ((uint64_t)row * a.heads + head) * a.dim;
 #pragma unroll
                     for (int c = 0; c < DP; c += 32) {
                         uint32_t o[32];
-                        tmem_ld_32x32(t_o + c, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st_32x32(t_o + c, o);
-                    }
-                }
-                const float less = top == -INFINITY ? 0.0f : -top;
-                const float2 by2 = make_float2(by, by), less2 = make_float2(less, less);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t p[32];
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        const int at = h * 64 + 2 * c;
-                        float2 x = make_float2(__uint_as_float(w[at / 32][at % 32]), __uint_as_float(w[at / 32][at % 32 + 1]));
-                        x = fg_fma2(x, by2, less2);
-                        x = make_float2(fg_ex2_fast(x.x), fg_ex2_fast(x.y));
-                        sum = fg_add2(sum, x);
-                        p[c] = pack2<T>(x.x, x.y);
-                    }
-                    tmem_st_32x32(t_s + h * 32, p);
-                }
-                tmem_st_wait();
-                tc_fence_before();
-                mbar_arrive(p_full(t));
-            }
-            const float total = sum.x + sum.y;
-            if (ok && (t ? n_1 : n_0)) ok = await(o_full(t), 0, a.dev_status, FG_DEVERR_EPI_WAIT);
-            if (ok && (t ? tok_1 : tok_0)) {
-                tc_fence_after();
-                const uint32_t row = s.q0 + i;
-                const float f = total == 0.0f ? 0.0f : 1.0f / total;
-                T* const out = static_cast<T*>(a.out) + ((uint64_t)row * a.heads + head) * a.dim;
-#pragma unroll
-                for (int c = 0; c < DP; c += 32) {
-                    uint32_t o[32];
-                    if ((t ? n_1 : n_0)) {      // a tile that sees nothing has no sums
-                        tmem_ld_32x32(t_o + c, o);
-                        tmem_ld_wait();
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (total != 0.0f) {
-                            v.x = pack2<T>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
-                            v.y = pack2<T>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
-                            v.z = pack2<T>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f);
-                            v.w = pack2<T>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
+                        if (n) {      // a tile that sees nothing has no sums
+                            tmem_ld_32x32(t_o + c, o);
+                            tmem_ld_wait();
+                            if (c + 32 == DP) {
+                                tc_fence_before();
+                                mbar_arrive(o_empty(t));
+                            }
                         }
-                        if (there && (uint32_t)(c + e) < a.dim) *reinterpret_cast<uint4*>(out + c + e) = v;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint4 v = make_uint4(0, 0, 0, 0);
+                            uint32_t* const u = o + e;
+                            if (total != 0.0f) {
+                                v.x = pack2<T>(__uint_as_float(u[0]) * f, __uint_as_float(u[1]) * f);
+                                v.y = pack2<T>(__uint_as_float(u[2]) * f, __uint_as_float(u[3]) * f);
+                                v.z = pack2<T>(__uint_as_float(u[4]) * f, __uint_as_float(u[5]) * f);
+                                v.w = pack2<T>(__uint_as_float(u[6]) * f, __uint_as_float(u[7]) * f);
+                            }
+                            if (there && (uint32_t)(c + e) < a.dim) *reinterpret_cast<uint4*>(out + c + e) = v;
+                        }
                     }
+                    if (there && a.lse) a.lse[(uint64_t)head * a.queries + row] = (top + __log2f(total)) * kFgLn2;
                 }
-                if (there && a.lse) a.lse[(uint64_t)head * a.queries + row] = (top + __log2f(total)) * kFgLn2;
+                pairs += n != 0;
             }
         }
     }
@@ -660,15 +768,26 @@ struct BwdBlock {
     // 128 x n products of two tiles' rows over head_dim.
     __device__ __forceinline__ void rows_by_rows(uint32_t d, uint32_t x, uint32_t y, uint32_t id, uint32_t steps) const {
         const uint64_t x_d = make_desc_kmajor<128>(x), y_d = make_desc_kmajor<128>(y);
-        for (uint32_t c = 0; c < steps; ++c) {
-            const uint64_t at = (uint64_t)((c & 3) * 2 + (c >> 2) * (kHalfBytes >> 4));
-            mma_f16(d, x_d + at, y_d + at, id, c != 0);
-        }
+        if (steps == DP / 16) {
+#pragma unroll
+            for (uint32_t c = 0; c < DP / 16; ++c) {
+                const uint64_t at = (uint64_t)((c & 3) * 2 + (c >> 2) * (kHalfBytes >> 4));
+                mma_f16(d, x_d + at, y_d + at, id, c != 0);
+            }
+        } else
+            for (uint32_t c = 0; c < steps; ++c) {
+                const uint64_t at = (uint64_t)((c & 3) * 2 + (c >> 2) * (kHalfBytes >> 4));
+                mma_f16(d, x_d + at, y_d + at, id, c != 0);
+            }
     }
     // d += (what the two groups left behind `w`) times the first 16 * steps rows of a tile.
     __device__ __forceinline__ void weights_by_rows(uint32_t d, uint32_t w, uint32_t tile, uint32_t id, uint32_t steps, uint32_t add) const {
         const uint64_t t_d = make_desc_mnmajor(tile, kHalfBytes, 1024, 2);
-        for (uint32_t c = 0; c < steps; ++c) mma_f16_ta(d, w + (c & 3) * 8 + (c >> 2) * 64, t_d + (uint64_t)(c * 128), id, add | c);
+        if (steps == 8) {
+#pragma unroll
+            for (uint32_t c = 0; c < 8; ++c) mma_f16_ta(d, w + (c & 3) * 8 + (c >> 2) * 64, t_d + (uint64_t)(c * 128), id, add | c);
+        } else
+            for (uint32_t c = 0; c < steps; ++c) mma_f16_ta(d, w + (c & 3) * 8 + (c >> 2) * 64, t_d + (uint64_t)(c * 128), id, add | c);
     }
 };
 
@@ -706,7 +825,7 @@ attn_tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const FgAttnSeq s(a, b);
         const uint64_t tok0_ = (uint64_t)tile * tokens;
         const uint32_t tok0 = tok0_ < s.nq ? (uint32_t)tok0_ : s.nq, n_tok = min(tokens, s.nq - tok0);
-        const uint32_t hi = n_tok ? s.seen(a, tok0 + n_tok - 1) : 0, n = (hi + kRows - 1) / kRows;
+        const uint32_t hi = __shfl_sync(0xffffffffu, n_tok ? s.seen(a, tok0 + n_tok - 1) : 0, 0), n = (hi + kRows - 1) / kRows;
         const uint32_t fmt = kFormat<T>, dim16 = round_up(a.dim, 16), steps = dim16 / 16;
         if (warp >= 8) reg_release<72>();
         if (warp == 8) {
@@ -867,9 +986,9 @@ attn_tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         const FgAttnSeq s(a, b);
         const uint64_t j0_ = (uint64_t)tile * kRows;
         const uint32_t j0 = j0_ < s.nk ? (uint32_t)j0_ : s.nk, n_key = min((uint32_t)kRows, s.nk - j0);
-        const uint32_t tok0 = n_key ? s.first_query(a, j0) : s.nq, n = (s.nq - tok0 + tokens - 1) / tokens;
+        const uint32_t tok0 = n_key ? s.first_query(a, j0) : s.nq, left = __shfl_sync(0xffffffffu, s.nq - tok0, 0), n = (left + tokens - 1) / tokens;
         const uint32_t fmt = kFormat<T>, dim16 = round_up(a.dim, 16), steps = dim16 / 16;
-        auto n_row = [&](uint32_t i) { return min(tokens, s.nq - tok0 - i * tokens) * a.group; };
+        auto n_row = [&](uint32_t i) { return min(tokens, left - i * tokens) * a.group; };
         if (warp >= 8) reg_release<72>();
         if (warp == 8) {
             // ---- loads: k and v, then q (read twice, and last) and dout ----
@@ -1144,8 +1263,9 @@ int32_t fwd_launch(fg_ctx* ctx, const FgAttnArgs& a) {
     if ((s = make_map(ctx, &k, a.k, half, a.dim, a.kv_heads, a.keys, a.k_stride, 1, kRows)) != FG_OK) return s;
     if ((s = make_map(ctx, &v, a.v, half, a.dim, a.kv_heads, a.keys, a.v_stride, 1, kRows)) != FG_OK) return s;
     const uint64_t tiles = fg_attn_tiles(a.sequences, a.queries, 1, 2 * tokens);
-    if (tiles * a.kv_heads >= 1ull << 31) return fg_fail(ctx, FG_ERR_INVALID_ARGUMENT, "attention: tensor too large");
-    fg_launch(ctx, attn_tc_fwd_kernel<T, DP>, (unsigned)(tiles * a.kv_heads), Cfg::kThreads, Cfg::kSmem, q, k, v, a, tokens, (uint32_t)tiles);
+    if (tiles * a.kv_heads >= (1ull << 31) - 65536) return fg_fail(ctx, FG_ERR_INVALID_ARGUMENT, "attention: tensor too large");
+    const uint64_t all = tiles * a.kv_heads, sms = fg_free_sms(ctx);
+    fg_launch(ctx, attn_tc_fwd_kernel<T, DP>, (unsigned)(all < sms ? all : sms), Cfg::kThreads, Cfg::kSmem, q, k, v, a, tokens, (uint32_t)tiles, fg_arrivals(ctx));
     FG_LAUNCHED(ctx);
     return FG_OK;
 }
