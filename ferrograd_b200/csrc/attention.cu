@@ -19,14 +19,12 @@ constexpr uint32_t kMaxDim = 256;
 // Threads are 16 x 16: thread (y, x) has rows y * RT .. and keys x, x + 16, .. of a tile's scores, and the same rows (backward over keys: keys) by
 // columns 4 x .. + 64 j of a sum.  Rows of a tile are (query, head of the group) pairs, so the heads of a group share the keys' tile.
 // Rows in shared memory are f32, padded by four words: 16 threads that read 16 bytes each of 16 rows take two passes, the least for 256 bytes.
-__host__ __device__ constexpr int tile_of(int dm) { return dm > 128 ? 32 : 64; }
-
 // Rows [first, first + n) of a tensor's `dim` columns into shared memory, zeros behind the last row and column.
 template <typename T, int kRows, int DM, typename F>
 __device__ __forceinline__ void fetch(float* to, uint32_t n, uint32_t dim, F row) {
     constexpr int kPitch = DM + 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll 4
+#pragma unroll 8
     for (int r = warp; r < kRows; r += kThreads / 32) {
         const T* p = (uint32_t)r < n ? row((uint32_t)r) : nullptr;
 #pragma unroll
@@ -41,6 +39,7 @@ __device__ __forceinline__ void dots(const float* a, const float* b, uint32_t di
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < CT; ++j) s[i][j] = 0.0f;
+#pragma unroll 4
     for (uint32_t d = 0; d < dim; d += 4) {
         float4 x[RT], y[CT];
 #pragma unroll
@@ -99,6 +98,17 @@ __device__ __forceinline__ float half_warp_sum(float v) {
     for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+// Which query and head of the group rows of a tile are: one 64-bit division for a tile, a 32-bit one for a row.
+struct RowPlace {
+    uint32_t i0, g0, group;
+    __device__ __forceinline__ RowPlace(uint64_t first, uint32_t group_) : group(group_) {
+        i0 = (uint32_t)(first / group_);
+        g0 = (uint32_t)(first - (uint64_t)i0 * group_);
+    }
+    __device__ __forceinline__ uint32_t query(uint32_t r) const { return group == 1 ? i0 + r : i0 + (g0 + r) / group; }
+    __device__ __forceinline__ uint32_t head(uint32_t r) const { return group == 1 ? 0 : (g0 + r) % group; }
+};
+
 constexpr int kKeys = 64;
 constexpr size_t rows_bytes(int rt, int dm) { return sizeof(float) * ((size_t)(16 * rt + 2 * kKeys) * (dm + 4) + 16 * rt * (kKeys + 4)); }
 template <typename T, int RT, int DM>
@@ -117,18 +127,15 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const FgAttnArgs a)
     const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
     const T *const q = static_cast<const T*>(a.q), *const k = static_cast<const T*>(a.k) + (uint64_t)s.k0 * a.k_stride + (uint64_t)kv * dim,
                   *const v = static_cast<const T*>(a.v) + (uint64_t)s.k0 * a.v_stride + (uint64_t)kv * dim;
-    fetch<T, R, DM>(qs, n, dim, [&](uint32_t r) {
-        const uint64_t at = first + r;
-        const uint32_t i = (uint32_t)(at / a.group), g = (uint32_t)(at - (uint64_t)i * a.group);
-        return q + (uint64_t)(s.q0 + i) * a.q_stride + (uint64_t)(kv * a.group + g) * dim;
-    });
+    const RowPlace place(first, a.group);
+    fetch<T, R, DM>(qs, n, dim, [&](uint32_t r) { return q + (uint64_t)(s.q0 + place.query(r)) * a.q_stride + (uint64_t)(kv * a.group + place.head(r)) * dim; });
     uint32_t seen[RT];
     float top[RT], sum[RT];
     float4 acc[RT][DM / 64];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
         const uint32_t r = y * RT + i;
-        seen[i] = r < n ? s.seen(a, (uint32_t)((first + r) / a.group)) : 0;
+        seen[i] = r < n ? s.seen(a, place.query(r)) : 0;
         top[i] = -INFINITY;
         sum[i] = 0.0f;
 #pragma unroll
@@ -136,7 +143,7 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const FgAttnArgs a)
     }
     uint32_t lo, hi;
     if (!s.share(a, blockIdx.z, &lo, &hi)) return;
-    hi = min(hi, s.seen(a, (uint32_t)((first + n - 1) / a.group)));
+    hi = min(hi, s.seen(a, place.query(n - 1)));
     const float by = a.scale * kFgLog2e;
     for (uint32_t j0 = lo; j0 < hi; j0 += kKeys) {
         const uint32_t there = min((uint32_t)kKeys, s.nk - j0);
@@ -187,8 +194,7 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const FgAttnArgs a)
     for (int i = 0; i < RT; ++i) {
         const uint32_t r = y * RT + i;
         if (r >= n) continue;
-        const uint64_t at = first + r;
-        const uint32_t row = s.q0 + (uint32_t)(at / a.group), head = kv * a.group + (uint32_t)(at % a.group);
+        const uint32_t row = s.q0 + place.query(r), head = kv * a.group + place.head(r);
         const uint64_t line = (uint64_t)row * a.heads + head;
         if (a.splits > 1) {
             const uint64_t part = (uint64_t)blockIdx.z * a.queries * a.heads + line;
@@ -201,42 +207,68 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const FgAttnArgs a)
     }
 }
 
-// Shares of the keys joined: a warp per row.  The same numbering of rows as the kernel before it, 8 rows a block.
+// Shares of the keys joined: four warps a row (a query's head), each with every fourth share; the same numbering of rows as the kernel before it, 2 rows
+// a block.  All of a warp's loads are independent of one another (128 shares of a row one after the other took 50 us).
+constexpr uint32_t kMaxSplits = 128, kJoinRows = 2, kJoinWarps = 4;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) attn_join_kernel(const FgAttnArgs a) {
+    __shared__ float sums[kJoinRows][kJoinWarps][kMaxDim];
     fg_grid_enter();
     uint32_t tile;
-    const int b = fg_attn_find(a.q_starts, a.sequences, a.queries, a.heads, 8, blockIdx.x, &tile);
+    const int b = fg_attn_find(a.q_starts, a.sequences, a.queries, a.heads, kJoinRows, blockIdx.x, &tile);
     if (b < 0) return;
     const FgAttnSeq s(a, b);
-    const uint64_t at = (uint64_t)tile * 8 + (threadIdx.x >> 5);
-    if (at >= (uint64_t)s.nq * a.heads) return;
-    const uint32_t lane = threadIdx.x & 31, row = s.q0 + (uint32_t)(at / a.heads), head = (uint32_t)(at % a.heads);
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp / kJoinWarps, part = warp % kJoinWarps;
+    const uint64_t at = (uint64_t)tile * kJoinRows + mine;
+    const bool there = at < (uint64_t)s.nq * a.heads;
+    const uint32_t row = s.q0 + (uint32_t)(at / a.heads), head = (uint32_t)(at % a.heads), splits = s.shares(a);
     const uint64_t line = (uint64_t)row * a.heads + head, pitch = (uint64_t)a.queries * a.heads;
-    const uint32_t splits = s.shares(a);
-    float top = -INFINITY;
-    for (uint32_t z = lane; z < splits; z += 32) top = fmaxf(top, a.part_stat[z * pitch + line].x);
+    float2 st[kMaxSplits / 32];
+    float top = -INFINITY, sum = 0.0f, acc[kMaxDim / 32];
+#pragma unroll
+    for (int i = 0; i < (int)kMaxSplits / 32; ++i) {
+        const uint32_t z = lane + 32 * i;
+        st[i] = there && z < splits ? a.part_stat[z * pitch + line] : make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, st[i].x);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, acc[kMaxDim / 32];
+#pragma unroll
+    for (int i = 0; i < (int)kMaxSplits / 32; ++i) {
+        st[i].x = st[i].y == 0.0f ? 0.0f : fg_ex2_fast(st[i].x - base);      // the share's factor; a share that saw nothing has none
+        sum = __fmaf_rn(st[i].x, st[i].y, sum);
+    }
+    sum = fg_warp_sum(sum);
 #pragma unroll
     for (int c = 0; c < (int)kMaxDim / 32; ++c) acc[c] = 0.0f;
-    for (uint32_t z = 0; z < splits; ++z) {
-        const float2 st = a.part_stat[z * pitch + line];
-        if (st.y == 0.0f) continue;
-        const float w = fg_ex2_fast(st.x - base), *const p = a.part_out + (z * pitch + line) * a.dim;
-        sum = __fmaf_rn(w, st.y, sum);
 #pragma unroll
-        for (int c = 0; c < (int)kMaxDim / 32; ++c)
-            if (lane + 32 * c < a.dim) acc[c] = __fmaf_rn(w, p[lane + 32 * c], acc[c]);
+    for (int i = 0; i < (int)kMaxSplits / 32; ++i) {
+        if (32u * i >= splits) break;
+#pragma unroll 4
+        for (uint32_t l = part; l < 32; l += kJoinWarps) {
+            const float w = __shfl_sync(0xffffffffu, st[i].x, l);
+            const float* const p = a.part_out + ((32 * i + l) * pitch + line) * a.dim;
+            if (there && w != 0.0f)
+#pragma unroll
+                for (int c = 0; c < (int)kMaxDim / 32; ++c)
+                    if (lane + 32 * c < a.dim) acc[c] = __fmaf_rn(w, __ldcg(p + lane + 32 * c), acc[c]);
+        }
     }
-    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T* const out = static_cast<T*>(a.out) + line * a.dim;
 #pragma unroll
     for (int c = 0; c < (int)kMaxDim / 32; ++c)
-        if (lane + 32 * c < a.dim) out[lane + 32 * c] = fg_narrow<T>(acc[c] * by);
-    if (lane == 0 && a.lse) a.lse[(uint64_t)head * a.queries + row] = (top + __log2f(sum)) * kFgLn2;
+        if (lane + 32 * c < a.dim) sums[mine][part][lane + 32 * c] = acc[c];
+    __syncthreads();
+    if (!there) return;
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* const out = static_cast<T*>(a.out) + line * a.dim;
+    for (uint32_t d = part * 32 + lane; d < a.dim; d += 32 * kJoinWarps) {
+        float v = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < kJoinWarps; ++w) v += sums[mine][w][d];
+        out[d] = fg_narrow<T>(v * by);
+    }
+    if (part == 0 && lane == 0 && a.lse) a.lse[(uint64_t)head * a.queries + row] = (top + __log2f(sum)) * kFgLn2;
 }
 
 // delta_i = dout_i . out_i, a warp per row; [heads][queries].
@@ -252,11 +284,11 @@ __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const T* out, cons
     if (lane == 0) delta[(line % heads) * queries + line / heads] = s;
 }
 
-constexpr size_t bwd_bytes(int dm) { return sizeof(float) * (4 * (size_t)tile_of(dm) * (dm + 4) + 2 * tile_of(dm) * (tile_of(dm) + 4) + 2 * tile_of(dm)); }
+constexpr size_t bwd_bytes(int dm, int n) { return sizeof(float) * (4 * (size_t)n * (dm + 4) + 2 * n * (n + 4) + 2 * n); }
 // The weights and the gradients of the scores of a tile of rows and keys, in shared memory by row.
-template <typename T, int DM>
+template <typename T, int DM, int N_>
 struct BwdTile {
-    static constexpr int N = tile_of(DM), RT = N / 16, kPitch = DM + 4, kP = N + 4;
+    static constexpr int N = N_, RT = N / 16, kPitch = DM + 4, kP = N + 4;
     float *qs, *dos, *ks, *vs, *ps, *ds, *stat;      // stat: lse in powers of two, delta
     __device__ __forceinline__ explicit BwdTile(float* shared) {
         qs = shared;
@@ -272,11 +304,10 @@ struct BwdTile {
         fetch<T, N, DM>(ks, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.k) + (uint64_t)(s.k0 + j0 + r) * a.k_stride + (uint64_t)kv * a.dim; });
         fetch<T, N, DM>(vs, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.v) + (uint64_t)(s.k0 + j0 + r) * a.v_stride + (uint64_t)kv * a.dim; });
     }
-    __device__ __forceinline__ void rows(const FgAttnArgs& a, const FgAttnSeq& s, uint32_t kv, uint64_t first, uint32_t n) {
+    __device__ __forceinline__ void rows(const FgAttnArgs& a, const FgAttnSeq& s, uint32_t kv, const RowPlace& at, uint32_t n) {
         auto place = [&](uint32_t r, uint32_t* i, uint32_t* head) {
-            const uint64_t at = first + r;
-            *i = s.q0 + (uint32_t)(at / a.group);
-            *head = kv * a.group + (uint32_t)(at % a.group);
+            *i = s.q0 + at.query(r);
+            *head = kv * a.group + at.head(r);
         };
         fetch<T, N, DM>(qs, n, a.dim, [&](uint32_t r) {
             uint32_t i, h;
@@ -300,9 +331,9 @@ struct BwdTile {
             stat[N + threadIdx.x] = delta;
         }
     }
-    // Rows first .. first + n of the sequence against keys from j0 on; p is left out where it is not wanted.
+    // n rows from `at` on against keys from j0 on; p is left out where it is not wanted.
     template <bool kP_>
-    __device__ __forceinline__ void weights(const FgAttnArgs& a, const FgAttnSeq& s, uint64_t first, uint32_t n, uint32_t j0) {
+    __device__ __forceinline__ void weights(const FgAttnArgs& a, const FgAttnSeq& s, const RowPlace& at, uint32_t n, uint32_t j0) {
         const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
         float p[RT][RT], dp[RT][RT];
         dots<RT, RT, DM>(qs, ks, a.dim, y * RT, x, p);
@@ -310,7 +341,7 @@ struct BwdTile {
         const float by = a.scale * kFgLog2e;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            const uint32_t r = y * RT + i, seen = r < n ? s.seen(a, (uint32_t)((first + r) / a.group)) : 0;
+            const uint32_t r = y * RT + i, seen = r < n ? s.seen(a, at.query(r)) : 0;
             const float lse = stat[r], delta = stat[N + r];
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
@@ -322,30 +353,30 @@ struct BwdTile {
     }
 };
 
-template <typename T, int DM>
-__global__ void __launch_bounds__(kThreads) attn_dq_kernel(const FgAttnArgs a) {
-    using B = BwdTile<T, DM>;
-    constexpr int N = B::N, RT = B::RT;
-    extern __shared__ float shared[];
-    fg_grid_enter();
+template <typename T, int DM, int N>
+__device__ __forceinline__ void dq_tile(const FgAttnArgs& a, float* shared, uint64_t number) {
+    using B = BwdTile<T, DM, N>;
+    constexpr int RT = B::RT;
     B t(shared);
     uint32_t tile;
-    const int b = fg_attn_find(a.q_starts, a.sequences, a.queries, a.group, N, gridDim.x - 1 - blockIdx.x, &tile);
+    const int b = fg_attn_find(a.q_starts, a.sequences, a.queries, a.group, N, number, &tile);
     if (b < 0) return;
     const FgAttnSeq s(a, b);
     const uint64_t rows = (uint64_t)s.nq * a.group, first = (uint64_t)tile * N;
     if (first >= rows) return;
     const uint32_t n = rows - first < N ? (uint32_t)(rows - first) : N, kv = blockIdx.y;
     const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-    t.rows(a, s, kv, first, n);
+    const RowPlace place(first, a.group);
+    t.rows(a, s, kv, place, n);
     float4 acc[RT][DM / 64] = {};
-    const uint32_t hi = s.seen(a, (uint32_t)((first + n - 1) / a.group));
+    const uint32_t hi = s.seen(a, place.query(n - 1));
     for (uint32_t j0 = 0; j0 < hi; j0 += N) {
         __syncthreads();
         t.keys(a, s, kv, j0);
         __syncthreads();
-        t.template weights<false>(a, s, first, n, j0);
+        t.template weights<false>(a, s, place, n, j0);
         __syncwarp();
+#pragma unroll 2
         for (int c = 0; c < N; c += 4) {
             float4 w[RT];
 #pragma unroll
@@ -363,21 +394,18 @@ __global__ void __launch_bounds__(kThreads) attn_dq_kernel(const FgAttnArgs a) {
     for (int i = 0; i < RT; ++i) {
         const uint32_t r = y * RT + i;
         if (r >= n) continue;
-        const uint64_t at = first + r;
-        T* const to = static_cast<T*>(a.dq) + (s.q0 + at / a.group) * a.q_stride + (kv * a.group + at % a.group) * a.dim;
+        T* const to = static_cast<T*>(a.dq) + (uint64_t)(s.q0 + place.query(r)) * a.q_stride + (uint64_t)(kv * a.group + place.head(r)) * a.dim;
         put_row<T, DM>(to, x, a.dim, acc[i], a.scale);
     }
 }
 
-template <typename T, int DM>
-__global__ void __launch_bounds__(kThreads) attn_dkv_kernel(const FgAttnArgs a) {
-    using B = BwdTile<T, DM>;
-    constexpr int N = B::N, RT = B::RT;
-    extern __shared__ float shared[];
-    fg_grid_enter();
+template <typename T, int DM, int N>
+__device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uint64_t number) {
+    using B = BwdTile<T, DM, N>;
+    constexpr int RT = B::RT;
     B t(shared);
     uint32_t tile;
-    const int b = fg_attn_find(a.k_starts, a.sequences, a.keys, 1, N, blockIdx.x, &tile);
+    const int b = fg_attn_find(a.k_starts, a.sequences, a.keys, 1, N, number, &tile);
     if (b < 0) return;
     const FgAttnSeq s(a, b);
     const uint64_t j0_ = (uint64_t)tile * N;
@@ -389,11 +417,13 @@ __global__ void __launch_bounds__(kThreads) attn_dkv_kernel(const FgAttnArgs a) 
     const uint64_t rows = (uint64_t)s.nq * a.group;
     for (uint64_t first = (uint64_t)s.first_query(a, j0) * a.group; first < rows; first += N) {
         const uint32_t n = rows - first < N ? (uint32_t)(rows - first) : N;
+        const RowPlace place(first, a.group);
         __syncthreads();
-        t.rows(a, s, kv, first, n);
+        t.rows(a, s, kv, place, n);
         __syncthreads();
-        t.template weights<true>(a, s, first, n, j0);
+        t.template weights<true>(a, s, place, n, j0);
         __syncthreads();
+#pragma unroll 4
         for (int r = 0; r < N; ++r) {
             float p[RT], d[RT];
 #pragma unroll
@@ -414,6 +444,15 @@ __global__ void __launch_bounds__(kThreads) attn_dkv_kernel(const FgAttnArgs a) 
     }
 }
 
+// Tiles of keys first (they have more to do), then tiles of rows, the longest of either first.
+template <typename T, int DM, int N>
+__global__ void __launch_bounds__(kThreads) attn_bwd_kernel(const FgAttnArgs a, uint32_t key_tiles, uint32_t row_tiles) {
+    extern __shared__ float shared[];
+    fg_grid_enter();
+    if (blockIdx.x < key_tiles) dkv_tile<T, DM, N>(a, shared, blockIdx.x);
+    else dq_tile<T, DM, N>(a, shared, row_tiles - 1 - (blockIdx.x - key_tiles));
+}
+
 // More shared memory than a kernel may have by default, to the most it is ever given: once per kernel (`done`) and device.
 template <typename K>
 int32_t allow_shared(fg_ctx* ctx, std::atomic<uint64_t>& done, K kernel, size_t bytes) {
@@ -422,38 +461,38 @@ int32_t allow_shared(fg_ctx* ctx, std::atomic<uint64_t>& done, K kernel, size_t 
     done.fetch_or(1ull << (ctx->device & 63), std::memory_order_release);
     return FG_OK;
 }
-template <typename K>
-int32_t launch(fg_ctx* ctx, std::atomic<uint64_t>& done, K kernel, dim3 grid, size_t bytes, const FgAttnArgs& a) {
-    const int32_t s = allow_shared(ctx, done, kernel, bytes);
-    if (s != FG_OK) return s;
-    fg_launch(ctx, kernel, grid, kThreads, bytes, a);
-    FG_LAUNCHED(ctx);
-    return FG_OK;
-}
 template <typename T, int RT, int DM>
 int32_t rows_launch(fg_ctx* ctx, const FgAttnArgs& a) {
     static std::atomic<uint64_t> done{0};
     const dim3 grid((unsigned)fg_attn_tiles(a.sequences, a.queries, a.group, 16 * RT), a.kv_heads, a.splits);
-    return launch(ctx, done, attn_rows_kernel<T, RT, DM>, grid, rows_bytes(RT, DM), a);
+    const int32_t s = allow_shared(ctx, done, attn_rows_kernel<T, RT, DM>, rows_bytes(RT, DM));
+    if (s != FG_OK) return s;
+    fg_launch(ctx, attn_rows_kernel<T, RT, DM>, grid, kThreads, rows_bytes(RT, DM), a);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
 }
-template <typename T, int DM>
-int32_t dq_launch(fg_ctx* ctx, const FgAttnArgs& a) {
+template <typename T, int DM, int N>
+int32_t bwd_launch(fg_ctx* ctx, const FgAttnArgs& a) {
     static std::atomic<uint64_t> done{0};
-    return launch(ctx, done, attn_dq_kernel<T, DM>, dim3((unsigned)fg_attn_tiles(a.sequences, a.queries, a.group, tile_of(DM)), a.kv_heads), bwd_bytes(DM), a);
+    const uint32_t key_tiles = a.dk && a.keys ? (uint32_t)fg_attn_tiles(a.sequences, a.keys, 1, N) : 0;
+    const uint32_t row_tiles = a.dq && a.queries ? (uint32_t)fg_attn_tiles(a.sequences, a.queries, a.group, N) : 0;
+    if (!key_tiles && !row_tiles) return FG_OK;
+    const int32_t s = allow_shared(ctx, done, attn_bwd_kernel<T, DM, N>, bwd_bytes(DM, N));
+    if (s != FG_OK) return s;
+    fg_launch(ctx, attn_bwd_kernel<T, DM, N>, dim3(key_tiles + row_tiles, a.kv_heads), kThreads, bwd_bytes(DM, N), a, key_tiles, row_tiles);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
 }
-template <typename T, int DM>
-int32_t dkv_launch(fg_ctx* ctx, const FgAttnArgs& a) {
-    static std::atomic<uint64_t> done{0};
-    return launch(ctx, done, attn_dkv_kernel<T, DM>, dim3((unsigned)fg_attn_tiles(a.sequences, a.keys, 1, tile_of(DM)), a.kv_heads), bwd_bytes(DM), a);
-}
+// Are there fewer than two blocks of 64 rows for an SM?  Smaller tiles then.
+bool few_tiles(const fg_ctx* ctx, const FgAttnArgs& a) { return fg_attn_tiles(a.sequences, a.queries, a.group, 64) * a.kv_heads < 2ull * ctx->sm_count; }
 
-// Few queries per sequence leave few blocks of rows, so their keys go in shares: about 24 blocks for an SM, each with 64 keys at least and
-// 4096 at most.
+// Few queries per sequence leave few blocks of rows, so their keys go in shares: about 16 blocks for an SM, so that shares of sequences of different
+// lengths even out, each with 128 keys at least and 4096 at most.
 int32_t in_shares(fg_ctx* ctx, FgAttnArgs& a) {
-    const uint64_t units = (uint64_t)a.keys * a.kv_heads / (24ull * ctx->sm_count);
-    const uint64_t chunk = (units < 64 ? 64 : units > 4096 ? 4096 : units) / 64 * 64, usual = a.keys / a.sequences + 1;
+    const uint64_t units = (uint64_t)a.keys * a.kv_heads / (16ull * ctx->sm_count);
+    const uint64_t chunk = (units < 128 ? 128 : units > 4096 ? 4096 : units) / 64 * 64, usual = a.keys / a.sequences + 1;
     uint64_t splits = (a.sequences == 1 ? usual : 4 * usual) / chunk + 1;
-    if (splits > 128) splits = 128;
+    if (splits > kMaxSplits) splits = kMaxSplits;
     a.chunk = (uint32_t)chunk;
     a.splits = (uint32_t)splits;
     if (splits == 1) return FG_OK;
@@ -480,10 +519,10 @@ int32_t attention_fwd(fg_ctx* ctx, FgAttnArgs a) {
     }
     int32_t s;
     if (tc) s = fg_attn_few(ctx, dtype_of<T>, a, (uint32_t)rows);
-    else if (few) s = a.dim <= 64 ? rows_launch<T, 1, 64>(ctx, a) : a.dim <= 128 ? rows_launch<T, 1, 128>(ctx, a) : rows_launch<T, 1, 256>(ctx, a);
+    else if (few || few_tiles(ctx, a)) s = a.dim <= 64 ? rows_launch<T, 1, 64>(ctx, a) : a.dim <= 128 ? rows_launch<T, 1, 128>(ctx, a) : rows_launch<T, 1, 256>(ctx, a);
     else s = a.dim <= 64 ? rows_launch<T, 4, 64>(ctx, a) : a.dim <= 128 ? rows_launch<T, 4, 128>(ctx, a) : rows_launch<T, 4, 256>(ctx, a);
     if (s != FG_OK || a.splits == 1) return s;
-    fg_launch(ctx, attn_join_kernel<T>, (unsigned)fg_attn_tiles(a.sequences, a.queries, a.heads, 8), kThreads, 0, a);
+    fg_launch(ctx, attn_join_kernel<T>, (unsigned)fg_attn_tiles(a.sequences, a.queries, a.heads, kJoinRows), kThreads, 0, a);
     FG_LAUNCHED(ctx);
     return FG_OK;
 }
@@ -501,15 +540,9 @@ int32_t attention_bwd(fg_ctx* ctx, FgAttnArgs a) {
         fg_launch(ctx, attn_delta_kernel<T>, (unsigned)((lines + 7) / 8), kThreads, 0, (const T*)a.out, (const T*)a.dout, (float*)w, a.queries, a.heads, a.dim);
         FG_LAUNCHED(ctx);
     }
-    if (a.dq && lines) {
-        s = a.dim <= 64 ? dq_launch<T, 64>(ctx, a) : a.dim <= 128 ? dq_launch<T, 128>(ctx, a) : dq_launch<T, 256>(ctx, a);
-        if (s != FG_OK) return s;
-    }
-    if (a.dk && a.keys) {
-        s = a.dim <= 64 ? dkv_launch<T, 64>(ctx, a) : a.dim <= 128 ? dkv_launch<T, 128>(ctx, a) : dkv_launch<T, 256>(ctx, a);
-        if (s != FG_OK) return s;
-    }
-    return FG_OK;
+    if (a.dim > 128) return bwd_launch<T, 256, 32>(ctx, a);
+    if (few_tiles(ctx, a)) return a.dim <= 64 ? bwd_launch<T, 64, 32>(ctx, a) : bwd_launch<T, 128, 32>(ctx, a);
+    return a.dim <= 64 ? bwd_launch<T, 64, 64>(ctx, a) : bwd_launch<T, 128, 64>(ctx, a);
 }
 
 // Bytes from the first to behind the last element of a tensor of `rows` tokens.
@@ -530,7 +563,7 @@ int32_t check(fg_ctx* ctx, int32_t dtype, FgAttnArgs& a) {
     FG_REQUIRE(ctx, a.q_stride >= q_line && a.k_stride >= k_line && a.v_stride >= k_line, "attention: a stride is shorter than a token's heads");
     FG_REQUIRE(ctx, a.q_stride < (1u << 30) && a.k_stride < (1u << 30) && a.v_stride < (1u << 30), "attention: stride too large");
     a.group = a.heads / a.kv_heads;
-    FG_REQUIRE(ctx, fg_attn_tiles(a.sequences, a.queries, a.heads, 8) < (1ull << 31), "attention: tensor too large");
+    FG_REQUIRE(ctx, fg_attn_tiles(a.sequences, a.queries, a.heads, 2) < (1ull << 31), "attention: tensor too large");
     FG_REQUIRE(ctx, !a.queries || (a.q && a.out), "attention: NULL pointer");
     FG_REQUIRE(ctx, !a.keys || (a.k && a.v), "attention: NULL pointer");
     FG_REQUIRE(ctx, !a.sequences || (a.q_starts && a.k_starts), "attention: NULL pointer");

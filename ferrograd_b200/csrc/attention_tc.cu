@@ -115,7 +115,7 @@ attn_tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     auto next = [&](FwdWork& w, bool& ok) {
         if (!(ok = await(work_full(taken % W), (taken / W) & 1, a.dev_status, FG_DEVERR_EPI_WAIT))) return false;
         volatile const FwdWork& from = works[taken % W];
-#define FG_TAKE(field) w.field = __shfl_sync(0xffffffffu, from.field, 0);
+#define FG_TAKE(field) w.field = from.field;
         FG_FWD_WORK(FG_TAKE)
 #undef FG_TAKE
         __syncwarp();
@@ -809,18 +809,13 @@ __device__ __forceinline__ void put_sums(uint32_t from, T* to, bool there, int c
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(BwdCfg<DP>::kThreads, 1)
-attn_tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_k,
-                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FgAttnArgs a, uint32_t tokens, uint32_t tiles) {
+__device__ __forceinline__ void tc_dq_tile(const CUtensorMap& tm_q, const CUtensorMap& tm_do, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const FgAttnArgs& a,
+                                           uint32_t tokens, uint32_t number, uint32_t kv, const BwdBlock<DP>& blk) {
     using Cfg = BwdCfg<DP>;
-    extern __shared__ __align__(1024) unsigned char raw[];
-    if (!BwdBlock<DP>::fits(raw, a)) return;
-    const BwdBlock<DP> blk(raw, a);
     const int warp = blk.warp;
     const uint32_t tmem = blk.tmem, t_dp = tmem + 256, t_dq = tmem + 384;      // scores at 0 and 128
-    const uint32_t kv = blockIdx.x % a.kv_heads;
     uint32_t tile;
-    const int b = blk.go ? fg_attn_find(a.q_starts, a.sequences, a.queries, 1, tokens, tiles - 1 - blockIdx.x / a.kv_heads, &tile) : -1;
+    const int b = blk.go ? fg_attn_find(a.q_starts, a.sequences, a.queries, 1, tokens, number, &tile) : -1;
     if (b >= 0) {
         const FgAttnSeq s(a, b);
         const uint64_t tok0_ = (uint64_t)tile * tokens;
@@ -966,22 +961,16 @@ attn_tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
         }
     }
-    blk.end();
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(BwdCfg<DP>::kThreads, 1)
-attn_tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_k,
-                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FgAttnArgs a, uint32_t tokens) {
+__device__ __forceinline__ void tc_dkv_tile(const CUtensorMap& tm_q, const CUtensorMap& tm_do, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const FgAttnArgs& a,
+                                            uint32_t tokens, uint32_t number, uint32_t kv, const BwdBlock<DP>& blk) {
     using Cfg = BwdCfg<DP>;
-    extern __shared__ __align__(1024) unsigned char raw[];
-    if (!BwdBlock<DP>::fits(raw, a)) return;
-    const BwdBlock<DP> blk(raw, a);
     const int warp = blk.warp, lane = blk.lane;
     const uint32_t tmem = blk.tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;      // scores at 0
-    const uint32_t kv = blockIdx.x % a.kv_heads;
     uint32_t tile;
-    const int b = blk.go ? fg_attn_find(a.k_starts, a.sequences, a.keys, 1, kRows, blockIdx.x / a.kv_heads, &tile) : -1;
+    const int b = blk.go ? fg_attn_find(a.k_starts, a.sequences, a.keys, 1, kRows, number, &tile) : -1;
     if (b >= 0) {
         const FgAttnSeq s(a, b);
         const uint64_t j0_ = (uint64_t)tile * kRows;
@@ -1171,6 +1160,19 @@ attn_tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             }
         }
     }
+}
+
+// Tiles of keys first (they have more to do), then tiles of rows, which fill the SMs that the last of those leave; the longest of either first.
+template <typename T, int DP>
+__global__ void __launch_bounds__(BwdCfg<DP>::kThreads, 1)
+attn_tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_k,
+                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FgAttnArgs a, uint32_t tokens, uint32_t key_tiles, uint32_t row_tiles) {
+    extern __shared__ __align__(1024) unsigned char raw[];
+    if (!BwdBlock<DP>::fits(raw, a)) return;
+    const BwdBlock<DP> blk(raw, a);
+    const uint32_t number = blockIdx.x / a.kv_heads, kv = blockIdx.x % a.kv_heads;
+    if (number < key_tiles) tc_dkv_tile<T, DP>(tm_q, tm_do, tm_k, tm_v, a, tokens, number, kv, blk);
+    else tc_dq_tile<T, DP>(tm_q, tm_do, tm_k, tm_v, a, tokens, row_tiles - 1 - (number - key_tiles), kv, blk);
     blk.end();
 }
 
@@ -1303,20 +1305,13 @@ int32_t bwd_launch(fg_ctx* ctx, FgAttnArgs a) {
     if ((s = make_map(ctx, &d, a.dout, half, a.dim, a.heads, a.queries, (uint64_t)a.heads * a.dim, a.group, tokens)) != FG_OK) return s;
     if ((s = make_map(ctx, &k, a.k, half, a.dim, a.kv_heads, a.keys, a.k_stride, 1, kRows)) != FG_OK) return s;
     if ((s = make_map(ctx, &v, a.v, half, a.dim, a.kv_heads, a.keys, a.v_stride, 1, kRows)) != FG_OK) return s;
-    const uint64_t row_tiles = fg_attn_tiles(a.sequences, a.queries, 1, tokens), key_tiles = fg_attn_tiles(a.sequences, a.keys, 1, kRows);
-    if (row_tiles * a.kv_heads >= 1ull << 31 || key_tiles * a.kv_heads >= 1ull << 31) return fg_fail(ctx, FG_ERR_INVALID_ARGUMENT, "attention: tensor too large");
-    if (a.dq) {
-        static std::atomic<uint64_t> done{0};
-        if ((s = allow_shared(ctx, done, attn_tc_dq_kernel<T, DP>, Cfg::kSmem)) != FG_OK) return s;
-        fg_launch(ctx, attn_tc_dq_kernel<T, DP>, (unsigned)(row_tiles * a.kv_heads), Cfg::kThreads, Cfg::kSmem, q, d, k, v, a, tokens, (uint32_t)row_tiles);
-        FG_LAUNCHED(ctx);
-    }
-    if (a.dk) {
-        static std::atomic<uint64_t> done{0};
-        if ((s = allow_shared(ctx, done, attn_tc_dkv_kernel<T, DP>, Cfg::kSmem)) != FG_OK) return s;
-        fg_launch(ctx, attn_tc_dkv_kernel<T, DP>, (unsigned)(key_tiles * a.kv_heads), Cfg::kThreads, Cfg::kSmem, q, d, k, v, a, tokens);
-        FG_LAUNCHED(ctx);
-    }
+    const uint64_t row_tiles = a.dq ? fg_attn_tiles(a.sequences, a.queries, 1, tokens) : 0, key_tiles = a.dk ? fg_attn_tiles(a.sequences, a.keys, 1, kRows) : 0;
+    const uint64_t blocks = (row_tiles + key_tiles) * a.kv_heads;
+    if (blocks >= 1ull << 31) return fg_fail(ctx, FG_ERR_INVALID_ARGUMENT, "attention: tensor too large");
+    static std::atomic<uint64_t> done{0};
+    if ((s = allow_shared(ctx, done, attn_tc_bwd_kernel<T, DP>, Cfg::kSmem)) != FG_OK) return s;
+    fg_launch(ctx, attn_tc_bwd_kernel<T, DP>, (unsigned)blocks, Cfg::kThreads, Cfg::kSmem, q, d, k, v, a, tokens, (uint32_t)key_tiles, (uint32_t)row_tiles);
+    FG_LAUNCHED(ctx);
     return FG_OK;
 }
 
