@@ -486,11 +486,16 @@ int32_t bwd_launch(fg_ctx* ctx, const FgAttnArgs& a) {
 // Are there fewer than two blocks of 64 rows for an SM?  Smaller tiles then.
 bool few_tiles(const fg_ctx* ctx, const FgAttnArgs& a) { return fg_attn_tiles(a.sequences, a.queries, a.group, 64) * a.kv_heads < 2ull * ctx->sm_count; }
 
-// Few queries per sequence leave few blocks of rows, so their keys go in shares: about 16 blocks for an SM, so that shares of sequences of different
-// lengths even out, each with 128 keys at least and 4096 at most.
+// Few queries per sequence leave few blocks of rows, so their keys go in shares.  A block costs some 3 us beside its keys (0.4 us for 64 of 128 columns), so a
+// share has 512 keys or more, up to 4096 where there are enough for 16 blocks an SM (shares of sequences of different lengths even out then); fewer, but 128
+// at least, only while there are not two blocks for every SM, which run at a time.  One sequence is cut for those two.  4 sequences of 5000 keys, 8 heads of 128:
+// 40 us in shares of 128, XX like this.
 int32_t in_shares(fg_ctx* ctx, FgAttnArgs& a) {
-    const uint64_t units = (uint64_t)a.keys * a.kv_heads / (16ull * ctx->sm_count);
-    const uint64_t chunk = (units < 128 ? 128 : units > 4096 ? 4096 : units) / 64 * 64, usual = a.keys / a.sequences + 1;
+    const uint64_t all = (uint64_t)a.keys * a.kv_heads, once = all / (2ull * ctx->sm_count) + 63, usual = a.keys / a.sequences + 1;
+    uint64_t chunk = all / (16ull * ctx->sm_count);
+    chunk = chunk < 512 ? 512 : chunk > 4096 ? 4096 : chunk;
+    if (a.sequences == 1 || chunk > once) chunk = once;
+    chunk = (chunk < 128 ? 128 : chunk) / 64 * 64;
     uint64_t splits = (a.sequences == 1 ? usual : 4 * usual) / chunk + 1;
     if (splits > kMaxSplits) splits = kMaxSplits;
     a.chunk = (uint32_t)chunk;
