@@ -1204,25 +1204,29 @@ __global__ void __launch_bounds__(256) attn_tc_delta_kernel(const FgAttnArgs a, 
         if (sub == 0 && line < lines) delta[line % a.heads * a.queries + line / a.heads] = d;
     }
 }
-// The largest |x| of the sequences' rows (as bits, so NaN is larger than infinity): 64 rows of `line` 16-byte words a block.
+// The largest |dout| and |v| of the sequences' rows (as bits, so NaN is larger than infinity): 64 rows a block, first those of dout.
 template <typename T>
-__global__ void __launch_bounds__(256) attn_most_kernel(const FgAttnArgs a, const T* x, uint64_t stride, uint32_t line, int keys, uint32_t* most) {
+__global__ void __launch_bounds__(256) attn_most_kernel(const FgAttnArgs a, uint32_t row_tiles, uint32_t* most) {
     fg_grid_enter();
+    const bool keys = blockIdx.x >= row_tiles;
     uint32_t tile;
-    const int b = fg_attn_find(keys ? a.k_starts : a.q_starts, a.sequences, keys ? a.keys : a.queries, 1, 64, blockIdx.x, &tile);
+    const int b = fg_attn_find(keys ? a.k_starts : a.q_starts, a.sequences, keys ? a.keys : a.queries, 1, 64, blockIdx.x - (keys ? row_tiles : 0), &tile);
     if (b < 0) return;
     const FgAttnSeq s(a, b);
-    const uint64_t n = keys ? s.nk : s.nq, r0 = (uint64_t)tile * 64;
+    const uint64_t n = keys ? s.nk : s.nq, r0 = (uint64_t)tile * 64, stride = keys ? a.v_stride : (uint64_t)a.heads * a.dim;
+    const uint32_t line = (keys ? a.kv_heads : a.heads) * a.dim / 8;      // 16-byte words
+    const T* const x = static_cast<const T*>(keys ? a.v : a.dout) + (uint64_t)(keys ? s.k0 : s.q0) * stride;
     uint32_t m = 0;
     for (uint64_t r = r0 + (threadIdx.x >> 5); r < n && r < r0 + 64; r += 8)
+#pragma unroll 4
         for (uint32_t c = threadIdx.x & 31; c < line; c += 32) {
             float v[8];
-            FgPack<T>::widen(*reinterpret_cast<const uint4*>(x + ((keys ? s.k0 : s.q0) + r) * stride + c * 8), v);
+            FgPack<T>::widen(*reinterpret_cast<const uint4*>(x + r * stride + c * 8), v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(fabsf(v[e])));
         }
     m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0 && m) atomicMax(most, m);      // (the largest of numbers: whoever comes first)
+    if ((threadIdx.x & 31) == 0 && m) atomicMax(most + keys, m);      // (the largest of numbers: whoever comes first)
 }
 
 // ---- host ----
@@ -1293,10 +1297,8 @@ int32_t bwd_launch(fg_ctx* ctx, FgAttnArgs a) {
     }
     if (half) {
         FG_CUDA(ctx, FG_ERR_FAILED_BUFFER_COPY, cudaMemsetAsync(most, 0, 8, ctx->stream));
-        fg_launch(ctx, attn_most_kernel<T>, (unsigned)fg_attn_tiles(a.sequences, a.queries, 1, 64), 256, 0, a, (const T*)a.dout, (uint64_t)a.heads * a.dim,
-                  a.heads * a.dim / 8, 0, most);
-        FG_LAUNCHED(ctx);
-        fg_launch(ctx, attn_most_kernel<T>, (unsigned)fg_attn_tiles(a.sequences, a.keys, 1, 64), 256, 0, a, (const T*)a.v, a.v_stride, a.kv_heads * a.dim / 8, 1, most + 1);
+        const uint64_t row_tiles = fg_attn_tiles(a.sequences, a.queries, 1, 64), both = row_tiles + fg_attn_tiles(a.sequences, a.keys, 1, 64);
+        fg_launch(ctx, attn_most_kernel<T>, (unsigned)both, 256, 0, a, (uint32_t)row_tiles, most);
         FG_LAUNCHED(ctx);
     }
     const uint32_t tokens = kRows / a.group;

@@ -200,8 +200,8 @@ __device__ __forceinline__ void place_entries(const uint64_t* list, uint32_t n, 
 }
 
 // A row per cluster of blocks, each with a stretch of it.
-// The alternatives: each of the 8 warps' ceil(top / 8) largest among its lanes' largest entries are `top` entries or more, so the least of them is a bound that
-// the top entries reach, and few others do: a second reading (from the L2) lists those, and the list is put in order by counting how many are larger.  Where
+// The alternatives: the warps that have words each name the same number of their lanes' largest entries, `top` or more together, so the least of them is a bound
+// that the top entries reach, and few others do: a second reading (from the L2) lists those, and the list is put in order by counting how many are larger.  Where
 // more than the list holds reach the bound (a few threads have them), the largest below the one before is sought top times over.  The blocks' lists go to
 // the first, which puts them in order the same way.
 template <typename T, bool kEntropy, bool kTop>
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_row_kernel(const LogprobA
     constexpr int E = FgPack<T>::E, kWarps = kThreads / 32;
     __shared__ Part parts[kWarps], others[kMaxCluster];
     __shared__ uint64_t keys[kWarps], list[kTop ? kList : 1], sorted[kTop ? kMaxTop : 1], all[kTop ? kMaxTop * kMaxCluster : 1];
-    __shared__ uint32_t count;
+    __shared__ uint32_t count, names[kWarps];
     fg_grid_enter();
     const uint32_t blocks = a.blocks, rank = blockIdx.x % blocks, r = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31;
     const uint32_t target = a.targets ? a.targets[r] : 0;
@@ -231,16 +231,17 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_row_kernel(const LogprobA
     p.join_lanes(by);
     if (lane == 0) parts[tid >> 5] = p;
     if (kTop) {
-        uint32_t v = (uint32_t)(scan.best >> 32);
+        const uint32_t busy = min((uint32_t)kWarps, (to - from + 31) / 32), each = (a.top + (busy ? busy : 1) - 1) / (busy ? busy : 1);
+        uint32_t v = (uint32_t)(scan.best >> 32), named = 0;
         uint64_t least = ~0ull;
-        for (uint32_t i = 0; i < a.top; i += kWarps) {
+        for (; named < each; ++named) {
             const uint32_t most = __reduce_max_sync(0xffffffffu, v), from_lane = __ffs(__ballot_sync(0xffffffffu, v == most)) - 1;
+            if (most == 0) break;      // no more
             const uint64_t k = __shfl_sync(0xffffffffu, scan.best, from_lane);
             if (k < least) least = k;
             if (lane == from_lane) v = 0;
-            if (most == 0) least = 0;      // fewer than that
         }
-        if (lane == 0) keys[tid >> 5] = least;
+        if (lane == 0) { keys[tid >> 5] = least; names[tid >> 5] = named; }
         if (tid == 0) count = 0;
         if (tid < kMaxTop) sorted[tid] = 0;
     }
@@ -249,10 +250,14 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_row_kernel(const LogprobA
     p.join_lanes(by);      // (every warp)
     uint32_t n = 0;        // of this block's alternatives
     if (kTop) {
-        uint64_t least = keys[0];
+        uint64_t least = ~0ull;
+        uint32_t named = 0;
 #pragma unroll
-        for (int i = 1; i < kWarps; ++i) least = least < keys[i] ? least : keys[i];
-        if (least == 0) least = 1;      // every entry that may be an alternative
+        for (int i = 0; i < kWarps; ++i) {
+            least = least < keys[i] ? least : keys[i];
+            named += names[i];
+        }
+        if (named < a.top) least = 1;      // every entry that may be an alternative
         // The entries of this block that reach `floor`: found by words, their indices from a short loop (unrolled into every entry's place it took longer to
         // fetch than to run).
         auto each = [&](float floor, auto take) {

@@ -161,6 +161,101 @@ __global__ void __launch_bounds__(kMaxThreads, C::kTight && C::N <= 16 ? 2 : 1) 
     }
 }
 
+// e4m3 of rows that do not lie straight, or of groups that are more than a warp's packs: kWarps warps a row, a warp has kUnits stretches of 128 columns, a lane every
+// 32nd of them, so groups of 32, 64, 128 and 256 columns are found within a warp.  Read once; elements, not words.
+template <typename T, int kWarps, int kUnits, bool kRes>
+__global__ void __launch_bounds__(256) rms8_ragged_kernel(const RmsArgs a) {
+    constexpr int kPer = 8 / kWarps;      // rows of a block
+    __shared__ float red[2][8];
+    fg_grid_enter();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kWarps;
+    const uint64_t r = (uint64_t)blockIdx.x * kPer + warp / kWarps;
+    const bool there = r < a.rows;
+    const uint64_t at = r * a.cols;
+    const uint32_t first = part * (kUnits * 128) + lane;
+    const T *const x = static_cast<const T*>(a.x) + at, *const res = kRes ? static_cast<const T*>(a.residual) + at : nullptr, *const gamma = static_cast<const T*>(a.gamma);
+    float v[kUnits][4];
+#pragma unroll
+    for (int i = 0; i < kUnits * 4; ++i) {
+        const uint32_t c = first + 32 * i;
+        v[i / 4][i % 4] = there && c < a.cols ? fg_widen(x[c]) : 0.0f;
+    }
+    if (kRes)
+#pragma unroll
+        for (int i = 0; i < kUnits * 4; ++i) {
+            const uint32_t c = first + 32 * i;
+            if (there && c < a.cols) v[i / 4][i % 4] = fg_widen(fg_narrow<T>(v[i / 4][i % 4] + fg_widen(res[c])));
+        }
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kUnits * 4; ++i) s = __fmaf_rn(v[i / 4][i % 4], v[i / 4][i % 4], s);
+    s = fg_warp_sum(s);
+    if (kWarps > 1) {
+        if (lane == 0) red[0][warp] = s;
+        __syncthreads();
+        s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) s += red[0][w];
+    }
+    const float rstd = 1.0f / sqrtf(s / (float)a.cols + a.eps);
+    float most[kUnits][4];
+#pragma unroll
+    for (int i = 0; i < kUnits * 4; ++i) {
+        const uint32_t c = first + 32 * i;
+        if (there && c < a.cols) {
+            if (a.sum) static_cast<T*>(a.sum)[at + c] = fg_narrow<T>(v[i / 4][i % 4]);
+            v[i / 4][i % 4] *= rstd * (gamma ? fg_widen(gamma[c]) : 1.0f);
+        }
+        most[i / 4][i % 4] = fabsf(v[i / 4][i % 4]);
+    }
+    const bool whole = a.groups == 1;      // one scale a row
+    if (whole || a.group >= 64)
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            most[u][0] = most[u][1] = fmaxf(most[u][0], most[u][1]);
+            most[u][2] = most[u][3] = fmaxf(most[u][2], most[u][3]);
+        }
+    if (whole || a.group >= 128)
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) most[u][0] = most[u][1] = most[u][2] = most[u][3] = fmaxf(most[u][0], most[u][2]);
+    if (whole || a.group == 256)
+#pragma unroll
+        for (int u = 0; u + 1 < kUnits; u += 2) {
+            const float m = fmaxf(most[u][0], most[u + 1][0]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most[u][e] = most[u + 1][e] = m;
+        }
+    if (whole) {
+        float m = most[0][0];
+#pragma unroll
+        for (int u = 1; u < kUnits; ++u) m = fmaxf(m, most[u][0]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (kWarps > 1) {
+            if (lane == 0) red[1][warp] = m;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red[1][w]);
+        }
+#pragma unroll
+        for (int i = 0; i < kUnits * 4; ++i) most[i / 4][i % 4] = m;
+    } else
+#pragma unroll
+        for (int i = 0; i < kUnits * 4; ++i)
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) most[i / 4][i % 4] = fmaxf(most[i / 4][i % 4], __shfl_xor_sync(0xffffffffu, most[i / 4][i % 4], o));
+    uint8_t* const y = static_cast<uint8_t*>(a.y) + at;
+#pragma unroll
+    for (int i = 0; i < kUnits * 4; ++i) {
+        const uint32_t c = first + 32 * i;
+        if (!there || c >= a.cols) continue;
+        const float scale = most[i / 4][i % 4] / kE4m3Max;
+        y[c] = to_e4m3(v[i / 4][i % 4], scale);
+        if (whole ? c == 0 : c % a.group == 0) a.scale[r * a.groups + (whole ? 0 : c / a.group)] = scale;
+    }
+    if (there && part == 0 && lane == 0 && a.rstd) a.rstd[r] = rstd;
+}
+
 // The backward pass the same way: kSum with what reaches h by other ways.  With the parameter's gradient (kParams) a thread sums its columns over the rows of its
 // group, a block adds its groups and leaves one row of parts: [block][pitch].
 template <typename C, bool kSum, bool kParams>
@@ -378,28 +473,49 @@ __global__ void __launch_bounds__(256) rms_bwd_stream_kernel(const RmsBwdArgs a)
     }
 }
 
-// dgamma by columns, over chunks of rows: part is [chunks][cols].
+// dgamma by columns, over chunks of rows: part is [chunks][cols].  A warp takes 32 columns, or as many packs of rows that lie straight, and every 8th row.
 constexpr uint32_t kChunk = 256;
-template <typename T>
+template <typename T, bool kPacked>
 __global__ void __launch_bounds__(256) rms_columns_kernel(const RmsBwdArgs a, float* part) {
-    __shared__ float red[8][32];
+    constexpr int E = kPacked ? FgPack<T>::E : 1, kRows = 4;
+    __shared__ float red[8][32][E];
     fg_grid_enter();
-    const uint64_t c = (uint64_t)blockIdx.x * 32 + threadIdx.x;
+    const uint64_t c = ((uint64_t)blockIdx.x * 32 + threadIdx.x) * E;
     const uint32_t r0 = blockIdx.y * kChunk, r1 = min(a.rows, r0 + kChunk);
-    float s = 0.0f;
+    const T *const x = static_cast<const T*>(a.x) + c, *const dy = static_cast<const T*>(a.dy) + c;
+    float s[E] = {};
     if (c < a.cols)
-        for (uint32_t r = r0 + threadIdx.y; r < r1; r += 8) {
-            const uint64_t at = (uint64_t)r * a.cols + c;
-            s = __fmaf_rn(fg_widen(static_cast<const T*>(a.dy)[at]), fg_widen(static_cast<const T*>(a.x)[at]) * a.rstd[r], s);
-        }
-    red[threadIdx.y][threadIdx.x] = s;
-    __syncthreads();
-    if (threadIdx.y == 0 && c < a.cols) {
-        s = 0.0f;
+        for (uint32_t r = r0 + threadIdx.y; r < r1; r += 8 * kRows) {
+            float u[kRows][E], v[kRows][E], rstd[kRows];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
-        part[(uint64_t)blockIdx.y * a.cols + c] = s;
-    }
+            for (int j = 0; j < kRows; ++j) {
+                const uint32_t row = r + 8 * j;
+                const bool there = row < r1;
+                rstd[j] = there ? a.rstd[row] : 0.0f;
+                if constexpr (kPacked) {
+                    FgPack<T>::widen(there ? *reinterpret_cast<const uint4*>(x + (uint64_t)row * a.cols) : make_uint4(0, 0, 0, 0), u[j]);
+                    FgPack<T>::widen(there ? *reinterpret_cast<const uint4*>(dy + (uint64_t)row * a.cols) : make_uint4(0, 0, 0, 0), v[j]);
+                } else {
+                    u[j][0] = there ? fg_widen(x[(uint64_t)row * a.cols]) : 0.0f;
+                    v[j][0] = there ? fg_widen(dy[(uint64_t)row * a.cols]) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kRows; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) s[e] = __fmaf_rn(v[j][e], u[j][e] * rstd[j], s[e]);
+        }
+#pragma unroll
+    for (int e = 0; e < E; ++e) red[threadIdx.y][threadIdx.x][e] = s[e];
+    __syncthreads();
+    if (threadIdx.y == 0 && c < a.cols)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            float t = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t += red[i][threadIdx.x][e];
+            part[(uint64_t)blockIdx.y * a.cols + c + e] = t;
+        }
 }
 template <typename T>
 __global__ void __launch_bounds__(256) rms_fold_kernel(const RmsBwdArgs a, const float* part, uint32_t chunks) {
@@ -454,6 +570,13 @@ int32_t fwd_ragged(fg_ctx* ctx, const RmsArgs& a, bool* took) {
     *took = false;
     return FG_OK;
 }
+template <typename T, int kWarps, int kUnits>
+int32_t ragged_e4m3(fg_ctx* ctx, const RmsArgs& a) {
+    constexpr uint32_t kPer = 8 / kWarps;
+    fg_launch(ctx, a.residual ? rms8_ragged_kernel<T, kWarps, kUnits, true> : rms8_ragged_kernel<T, kWarps, kUnits, false>, (unsigned)(((uint64_t)a.rows + kPer - 1) / kPer), 256, 0, a);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
+}
 template <typename T>
 int32_t rms_fwd(fg_ctx* ctx, const RmsArgs& a) {
     constexpr uint32_t E = FgPack<T>::E;
@@ -467,6 +590,12 @@ int32_t rms_fwd(fg_ctx* ctx, const RmsArgs& a) {
     } else if (straight && fg_aligned16(a.y)) s = res ? fwd_straight<T, true, false>(ctx, a, 0, &took) : fwd_straight<T, false, false>(ctx, a, 0, &took);
     else s = res ? fwd_ragged<T, true>(ctx, a, &took) : fwd_ragged<T, false>(ctx, a, &took);
     if (took) return s;
+    // A row by one warp or eight, 4 to 32 elements a lane (64 spill: 4504 x 9394 f16 984 us, 172 read once per sum).
+    if (a.scale && a.rows < 1u << 31) {
+        if (a.cols <= 128 && a.group != 256) return ragged_e4m3<T, 1, 1>(ctx, a);
+        if (a.cols <= 1024) return ragged_e4m3<T, 1, 8>(ctx, a);
+        if (a.cols <= 4096) return ragged_e4m3<T, 8, 4>(ctx, a);
+    }
     fg_launch(ctx, a.scale ? rms_stream_kernel<T, true> : rms_stream_kernel<T, false>, rows_grid(ctx, a.rows), 256, 0, a);
     FG_LAUNCHED(ctx);
     return FG_OK;
@@ -541,14 +670,18 @@ int32_t rms_bwd(fg_ctx* ctx, const RmsBwdArgs& a) {
             b.dy = static_cast<const T*>(a.dy) + skip * a.cols;
             b.rstd = a.rstd + skip;
             b.rows = a.rows - (uint32_t)skip;
-            fg_launch(ctx, rms_columns_kernel<T>, dim3((unsigned)(((uint64_t)a.cols + 31) / 32), chunks - c0 < 65535 ? chunks - c0 : 65535), dim3(32, 8), 0, b,
-                      (float*)w + (uint64_t)c0 * a.cols);
+            const uint32_t E = straight ? FgPack<T>::E : 1;
+            fg_launch(ctx, straight ? rms_columns_kernel<T, true> : rms_columns_kernel<T, false>,
+                      dim3((unsigned)(((uint64_t)a.cols + 32 * E - 1) / (32 * E)), chunks - c0 < 65535 ? chunks - c0 : 65535), dim3(32, 8), 0, b, (float*)w + (uint64_t)c0 * a.cols);
             FG_LAUNCHED(ctx);
         }
         fg_launch(ctx, rms_fold_kernel<T>, (unsigned)(((uint64_t)a.cols + 255) / 256), 256, 0, a, (const float*)w, chunks);
         FG_LAUNCHED(ctx);
     }
     if (!a.dx) return FG_OK;
+    // dx alone leaves a thread room for 32 columns.
+    const HeldPlan q = straight ? held_plan(ctx, a.rows, a.cols / FgPack<T>::E, 2 * usual, 2 * usual, 2 * usual, tensors, 512) : HeldPlan{};
+    if (q.threads) return a.dsum ? launch_bwd<StraightPart<T, 2 * usual, 3>, true, false>(ctx, a, q, nullptr, 0) : launch_bwd<StraightPart<T, 2 * usual, 2>, false, false>(ctx, a, q, nullptr, 0);
     fg_launch(ctx, rms_bwd_stream_kernel<T>, rows_grid(ctx, a.rows), 256, 0, a);
     FG_LAUNCHED(ctx);
     return FG_OK;
