@@ -98,6 +98,88 @@ __device__ __forceinline__ float half_warp_sum(float v) {
     for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+// ---- f32 products on the tensor cores ----
+// An f32 number is the sum of two tf32 numbers of 11 bits and 2^-22 of itself, and x y = hi hi + hi lo + lo hi within 3 * 2^-22 |x y|: three
+// instructions of 16 x 8 x 8 products, whose sums are f32.  The instruction cuts what it adds to its sums, so a sum over many tiles is
+// made of one that starts at zero for every tile, added in plain f32.
+struct Tf32 { uint32_t hi, lo; };
+__device__ __forceinline__ Tf32 tf32_halves(float x) {
+    const uint32_t hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    return Tf32{hi, __float_as_uint(x - __uint_as_float(hi)) + 0x1000u};
+}
+__device__ __forceinline__ void mma_16x8x8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+struct Left {      // a 16 x 8 block in halves: lane l has rows l / 4 and 8 more, columns l % 4 and 4 more
+    uint32_t hi[4], lo[4];
+    __device__ __forceinline__ Left(float a0, float a1, float a2, float a3) {
+        const float x[4] = {a0, a1, a2, a3};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const Tf32 t = tf32_halves(x[i]);
+            hi[i] = t.hi;
+            lo[i] = t.lo;
+        }
+    }
+    __device__ __forceinline__ void times(float b0, float b1, float (&d)[4]) const {
+        const Tf32 x = tf32_halves(b0), y = tf32_halves(b1);
+        mma_16x8x8(d, lo, x.hi, y.hi);
+        mma_16x8x8(d, hi, x.lo, y.lo);
+        mma_16x8x8(d, hi, x.hi, y.hi);
+    }
+};
+// 16 rows of a by 8 * NT rows of b, over dim columns (zeros behind): lane l has rows l / 4, + 8 and columns 8 t + 2 (l % 4), + 1.
+template <int NT, int DM>
+__device__ __forceinline__ void row_products(const float* a, const float* b, uint32_t dim, float (&s)[NT][4]) {
+    constexpr int kPitch = DM + 4;
+    const int g = (threadIdx.x & 31) >> 2, q = threadIdx.x & 3;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][e] = 0.0f;
+#pragma unroll 2
+    for (uint32_t d = q; d < dim + q; d += 8) {
+        const float* const x = a + g * kPitch + d;
+        const Left left(x[0], x[8 * kPitch], x[4], x[8 * kPitch + 4]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float* const y = b + (8 * t + g) * kPitch + d;
+            left.times(y[0], y[4], s[t]);
+        }
+    }
+}
+// acc += (16 x 8 * steps block given by `left`) times rows of b: 8 * NT columns of it from b on.
+template <int NT, int DM, typename F>
+__device__ __forceinline__ void add_products(F left, const float* b, int steps, float (&acc)[NT][4]) {
+    constexpr int kPitch = DM + 4, kOnce = NT < 4 ? NT : 4;
+    const int g = (threadIdx.x & 31) >> 2, q = threadIdx.x & 3;
+#pragma unroll
+    for (int t0 = 0; t0 < NT; t0 += kOnce) {
+        float f[kOnce][4] = {};
+#pragma unroll 2
+        for (int k = 0; k < steps; ++k) {
+            const Left x = left(k);
+            const float* const y = b + (8 * k + q) * kPitch + 8 * t0 + g;
+#pragma unroll
+            for (int t = 0; t < kOnce; ++t) x.times(y[8 * t], y[4 * kPitch + 8 * t], f[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < kOnce; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[t0 + t][e] += f[t][e];
+    }
+}
+// The lane's columns of a row (e0 = 0: row l / 4; 2: the one 8 below) to memory.
+template <typename T, int NT>
+__device__ __forceinline__ void put_columns(T* to, int c0, uint32_t dim, const float (&v)[NT][4], int e0, float by) {
+    const int c = c0 + 2 * (threadIdx.x & 3);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        if ((uint32_t)(c + 8 * t) < dim) to[c + 8 * t] = fg_narrow<T>(v[t][e0] * by);
+        if ((uint32_t)(c + 8 * t + 1) < dim) to[c + 8 * t + 1] = fg_narrow<T>(v[t][e0 + 1] * by);
+    }
+}
 // Which query and head of the group rows of a tile are: one 64-bit division for a tile, a 32-bit one for a row.
 struct RowPlace {
     uint32_t i0, g0, group;
@@ -207,6 +289,112 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const FgAttnArgs a)
     }
 }
 
+// Many rows: a warp has 16 of a block's 128, and all keys of a tile.  The weights of a tile stay in registers as the left side of the product with v: the lane that has the
+// scores of keys 2 (l % 4) and + 1 takes them for columns l % 4 and + 4, with v's rows in that order.
+constexpr size_t many_bytes(int dm) { return sizeof(float) * (size_t)(128 + 2 * kKeys) * (dm + 4); }
+template <typename T, int DM>
+__global__ void __launch_bounds__(kThreads) attn_many_kernel(const FgAttnArgs a) {
+    constexpr int R = 128, kPitch = DM + 4, NT = kKeys / 8, NS = DM / 8;
+    extern __shared__ float shared[];
+    float *const qs = shared, *const ks = qs + R * kPitch, *const vs = ks + kKeys * kPitch;
+    fg_grid_enter();
+    uint32_t tile;
+    const int b = fg_attn_find(a.q_starts, a.sequences, a.queries, a.group, R, gridDim.x - 1 - blockIdx.x, &tile);
+    if (b < 0) return;
+    const FgAttnSeq s(a, b);
+    const uint64_t rows = (uint64_t)s.nq * a.group, first = (uint64_t)tile * R;
+    if (first >= rows) return;
+    const uint32_t n = rows - first < R ? (uint32_t)(rows - first) : R, kv = blockIdx.y, dim = a.dim, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const uint32_t block = (threadIdx.x >> 5) * 16;
+    const T *const qp = static_cast<const T*>(a.q), *const kp = static_cast<const T*>(a.k) + (uint64_t)s.k0 * a.k_stride + (uint64_t)kv * dim,
+                  *const vp = static_cast<const T*>(a.v) + (uint64_t)s.k0 * a.v_stride + (uint64_t)kv * dim;
+    const RowPlace place(first, a.group);
+    fetch<T, R, DM>(qs, n, dim, [&](uint32_t r) { return qp + (uint64_t)(s.q0 + place.query(r)) * a.q_stride + (uint64_t)(kv * a.group + place.head(r)) * dim; });
+    uint32_t seen[2];
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, acc[NS][4] = {};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) seen[h] = block + g + 8 * h < n ? s.seen(a, place.query(block + g + 8 * h)) : 0;
+    const uint32_t hi = s.seen(a, place.query(n - 1));
+    const float by = a.scale * kFgLog2e;
+    for (uint32_t j0 = 0; j0 < hi; j0 += kKeys) {
+        const uint32_t there = min((uint32_t)kKeys, s.nk - j0);
+        __syncthreads();
+        fetch<T, kKeys, DM>(ks, there, dim, [&](uint32_t r) { return kp + (uint64_t)(j0 + r) * a.k_stride; });
+        fetch<T, kKeys, DM>(vs, there, dim, [&](uint32_t r) { return vp + (uint64_t)(j0 + r) * a.v_stride; });
+        __syncthreads();
+        float p[NT][4];
+        row_products<NT, DM>(qs + block * kPitch, ks, dim, p);
+        // An infinity times half of a number is no number where the half is zero: such scores are made again in one product.
+        bool odd = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= p[t][e] != p[t][e];
+        if (__any_sync(0xffffffffu, odd))
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (p[t][e] != p[t][e]) {
+                        const float *const x = qs + (block + g + 4 * (e & 2)) * kPitch, *const y = ks + (8 * t + 2 * q + (e & 1)) * kPitch;
+                        float v = 0.0f;
+#pragma unroll 1
+                        for (uint32_t d = 0; d < dim; ++d) v = __fmaf_rn(x[d], y[d], v);
+                        p[t][e] = v;
+                    }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 2 * h; e < 2 * h + 2; ++e) {
+                    p[t][e] = j0 + 8 * t + 2 * q + (e & 1) < seen[h] ? p[t][e] * by : -INFINITY;
+                    most = fmaxf(most, p[t][e]);
+                }
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2)), top[h]);
+            const float base = most == -INFINITY ? 0.0f : most, less = fg_ex2_fast(top[h] - base);
+            top[h] = most;
+            sum[h] *= less;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 2 * h; e < 2 * h + 2; ++e) {
+                    p[t][e] = fg_ex2_fast(p[t][e] - base);
+                    sum[h] += p[t][e];
+                }
+#pragma unroll
+            for (int t = 0; t < NS; ++t) { acc[t][2 * h] *= less; acc[t][2 * h + 1] *= less; }
+        }
+#pragma unroll
+        for (int t0 = 0; t0 < NS; t0 += 4) {
+            float f[4][4] = {};
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+                const Left x(p[k][0], p[k][2], p[k][1], p[k][3]);
+                const float* const y = vs + (8 * k + 2 * q) * kPitch + 8 * t0 + g;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) x.times(y[8 * t], y[kPitch + 8 * t], f[t]);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[t0 + t][e] += f[t][e];
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+        const uint32_t r = block + g + 8 * h;
+        if (r >= n) continue;
+        const uint32_t row = s.q0 + place.query(r), head = kv * a.group + place.head(r);
+        put_columns<T, NS>(static_cast<T*>(a.out) + ((uint64_t)row * a.heads + head) * dim, 0, dim, acc, 2 * h, sum[h] == 0.0f ? 0.0f : 1.0f / sum[h]);
+        if (q == 0 && a.lse) a.lse[(uint64_t)head * a.queries + row] = (top[h] + __log2f(sum[h])) * kFgLn2;
+    }
+}
+
 // Shares of the keys joined: four warps a row (a query's head), each with every fourth share; the same numbering of rows as the kernel before it, 2 rows
 // a block.  All of a warp's loads are independent of one another (128 shares of a row one after the other took 50 us).
 constexpr uint32_t kMaxSplits = 128, kJoinRows = 2, kJoinWarps = 4;
@@ -288,7 +476,7 @@ constexpr size_t bwd_bytes(int dm, int n) { return sizeof(float) * (4 * (size_t)
 // The weights and the gradients of the scores of a tile of rows and keys, in shared memory by row.
 template <typename T, int DM, int N_>
 struct BwdTile {
-    static constexpr int N = N_, RT = N / 16, kPitch = DM + 4, kP = N + 4;
+    static constexpr int N = N_, kPitch = DM + 4, kP = N + 4;
     float *qs, *dos, *ks, *vs, *ps, *ds, *stat;      // stat: lse in powers of two, delta
     __device__ __forceinline__ explicit BwdTile(float* shared) {
         qs = shared;
@@ -331,32 +519,50 @@ struct BwdTile {
             stat[N + threadIdx.x] = delta;
         }
     }
+    // The warps: kBlocks of 16 rows (of the sums: rows, or keys) by kSides shares of the columns.
+    static constexpr int kBlocks = N / 16, kSides = 8 / kBlocks, NT = N / 8 / kSides, NS = DM / 8 / kSides;
+    static __device__ __forceinline__ int block() { return (threadIdx.x >> 5) / kSides * 16; }
+    static __device__ __forceinline__ int side() { return (threadIdx.x >> 5) % kSides; }
     // n rows from `at` on against keys from j0 on; p is left out where it is not wanted.
     template <bool kP_>
     __device__ __forceinline__ void weights(const FgAttnArgs& a, const FgAttnSeq& s, const RowPlace& at, uint32_t n, uint32_t j0) {
-        const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-        float p[RT][RT], dp[RT][RT];
-        dots<RT, RT, DM>(qs, ks, a.dim, y * RT, x, p);
-        dots<RT, RT, DM>(dos, vs, a.dim, y * RT, x, dp);
+        const int g = (threadIdx.x & 31) >> 2, q = threadIdx.x & 3, c0 = side() * NT * 8;
+        float p[NT][4], dp[NT][4];
+        row_products<NT, DM>(qs + block() * kPitch, ks + c0 * kPitch, a.dim, p);
+        row_products<NT, DM>(dos + block() * kPitch, vs + c0 * kPitch, a.dim, dp);
         const float by = a.scale * kFgLog2e;
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            const uint32_t r = y * RT + i, seen = r < n ? s.seen(a, at.query(r)) : 0;
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t r = block() + g + 8 * h, seen = r < n ? s.seen(a, at.query(r)) : 0;
             const float lse = stat[r], delta = stat[N + r];
 #pragma unroll
-            for (int j = 0; j < RT; ++j) {
-                const float w = j0 + x + 16 * j < seen ? fg_ex2_fast(__fmaf_rn(p[i][j], by, -lse)) : 0.0f;
-                if (kP_) ps[r * kP + x + 16 * j] = w;
-                ds[r * kP + x + 16 * j] = w == 0.0f ? 0.0f : w * (dp[i][j] - delta);
+            for (int t = 0; t < NT; ++t) {
+                float w[2], d[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    w[e] = j0 + c0 + 8 * t + 2 * q + e < seen ? fg_ex2_fast(__fmaf_rn(p[t][2 * h + e], by, -lse)) : 0.0f;
+                    d[e] = w[e] == 0.0f ? 0.0f : w[e] * (dp[t][2 * h + e] - delta);
+                }
+                const uint32_t to = r * kP + c0 + 8 * t + 2 * q;
+                if (kP_) *reinterpret_cast<float2*>(ps + to) = make_float2(w[0], w[1]);
+                *reinterpret_cast<float2*>(ds + to) = make_float2(d[0], d[1]);
             }
         }
+    }
+    // acc += w (this warp's 16 rows of ds, or columns of ps or ds) times rows of `tile`.
+    __device__ __forceinline__ void add_rows(const float* w, const float* tile, float (&acc)[NS][4]) const {
+        const float* const x = w + (block() + ((threadIdx.x & 31) >> 2)) * kP + (threadIdx.x & 3);
+        add_products<NS, DM>([&](int k) { return Left(x[8 * k], x[8 * kP + 8 * k], x[8 * k + 4], x[8 * kP + 8 * k + 4]); }, tile + side() * NS * 8, N / 8, acc);
+    }
+    __device__ __forceinline__ void add_columns(const float* w, const float* tile, float (&acc)[NS][4]) const {
+        const float* const x = w + (threadIdx.x & 3) * kP + block() + ((threadIdx.x & 31) >> 2);
+        add_products<NS, DM>([&](int k) { return Left(x[8 * k * kP], x[8 * k * kP + 8], x[(8 * k + 4) * kP], x[(8 * k + 4) * kP + 8]); }, tile + side() * NS * 8, N / 8, acc);
     }
 };
 
 template <typename T, int DM, int N>
 __device__ __forceinline__ void dq_tile(const FgAttnArgs& a, float* shared, uint64_t number) {
     using B = BwdTile<T, DM, N>;
-    constexpr int RT = B::RT;
     B t(shared);
     uint32_t tile;
     const int b = fg_attn_find(a.q_starts, a.sequences, a.queries, a.group, N, number, &tile);
@@ -365,44 +571,30 @@ __device__ __forceinline__ void dq_tile(const FgAttnArgs& a, float* shared, uint
     const uint64_t rows = (uint64_t)s.nq * a.group, first = (uint64_t)tile * N;
     if (first >= rows) return;
     const uint32_t n = rows - first < N ? (uint32_t)(rows - first) : N, kv = blockIdx.y;
-    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
     const RowPlace place(first, a.group);
     t.rows(a, s, kv, place, n);
-    float4 acc[RT][DM / 64] = {};
+    float acc[B::NS][4] = {};
     const uint32_t hi = s.seen(a, place.query(n - 1));
     for (uint32_t j0 = 0; j0 < hi; j0 += N) {
         __syncthreads();
         t.keys(a, s, kv, j0);
         __syncthreads();
         t.template weights<false>(a, s, place, n, j0);
-        __syncwarp();
-#pragma unroll 2
-        for (int c = 0; c < N; c += 4) {
-            float4 w[RT];
-#pragma unroll
-            for (int i = 0; i < RT; ++i) w[i] = *reinterpret_cast<const float4*>(t.ds + (y * RT + i) * B::kP + c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float u[RT];
-#pragma unroll
-                for (int i = 0; i < RT; ++i) u[i] = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
-                add_row<RT, DM>(t.ks + (c + e) * B::kPitch, x, u, acc);
-            }
-        }
+        __syncthreads();
+        t.add_rows(t.ds, t.ks, acc);
     }
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const uint32_t r = y * RT + i;
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t r = B::block() + ((threadIdx.x & 31) >> 2) + 8 * h;
         if (r >= n) continue;
         T* const to = static_cast<T*>(a.dq) + (uint64_t)(s.q0 + place.query(r)) * a.q_stride + (uint64_t)(kv * a.group + place.head(r)) * a.dim;
-        put_row<T, DM>(to, x, a.dim, acc[i], a.scale);
+        put_columns<T, B::NS>(to, B::side() * B::NS * 8, a.dim, acc, 2 * h, a.scale);
     }
 }
 
 template <typename T, int DM, int N>
 __device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uint64_t number) {
     using B = BwdTile<T, DM, N>;
-    constexpr int RT = B::RT;
     B t(shared);
     uint32_t tile;
     const int b = fg_attn_find(a.k_starts, a.sequences, a.keys, 1, N, number, &tile);
@@ -411,9 +603,8 @@ __device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uin
     const uint64_t j0_ = (uint64_t)tile * N;
     if (j0_ >= s.nk) return;
     const uint32_t j0 = (uint32_t)j0_, kv = blockIdx.y;
-    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
     t.keys(a, s, kv, j0);
-    float4 dk[RT][DM / 64] = {}, dv[RT][DM / 64] = {};
+    float dk[B::NS][4] = {}, dv[B::NS][4] = {};
     const uint64_t rows = (uint64_t)s.nq * a.group;
     for (uint64_t first = (uint64_t)s.first_query(a, j0) * a.group; first < rows; first += N) {
         const uint32_t n = rows - first < N ? (uint32_t)(rows - first) : N;
@@ -423,24 +614,15 @@ __device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uin
         __syncthreads();
         t.template weights<true>(a, s, place, n, j0);
         __syncthreads();
-#pragma unroll 4
-        for (int r = 0; r < N; ++r) {
-            float p[RT], d[RT];
-#pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                p[i] = t.ps[r * B::kP + y * RT + i];
-                d[i] = t.ds[r * B::kP + y * RT + i];
-            }
-            add_row<RT, DM>(t.dos + r * B::kPitch, x, p, dv);
-            add_row<RT, DM>(t.qs + r * B::kPitch, x, d, dk);
-        }
+        t.add_columns(t.ps, t.dos, dv);
+        t.add_columns(t.ds, t.qs, dk);
     }
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const uint32_t j = j0 + y * RT + i;
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t j = j0 + B::block() + ((threadIdx.x & 31) >> 2) + 8 * h;
         if (j >= s.nk) continue;
-        put_row<T, DM>(static_cast<T*>(a.dk) + (uint64_t)(s.k0 + j) * a.k_stride + (uint64_t)kv * a.dim, x, a.dim, dk[i], a.scale);
-        put_row<T, DM>(static_cast<T*>(a.dv) + (uint64_t)(s.k0 + j) * a.v_stride + (uint64_t)kv * a.dim, x, a.dim, dv[i], 1.0f);
+        put_columns<T, B::NS>(static_cast<T*>(a.dk) + (uint64_t)(s.k0 + j) * a.k_stride + (uint64_t)kv * a.dim, B::side() * B::NS * 8, a.dim, dk, 2 * h, a.scale);
+        put_columns<T, B::NS>(static_cast<T*>(a.dv) + (uint64_t)(s.k0 + j) * a.v_stride + (uint64_t)kv * a.dim, B::side() * B::NS * 8, a.dim, dv, 2 * h, 1.0f);
     }
 }
 
@@ -468,6 +650,15 @@ int32_t rows_launch(fg_ctx* ctx, const FgAttnArgs& a) {
     const int32_t s = allow_shared(ctx, done, attn_rows_kernel<T, RT, DM>, rows_bytes(RT, DM));
     if (s != FG_OK) return s;
     fg_launch(ctx, attn_rows_kernel<T, RT, DM>, grid, kThreads, rows_bytes(RT, DM), a);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
+}
+template <typename T, int DM>
+int32_t many_launch(fg_ctx* ctx, const FgAttnArgs& a) {
+    static std::atomic<uint64_t> done{0};
+    const int32_t s = allow_shared(ctx, done, attn_many_kernel<T, DM>, many_bytes(DM));
+    if (s != FG_OK) return s;
+    fg_launch(ctx, attn_many_kernel<T, DM>, dim3((unsigned)fg_attn_tiles(a.sequences, a.queries, a.group, 128), a.kv_heads), kThreads, many_bytes(DM), a);
     FG_LAUNCHED(ctx);
     return FG_OK;
 }
@@ -525,7 +716,7 @@ int32_t attention_fwd(fg_ctx* ctx, FgAttnArgs a) {
     int32_t s;
     if (tc) s = fg_attn_few(ctx, dtype_of<T>, a, (uint32_t)rows);
     else if (few || few_tiles(ctx, a)) s = a.dim <= 64 ? rows_launch<T, 1, 64>(ctx, a) : a.dim <= 128 ? rows_launch<T, 1, 128>(ctx, a) : rows_launch<T, 1, 256>(ctx, a);
-    else s = a.dim <= 64 ? rows_launch<T, 4, 64>(ctx, a) : a.dim <= 128 ? rows_launch<T, 4, 128>(ctx, a) : rows_launch<T, 4, 256>(ctx, a);
+    else s = a.dim <= 64 ? many_launch<T, 64>(ctx, a) : a.dim <= 128 ? many_launch<T, 128>(ctx, a) : rows_launch<T, 4, 256>(ctx, a);
     if (s != FG_OK || a.splits == 1) return s;
     fg_launch(ctx, attn_join_kernel<T>, (unsigned)fg_attn_tiles(a.sequences, a.queries, a.heads, kJoinRows), kThreads, 0, a);
     FG_LAUNCHED(ctx);

@@ -1,13 +1,15 @@
 """Attention over packed sequences against the formulas in 64 bits.
 
-Bounds, with U = 2^-24 (a sum of n f32 terms is off by at most n U of the sum of their sizes) and h the half step of the storage type:
-  score      e_s = (dim + 8) U scale (|q|.|k|): its products and sum, the factor, the difference from the row's largest, lse
+Bounds, with U = 2^-24 (a sum of n f32 terms is off by at most n U of the sum of their sizes) and h the half step of the storage type.  An f32 product
+on the tensor cores is three of numbers of 11 bits: x = hi + lo + r with |r| <= 2^-22 |x|, and lo lo, at most 2^-22 |x y|, is left out, so it is off by
+3 * 2^-22 |x y| = 12 U |x y|; their sums, three instructions for 8 terms that each cut less than 2 U of the sum, stay within U a term.
+  score      e_s = (dim + 20) U scale (|q|.|k|): its products and sum, the factor, the difference from the row's largest, lse
   weight     relative e_p = e_s + 2^-20 + 4 U |lse| (the exponential, the sums that normalise it), and h where the weights are rounded to 16 bits;
              f16 weights below 2^-14 of the largest are off by 2^-25 of it; weights below 2^-126 are zero
-  out        sum of p e_p (|v| + |out|), n U sum of p |v|, and h |out|
-  ds         p (e_p |dp - delta| + (dim + 4) U (|dout|.|v| + |dout|.|out|)), and h |ds| rounded to 16 bits (f16: and 2^-24 of what the largest dout
+  out        sum of p e_p (|v| + |out|), (n + 20) U sum of p |v|, and h |out|
+  ds         p (e_p |dp - delta| + (dim + 16) U (|dout|.|v| + |dout|.|out|)), and h |ds| rounded to 16 bits (f16: and 2^-24 of what the largest dout
              and v can give, the operands being scaled by a power of two with that)
-  gradients  the sums of these with |k|, |q| and |dout|, n U of the sums of sizes, and h of the result
+  gradients  the sums of these with |k|, |q| and |dout|, (n + 20) U of the sums of sizes, and h of the result
 """
 import numpy as np
 import pytest
@@ -79,7 +81,7 @@ class Case:
         with np.errstate(divide="ignore"):
             lse = np.where(total > 0, top + np.log(total), -np.inf)
         p = e / np.where(total > 0, total, 1.0)[:, None]
-        e_s = (self.dim + 8) * U * abs(float(self.scale)) * (np.abs(q) @ np.abs(k).T)
+        e_s = (self.dim + 20) * U * abs(float(self.scale)) * (np.abs(q) @ np.abs(k).T)
         return p, lse, e_s + 2.0 ** -20 + 4 * U * np.where(np.isfinite(lse), np.abs(lse), 0.0)[:, None]
 
     def forward(self, few=False):
@@ -97,7 +99,7 @@ class Case:
                 e = p * (e_p + (half if tc else 0.0)) + 2.0 ** -126 * (p > 0)
                 if tc and self.dtype == "f16":
                     e = e + p.max(1, initial=0.0)[:, None] * 2.0 ** -24 * (p > 0)
-                e_out[q0:q0 + nq, h] = e @ np.abs(v) + np.abs(o) * e.sum(1)[:, None] + (nk + 8) * U * (p @ np.abs(v)) + half * np.abs(o) + TINY[self.dtype]
+                e_out[q0:q0 + nq, h] = e @ np.abs(v) + np.abs(o) * e.sum(1)[:, None] + (nk + 20) * U * (p @ np.abs(v)) + half * np.abs(o) + TINY[self.dtype]
                 e_lse[h, q0:q0 + nq] = (p * e_p).sum(1) + (nk + 8) * U + 4 * U * np.where(np.isfinite(lse[h, q0:q0 + nq]), np.abs(lse[h, q0:q0 + nq]), 0.0)
         return out, lse, e_out, e_lse
 
@@ -120,7 +122,7 @@ class Case:
                 p = p * np.exp(np.where(ok, true_lse - np.where(ok, given, 0.0), 0.0))[:, None]
                 dp, delta = do @ v.T, (do * o).sum(1)[:, None]
                 ds = p * (dp - delta)
-                e_ds = p * (e_p * np.abs(dp - delta) + (self.dim + 4) * U * (np.abs(do) @ np.abs(v).T + (np.abs(do) * np.abs(o)).sum(1)[:, None]))
+                e_ds = p * (e_p * np.abs(dp - delta) + (self.dim + 16) * U * (np.abs(do) @ np.abs(v).T + (np.abs(do) * np.abs(o)).sum(1)[:, None]))
                 e_ds = e_ds + 2.0 ** -126 * np.abs(dp - delta) * (p > 0)
                 e_pp = p * e_p + 2.0 ** -126 * (p > 0)
                 if tc:
@@ -129,9 +131,9 @@ class Case:
                 g["dq"][i, h] += float(self.scale) * ds @ k
                 g["dk"][j, w] += float(self.scale) * ds.T @ q
                 g["dv"][j, w] += p.T @ do
-                e["dq"][i, h] += sc * (e_ds @ np.abs(k) + (nk + 8) * U * np.abs(ds) @ np.abs(k))
-                e["dk"][j, w] += sc * (e_ds.T @ np.abs(q) + (nq * self.heads + 8) * U * np.abs(ds).T @ np.abs(q))
-                e["dv"][j, w] += e_pp.T @ np.abs(do) + (nq * self.heads + 8) * U * p.T @ np.abs(do)
+                e["dq"][i, h] += sc * (e_ds @ np.abs(k) + (nk + 20) * U * np.abs(ds) @ np.abs(k))
+                e["dk"][j, w] += sc * (e_ds.T @ np.abs(q) + (nq * self.heads + 20) * U * np.abs(ds).T @ np.abs(q))
+                e["dv"][j, w] += e_pp.T @ np.abs(do) + (nq * self.heads + 20) * U * p.T @ np.abs(do)
         for n in g:
             e[n] += half * np.abs(g[n]) + TINY[self.dtype]
         return g, e
