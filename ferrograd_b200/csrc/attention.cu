@@ -14,6 +14,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr uint32_t kMaxDim = 256;
+template <typename T> constexpr int32_t dtype_of = sizeof(T) == 4 ? FG_DTYPE_F32 : std::is_same_v<T, __half> ? FG_DTYPE_F16 : FG_DTYPE_BF16;
 
 // ---- plain FMAs: f32, and 16-bit tensors that the tensor cores' kernels do not take ----
 // Threads are 16 x 16: thread (y, x) has rows y * RT .. and keys x, x + 16, .. of a tile's scores, and the same rows (backward over keys: keys) by
@@ -593,7 +594,7 @@ __device__ __forceinline__ void dq_tile(const FgAttnArgs& a, float* shared, uint
 }
 
 template <typename T, int DM, int N>
-__device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uint64_t number) {
+__device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uint64_t number, uint32_t share) {
     using B = BwdTile<T, DM, N>;
     B t(shared);
     uint32_t tile;
@@ -605,8 +606,9 @@ __device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uin
     const uint32_t j0 = (uint32_t)j0_, kv = blockIdx.y;
     t.keys(a, s, kv, j0);
     float dk[B::NS][4] = {}, dv[B::NS][4] = {};
-    const uint64_t rows = (uint64_t)s.nq * a.group;
-    for (uint64_t first = (uint64_t)s.first_query(a, j0) * a.group; first < rows; first += N) {
+    const uint64_t start = (uint64_t)s.first_query(a, j0) * a.group, all = (uint64_t)s.nq * a.group;
+    const uint64_t each = ((all - start + N - 1) / N + a.row_shares - 1) / a.row_shares * N, rows = min(all, start + (share + 1) * each);
+    for (uint64_t first = start + share * each; first < rows; first += N) {
         const uint32_t n = rows - first < N ? (uint32_t)(rows - first) : N;
         const RowPlace place(first, a.group);
         __syncthreads();
@@ -621,6 +623,11 @@ __device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uin
     for (int h = 0; h < 2; ++h) {
         const uint32_t j = j0 + B::block() + ((threadIdx.x & 31) >> 2) + 8 * h;
         if (j >= s.nk) continue;
+        if (a.row_shares > 1) {
+            put_columns<float, B::NS>(fg_attn_part(a, share, 0, s.k0 + j, kv), B::side() * B::NS * 8, a.dim, dk, 2 * h, a.scale);
+            put_columns<float, B::NS>(fg_attn_part(a, share, 1, s.k0 + j, kv), B::side() * B::NS * 8, a.dim, dv, 2 * h, 1.0f);
+            continue;
+        }
         put_columns<T, B::NS>(static_cast<T*>(a.dk) + (uint64_t)(s.k0 + j) * a.k_stride + (uint64_t)kv * a.dim, B::side() * B::NS * 8, a.dim, dk, 2 * h, a.scale);
         put_columns<T, B::NS>(static_cast<T*>(a.dv) + (uint64_t)(s.k0 + j) * a.v_stride + (uint64_t)kv * a.dim, B::side() * B::NS * 8, a.dim, dv, 2 * h, 1.0f);
     }
@@ -631,8 +638,31 @@ template <typename T, int DM, int N>
 __global__ void __launch_bounds__(kThreads) attn_bwd_kernel(const FgAttnArgs a, uint32_t key_tiles, uint32_t row_tiles) {
     extern __shared__ float shared[];
     fg_grid_enter();
-    if (blockIdx.x < key_tiles) dkv_tile<T, DM, N>(a, shared, blockIdx.x);
-    else dq_tile<T, DM, N>(a, shared, row_tiles - 1 - (blockIdx.x - key_tiles));
+    const uint32_t key_blocks = key_tiles * a.row_shares;
+    if (blockIdx.x < key_blocks) dkv_tile<T, DM, N>(a, shared, blockIdx.x / a.row_shares, blockIdx.x % a.row_shares);
+    else dq_tile<T, DM, N>(a, shared, row_tiles - 1 - (blockIdx.x - key_blocks));
+}
+
+// The shares' sums of the sequences' keys, added in order: 8 keys a block.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) attn_fold_kernel(const FgAttnArgs a) {
+    fg_grid_enter();
+    uint32_t tile;
+    const int b = fg_attn_find(a.k_starts, a.sequences, a.keys, 1, 8, blockIdx.x, &tile);
+    if (b < 0) return;
+    const FgAttnSeq s(a, b);
+    const uint32_t line = a.kv_heads * a.dim;
+    const uint64_t pitch = 2ull * a.keys * line;
+    for (uint64_t j = (uint64_t)tile * 8 + (threadIdx.x >> 5); j < s.nk && j < ((uint64_t)tile + 1) * 8; j += 8)
+        for (uint32_t c = threadIdx.x & 31; c < 2 * line; c += 32) {
+            const uint32_t which = c >= line, d = c - (which ? line : 0);
+            const float* const from = a.part_kv + ((uint64_t)which * a.keys + s.k0 + j) * line + d;
+            float v = 0.0f;
+#pragma unroll 4
+            for (uint32_t z = 0; z < a.row_shares; ++z) v += from[z * pitch];
+            if (which) static_cast<T*>(a.dv)[(s.k0 + j) * a.v_stride + d] = fg_narrow<T>(v);
+            else static_cast<T*>(a.dk)[(s.k0 + j) * a.k_stride + d] = fg_narrow<T>(v);
+        }
 }
 
 // More shared memory than a kernel may have by default, to the most it is ever given: once per kernel (`done`) and device.
@@ -670,9 +700,9 @@ int32_t bwd_launch(fg_ctx* ctx, const FgAttnArgs& a) {
     if (!key_tiles && !row_tiles) return FG_OK;
     const int32_t s = allow_shared(ctx, done, attn_bwd_kernel<T, DM, N>, bwd_bytes(DM, N));
     if (s != FG_OK) return s;
-    fg_launch(ctx, attn_bwd_kernel<T, DM, N>, dim3(key_tiles + row_tiles, a.kv_heads), kThreads, bwd_bytes(DM, N), a, key_tiles, row_tiles);
+    fg_launch(ctx, attn_bwd_kernel<T, DM, N>, dim3(key_tiles * a.row_shares + row_tiles, a.kv_heads), kThreads, bwd_bytes(DM, N), a, key_tiles, row_tiles);
     FG_LAUNCHED(ctx);
-    return FG_OK;
+    return a.row_shares > 1 ? fg_attn_fold(ctx, dtype_of<T>, a) : FG_OK;
 }
 // Are there fewer than two blocks of 64 rows for an SM?  Smaller tiles then.
 bool few_tiles(const fg_ctx* ctx, const FgAttnArgs& a) { return fg_attn_tiles(a.sequences, a.queries, a.group, 64) * a.kv_heads < 2ull * ctx->sm_count; }
@@ -701,8 +731,6 @@ int32_t in_shares(fg_ctx* ctx, FgAttnArgs& a) {
     return FG_OK;
 }
 
-template <typename T> constexpr int32_t dtype_of = sizeof(T) == 4 ? FG_DTYPE_F32 : std::is_same_v<T, __half> ? FG_DTYPE_F16 : FG_DTYPE_BF16;
-
 template <typename T>
 int32_t attention_fwd(fg_ctx* ctx, FgAttnArgs a) {
     const uint64_t rows = ((uint64_t)a.queries * a.group + a.sequences - 1) / a.sequences;      // of a sequence, on average
@@ -728,16 +756,15 @@ int32_t attention_bwd(fg_ctx* ctx, FgAttnArgs a) {
     a.splits = 1;
     if (fg_attn_tc_suits(ctx, dtype_of<T>, a)) return fg_attn_tc_bwd(ctx, dtype_of<T>, a);
     const uint64_t lines = (uint64_t)a.queries * a.heads;
-    void* w;
-    int32_t s = fg_ws_alloc(ctx, 4 * lines, &w);
+    const bool small = a.dim > 128 || few_tiles(ctx, a);
+    const int32_t s = fg_attn_bwd_room(ctx, a, small ? 32 : 64);
     if (s != FG_OK) return s;
-    a.delta = (const float*)w;
     if (lines) {
-        fg_launch(ctx, attn_delta_kernel<T>, (unsigned)((lines + 7) / 8), kThreads, 0, (const T*)a.out, (const T*)a.dout, (float*)w, a.queries, a.heads, a.dim);
+        fg_launch(ctx, attn_delta_kernel<T>, (unsigned)((lines + 7) / 8), kThreads, 0, (const T*)a.out, (const T*)a.dout, const_cast<float*>(a.delta), a.queries, a.heads, a.dim);
         FG_LAUNCHED(ctx);
     }
     if (a.dim > 128) return bwd_launch<T, 256, 32>(ctx, a);
-    if (few_tiles(ctx, a)) return a.dim <= 64 ? bwd_launch<T, 64, 32>(ctx, a) : bwd_launch<T, 128, 32>(ctx, a);
+    if (small) return a.dim <= 64 ? bwd_launch<T, 64, 32>(ctx, a) : bwd_launch<T, 128, 32>(ctx, a);
     return a.dim <= 64 ? bwd_launch<T, 64, 64>(ctx, a) : bwd_launch<T, 128, 64>(ctx, a);
 }
 
@@ -780,7 +807,32 @@ bool rows_meet(const void* p, uint64_t np, const void* q, uint64_t nq, uint64_t 
     return (uint64_t)r < p_line || (uint64_t)r + q_line > stride;
 }
 
+template <typename T>
+int32_t fold(fg_ctx* ctx, const FgAttnArgs& a) {
+    fg_launch(ctx, attn_fold_kernel<T>, (unsigned)fg_attn_tiles(a.sequences, a.keys, 1, 8), kThreads, 0, a);
+    FG_LAUNCHED(ctx);
+    return FG_OK;
+}
+
 }  // namespace
+
+int32_t fg_attn_bwd_room(fg_ctx* ctx, FgAttnArgs& a, uint32_t rows) {
+    const uint64_t blocks = a.dk ? fg_attn_tiles(a.sequences, a.keys, 1, rows) * a.kv_heads : 0, lines = (uint64_t)a.queries * a.heads;
+    a.row_shares = 1;
+    if (blocks && blocks < (uint64_t)ctx->sm_count) {
+        const uint64_t want = 2ull * ctx->sm_count / blocks, have = (uint64_t)a.queries * a.group / a.sequences / (4 * rows), shares = want < have ? want : have;
+        if (shares >= 2) a.row_shares = (uint32_t)(shares < 64 ? shares : 64);
+    }
+    const uint64_t first = (256 + 4 * lines + 255) / 256 * 256;
+    void* w;
+    const int32_t s = fg_ws_alloc(ctx, first + (a.row_shares > 1 ? 8ull * a.row_shares * a.keys * a.kv_heads * a.dim : 0), &w);
+    if (s != FG_OK) return s;
+    a.most = static_cast<const uint32_t*>(w);
+    a.delta = static_cast<const float*>(w) + 64;
+    a.part_kv = reinterpret_cast<float*>(static_cast<char*>(w) + first);
+    return FG_OK;
+}
+int32_t fg_attn_fold(fg_ctx* ctx, int32_t dtype, const FgAttnArgs& a) { return FG_BY_DTYPE(dtype, fold, ctx, a); }
 
 extern "C" {
 

@@ -801,9 +801,16 @@ __device__ __forceinline__ void put_sums(uint32_t from, T* to, bool there, int c
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
+            if constexpr (sizeof(T) == 4) {
+                float4* const p = reinterpret_cast<float4*>(to + c + e);
+                if (!there || c + e >= columns) continue;
+                p[0] = make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
+                p[1] = make_float4(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f, __uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
+            } else {
             const uint4 v = make_uint4(pack2<T>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f), pack2<T>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f),
                                        pack2<T>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f), pack2<T>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f));
             if (there && c + e < columns) *reinterpret_cast<uint4*>(to + c + e) = v;
+            }
         }
     }
 }
@@ -965,7 +972,7 @@ __device__ __forceinline__ void tc_dq_tile(const CUtensorMap& tm_q, const CUtens
 
 template <typename T, int DP>
 __device__ __forceinline__ void tc_dkv_tile(const CUtensorMap& tm_q, const CUtensorMap& tm_do, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const FgAttnArgs& a,
-                                            uint32_t tokens, uint32_t number, uint32_t kv, const BwdBlock<DP>& blk) {
+                                            uint32_t tokens, uint32_t number, uint32_t share, uint32_t kv, const BwdBlock<DP>& blk) {
     using Cfg = BwdCfg<DP>;
     const int warp = blk.warp, lane = blk.lane;
     const uint32_t tmem = blk.tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;      // scores at 0
@@ -975,7 +982,9 @@ __device__ __forceinline__ void tc_dkv_tile(const CUtensorMap& tm_q, const CUten
         const FgAttnSeq s(a, b);
         const uint64_t j0_ = (uint64_t)tile * kRows;
         const uint32_t j0 = j0_ < s.nk ? (uint32_t)j0_ : s.nk, n_key = min((uint32_t)kRows, s.nk - j0);
-        const uint32_t tok0 = n_key ? s.first_query(a, j0) : s.nq, left = __shfl_sync(0xffffffffu, s.nq - tok0, 0), n = (left + tokens - 1) / tokens;
+        const uint32_t seen0 = n_key ? s.first_query(a, j0) : s.nq, each = ((s.nq - seen0 + tokens - 1) / tokens + a.row_shares - 1) / a.row_shares;
+        const uint32_t tok0 = (uint32_t)min((uint64_t)s.nq, seen0 + (uint64_t)share * each * tokens);      // of this share
+        const uint32_t left = __shfl_sync(0xffffffffu, (uint32_t)min((uint64_t)(s.nq - tok0), (uint64_t)each * tokens), 0), n = (left + tokens - 1) / tokens;
         const uint32_t fmt = kFormat<T>, dim16 = round_up(a.dim, 16), steps = dim16 / 16;
         auto n_row = [&](uint32_t i) { return min(tokens, left - i * tokens) * a.group; };
         if (warp >= 8) reg_release<72>();
@@ -1154,7 +1163,12 @@ __device__ __forceinline__ void tc_dkv_tile(const CUtensorMap& tm_q, const CUten
                 tc_fence_after();
                 T* const to = side ? static_cast<T*>(a.dk) + (uint64_t)(s.k0 + key) * a.k_stride + (uint64_t)kv * a.dim
                                    : static_cast<T*>(a.dv) + (uint64_t)(s.k0 + key) * a.v_stride + (uint64_t)kv * a.dim;
-                if (n) put_sums<T, DP>((side ? t_dk : t_dv) + lanes, to, there, (int)a.dim, side ? a.scale / factor : 1.0f);
+                if (a.row_shares > 1) {
+                    float* const part = fg_attn_part(a, share, side ? 0 : 1, s.k0 + key, kv);
+                    if (n) put_sums<float, DP>((side ? t_dk : t_dv) + lanes, part, there, (int)a.dim, side ? a.scale / factor : 1.0f);
+                    else if (there)
+                        for (uint32_t c = 0; c < a.dim; c += 4) *reinterpret_cast<uint4*>(part + c) = make_uint4(0, 0, 0, 0);
+                } else if (n) put_sums<T, DP>((side ? t_dk : t_dv) + lanes, to, there, (int)a.dim, side ? a.scale / factor : 1.0f);
                 else if (there)
                     for (uint32_t c = 0; c < a.dim; c += 8) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
             }
@@ -1170,9 +1184,9 @@ attn_tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     extern __shared__ __align__(1024) unsigned char raw[];
     if (!BwdBlock<DP>::fits(raw, a)) return;
     const BwdBlock<DP> blk(raw, a);
-    const uint32_t number = blockIdx.x / a.kv_heads, kv = blockIdx.x % a.kv_heads;
-    if (number < key_tiles) tc_dkv_tile<T, DP>(tm_q, tm_do, tm_k, tm_v, a, tokens, number, kv, blk);
-    else tc_dq_tile<T, DP>(tm_q, tm_do, tm_k, tm_v, a, tokens, row_tiles - 1 - (number - key_tiles), kv, blk);
+    const uint32_t number = blockIdx.x / a.kv_heads, kv = blockIdx.x % a.kv_heads, key_blocks = key_tiles * a.row_shares;
+    if (number < key_blocks) tc_dkv_tile<T, DP>(tm_q, tm_do, tm_k, tm_v, a, tokens, number / a.row_shares, number % a.row_shares, kv, blk);
+    else tc_dq_tile<T, DP>(tm_q, tm_do, tm_k, tm_v, a, tokens, row_tiles - 1 - (number - key_blocks), kv, blk);
     blk.end();
 }
 
@@ -1281,13 +1295,10 @@ int32_t bwd_launch(fg_ctx* ctx, FgAttnArgs a) {
     using Cfg = BwdCfg<DP>;
     constexpr bool half = std::is_same_v<T, __half>;
     const uint64_t lines = (uint64_t)a.queries * a.heads;
-    void* w;
-    int32_t s = fg_ws_alloc(ctx, 256 + 4 * lines, &w);
+    int32_t s = fg_attn_bwd_room(ctx, a, kRows);
     if (s != FG_OK) return s;
-    uint32_t* const most = static_cast<uint32_t*>(w);
-    float* const delta = static_cast<float*>(w) + 64;
-    a.most = most;
-    a.delta = delta;
+    uint32_t* const most = const_cast<uint32_t*>(a.most);
+    float* const delta = const_cast<float*>(a.delta);
     const uint32_t lanes = a.dim > 64 ? 16 : a.dim > 32 ? 8 : a.dim > 16 ? 4 : a.dim > 8 ? 2 : 1, per = 1024 / lanes;
     const auto kernel = lanes == 16 ? attn_tc_delta_kernel<T, 16> : lanes == 8 ? attn_tc_delta_kernel<T, 8> : lanes == 4 ? attn_tc_delta_kernel<T, 4>
                         : lanes == 2 ? attn_tc_delta_kernel<T, 2> : attn_tc_delta_kernel<T, 1>;
@@ -1308,13 +1319,13 @@ int32_t bwd_launch(fg_ctx* ctx, FgAttnArgs a) {
     if ((s = make_map(ctx, &k, a.k, half, a.dim, a.kv_heads, a.keys, a.k_stride, 1, kRows)) != FG_OK) return s;
     if ((s = make_map(ctx, &v, a.v, half, a.dim, a.kv_heads, a.keys, a.v_stride, 1, kRows)) != FG_OK) return s;
     const uint64_t row_tiles = a.dq ? fg_attn_tiles(a.sequences, a.queries, 1, tokens) : 0, key_tiles = a.dk ? fg_attn_tiles(a.sequences, a.keys, 1, kRows) : 0;
-    const uint64_t blocks = (row_tiles + key_tiles) * a.kv_heads;
+    const uint64_t blocks = (row_tiles + key_tiles * a.row_shares) * a.kv_heads;
     if (blocks >= 1ull << 31) return fg_fail(ctx, FG_ERR_INVALID_ARGUMENT, "attention: tensor too large");
     static std::atomic<uint64_t> done{0};
     if ((s = allow_shared(ctx, done, attn_tc_bwd_kernel<T, DP>, Cfg::kSmem)) != FG_OK) return s;
     fg_launch(ctx, attn_tc_bwd_kernel<T, DP>, (unsigned)blocks, Cfg::kThreads, Cfg::kSmem, q, d, k, v, a, tokens, (uint32_t)key_tiles, (uint32_t)row_tiles);
     FG_LAUNCHED(ctx);
-    return FG_OK;
+    return a.row_shares > 1 ? fg_attn_fold(ctx, half ? FG_DTYPE_F16 : FG_DTYPE_BF16, a) : FG_OK;
 }
 
 template <typename T, int DP, int kW>

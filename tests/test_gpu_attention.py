@@ -351,6 +351,14 @@ def test_scales(ctx, scale, dtype):
     check_backward(ctx, d)
 
 
+@pytest.mark.parametrize("dtype,dim", [("f32", 32), ("f32", 160), ("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_few_keys_many_rows(ctx, dtype, dim, causal):
+    # a head of keys for many heads of queries: the rows of a tile of keys go in shares, some of them empty
+    for lens in (SELF(700), [(500, 70), (300, 200), (0, 9), (40, 40)]):
+        check_backward(ctx, OnDevice(ctx, Case(23, dtype, dim, 16, 1, lens, causal)))
+
+
 def test_small_gradients_f16(ctx):
     # dout of 1e-4: the gradients of the scores are far below the smallest normal number of f16
     c = Case(11, "f16", 64, 2, 1, SELF(300))
