@@ -1,11 +1,12 @@
-// Attention over packed sequences with grouped heads, forward and backward: the entry points and the kernels in plain FMAs.
+// Attention over packed sequences with grouped heads, forward and backward: the entry points, and the kernels for f32 and for 16-bit tensors that the tensor
+// cores do not take as they lie.
 //
 // Forward, per head: s_ij = scale * q_i . k_j for the keys j that row i sees, o_i = sum_j p_ij v_j with p_ij = exp(s_ij - m) / l, where m is the
 // largest s_ij and l the sum of exp(s_ij - m).  One pass over the keys: when a tile of keys raises m, what was summed so far is multiplied by
 // exp(old m - new m).  Exponents are powers of two (s * log2 e).  lse_i = m + log l is what the backward pass takes.
 // Backward, with delta_i = dout_i . out_i: p_ij = exp(s_ij - lse_i); ds_ij = p_ij * (dout_i . v_j - delta_i); dq_i = scale * sum_j ds_ij k_j;
-// dk_j = scale * sum_i ds_ij q_i; dv_j = sum_i p_ij dout_i.  One kernel has a block of rows and goes over their keys for dq, another a block of
-// keys and goes over their rows, those of all heads of the group, for dk and dv: nothing is added in memory, so the order of sums is fixed.
+// dk_j = scale * sum_i ds_ij q_i; dv_j = sum_i p_ij dout_i.  A block has a tile of rows and goes over their keys for dq, or a tile of keys and goes over
+// their rows, those of all heads of the group, for dk and dv: nothing is added atomically, so the order of sums is fixed.
 #include <atomic>
 
 #include "attention_tc.cuh"
@@ -16,17 +17,16 @@ constexpr int kThreads = 256;
 constexpr uint32_t kMaxDim = 256;
 template <typename T> constexpr int32_t dtype_of = sizeof(T) == 4 ? FG_DTYPE_F32 : std::is_same_v<T, __half> ? FG_DTYPE_F16 : FG_DTYPE_BF16;
 
-// ---- plain FMAs: f32, and 16-bit tensors that the tensor cores' kernels do not take ----
-// Threads are 16 x 16: thread (y, x) has rows y * RT .. and keys x, x + 16, .. of a tile's scores, and the same rows (backward over keys: keys) by
-// columns 4 x .. + 64 j of a sum.  Rows of a tile are (query, head of the group) pairs, so the heads of a group share the keys' tile.
+// ---- plain FMAs: few rows, and head_dim over 128 forward ----
+// Threads are 16 x 16: thread (y, x) has rows y * RT .. and keys x, x + 16, .. of a tile's scores, and the same rows by columns 4 x .. + 64 j of a sum.  Rows of a tile are (query, head of the group) pairs, so the heads of a group share the keys' tile.
 // Rows in shared memory are f32, padded by four words: 16 threads that read 16 bytes each of 16 rows take two passes, the least for 256 bytes.
 // Rows [first, first + n) of a tensor's `dim` columns into shared memory, zeros behind the last row and column.
-template <typename T, int kRows, int DM, typename F>
+template <typename T, int kRows, int DM, int kWarps = kThreads / 32, typename F>
 __device__ __forceinline__ void fetch(float* to, uint32_t n, uint32_t dim, F row) {
     constexpr int kPitch = DM + 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll 8
-    for (int r = warp; r < kRows; r += kThreads / 32) {
+    for (int r = warp; r < kRows; r += kWarps) {
         const T* p = (uint32_t)r < n ? row((uint32_t)r) : nullptr;
 #pragma unroll
         for (int c = 0; c < DM; c += 32) to[r * kPitch + c + lane] = p && (uint32_t)(c + lane) < dim ? fg_widen(p[c + lane]) : 0.0f;
@@ -475,9 +475,11 @@ __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const T* out, cons
 
 constexpr size_t bwd_bytes(int dm, int n) { return sizeof(float) * (4 * (size_t)n * (dm + 4) + 2 * n * (n + 4) + 2 * n); }
 // The weights and the gradients of the scores of a tile of rows and keys, in shared memory by row.
+// A block of 64 rows and 64 keys of 128 columns has an SM to itself, and 16 warps: 4000 tokens, 8 heads over one, all pairs, 6121 us (6743 with 8).
+constexpr int bwd_warps(int dm, int n) { return dm == 128 && n == 64 ? 16 : 8; }
 template <typename T, int DM, int N_>
 struct BwdTile {
-    static constexpr int N = N_, kPitch = DM + 4, kP = N + 4;
+    static constexpr int N = N_, kWarps = bwd_warps(DM, N), kPitch = DM + 4, kP = N + 4;
     float *qs, *dos, *ks, *vs, *ps, *ds, *stat;      // stat: lse in powers of two, delta
     __device__ __forceinline__ explicit BwdTile(float* shared) {
         qs = shared;
@@ -490,20 +492,20 @@ struct BwdTile {
     }
     __device__ __forceinline__ void keys(const FgAttnArgs& a, const FgAttnSeq& s, uint32_t kv, uint32_t j0) {
         const uint32_t n = s.nk - j0;
-        fetch<T, N, DM>(ks, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.k) + (uint64_t)(s.k0 + j0 + r) * a.k_stride + (uint64_t)kv * a.dim; });
-        fetch<T, N, DM>(vs, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.v) + (uint64_t)(s.k0 + j0 + r) * a.v_stride + (uint64_t)kv * a.dim; });
+        fetch<T, N, DM, kWarps>(ks, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.k) + (uint64_t)(s.k0 + j0 + r) * a.k_stride + (uint64_t)kv * a.dim; });
+        fetch<T, N, DM, kWarps>(vs, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.v) + (uint64_t)(s.k0 + j0 + r) * a.v_stride + (uint64_t)kv * a.dim; });
     }
     __device__ __forceinline__ void rows(const FgAttnArgs& a, const FgAttnSeq& s, uint32_t kv, const RowPlace& at, uint32_t n) {
         auto place = [&](uint32_t r, uint32_t* i, uint32_t* head) {
             *i = s.q0 + at.query(r);
             *head = kv * a.group + at.head(r);
         };
-        fetch<T, N, DM>(qs, n, a.dim, [&](uint32_t r) {
+        fetch<T, N, DM, kWarps>(qs, n, a.dim, [&](uint32_t r) {
             uint32_t i, h;
             place(r, &i, &h);
             return static_cast<const T*>(a.q) + (uint64_t)i * a.q_stride + (uint64_t)h * a.dim;
         });
-        fetch<T, N, DM>(dos, n, a.dim, [&](uint32_t r) {
+        fetch<T, N, DM, kWarps>(dos, n, a.dim, [&](uint32_t r) {
             uint32_t i, h;
             place(r, &i, &h);
             return static_cast<const T*>(a.dout) + ((uint64_t)i * a.heads + h) * a.dim;
@@ -521,7 +523,7 @@ struct BwdTile {
         }
     }
     // The warps: kBlocks of 16 rows (of the sums: rows, or keys) by kSides shares of the columns.
-    static constexpr int kBlocks = N / 16, kSides = 8 / kBlocks, NT = N / 8 / kSides, NS = DM / 8 / kSides;
+    static constexpr int kBlocks = N / 16, kSides = kWarps / kBlocks, NT = N / 8 / kSides, NS = DM / 8 / kSides;
     static __device__ __forceinline__ int block() { return (threadIdx.x >> 5) / kSides * 16; }
     static __device__ __forceinline__ int side() { return (threadIdx.x >> 5) % kSides; }
     // n rows from `at` on against keys from j0 on; p is left out where it is not wanted.
@@ -635,7 +637,7 @@ __device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uin
 
 // Tiles of keys first (they have more to do), then tiles of rows, the longest of either first.
 template <typename T, int DM, int N>
-__global__ void __launch_bounds__(kThreads) attn_bwd_kernel(const FgAttnArgs a, uint32_t key_tiles, uint32_t row_tiles) {
+__global__ void __launch_bounds__(32 * bwd_warps(DM, N)) attn_bwd_kernel(const FgAttnArgs a, uint32_t key_tiles, uint32_t row_tiles) {
     extern __shared__ float shared[];
     fg_grid_enter();
     const uint32_t key_blocks = key_tiles * a.row_shares;
@@ -700,7 +702,7 @@ int32_t bwd_launch(fg_ctx* ctx, const FgAttnArgs& a) {
     if (!key_tiles && !row_tiles) return FG_OK;
     const int32_t s = allow_shared(ctx, done, attn_bwd_kernel<T, DM, N>, bwd_bytes(DM, N));
     if (s != FG_OK) return s;
-    fg_launch(ctx, attn_bwd_kernel<T, DM, N>, dim3(key_tiles * a.row_shares + row_tiles, a.kv_heads), kThreads, bwd_bytes(DM, N), a, key_tiles, row_tiles);
+    fg_launch(ctx, attn_bwd_kernel<T, DM, N>, dim3(key_tiles * a.row_shares + row_tiles, a.kv_heads), 32 * bwd_warps(DM, N), bwd_bytes(DM, N), a, key_tiles, row_tiles);
     FG_LAUNCHED(ctx);
     return a.row_shares > 1 ? fg_attn_fold(ctx, dtype_of<T>, a) : FG_OK;
 }
@@ -708,13 +710,13 @@ int32_t bwd_launch(fg_ctx* ctx, const FgAttnArgs& a) {
 bool few_tiles(const fg_ctx* ctx, const FgAttnArgs& a) { return fg_attn_tiles(a.sequences, a.queries, a.group, 64) * a.kv_heads < 2ull * ctx->sm_count; }
 
 // Few queries per sequence leave few blocks of rows, so their keys go in shares.  A block costs some 3 us beside its keys (0.4 us for 64 of 128 columns), so a
-// share has 512 keys or more, up to 4096 where there are enough for 16 blocks an SM (shares of sequences of different lengths even out then); fewer, but 128
+// share has 512 keys or more, up to 16384 where there are enough for 16 blocks an SM (shares of sequences of different lengths even out then); fewer, but 128
 // at least, only while there are not two blocks for every SM, which run at a time.  One sequence is cut for those two.  4 sequences of 5000 keys, 8 heads of 128:
-// 40 us in shares of 128, XX like this.
+// 40 us in shares of 128, 28 like this.
 int32_t in_shares(fg_ctx* ctx, FgAttnArgs& a) {
     const uint64_t all = (uint64_t)a.keys * a.kv_heads, once = all / (2ull * ctx->sm_count) + 63, usual = a.keys / a.sequences + 1;
     uint64_t chunk = all / (16ull * ctx->sm_count);
-    chunk = chunk < 512 ? 512 : chunk > 4096 ? 4096 : chunk;
+    chunk = chunk < 512 ? 512 : chunk > 16384 ? 16384 : chunk;
     if (a.sequences == 1 || chunk > once) chunk = once;
     chunk = (chunk < 128 ? 128 : chunk) / 64 * 64;
     uint64_t splits = (a.sequences == 1 ? usual : 4 * usual) / chunk + 1;

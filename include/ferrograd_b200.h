@@ -362,10 +362,12 @@ int32_t fg_sample(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, cons
  * left as they were, and so are their gradients.  A key behind its sequence's end reaches nothing, whatever its rows hold.  A NaN or an infinity in v
  * (in the backward pass: in any tensor) may reach the rows of its own sequence that do not see it.
  * q_stride, k_stride and v_stride are elements from a token to the next, 0 for dense ones: q, k and v may be columns of
- * one tensor.  head_dim is at most 256.  16-bit tensors with head_dim a multiple of 8 up to 128, on 16-byte boundaries with strides that are multiples of 8, are
- * multiplied on the tensor cores: the weights, and backward the gradients of the scores, are then rounded to the
- * storage type before they are multiplied with v, dout, k and q.  Everything else runs in f32.  Up to 16 (query, head of a group) rows per
- * sequence on average (generated tokens) the keys of a sequence are shared out over the device.  An output that overlaps an
+ * one tensor.  head_dim is at most 256.  16-bit tensors with head_dim a multiple of 8 up to 128, on 16-byte boundaries with strides that are multiples of 8,
+ * and a scale above zero, are multiplied on the tensor cores as they lie: the weights, and backward the gradients of the scores, are then rounded to the
+ * storage type before they are multiplied with v, dout, k and q.  Everything else is computed in f32 (products within 2^-20 of their size).
+ * Up to 64 (query, head of a group) rows per sequence on average (16 in f32) the calls are those of generated tokens: the keys of a sequence are
+ * shared out over the device, and a row's keys are read for every 16 to 64 rows, so a long prompt among many generated tokens is better a call of its own.
+ * An output that overlaps an
  * input is refused. */
 int32_t fg_attention_fwd(fg_ctx* ctx, int32_t dtype, uint32_t sequences, uint32_t queries, uint32_t keys,
                          uint32_t heads, uint32_t kv_heads, uint32_t head_dim, const uint32_t* q_starts,

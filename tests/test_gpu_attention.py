@@ -258,7 +258,7 @@ def test_dims(ctx, dim, dtype):
     check_backward(ctx, d)
 
 
-@pytest.mark.parametrize("heads,kv", [(1, 1), (8, 8), (8, 1), (15, 3), (7, 1), (64, 2)])
+@pytest.mark.parametrize("heads,kv", [(1, 1), (8, 8), (8, 1), (15, 3), (7, 1), (64, 2), (130, 1), (128, 1)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_heads(ctx, heads, kv, dtype):
     d = OnDevice(ctx, Case(3, dtype, 64, heads, kv, SELF(70, 140)))
