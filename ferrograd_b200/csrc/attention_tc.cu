@@ -652,7 +652,7 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 }
 
 // ---- backward ----
-// Both kernels have a row (of dq) or a key (of dk, dv) per lane, two groups of four warps with half of the columns each, warp 8 loads, warp 9
+// Both kinds of tile have a row (of dq) or a key (of dk, dv) per lane, two groups of four warps with half of the columns each, warp 8 loads, warp 9
 // multiplies.  Weights are made again from lse.  What a tile's threads leave in tensor memory as an A operand takes the place of what they
 // read: columns c / 2 behind the group's first.
 //
