@@ -426,7 +426,7 @@ int32_t logprobs_fwd(fg_ctx* ctx, const LogprobArgs& a) {
     const bool entropy = a.entropy;
     if (a.top) return entropy ? row_launch<T, true, true>(ctx, a) : row_launch<T, false, true>(ctx, a);
     if ((uint64_t)a.cols * sizeof(T) <= 8192 && a.rows > 4u * ctx->sm_count) {
-        fg_launch(ctx, entropy ? logprob_warp_kernel<T, true> : logprob_warp_kernel<T, false>, (a.rows + 7) / 8, kThreads, 0, a);
+        fg_launch(ctx, entropy ? logprob_warp_kernel<T, true> : logprob_warp_kernel<T, false>, (unsigned)(((uint64_t)a.rows + 7) / 8), kThreads, 0, a);
         FG_LAUNCHED(ctx);
         return FG_OK;
     }
