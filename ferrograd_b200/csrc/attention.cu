@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const FgAttnArgs a)
         fetch<T, kKeys, DM>(ks, there, dim, [&](uint32_t r) { return k + (uint64_t)(j0 + r) * a.k_stride; });
         fetch<T, kKeys, DM>(vs, there, dim, [&](uint32_t r) { return v + (uint64_t)(j0 + r) * a.v_stride; });
         __syncthreads();
-        float p[RT][4];
+        float p[RT][4], fade[RT];
         dots<RT, 4, DM>(qs, ks, dim, y * RT, x, p);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -254,10 +254,14 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const FgAttnArgs a)
             }
             top[i] = most;
             sum[i] = __fmaf_rn(sum[i], less, half_warp_sum(l));
-#pragma unroll
-            for (int j = 0; j < DM / 64; ++j) { acc[i][j].x *= less; acc[i][j].y *= less; acc[i][j].z *= less; acc[i][j].w *= less; }
+            fade[i] = less;
         }
         __syncwarp();
+        float4 of_tile[RT][DM / 64];      // (added key by key to the sums of a long share: 4.7e-7 off at 3400 keys instead of 2.9e-7)
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < DM / 64; ++j) of_tile[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int c = 0; c < kKeys; c += 4) {
             float4 w[RT];
 #pragma unroll
@@ -267,9 +271,17 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const FgAttnArgs a)
                 float u[RT];
 #pragma unroll
                 for (int i = 0; i < RT; ++i) u[i] = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
-                add_row<RT, DM>(vs + (c + e) * kPitch, x, u, acc);
+                add_row<RT, DM>(vs + (c + e) * kPitch, x, u, of_tile);
             }
         }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < DM / 64; ++j) {
+                const float4 t = of_tile[i][j];
+                float4& o = acc[i][j];
+                o = make_float4(__fmaf_rn(o.x, fade[i], t.x), __fmaf_rn(o.y, fade[i], t.y), __fmaf_rn(o.z, fade[i], t.z), __fmaf_rn(o.w, fade[i], t.w));
+            }
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
