@@ -17,20 +17,41 @@ constexpr int kThreads = 256;
 constexpr uint32_t kMaxDim = 256;
 template <typename T> constexpr int32_t dtype_of = sizeof(T) == 4 ? FG_DTYPE_F32 : std::is_same_v<T, __half> ? FG_DTYPE_F16 : FG_DTYPE_BF16;
 
+// Is x a number that stays one when it is rounded to 11 bits, as the products on the tensor cores below take it?
+__device__ __forceinline__ bool has_halves(float x) { return fabsf(x) < __uint_as_float(0x7f7ff000u); }
+// Was there one that is not, among those met (or a number within a thousandth of the largest)?  kByProduct: by two products, in a pipe that the gradients' kernels have room in, instead of a
+// comparison (4000 tokens of 128 columns, all pairs: 6628 us and 6885; forward 4096 tokens, 8 heads: 1345 and 1315).
+template <bool kByProduct>
+struct Odd {
+    float z = 0.0f;
+    bool any = false;
+    __device__ __forceinline__ void meet(float x) {
+        if (kByProduct) z = __fmaf_rn(x * 1.001f, 0.0f, z);
+        else any |= !has_halves(x);
+    }
+    __device__ __forceinline__ explicit operator bool() const { return kByProduct ? z != z : any; }
+};
+
 // ---- plain FMAs: few rows, and head_dim over 128 forward ----
 // Threads are 16 x 16: thread (y, x) has rows y * RT .. and keys x, x + 16, .. of a tile's scores, and the same rows by columns 4 x .. + 64 j of a sum.  Rows of a tile are (query, head of the group) pairs, so the heads of a group share the keys' tile.
 // Rows in shared memory are f32, padded by four words: 16 threads that read 16 bytes each of 16 rows take two passes, the least for 256 bytes.
-// Rows [first, first + n) of a tensor's `dim` columns into shared memory, zeros behind the last row and column.
-template <typename T, int kRows, int DM, int kWarps = kThreads / 32, typename F>
-__device__ __forceinline__ void fetch(float* to, uint32_t n, uint32_t dim, F row) {
+// Rows [first, first + n) of a tensor's `dim` columns into shared memory, zeros behind the last row and column.  Has this thread met a number that has no usual halves?
+template <typename T, int kRows, int DM, int kWarps = kThreads / 32, bool kByProduct = false, typename F>
+__device__ __forceinline__ bool fetch(float* to, uint32_t n, uint32_t dim, F row) {
     constexpr int kPitch = DM + 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Odd<kByProduct> odd;
 #pragma unroll 8
     for (int r = warp; r < kRows; r += kWarps) {
         const T* p = (uint32_t)r < n ? row((uint32_t)r) : nullptr;
 #pragma unroll
-        for (int c = 0; c < DM; c += 32) to[r * kPitch + c + lane] = p && (uint32_t)(c + lane) < dim ? fg_widen(p[c + lane]) : 0.0f;
+        for (int c = 0; c < DM; c += 32) {
+            const float x = p && (uint32_t)(c + lane) < dim ? fg_widen(p[c + lane]) : 0.0f;
+            to[r * kPitch + c + lane] = x;
+            odd.meet(x);
+        }
     }
+    return (bool)odd;
 }
 // RT x CT products of rows of two tiles: a's rows a0 + i, b's rows b0 + 16 * j.
 template <int RT, int CT, int DM>
@@ -104,38 +125,50 @@ __device__ __forceinline__ float half_warp_sum(float v) {
 // instructions of 16 x 8 x 8 products, whose sums are f32.  The instruction cuts what it adds to its sums, always towards zero, so every three start at
 // zero and are added in plain f32 (a chain of them over a tile was three times as far off: 1.0e-6 of the gradients of 501 tokens, 3.4e-7 like this, for a
 // twentieth of the gradients' time).
-struct Tf32 { uint32_t hi, lo; };
+// kAny: x may be NaN, an infinity or a number that rounds to one.  The first two are their own high half and have no other, so that they meet the other side's number once, whole
+// (half of an infinity times a low half of the other sign would be no number, nor would it be times a half that is zero); the last is cut.  NaN is written anew:
+// added to, its bits could become those of a zero.  Tiles that hold such a number are known when they are fetched, and only those are multiplied in this way.
+struct Tf32 { uint32_t hi, lo, cross; };      // cross: what meets the other side's low half
+template <bool kAny>
 __device__ __forceinline__ Tf32 tf32_halves(float x) {
-    const uint32_t hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-    return Tf32{hi, __float_as_uint(x - __uint_as_float(hi)) + 0x1000u};
+    const uint32_t bits = __float_as_uint(x);
+    if (kAny && !has_halves(x)) {
+        const bool number = fabsf(x) < INFINITY;
+        const uint32_t hi = number ? bits & 0xffffe000u : x != x ? 0x7fffe000u : bits;
+        return Tf32{hi, number ? __float_as_uint(x - __uint_as_float(hi)) : 0u, number ? hi : 0u};
+    }
+    const uint32_t hi = (bits + 0x1000u) & 0xffffe000u;
+    return Tf32{hi, __float_as_uint(x - __uint_as_float(hi)) + 0x1000u, hi};
 }
 __device__ __forceinline__ void mma_16x8x8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+template <bool kAny>
 struct Left {      // a 16 x 8 block in halves: lane l has rows l / 4 and 8 more, columns l % 4 and 4 more
-    uint32_t hi[4], lo[4];
+    uint32_t hi[4], lo[4], cross[4];
     __device__ __forceinline__ Left(float a0, float a1, float a2, float a3) {
         const float x[4] = {a0, a1, a2, a3};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const Tf32 t = tf32_halves(x[i]);
+            const Tf32 t = tf32_halves<kAny>(x[i]);
             hi[i] = t.hi;
             lo[i] = t.lo;
+            cross[i] = t.cross;
         }
     }
     __device__ __forceinline__ void times(float b0, float b1, float (&d)[4]) const {
-        const Tf32 x = tf32_halves(b0), y = tf32_halves(b1);
+        const Tf32 x = tf32_halves<kAny>(b0), y = tf32_halves<kAny>(b1);
         float f[4] = {};
-        mma_16x8x8(f, lo, x.hi, y.hi);
-        mma_16x8x8(f, hi, x.lo, y.lo);
+        mma_16x8x8(f, lo, x.cross, y.cross);
+        mma_16x8x8(f, cross, x.lo, y.lo);
         mma_16x8x8(f, hi, x.hi, y.hi);
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[e] += f[e];
     }
 };
 // 16 rows of a by 8 * NT rows of b, over dim columns (zeros behind): lane l has rows l / 4, + 8 and columns 8 t + 2 (l % 4), + 1.
-template <int NT, int DM>
+template <bool kAny, int NT, int DM>
 __device__ __forceinline__ void row_products(const float* a, const float* b, uint32_t dim, float (&s)[NT][4]) {
     constexpr int kPitch = DM + 4;
     const int g = (threadIdx.x & 31) >> 2, q = threadIdx.x & 3;
@@ -146,7 +179,7 @@ __device__ __forceinline__ void row_products(const float* a, const float* b, uin
 #pragma unroll 2
     for (uint32_t d = q; d < dim + q; d += 8) {
         const float* const x = a + g * kPitch + d;
-        const Left left(x[0], x[8 * kPitch], x[4], x[8 * kPitch + 4]);
+        const Left<kAny> left(x[0], x[8 * kPitch], x[4], x[8 * kPitch + 4]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const float* const y = b + (8 * t + g) * kPitch + d;
@@ -155,7 +188,7 @@ __device__ __forceinline__ void row_products(const float* a, const float* b, uin
     }
 }
 // acc += (16 x 8 * steps block given by `left`) times rows of b: 8 * NT columns of it from b on.
-template <int NT, int DM, typename F>
+template <bool kAny, int NT, int DM, typename F>
 __device__ __forceinline__ void add_products(F left, const float* b, int steps, float (&acc)[NT][4]) {
     constexpr int kPitch = DM + 4, kOnce = NT < 4 ? NT : 4;
     const int g = (threadIdx.x & 31) >> 2, q = threadIdx.x & 3;
@@ -163,7 +196,7 @@ __device__ __forceinline__ void add_products(F left, const float* b, int steps, 
     for (int t0 = 0; t0 < NT; t0 += kOnce)
 #pragma unroll 2
         for (int k = 0; k < steps; ++k) {
-            const Left x = left(k);
+            const Left<kAny> x = left(k);
             const float* const y = b + (8 * k + q) * kPitch + 8 * t0 + g;
 #pragma unroll
             for (int t = 0; t < kOnce; ++t) x.times(y[8 * t], y[4 * kPitch + 8 * t], acc[t0 + t]);
@@ -302,6 +335,38 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const FgAttnArgs a)
 
 // Many rows: a warp has 16 of a block's 128, and all keys of a tile.  The weights of a tile stay in registers as the left side of the product with v: the lane that has the
 // scores of keys 2 (l % 4) and + 1 takes them for columns l % 4 and + 4, with v's rows in that order.
+template <bool kAny, int NT, int NS, int DM>
+__device__ __forceinline__ void add_weighted(const float (&p)[NT][4], const float* vs, float (&acc)[NS][4]) {
+    constexpr int kPitch = DM + 4;
+    const int g = (threadIdx.x & 31) >> 2, q = threadIdx.x & 3;
+    // (sums of a tile's own: added straight to the rows' sums, 4096 tokens took 1838 us instead of 1686)
+#pragma unroll
+    for (int t0 = 0; t0 < NS; t0 += 4) {
+        float f[4][4] = {};
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+            const Left<kAny> x(p[k][0], p[k][2], p[k][1], p[k][3]);
+            const float* const y = vs + (8 * k + 2 * q) * kPitch + 8 * t0 + g;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) x.times(y[8 * t], y[kPitch + 8 * t], f[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[t0 + t][e] += f[t][e];
+    }
+}
+// The products of tiles with odd numbers are functions of their own: inlined beside the usual ones, they took 4096 tokens of 128 columns from 1315 to 1407 us.  (What a function gets the
+// address of does not stay in registers, so it is a copy.)
+template <int N, int M>
+__device__ __forceinline__ void copy(float (&to)[N][M], const float (&from)[N][M]) {
+#pragma unroll
+    for (int i = 0; i < N * M; ++i) to[i / M][i % M] = from[i / M][i % M];
+}
+template <int NT, int DM>
+__noinline__ __device__ void odd_row_products(const float* a, const float* b, uint32_t dim, float (&s)[NT][4]) { row_products<true, NT, DM>(a, b, dim, s); }
+template <int NT, int NS, int DM>
+__noinline__ __device__ void odd_add_weighted(const float (&p)[NT][4], const float* vs, float (&acc)[NS][4]) { add_weighted<true, NT, NS, DM>(p, vs, acc); }
 constexpr size_t many_bytes(int dm) { return sizeof(float) * (size_t)(128 + 2 * kKeys) * (dm + 4); }
 template <typename T, int DM>
 __global__ void __launch_bounds__(kThreads) attn_many_kernel(const FgAttnArgs a) {
@@ -320,7 +385,7 @@ __global__ void __launch_bounds__(kThreads) attn_many_kernel(const FgAttnArgs a)
     const T *const qp = static_cast<const T*>(a.q), *const kp = static_cast<const T*>(a.k) + (uint64_t)s.k0 * a.k_stride + (uint64_t)kv * dim,
                   *const vp = static_cast<const T*>(a.v) + (uint64_t)s.k0 * a.v_stride + (uint64_t)kv * dim;
     const RowPlace place(first, a.group);
-    fetch<T, R, DM>(qs, n, dim, [&](uint32_t r) { return qp + (uint64_t)(s.q0 + place.query(r)) * a.q_stride + (uint64_t)(kv * a.group + place.head(r)) * dim; });
+    const bool odd_rows = fetch<T, R, DM>(qs, n, dim, [&](uint32_t r) { return qp + (uint64_t)(s.q0 + place.query(r)) * a.q_stride + (uint64_t)(kv * a.group + place.head(r)) * dim; });
     uint32_t seen[2];
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, acc[NS][4] = {};
 #pragma unroll
@@ -330,29 +395,15 @@ __global__ void __launch_bounds__(kThreads) attn_many_kernel(const FgAttnArgs a)
     for (uint32_t j0 = 0; j0 < hi; j0 += kKeys) {
         const uint32_t there = min((uint32_t)kKeys, s.nk - j0);
         __syncthreads();
-        fetch<T, kKeys, DM>(ks, there, dim, [&](uint32_t r) { return kp + (uint64_t)(j0 + r) * a.k_stride; });
-        fetch<T, kKeys, DM>(vs, there, dim, [&](uint32_t r) { return vp + (uint64_t)(j0 + r) * a.v_stride; });
-        __syncthreads();
+        const bool odd_keys = fetch<T, kKeys, DM>(ks, there, dim, [&](uint32_t r) { return kp + (uint64_t)(j0 + r) * a.k_stride; });
+        const bool odd_values = fetch<T, kKeys, DM>(vs, there, dim, [&](uint32_t r) { return vp + (uint64_t)(j0 + r) * a.v_stride; });
+        const bool odd = __syncthreads_or(odd_rows | odd_keys | odd_values);
         float p[NT][4];
-        row_products<NT, DM>(qs + block * kPitch, ks, dim, p);
-        // An infinity times half of a number is no number where the half is zero: such scores are made again in one product.
-        bool odd = false;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= p[t][e] != p[t][e];
-        if (__any_sync(0xffffffffu, odd))
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (p[t][e] != p[t][e]) {
-                        const float *const x = qs + (block + g + 4 * (e & 2)) * kPitch, *const y = ks + (8 * t + 2 * q + (e & 1)) * kPitch;
-                        float v = 0.0f;
-#pragma unroll 1
-                        for (uint32_t d = 0; d < dim; ++d) v = __fmaf_rn(x[d], y[d], v);
-                        p[t][e] = v;
-                    }
+        if (odd) {
+            float x[NT][4];
+            odd_row_products<NT, DM>(qs + block * kPitch, ks, dim, x);
+            copy(p, x);
+        } else row_products<false, NT, DM>(qs + block * kPitch, ks, dim, p);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float most = -INFINITY;
@@ -378,22 +429,14 @@ __global__ void __launch_bounds__(kThreads) attn_many_kernel(const FgAttnArgs a)
 #pragma unroll
             for (int t = 0; t < NS; ++t) { acc[t][2 * h] *= less; acc[t][2 * h + 1] *= less; }
         }
-        // (sums of a tile's own: added straight to the rows' sums, 4096 tokens took 1838 us instead of 1686)
-#pragma unroll
-        for (int t0 = 0; t0 < NS; t0 += 4) {
-            float f[4][4] = {};
-#pragma unroll
-            for (int k = 0; k < NT; ++k) {
-                const Left x(p[k][0], p[k][2], p[k][1], p[k][3]);
-                const float* const y = vs + (8 * k + 2 * q) * kPitch + 8 * t0 + g;
-#pragma unroll
-                for (int t = 0; t < 4; ++t) x.times(y[8 * t], y[kPitch + 8 * t], f[t]);
-            }
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[t0 + t][e] += f[t][e];
-        }
+        // (A weight that is no number makes its row's sum none, and that the row, whatever its products are.)
+        if (odd) {
+            float w[NT][4], o[NS][4];
+            copy(w, p);
+            copy(o, acc);
+            odd_add_weighted<NT, NS, DM>(w, vs, o);
+            copy(acc, o);
+        } else add_weighted<false, NT, NS, DM>(p, vs, acc);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -486,8 +529,10 @@ __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const T* out, cons
 
 constexpr size_t bwd_bytes(int dm, int n) { return sizeof(float) * (4 * (size_t)n * (dm + 4) + 2 * n * (n + 4) + 2 * n); }
 // The weights and the gradients of the scores of a tile of rows and keys, in shared memory by row.
-// A block of 64 rows and 64 keys of 128 columns has an SM to itself, and 16 warps: 4000 tokens, 8 heads over one, all pairs, 6441 us (a tenth more with 8).
+// A block of 64 rows and 64 keys of 128 columns has an SM to itself, and 16 warps: 4000 tokens, 8 heads over one, all pairs, 6578 us (a tenth more with 8).
 constexpr int bwd_warps(int dm, int n) { return dm == 128 && n == 64 ? 16 : 8; }
+// Blocks that an SM has registers for.  (32 rows of 64 columns: four, with some registers spilled, take 501 tokens 53.5 us instead of 50.4, and 1900 tokens 460 instead of 474.)
+constexpr int bwd_blocks(int dm, int n) { return dm == 64 && n == 32 ? 3 : dm == 64 || n == 32 ? 2 : 1; }
 template <typename T, int DM, int N_>
 struct BwdTile {
     static constexpr int N = N_, kWarps = bwd_warps(DM, N), kPitch = DM + 4, kP = N + 4;
@@ -501,22 +546,23 @@ struct BwdTile {
         ds = ps + N * kP;
         stat = ds + N * kP;
     }
-    __device__ __forceinline__ void keys(const FgAttnArgs& a, const FgAttnSeq& s, uint32_t kv, uint32_t j0) {
+    // Both, like fetch(), say whether this thread has met a number that has no usual halves.
+    __device__ __forceinline__ bool keys(const FgAttnArgs& a, const FgAttnSeq& s, uint32_t kv, uint32_t j0) {
         const uint32_t n = s.nk - j0;
-        fetch<T, N, DM, kWarps>(ks, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.k) + (uint64_t)(s.k0 + j0 + r) * a.k_stride + (uint64_t)kv * a.dim; });
-        fetch<T, N, DM, kWarps>(vs, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.v) + (uint64_t)(s.k0 + j0 + r) * a.v_stride + (uint64_t)kv * a.dim; });
+        const bool odd = fetch<T, N, DM, kWarps, true>(ks, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.k) + (uint64_t)(s.k0 + j0 + r) * a.k_stride + (uint64_t)kv * a.dim; });
+        return odd | fetch<T, N, DM, kWarps, true>(vs, n, a.dim, [&](uint32_t r) { return static_cast<const T*>(a.v) + (uint64_t)(s.k0 + j0 + r) * a.v_stride + (uint64_t)kv * a.dim; });
     }
-    __device__ __forceinline__ void rows(const FgAttnArgs& a, const FgAttnSeq& s, uint32_t kv, const RowPlace& at, uint32_t n) {
+    __device__ __forceinline__ bool rows(const FgAttnArgs& a, const FgAttnSeq& s, uint32_t kv, const RowPlace& at, uint32_t n) {
         auto place = [&](uint32_t r, uint32_t* i, uint32_t* head) {
             *i = s.q0 + at.query(r);
             *head = kv * a.group + at.head(r);
         };
-        fetch<T, N, DM, kWarps>(qs, n, a.dim, [&](uint32_t r) {
+        bool odd = fetch<T, N, DM, kWarps, true>(qs, n, a.dim, [&](uint32_t r) {
             uint32_t i, h;
             place(r, &i, &h);
             return static_cast<const T*>(a.q) + (uint64_t)i * a.q_stride + (uint64_t)h * a.dim;
         });
-        fetch<T, N, DM, kWarps>(dos, n, a.dim, [&](uint32_t r) {
+        odd |= fetch<T, N, DM, kWarps, true>(dos, n, a.dim, [&](uint32_t r) {
             uint32_t i, h;
             place(r, &i, &h);
             return static_cast<const T*>(a.dout) + ((uint64_t)i * a.heads + h) * a.dim;
@@ -532,18 +578,20 @@ struct BwdTile {
             stat[threadIdx.x] = lse == -INFINITY ? INFINITY : lse * kFgLog2e;      // a row that saw nothing weighs nothing
             stat[N + threadIdx.x] = delta;
         }
+        return odd;
     }
     // The warps: kBlocks of 16 rows (of the sums: rows, or keys) by kSides shares of the columns.
     static constexpr int kBlocks = N / 16, kSides = kWarps / kBlocks, NT = N / 8 / kSides, NS = DM / 8 / kSides;
     static __device__ __forceinline__ int block() { return (threadIdx.x >> 5) / kSides * 16; }
     static __device__ __forceinline__ int side() { return (threadIdx.x >> 5) % kSides; }
-    // n rows from `at` on against keys from j0 on; p is left out where it is not wanted.
-    template <bool kP_>
-    __device__ __forceinline__ void weights(const FgAttnArgs& a, const FgAttnSeq& s, const RowPlace& at, uint32_t n, uint32_t j0) {
+    // n rows from `at` on against keys from j0 on; p is left out where it is not wanted.  Has this thread left a number that has no usual halves?
+    template <bool kP_, bool kAny>
+    __device__ __forceinline__ bool weights(const FgAttnArgs& a, const FgAttnSeq& s, const RowPlace& at, uint32_t n, uint32_t j0) {
         const int g = (threadIdx.x & 31) >> 2, q = threadIdx.x & 3, c0 = side() * NT * 8;
         float p[NT][4], dp[NT][4];
-        row_products<NT, DM>(qs + block() * kPitch, ks + c0 * kPitch, a.dim, p);
-        row_products<NT, DM>(dos + block() * kPitch, vs + c0 * kPitch, a.dim, dp);
+        row_products<kAny, NT, DM>(qs + block() * kPitch, ks + c0 * kPitch, a.dim, p);
+        row_products<kAny, NT, DM>(dos + block() * kPitch, vs + c0 * kPitch, a.dim, dp);
+        Odd<true> odd;
         const float by = a.scale * kFgLog2e;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -556,21 +604,26 @@ struct BwdTile {
                 for (int e = 0; e < 2; ++e) {
                     w[e] = j0 + c0 + 8 * t + 2 * q + e < seen ? fg_ex2_fast(__fmaf_rn(p[t][2 * h + e], by, -lse)) : 0.0f;
                     d[e] = w[e] == 0.0f ? 0.0f : w[e] * (dp[t][2 * h + e] - delta);
+                    odd.meet(w[e]);
+                    odd.meet(d[e]);
                 }
                 const uint32_t to = r * kP + c0 + 8 * t + 2 * q;
                 if (kP_) *reinterpret_cast<float2*>(ps + to) = make_float2(w[0], w[1]);
                 *reinterpret_cast<float2*>(ds + to) = make_float2(d[0], d[1]);
             }
         }
+        return (bool)odd;
     }
     // acc += w (this warp's 16 rows of ds, or columns of ps or ds) times rows of `tile`.
+    template <bool kAny>
     __device__ __forceinline__ void add_rows(const float* w, const float* tile, float (&acc)[NS][4]) const {
         const float* const x = w + (block() + ((threadIdx.x & 31) >> 2)) * kP + (threadIdx.x & 3);
-        add_products<NS, DM>([&](int k) { return Left(x[8 * k], x[8 * kP + 8 * k], x[8 * k + 4], x[8 * kP + 8 * k + 4]); }, tile + side() * NS * 8, N / 8, acc);
+        add_products<kAny, NS, DM>([&](int k) { return Left<kAny>(x[8 * k], x[8 * kP + 8 * k], x[8 * k + 4], x[8 * kP + 8 * k + 4]); }, tile + side() * NS * 8, N / 8, acc);
     }
+    template <bool kAny>
     __device__ __forceinline__ void add_columns(const float* w, const float* tile, float (&acc)[NS][4]) const {
         const float* const x = w + (threadIdx.x & 3) * kP + block() + ((threadIdx.x & 31) >> 2);
-        add_products<NS, DM>([&](int k) { return Left(x[8 * k * kP], x[8 * k * kP + 8], x[(8 * k + 4) * kP], x[(8 * k + 4) * kP + 8]); }, tile + side() * NS * 8, N / 8, acc);
+        add_products<kAny, NS, DM>([&](int k) { return Left<kAny>(x[8 * k * kP], x[8 * k * kP + 8], x[(8 * k + 4) * kP], x[(8 * k + 4) * kP + 8]); }, tile + side() * NS * 8, N / 8, acc);
     }
 };
 
@@ -586,16 +639,17 @@ __device__ __forceinline__ void dq_tile(const FgAttnArgs& a, float* shared, uint
     if (first >= rows) return;
     const uint32_t n = rows - first < N ? (uint32_t)(rows - first) : N, kv = blockIdx.y;
     const RowPlace place(first, a.group);
-    t.rows(a, s, kv, place, n);
+    const bool odd_rows = t.rows(a, s, kv, place, n);
     float acc[B::NS][4] = {};
     const uint32_t hi = s.seen(a, place.query(n - 1));
     for (uint32_t j0 = 0; j0 < hi; j0 += N) {
         __syncthreads();
-        t.keys(a, s, kv, j0);
-        __syncthreads();
-        t.template weights<false>(a, s, place, n, j0);
-        __syncthreads();
-        t.add_rows(t.ds, t.ks, acc);
+        const bool odd_keys = t.keys(a, s, kv, j0);
+        bool odd = __syncthreads_or(odd_rows | odd_keys);
+        odd |= odd ? t.template weights<false, true>(a, s, place, n, j0) : t.template weights<false, false>(a, s, place, n, j0);
+        odd = __syncthreads_or(odd);
+        if (odd) t.template add_rows<true>(t.ds, t.ks, acc);
+        else t.template add_rows<false>(t.ds, t.ks, acc);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -617,7 +671,7 @@ __device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uin
     const uint64_t j0_ = (uint64_t)tile * N;
     if (j0_ >= s.nk) return;
     const uint32_t j0 = (uint32_t)j0_, kv = blockIdx.y;
-    t.keys(a, s, kv, j0);
+    const bool odd_keys = t.keys(a, s, kv, j0);
     float dk[B::NS][4] = {}, dv[B::NS][4] = {};
     const uint64_t start = (uint64_t)s.first_query(a, j0) * a.group, all = (uint64_t)s.nq * a.group;
     const uint64_t each = ((all - start + N - 1) / N + a.row_shares - 1) / a.row_shares * N, rows = min(all, start + (share + 1) * each);
@@ -625,12 +679,17 @@ __device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uin
         const uint32_t n = rows - first < N ? (uint32_t)(rows - first) : N;
         const RowPlace place(first, a.group);
         __syncthreads();
-        t.rows(a, s, kv, place, n);
-        __syncthreads();
-        t.template weights<true>(a, s, place, n, j0);
-        __syncthreads();
-        t.add_columns(t.ps, t.dos, dv);
-        t.add_columns(t.ds, t.qs, dk);
+        const bool odd_rows = t.rows(a, s, kv, place, n);
+        bool odd = __syncthreads_or(odd_rows | odd_keys);
+        odd |= odd ? t.template weights<true, true>(a, s, place, n, j0) : t.template weights<true, false>(a, s, place, n, j0);
+        odd = __syncthreads_or(odd);
+        if (odd) {
+            t.template add_columns<true>(t.ps, t.dos, dv);
+            t.template add_columns<true>(t.ds, t.qs, dk);
+        } else {
+            t.template add_columns<false>(t.ps, t.dos, dv);
+            t.template add_columns<false>(t.ds, t.qs, dk);
+        }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -648,7 +707,7 @@ __device__ __forceinline__ void dkv_tile(const FgAttnArgs& a, float* shared, uin
 
 // Tiles of keys first (they have more to do), then tiles of rows, the longest of either first.
 template <typename T, int DM, int N>
-__global__ void __launch_bounds__(32 * bwd_warps(DM, N)) attn_bwd_kernel(const FgAttnArgs a, uint32_t key_tiles, uint32_t row_tiles) {
+__global__ void __launch_bounds__(32 * bwd_warps(DM, N), bwd_blocks(DM, N)) attn_bwd_kernel(const FgAttnArgs a, uint32_t key_tiles, uint32_t row_tiles) {
     extern __shared__ float shared[];
     fg_grid_enter();
     const uint32_t key_blocks = key_tiles * a.row_shares;
