@@ -611,7 +611,7 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             float all = -INFINITY;
 #pragma unroll
             for (int w = 0; w < 4 / kW; ++w) all = fmaxf(all, stat[w * kW + warp % kW][lane / 4 + 8 * e].x);
-            const float f = top[e] == -INFINITY ? 0.0f : fg_ex2_fast(top[e] - all);
+            const float f = fg_ex2_fast(top[e] - (all == -INFINITY ? 0.0f : all));
 #pragma unroll
             for (int c = 0; c < DP / 8; ++c)
                 *reinterpret_cast<float2*>(sums + (warp * 16 + lane / 4 + 8 * e) * kPitch + 8 * c + 2 * (lane % 4)) = make_float2(o[c][2 * e] * f, o[c][2 * e + 1] * f);
@@ -622,10 +622,12 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             float all = -INFINITY, total = 0.0f;
 #pragma unroll
             for (int w = 0; w < 4 / kW; ++w) all = fmaxf(all, stat[w * kW + w0][in].x);
+            // (A part without a largest score has a sum of zero, or none where its scores are no numbers, which the row's then is not either.)
+            const float base_all = all == -INFINITY ? 0.0f : all;
 #pragma unroll
             for (int w = 0; w < 4 / kW; ++w) {
                 const float2 st = stat[w * kW + w0][in];
-                if (st.x != -INFINITY) total = __fmaf_rn(fg_ex2_fast(st.x - all), st.y, total);
+                total = __fmaf_rn(fg_ex2_fast(st.x - base_all), st.y, total);
             }
             const uint32_t row = s.q0 + (uint32_t)((r0 + r) / a.group), head = kv * a.group + (uint32_t)((r0 + r) % a.group);
             const uint64_t line = (uint64_t)row * a.heads + head;

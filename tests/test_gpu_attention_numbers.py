@@ -206,3 +206,54 @@ def test_infinite_scores(ctx, size, dim):
     rest.seqs = [(5, nq - 5, 5, nk - 5), other]
     out, _, bound, _ = rest.forward()
     assert (np.abs(got[5:] - out[5:]) <= bound[5:]).all()
+
+
+CACHES = [("f32", 64, 4, 2), ("f32", 200, 2, 1), ("bf16", 128, 8, 2), ("f16", 64, 4, 4), ("f16", 128, 20, 1), ("bf16", 64, 40, 1), ("bf16", 36, 4, 2)]
+
+
+@pytest.mark.parametrize("dtype,dim,heads,kv", CACHES)
+@pytest.mark.parametrize("lens", [[(1, 1), (1, 1), (1, 1)], [(1, 40), (1, 100), (1, 30)], [(1, 30), (1, 5000), (1, 4000)], [(2, 70), (3, 9000)]],
+                         ids=["one key", "one share", "shares", "more tokens"])
+def test_generated_tokens(ctx, dtype, dim, heads, kv, lens):
+    # a query that is no number, and a key: the rows that see it are none, and their lse is none; the others are what they are without it
+    c = Case(41, dtype, dim, heads, kv, lens)
+    d = OnDevice(ctx, c)
+    d.forward()
+    check_forward(d)
+    out, lse, e_out, e_lse = c.forward()
+    q0, nq, k0, nk = c.seqs[1]
+    h, group = heads // 2, heads // kv
+    w = h // group
+    for word in NAN[dtype]:
+        for which, at in (("q", (q0 + nq - 1, h, 3)), ("k", (k0 + nk // 2, w, 3)), ("k", (k0 + nk - 1, w, 3))):
+            x = WithBits(ctx, getattr(c, which), dtype, at, word)
+            e = OnDevice(ctx, c)
+            setattr(e, which, x.ptr)
+            e.forward()
+            got, got_lse = e.out.get(), e.lse.get()
+            bad = np.zeros((c.n, heads), bool)
+            if which == "q":
+                bad[q0 + nq - 1, h] = True
+            else:
+                first = at[0] - k0 - (nk - nq)          # the first query that sees the key
+                bad[q0 + max(first, 0):q0 + nq, w * group:(w + 1) * group] = True
+            assert np.isnan(got[bad]).all() and np.isnan(got_lse.T[bad]).all(), (which, hex(word))
+            assert (np.abs(got[~bad] - out[~bad]) <= e_out[~bad]).all() and (np.abs(got_lse.T[~bad] - lse.T[~bad]) <= e_lse.T[~bad]).all(), (which, hex(word))
+
+
+@pytest.mark.parametrize("dtype,dim,heads,kv", CACHES)
+def test_generated_tokens_infinite_scores(ctx, dtype, dim, heads, kv):
+    # all scores of a row -inf: zeros and -inf, in one share and in several; a score of +inf has no weights
+    for n in (1, 50, 5000):
+        c = Case(42, dtype, dim, heads, kv, [(1, n), (1, n)])
+        c.q[:, :, 0] = np.abs(c.q[:, :, 0]) + 1
+        c.k[n:, :, 0] = -np.inf
+        d = OnDevice(ctx, c)
+        d.forward()
+        out, lse = d.out.get(), d.lse.get()
+        assert (out[1] == 0).all() and np.isneginf(lse[:, 1]).all() and np.isfinite(out[0]).all() and np.isfinite(lse[:, 0]).all()
+        c.k[n:, :, 0] = np.inf
+        d = OnDevice(ctx, c)
+        d.forward()
+        out, lse = d.out.get(), d.lse.get()
+        assert np.isnan(out[1]).all() and np.isnan(lse[:, 1]).all() and np.isfinite(out[0]).all() and np.isfinite(lse[:, 0]).all()
