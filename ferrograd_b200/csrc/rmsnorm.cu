@@ -393,8 +393,8 @@ __global__ void __launch_bounds__(256) rms_stream_kernel(const RmsArgs a) {
     __shared__ float red[64];
     fg_grid_enter();
     const T* const gamma = static_cast<const T*>(a.gamma);
-    for (uint32_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const uint64_t at = (uint64_t)r * a.cols;
+    for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const uint64_t at = r * a.cols;
         const T *const x = static_cast<const T*>(a.x) + at, *const res = a.residual ? static_cast<const T*>(a.residual) + at : nullptr;
         T* const sum = a.sum ? static_cast<T*>(a.sum) + at : nullptr;
         auto h_at = [&](uint64_t c) { return res ? fg_widen(fg_narrow<T>(fg_widen(x[c]) + fg_widen(res[c]))) : fg_widen(x[c]); };
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(256) rms_stream_kernel(const RmsArgs a) {
                         if (sum) sum[c] = fg_narrow<T>(h);
                         y[c] = to_e4m3(y_of(h, c), scale);
                     }
-                    if (lane == 0) a.scale[(uint64_t)r * a.groups + g] = scale;
+                    if (lane == 0) a.scale[r * a.groups + g] = scale;
                 }
             } else {
                 float most = 0.0f;
@@ -458,8 +458,8 @@ __global__ void __launch_bounds__(256) rms_bwd_stream_kernel(const RmsBwdArgs a)
     __shared__ float red[64];
     fg_grid_enter();
     const T* const gamma = static_cast<const T*>(a.gamma);
-    for (uint32_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const uint64_t at = (uint64_t)r * a.cols;
+    for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const uint64_t at = r * a.cols;
         const T *const x = static_cast<const T*>(a.x) + at, *const dy = static_cast<const T*>(a.dy) + at, *const dsum = a.dsum ? static_cast<const T*>(a.dsum) + at : nullptr;
         T* const dx = static_cast<T*>(a.dx) + at;
         const float rstd = a.rstd[r];
@@ -591,7 +591,7 @@ int32_t rms_fwd(fg_ctx* ctx, const RmsArgs& a) {
     else s = res ? fwd_ragged<T, true>(ctx, a, &took) : fwd_ragged<T, false>(ctx, a, &took);
     if (took) return s;
     // A row by one warp or eight, 4 to 32 elements a lane (64 spill: 4504 x 9394 f16 984 us, 172 read once per sum).
-    if (a.scale && a.rows < 1u << 31) {
+    if (a.scale) {
         if (a.cols <= 128 && a.group != 256) return ragged_e4m3<T, 1, 1>(ctx, a);
         if (a.cols <= 1024) return ragged_e4m3<T, 1, 8>(ctx, a);
         if (a.cols <= 4096) return ragged_e4m3<T, 8, 4>(ctx, a);
