@@ -26,11 +26,19 @@ struct RmsBwdArgs {
 };
 constexpr float kE4m3Max = 448.0f;
 
-// y / s in e4m3.  1 / s has to be finite and normal, or y is divided; a group of zeros stays one.
-__device__ __forceinline__ bool has_inverse(float s) { return s > 1e-37f && s < 1e37f; }
+// y / s in e4m3, rounded from the f32 quotient; a group of zeros stays one.  The quotient is the product with 1 / s and a step that adds what is left of y times 1 / s (P. Markstein,
+// Computation of elementary functions on the IBM RISC System/6000 processor, 1990): exact enough that no byte differs, where a quotient beside a border between bytes took the product alone over
+// it.  s has to leave the remainder its bits, or y is divided, which for all of them took 16384 x 4096 bf16 from 97 us to 143.
+__device__ __forceinline__ bool has_inverse(float s) { return s > 1e-25f && s < 1e37f; }
 __device__ __forceinline__ float divided(float y, float s) { return s > 0.0f ? y / s : y * 0.0f; }
 __device__ __forceinline__ uint8_t to_e4m3(float y, float s) {
-    return (uint8_t)__nv_cvt_float_to_fp8(has_inverse(s) ? y * (1.0f / s) : divided(y, s), __NV_SATFINITE, __NV_E4M3);
+    float q;
+    if (has_inverse(s)) {
+        const float by = 1.0f / s;
+        q = y * by;
+        q = __fmaf_rn(__fmaf_rn(-s, q, y), by, q);
+    } else q = divided(y, s);
+    return (uint8_t)__nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
 }
 // 2 * P of them, four in a word.
 template <int P>
@@ -38,7 +46,13 @@ __device__ __forceinline__ void put_e4m3(float (&y)[2 * P], float s, uint32_t (&
     if (has_inverse(s)) {
         const float by = 1.0f / s;
 #pragma unroll
-        for (int e = 0; e < 2 * P; ++e) y[e] *= by;
+        for (int e = 0; e < 2 * P; e += 2) {
+            const float2 x = make_float2(y[e], y[e + 1]), by2 = make_float2(by, by);
+            float2 q = fg_mul2(x, by2);
+            q = fg_fma2(fg_fma2(q, make_float2(-s, -s), x), by2, q);
+            y[e] = q.x;
+            y[e + 1] = q.y;
+        }
     } else
 #pragma unroll
         for (int e = 0; e < 2 * P; ++e) y[e] = divided(y[e], s);

@@ -390,8 +390,8 @@ int32_t fg_attention_bwd(fg_ctx* ctx, int32_t dtype, uint32_t sequences, uint32_
 int32_t fg_rmsnorm_fwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* x, const void* residual,
                        const void* gamma, float eps, void* sum_out, void* y, float* rstd_out);
 /* The same with y in 8 bits (e4m3: 4 bits of exponent, 3 of fraction, largest number 448): for each group of `group` columns (32, 64, 128 or
- * 256; the last group of a row may be shorter; 0: the whole row) scale_out[row, group] = (largest |y| of the group) / 448, and the bytes are y / scale,
- * rounded to nearest even.  scale_out is f32 [rows, groups of a row].  A group of zeros has scale 0 and bytes 0. */
+ * 256; the last group of a row may be shorter; 0: the whole row) scale_out[row, group] = (largest |y| of the group) / 448, and the bytes are the f32 quotients
+ * y / scale, rounded to nearest even.  scale_out is f32 [rows, groups of a row].  A group of zeros has scale 0 and bytes 0. */
 int32_t fg_rmsnorm_fwd_e4m3(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, const void* x,
                             const void* residual, const void* gamma, float eps, uint32_t group, void* sum_out,
                             uint8_t* y, float* scale_out, float* rstd_out);
