@@ -77,3 +77,22 @@ def test_borders_between_bytes(ctx, cols, group):
         want = from_quotients(y / np.repeat(scale, each, 1)[:, :cols])
         assert np.array_equal(bytes_ & 0x7f, want & 0x7f), f"{(bytes_ != want).sum()} of {want.size} bytes"
         assert np.array_equal(bytes_[want != 0x80], want[want != 0x80])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cols", [4096, 64, 1001, 3999, 20000])
+def test_zeros_of_both_signs(ctx, dtype, cols):
+    # groups of zeros have bytes of 0, whatever the zeros' signs and those of gamma are; a NaN stays one
+    x = np.zeros((4, cols), np.float32)
+    x[1] = -0.0
+    x[2, ::2] = -0.0
+    x[3] = np.nan
+    gamma = np.where(np.arange(cols) % 3 == 0, -1.0, 1.0)
+    for group in (0, 64):
+        groups = -(-cols // group) if group else 1
+        for g in (None, Placed(ctx, gamma, dtype)):
+            q, scale = Bytes(ctx, 4 * cols, 0), empty(ctx, (4, groups))
+            ctx.rmsnorm_fwd_e4m3(Placed(ctx, x, dtype), g, q, scale, 4, cols, group=group, dtype=dtype)
+            b = q.get().reshape(4, cols)
+            assert (b[:3] == 0).all() and (scale.get()[:3] == 0).all()
+            assert ((b[3] & 0x7f) == 0x7f).all()
