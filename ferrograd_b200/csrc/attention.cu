@@ -829,7 +829,7 @@ int32_t attention_bwd(fg_ctx* ctx, FgAttnArgs a) {
     if (fg_attn_tc_suits(ctx, dtype_of<T>, a)) return fg_attn_tc_bwd(ctx, dtype_of<T>, a);
     const uint64_t lines = (uint64_t)a.queries * a.heads;
     const bool small = a.dim > 128 || few_tiles(ctx, a);
-    const int32_t s = fg_attn_bwd_room(ctx, a, small ? 32 : 64);
+    const int32_t s = fg_attn_bwd_room(ctx, a, small ? 32 : 64, false);
     if (s != FG_OK) return s;
     if (lines) {
         fg_launch(ctx, attn_delta_kernel<T>, (unsigned)((lines + 7) / 8), kThreads, 0, (const T*)a.out, (const T*)a.dout, const_cast<float*>(a.delta), a.queries, a.heads, a.dim);
@@ -888,19 +888,19 @@ int32_t fold(fg_ctx* ctx, const FgAttnArgs& a) {
 
 }  // namespace
 
-int32_t fg_attn_bwd_room(fg_ctx* ctx, FgAttnArgs& a, uint32_t rows) {
+int32_t fg_attn_bwd_room(fg_ctx* ctx, FgAttnArgs& a, uint32_t rows, bool with_most) {
     const uint64_t blocks = a.dk ? fg_attn_tiles(a.sequences, a.keys, 1, rows) * a.kv_heads : 0, lines = (uint64_t)a.queries * a.heads;
     a.row_shares = 1;
     if (blocks && blocks < (uint64_t)ctx->sm_count) {
         const uint64_t want = 2ull * ctx->sm_count / blocks, have = (uint64_t)a.queries * a.group / a.sequences / (4 * rows), shares = want < have ? want : have;
         if (shares >= 2) a.row_shares = (uint32_t)(shares < 64 ? shares : 64);
     }
-    const uint64_t first = (256 + 4 * lines + 255) / 256 * 256;
+    const uint64_t most = with_most ? (8ull * a.sequences * a.kv_heads + 255) / 256 * 256 : 0, first = most + (4 * lines + 255) / 256 * 256;
     void* w;
     const int32_t s = fg_ws_alloc(ctx, first + (a.row_shares > 1 ? 8ull * a.row_shares * a.keys * a.kv_heads * a.dim : 0), &w);
     if (s != FG_OK) return s;
     a.most = static_cast<const uint32_t*>(w);
-    a.delta = static_cast<const float*>(w) + 64;
+    a.delta = reinterpret_cast<const float*>(static_cast<const char*>(w) + most);
     a.part_kv = reinterpret_cast<float*>(static_cast<char*>(w) + first);
     return FG_OK;
 }

@@ -22,7 +22,7 @@ struct FgAttnArgs {
     // Few tiles of keys: each tile's rows in shares, which leave sums in f32 for fg_attn_fold.  row_shares == 1: none
     uint32_t row_shares;
     float* part_kv;            // [row_shares][dk, dv][keys][kv_heads][dim]
-    const uint32_t* most;      // f16 on the tensor cores: the largest |dout| and |v|, as bits
+    const uint32_t* most;      // f16 on the tensor cores: the largest |dout| and |v| of each sequence's heads that share one of k and v, as bits: [sequences][kv_heads][2]
     int* dev_status;
 };
 
@@ -92,9 +92,9 @@ inline uint64_t fg_attn_tiles(uint32_t sequences, uint32_t total, uint32_t per, 
 __device__ __forceinline__ float* fg_attn_part(const FgAttnArgs& a, uint32_t z, uint32_t which, uint64_t key, uint32_t kv) {
     return a.part_kv + (((uint64_t)(z * 2 + which) * a.keys + key) * a.kv_heads + kv) * a.dim;
 }
-// The backward pass's room in the arena (a.delta, a.most, a.part_kv), and into how many shares of rows each tile of `rows` keys is cut: fewer tiles than SMs are
+// The backward pass's room in the arena (a.delta, a.part_kv and, where it is wanted, a.most), and into how many shares of rows each tile of `rows` keys is cut: fewer tiles than SMs are
 // brought to about two blocks an SM, by shares of four tiles of `rows` rows or more.
-int32_t fg_attn_bwd_room(fg_ctx* ctx, FgAttnArgs& a, uint32_t rows);
+int32_t fg_attn_bwd_room(fg_ctx* ctx, FgAttnArgs& a, uint32_t rows, bool with_most);
 int32_t fg_attn_fold(fg_ctx* ctx, int32_t dtype, const FgAttnArgs& a);      // adds the shares, in order
 
 constexpr float kFgLog2e = 1.4426950408889634f, kFgLn2 = 0.6931471805599453f;

@@ -671,9 +671,11 @@ struct BwdCfg {
     static constexpr size_t kUsed = (size_t)(2 + kTwice + kOnce) * kTile + 2 * 2 * kRows * 4 + 8 * kBars + 16;
     static constexpr size_t kSmem = kUsed + (kUsed + 1024 <= 227 * 1024 ? 1024 : 227 * 1024 - kUsed);
 };
-// The f16 operands' factor: a power of two that brings the largest gradient of a score near 2^13, if dout and v are as large as they can be.
-__device__ __forceinline__ float gradient_factor(const uint32_t* most, uint32_t dim) {
-    const float m = __uint_as_float(most[0]) * __uint_as_float(most[1]) * (float)dim;
+// The f16 operands' factor: a power of two that brings the largest gradient of a score near 2^13, if dout and v are as large as they can be in sequence b's heads that share
+// kv's.  (One for the whole call left gradients that are 10^5 times smaller than another sequence's two or three bits.)
+__device__ __forceinline__ float gradient_factor(const FgAttnArgs& a, uint32_t b, uint32_t kv) {
+    const uint32_t* const most = a.most + 2 * ((uint64_t)b * a.kv_heads + kv);
+    const float m = __uint_as_float(most[0]) * __uint_as_float(most[1]) * (float)a.dim;
     if (!(m > 0.0f && m < INFINITY)) return 1.0f;
     const int e = 13 - ilogbf(m);
     return ldexpf(1.0f, e > 60 ? 60 : e < -60 ? -60 : e);
@@ -917,7 +919,7 @@ __device__ __forceinline__ void tc_dq_tile(const CUtensorMap& tm_q, const CUtens
                 lse = lse == -INFINITY ? INFINITY : lse * kFgLog2e;
                 delta = a.delta[line];
             }
-            const float factor = std::is_same_v<T, __half> ? gradient_factor(a.most, a.dim) : 1.0f, by = a.scale * kFgLog2e;
+            const float factor = std::is_same_v<T, __half> ? gradient_factor(a, b, kv) : 1.0f, by = a.scale * kFgLog2e;
             const float2 by2 = make_float2(by, by), lse2 = make_float2(-lse, -lse), factor2 = make_float2(factor, factor), delta2 = make_float2(-delta * factor, -delta * factor);
             bool ok = true;
             for (uint32_t j = 0; j < n; ++j) {
@@ -1071,7 +1073,7 @@ __device__ __forceinline__ void tc_dkv_tile(const CUtensorMap& tm_q, const CUten
             blk.drain(a);
         } else if (warp >= 10) {
             // ---- lse (in powers of two; infinite where a row weighs nothing) and delta of the tiles' rows ----
-            const float factor = std::is_same_v<T, __half> ? gradient_factor(a.most, a.dim) : 1.0f;
+            const float factor = std::is_same_v<T, __half> ? gradient_factor(a, b, kv) : 1.0f;
             const uint32_t first = (warp - 10) * 32 + lane;
             for (uint32_t i = 0; i < n; ++i) {
                 if (!await(blk.stats_empty(i & 1), ((i >> 1) & 1) ^ 1, a.dev_status, FG_DEVERR_TMA_WAIT)) break;
@@ -1096,7 +1098,7 @@ __device__ __forceinline__ void tc_dkv_tile(const CUtensorMap& tm_q, const CUten
             const uint32_t side = warp >> 2, key = j0 + (threadIdx.x & 127), lanes = (uint32_t)(warp & 3) << 21;
             const bool there = (threadIdx.x & 127) < n_key;
             const uint32_t first = there ? s.first_query(a, key) : s.nq;      // the first query that sees the key
-            const float factor = std::is_same_v<T, __half> ? gradient_factor(a.most, a.dim) : 1.0f, by = a.scale * kFgLog2e;
+            const float factor = std::is_same_v<T, __half> ? gradient_factor(a, b, kv) : 1.0f, by = a.scale * kFgLog2e;
             const float2 by2 = make_float2(by, by), factor2 = make_float2(factor, factor);
             bool ok = true;
             for (uint32_t i = 0; i < n; ++i) {
@@ -1220,7 +1222,7 @@ __global__ void __launch_bounds__(256) attn_tc_delta_kernel(const FgAttnArgs a, 
         if (sub == 0 && line < lines) delta[line % a.heads * a.queries + line / a.heads] = d;
     }
 }
-// The largest |dout| and |v| of the sequences' rows (as bits, so NaN is larger than infinity): 64 rows a block, first those of dout.
+// The largest |dout| and |v| of the sequences' rows, by heads of k and v (as bits, so NaN is larger than infinity): 64 rows of a head, or of its queries' heads, a block, first those of dout.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_most_kernel(const FgAttnArgs a, uint32_t row_tiles, uint32_t* most) {
     fg_grid_enter();
@@ -1229,20 +1231,22 @@ __global__ void __launch_bounds__(256) attn_most_kernel(const FgAttnArgs a, uint
     const int b = fg_attn_find(keys ? a.k_starts : a.q_starts, a.sequences, keys ? a.keys : a.queries, 1, 64, blockIdx.x - (keys ? row_tiles : 0), &tile);
     if (b < 0) return;
     const FgAttnSeq s(a, b);
-    const uint64_t n = keys ? s.nk : s.nq, r0 = (uint64_t)tile * 64, stride = keys ? a.v_stride : (uint64_t)a.heads * a.dim;
-    const uint32_t line = (keys ? a.kv_heads : a.heads) * a.dim / 8;      // 16-byte words
-    const T* const x = static_cast<const T*>(keys ? a.v : a.dout) + (uint64_t)(keys ? s.k0 : s.q0) * stride;
+    const uint64_t rows = keys ? s.nk : s.nq, r0 = (uint64_t)tile * 64, stride = keys ? a.v_stride : (uint64_t)a.heads * a.dim;
+    if (r0 >= rows) return;
+    const uint32_t kv = blockIdx.y, width = (keys ? 1 : a.group) * a.dim, line = width / 8;      // (in 16-byte words)
+    const uint32_t n = (uint32_t)min((uint64_t)64, rows - r0) * line;
+    const T* const x = static_cast<const T*>(keys ? a.v : a.dout) + ((keys ? s.k0 : s.q0) + r0) * stride + (uint64_t)kv * width;
     uint32_t m = 0;
-    for (uint64_t r = r0 + (threadIdx.x >> 5); r < n && r < r0 + 64; r += 8)
 #pragma unroll 4
-        for (uint32_t c = threadIdx.x & 31; c < line; c += 32) {
-            float v[8];
-            FgPack<T>::widen(*reinterpret_cast<const uint4*>(x + r * stride + c * 8), v);
+    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+        const uint32_t r = i / line, c = i - r * line;
+        float v[8];
+        FgPack<T>::widen(*reinterpret_cast<const uint4*>(x + r * stride + c * 8), v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(fabsf(v[e])));
-        }
+        for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(fabsf(v[e])));
+    }
     m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0 && m) atomicMax(most + keys, m);      // (the largest of numbers: whoever comes first)
+    if ((threadIdx.x & 31) == 0 && m) atomicMax(most + 2 * ((uint64_t)b * a.kv_heads + kv) + keys, m);      // (the largest of numbers: whoever comes first)
 }
 
 // ---- host ----
@@ -1297,7 +1301,7 @@ int32_t bwd_launch(fg_ctx* ctx, FgAttnArgs a) {
     using Cfg = BwdCfg<DP>;
     constexpr bool half = std::is_same_v<T, __half>;
     const uint64_t lines = (uint64_t)a.queries * a.heads;
-    int32_t s = fg_attn_bwd_room(ctx, a, kRows);
+    int32_t s = fg_attn_bwd_room(ctx, a, kRows, half);
     if (s != FG_OK) return s;
     uint32_t* const most = const_cast<uint32_t*>(a.most);
     float* const delta = const_cast<float*>(a.delta);
@@ -1309,9 +1313,9 @@ int32_t bwd_launch(fg_ctx* ctx, FgAttnArgs a) {
         FG_LAUNCHED(ctx);
     }
     if (half) {
-        FG_CUDA(ctx, FG_ERR_FAILED_BUFFER_COPY, cudaMemsetAsync(most, 0, 8, ctx->stream));
+        FG_CUDA(ctx, FG_ERR_FAILED_BUFFER_COPY, cudaMemsetAsync(most, 0, 8ull * a.sequences * a.kv_heads, ctx->stream));
         const uint64_t row_tiles = fg_attn_tiles(a.sequences, a.queries, 1, 64), both = row_tiles + fg_attn_tiles(a.sequences, a.keys, 1, 64);
-        fg_launch(ctx, attn_most_kernel<T>, (unsigned)both, 256, 0, a, (uint32_t)row_tiles, most);
+        fg_launch(ctx, attn_most_kernel<T>, dim3((unsigned)both, a.kv_heads), 256, 0, a, (uint32_t)row_tiles, most);
         FG_LAUNCHED(ctx);
     }
     const uint32_t tokens = kRows / a.group;

@@ -364,7 +364,8 @@ int32_t fg_sample(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, cons
  * q_stride, k_stride and v_stride are elements from a token to the next, 0 for dense ones: q, k and v may be columns of
  * one tensor.  head_dim is at most 256.  16-bit tensors with head_dim a multiple of 8 up to 128, on 16-byte boundaries with strides that are multiples of 8,
  * and a scale above zero, are multiplied on the tensor cores as they lie: the weights, and backward the gradients of the scores, are then rounded to the
- * storage type before they are multiplied with v, dout, k and q.  Everything else is computed in f32 (products within 2^-20 of their size).
+ * storage type before they are multiplied with v, dout, k and q (the latter in f16 after a power of two for each sequence and head of k and v, which its largest
+ * dout and v decide).  Everything else is computed in f32 (products within 2^-20 of their size).
  * Up to 64 (query, head of a group) rows per sequence on average (16 in f32) the calls are those of generated tokens: the keys of a sequence are
  * shared out over the device, and a row's keys are read for every 16 to 64 rows, so a long prompt among many generated tokens is better a call of its own.
  * An output that overlaps an

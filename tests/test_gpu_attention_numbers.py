@@ -257,3 +257,43 @@ def test_generated_tokens_infinite_scores(ctx, dtype, dim, heads, kv):
         d.forward()
         out, lse = d.out.get(), d.lse.get()
         assert np.isnan(out[1]).all() and np.isnan(lse[:, 1]).all() and np.isfinite(out[0]).all() and np.isfinite(lse[:, 0]).all()
+
+
+# f16 gradients of the scores are multiplied in f16, by a power of two that brings them into its range.
+def one_head(c, b, w):
+    """Sequence b's heads that share head w of k and v, as a case by itself."""
+    q0, nq, k0, nk = c.seqs[b]
+    group = c.heads // c.kv
+    x = Case(0, c.dtype, c.dim, group, 1, [(nq, nk)], c.causal, scale=c.scale)
+    i, j, h = slice(q0, q0 + nq), slice(k0, k0 + nk), slice(w * group, (w + 1) * group)
+    x.q, x.dout, x.k, x.v = c.q[i, h], c.dout[i, h], c.k[j, w:w + 1], c.v[j, w:w + 1]
+    return x, i, j, h
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens", [SELF(300, 200), [(300, 300), (500, 70), (40, 200)]], ids=["few", "more"])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_factors_of_sequences_and_heads(ctx, dim, lens, infinite):
+    # dout up to 4 * 10^5 times as large in one sequence, or head of k and v, as in another: each is as exact as it is alone; an infinity, too, is its own sequence's and head's
+    c = Case(43, "f16", dim, 4, 2, lens)
+    for b, (q0, nq, _, _) in enumerate(c.seqs):
+        for w in range(2):
+            c.dout[q0:q0 + nq, 2 * w:2 * w + 2] *= (8000.0, 0.02)[(b + w) % 2]
+    c.dout = rounded(c.dout, "f16")
+    out, lse, _, _ = c.forward()
+    out, lse = rounded(out, "f16"), lse.astype(np.float32)
+    dout = c.dout.copy()
+    if infinite:
+        dout[17, 1, 3] = np.inf
+    d = OnDevice(ctx, c)
+    d.backward(Placed(ctx, out, "f16"), Placed(ctx, lse), Placed(ctx, dout, "f16"))
+    got = d.gradients()
+    for b in range(len(lens)):
+        for w in range(2):
+            if infinite and b == w == 0:
+                continue
+            x, i, j, h = one_head(c, b, w)
+            want, bound = x.backward(out[i, h], lse[h, i])
+            for n, mine in (("dq", got["dq"][i, h]), ("dk", got["dk"][j, w:w + 1]), ("dv", got["dv"][j, w:w + 1])):
+                assert np.abs(want[n]).max() < 6e4
+                compare(mine, want[n], bound[n], np.ones(len(mine), bool), f"{n} of {b}, {w}")
