@@ -850,7 +850,7 @@ int32_t check(fg_ctx* ctx, int32_t dtype, FgAttnArgs& a) {
     FG_REQUIRE(ctx, a.kv_heads <= 65535, "attention: too many heads");
     FG_REQUIRE(ctx, a.dim >= 1 && a.dim <= kMaxDim, "attention: head_dim must be 1 to 256");
     FG_REQUIRE(ctx, a.queries < (1u << 31) && a.keys < (1u << 31) && a.sequences < (1u << 24) && a.heads < (1u << 20), "attention: tensor too large");
-    FG_REQUIRE(ctx, a.scale >= -3.402823466e38f && a.scale <= 3.402823466e38f, "attention: scale must be a number");
+    FG_REQUIRE(ctx, a.scale >= -0x1p127f && a.scale <= 0x1p127f, "attention: scale must be a number, 2^127 at most");      // (times log2 e it stays one)
     const uint64_t q_line = (uint64_t)a.heads * a.dim, k_line = (uint64_t)a.kv_heads * a.dim;
     if (!a.q_stride) a.q_stride = q_line;
     if (!a.k_stride) a.k_stride = k_line;

@@ -454,7 +454,7 @@ int32_t fg_logprobs_fwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols
     FG_REQUIRE(ctx, logits, "fg_logprobs_fwd: NULL pointer");
     FG_REQUIRE(ctx, cols >= 1 && cols <= 1u << 31, "fg_logprobs_fwd: cols must be 1 to 2^31");
     FG_REQUIRE(ctx, (uint64_t)rows * cols < (1ull << 40), "fg_logprobs_fwd: tensor too large");
-    FG_REQUIRE(ctx, scale > 0.0f && scale <= 3.402823466e38f, "fg_logprobs_fwd: scale must be a number > 0");
+    FG_REQUIRE(ctx, scale > 0.0f && scale <= 0x1p127f, "fg_logprobs_fwd: scale must be > 0, and 2^127 at most");      // (times log2 e it stays a number)
     FG_REQUIRE(ctx, !logprob_out || targets, "fg_logprobs_fwd: logprob_out without targets");
     FG_REQUIRE(ctx, top <= kMaxTop && top <= cols, "fg_logprobs_fwd: top must be at most 64 and at most cols");
     FG_REQUIRE(ctx, !top || (top_ids_out && top_logprobs_out), "fg_logprobs_fwd: top without outputs");
@@ -481,7 +481,7 @@ int32_t fg_logprobs_bwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols
     FG_REQUIRE(ctx, logits && lse && dlogits, "fg_logprobs_bwd: NULL pointer");
     FG_REQUIRE(ctx, cols >= 1 && cols <= 1u << 31, "fg_logprobs_bwd: cols must be 1 to 2^31");
     FG_REQUIRE(ctx, (uint64_t)rows * cols < (1ull << 40), "fg_logprobs_bwd: tensor too large");
-    FG_REQUIRE(ctx, scale > 0.0f && scale <= 3.402823466e38f, "fg_logprobs_bwd: scale must be a number > 0");
+    FG_REQUIRE(ctx, scale > 0.0f && scale <= 0x1p127f, "fg_logprobs_bwd: scale must be > 0, and 2^127 at most");
     FG_REQUIRE(ctx, dlogprob || dentropy, "fg_logprobs_bwd: no gradient given");
     FG_REQUIRE(ctx, !dlogprob || targets, "fg_logprobs_bwd: dlogprob without targets");
     FG_REQUIRE(ctx, !dentropy || entropy, "fg_logprobs_bwd: dentropy without the entropies");

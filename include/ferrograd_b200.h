@@ -362,7 +362,7 @@ int32_t fg_sample(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols, cons
  * left as they were, and so are their gradients.  A key behind its sequence's end reaches nothing, whatever its rows hold.  A NaN or an infinity in v
  * (in the backward pass: in any tensor) may reach the rows of its own sequence that do not see it.
  * q_stride, k_stride and v_stride are elements from a token to the next, 0 for dense ones: q, k and v may be columns of
- * one tensor.  head_dim is at most 256.  16-bit tensors with head_dim a multiple of 8 up to 128, on 16-byte boundaries with strides that are multiples of 8,
+ * one tensor.  head_dim is at most 256, |scale| at most 2^127.  16-bit tensors with head_dim a multiple of 8 up to 128, on 16-byte boundaries with strides that are multiples of 8,
  * and a scale above zero, are multiplied on the tensor cores as they lie: the weights, and backward the gradients of the scores, are then rounded to the
  * storage type before they are multiplied with v, dout, k and q (the latter in f16 after a power of two for each sequence and head of k and v, which its largest
  * dout and v decide).  Everything else is computed in f32 (products within 2^-20 of their size).
@@ -404,7 +404,7 @@ int32_t fg_rmsnorm_bwd(fg_ctx* ctx, int32_t dtype, uint32_t rows, uint32_t cols,
                        const void* gamma, const float* rstd, const void* dsum, void* dx, void* dgamma,
                        int32_t accumulate_params);
 
-/* For each row of logits [rows, cols], with z = scale * logits (scale > 0: one over a temperature):
+/* For each row of logits [rows, cols], with z = scale * logits (scale > 0, at most 2^127: one over a temperature):
  *   lse_out      log(sum(exp(z)))                               f32 [rows]
  *   logprob_out  z[targets[row]] - lse                          f32 [rows]
  *   entropy_out  -sum(p * log p) with p = exp(z - lse)          f32 [rows]
