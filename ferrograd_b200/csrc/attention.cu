@@ -803,6 +803,17 @@ int32_t in_shares(fg_ctx* ctx, FgAttnArgs& a) {
     return FG_OK;
 }
 
+// Few rows of a sequence, on average: its keys go in shares.  Otherwise tiles of rows have all of their keys.  Both sides of the border, us, in shares (and in tiles), 32 heads over 8 of 128 columns:
+//   bf16, rows        16            48            64            96            128
+//   1 x 100000 keys   82 (1475)     145 (1466)    146 (1441)    277 (1438)    280 (1235)
+//   8 x 20000         149 (458)     294 (455)     310 (447)     559 (446)     592 (386)
+//   64 x 4000         214 (267)     457 (266)     489 (261)     882 (261)     945 (232)
+//   64 x 500          67 (48)       141 (48)      165 (47)      270 (48)      319 (48)
+//   f32, rows         8             16            32            64
+//   1 x 100000 keys   610 (14353)   611 (14357)   1187 (14388)  2113 (14386)
+//   64 x 4000         1565 (3949)   1577 (3957)   2779 (3970)   5352 (3977)
+//   64 x 500          251 (534)     265 (538)     449 (541)     849 (548)
+// 64 rows are right for some sequences with long caches; where there are enough sequences for all SMs, tiles would be from 32 rows on, and for short caches from 16.
 template <typename T>
 int32_t attention_fwd(fg_ctx* ctx, FgAttnArgs a) {
     const uint64_t rows = ((uint64_t)a.queries * a.group + a.sequences - 1) / a.sequences;      // of a sequence, on average
