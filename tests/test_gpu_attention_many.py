@@ -3,8 +3,8 @@ tensors off 16-byte boundaries, heads of more than 128 columns.  Formulas and bo
 import numpy as np
 import pytest
 
-from test_gpu_attention import Case, check_backward, check_forward, OnDevice, SELF
-from token_ops import Placed, rounded
+from test_gpu_attention import Case, check_backward, check_forward, compare, OnDevice, SELF
+from token_ops import bits, Placed, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,52 @@ def test_large_scores(ctx):
         d.forward()
         check_forward(d)
         check_backward(ctx, d)
+
+
+@pytest.mark.parametrize("dtype,dim,heads,kv", [("bf16", 128, 4, 1), ("f16", 64, 4, 2), ("f32", 64, 4, 2), ("f32", 128, 16, 4)])
+@pytest.mark.parametrize("first,then,slot", [([(300, 300), (40, 40), (900, 900)], [(0, 0), (1210, 1210), (30, 30)], None), ([(1, 700), (1, 3), (1, 0)], [(1, 2), (1, 0), (1, 5000)], 5000),
+                                             ([(2, 30), (1, 900), (0, 7)], [(0, 0), (3, 1200), (0, 1200)], 1200)], ids=["prompts", "tokens", "moved"])
+def test_recorded_with_new_lengths(ctx, dtype, dim, heads, kv, first, then, slot):
+    # starts and lengths are read when the kernels run: a plan of one batch, played for another
+    a, b = (Case(54, dtype, dim, heads, kv, lens, slot=slot) for lens in (first, then))
+    d = OnDevice(ctx, a)
+
+    def both():
+        d.forward()
+        d.backward(*t)
+
+    def given(c):
+        out, lse, _, _ = c.forward()
+        return Placed(ctx, rounded(out, dtype), dtype), Placed(ctx, lse.astype(np.float32)), Placed(ctx, c.dout, dtype)
+
+    t, u = given(a), given(b)
+    both()
+    ctx.sync()
+    ctx.plan_begin()
+    both()
+    plan = ctx.plan_end()
+    plan.launch()
+    check_forward(d)
+    for x, y in zip(t, u):
+        ctx.upload(x.t.data, ctx.to_numpy(y.t))
+    ctx.upload(d.q_starts.t.data, ctx.to_numpy(Placed(ctx, np.asarray(b.q_starts), "u32").t))
+    ctx.upload(d.k_starts.t.data, ctx.to_numpy(Placed(ctx, np.asarray(b.k_starts), "u32").t))
+    if slot:
+        ctx.upload(d.k_lengths.t.data, ctx.to_numpy(Placed(ctx, np.asarray(b.k_lengths), "u32").t))
+    for x in (d.out, d.lse, *d.g):      # NaN where the new batch has nothing
+        ctx.upload(x.t.data, cleared(x, ctx))
+    d.c = b
+    plan.launch()
+    ctx.sync()
+    check_forward(d)
+    want, bound = b.backward(rounded(b.forward()[0], dtype), b.forward()[1].astype(np.float32))
+    rows = b.rows
+    for n, got in d.gradients().items():
+        compare(got, want[n], bound[n], rows[0] if n == "dq" else rows[1], n)
+    plan.destroy()
+
+
+def cleared(x, ctx):
+    whole = ctx.to_numpy(x.t).copy()
+    whole[x.shift:x.shift + x.n] = bits(np.full(x.n, np.nan), x.dtype)
+    return whole
